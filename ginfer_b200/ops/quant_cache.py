@@ -15,11 +15,12 @@ All work goes to the current stream; nothing is kept between calls.
 """
 from __future__ import annotations
 
-from ctypes import c_float, c_int, c_void_p
+from ctypes import c_float, c_int, c_longlong, c_void_p
 
 import torch
 
 from . import _code, _fn, _ok, _p, _stream
+from .gemm_bf16 import num_sms
 
 KINDS = {"int8": torch.int8, "fp8": torch.float8_e4m3fn}
 _FP8 = {torch.int8: 0, torch.float8_e4m3fn: 1}
@@ -143,20 +144,37 @@ def read_slots(cache, slots: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     return out
 
 
-def _decode(q, nh, facts, block_table, lengths, scale, span, dtype=None):
+_DECODE_ARGS = ([c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p]
+                + [c_int] * 6 + [c_float, c_int, c_void_p] + [c_int] * 4 + [c_void_p, c_longlong, c_void_p])
+_F32 = {torch.float32: 1, torch.bfloat16: 0}
+# Requests of at most this many tokens are never cut into pieces, whose results need scratch (the kernel has the
+# same line: kLeastTiles tiles of 16 keys a piece, one tile for a cut that is not aligned).
+_WHOLE = 16 * 31
+
+
+def _decode(q, nh, facts, block_table, lengths, scale, span, fused=None):
+    """``fused``: ``(address, rows, rotated channels)`` of the table of angles and ``neighbours``."""
     codes, scales, fp8, pages, nkv, page, hd = facts
     _heads(nh, nkv)
-    x, stride, code = _rows(q, nh * hd, "q")
+    x, stride, code = _rows(q, (nh if fused is None else nh + 2 * nkv) * hd, "q" if fused is None else "qkv")
     B, W = block_table.shape
     if q.shape[0] != B:
         raise ValueError(f"{q.shape[0]} queries for {B} requests")
-    out = torch.empty((B, nh * hd), dtype=dtype or q.dtype, device=q.device)
-    f = _fn("quant_attention", "gf_quant_decode",
-            [c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p,
-             c_int] + [c_int] * 5 + [c_float, c_void_p], (f"GF_HEAD_DIM={hd}",))
-    _ok(f(x, stride, code, _p(codes), fp8, _p(scales), _ints(block_table, (B, W), "block_table"), W, W,
-          _ints(lengths, (B,), "lengths"), _p(out), _code(out.dtype), B, nh, nkv, page, int(span), float(scale),
-          _stream()), "quant_cache.decode")
+    out = torch.empty((B, nh * hd), dtype=q.dtype, device=q.device)
+    defines = (f"GF_HEAD_DIM={hd}",)
+    sms = num_sms(q.device)
+    scratch, words = None, 0
+    if W * page > _WHOLE:
+        size = _fn("quant_attention", "gf_quant_decode_scratch", [c_int] * 4, defines, kernels=0, restype=c_longlong)
+        words = size(B, nh, nkv, sms) // 4
+        scratch = torch.empty(words, dtype=torch.float32, device=q.device)
+    f = _fn("quant_attention", "gf_quant_decode", _DECODE_ARGS, defines)
+    table, rows, rot, neighbours = (None, 0, 0, 0) if fused is None else fused
+    f32 = _F32[q.dtype]
+    _ok(f(x, stride, f32, _p(codes), fp8, _p(scales), _ints(block_table, (B, W), "block_table"), W, W,
+          _ints(lengths, (B,), "lengths"), _p(out), f32, B, nh, nkv, page, int(span), float(scale),
+          int(fused is not None), table, rows, rot, int(neighbours), sms, _p(scratch), 4 * words, _stream()),
+        "quant_cache.decode")
     return out
 
 
@@ -175,10 +193,4 @@ def step(qkv: torch.Tensor, nh: int, table, cache, block_table: torch.Tensor, le
     the last of request ``b``'s ``lengths[b]`` tokens; q and k are rotated, k and v written (as
     :func:`write` does), and the token attends over the cache, itself among the keys (as :func:`decode`)."""
     facts = _cache(cache)
-    page = facts[5]
-    last = (lengths - 1).clamp(min=0)
-    slots = block_table.gather(1, (last // page)[:, None].long())[:, 0] * page + last % page
-    slots = torch.where(lengths > 0, slots, -1).to(torch.int32)
-    # (in 32 bits: the rotated q is not rounded on its way to the scores)
-    q = write(qkv.float(), nh, table, last, slots, cache, neighbours=neighbours)
-    return _decode(q, nh, facts, block_table, lengths, scale, window, qkv.dtype)
+    return _decode(qkv, nh, facts, block_table, lengths, scale, window, (*_angles(table, facts[6]), neighbours))

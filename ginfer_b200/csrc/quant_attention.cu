@@ -24,10 +24,9 @@
 // are the sum of two halves (22 bits), and tiles' products are added up outside the tensor cores.  Scores,
 // maxima, sums and O are 32-bit.
 //
-// The work is cut into pieces of equal numbers of 16-key tiles, whatever the requests' lengths: see
-// find_piece.  A piece is a block of four warps, which take its tiles in turn.  Where a request has several
-// pieces, they leave their results (normalised, with maximum and sum) in scratch, and a second kernel joins
-// them in order.
+// A block is four warps, which take the tiles of its share of the work in turn (how it is shared out: see
+// Cursor), each through a ring of stages of its own that cp.async fills: nothing but an item's start and end
+// synchronises the block.
 #include <algorithm>
 #include <cstdlib>
 #include <type_traits>
@@ -38,21 +37,34 @@
 #define GF_HEAD_DIM 128
 #endif
 
+// (Internal to this library: a static of a template would be shared with the libraries of other head sizes.)
 namespace gf {
+namespace {
 
 constexpr int HD = GF_HEAD_DIM;
 static_assert(HD % 16 == 0 && HD >= 16 && HD <= 256, "head size must be a multiple of 16, <= 256");
 constexpr float kLog2E = 1.4426950408889634f;
 constexpr int TILE = 16, WARPS = 4, THREADS = WARPS * 32;
-constexpr int KW = HD % 64 == 0 ? 16 : HD % 32 == 0 ? 8 : 4;     // bytes of a key a thread loads at once
+constexpr int KW = HD % 64 == 0 ? 16 : HD % 32 == 0 ? 8 : 4;     // bytes of a key a thread reads at once
 constexpr int VW = HD % 128 == 0 ? 16 : HD % 64 == 0 ? 8 : HD % 32 == 0 ? 4 : 2;
 constexpr int KWORDS = HD / 16;                                  // words of a key a thread holds
-constexpr int VWORDS = VW >= 4 ? HD / 32 : HD / 16;              // of a value (2-byte loads: a word each)
 constexpr int MT = HD / 16;                                      // row tiles of O^T
-// values of the next tile are loaded a tile ahead like its keys, where registers allow
-constexpr bool kValuesAhead = HD <= 128;
-// the fewest tiles a piece is worth
-constexpr int kLeastTiles = 8 * WARPS;
+constexpr int CH = HD / 16;                                      // 16-byte chunks of a row
+// Rows in shared memory are 16 bytes apart in banks: a quarter warp's reads of keys (two rows, four
+// places of 16 bytes) and of values (four rows, two places) then hit every bank once.
+constexpr int ROW = HD + 16;
+constexpr int SCALES_AT = 2 * TILE * ROW, STAGE = SCALES_AT + TILE * 16 + 16;
+#ifndef GF_STAGES
+#define GF_STAGES 3
+#endif
+#ifndef GF_OCC
+#define GF_OCC 3
+#endif
+constexpr int STAGES = GF_STAGES;
+// the fewest tiles of a block's run
+constexpr int kLeastTiles = 4 * WARPS;
+// requests that see at most so many keys are one block's work a kv head
+constexpr int kShortKeys = 1024;
 constexpr int kMostBlocks = 8;          // of the blocks that fit an SM, so many are counted on
 
 struct DecodeArgs {
@@ -62,14 +74,16 @@ struct DecodeArgs {
   float* scales;
   const int* block_table;
   int table_stride, limit;    // limit: no request is longer (table width * page)
+  int pages;                  // of the cache: an entry of the table beyond it is taken for the nearest
   const int* lengths;
   void* out;
   int out_f32, B, nh, nkv, page, page_shift, span;
   float scale;
   int chunks, rows;           // a kv head's query heads in `chunks` blocks of up to `rows`
-  int slots;                  // blocks that fit the GPU at once
-  float* po;                  // [pieces * heads][rows][HD]
-  float2* pml;                // [pieces * heads][rows]
+  int stream;                 // blocks share the tiles evenly (see Cursor), else a block an item
+  int2* info;                 // [heads * B], stream: the block an item starts in, how many it is spread over
+  float* po;                  // [blocks][2][rows][HD]: the parts of the item a block ends in the middle of or starts
+  float2* pml;                // [blocks][2][rows]      in the middle of (0: it has begun before this block)
   // the fused step
   const float* table;
   int table_rows, rot, neighbours;
@@ -82,99 +96,100 @@ __device__ __forceinline__ float fast_exp2(float x) {
 }
 
 // ------------------------------------------------------------------------------------- division of the work
-// Request b has n_b tiles (positions first_visible .. len - 1, cut at multiples of 16).  With room for N
-// pieces a kv head at once (N = slots / heads) a piece holds at most
-//     size = sum n_b / (N - B + 1) tiles   where 2 B <= N: then all pieces run at once
-//     size = sum n_b heads / (2 slots)     else: two rounds and the requests' remainders even out
-// and request b has max(1, n_b / size rounded up) pieces.  Every warp of a block works this out for itself.
-struct Piece {
-  int b, first, last, lo, len;    // tiles [first, last) of request b; its keys are lo .. len - 1
-  int pieces, index;              // how many pieces b has, which this is
-};
+// An item is a (chunk of query heads that share a kv head, request), request by request within a chunk, and its
+// tiles are the positions first_visible .. len - 1 cut at multiples of 16; a request without a token counts as one.
+// Where requests are short (DecodeArgs.stream 0) a block takes an item.  Else the items' tiles are one long
+// sequence, and every block takes an equal run of it: they all end at the same time, whatever the lengths.  A run
+// begins and ends inside items; such parts are joined by a second kernel.
 __device__ __forceinline__ int request_length(const DecodeArgs& a, int b) {
   return max(min(fresh_index(a.lengths + b), a.limit), 0);
 }
+__device__ __forceinline__ int first_tile(const DecodeArgs& a, int len) {
+  return len > 0 ? first_visible_key(len - 1, a.span) >> 4 : 0;
+}
 __device__ __forceinline__ int request_tiles(const DecodeArgs& a, int len) {
-  return len > 0 ? ((len - 1) >> 4) - (first_visible_key(len - 1, a.span) >> 4) + 1 : 0;
+  return len > 0 ? ((len - 1) >> 4) - first_tile(a, len) + 1 : 1;
 }
-__device__ __forceinline__ int piece_size(const DecodeArgs& a, int lane) {
-  long long total = 0;
-  for (int b = lane; b < a.B; b += 32) total += request_tiles(a, request_length(a, b));
+struct Cursor {
+  int hc, b, len;             // the item
+  int off, todo, run;         // tiles of it before this block's, tiles left to this block, tiles a block
+};
+constexpr int EACH = 4;       // requests a thread keeps in registers
+// The run of block `k` of `blocks`, found by the whole block; todo = 0: there is nothing left for it.
+__device__ __forceinline__ Cursor find_run(const DecodeArgs& a, int k, int blocks, int heads) {
+  __shared__ unsigned counts[WARPS];
+  __shared__ Cursor found;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int each = (a.B + THREADS - 1) / THREADS, b0 = threadIdx.x * each, b1 = min(b0 + each, a.B);
+  int n[EACH], len[EACH];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  const int heads = a.nkv * a.chunks, N = a.slots / heads;
-  const long long size = 2 * a.B <= N ? (total + N - a.B) / (N - a.B + 1)
-                                      : (total * heads + 2 * a.slots - 1) / (2 * a.slots);
-  return (int)max(size, (long long)kLeastTiles);
-}
-// The piece with number `want` in the order of the requests; b = -1: there are fewer.
-__device__ __forceinline__ Piece find_piece(const DecodeArgs& a, int want, int lane) {
-  const int size = piece_size(a, lane);
-  Piece r;
-  r.b = -1;
-  int before = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 32) {
-    const int b = b0 + lane;
-    const int len = b < a.B ? request_length(a, b) : 0;
-    const int n = request_tiles(a, len);
-    const int mine = b < a.B ? max(1, (n + size - 1) / size) : 0;
-    int sum = mine;
+  for (int i = 0; i < EACH; ++i) len[i] = i < each && b0 + i < b1 ? request_length(a, b0 + i) : -1;
+  unsigned mine = 0;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += up;
-    }
-    const int start = before + sum - mine;
-    const unsigned hit = __ballot_sync(0xffffffffu, want >= start && want < start + mine);
-    if (hit) {
-      const int src = __ffs(hit) - 1;
-      r.b = b0 + src;
-      r.len = __shfl_sync(0xffffffffu, len, src);
-      r.pieces = __shfl_sync(0xffffffffu, mine, src);
-      r.index = want - __shfl_sync(0xffffffffu, start, src);
-      const int tiles = __shfl_sync(0xffffffffu, n, src);
-      r.lo = r.len > 0 ? first_visible_key(r.len - 1, a.span) : 0;
-      const int t0 = r.lo >> 4;
-      r.first = t0 + min(r.index * size, tiles);
-      r.last = t0 + min((r.index + 1) * size, tiles);
-      return r;
-    }
-    before += __shfl_sync(0xffffffffu, sum, 31);
+  for (int i = 0; i < EACH; ++i) n[i] = len[i] >= 0 ? request_tiles(a, len[i]) : 0, mine += n[i];
+  for (int b = b0 + EACH; b < b1; ++b) mine += request_tiles(a, request_length(a, b));
+  unsigned sum = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned up = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += up;
   }
-  return r;
+  if (lane == 31) counts[warp] = sum;
+  if (threadIdx.x == 0) found.todo = 0;
+  __syncthreads();
+  unsigned start = sum - mine, total = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    if (w < warp) start += counts[w];
+    total += counts[w];
+  }
+  const unsigned long long all = (unsigned long long)total * heads;
+  const unsigned long long run = max((all + blocks - 1) / blocks, (unsigned long long)kLeastTiles);
+  const unsigned long long at = run * k;
+  if (at < all) {
+    const unsigned hc = (unsigned)(at / total), rest = (unsigned)(at - (unsigned long long)hc * total);
+    if (rest >= start && rest < start + mine) {
+      int left = (int)(rest - start);
+      for (int b = b0; b < b1; ++b) {
+        const int i = b - b0, ln = i < EACH ? (i == 0 ? len[0] : i == 1 ? len[1] : i == 2 ? len[2] : len[3])
+                                            : request_length(a, b);
+        const int tiles = request_tiles(a, ln);
+        if (left < tiles) {
+          found = {(int)hc, b, ln, left, (int)min(run, all - at), (int)run};
+          break;
+        }
+        left -= tiles;
+      }
+    }
+  }
+  __syncthreads();
+  return found;
 }
 
 // ------------------------------------------------------------------------------------- a tile
-struct Tile {
-  uint32_t k[2][KWORDS];      // keys g and g + 8: channels as the thread's places want them
-  uint32_t v[4][VWORDS];      // keys 2t, 2t + 1, 2t + 8, 2t + 9
-  float2 sc[2];               // (key, value) scales of keys g and g + 8
-};
-template <int BYTES> __device__ __forceinline__ void load_bytes(const uint8_t* p, uint32_t* r);
-template <> __device__ __forceinline__ void load_bytes<16>(const uint8_t* p, uint32_t* r) {
-  const uint4 x = __ldcg(reinterpret_cast<const uint4*>(p));
+template <int BYTES> __device__ __forceinline__ void read_bytes(const uint8_t* p, uint32_t* r);
+template <> __device__ __forceinline__ void read_bytes<16>(const uint8_t* p, uint32_t* r) {
+  const uint4 x = *reinterpret_cast<const uint4*>(p);
   r[0] = x.x, r[1] = x.y, r[2] = x.z, r[3] = x.w;
 }
-template <> __device__ __forceinline__ void load_bytes<8>(const uint8_t* p, uint32_t* r) {
-  const uint2 x = __ldcg(reinterpret_cast<const uint2*>(p));
+template <> __device__ __forceinline__ void read_bytes<8>(const uint8_t* p, uint32_t* r) {
+  const uint2 x = *reinterpret_cast<const uint2*>(p);
   r[0] = x.x, r[1] = x.y;
 }
-template <> __device__ __forceinline__ void load_bytes<4>(const uint8_t* p, uint32_t* r) {
-  r[0] = __ldcg(reinterpret_cast<const uint32_t*>(p));
+template <> __device__ __forceinline__ void read_bytes<4>(const uint8_t* p, uint32_t* r) {
+  r[0] = *reinterpret_cast<const uint32_t*>(p);
 }
-template <> __device__ __forceinline__ void load_bytes<2>(const uint8_t* p, uint32_t* r) {
-  r[0] = __ldcg(reinterpret_cast<const unsigned short*>(p));
+template <> __device__ __forceinline__ void read_bytes<2>(const uint8_t* p, uint32_t* r) {
+  r[0] = *reinterpret_cast<const uint16_t*>(p);
 }
-__device__ __forceinline__ void load_key(const uint8_t* row, int t, uint32_t (&r)[KWORDS]) {
-#pragma unroll
-  for (int j = 0; j < HD / (4 * KW); ++j) load_bytes<KW>(row + (j * 4 + t) * KW, r + j * (KW / 4));
+__device__ __forceinline__ void copy16(void* dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(smem_u32(dst)), "l"(src),
+               "r"(there ? 16 : 0) : "memory");            // (not there: zeros)
 }
-__device__ __forceinline__ void load_value(const uint8_t* row, int g, uint32_t (&r)[VWORDS]) {
-  constexpr int STEP = VW >= 4 ? VW / 4 : 1;
-#pragma unroll
-  for (int j = 0; j < HD / (8 * VW); ++j) load_bytes<VW>(row + (j * 8 + g) * VW, r + j * STEP);
+template <int N> __device__ __forceinline__ void wait_copies() {
+  asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
 }
-// Where a key lies.  WHOLE: pages are a multiple of the tile, a tile has one page.
+// Where a key lies.
 struct Place {
   const uint8_t* codes;       // the key's row; its value's lies page * HD behind
   const float2* scales;
@@ -183,51 +198,72 @@ __device__ __forceinline__ Place place_of(const DecodeArgs& a, int kvh, int page
   const size_t at = (size_t)page_number * a.nkv + kvh;
   return {a.codes + (at * 2 * a.page + off) * HD, reinterpret_cast<const float2*>(a.scales) + at * a.page + off};
 }
+__device__ __forceinline__ int page_in(const DecodeArgs& a, int number) {
+  return min(max(number, 0), a.pages - 1);
+}
 __device__ __forceinline__ int logical_page(const DecodeArgs& a, int c) {
   return a.page_shift >= 0 ? c >> a.page_shift : c / a.page;
 }
-__device__ __forceinline__ Place place_of_key(const DecodeArgs& a, const Piece& pc, int kvh, int c) {
-  c = min(max(c, pc.lo), pc.len - 1);            // (a masked key: any that is there)
-  const int lp = logical_page(a, c);
-  return place_of(a, kvh, fresh_index(a.block_table + (size_t)pc.b * a.table_stride + lp), c - lp * a.page);
-}
-template <bool WHOLE, bool KEYS, bool VALUES>
-__device__ __forceinline__ void load_tile(Tile& x, const DecodeArgs& a, const Piece& pc, int kvh, int tile,
-                                          int page_number, int g, int t) {
-  const int c0 = tile * TILE;
-  if constexpr (WHOLE) {
-    const Place p = place_of(a, kvh, page_number, c0 - logical_page(a, c0) * a.page);
-    if constexpr (KEYS) {
-      load_key(p.codes + g * HD, t, x.k[0]);
-      load_key(p.codes + (g + 8) * HD, t, x.k[1]);
-      x.sc[0] = __ldcg(p.scales + g);
-      x.sc[1] = __ldcg(p.scales + g + 8);
-    }
-    if constexpr (VALUES) {
-      const uint8_t* v = p.codes + (size_t)a.page * HD + 2 * t * HD;
-      load_value(v, g, x.v[0]);
-      load_value(v + HD, g, x.v[1]);
-      load_value(v + 8 * HD, g, x.v[2]);
-      load_value(v + 9 * HD, g, x.v[3]);
-    }
-  } else {
-    if constexpr (KEYS) {
+// A warp's view of the piece's tiles.  WHOLE: pages are a multiple of the tile, a tile has one page; else a lane
+// knows the page of row `lane % 16`.  Rows outside [lo, end) are zeros and nothing of them is read.
+template <bool WHOLE> struct Tiles {
+  const DecodeArgs& a;
+  const int* tbl;
+  int kvh, lo, end, last, lane;
+  __device__ __forceinline__ int row_key(int tile, int r) const { return min(max(tile * TILE + r, lo), end - 1); }
+  __device__ __forceinline__ int page_of(int tile) const {
+    if (tile >= last || lo >= end) return 0;
+    return page_in(a, fresh_index(tbl + logical_page(a, WHOLE ? tile * TILE : row_key(tile, lane & 15))));
+  }
+  __device__ __forceinline__ void copy(uint8_t* stage, int tile, int page_number) const {
+    const int c0 = tile * TILE;
+    const size_t values = (size_t)a.page * HD;
+    const uint8_t* base = nullptr;
+    if constexpr (WHOLE) base = place_of(a, kvh, page_number, c0 - logical_page(a, c0) * a.page).codes;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const Place p = place_of_key(a, pc, kvh, c0 + g + 8 * i);
-        load_key(p.codes, t, x.k[i]);
-        x.sc[i] = __ldcg(p.scales);
+    for (int i = 0; i < (TILE * CH + 31) / 32; ++i) {
+      const int idx = lane + 32 * i, row = idx / CH, ch = idx - row * CH;
+      const bool used = TILE * CH % 32 == 0 || idx < TILE * CH;
+      const bool there = c0 + row >= lo && c0 + row < end;
+      const uint8_t* src = a.codes;
+      if constexpr (WHOLE) {
+        src = base + idx * 16;
+      } else {
+        const int pg = __shfl_sync(0xffffffffu, page_number, row & 15);
+        const int c = row_key(tile, row);
+        if (there) src = place_of(a, kvh, pg, c - logical_page(a, c) * a.page).codes + ch * 16;
+      }
+      if (used) {
+        copy16(stage + row * ROW + ch * 16, src, there);
+        copy16(stage + (TILE + row) * ROW + ch * 16, there ? src + values : src, there);
       }
     }
-    if constexpr (VALUES) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        load_value(place_of_key(a, pc, kvh, c0 + 2 * t + (i & 1) + 8 * (i >> 1)).codes + (size_t)a.page * HD, g,
-                   x.v[i]);
+    // the scales: pairs of keys; where a key's neighbour lies elsewhere, the 16 bytes that its own are in
+    if constexpr (WHOLE) {
+      const Place pl = place_of(a, kvh, page_number, c0 - logical_page(a, c0) * a.page);
+      if (lane < TILE / 2) copy16(stage + SCALES_AT + lane * 16, pl.scales + 2 * lane, true);
+    } else if (lane < TILE) {
+      const int c = row_key(tile, lane);
+      const bool there = c0 + lane >= lo && c0 + lane < end;
+      const size_t at = there ? (size_t)place_of(a, kvh, page_number, c - logical_page(a, c) * a.page).scales : (size_t)a.codes;
+      const uint32_t odd = (uint32_t)at & 8u;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(smem_u32(stage + SCALES_AT + lane * 16)),
+                   "l"(at - odd), "r"(there ? (odd ? 16 : 8) : 0) : "memory");
+      stage[SCALES_AT + TILE * 16 + lane] = (uint8_t)odd;
     }
   }
-}
+  // The (key, value) scales of key r of a tile.
+  __device__ __forceinline__ float2 scales(const uint8_t* stage, int r) const {
+    const uint8_t* at = stage + SCALES_AT;
+    return *reinterpret_cast<const float2*>(WHOLE ? at + r * 8 : at + r * 16 + at[TILE * 16 + r]);
+  }
+};
 
+// Two codes plus 128 (the bytes 2i, 2i + 1 of a word) as the halves 2^-24 (code + 128), below the smallest normal one:
+// a byte permutation, no arithmetic.
+__device__ __forceinline__ uint32_t raised_halves(uint32_t w, int i) {
+  return __byte_perm(w, 0u, i ? 0x4342 : 0x4140);
+}
 // Two codes in the bytes 2i, 2i + 1 of a word, as two halves.
 template <bool FP8> __device__ __forceinline__ uint32_t halves(uint32_t w, int i) {
   if constexpr (FP8) {
@@ -261,118 +297,204 @@ __device__ __forceinline__ float power_back(int f) {
 }
 
 // ------------------------------------------------------------------------------------- q, and the new token
-// Channel c of head row x at the token's position.
-__device__ __forceinline__ float row_value(const DecodeArgs& a, size_t at, int c) {
-  return a.q_f32 ? fresh(reinterpret_cast<const float*>(a.q) + at + c)
-                 : fresh(reinterpret_cast<const bf16*>(a.q) + at + c);
+// A lane's channels of head rows: lane, lane + 32, ...  Everything is asked for before anything is used.
+constexpr int N = (HD + 31) / 32;
+__device__ __forceinline__ float row_value(const DecodeArgs& a, size_t at) {
+  return a.q_f32 ? fresh(reinterpret_cast<const float*>(a.q) + at) : fresh(reinterpret_cast<const bf16*>(a.q) + at);
 }
-__device__ __forceinline__ float rotated_value(const DecodeArgs& a, size_t at, int c, const float* cs) {
-  const float x = row_value(a, at, c);
-  if (c >= a.rot) return x;
+__device__ __forceinline__ void load_row(const DecodeArgs& a, size_t at, bool there, int lane, float (&x)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = there && i * 32 + lane < HD ? row_value(a, at + i * 32 + lane) : 0.f;
+}
+// The channel that channel c turns with, and which of the pair c is.
+__device__ __forceinline__ int partner(const DecodeArgs& a, int c, bool& second) {
   const int half = a.rot >> 1;
-  const bool second = a.neighbours ? (c & 1) : c >= half;
-  const int j = a.neighbours ? c >> 1 : second ? c - half : c;
-  const float o = row_value(a, at, a.neighbours ? c ^ 1 : second ? c - half : c + half);
-  return second ? turned_second(o, x, cs[j], cs[half + j]) : turned_first(x, o, cs[j], cs[half + j]);
+  second = a.neighbours ? (c & 1) : c >= half;
+  return a.neighbours ? c ^ 1 : second ? c - half : c + half;
 }
-
-// ------------------------------------------------------------------------------------- a piece
-// NT: tiles of 8 query heads.  PARTS: halves that make up q and a weight.  STEP: q | k | v rows, unrotated.
-template <int NT, bool FP8, int PARTS, bool WHOLE, bool STEP>
-__global__ void __launch_bounds__(THREADS, (NT == 1 && HD <= 128 && PARTS == 1) ? 3 : 2)
-quant_decode_kernel(const DecodeArgs a) {
-  constexpr int R = 8 * NT, N = (HD + 31) / 32;
-  extern __shared__ __align__(16) float so[];                    // [WARPS][R][HD], at the end
-  __shared__ __align__(16) __half qh[PARTS][R][HD];
-  __shared__ float qs[R], sm[WARPS][R], sl[WARPS][R], ww[WARPS][R], total[R];
-  pdl_trigger();
-  pdl_wait();
-  const int heads = a.nkv * a.chunks;
-  const int hc = blockIdx.x % heads, kvh = hc / a.chunks, chunk = hc - kvh * a.chunks;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const Piece pc = find_piece(a, blockIdx.x / heads, lane);
-  if (pc.b < 0) return;
-  const int G = a.nh / a.nkv, h0 = kvh * G + chunk * a.rows, nrows = min(a.rows, G - chunk * a.rows);
-  if (pc.len <= 0) {
-    for (int i = threadIdx.x; i < nrows * HD; i += THREADS) {
-      const size_t at = ((size_t)pc.b * a.nh + h0) * HD + i;
-      if (a.out_f32) reinterpret_cast<float*>(a.out)[at] = 0.f;
-      else reinterpret_cast<bf16*>(a.out)[at] = __float2bfloat16_rn(0.f);
-    }
-    return;
-  }
-  const int* tbl = a.block_table + (size_t)pc.b * a.table_stride;
-  const size_t row = (size_t)pc.b * a.q_stride;
-  const int p = pc.len - 1;
-  const float* cs = nullptr;
-  if constexpr (STEP) cs = a.table + (size_t)min(p, a.table_rows - 1) * a.rot;
-
-  if constexpr (STEP) {
-    // The new token's row of keys and of values: the piece that holds it writes it (every chunk of heads the
-    // same bytes) and reads it back with its tile.
-    if (pc.index == pc.pieces - 1 && warp < 2) {
-      const size_t at = row + (size_t)(a.nh + warp * a.nkv + kvh) * HD;
-      float x[N];
-      uint32_t top = 0;
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int c = i * 32 + lane;
-        x[i] = c >= HD ? 0.f : warp == 0 ? rotated_value(a, at, c, cs) : row_value(a, at, c);
-        top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-      }
-      const RowScale rs = row_scale(group_max_bits<32>(top), FP8);
-      const int lp = logical_page(a, p), off = p - lp * a.page;
-      const Place pl = place_of(a, kvh, fresh_index(tbl + lp), off);
-      uint8_t* dst = const_cast<uint8_t*>(pl.codes) + (size_t)warp * a.page * HD;
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (i * 32 + lane < HD) dst[i * 32 + lane] = (uint8_t)code_of(x[i], rs, FP8);
-      if (lane == 0) reinterpret_cast<float*>(const_cast<float2*>(pl.scales))[warp] = rs.scale;
-    }
-  }
-  // q in halves, a row's largest element in [2^14, 2^15)
-  for (int r = warp; r < R; r += WARPS) {
-    const size_t at = row + (size_t)(h0 + r) * HD;
-    float x[N];
-    uint32_t top = 0;
+struct Angles {
+  float c[N], s[N];
+  __device__ __forceinline__ void load(const DecodeArgs& a, int p, int lane) {
+    const float* cs = a.table + (size_t)min(p, a.table_rows - 1) * a.rot;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int c = i * 32 + lane;
-      x[i] = r >= nrows || c >= HD ? 0.f : STEP ? rotated_value(a, at, c, cs) : row_value(a, at, c);
-      top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+      const int ch = i * 32 + lane, half = a.rot >> 1;
+      const int j = a.neighbours ? ch >> 1 : ch >= half ? ch - half : ch;
+      c[i] = ch < a.rot ? __ldg(cs + j) : 1.f;
+      s[i] = ch < a.rot ? __ldg(cs + half + j) : 0.f;
     }
-    top = group_max_bits<32>(top);
+  }
+};
+__device__ __forceinline__ void load_partners(const DecodeArgs& a, size_t at, bool there, int lane, float (&y)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    bool second;
+    const int c = i * 32 + lane;
+    y[i] = there && c < a.rot ? row_value(a, at + partner(a, c, second)) : 0.f;
+  }
+}
+__device__ __forceinline__ void turn_row(const DecodeArgs& a, const Angles& an, int lane, float (&x)[N], const float (&y)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    bool second;
+    const int c = i * 32 + lane;
+    partner(a, c, second);
+    if (c < a.rot)
+      x[i] = second ? turned_second(y[i], x[i], an.c[i], an.s[i]) : turned_first(x[i], y[i], an.c[i], an.s[i]);
+  }
+}
+__device__ __forceinline__ uint32_t row_top(const float (&x)[N]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+  return group_max_bits<32>(top);
+}
+
+// ------------------------------------------------------------------------------------- a block's run
+// NT: tiles of 8 query heads.  PARTS: halves that make up q and a weight.  STEP: q | k | v rows, unrotated.
+template <int NT, bool FP8, int PARTS, bool WHOLE, bool STEP>
+__global__ void __launch_bounds__(THREADS, (NT == 1 && HD <= 128 && PARTS == 1) ? GF_OCC : 2)
+quant_decode_kernel(const DecodeArgs a) {
+  constexpr int R = 8 * NT, RW = R / WARPS;                      // rows of q in all, and a warp
+  constexpr bool RAISED = !FP8 && PARTS == 1;                    // K's codes as halves of code + 128
+  constexpr int OROW = HD + 2;                                   // (floats: two rows apart, other banks)
+  extern __shared__ __align__(16) uint8_t ring[];                // [WARPS][STAGES][keys | values][TILE][ROW]
+  float* so = reinterpret_cast<float*>(ring);                    // [WARPS][R][OROW], at an item's end
+  __shared__ __align__(16) __half qh[PARTS][R][HD];
+  __shared__ float qs[R], q_sum[R], sm[WARPS][R], sl[WARPS][R], back[WARPS];
+  __shared__ __align__(16) uint8_t fresh_row[2][HD];             // STEP: the new token's codes and scales
+  __shared__ float fresh_scale[2];
+  pdl_trigger();
+  pdl_wait();
+  const int heads = a.nkv * a.chunks, G = a.nh / a.nkv;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  uint8_t* mine = ring + warp * STAGES * STAGE;
+  Cursor cur;
+  if (a.stream) {
+    cur = find_run(a, blockIdx.x, gridDim.x, heads);
+  } else {
+    cur.b = blockIdx.x / heads, cur.hc = blockIdx.x - cur.b * heads, cur.len = request_length(a, cur.b);
+    cur.off = 0, cur.todo = cur.run = request_tiles(a, cur.len);
+  }
+  while (cur.todo > 0) {
+  const int kvh = cur.hc / a.chunks, chunk = cur.hc - kvh * a.chunks;
+  const int h0 = kvh * G + chunk * a.rows, nrows = min(a.rows, G - chunk * a.rows);
+  const int len = cur.len, p = len - 1, t0 = first_tile(a, len), n_tiles = request_tiles(a, len);
+  const int first = t0 + cur.off, last = first + min(n_tiles - cur.off, cur.todo);
+  const bool starts = cur.off == 0, ends = last == t0 + n_tiles;
+  const int lo = len > 0 ? first_visible_key(p, a.span) : 0;
+  const int* tbl = a.block_table + (size_t)cur.b * a.table_stride;
+  const size_t row = (size_t)cur.b * a.q_stride, out_at = ((size_t)cur.b * a.nh + h0) * HD;
+  if (a.stream && starts && threadIdx.x == 0)
+    a.info[cur.hc * a.B + cur.b] = make_int2(blockIdx.x, 1 + (t0 + n_tiles - last + cur.run - 1) / cur.run);
+  // where the next item is
+  cur.todo -= last - first, cur.off = 0;
+  if (++cur.b == a.B) cur.b = 0, ++cur.hc;
+  if (cur.todo > 0) cur.len = request_length(a, cur.b);
+  if (len == 0) {
+    for (int i = threadIdx.x; i < nrows * HD; i += THREADS) {
+      if (a.out_f32) reinterpret_cast<float*>(a.out)[out_at + i] = 0.f;
+      else reinterpret_cast<bf16*>(a.out)[out_at + i] = __float2bfloat16_rn(0.f);
+    }
+    continue;
+  }
+
+  // Everything that the item's start waits for is asked for at once: pages, q, the new token, angles.
+  const Tiles<WHOLE> tiles{a, tbl, kvh, lo, STEP ? p : len, last, lane};
+  int pages[STAGES];
+#pragma unroll
+  for (int i = 0; i < STAGES; ++i) pages[i] = tiles.page_of(first + warp + i * WARPS);
+  float x[RW][N], y[RW][N], nx[N], ny[N];
+  Angles an;
+  // the new token's row of keys (the last warp's, whose rows of q may not exist) and of values (the one before)
+  const bool news = STEP && ends && warp >= WARPS - 2, keys = warp == WARPS - 1;
+  const size_t new_at = row + (size_t)(a.nh + (keys ? 0 : a.nkv) + kvh) * HD;
+  int new_page = 0;
+#pragma unroll
+  for (int i = 0; i < RW; ++i) load_row(a, row + (size_t)(h0 + warp + i * WARPS) * HD, warp + i * WARPS < nrows, lane, x[i]);
+  if constexpr (STEP) {
+    an.load(a, p, lane);
+#pragma unroll
+    for (int i = 0; i < RW; ++i)
+      load_partners(a, row + (size_t)(h0 + warp + i * WARPS) * HD, warp + i * WARPS < nrows, lane, y[i]);
+    load_row(a, new_at, news, lane, nx);
+    load_partners(a, new_at, news && keys, lane, ny);
+    if (news) new_page = page_in(a, fresh_index(tbl + logical_page(a, p)));
+  }
+  // the first tiles are on their way while q is prepared (of the new token nothing is read)
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) {
+    const int tile = first + warp + i * WARPS;
+    if (tile < last) tiles.copy(mine + i * STAGE, tile, pages[i]);
+    asm volatile("cp.async.commit_group;\n");
+  }
+  int page_number = pages[STAGES - 1];
+  if constexpr (STEP) {
+    // The block that has the item's last tile writes the new token (every chunk of heads the same bytes) and
+    // keeps it for its own tile.
+    if (news) {
+      if (keys) turn_row(a, an, lane, nx, ny);
+      const RowScale rs = row_scale(row_top(nx), FP8);
+      const Place pl = place_of(a, kvh, new_page, p - logical_page(a, p) * a.page);
+      const int which = keys ? 0 : 1;
+      uint8_t* dst = const_cast<uint8_t*>(pl.codes) + (size_t)which * a.page * HD;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (i * 32 + lane < HD)
+          dst[i * 32 + lane] = fresh_row[which][i * 32 + lane] = (uint8_t)code_of(nx[i], rs, FP8);
+      if (lane == 0)
+        reinterpret_cast<float*>(const_cast<float2*>(pl.scales))[which] = fresh_scale[which] = rs.scale;
+    }
+#pragma unroll
+    for (int i = 0; i < RW; ++i) turn_row(a, an, lane, x[i], y[i]);
+  }
+  // q in halves, a row's largest element in [2^14, 2^15)
+#pragma unroll
+  for (int j = 0; j < RW; ++j) {
+    const int r = warp + j * WARPS;
+    const uint32_t top = row_top(x[j]);
     // 2^up takes the largest element to [2^14, 2^15); what is no number stays none
     const int e = top >= 0x7f800000u ? 127 : max((int)(top >> 23), 1), up = min(127 + 14 - e, 126);
     const float f = __uint_as_float((uint32_t)(127 + up) << 23);
+    float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int c = i * 32 + lane;
       if (c < HD) {
-        qh[0][r][c] = __float2half_rn(x[i] * f);
-        if constexpr (PARTS == 2) qh[1][r][c] = __float2half_rn(half_rest(x[i] * f));
+        qh[0][r][c] = __float2half_rn(x[j][i] * f);
+        if constexpr (RAISED) sum += __half2float(__float2half_rn(x[j][i] * f));
+        if constexpr (PARTS == 2) qh[1][r][c] = __float2half_rn(half_rest(x[j][i] * f));
       }
     }
-    if (lane == 0) qs[r] = a.scale * kLog2E * __uint_as_float((uint32_t)(127 - up) << 23);
+    if constexpr (RAISED) sum = warp_sum(sum);
+    if (lane == 0) {
+      qs[r] = a.scale * kLog2E * __uint_as_float((uint32_t)(127 - up) << 23);
+      q_sum[r] = sum;
+    }
   }
   __syncthreads();
 
   uint32_t qf[PARTS][NT][KWORDS][2];
 #pragma unroll
-  for (int w = 0; w < KWORDS; ++w) {
-    constexpr int STEPS = KW / 4;
-    const int c = ((w / STEPS) * 4 + t) * KW + (w % STEPS) * 4;      // the channels of a key's word w
+  for (int w = 0; w < KWORDS; ++w)
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int i = 0; i < PARTS; ++i) {
-        const uint2 two = *reinterpret_cast<const uint2*>(&qh[i][n * 8 + g][c]);
+        // (a thread's channels: a quarter of the head, four a word)
+        const uint2 two = *reinterpret_cast<const uint2*>(&qh[i][n * 8 + g][t * (HD / 4) + 4 * w]);
         qf[i][n][w][0] = two.x, qf[i][n][w][1] = two.y;
       }
-  }
-  float qscale[NT][2];
+  // a score is (product * qscale + qshift) * the key's scale
+  float qscale[NT][2], qshift[NT][2];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) qscale[n][0] = qs[n * 8 + 2 * t], qscale[n][1] = qs[n * 8 + 2 * t + 1];
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      qscale[n][j] = qs[n * 8 + 2 * t + j];
+      qshift[n][j] = -128.f * q_sum[n * 8 + 2 * t + j] * qscale[n][j];
+      if constexpr (RAISED) qscale[n][j] *= 16777216.f;
+    }
 
   float o[NT][MT][4], m[NT][2], l[NT][2];
   int f = 254;               // weights are multiplied by 2^(f - 127)
@@ -382,40 +504,70 @@ quant_decode_kernel(const DecodeArgs a) {
 #pragma unroll
     for (int i = 0; i < MT; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
   }
-  const auto page_at = [&](int tile) {
-    return WHOLE && tile < pc.last ? fresh_index(tbl + logical_page(a, tile * TILE)) : 0;
-  };
-  const auto work = [&](Tile& x, int tile) {
+
+  int at_stage = 0, to_stage = STAGES - 1;
+  for (int tile = first + warp; tile < last; tile += WARPS) {
+    wait_copies<STAGES - 2>();
+    __syncwarp();              // every lane's copies have landed, and the stage before has been read
+    uint8_t* stage = mine + at_stage * STAGE;
     const int c0 = tile * TILE;
-    const bool edge = c0 < pc.lo || c0 + TILE > pc.len;
+    float2 sc[2] = {tiles.scales(stage, g), tiles.scales(stage, g + 8)};
+    {
+      const int far = tile + (STAGES - 1) * WARPS;
+      const int ahead = tiles.page_of(far + WARPS);
+      if (far < last) tiles.copy(mine + to_stage * STAGE, far, page_number);
+      asm volatile("cp.async.commit_group;\n");
+      page_number = ahead;
+    }
+    at_stage = at_stage + 1 == STAGES ? 0 : at_stage + 1;
+    to_stage = to_stage + 1 == STAGES ? 0 : to_stage + 1;
+    if constexpr (STEP) {
+      if (c0 + TILE > p) {     // the tile of the new token
+        for (int i = lane; i < 2 * CH; i += 32) {
+          const int which = i / CH, ch = i - which * CH;
+          *reinterpret_cast<uint4*>(stage + (which * TILE + p - c0) * ROW + ch * 16) =
+              *reinterpret_cast<const uint4*>(&fresh_row[which][ch * 16]);
+        }
+        __syncwarp();
+        const float2 mine_sc = make_float2(fresh_scale[0], fresh_scale[1]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (c0 + g + 8 * i == p) sc[i] = mine_sc;
+      }
+    }
     float s[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+    {
+      uint32_t k[2][KWORDS];
 #pragma unroll
-    for (int w = 0; w < KWORDS; ++w) {
-      const uint32_t k0 = FP8 ? x.k[0][w] : x.k[0][w] ^ 0x80808080u, k1 = FP8 ? x.k[1][w] : x.k[1][w] ^ 0x80808080u;
-      const uint32_t A[4] = {halves<FP8>(k0, 0), halves<FP8>(k1, 0), halves<FP8>(k0, 1), halves<FP8>(k1, 1)};
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+        for (int j = 0; j < KWORDS / (KW / 4); ++j)
+          read_bytes<KW>(stage + (g + 8 * i) * ROW + t * (HD / 4) + j * KW, &k[i][j * (KW / 4)]);
 #pragma unroll
-        for (int i = PARTS - 1; i >= 0; --i) mma_f16(s[n], A, qf[i][n][w][0], qf[i][n][w][1]);
+      for (int w = 0; w < KWORDS; ++w) {
+        const uint32_t k0 = FP8 ? k[0][w] : k[0][w] ^ 0x80808080u, k1 = FP8 ? k[1][w] : k[1][w] ^ 0x80808080u;
+        uint32_t A[4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          A[2 * i] = RAISED ? raised_halves(k0, i) : halves<FP8>(k0, i);
+          A[2 * i + 1] = RAISED ? raised_halves(k1, i) : halves<FP8>(k1, i);
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = PARTS - 1; i >= 0; --i) mma_f16(s[n], A, qf[i][n][w][0], qf[i][n][w][1]);
+      }
     }
-    float2 sc[2] = {x.sc[0], x.sc[1]};
     bool seen[2] = {true, true};
-    if (edge) {
-      // masked keys: whatever lies there counts as nothing
+    if (c0 < lo || c0 + TILE > len) {
+      // masked keys: whatever lies there counts as nothing (their codes are zeros already)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int c = c0 + g + 8 * i;
-        seen[i] = c >= pc.lo && c < pc.len;
+        seen[i] = c >= lo && c < len;
         if (!seen[i]) sc[i] = make_float2(0.f, 0.f);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int c = c0 + 2 * t + (i & 1) + 8 * (i >> 1);
-        if (c < pc.lo || c >= pc.len)
-#pragma unroll
-          for (int w = 0; w < VWORDS; ++w) x.v[i][w] = 0u;
       }
     }
     float mn[NT][2];
@@ -424,8 +576,10 @@ quant_decode_kernel(const DecodeArgs a) {
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        s[n][j] = seen[0] ? s[n][j] * sc[0].x * qscale[n][j] : -INFINITY;
-        s[n][2 + j] = seen[1] ? s[n][2 + j] * sc[1].x * qscale[n][j] : -INFINITY;
+        const float s0 = RAISED ? fmaf(s[n][j], qscale[n][j], qshift[n][j]) : s[n][j] * qscale[n][j];
+        const float s1 = RAISED ? fmaf(s[n][2 + j], qscale[n][j], qshift[n][j]) : s[n][2 + j] * qscale[n][j];
+        s[n][j] = seen[0] ? s0 * sc[0].x : -INFINITY;
+        s[n][2 + j] = seen[1] ? s1 * sc[1].x : -INFINITY;
         float top = fmaxf(s[n][j], s[n][2 + j]);
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
@@ -437,7 +591,7 @@ quant_decode_kernel(const DecodeArgs a) {
     const uint32_t vtop = __reduce_max_sync(0xffffffffu, max(b0 < 0x7f800000u ? b0 : 0u, b1 < 0x7f800000u ? b1 : 0u));
     const int fn = min(f, 127 + 14 + 127 - (int)(vtop >> 23));
     if (__any_sync(0xffffffffu, moved) || fn != f) {
-      const float back = fn == f ? 1.f : f - fn > 126 ? 0.f : __uint_as_float((uint32_t)(127 + fn - f) << 23);
+      const float shrink = fn == f ? 1.f : f - fn > 126 ? 0.f : __uint_as_float((uint32_t)(127 + fn - f) << 23);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         float corr[2];
@@ -445,7 +599,7 @@ quant_decode_kernel(const DecodeArgs a) {
         for (int j = 0; j < 2; ++j) {
           corr[j] = mn[n][j] == m[n][j] ? 1.f : fast_exp2(m[n][j] - mn[n][j]);
           l[n][j] *= corr[j];
-          corr[j] *= back;
+          corr[j] *= shrink;
           m[n][j] = mn[n][j];
         }
 #pragma unroll
@@ -488,57 +642,36 @@ quant_decode_kernel(const DecodeArgs a) {
       }
     };
 #pragma unroll
-    for (int w = 0; w < VWORDS; ++w) {
-      if constexpr (!FP8) {
+    for (int j = 0; j < HD / (8 * VW); ++j) {
+      constexpr int WORDS = VW >= 4 ? VW / 4 : 1;
+      uint32_t v[4][WORDS];          // keys 2t, 2t + 1, 2t + 8, 2t + 9
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x.v[i][w] ^= 0x80808080u;
+      for (int i = 0; i < 4; ++i) {
+        read_bytes<VW>(stage + (TILE + 2 * t + (i & 1) + 8 * (i >> 1)) * ROW + (j * 8 + g) * VW, v[i]);
+        if constexpr (!FP8) {
+#pragma unroll
+          for (int w = 0; w < WORDS; ++w) v[i][w] ^= 0x80808080u;
+        }
       }
-      const uint32_t u0 = __byte_perm(x.v[0][w], x.v[1][w], 0x5140), u1 = __byte_perm(x.v[2][w], x.v[3][w], 0x5140);
-      const uint32_t A[4] = {halves<FP8>(u0, 0), halves<FP8>(u0, 1), halves<FP8>(u1, 0), halves<FP8>(u1, 1)};
-      if constexpr (VW >= 4) {
-        add(2 * w, A);
-        const uint32_t y0 = __byte_perm(x.v[0][w], x.v[1][w], 0x7362);
-        const uint32_t y1 = __byte_perm(x.v[2][w], x.v[3][w], 0x7362);
-        const uint32_t C[4] = {halves<FP8>(y0, 0), halves<FP8>(y0, 1), halves<FP8>(y1, 0), halves<FP8>(y1, 1)};
-        add(2 * w + 1, C);
-      } else {
-        add(w, A);
+#pragma unroll
+      for (int w = 0; w < WORDS; ++w) {
+        const uint32_t u0 = __byte_perm(v[0][w], v[1][w], 0x5140), u1 = __byte_perm(v[2][w], v[3][w], 0x5140);
+        const uint32_t A[4] = {halves<FP8>(u0, 0), halves<FP8>(u0, 1), halves<FP8>(u1, 0), halves<FP8>(u1, 1)};
+        if constexpr (VW >= 4) {
+          add(2 * (j * WORDS + w), A);
+          const uint32_t y0 = __byte_perm(v[0][w], v[1][w], 0x7362), y1 = __byte_perm(v[2][w], v[3][w], 0x7362);
+          const uint32_t C[4] = {halves<FP8>(y0, 0), halves<FP8>(y0, 1), halves<FP8>(y1, 0), halves<FP8>(y1, 1)};
+          add(2 * (j * WORDS + w) + 1, C);
+        } else {
+          add(j, A);
+        }
       }
-    }
-  };
-
-  int tile = pc.first + warp;
-  if (tile < pc.last) {
-    Tile x, y;
-    const int pg0 = page_at(tile);
-    int pg = page_at(tile + WARPS);
-    load_tile<WHOLE, true, kValuesAhead>(x, a, pc, kvh, tile, pg0, g, t);
-    int pg_x = pg0;
-    while (true) {
-      const int next = tile + WARPS;
-      const int pg_y = pg;
-      if constexpr (!kValuesAhead) load_tile<WHOLE, false, true>(x, a, pc, kvh, tile, pg_x, g, t);
-      if (next < pc.last) {
-        load_tile<WHOLE, true, kValuesAhead>(y, a, pc, kvh, next, pg_y, g, t);
-        pg = page_at(next + WARPS);
-      }
-      work(x, tile);
-      if (next >= pc.last) break;
-      tile = next + WARPS;
-      pg_x = pg;
-      if constexpr (!kValuesAhead) load_tile<WHOLE, false, true>(y, a, pc, kvh, next, pg_y, g, t);
-      if (tile < pc.last) {
-        load_tile<WHOLE, true, kValuesAhead>(x, a, pc, kvh, tile, pg_x, g, t);
-        pg = page_at(tile + WARPS);
-      }
-      work(y, next);
-      if (tile >= pc.last) break;
     }
   }
-
+  wait_copies<0>();
   // the four warps' results
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
+  for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 4);
@@ -546,119 +679,139 @@ quant_decode_kernel(const DecodeArgs a) {
       l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 16);
       if (g == 0) sm[warp][n * 8 + 2 * t + j] = m[n][j], sl[warp][n * 8 + 2 * t + j] = l[n][j];
     }
+  if (lane == 0) back[warp] = power_back(f);
+  __syncthreads();             // the ring becomes the warps' results
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
     constexpr int STEP_W = VW >= 4 ? VW / 4 : 1, PER = VW >= 4 ? 2 : 1;
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       const int w = i / PER;
       const int c = ((w / STEP_W) * 8 + g) * VW + (w % STEP_W) * 4 + (i % PER) * 2;
-      float* at = so + ((size_t)warp * R + n * 8 + 2 * t) * HD + c;
+      float* at = so + ((size_t)warp * R + n * 8 + 2 * t) * OROW + c;
       *reinterpret_cast<float2*>(at) = make_float2(o[n][i][0], o[n][i][2]);
-      *reinterpret_cast<float2*>(at + HD) = make_float2(o[n][i][1], o[n][i][3]);
+      *reinterpret_cast<float2*>(at + OROW) = make_float2(o[n][i][1], o[n][i][3]);
     }
   }
-  if (lane == 0) ww[warp][0] = power_back(f);
   __syncthreads();
-  float back = 0.f;
-  if (threadIdx.x < WARPS * R) back = ww[threadIdx.x / R][0];
-  __syncthreads();
-  if (threadIdx.x < WARPS * R) {
-    const int w = threadIdx.x / R, r = threadIdx.x - w * R;
+  const bool whole = starts && ends;
+  const size_t part = ((size_t)blockIdx.x * 2 + (starts ? 1 : 0)) * a.rows;
+  for (int i = threadIdx.x; i < nrows * (HD / 2); i += THREADS) {
+    const int r = i / (HD / 2), c = 2 * (i - r * (HD / 2));
     float top = sm[0][r];
 #pragma unroll
-    for (int i = 1; i < WARPS; ++i) top = fmaxf(top, sm[i][r]);
-    // (a warp without tiles has sums of zero; one whose scores are no numbers passes that on)
-    const float e = sm[w][r] == -INFINITY ? 0.f : fast_exp2(sm[w][r] - top);
-    ww[w][r] = e * back;
-    sl[w][r] *= e;
-  }
-  __syncthreads();
-  if (threadIdx.x < R) {
-    float sum = 0.f;
+    for (int w = 1; w < WARPS; ++w) top = fmaxf(top, sm[w][r]);
+    float sum = 0.f, v0 = 0.f, v1 = 0.f;
 #pragma unroll
-    for (int i = 0; i < WARPS; ++i) sum += sl[i][threadIdx.x];
-    total[threadIdx.x] = sum;
+    for (int w = 0; w < WARPS; ++w) {
+      // (a warp without tiles has sums of zero; one whose scores are no numbers passes that on)
+      const float e = sm[w][r] == -INFINITY ? 0.f : fast_exp2(sm[w][r] - top), eb = e * back[w];
+      const float2 v = *reinterpret_cast<const float2*>(so + (size_t)(w * R + r) * OROW + c);
+      sum += e * sl[w][r], v0 += eb * v.x, v1 += eb * v.y;
+    }
+    v0 /= sum, v1 /= sum;
+    const size_t at = out_at + (size_t)r * HD + c;
+    if (!whole) {
+      *reinterpret_cast<float2*>(a.po + (part + r) * HD + c) = make_float2(v0, v1);
+      if (c == 0) a.pml[part + r] = make_float2(top, sum);
+    } else if (a.out_f32) {
+      *reinterpret_cast<float2*>(reinterpret_cast<float*>(a.out) + at) = make_float2(v0, v1);
+    } else {
+      *reinterpret_cast<__nv_bfloat162*>(reinterpret_cast<bf16*>(a.out) + at) = __floats2bfloat162_rn(v0, v1);
+    }
   }
-  __syncthreads();
-  const bool single = pc.pieces == 1;
-  float* po = a.po + (size_t)blockIdx.x * a.rows * HD;
-  for (int i = threadIdx.x; i < nrows * HD; i += THREADS) {
-    const int r = i / HD;
-    float acc = 0.f;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) acc += ww[w][r] * so[(size_t)w * R * HD + i];
-    acc /= total[r];
-    const size_t at = ((size_t)pc.b * a.nh + h0) * HD + i;
-    if (!single) po[i] = acc;
-    else if (a.out_f32) reinterpret_cast<float*>(a.out)[at] = acc;
-    else reinterpret_cast<bf16*>(a.out)[at] = __float2bfloat16_rn(acc);
-  }
-  if (!single && threadIdx.x < nrows) {
-    float top = sm[0][threadIdx.x];
-#pragma unroll
-    for (int i = 1; i < WARPS; ++i) top = fmaxf(top, sm[i][threadIdx.x]);
-    a.pml[(size_t)blockIdx.x * a.rows + threadIdx.x] = make_float2(top, total[threadIdx.x]);
+  if (cur.todo > 0) __syncthreads();
   }
 }
 
-// A block a (request, chunk of heads, head): the pieces' results, weighted by their shares of the sum, in order.
-constexpr int JOIN_THREADS = 256, JOIN_LANES = HD / 4, JOIN_GROUPS = JOIN_THREADS / JOIN_LANES;
+// A block an item and `gridDim.y`-th of its heads: the pieces' results, weighted by their shares of the sum.
+// A team of HD / 4 threads takes a head where there are few pieces, else every TEAMS-th piece of every head:
+// its loads are then under way together, and the teams' sums are added in order.
+constexpr int JOIN_THREADS = 256, TEAM = HD / 4, TEAMS = JOIN_THREADS / TEAM, JOIN_AT_ONCE = 8, FEW_PIECES = 8;
+struct Joined {
+  float4 o;
+  float m, l;
+  __device__ __forceinline__ void add(float4 v, float vm, float vl) {
+    const float top = fmaxf(m, vm);
+    const float mine = m == -INFINITY ? 0.f : fast_exp2(m - top);
+    const float w = (vm == -INFINITY ? 0.f : fast_exp2(vm - top)) * vl;
+    o.x = fmaf(w, v.x, mine * o.x), o.y = fmaf(w, v.y, mine * o.y);
+    o.z = fmaf(w, v.z, mine * o.z), o.w = fmaf(w, v.w, mine * o.w);
+    l = mine * l + w, m = top;
+  }
+};
 __global__ void __launch_bounds__(JOIN_THREADS)
 quant_join_kernel(const DecodeArgs a) {
-  __shared__ float4 part[JOIN_GROUPS][JOIN_LANES];
-  __shared__ float part_l[JOIN_GROUPS];
+  __shared__ float4 part[TEAMS][TEAM];
+  __shared__ float2 part_ml[TEAMS];
   pdl_trigger();
   pdl_wait();
-  const int h = blockIdx.x, b = blockIdx.y, G = a.nh / a.nkv, heads = a.nkv * a.chunks;
-  const int kvh = h / G, chunk = (h - kvh * G) / a.rows, r = h - kvh * G - chunk * a.rows;
-  const int lane = threadIdx.x & 31;
-  const int size = piece_size(a, lane);
-  int before = 0, pieces = 1;
-  for (int b0 = 0; b0 <= b; b0 += 32) {
-    const int i = b0 + lane;
-    int n = i <= b ? max(1, (request_tiles(a, request_length(a, i)) + size - 1) / size) : 0;
-    pieces = __shfl_sync(0xffffffffu, n, b & 31);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-    before += n;
-  }
-  if (pieces == 1) return;
-  before -= pieces;
-  const float2* ml = a.pml + ((size_t)before * heads + kvh * a.chunks + chunk) * a.rows + r;
-  const float* po = a.po + (((size_t)before * heads + kvh * a.chunks + chunk) * a.rows + r) * HD;
-  const size_t step = (size_t)heads * a.rows;
-  float top = -INFINITY;
-  for (int i = lane; i < pieces; i += 32) top = fmaxf(top, __ldcg(ml + i * step).x);
-  top = warp_max(top);
-  const int group = threadIdx.x / JOIN_LANES, c = threadIdx.x - group * JOIN_LANES;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float sum = 0.f;
-#pragma unroll 4
-  for (int i = group; i < pieces && group < JOIN_GROUPS; i += JOIN_GROUPS) {
-    const float2 x = __ldcg(ml + i * step);
-    const float4 v = __ldcg(reinterpret_cast<const float4*>(po + i * step * HD) + c);
-    const float w = (x.x == -INFINITY ? 0.f : fast_exp2(x.x - top)) * x.y;
-    sum += w;
-    acc.x += w * v.x, acc.y += w * v.y, acc.z += w * v.z, acc.w += w * v.w;
-  }
-  if (group < JOIN_GROUPS) part[group][c] = acc;          // (head sizes that do not divide the block)
-  if (group < JOIN_GROUPS && c == 0) part_l[group] = sum;
-  __syncthreads();
-  if (group == 0) {
-#pragma unroll
-    for (int i = 1; i < JOIN_GROUPS; ++i) {
-      const float4 v = part[i][c];
-      acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
-      sum += part_l[i];
-    }
-    const float inv = 1.f / sum;
-    const size_t at = ((size_t)b * a.nh + h) * HD + 4 * c;
+  const int hc = blockIdx.x / a.B, b = blockIdx.x - hc * a.B;
+  const int kvh = hc / a.chunks, chunk = hc - kvh * a.chunks, G = a.nh / a.nkv;
+  const int h0 = kvh * G + chunk * a.rows, nrows = min(a.rows, G - chunk * a.rows);
+  const int2 info = __ldcg(a.info + blockIdx.x);
+  if (info.y == 1) return;
+  const int team = threadIdx.x / TEAM, c = threadIdx.x - team * TEAM;
+  // the item's first piece is the second part of its block, the others are the first parts of theirs
+  const size_t first = (size_t)info.x * 2 * a.rows;
+  const bool few = info.y <= FEW_PIECES;
+  const int start = few ? 0 : team, stride = few ? 1 : TEAMS;
+  const auto store = [&](int r, float4 v, float inv) {
+    const size_t at = ((size_t)b * a.nh + h0 + r) * HD + 4 * c;
+    v.x *= inv, v.y *= inv, v.z *= inv, v.w *= inv;
     if (a.out_f32) {
-      *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + at) =
-          make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+      *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + at) = v;
     } else {
       __nv_bfloat162* d = reinterpret_cast<__nv_bfloat162*>(reinterpret_cast<bf16*>(a.out) + at);
-      d[0] = __floats2bfloat162_rn(acc.x * inv, acc.y * inv);
-      d[1] = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
+      d[0] = __floats2bfloat162_rn(v.x, v.y);
+      d[1] = __floats2bfloat162_rn(v.z, v.w);
+    }
+  };
+  for (int r0 = few ? blockIdx.y * TEAMS : blockIdx.y; r0 < nrows; r0 += few ? gridDim.y * TEAMS : gridDim.y) {
+    const int r = few ? r0 + team : r0;
+    Joined sum = {make_float4(0.f, 0.f, 0.f, 0.f), -INFINITY, 0.f};
+    if (team < TEAMS && r < nrows) {                      // (head sizes that do not divide the block)
+      const float2* ml = a.pml + first + r;
+      const float* po = a.po + (first + r) * HD + 4 * c;
+      for (int i0 = start; i0 < info.y; i0 += JOIN_AT_ONCE * stride) {
+        float2 x[JOIN_AT_ONCE];
+        float4 v[JOIN_AT_ONCE];
+#pragma unroll
+        for (int k = 0; k < JOIN_AT_ONCE; ++k) {
+          const int i = i0 + k * stride;
+          x[k] = make_float2(-INFINITY, 0.f), v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (i < info.y) {
+            const size_t part = (size_t)(i ? 2 * i : 1) * a.rows;
+            x[k] = __ldcg(ml + part);
+            v[k] = __ldcg(reinterpret_cast<const float4*>(po + part * HD));
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < JOIN_AT_ONCE; ++k) sum.add(v[k], x[k].x, x[k].y);
+      }
+    }
+    if (few) {
+      if (team < TEAMS && r < nrows) store(r, sum.o, 1.f / sum.l);
+      continue;
+    }
+    __syncthreads();                                      // (the row before has been read)
+    if (team < TEAMS) part[team][c] = sum.o;
+    if (team < TEAMS && c == 0) part_ml[team] = make_float2(sum.m, sum.l);
+    __syncthreads();
+    if (team == 0) {
+      // a team's o is not divided by its sum
+#pragma unroll
+      for (int i = 1; i < TEAMS; ++i) {
+        const float4 v = part[i][c];
+        const float2 x = part_ml[i];
+        const float top = fmaxf(sum.m, x.x);
+        const float mine = sum.m == -INFINITY ? 0.f : fast_exp2(sum.m - top);
+        const float w = x.x == -INFINITY ? 0.f : fast_exp2(x.x - top);
+        sum.o.x = fmaf(w, v.x, mine * sum.o.x), sum.o.y = fmaf(w, v.y, mine * sum.o.y);
+        sum.o.z = fmaf(w, v.z, mine * sum.o.z), sum.o.w = fmaf(w, v.w, mine * sum.o.w);
+        sum.l = mine * sum.l + w * x.y, sum.m = top;
+      }
+      store(r, sum.o, 1.f / sum.l);
     }
   }
 }
@@ -666,7 +819,7 @@ quant_join_kernel(const DecodeArgs a) {
 template <int NT, bool FP8, int PARTS, bool WHOLE, bool STEP>
 int launch_decode(DecodeArgs a, int sms, void* scratch, size_t scratch_bytes, cudaStream_t stream) {
   constexpr auto kernel = quant_decode_kernel<NT, FP8, PARTS, WHOLE, STEP>;
-  constexpr int smem = WARPS * 8 * NT * HD * 4;
+  constexpr int smem = std::max(WARPS * STAGES * STAGE, WARPS * 8 * NT * (HD + 2) * 4);
   static OncePerDevice once;
   static int blocks_a_sm[OncePerDevice::kMaxDevices];
   int dev = 0;
@@ -678,27 +831,27 @@ int launch_decode(DecodeArgs a, int sms, void* scratch, size_t scratch_bytes, cu
   });
   if (rc) return rc;
   if (cudaGetDevice(&dev) != cudaSuccess) return -9;
-  a.slots = sms * std::min(std::max(1, blocks_a_sm[dev]), kMostBlocks);
-  const int heads = a.nkv * a.chunks, N = a.slots / heads;
-  // the most pieces there can be (find_piece), and the most there are worth their while
-  long long pieces = 2 * a.B <= N ? N + 1 : (2LL * a.slots + heads - 1) / heads + a.B;
+  const int heads = a.nkv * a.chunks;
+  const long long items = (long long)a.B * heads;
   const long long keys = a.span ? std::min(std::abs((long long)a.span), (long long)a.limit) : a.limit;
-  const long long tiles = (keys + TILE - 1) / TILE + 1;
-  pieces = std::min(pieces, (long long)a.B * ((tiles + kLeastTiles - 1) / kLeastTiles));
-  const long long blocks = std::max(pieces, (long long)a.B) * heads;
-  if (blocks > 0x7fffffffLL) return -5;
-  const bool joined = pieces > a.B;
-  if (joined) {
-    const size_t rows = (size_t)blocks * a.rows;
-    if (scratch_bytes < rows * (HD + 2) * 4) return -7;
-    a.po = (float*)scratch;
-    a.pml = (float2*)((float*)scratch + rows * HD);
+  a.stream = keys > kShortKeys;
+  const long long blocks = a.stream ? (long long)sms * std::min(std::max(1, blocks_a_sm[dev]), kMostBlocks) : items;
+  if (items > 0x7fffffffLL || blocks > 0x7fffffffLL) return -5;
+  if (a.stream) {
+    const size_t rows = (size_t)blocks * 2 * a.rows, head = ((size_t)items * 8 + 15) / 16 * 16;
+    if (scratch_bytes < head + rows * (HD + 2) * 4) return -7;
+    a.info = (int2*)scratch;
+    a.po = (float*)((char*)scratch + head);
+    a.pml = (float2*)(a.po + rows * HD);
   }
-  int e = launch_kernel(kernel, dim3((unsigned)blocks), dim3(THREADS), smem, stream, a);
-  if (e || !joined) return e;
-  return launch_kernel(quant_join_kernel, dim3(a.nh, a.B), dim3(JOIN_THREADS), 0, stream, a);
+  const int e = launch_kernel(kernel, dim3((unsigned)blocks), dim3(THREADS), smem, stream, a);
+  if (e || !a.stream) return e;
+  // few items: a block a head
+  const int split = items * a.rows <= 8LL * sms ? a.rows : 1;
+  return launch_kernel(quant_join_kernel, dim3((unsigned)items, split), dim3(JOIN_THREADS), 0, stream, a);
 }
 
+}  // namespace
 }  // namespace gf
 
 using namespace gf;
@@ -707,26 +860,27 @@ GF_DEFINE_PDL_SWITCH
 
 // Scratch that any call with these sizes is content with.
 GF_EXPORT long long gf_quant_decode_scratch(int B, int nh, int nkv, int sms) {
-  const int G = nh / nkv, chunks = (G + 15) / 16, rows = (G + chunks - 1) / chunks, heads = nkv * chunks;
-  const long long slots = (long long)sms * kMostBlocks;
-  return (2 * slots + (long long)(B + 2) * heads) * rows * (HD + 2) * 4;
+  const int G = nh / nkv, chunks = (G + 15) / 16, rows = (G + chunks - 1) / chunks;
+  return (long long)sms * kMostBlocks * 2 * rows * (HD + 2) * 4 + 8LL * B * nkv * chunks + 16;
 }
 
 // q [B, nh HD], or with `step` q | k | v [B, (nh + 2 nkv) HD] and the table of angles as gf_quant_write takes it.
 GF_EXPORT int gf_quant_decode(const void* q, int q_stride, int q_f32, void* codes, int fp8, float* scales,
-                              const int* block_table, int table_stride, int table_width, const int* lengths,
+                              const int* block_table, int table_stride, int table_width, const int* lengths, int pages,
                               void* out, int out_f32, int B, int nh, int nkv, int page, int span, float scale,
                               int step, const float* table, int table_rows, int rot, int neighbours, int sms,
                               void* scratch, long long scratch_bytes, void* stream) {
   if (B <= 0) return B < 0 ? -3 : 0;
-  if (nkv < 1 || nh < nkv || nh % nkv || page < 1 || table_width < 0 || B > 65535 || sms < 1) return -3;
+  if (nkv < 1 || nh < nkv || nh % nkv || page < 1 || pages < 1 || table_width < 0 || B > 65535 || sms < 1)
+    return -3;
+  if ((size_t)codes % 16 || (size_t)scales % 8) return -3;
   if (step && (rot < 0 || rot % 2 || rot > HD || (rot && (!table || table_rows < 1)))) return -3;
   DecodeArgs a = {};
   a.q = q, a.q_stride = q_stride, a.q_f32 = q_f32;
   a.codes = (uint8_t*)codes, a.scales = scales;
   a.block_table = block_table, a.table_stride = table_stride;
   a.limit = (int)min((long long)table_width * page, 0x7fffffe0LL);
-  a.lengths = lengths, a.out = out, a.out_f32 = out_f32;
+  a.pages = pages, a.lengths = lengths, a.out = out, a.out_f32 = out_f32;
   a.B = B, a.nh = nh, a.nkv = nkv, a.page = page, a.span = span, a.scale = scale;
   a.page_shift = (page & (page - 1)) == 0 ? __builtin_ctz(page) : -1;
   a.table = table, a.table_rows = table_rows > 0 ? table_rows : 1, a.rot = rot, a.neighbours = neighbours;
@@ -740,7 +894,7 @@ GF_EXPORT int gf_quant_decode(const void* q, int q_stride, int q_f32, void* code
     return x ? next(std::true_type()) : next(std::false_type());
   };
   return pick_bool(fp8 != 0, [&](auto kind) {
-    return pick_bool(page % TILE == 0, [&](auto whole) {
+    return pick_bool(page % TILE == 0 && (size_t)scales % 16 == 0, [&](auto whole) {
       return pick_bool(step != 0, [&](auto fused) {
         using One = std::integral_constant<int, 1>;
         using Two = std::integral_constant<int, 2>;

@@ -69,7 +69,7 @@ constexpr int kMostBlocks = 8;          // of the blocks that fit an SM, so many
 
 struct DecodeArgs {
   const void* q;              // rows of q, or of q | k | v (fused)
-  int q_stride, q_f32;
+  int q_stride;
   uint8_t* codes;
   float* scales;
   const int* block_table;
@@ -144,10 +144,12 @@ __device__ __forceinline__ Cursor find_run(const DecodeArgs& a, int k, int block
     total += counts[w];
   }
   const unsigned long long all = (unsigned long long)total * heads;
-  const unsigned long long run = max((all + blocks - 1) / blocks, (unsigned long long)kLeastTiles);
-  const unsigned long long at = run * k;
+  const bool narrow = all < 0xffff0000ull;         // (64-bit divisions cost more than the rest of this)
+  const unsigned long long share = narrow ? ((unsigned)all + blocks - 1) / (unsigned)blocks : (all + blocks - 1) / blocks;
+  const unsigned long long run = max(share, (unsigned long long)kLeastTiles), at = run * k;
   if (at < all) {
-    const unsigned hc = (unsigned)(at / total), rest = (unsigned)(at - (unsigned long long)hc * total);
+    const unsigned hc = narrow ? (unsigned)at / total : (unsigned)(at / total);
+    const unsigned rest = (unsigned)(at - (unsigned long long)hc * total);
     if (rest >= start && rest < start + mine) {
       int left = (int)(rest - start);
       for (int b = b0; b < b1; ++b) {
@@ -291,7 +293,11 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
 }
 // what a float loses when it is rounded to a half
 __device__ __forceinline__ float half_rest(float x) { return x - __half2float(__float2half_rn(x)); }
-// 2^(127 - f) for 14 <= f <= 254
+// Weights are p times a value's scale times 2^(f - 127).  p is at most 2^kSlack; with a scale's exponent (biased) e,
+// f <= kTop - e keeps the weight below 2^15.
+constexpr float kSlack = 7.f;
+constexpr int kTop = 127 + 127 + 14 - 7;
+// 2^(127 - f) for 7 <= f <= 254
 __device__ __forceinline__ float power_back(int f) {
   return __uint_as_float(f == 254 ? 0x00400000u : (uint32_t)(254 - f) << 23);
 }
@@ -299,12 +305,13 @@ __device__ __forceinline__ float power_back(int f) {
 // ------------------------------------------------------------------------------------- q, and the new token
 // A lane's channels of head rows: lane, lane + 32, ...  Everything is asked for before anything is used.
 constexpr int N = (HD + 31) / 32;
-__device__ __forceinline__ float row_value(const DecodeArgs& a, size_t at) {
-  return a.q_f32 ? fresh(reinterpret_cast<const float*>(a.q) + at) : fresh(reinterpret_cast<const bf16*>(a.q) + at);
+template <typename T> __device__ __forceinline__ float row_value(const DecodeArgs& a, size_t at) {
+  return fresh(reinterpret_cast<const T*>(a.q) + at);
 }
+template <typename T>
 __device__ __forceinline__ void load_row(const DecodeArgs& a, size_t at, bool there, int lane, float (&x)[N]) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) x[i] = there && i * 32 + lane < HD ? row_value(a, at + i * 32 + lane) : 0.f;
+  for (int i = 0; i < N; ++i) x[i] = there && i * 32 + lane < HD ? row_value<T>(a, at + i * 32 + lane) : 0.f;
 }
 // The channel that channel c turns with, and which of the pair c is.
 __device__ __forceinline__ int partner(const DecodeArgs& a, int c, bool& second) {
@@ -325,12 +332,13 @@ struct Angles {
     }
   }
 };
+template <typename T>
 __device__ __forceinline__ void load_partners(const DecodeArgs& a, size_t at, bool there, int lane, float (&y)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     bool second;
     const int c = i * 32 + lane;
-    y[i] = there && c < a.rot ? row_value(a, at + partner(a, c, second)) : 0.f;
+    y[i] = there && c < a.rot ? row_value<T>(a, at + partner(a, c, second)) : 0.f;
   }
 }
 __device__ __forceinline__ void turn_row(const DecodeArgs& a, const Angles& an, int lane, float (&x)[N], const float (&y)[N]) {
@@ -351,17 +359,26 @@ __device__ __forceinline__ uint32_t row_top(const float (&x)[N]) {
 }
 
 // ------------------------------------------------------------------------------------- a block's run
-// NT: tiles of 8 query heads.  PARTS: halves that make up q and a weight.  STEP: q | k | v rows, unrotated.
-template <int NT, bool FP8, int PARTS, bool WHOLE, bool STEP>
-__global__ void __launch_bounds__(THREADS, (NT == 1 && HD <= 128 && PARTS == 1) ? GF_OCC : 2)
+struct Item {
+  int b, hc, len, lo, first, last;         // its tiles here
+  bool starts, ends;                       // whether they are its first, its last
+};
+// NT: tiles of 8 query heads.  T: the type of q and the result (32-bit ones take two halves each).  STEP: q | k | v
+// rows, unrotated.
+template <int NT, bool FP8, typename T, bool WHOLE, bool STEP>
+__global__ void __launch_bounds__(THREADS, (NT == 1 && HD <= 128 && sizeof(T) == 2) ? GF_OCC : 2)
 quant_decode_kernel(const DecodeArgs a) {
+  constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;
   constexpr int R = 8 * NT, RW = R / WARPS;                      // rows of q in all, and a warp
   constexpr bool RAISED = !FP8 && PARTS == 1;                    // K's codes as halves of code + 128
   constexpr int OROW = HD + 2;                                   // (floats: two rows apart, other banks)
-  extern __shared__ __align__(16) uint8_t ring[];                // [WARPS][STAGES][keys | values][TILE][ROW]
-  float* so = reinterpret_cast<float*>(ring);                    // [WARPS][R][OROW], at an item's end
+  // [WARPS][STAGES][keys | values][TILE][ROW]; a warp's results at an item's end go into its stage that is not under
+  // way, or where that is too small behind the ring
+  extern __shared__ __align__(16) uint8_t ring[];
+  constexpr bool IN_STAGE = R * OROW * 4 <= STAGE;
   __shared__ __align__(16) __half qh[PARTS][R][HD];
   __shared__ float qs[R], q_sum[R], sm[WARPS][R], sl[WARPS][R], back[WARPS];
+  __shared__ int so_at[WARPS];
   __shared__ __align__(16) uint8_t fresh_row[2][HD];             // STEP: the new token's codes and scales
   __shared__ float fresh_scale[2];
   pdl_trigger();
@@ -376,351 +393,398 @@ quant_decode_kernel(const DecodeArgs a) {
     cur.b = blockIdx.x / heads, cur.hc = blockIdx.x - cur.b * heads, cur.len = request_length(a, cur.b);
     cur.off = 0, cur.todo = cur.run = request_tiles(a, cur.len);
   }
-  while (cur.todo > 0) {
-  const int kvh = cur.hc / a.chunks, chunk = cur.hc - kvh * a.chunks;
-  const int h0 = kvh * G + chunk * a.rows, nrows = min(a.rows, G - chunk * a.rows);
-  const int len = cur.len, p = len - 1, t0 = first_tile(a, len), n_tiles = request_tiles(a, len);
-  const int first = t0 + cur.off, last = first + min(n_tiles - cur.off, cur.todo);
-  const bool starts = cur.off == 0, ends = last == t0 + n_tiles;
-  const int lo = len > 0 ? first_visible_key(p, a.span) : 0;
-  const int* tbl = a.block_table + (size_t)cur.b * a.table_stride;
-  const size_t row = (size_t)cur.b * a.q_stride, out_at = ((size_t)cur.b * a.nh + h0) * HD;
-  if (a.stream && starts && threadIdx.x == 0)
-    a.info[cur.hc * a.B + cur.b] = make_int2(blockIdx.x, 1 + (t0 + n_tiles - last + cur.run - 1) / cur.run);
-  // where the next item is
-  cur.todo -= last - first, cur.off = 0;
-  if (++cur.b == a.B) cur.b = 0, ++cur.hc;
-  if (cur.todo > 0) cur.len = request_length(a, cur.b);
-  if (len == 0) {
-    for (int i = threadIdx.x; i < nrows * HD; i += THREADS) {
-      if (a.out_f32) reinterpret_cast<float*>(a.out)[out_at + i] = 0.f;
-      else reinterpret_cast<bf16*>(a.out)[out_at + i] = __float2bfloat16_rn(0.f);
+  const auto head_of = [&](int hc) { return (hc / a.chunks) * G + (hc % a.chunks) * a.rows; };
+  const auto rows_of = [&](int hc) { return min(a.rows, G - (hc % a.chunks) * a.rows); };
+  // The block's next item that has tokens; the others get their zeros.
+  int ahead_len = 0;                       // the length of the request behind the cursor's, on its way
+  const auto next_item = [&](Item& it) {
+    while (cur.todo > 0) {
+      const int len = cur.len, t0 = first_tile(a, len), n = request_tiles(a, len);
+      it.b = cur.b, it.hc = cur.hc, it.len = len, it.lo = len > 0 ? first_visible_key(len - 1, a.span) : 0;
+      it.first = t0 + cur.off, it.last = it.first + min(n - cur.off, cur.todo);
+      it.starts = cur.off == 0, it.ends = it.last == t0 + n;
+      if (a.stream && it.starts && threadIdx.x == 0)
+        a.info[it.hc * a.B + it.b] = make_int2(blockIdx.x, 1 + (t0 + n - it.last + cur.run - 1) / cur.run);
+      cur.todo -= it.last - it.first, cur.off = 0;
+      if (++cur.b == a.B) cur.b = 0, ++cur.hc;
+      if (len > 0) return true;
+      for (int i = threadIdx.x; i < rows_of(it.hc) * HD; i += THREADS)
+        reinterpret_cast<T*>(a.out)[((size_t)it.b * a.nh + head_of(it.hc)) * HD + i] = from_f32<T>(0.f);
+      if (cur.todo > 0) cur.len = request_length(a, cur.b);
     }
-    continue;
-  }
+    return false;
+  };
 
-  // Everything that the item's start waits for is asked for at once: pages, q, the new token, angles.
-  const Tiles<WHOLE> tiles{a, tbl, kvh, lo, STEP ? p : len, last, lane};
   int pages[STAGES];
+  const auto tiles_of = [&](const Item& it) {
+    return Tiles<WHOLE>{a, a.block_table + (size_t)it.b * a.table_stride, it.hc / a.chunks, it.lo,
+                        STEP ? it.len - 1 : it.len, it.last, lane};
+  };
+  const auto ask_pages = [&](const Item& it) {
 #pragma unroll
-  for (int i = 0; i < STAGES; ++i) pages[i] = tiles.page_of(first + warp + i * WARPS);
-  float x[RW][N], y[RW][N], nx[N], ny[N];
-  Angles an;
-  // the new token's row of keys (the last warp's, whose rows of q may not exist) and of values (the one before)
-  const bool news = STEP && ends && warp >= WARPS - 2, keys = warp == WARPS - 1;
-  const size_t new_at = row + (size_t)(a.nh + (keys ? 0 : a.nkv) + kvh) * HD;
-  int new_page = 0;
-#pragma unroll
-  for (int i = 0; i < RW; ++i) load_row(a, row + (size_t)(h0 + warp + i * WARPS) * HD, warp + i * WARPS < nrows, lane, x[i]);
-  if constexpr (STEP) {
-    an.load(a, p, lane);
-#pragma unroll
-    for (int i = 0; i < RW; ++i)
-      load_partners(a, row + (size_t)(h0 + warp + i * WARPS) * HD, warp + i * WARPS < nrows, lane, y[i]);
-    load_row(a, new_at, news, lane, nx);
-    load_partners(a, new_at, news && keys, lane, ny);
-    if (news) new_page = page_in(a, fresh_index(tbl + logical_page(a, p)));
-  }
-  // the first tiles are on their way while q is prepared (of the new token nothing is read)
-#pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) {
-    const int tile = first + warp + i * WARPS;
-    if (tile < last) tiles.copy(mine + i * STAGE, tile, pages[i]);
-    asm volatile("cp.async.commit_group;\n");
-  }
-  int page_number = pages[STAGES - 1];
-  if constexpr (STEP) {
-    // The block that has the item's last tile writes the new token (every chunk of heads the same bytes) and
-    // keeps it for its own tile.
-    if (news) {
-      if (keys) turn_row(a, an, lane, nx, ny);
-      const RowScale rs = row_scale(row_top(nx), FP8);
-      const Place pl = place_of(a, kvh, new_page, p - logical_page(a, p) * a.page);
-      const int which = keys ? 0 : 1;
-      uint8_t* dst = const_cast<uint8_t*>(pl.codes) + (size_t)which * a.page * HD;
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (i * 32 + lane < HD)
-          dst[i * 32 + lane] = fresh_row[which][i * 32 + lane] = (uint8_t)code_of(nx[i], rs, FP8);
-      if (lane == 0)
-        reinterpret_cast<float*>(const_cast<float2*>(pl.scales))[which] = fresh_scale[which] = rs.scale;
-    }
-#pragma unroll
-    for (int i = 0; i < RW; ++i) turn_row(a, an, lane, x[i], y[i]);
-  }
-  // q in halves, a row's largest element in [2^14, 2^15)
-#pragma unroll
-  for (int j = 0; j < RW; ++j) {
-    const int r = warp + j * WARPS;
-    const uint32_t top = row_top(x[j]);
-    // 2^up takes the largest element to [2^14, 2^15); what is no number stays none
-    const int e = top >= 0x7f800000u ? 127 : max((int)(top >> 23), 1), up = min(127 + 14 - e, 126);
-    const float f = __uint_as_float((uint32_t)(127 + up) << 23);
-    float sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = i * 32 + lane;
-      if (c < HD) {
-        qh[0][r][c] = __float2half_rn(x[j][i] * f);
-        if constexpr (RAISED) sum += __half2float(__float2half_rn(x[j][i] * f));
-        if constexpr (PARTS == 2) qh[1][r][c] = __float2half_rn(half_rest(x[j][i] * f));
-      }
-    }
-    if constexpr (RAISED) sum = warp_sum(sum);
-    if (lane == 0) {
-      qs[r] = a.scale * kLog2E * __uint_as_float((uint32_t)(127 - up) << 23);
-      q_sum[r] = sum;
-    }
-  }
-  __syncthreads();
-
-  uint32_t qf[PARTS][NT][KWORDS][2];
-#pragma unroll
-  for (int w = 0; w < KWORDS; ++w)
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int i = 0; i < PARTS; ++i) {
-        // (a thread's channels: a quarter of the head, four a word)
-        const uint2 two = *reinterpret_cast<const uint2*>(&qh[i][n * 8 + g][t * (HD / 4) + 4 * w]);
-        qf[i][n][w][0] = two.x, qf[i][n][w][1] = two.y;
-      }
-  // a score is (product * qscale + qshift) * the key's scale
-  float qscale[NT][2], qshift[NT][2];
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      qscale[n][j] = qs[n * 8 + 2 * t + j];
-      qshift[n][j] = -128.f * q_sum[n * 8 + 2 * t + j] * qscale[n][j];
-      if constexpr (RAISED) qscale[n][j] *= 16777216.f;
-    }
+    for (int i = 0; i < STAGES; ++i) pages[i] = tiles_of(it).page_of(it.first + warp + i * WARPS);
+  };
 
   float o[NT][MT][4], m[NT][2], l[NT][2];
-  int f = 254;               // weights are multiplied by 2^(f - 127)
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.f;
-#pragma unroll
-    for (int i = 0; i < MT; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
-  }
-
+  int f = 254;                             // weights are multiplied by 2^(f - 127)
   int at_stage = 0, to_stage = STAGES - 1;
-  for (int tile = first + warp; tile < last; tile += WARPS) {
-    wait_copies<STAGES - 2>();
-    __syncwarp();              // every lane's copies have landed, and the stage before has been read
-    uint8_t* stage = mine + at_stage * STAGE;
-    const int c0 = tile * TILE;
-    float2 sc[2] = {tiles.scales(stage, g), tiles.scales(stage, g + 8)};
-    {
-      const int far = tile + (STAGES - 1) * WARPS;
-      const int ahead = tiles.page_of(far + WARPS);
-      if (far < last) tiles.copy(mine + to_stage * STAGE, far, page_number);
-      asm volatile("cp.async.commit_group;\n");
-      page_number = ahead;
-    }
-    at_stage = at_stage + 1 == STAGES ? 0 : at_stage + 1;
-    to_stage = to_stage + 1 == STAGES ? 0 : to_stage + 1;
-    if constexpr (STEP) {
-      if (c0 + TILE > p) {     // the tile of the new token
-        for (int i = lane; i < 2 * CH; i += 32) {
-          const int which = i / CH, ch = i - which * CH;
-          *reinterpret_cast<uint4*>(stage + (which * TILE + p - c0) * ROW + ch * 16) =
-              *reinterpret_cast<const uint4*>(&fresh_row[which][ch * 16]);
-        }
-        __syncwarp();
-        const float2 mine_sc = make_float2(fresh_scale[0], fresh_scale[1]);
+  Item it, done;
+  bool have = next_item(it), had = false;
+  if (have) ask_pages(it);
+  while (true) {
+    // ---- an item's start: all that it waits for is asked for before anything is used
+    const int kvh = it.hc / a.chunks, h0 = head_of(it.hc), nrows = rows_of(it.hc), p = it.len - 1;
+    const size_t row = (size_t)it.b * a.q_stride;
+    const Tiles<WHOLE> tiles = tiles_of(it);
+    float x[RW][N], y[RW][N], nx[N], ny[N];
+    Angles an;
+    // the new token's row of keys (the last warp's, whose rows of q may not exist) and of values (the one before)
+    const bool news = STEP && it.ends && warp >= WARPS - 2, keys = warp == WARPS - 1;
+    int new_page = 0, page_number = 0;
+    if (have) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (c0 + g + 8 * i == p) sc[i] = mine_sc;
+      for (int i = 0; i < RW; ++i)
+        load_row<T>(a, row + (size_t)(h0 + warp + i * WARPS) * HD, warp + i * WARPS < nrows, lane, x[i]);
+      if constexpr (STEP) {
+        an.load(a, p, lane);
+#pragma unroll
+        for (int i = 0; i < RW; ++i)
+          load_partners<T>(a, row + (size_t)(h0 + warp + i * WARPS) * HD, warp + i * WARPS < nrows, lane, y[i]);
+        const size_t new_at = row + (size_t)(a.nh + (keys ? 0 : a.nkv) + kvh) * HD;
+        load_row<T>(a, new_at, news, lane, nx);
+        load_partners<T>(a, new_at, news && keys, lane, ny);
+        if (news) new_page = page_in(a, fresh_index(tiles.tbl + logical_page(a, p)));
       }
-    }
-    float s[NT][4];
+      if (cur.todo > 0) ahead_len = request_length(a, cur.b);
+      // (of the new token nothing is read)
+      int stage = at_stage;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-    {
-      uint32_t k[2][KWORDS];
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < KWORDS / (KW / 4); ++j)
-          read_bytes<KW>(stage + (g + 8 * i) * ROW + t * (HD / 4) + j * KW, &k[i][j * (KW / 4)]);
-#pragma unroll
-      for (int w = 0; w < KWORDS; ++w) {
-        const uint32_t k0 = FP8 ? k[0][w] : k[0][w] ^ 0x80808080u, k1 = FP8 ? k[1][w] : k[1][w] ^ 0x80808080u;
-        uint32_t A[4];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          A[2 * i] = RAISED ? raised_halves(k0, i) : halves<FP8>(k0, i);
-          A[2 * i + 1] = RAISED ? raised_halves(k1, i) : halves<FP8>(k1, i);
-        }
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int i = PARTS - 1; i >= 0; --i) mma_f16(s[n], A, qf[i][n][w][0], qf[i][n][w][1]);
+      for (int i = 0; i < STAGES - 1; ++i) {
+        const int tile = it.first + warp + i * WARPS;
+        if (tile < it.last) tiles.copy(mine + stage * STAGE, tile, pages[i]);
+        asm volatile("cp.async.commit_group;\n");
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
       }
+      page_number = pages[STAGES - 1];
     }
-    bool seen[2] = {true, true};
-    if (c0 < lo || c0 + TILE > len) {
-      // masked keys: whatever lies there counts as nothing (their codes are zeros already)
+
+    // ---- the end of the item before: the four warps' results
+    if (had) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int c = c0 + g + 8 * i;
-        seen[i] = c >= lo && c < len;
-        if (!seen[i]) sc[i] = make_float2(0.f, 0.f);
-      }
-    }
-    float mn[NT][2];
-    bool moved = false;
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float s0 = RAISED ? fmaf(s[n][j], qscale[n][j], qshift[n][j]) : s[n][j] * qscale[n][j];
-        const float s1 = RAISED ? fmaf(s[n][2 + j], qscale[n][j], qshift[n][j]) : s[n][2 + j] * qscale[n][j];
-        s[n][j] = seen[0] ? s0 * sc[0].x : -INFINITY;
-        s[n][2 + j] = seen[1] ? s1 * sc[1].x : -INFINITY;
-        float top = fmaxf(s[n][j], s[n][2 + j]);
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-        mn[n][j] = fmaxf(m[n][j], top);
-        moved |= mn[n][j] != m[n][j];
-      }
-    const uint32_t b0 = __float_as_uint(sc[0].y), b1 = __float_as_uint(sc[1].y);
-    const uint32_t vtop = __reduce_max_sync(0xffffffffu, max(b0 < 0x7f800000u ? b0 : 0u, b1 < 0x7f800000u ? b1 : 0u));
-    const int fn = min(f, 127 + 14 + 127 - (int)(vtop >> 23));
-    if (__any_sync(0xffffffffu, moved) || fn != f) {
-      const float shrink = fn == f ? 1.f : f - fn > 126 ? 0.f : __uint_as_float((uint32_t)(127 + fn - f) << 23);
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float corr[2];
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          corr[j] = mn[n][j] == m[n][j] ? 1.f : fast_exp2(m[n][j] - mn[n][j]);
-          l[n][j] *= corr[j];
-          corr[j] *= shrink;
-          m[n][j] = mn[n][j];
+          l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 4);
+          l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 8);
+          l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 16);
+          if (g == 0) sm[warp][n * 8 + 2 * t + j] = m[n][j], sl[warp][n * 8 + 2 * t + j] = l[n][j];
         }
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-          o[n][i][0] *= corr[0], o[n][i][1] *= corr[1], o[n][i][2] *= corr[0], o[n][i][3] *= corr[1];
-      }
-      f = fn;
-    }
-    const float up = __uint_as_float((uint32_t)f << 23);
-    const float vs0 = sc[0].y * up, vs1 = sc[1].y * up;
-    uint32_t P[PARTS][NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      float w[4];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float p0 = fast_exp2(s[n][j] - m[n][j]), p1 = fast_exp2(s[n][2 + j] - m[n][j]);
-        l[n][j] += p0 + p1;
-        w[j] = p0 * vs0, w[2 + j] = p1 * vs1;
-      }
-      P[0][n][0] = transposed(pack_half(w[0], w[1]));
-      P[0][n][1] = transposed(pack_half(w[2], w[3]));
-      if constexpr (PARTS == 2) {
-        P[1][n][0] = transposed(pack_half(half_rest(w[0]), half_rest(w[1])));
-        P[1][n][1] = transposed(pack_half(half_rest(w[2]), half_rest(w[3])));
-      }
-    }
-    const auto add = [&](int i, const uint32_t (&A)[4]) {
+      const int place = IN_STAGE ? (warp * STAGES + to_stage) * STAGE : WARPS * STAGES * STAGE + warp * R * OROW * 4;
+      if (lane == 0) back[warp] = power_back(f), so_at[warp] = place;
+      __syncwarp();                        // (the stage's tile has been read)
+      float* so = reinterpret_cast<float*>(ring + place);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
+        constexpr int STEP_W = VW >= 4 ? VW / 4 : 1, PER = VW >= 4 ? 2 : 1;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          const int w = i / PER;
+          const int c = ((w / STEP_W) * 8 + g) * VW + (w % STEP_W) * 4 + (i % PER) * 2;
+          float* at = so + (n * 8 + 2 * t) * OROW + c;
+          *reinterpret_cast<float2*>(at) = make_float2(o[n][i][0], o[n][i][2]);
+          *reinterpret_cast<float2*>(at + OROW) = make_float2(o[n][i][1], o[n][i][3]);
+        }
+      }
+      __syncthreads();
+      const bool whole = done.starts && done.ends;
+      const size_t part = ((size_t)blockIdx.x * 2 + (done.starts ? 1 : 0)) * a.rows;
+      const size_t out_at = ((size_t)done.b * a.nh + head_of(done.hc)) * HD;
+      const int n_out = rows_of(done.hc) * (HD / 2);
+#pragma unroll 1
+      for (int i = threadIdx.x; i < n_out; i += THREADS) {
+        const int r = i / (HD / 2), c = 2 * (i - r * (HD / 2));
+        float top = sm[0][r];
+#pragma unroll
+        for (int w = 1; w < WARPS; ++w) top = fmaxf(top, sm[w][r]);
+        float sum = 0.f, v0 = 0.f, v1 = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+          // (a warp without tiles has sums of zero; one whose scores are no numbers passes that on)
+          const float e = sm[w][r] == -INFINITY ? 0.f : fast_exp2(sm[w][r] - top), eb = e * back[w];
+          const float2 v = *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(ring + so_at[w]) + r * OROW + c);
+          sum += e * sl[w][r], v0 += eb * v.x, v1 += eb * v.y;
+        }
+        const float inv = __fdividef(1.f, sum);
+        v0 *= inv, v1 *= inv;
+        if (!whole) {
+          *reinterpret_cast<float2*>(a.po + (part + r) * HD + c) = make_float2(v0, v1);
+          if (c == 0) a.pml[part + r] = make_float2(top, sum);
+        } else if constexpr (sizeof(T) == 4) {
+          *reinterpret_cast<float2*>(reinterpret_cast<float*>(a.out) + out_at + 2 * i) = make_float2(v0, v1);
+        } else {
+          *reinterpret_cast<__nv_bfloat162*>(reinterpret_cast<bf16*>(a.out) + out_at + 2 * i) = __floats2bfloat162_rn(v0, v1);
+        }
+      }
+    }
+    if (!have) break;
+
+    // ---- q, and the new token
+    if constexpr (STEP) {
+      // The block that has the item's last tile writes the new token (every chunk of heads the same bytes) and
+      // keeps it for its own tile.
+      if (news) {
+        if (keys) turn_row(a, an, lane, nx, ny);
+        const RowScale rs = row_scale(row_top(nx), FP8);
+        const Place pl = place_of(a, kvh, new_page, p - logical_page(a, p) * a.page);
+        const int which = keys ? 0 : 1;
+        uint8_t* dst = const_cast<uint8_t*>(pl.codes) + (size_t)which * a.page * HD;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (i * 32 + lane < HD)
+            dst[i * 32 + lane] = fresh_row[which][i * 32 + lane] = (uint8_t)code_of(nx[i], rs, FP8);
+        if (lane == 0)
+          reinterpret_cast<float*>(const_cast<float2*>(pl.scales))[which] = fresh_scale[which] = rs.scale;
+      }
+#pragma unroll
+      for (int i = 0; i < RW; ++i) turn_row(a, an, lane, x[i], y[i]);
+    }
+    // q in halves, a row's largest element in [2^14, 2^15)
+#pragma unroll
+    for (int j = 0; j < RW; ++j) {
+      const int r = warp + j * WARPS;
+      const uint32_t top = row_top(x[j]);
+      // 2^up takes the largest element to [2^14, 2^15); what is no number stays none
+      const int e = top >= 0x7f800000u ? 127 : max((int)(top >> 23), 1), up = min(127 + 14 - e, 126);
+      const float scale_up = __uint_as_float((uint32_t)(127 + up) << 23);
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int c = i * 32 + lane;
+        if (c < HD) {
+          qh[0][r][c] = __float2half_rn(x[j][i] * scale_up);
+          if constexpr (RAISED) sum += __half2float(__float2half_rn(x[j][i] * scale_up));
+          if constexpr (PARTS == 2) qh[1][r][c] = __float2half_rn(half_rest(x[j][i] * scale_up));
+        }
+      }
+      if constexpr (RAISED) sum = warp_sum(sum);
+      if (lane == 0) {
+        qs[r] = a.scale * kLog2E * __uint_as_float((uint32_t)(127 - up) << 23);
+        q_sum[r] = sum;
+      }
+    }
+    __syncthreads();
+    uint32_t qf[PARTS][NT][KWORDS][2];
+#pragma unroll
+    for (int w = 0; w < KWORDS; ++w)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) {
+          // (a thread's channels: a quarter of the head, four a word)
+          const uint2 two = *reinterpret_cast<const uint2*>(&qh[i][n * 8 + g][t * (HD / 4) + 4 * w]);
+          qf[i][n][w][0] = two.x, qf[i][n][w][1] = two.y;
+        }
+    // a score is (product * qscale + qshift) * the key's scale
+    float qscale[NT][2], qshift[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        qscale[n][j] = qs[n * 8 + 2 * t + j];
+        qshift[n][j] = -128.f * q_sum[n * 8 + 2 * t + j] * qscale[n][j];
+        if constexpr (RAISED) qscale[n][j] *= 16777216.f;
+        m[n][j] = -INFINITY, l[n][j] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+    }
+    f = 254;
+
+    // ---- where the block goes next (its pages are there when this item's tiles are done)
+    done = it, had = true;
+    const int lo = it.lo, len = it.len, last = it.last, first = it.first;
+    cur.len = ahead_len;
+    have = next_item(it);
+    if (have) ask_pages(it);
+
+    // ---- the tiles
+#pragma unroll 1
+    for (int tile = first + warp; tile < last; tile += WARPS) {
+      wait_copies<STAGES - 2>();
+      __syncwarp();            // every lane's copies have landed, and the stage before has been read
+      uint8_t* stage = mine + at_stage * STAGE;
+      const int c0 = tile * TILE;
+      {
+        const int far = tile + (STAGES - 1) * WARPS;
+        const int next_page = tiles.page_of(far + WARPS);
+        if (far < last) tiles.copy(mine + to_stage * STAGE, far, page_number);
+        asm volatile("cp.async.commit_group;\n");
+        page_number = next_page;
+      }
+      at_stage = at_stage + 1 == STAGES ? 0 : at_stage + 1;
+      to_stage = to_stage + 1 == STAGES ? 0 : to_stage + 1;
+      float2 sc[2] = {tiles.scales(stage, g), tiles.scales(stage, g + 8)};
+      if constexpr (STEP) {
+        if (c0 + TILE >= len) {     // the tile of the new token
+          const int r = len - 1 - c0;
+          for (int i = lane; i < 2 * CH; i += 32) {
+            const int which = i / CH, ch = i - which * CH;
+            *reinterpret_cast<uint4*>(stage + (which * TILE + r) * ROW + ch * 16) =
+                *reinterpret_cast<const uint4*>(&fresh_row[which][ch * 16]);
+          }
+          __syncwarp();
+          const float2 mine_sc = make_float2(fresh_scale[0], fresh_scale[1]);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (g + 8 * i == r) sc[i] = mine_sc;
+        }
+      }
+      // S^T, in two chains of products
+      constexpr int CHAINS = KWORDS > 1 ? 2 : 1;
+      float s2[CHAINS][NT][4];
+#pragma unroll
+      for (int c = 0; c < CHAINS; ++c)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) s2[c][n][0] = s2[c][n][1] = s2[c][n][2] = s2[c][n][3] = 0.f;
+      {
+        uint32_t k[2][KWORDS];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < KWORDS / (KW / 4); ++j)
+            read_bytes<KW>(stage + (g + 8 * i) * ROW + t * (HD / 4) + j * KW, &k[i][j * (KW / 4)]);
+#pragma unroll
+        for (int w = 0; w < KWORDS; ++w) {
+          const uint32_t k0 = FP8 ? k[0][w] : k[0][w] ^ 0x80808080u, k1 = FP8 ? k[1][w] : k[1][w] ^ 0x80808080u;
+          uint32_t A[4];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            A[2 * i] = RAISED ? raised_halves(k0, i) : halves<FP8>(k0, i);
+            A[2 * i + 1] = RAISED ? raised_halves(k1, i) : halves<FP8>(k1, i);
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = PARTS - 1; i >= 0; --i) mma_f16(s2[w % CHAINS][n], A, qf[i][n][w][0], qf[i][n][w][1]);
+        }
+      }
+      bool seen[2] = {true, true};
+      if (c0 < lo || c0 + TILE > len) {
+        // masked keys: whatever lies there counts as nothing (their codes are zeros already)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int c = c0 + g + 8 * i;
+          seen[i] = c >= lo && c < len;
+          if (!seen[i]) sc[i] = make_float2(0.f, 0.f);
+        }
+      }
+      // Scores in units of log2.  m and f are raised only when a score is 2^7 times what m stands for, or a value's
+      // scale above what f stands for: a weight is below 2^(14 + 1 - 8 + 8) until then.
+      float s[NT][4];
+      bool above = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float r0 = s2[0][n][j], r1 = s2[0][n][2 + j];
+          if constexpr (CHAINS == 2) r0 += s2[1][n][j], r1 += s2[1][n][2 + j];
+          r0 = RAISED ? fmaf(r0, qscale[n][j], qshift[n][j]) : r0 * qscale[n][j];
+          r1 = RAISED ? fmaf(r1, qscale[n][j], qshift[n][j]) : r1 * qscale[n][j];
+          s[n][j] = seen[0] ? r0 * sc[0].x : -INFINITY;
+          s[n][2 + j] = seen[1] ? r1 * sc[1].x : -INFINITY;
+          above |= fmaxf(s[n][j], s[n][2 + j]) > m[n][j] + kSlack;
+        }
+      {
+        // a scale's bits against those of the first power of two that is too large for f
+        const uint32_t bound = (uint32_t)(kTop - f + 1) << 23;
+        const uint32_t b0 = __float_as_uint(sc[0].y), b1 = __float_as_uint(sc[1].y);
+        above |= (b0 >= bound && b0 < 0x7f800000u) || (b1 >= bound && b1 < 0x7f800000u);
+        if (__any_sync(0xffffffffu, above)) {
+          const uint32_t vtop = __reduce_max_sync(0xffffffffu, max(b0 < 0x7f800000u ? b0 : 0u, b1 < 0x7f800000u ? b1 : 0u));
+          const int fn = min(f, kTop - (int)(vtop >> 23));
+          const float shrink = fn == f ? 1.f : f - fn > 126 ? 0.f : __uint_as_float((uint32_t)(127 + fn - f) << 23);
+          f = fn;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            float corr[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float top = fmaxf(s[n][j], s[n][2 + j]);
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+              const float mn = fmaxf(m[n][j], top);
+              corr[j] = mn == m[n][j] ? 1.f : fast_exp2(m[n][j] - mn);
+              l[n][j] *= corr[j];
+              corr[j] *= shrink;
+              m[n][j] = mn;
+            }
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+              o[n][i][0] *= corr[0], o[n][i][1] *= corr[1], o[n][i][2] *= corr[0], o[n][i][3] *= corr[1];
+          }
+        }
+      }
+      const float up = __uint_as_float((uint32_t)f << 23);
+      const float vs0 = sc[0].y * up, vs1 = sc[1].y * up;
+      uint32_t P[PARTS][NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float w[4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float p0 = fast_exp2(s[n][j] - m[n][j]), p1 = fast_exp2(s[n][2 + j] - m[n][j]);
+          l[n][j] += p0 + p1;
+          w[j] = p0 * vs0, w[2 + j] = p1 * vs1;
+        }
+        P[0][n][0] = transposed(pack_half(w[0], w[1]));
+        P[0][n][1] = transposed(pack_half(w[2], w[3]));
         if constexpr (PARTS == 2) {
-          float d[4] = {0.f, 0.f, 0.f, 0.f};
-          mma_f16(d, A, P[1][n][0], P[1][n][1]);
-          mma_f16(d, A, P[0][n][0], P[0][n][1]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[n][i][e] += d[e];
-        } else {
-          mma_f16(o[n][i], A, P[0][n][0], P[0][n][1]);
+          P[1][n][0] = transposed(pack_half(half_rest(w[0]), half_rest(w[1])));
+          P[1][n][1] = transposed(pack_half(half_rest(w[2]), half_rest(w[3])));
         }
       }
-    };
+      const auto add = [&](int i, const uint32_t (&A)[4]) {
 #pragma unroll
-    for (int j = 0; j < HD / (8 * VW); ++j) {
-      constexpr int WORDS = VW >= 4 ? VW / 4 : 1;
-      uint32_t v[4][WORDS];          // keys 2t, 2t + 1, 2t + 8, 2t + 9
+        for (int n = 0; n < NT; ++n) {
+          if constexpr (PARTS == 2) {
+            float d[4] = {0.f, 0.f, 0.f, 0.f};
+            mma_f16(d, A, P[1][n][0], P[1][n][1]);
+            mma_f16(d, A, P[0][n][0], P[0][n][1]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        read_bytes<VW>(stage + (TILE + 2 * t + (i & 1) + 8 * (i >> 1)) * ROW + (j * 8 + g) * VW, v[i]);
-        if constexpr (!FP8) {
+            for (int e = 0; e < 4; ++e) o[n][i][e] += d[e];
+          } else {
+            mma_f16(o[n][i], A, P[0][n][0], P[0][n][1]);
+          }
+        }
+      };
 #pragma unroll
-          for (int w = 0; w < WORDS; ++w) v[i][w] ^= 0x80808080u;
+      for (int j = 0; j < HD / (8 * VW); ++j) {
+        constexpr int WORDS = VW >= 4 ? VW / 4 : 1;
+        uint32_t v[4][WORDS];          // keys 2t, 2t + 1, 2t + 8, 2t + 9
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          read_bytes<VW>(stage + (TILE + 2 * t + (i & 1) + 8 * (i >> 1)) * ROW + (j * 8 + g) * VW, v[i]);
+          if constexpr (!FP8) {
+#pragma unroll
+            for (int w = 0; w < WORDS; ++w) v[i][w] ^= 0x80808080u;
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < WORDS; ++w) {
+          const uint32_t u0 = __byte_perm(v[0][w], v[1][w], 0x5140), u1 = __byte_perm(v[2][w], v[3][w], 0x5140);
+          const uint32_t A[4] = {halves<FP8>(u0, 0), halves<FP8>(u0, 1), halves<FP8>(u1, 0), halves<FP8>(u1, 1)};
+          if constexpr (VW >= 4) {
+            add(2 * (j * WORDS + w), A);
+            const uint32_t y0 = __byte_perm(v[0][w], v[1][w], 0x7362), y1 = __byte_perm(v[2][w], v[3][w], 0x7362);
+            const uint32_t C[4] = {halves<FP8>(y0, 0), halves<FP8>(y0, 1), halves<FP8>(y1, 0), halves<FP8>(y1, 1)};
+            add(2 * (j * WORDS + w) + 1, C);
+          } else {
+            add(j, A);
+          }
         }
       }
-#pragma unroll
-      for (int w = 0; w < WORDS; ++w) {
-        const uint32_t u0 = __byte_perm(v[0][w], v[1][w], 0x5140), u1 = __byte_perm(v[2][w], v[3][w], 0x5140);
-        const uint32_t A[4] = {halves<FP8>(u0, 0), halves<FP8>(u0, 1), halves<FP8>(u1, 0), halves<FP8>(u1, 1)};
-        if constexpr (VW >= 4) {
-          add(2 * (j * WORDS + w), A);
-          const uint32_t y0 = __byte_perm(v[0][w], v[1][w], 0x7362), y1 = __byte_perm(v[2][w], v[3][w], 0x7362);
-          const uint32_t C[4] = {halves<FP8>(y0, 0), halves<FP8>(y0, 1), halves<FP8>(y1, 0), halves<FP8>(y1, 1)};
-          add(2 * (j * WORDS + w) + 1, C);
-        } else {
-          add(j, A);
-        }
-      }
     }
-  }
-  wait_copies<0>();
-  // the four warps' results
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 4);
-      l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 8);
-      l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 16);
-      if (g == 0) sm[warp][n * 8 + 2 * t + j] = m[n][j], sl[warp][n * 8 + 2 * t + j] = l[n][j];
-    }
-  if (lane == 0) back[warp] = power_back(f);
-  __syncthreads();             // the ring becomes the warps' results
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    constexpr int STEP_W = VW >= 4 ? VW / 4 : 1, PER = VW >= 4 ? 2 : 1;
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const int w = i / PER;
-      const int c = ((w / STEP_W) * 8 + g) * VW + (w % STEP_W) * 4 + (i % PER) * 2;
-      float* at = so + ((size_t)warp * R + n * 8 + 2 * t) * OROW + c;
-      *reinterpret_cast<float2*>(at) = make_float2(o[n][i][0], o[n][i][2]);
-      *reinterpret_cast<float2*>(at + OROW) = make_float2(o[n][i][1], o[n][i][3]);
-    }
-  }
-  __syncthreads();
-  const bool whole = starts && ends;
-  const size_t part = ((size_t)blockIdx.x * 2 + (starts ? 1 : 0)) * a.rows;
-  for (int i = threadIdx.x; i < nrows * (HD / 2); i += THREADS) {
-    const int r = i / (HD / 2), c = 2 * (i - r * (HD / 2));
-    float top = sm[0][r];
-#pragma unroll
-    for (int w = 1; w < WARPS; ++w) top = fmaxf(top, sm[w][r]);
-    float sum = 0.f, v0 = 0.f, v1 = 0.f;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      // (a warp without tiles has sums of zero; one whose scores are no numbers passes that on)
-      const float e = sm[w][r] == -INFINITY ? 0.f : fast_exp2(sm[w][r] - top), eb = e * back[w];
-      const float2 v = *reinterpret_cast<const float2*>(so + (size_t)(w * R + r) * OROW + c);
-      sum += e * sl[w][r], v0 += eb * v.x, v1 += eb * v.y;
-    }
-    v0 /= sum, v1 /= sum;
-    const size_t at = out_at + (size_t)r * HD + c;
-    if (!whole) {
-      *reinterpret_cast<float2*>(a.po + (part + r) * HD + c) = make_float2(v0, v1);
-      if (c == 0) a.pml[part + r] = make_float2(top, sum);
-    } else if (a.out_f32) {
-      *reinterpret_cast<float2*>(reinterpret_cast<float*>(a.out) + at) = make_float2(v0, v1);
-    } else {
-      *reinterpret_cast<__nv_bfloat162*>(reinterpret_cast<bf16*>(a.out) + at) = __floats2bfloat162_rn(v0, v1);
-    }
-  }
-  if (cur.todo > 0) __syncthreads();
   }
 }
 
@@ -816,10 +880,11 @@ quant_join_kernel(const DecodeArgs a) {
   }
 }
 
-template <int NT, bool FP8, int PARTS, bool WHOLE, bool STEP>
+template <int NT, bool FP8, typename T, bool WHOLE, bool STEP>
 int launch_decode(DecodeArgs a, int sms, void* scratch, size_t scratch_bytes, cudaStream_t stream) {
-  constexpr auto kernel = quant_decode_kernel<NT, FP8, PARTS, WHOLE, STEP>;
-  constexpr int smem = std::max(WARPS * STAGES * STAGE, WARPS * 8 * NT * (HD + 2) * 4);
+  constexpr auto kernel = quant_decode_kernel<NT, FP8, T, WHOLE, STEP>;
+  constexpr int results = 8 * NT * (HD + 2) * 4;
+  constexpr int smem = WARPS * (STAGES * STAGE + (results <= STAGE ? 0 : results));
   static OncePerDevice once;
   static int blocks_a_sm[OncePerDevice::kMaxDevices];
   int dev = 0;
@@ -865,9 +930,9 @@ GF_EXPORT long long gf_quant_decode_scratch(int B, int nh, int nkv, int sms) {
 }
 
 // q [B, nh HD], or with `step` q | k | v [B, (nh + 2 nkv) HD] and the table of angles as gf_quant_write takes it.
-GF_EXPORT int gf_quant_decode(const void* q, int q_stride, int q_f32, void* codes, int fp8, float* scales,
+GF_EXPORT int gf_quant_decode(const void* q, int q_stride, int f32, void* codes, int fp8, float* scales,
                               const int* block_table, int table_stride, int table_width, const int* lengths, int pages,
-                              void* out, int out_f32, int B, int nh, int nkv, int page, int span, float scale,
+                              void* out, int B, int nh, int nkv, int page, int span, float scale,
                               int step, const float* table, int table_rows, int rot, int neighbours, int sms,
                               void* scratch, long long scratch_bytes, void* stream) {
   if (B <= 0) return B < 0 ? -3 : 0;
@@ -876,18 +941,18 @@ GF_EXPORT int gf_quant_decode(const void* q, int q_stride, int q_f32, void* code
   if ((size_t)codes % 16 || (size_t)scales % 8) return -3;
   if (step && (rot < 0 || rot % 2 || rot > HD || (rot && (!table || table_rows < 1)))) return -3;
   DecodeArgs a = {};
-  a.q = q, a.q_stride = q_stride, a.q_f32 = q_f32;
+  a.q = q, a.q_stride = q_stride;
   a.codes = (uint8_t*)codes, a.scales = scales;
   a.block_table = block_table, a.table_stride = table_stride;
   a.limit = (int)min((long long)table_width * page, 0x7fffffe0LL);
-  a.pages = pages, a.lengths = lengths, a.out = out, a.out_f32 = out_f32;
+  a.pages = pages, a.lengths = lengths, a.out = out, a.out_f32 = f32;
   a.B = B, a.nh = nh, a.nkv = nkv, a.page = page, a.span = span, a.scale = scale;
   a.page_shift = (page & (page - 1)) == 0 ? __builtin_ctz(page) : -1;
   a.table = table, a.table_rows = table_rows > 0 ? table_rows : 1, a.rot = rot, a.neighbours = neighbours;
   const int G = nh / nkv;
   a.chunks = (G + 15) / 16, a.rows = (G + a.chunks - 1) / a.chunks;
-  const auto go = [&](auto nt, auto kind, auto parts, auto whole, auto fused) {
-    return launch_decode<decltype(nt)::value, decltype(kind)::value, decltype(parts)::value, decltype(whole)::value,
+  const auto go = [&](auto nt, auto kind, auto type, auto whole, auto fused) {
+    return launch_decode<decltype(nt)::value, decltype(kind)::value, decltype(type), decltype(whole)::value,
                          decltype(fused)::value>(a, sms, scratch, (size_t)scratch_bytes, (cudaStream_t)stream);
   };
   const auto pick_bool = [](bool x, auto next) {
@@ -898,8 +963,8 @@ GF_EXPORT int gf_quant_decode(const void* q, int q_stride, int q_f32, void* code
       return pick_bool(step != 0, [&](auto fused) {
         using One = std::integral_constant<int, 1>;
         using Two = std::integral_constant<int, 2>;
-        if (q_f32) return a.rows > 8 ? go(Two(), kind, Two(), whole, fused) : go(One(), kind, Two(), whole, fused);
-        return a.rows > 8 ? go(Two(), kind, One(), whole, fused) : go(One(), kind, One(), whole, fused);
+        if (f32) return a.rows > 8 ? go(Two(), kind, float(), whole, fused) : go(One(), kind, float(), whole, fused);
+        return a.rows > 8 ? go(Two(), kind, bf16(), whole, fused) : go(One(), kind, bf16(), whole, fused);
       });
     });
   });

@@ -145,7 +145,7 @@ def read_slots(cache, slots: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
 
 
 _DECODE_ARGS = ([c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p]
-                + [c_int] * 6 + [c_float, c_int, c_void_p] + [c_int] * 4 + [c_void_p, c_longlong, c_void_p])
+                + [c_int] * 5 + [c_float, c_int, c_void_p] + [c_int] * 4 + [c_void_p, c_longlong, c_void_p])
 _F32 = {torch.float32: 1, torch.bfloat16: 0}
 # Requests of at most this many visible tokens are one block's work a kv head and need no scratch (the kernel has the
 # same line: kShortKeys).
@@ -172,7 +172,7 @@ def _decode(q, nh, facts, block_table, lengths, scale, span, fused=None):
     table, rows, rot, neighbours = (None, 0, 0, 0) if fused is None else fused
     f32 = _F32[q.dtype]
     _ok(f(x, stride, f32, _p(codes), fp8, _p(scales), _ints(block_table, (B, W), "block_table"), W, W,
-          _ints(lengths, (B,), "lengths"), pages, _p(out), f32, B, nh, nkv, page, int(span), float(scale),
+          _ints(lengths, (B,), "lengths"), pages, _p(out), B, nh, nkv, page, int(span), float(scale),
           int(fused is not None), table, rows, rot, int(neighbours), sms, _p(scratch), 4 * words, _stream()),
         "quant_cache.decode")
     return out

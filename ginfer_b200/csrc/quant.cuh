@@ -7,29 +7,41 @@
 
 namespace gf {
 
-// ---- eight channels of a row
+// ---- eight channels of a row, as they lie in memory until they are used
 // vec: the address is a multiple of 16 bytes.  Always past L1: a kernel shortly before this one wrote them.
-__device__ __forceinline__ void load8(const float* p, float (&v)[8], int vec) {
-  if (vec) {
-    const float4 a = __ldcg(reinterpret_cast<const float4*>(p)), b = __ldcg(reinterpret_cast<const float4*>(p) + 1);
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = __ldcg(p + e);
+template <typename T> struct Raw8;
+template <> struct Raw8<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p, int vec) {
+    if (vec) {
+      a = __ldcg(reinterpret_cast<const float4*>(p)), b = __ldcg(reinterpret_cast<const float4*>(p) + 1);
+    } else {
+      a = make_float4(__ldcg(p), __ldcg(p + 1), __ldcg(p + 2), __ldcg(p + 3));
+      b = make_float4(__ldcg(p + 4), __ldcg(p + 5), __ldcg(p + 6), __ldcg(p + 7));
+    }
   }
-}
-__device__ __forceinline__ void load8(const bf16* p, float (&v)[8], int vec) {
-  if (vec) {
-    const uint4 a = __ldcg(reinterpret_cast<const uint4*>(p));
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  }
+};
+template <> struct Raw8<bf16> {
+  uint4 a;
+  __device__ __forceinline__ void load(const bf16* p, int vec) {
+    if (vec) {
+      a = __ldcg(reinterpret_cast<const uint4*>(p));
+    } else {
+      const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+      a.x = (uint32_t)__ldcg(h) | (uint32_t)__ldcg(h + 1) << 16, a.y = (uint32_t)__ldcg(h + 2) | (uint32_t)__ldcg(h + 3) << 16;
+      a.z = (uint32_t)__ldcg(h + 4) | (uint32_t)__ldcg(h + 5) << 16, a.w = (uint32_t)__ldcg(h + 6) | (uint32_t)__ldcg(h + 7) << 16;
+    }
+  }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
     const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       v[2 * e] = __uint_as_float(w[e] << 16), v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = fresh(p + e);
   }
-}
+};
 __device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
   reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
   reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
@@ -62,9 +74,9 @@ __device__ __forceinline__ uint32_t max_bits8(const float (&v)[8]) {
   for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(v[e]) & 0x7fffffffu);
   return m;
 }
-template <int LANES> __device__ __forceinline__ uint32_t group_max_bits(uint32_t m) {
+template <int LANES> __device__ __forceinline__ uint32_t group_max_bits(uint32_t m, unsigned mask = 0xffffffffu) {
 #pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(mask, m, o));
   return m;
 }
 struct RowScale {

@@ -19,10 +19,14 @@
 namespace gf {
 
 // -------------------------------------------------------------------------------------- write
-// A row is held by LANES lanes of 8 channels each; a group of LANES lanes takes HU heads of one token, so
-// that their loads are under way together and the angles of the token's position are read once for them.
+// A head's row is held by hd / 16 lanes of two times eight channels each, such that a lane's channels turn with
+// each other: 8 l .. and half + 8 l .. where halves turn (what does not turn follows in runs of 16), 16 l .. where
+// neighbours do.  A group of lanes takes HU heads of one token: their loads are under way together, and the angles
+// of the token's position are read once for them.  Halves that are no multiple of eight take the angles and partners
+// one by one.
+constexpr int WRITE_THREADS = 128;
 template <typename T, int LANES, int HU>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(WRITE_THREADS)
 quant_write_kernel(const T* __restrict__ qkv, int row_stride, int tokens, int nh, int nkv, int hd,
                    const float* __restrict__ table, int table_rows, int rot, int neighbours,
                    const int* __restrict__ positions, const int* __restrict__ slots, T* __restrict__ q_out,
@@ -32,90 +36,100 @@ quant_write_kernel(const T* __restrict__ qkv, int row_stride, int tokens, int nh
   pdl_wait();
   const int heads = nh + 2 * nkv, sets = (heads + HU - 1) / HU;
   const int lane = threadIdx.x & (LANES - 1);
-  const long long group = ((long long)blockIdx.x * blockDim.x + threadIdx.x) / LANES;
-  const int t = (int)(group / sets);
-  const int h0 = (int)(group - (long long)t * sets) * HU;
-  const bool here = t < tokens && lane * 8 < hd;
-  const int c0 = lane * 8;
+  const unsigned group = blockIdx.x * (unsigned)(WRITE_THREADS / LANES) + threadIdx.x / LANES;
+  const int t = (int)(group / (unsigned)sets), h0 = (int)(group - (unsigned)t * sets) * HU;
+  const bool here = t < tokens && lane * 16 < hd;
+  const int half = rot >> 1;
+  const bool plain = !neighbours && (half & 7) == 0;
+  const bool turns = lane * 16 < rot;              // (all of a lane's channels, or with neighbours some)
+  const int ca = plain && turns ? lane * 8 : lane * 16, cb = plain && turns ? half + lane * 8 : lane * 16 + 8;
   const T* row = qkv + (size_t)(here ? t : 0) * row_stride;
   const int slot = t < tokens ? fresh_index(slots + t) : -1;
   const bool keep = slot >= 0 && slot < num_slots;
+  // the lanes of this row: groups of a warp part ways where one has queries and another keys
+  const unsigned mask = (LANES == 32 ? 0xffffffffu : ((1u << (LANES & 31)) - 1u)) << (threadIdx.x & 31 & ~(LANES - 1));
 
-  float x[HU][8], y[HU][8];
-  const int half = rot >> 1;
-  // the channels that this lane's are paired with: its own where neighbours turn together
-  const bool turns = here && c0 < rot;
-  const int shift = c0 < half ? half : -half;
-  // (halves that are no multiple of 8: a lane's 8 channels may have partners on both sides)
-  const bool plain_pairs = !neighbours && (half & 7) == 0;
+  Raw8<T> ra[HU], rb[HU];
 #pragma unroll
   for (int i = 0; i < HU; ++i) {
-    const int h = h0 + i;
-    if (here && h < heads) {
-      load8(row + (size_t)h * hd + c0, x[i], vec);
-      if (turns && h < nh + nkv && plain_pairs) load8(row + (size_t)h * hd + c0 + shift, y[i], vec);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
-    }
+    if (!here || h0 + i >= heads) continue;
+    ra[i].load(row + (size_t)(h0 + i) * hd + ca, vec & 1);
+    rb[i].load(row + (size_t)(h0 + i) * hd + cb, vec & 1);
   }
-  if (turns && h0 < nh + nkv) {
-    const int p = min(max(fresh_index(positions + t), 0), table_rows - 1);
-    const float* cs = table + (size_t)p * rot;
-    float c[8], s[8];
-    if (neighbours) {
+  const float* cs = table;
+  float c[8], s[8];
+  const int j0 = lane * 8;                         // the first of the lane's eight pairs
+  const bool regular = neighbours || plain;
+  if (here && rot > 0 && h0 < nh + nkv) {
+    cs += (size_t)min(max(fresh_index(positions + t), 0), table_rows - 1) * rot;
+    if (turns && (half & 7) == 0 && (vec & 2)) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) c[e] = cs[(c0 >> 1) + e < half ? (c0 >> 1) + e : 0],
-                                  s[e] = cs[(c0 >> 1) + e < half ? half + (c0 >> 1) + e : 0];
-    } else if (plain_pairs) {
-      const int j = c0 < half ? c0 : c0 - half;
+      for (int e = 0; e < 8; e += 4) {             // (a row of the table is a multiple of 64 bytes)
+        const float4 cv = __ldg(reinterpret_cast<const float4*>(cs + j0 + e));
+        const float4 sv = __ldg(reinterpret_cast<const float4*>(cs + half + j0 + e));
+        c[e] = cv.x, c[e + 1] = cv.y, c[e + 2] = cv.z, c[e + 3] = cv.w;
+        s[e] = sv.x, s[e + 1] = sv.y, s[e + 2] = sv.z, s[e + 3] = sv.w;
+      }
+    } else if (turns && regular) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) c[e] = cs[j + e], s[e] = cs[half + j + e];
-    }
-#pragma unroll
-    for (int i = 0; i < HU; ++i) {
-      const int h = h0 + i;
-      if (h >= nh + nkv) continue;
-      if (neighbours) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (c0 + 2 * e < rot) turn_pair(x[i][2 * e], x[i][2 * e + 1], c[e], s[e]);
-      } else if (plain_pairs) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          x[i][e] = c0 < half ? turned_first(x[i][e], y[i][e], c[e], s[e])
-                              : turned_second(y[i][e], x[i][e], c[e], s[e]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int ch = c0 + e;
-          if (ch >= rot) continue;
-          const int j = ch < half ? ch : ch - half;
-          const float o = to_f32(row[(size_t)h * hd + (ch < half ? ch + half : j)]);
-          x[i][e] = ch < half ? turned_first(x[i][e], o, cs[j], cs[half + j])
-                              : turned_second(o, x[i][e], cs[j], cs[half + j]);
-        }
+      for (int e = 0; e < 8; ++e) {
+        const int j = min(j0 + e, half - 1);
+        c[e] = __ldg(cs + j), s[e] = __ldg(cs + half + j);
       }
     }
   }
 #pragma unroll
   for (int i = 0; i < HU; ++i) {
     const int h = h0 + i;
-    if (h < nh) {                          // a group's lanes agree on h: its shuffles below are whole
-      if (here) store8(q_out + (size_t)t * nh * hd + (size_t)h * hd + c0, x[i]);
+    if (h >= heads) break;                         // (a group's lanes agree on h: the shuffles below are whole)
+    float lo[8], hi[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) lo[e] = hi[e] = 0.f;
+    if (here) ra[i].get(lo), rb[i].get(hi);
+    if (here && turns && h < nh + nkv) {
+      if (plain) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) turn_pair(lo[e], hi[e], c[e], s[e]);
+      } else if (neighbours) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (j0 + e < half) turn_pair(lo[2 * e], lo[2 * e + 1], c[e], s[e]);
+          if (j0 + 4 + e < half) turn_pair(hi[2 * e], hi[2 * e + 1], c[4 + e], s[4 + e]);
+        }
+      }
     }
-    const bool kv = t < tokens && h >= nh && h < heads;
-    const uint32_t top = group_max_bits<LANES>(kv ? max_bits8(x[i]) : 0u);
-    if (kv && keep) {
-      const int which = h >= nh + nkv, kvh = h - nh - which * nkv;
-      const RowScale rs = row_scale(top, fp8);
-      const int pg = slot / page, off = slot - pg * page;
-      const size_t at = (size_t)pg * nkv + kvh;
-      if (here)
-        *reinterpret_cast<uint2*>(codes + ((at * 2 + which) * page + off) * hd + c0) =
-            quantise8(x[i], rs, fp8);
-      if (lane == 0) scales[(at * page + off) * 2 + which] = rs.scale;
+    if (here && !regular && h < nh + nkv && lane * 16 < rot) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int ch = lane * 16 + e;
+        float& own = e < 8 ? lo[e & 7] : hi[e & 7];
+        if (ch >= rot) continue;
+        const int j = ch < half ? ch : ch - half;
+        const float o = fresh(row + (size_t)h * hd + (ch < half ? ch + half : j));
+        own = ch < half ? turned_first(own, o, __ldg(cs + j), __ldg(cs + half + j))
+                        : turned_second(o, own, __ldg(cs + j), __ldg(cs + half + j));
+      }
     }
+    if (h < nh) {
+      if (here) {
+        T* q = q_out + (size_t)t * nh * hd + (size_t)h * hd;
+        store8(q + ca, lo);
+        store8(q + cb, hi);
+      }
+      continue;
+    }
+    const uint32_t top = group_max_bits<LANES>(max(max_bits8(lo), max_bits8(hi)), mask);
+    if (!keep) continue;
+    const int which = h >= nh + nkv, kvh = h - nh - which * nkv;
+    const RowScale rs = row_scale(top, fp8);
+    const int pg = slot / page, off = slot - pg * page;
+    const size_t at = (size_t)pg * nkv + kvh;
+    uint8_t* dst = codes + ((at * 2 + which) * page + off) * hd;
+    if (here) {
+      *reinterpret_cast<uint2*>(dst + ca) = quantise8(lo, rs, fp8);
+      *reinterpret_cast<uint2*>(dst + cb) = quantise8(hi, rs, fp8);
+    }
+    if (lane == 0) scales[(at * page + off) * 2 + which] = rs.scale;
   }
 }
 
@@ -127,11 +141,11 @@ int launch_write(const void* qkv, int row_stride, int tokens, int nh, int nkv, i
   const int heads = nh + 2 * nkv;
   const bool one = (long long)tokens * heads * LANES <= 148 * 1024;
   const int hu = one ? 1 : 4;
-  const long long threads = (long long)tokens * ((heads + hu - 1) / hu) * LANES;
-  const long long blocks = (threads + 255) / 256;
-  if (blocks > 0x7fffffffLL) return -5;
+  const long long groups = (long long)tokens * ((heads + hu - 1) / hu);
+  const long long blocks = (groups * LANES + WRITE_THREADS - 1) / WRITE_THREADS;
+  if (groups > 0x7fffffffLL || blocks > 0x7fffffffLL) return -5;
   const auto run = [&](auto kernel) {
-    return launch_kernel(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, (const T*)qkv, row_stride,
+    return launch_kernel(kernel, dim3((unsigned)blocks), dim3(WRITE_THREADS), 0, stream, (const T*)qkv, row_stride,
                          tokens, nh, nkv, hd, table, table_rows, rot, neighbours, positions, slots, (T*)q_out,
                          codes, fp8, scales, page, num_slots, vec);
   };
@@ -141,49 +155,82 @@ int launch_write(const void* qkv, int row_stride, int tokens, int nh, int nkv, i
 // -------------------------------------------------------------------------------------- read
 // Dense [2, B, S, kv heads, hd]: position s of request b through its block table where first <= s < length,
 // zeros elsewhere; or, with `slots`, row s of [2, 1, S, kv heads, hd] from slot slots[s] (negative: zeros).
+// A block takes READ_SPAN positions and works out where they lie once; a thread keeps its 16 bytes' place in a
+// token's result and walks down the positions, four loads under way.
+constexpr int READ_SPAN = 32, READ_THREADS = 256;
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(READ_THREADS)
 quant_read_kernel(const uint8_t* __restrict__ codes, int fp8, const float* __restrict__ scales,
                   const int* __restrict__ block_table, int table_stride, const int* __restrict__ lengths,
                   const int* __restrict__ first, const int* __restrict__ slots, int num_slots, int S, int nkv,
                   int hd, int page, T* __restrict__ out) {
+  constexpr int E = 16 / (int)sizeof(T);             // channels of a thread
+  __shared__ int2 token_at[READ_SPAN];               // page number (-1: zeros), place
   pdl_trigger();
   pdl_wait();
-  const int b = blockIdx.y;
-  const int chunks = hd / 16, per_token = 2 * nkv * chunks;
-  const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= (long long)S * per_token) return;
-  const int s = (int)(i / per_token);
-  int u = (int)(i - (long long)s * per_token);
-  const int which = u / (nkv * chunks);
-  u -= which * nkv * chunks;
-  const int kvh = u / chunks, ch = u - kvh * chunks;
-  int pg = -1, off = 0;
-  if (slots) {
-    const int slot = fresh_index(slots + s);
-    if (slot >= 0 && slot < num_slots) pg = slot / page, off = slot - pg * page;
-  } else if (s < fresh_index(lengths + b) && (!first || s >= fresh_index(first + b))) {
-    const int lp = s / page;
-    pg = fresh_index(block_table + (size_t)b * table_stride + lp), off = s - lp * page;
+  const int b = blockIdx.y, s0 = blockIdx.x * READ_SPAN, num_pages = num_slots / page;
+  if (threadIdx.x < READ_SPAN) {
+    const int s = s0 + threadIdx.x;
+    int pg = -1, off = 0;
+    if (s < S) {
+      if (slots) {
+        const int slot = fresh_index(slots + s);
+        if (slot >= 0 && slot < num_slots) pg = slot / page, off = slot - pg * page;
+      } else if (s < fresh_index(lengths + b) && (!first || s >= fresh_index(first + b))) {
+        const int lp = s / page;
+        pg = min(max(fresh_index(block_table + (size_t)b * table_stride + lp), 0), num_pages - 1), off = s - lp * page;
+      }
+    }
+    token_at[threadIdx.x] = make_int2(pg, off);
   }
-  float v[16];
-  if (pg >= 0) {
-    const size_t at = (size_t)pg * nkv + kvh;
-    const uint4 raw = *reinterpret_cast<const uint4*>(codes + ((at * 2 + which) * page + off) * hd + ch * 16);
-    const float sc = scales[(at * page + off) * 2 + which];
-    values16(raw, fp8, v);
+  __syncthreads();
+  const int chunks = hd / E, units = 2 * nkv * chunks;
+  // threads side by side in a token's result, and as many tokens at a time as then fit the block
+  const int wide = min(units, READ_THREADS), deep = READ_THREADS / wide;
+  const int down = threadIdx.x / wide;
+  if (down >= deep) return;
+  const int many = min(READ_SPAN, S - s0);
+  for (int u = threadIdx.x - down * wide; u < units; u += wide) {
+    const int which = u >= nkv * chunks, v = u - which * nkv * chunks, kvh = v / chunks, ch = v - kvh * chunks;
+    T* to = out + ((((size_t)which * gridDim.y + b) * S + s0) * nkv + kvh) * hd + ch * E;
+    const size_t step = (size_t)nkv * hd;
+    for (int d0 = down; d0 < many; d0 += 4 * deep) {
+      uint32_t raw[4][E / 4];
+      float sc[4];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) v[e] = __fmul_rn(v[e], sc);
-  } else {
+      for (int i = 0; i < 4; ++i) {
+        const int d = d0 + i * deep;
+        const int2 at = d < many ? token_at[d] : make_int2(-1, 0);
+        sc[i] = 0.f;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) v[e] = 0.f;
+        for (int e = 0; e < E / 4; ++e) raw[i][e] = 0u;
+        if (at.x >= 0) {
+          const size_t record = (size_t)at.x * nkv + kvh;
+          const uint8_t* from = codes + ((record * 2 + which) * page + at.y) * hd + ch * E;
+          if constexpr (E == 8) {
+            const uint2 r = __ldcg(reinterpret_cast<const uint2*>(from));
+            raw[i][0] = r.x, raw[i][1] = r.y;
+          } else {
+            raw[i][0] = __ldcg(reinterpret_cast<const uint32_t*>(from));
+          }
+          sc[i] = __ldcg(scales + (record * page + at.y) * 2 + which);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = d0 + i * deep;
+        if (d >= many) continue;
+        float x[E];
+#pragma unroll
+        for (int e = 0; e < E / 4; ++e) values4(raw[i][e], fp8, x + 4 * e);
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = token_at[d].x < 0 ? 0.f : __fmul_rn(x[e], sc[i]);
+        T* o = to + (size_t)d * step;
+        if constexpr (E == 8) store8(o, x);
+        else *reinterpret_cast<float4*>(o) = make_float4(x[0], x[1], x[2], x[3]);
+      }
+    }
   }
-  T* o = out + ((((size_t)which * gridDim.y + b) * S + s) * nkv + kvh) * hd + ch * 16;
-  float lo[8], hi[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) lo[e] = v[e], hi[e] = v[8 + e];
-  store8(o, lo);
-  store8(o + 8, hi);
 }
 
 }  // namespace gf
@@ -204,17 +251,18 @@ GF_EXPORT int gf_quant_write(const void* qkv, int row_stride, int dtype, int tok
       (rot && (!table || table_rows < 1)))
     return -3;
   const size_t es = dtype == GF_F32 ? 4 : 2;
-  const int vec = ((size_t)qkv % 16 == 0 && (size_t)row_stride * es % 16 == 0) ? 1 : 0;
+  if ((size_t)codes % 16 || (size_t)scales % 8) return -3;
+  // whether rows (1) and the table (2) can be read 16 bytes at a time
+  const int vec = ((size_t)qkv % 16 == 0 && (size_t)row_stride * es % 16 == 0 ? 1 : 0) | ((size_t)table % 16 == 0 ? 2 : 0);
   const auto go = [&](auto tag) {
     using T = decltype(tag);
     const auto run = [&](auto launch) {
       return launch(qkv, row_stride, tokens, nh, nkv, hd, table, table_rows, rot, neighbours, positions, slots,
                     q_out, (uint8_t*)codes, fp8, scales, page, num_slots, vec, (cudaStream_t)stream);
     };
-    if (hd <= 32) return run(launch_write<T, 4>);
-    if (hd <= 64) return run(launch_write<T, 8>);
-    if (hd <= 128) return run(launch_write<T, 16>);
-    return run(launch_write<T, 32>);
+    if (hd <= 64) return run(launch_write<T, 4>);
+    if (hd <= 128) return run(launch_write<T, 8>);
+    return run(launch_write<T, 16>);
   };
   return dtype == GF_F32 ? go(float()) : go(bf16());
 }
@@ -225,13 +273,11 @@ GF_EXPORT int gf_quant_read(const void* codes, int fp8, const float* scales, con
                             int num_slots, int B, int S, int nkv, int hd, int page, void* out, int dtype,
                             void* stream) {
   if (B <= 0 || S <= 0) return B < 0 || S < 0 ? -3 : 0;
-  if (hd % 16 || hd < 16 || hd > 256 || nkv < 1 || page < 1 || B > 65535) return -3;
-  const long long units = (long long)S * 2 * nkv * (hd / 16), blocks = (units + 255) / 256;
-  if (blocks > 0x7fffffffLL) return -5;
-  const dim3 grid((unsigned)blocks, (unsigned)B);
+  if (hd % 16 || hd < 16 || hd > 256 || nkv < 1 || page < 1 || B > 65535 || (size_t)codes % 16) return -3;
+  const dim3 grid((unsigned)(((long long)S + READ_SPAN - 1) / READ_SPAN), (unsigned)B);
   const auto go = [&](auto tag) {
     using T = decltype(tag);
-    return launch_kernel(quant_read_kernel<T>, grid, dim3(256), 0, (cudaStream_t)stream, (const uint8_t*)codes,
+    return launch_kernel(quant_read_kernel<T>, grid, dim3(READ_THREADS), 0, (cudaStream_t)stream, (const uint8_t*)codes,
                          fp8, scales, block_table, table_stride, lengths, first, slots, num_slots, S, nkv, hd,
                          page, (T*)out);
   };

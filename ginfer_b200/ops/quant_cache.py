@@ -129,7 +129,7 @@ def read(cache, block_table: torch.Tensor, lengths: torch.Tensor, dtype: torch.d
     f = _fn("quant_cache", "gf_quant_read", _READ_ARGS)
     _ok(f(_p(codes), fp8, _p(scales), _ints(block_table, (B, W), "block_table"), W,
           _ints(lengths, (B,), "lengths"), None if first is None else _ints(first, (B,), "first"), None,
-          0, B, W * page, nkv, hd, page, _p(out), _code(dtype), _stream()), "quant_cache.read")
+          pages * page, B, W * page, nkv, hd, page, _p(out), _code(dtype), _stream()), "quant_cache.read")
     return out
 
 

@@ -88,21 +88,32 @@ __device__ __forceinline__ RowScale row_scale(uint32_t top_bits, int fp8) {
                         1.17549435e-38f);
   return {s, __fdiv_rn(1.0f, s)};
 }
-__device__ __forceinline__ uint32_t code_of(float x, const RowScale& rs, int fp8) {
-  if (rs.inverse == 0.f) return 0u;
-  const float y = __fmul_rn(x, rs.inverse);
+// x / scale is at most Q (1 + 2^-22), which rounds to Q: nothing to saturate.  Integers: 1.5 * 2^23 added leaves the
+// integer, rounded to even, in the low bits.
+__device__ __forceinline__ uint32_t quantise4(const float* v, const RowScale& rs, int fp8) {
+  float y[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = __fmul_rn(v[e], rs.inverse);
+  uint32_t w;
   if (fp8) {
-    uint16_t r;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.f), "f"(y));
-    return r & 0xffu;
+    uint16_t lo, hi;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(y[1]), "f"(y[0]));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(y[3]), "f"(y[2]));
+    w = (uint32_t)lo | (uint32_t)hi << 16;
+  } else {
+    uint32_t n[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) n[e] = __float_as_uint(__fadd_rn(y[e], 12582912.f));
+    w = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
   }
-  return (uint32_t)min(max(__float2int_rn(y), -127), 127) & 0xffu;
+  return rs.inverse == 0.f ? 0u : w;
+}
+__device__ __forceinline__ uint32_t code_of(float x, const RowScale& rs, int fp8) {
+  const float v[4] = {x, 0.f, 0.f, 0.f};
+  return quantise4(v, rs, fp8) & 0xffu;
 }
 __device__ __forceinline__ uint2 quantise8(const float (&v)[8], const RowScale& rs, int fp8) {
-  uint32_t w[2] = {0u, 0u};
-#pragma unroll
-  for (int e = 0; e < 8; ++e) w[e >> 2] |= code_of(v[e], rs, fp8) << (8 * (e & 3));
-  return make_uint2(w[0], w[1]);
+  return make_uint2(quantise4(v, rs, fp8), quantise4(v + 4, rs, fp8));
 }
 
 // ---- codes back to numbers
@@ -112,7 +123,7 @@ __device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t two) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)two));
   return r;
 }
-// 1 / scale's counterpart: what a code stands for in units of its row's scale.
+// What four codes stand for in units of their row's scale.
 __device__ __forceinline__ void values4(uint32_t w, int fp8, float* v) {
   if (fp8) {
     const uint32_t lo = e4m3x2_to_half2(w), hi = e4m3x2_to_half2(w >> 16);

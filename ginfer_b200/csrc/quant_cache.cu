@@ -34,10 +34,10 @@ quant_write_kernel(const T* __restrict__ qkv, int row_stride, int tokens, int nh
                    int vec) {
   pdl_trigger();
   pdl_wait();
-  const int heads = nh + 2 * nkv, sets = (heads + HU - 1) / HU;
+  const int heads = nh + 2 * nkv;
   const int lane = threadIdx.x & (LANES - 1);
-  const unsigned group = blockIdx.x * (unsigned)(WRITE_THREADS / LANES) + threadIdx.x / LANES;
-  const int t = (int)(group / (unsigned)sets), h0 = (int)(group - (unsigned)t * sets) * HU;
+  // (a block's tokens all have the same heads: queries, keys or values, seldom two of them)
+  const int t = blockIdx.x * (WRITE_THREADS / LANES) + threadIdx.x / LANES, h0 = blockIdx.y * HU;
   const bool here = t < tokens && lane * 16 < hd;
   const int half = rot >> 1;
   const bool plain = !neighbours && (half & 7) == 0;
@@ -140,12 +140,11 @@ int launch_write(const void* qkv, int row_stride, int tokens, int nh, int nkv, i
                  cudaStream_t stream) {
   const int heads = nh + 2 * nkv;
   const bool one = (long long)tokens * heads * LANES <= 148 * 1024;
-  const int hu = one ? 1 : 4;
-  const long long groups = (long long)tokens * ((heads + hu - 1) / hu);
-  const long long blocks = (groups * LANES + WRITE_THREADS - 1) / WRITE_THREADS;
-  if (groups > 0x7fffffffLL || blocks > 0x7fffffffLL) return -5;
+  const int hu = one ? 1 : 4, sets = (heads + hu - 1) / hu, each = WRITE_THREADS / LANES;
+  if (sets > 65535) return -5;
+  const dim3 grid((unsigned)((tokens + each - 1) / each), (unsigned)sets);
   const auto run = [&](auto kernel) {
-    return launch_kernel(kernel, dim3((unsigned)blocks), dim3(WRITE_THREADS), 0, stream, (const T*)qkv, row_stride,
+    return launch_kernel(kernel, grid, dim3(WRITE_THREADS), 0, stream, (const T*)qkv, row_stride,
                          tokens, nh, nkv, hd, table, table_rows, rot, neighbours, positions, slots, (T*)q_out,
                          codes, fp8, scales, page, num_slots, vec);
   };

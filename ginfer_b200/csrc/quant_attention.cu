@@ -44,7 +44,9 @@ namespace {
 constexpr int HD = GF_HEAD_DIM;
 static_assert(HD % 16 == 0 && HD >= 16 && HD <= 256, "head size must be a multiple of 16, <= 256");
 constexpr float kLog2E = 1.4426950408889634f;
-constexpr int TILE = 16, WARPS = 4, THREADS = WARPS * 32;
+// Keys of a tile: 32 where a head is short, so that a tile is as many bytes and its steps overlap.
+constexpr int TK = HD <= 64 ? 2 : 1, TILE = 16 * TK, TILE_SHIFT = TK == 2 ? 5 : 4;
+constexpr int WARPS = 4, THREADS = WARPS * 32;
 constexpr int KW = HD % 64 == 0 ? 16 : HD % 32 == 0 ? 8 : 4;     // bytes of a key a thread reads at once
 constexpr int VW = HD % 128 == 0 ? 16 : HD % 64 == 0 ? 8 : HD % 32 == 0 ? 4 : 2;
 constexpr int KWORDS = HD / 16;                                  // words of a key a thread holds
@@ -53,7 +55,7 @@ constexpr int CH = HD / 16;                                      // 16-byte chun
 // Rows in shared memory are 16 bytes apart in banks: a quarter warp's reads of keys (two rows, four
 // places of 16 bytes) and of values (four rows, two places) then hit every bank once.
 constexpr int ROW = HD + 16;
-constexpr int SCALES_AT = 2 * TILE * ROW, STAGE = SCALES_AT + TILE * 16 + 16;
+constexpr int SCALES_AT = 2 * TILE * ROW, STAGE = SCALES_AT + TILE * 16 + TILE;
 #ifndef GF_STAGES
 #define GF_STAGES 3
 #endif
@@ -62,9 +64,10 @@ constexpr int SCALES_AT = 2 * TILE * ROW, STAGE = SCALES_AT + TILE * 16 + 16;
 #endif
 constexpr int STAGES = GF_STAGES;
 // the fewest tiles of a block's run
-constexpr int kLeastTiles = 4 * WARPS;
-// requests that see at most so many keys are one block's work a kv head
-constexpr int kShortKeys = 1024;
+constexpr int kLeastTiles = 4 * WARPS / TK;
+// Requests that see at most kShortKeys keys are one block's work a kv head; up to kMiddleKeys they are where that
+// gives the SMs enough blocks: the joining kernel costs 4 us, as much as 500 keys.
+constexpr int kShortKeys = 256, kMiddleKeys = 1024;
 constexpr int kMostBlocks = 8;          // of the blocks that fit an SM, so many are counted on
 
 struct DecodeArgs {
@@ -105,10 +108,10 @@ __device__ __forceinline__ int request_length(const DecodeArgs& a, int b) {
   return max(min(fresh_index(a.lengths + b), a.limit), 0);
 }
 __device__ __forceinline__ int first_tile(const DecodeArgs& a, int len) {
-  return len > 0 ? first_visible_key(len - 1, a.span) >> 4 : 0;
+  return len > 0 ? first_visible_key(len - 1, a.span) >> TILE_SHIFT : 0;
 }
 __device__ __forceinline__ int request_tiles(const DecodeArgs& a, int len) {
-  return len > 0 ? ((len - 1) >> 4) - first_tile(a, len) + 1 : 1;
+  return len > 0 ? ((len - 1) >> TILE_SHIFT) - first_tile(a, len) + 1 : 1;
 }
 struct Cursor {
   int hc, b, len;             // the item
@@ -206,8 +209,9 @@ __device__ __forceinline__ int page_in(const DecodeArgs& a, int number) {
 __device__ __forceinline__ int logical_page(const DecodeArgs& a, int c) {
   return a.page_shift >= 0 ? c >> a.page_shift : c / a.page;
 }
-// A warp's view of the piece's tiles.  WHOLE: pages are a multiple of the tile, a tile has one page; else a lane
-// knows the page of row `lane % 16`.  Rows outside [lo, end) are zeros and nothing of them is read.
+// A warp's view of an item's tiles.  A lane knows the page of a tile's row `lane`: where pages are a multiple of 16
+// (WHOLE) lanes 0 .. 15 know the first 16 rows', the others the next 16 rows'.  Rows outside [lo, end) are zeros
+// and nothing of them is read.
 template <bool WHOLE> struct Tiles {
   const DecodeArgs& a;
   const int* tbl;
@@ -215,13 +219,20 @@ template <bool WHOLE> struct Tiles {
   __device__ __forceinline__ int row_key(int tile, int r) const { return min(max(tile * TILE + r, lo), end - 1); }
   __device__ __forceinline__ int page_of(int tile) const {
     if (tile >= last || lo >= end) return 0;
-    return page_in(a, fresh_index(tbl + logical_page(a, WHOLE ? tile * TILE : row_key(tile, lane & 15))));
+    return page_in(a, fresh_index(tbl + logical_page(a, row_key(tile, WHOLE ? lane & (TILE - 16) : lane & (TILE - 1)))));
   }
   __device__ __forceinline__ void copy(uint8_t* stage, int tile, int page_number) const {
     const int c0 = tile * TILE;
     const size_t values = (size_t)a.page * HD;
-    const uint8_t* base = nullptr;
-    if constexpr (WHOLE) base = place_of(a, kvh, page_number, c0 - logical_page(a, c0) * a.page).codes;
+    const uint8_t* half[TK];
+    if constexpr (WHOLE) {
+#pragma unroll
+      for (int h = 0; h < TK; ++h) {
+        const int c = c0 + 16 * h;
+        half[h] = place_of(a, kvh, TK == 1 ? page_number : __shfl_sync(0xffffffffu, page_number, 16 * h),
+                           c - logical_page(a, c) * a.page).codes;
+      }
+    }
 #pragma unroll
     for (int i = 0; i < (TILE * CH + 31) / 32; ++i) {
       const int idx = lane + 32 * i, row = idx / CH, ch = idx - row * CH;
@@ -229,9 +240,9 @@ template <bool WHOLE> struct Tiles {
       const bool there = c0 + row >= lo && c0 + row < end;
       const uint8_t* src = a.codes;
       if constexpr (WHOLE) {
-        src = base + idx * 16;
+        src = (TK == 1 || row < 16 ? half[0] : half[TK - 1] - 16 * HD) + idx * 16;
       } else {
-        const int pg = __shfl_sync(0xffffffffu, page_number, row & 15);
+        const int pg = __shfl_sync(0xffffffffu, page_number, row & (TILE - 1));
         const int c = row_key(tile, row);
         if (there) src = place_of(a, kvh, pg, c - logical_page(a, c) * a.page).codes + ch * 16;
       }
@@ -242,8 +253,11 @@ template <bool WHOLE> struct Tiles {
     }
     // the scales: pairs of keys; where a key's neighbour lies elsewhere, the 16 bytes that its own are in
     if constexpr (WHOLE) {
-      const Place pl = place_of(a, kvh, page_number, c0 - logical_page(a, c0) * a.page);
-      if (lane < TILE / 2) copy16(stage + SCALES_AT + lane * 16, pl.scales + 2 * lane, true);
+      const int h = lane / 8, c = c0 + 16 * h;
+      const int pg = TK == 1 ? page_number : __shfl_sync(0xffffffffu, page_number, (16 * h) & 31);
+      if (lane < TILE / 2)
+        copy16(stage + SCALES_AT + lane * 16,
+               place_of(a, kvh, pg, c - logical_page(a, c) * a.page).scales + 2 * (lane & 7), true);
     } else if (lane < TILE) {
       const int c = row_key(tile, lane);
       const bool there = c0 + lane >= lo && c0 + lane < end;
@@ -382,6 +396,16 @@ quant_decode_kernel(const DecodeArgs a) {
   __shared__ __align__(16) uint8_t fresh_row[2][HD];             // STEP: the new token's codes and scales
   __shared__ float fresh_scale[2];
   pdl_trigger();
+  if (a.stream) {
+    // what an item's start waits for comes from far off (the cache has swept it out of L2): asked for early
+    const auto ask = [](const void* at) { asm volatile("prefetch.global.L2 [%0];" ::"l"(at)); };
+    const long long i = (long long)blockIdx.x * THREADS + threadIdx.x;
+    if (i * 32 < a.B) ask(a.lengths + i * 32);
+    if (i * 32 < (long long)a.B * a.table_stride) ask(a.block_table + i * 32);
+    constexpr int LINE = 128 / sizeof(T);
+    const long long lines = a.nh * HD / LINE;
+    if (i < a.B * lines) ask(reinterpret_cast<const T*>(a.q) + (size_t)(i / lines) * a.q_stride + (i % lines) * LINE);
+  }
   pdl_wait();
   const int heads = a.nkv * a.chunks, G = a.nh / a.nkv;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -623,7 +647,9 @@ quant_decode_kernel(const DecodeArgs a) {
       }
       at_stage = at_stage + 1 == STAGES ? 0 : at_stage + 1;
       to_stage = to_stage + 1 == STAGES ? 0 : to_stage + 1;
-      float2 sc[2] = {tiles.scales(stage, g), tiles.scales(stage, g + 8)};
+      float2 sc[2 * TK];           // of keys g, g + 8, ...
+#pragma unroll
+      for (int i = 0; i < 2 * TK; ++i) sc[i] = tiles.scales(stage, g + 8 * i);
       if constexpr (STEP) {
         if (c0 + TILE >= len) {     // the tile of the new token
           const int r = len - 1 - c0;
@@ -635,24 +661,26 @@ quant_decode_kernel(const DecodeArgs a) {
           __syncwarp();
           const float2 mine_sc = make_float2(fresh_scale[0], fresh_scale[1]);
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
+          for (int i = 0; i < 2 * TK; ++i)
             if (g + 8 * i == r) sc[i] = mine_sc;
         }
       }
-      // S^T, in two chains of products
+      // S^T, in two chains of products for each 16 keys
       constexpr int CHAINS = KWORDS > 1 ? 2 : 1;
-      float s2[CHAINS][NT][4];
+      float s[TK][NT][4];
 #pragma unroll
-      for (int c = 0; c < CHAINS; ++c)
+      for (int q = 0; q < TK; ++q) {
+        float s2[CHAINS][NT][4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) s2[c][n][0] = s2[c][n][1] = s2[c][n][2] = s2[c][n][3] = 0.f;
-      {
+        for (int c = 0; c < CHAINS; ++c)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) s2[c][n][0] = s2[c][n][1] = s2[c][n][2] = s2[c][n][3] = 0.f;
         uint32_t k[2][KWORDS];
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int j = 0; j < KWORDS / (KW / 4); ++j)
-            read_bytes<KW>(stage + (g + 8 * i) * ROW + t * (HD / 4) + j * KW, &k[i][j * (KW / 4)]);
+            read_bytes<KW>(stage + (16 * q + g + 8 * i) * ROW + t * (HD / 4) + j * KW, &k[i][j * (KW / 4)]);
 #pragma unroll
         for (int w = 0; w < KWORDS; ++w) {
           const uint32_t k0 = FP8 ? k[0][w] : k[0][w] ^ 0x80808080u, k1 = FP8 ? k[1][w] : k[1][w] ^ 0x80808080u;
@@ -667,122 +695,141 @@ quant_decode_kernel(const DecodeArgs a) {
 #pragma unroll
             for (int i = PARTS - 1; i >= 0; --i) mma_f16(s2[w % CHAINS][n], A, qf[i][n][w][0], qf[i][n][w][1]);
         }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[q][n][e] = CHAINS == 2 ? s2[0][n][e] + s2[CHAINS - 1][n][e] : s2[0][n][e];
       }
-      bool seen[2] = {true, true};
+      bool seen[2 * TK];
+#pragma unroll
+      for (int i = 0; i < 2 * TK; ++i) seen[i] = true;
       if (c0 < lo || c0 + TILE > len) {
         // masked keys: whatever lies there counts as nothing (their codes are zeros already)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < 2 * TK; ++i) {
           const int c = c0 + g + 8 * i;
           seen[i] = c >= lo && c < len;
           if (!seen[i]) sc[i] = make_float2(0.f, 0.f);
         }
       }
       // Scores in units of log2.  m and f are raised only when a score is 2^7 times what m stands for, or a value's
-      // scale above what f stands for: a weight is below 2^(14 + 1 - 8 + 8) until then.
-      float s[NT][4];
+      // scale above what f stands for: a weight is below 2^15 until then.
       bool above = false;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          float r0 = s2[0][n][j], r1 = s2[0][n][2 + j];
-          if constexpr (CHAINS == 2) r0 += s2[1][n][j], r1 += s2[1][n][2 + j];
-          r0 = RAISED ? fmaf(r0, qscale[n][j], qshift[n][j]) : r0 * qscale[n][j];
-          r1 = RAISED ? fmaf(r1, qscale[n][j], qshift[n][j]) : r1 * qscale[n][j];
-          s[n][j] = seen[0] ? r0 * sc[0].x : -INFINITY;
-          s[n][2 + j] = seen[1] ? r1 * sc[1].x : -INFINITY;
-          above |= fmaxf(s[n][j], s[n][2 + j]) > m[n][j] + kSlack;
-        }
-      {
-        // a scale's bits against those of the first power of two that is too large for f
-        const uint32_t bound = (uint32_t)(kTop - f + 1) << 23;
-        const uint32_t b0 = __float_as_uint(sc[0].y), b1 = __float_as_uint(sc[1].y);
-        above |= (b0 >= bound && b0 < 0x7f800000u) || (b1 >= bound && b1 < 0x7f800000u);
-        if (__any_sync(0xffffffffu, above)) {
-          const uint32_t vtop = __reduce_max_sync(0xffffffffu, max(b0 < 0x7f800000u ? b0 : 0u, b1 < 0x7f800000u ? b1 : 0u));
-          const int fn = min(f, kTop - (int)(vtop >> 23));
-          const float shrink = fn == f ? 1.f : f - fn > 126 ? 0.f : __uint_as_float((uint32_t)(127 + fn - f) << 23);
-          f = fn;
+          float top = -INFINITY;
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            float corr[2];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              float top = fmaxf(s[n][j], s[n][2 + j]);
-              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-              const float mn = fmaxf(m[n][j], top);
-              corr[j] = mn == m[n][j] ? 1.f : fast_exp2(m[n][j] - mn);
-              l[n][j] *= corr[j];
-              corr[j] *= shrink;
-              m[n][j] = mn;
-            }
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-              o[n][i][0] *= corr[0], o[n][i][1] *= corr[1], o[n][i][2] *= corr[0], o[n][i][3] *= corr[1];
+          for (int i = 0; i < 2 * TK; ++i) {
+            float& r = s[i >> 1][n][2 * (i & 1) + j];
+            r = RAISED ? fmaf(r, qscale[n][j], qshift[n][j]) : r * qscale[n][j];
+            r = seen[i] ? r * sc[i].x : -INFINITY;
+            top = fmaxf(top, r);
           }
+          above |= top > m[n][j] + kSlack;
+        }
+      // (a scale's bits against those of the first power of two that is too large for f)
+      uint32_t vtop = 0;
+#pragma unroll
+      for (int i = 0; i < 2 * TK; ++i) {
+        const uint32_t bits = __float_as_uint(sc[i].y);
+        vtop = max(vtop, bits < 0x7f800000u ? bits : 0u);
+      }
+      above |= vtop >= (uint32_t)(kTop - f + 1) << 23;
+      if (__any_sync(0xffffffffu, above)) {
+        const int fn = min(f, kTop - (int)(__reduce_max_sync(0xffffffffu, vtop) >> 23));
+        const float shrink = fn == f ? 1.f : f - fn > 126 ? 0.f : __uint_as_float((uint32_t)(127 + fn - f) << 23);
+        f = fn;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float corr[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 2 * TK; ++i) top = fmaxf(top, s[i >> 1][n][2 * (i & 1) + j]);
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+            const float mn = fmaxf(m[n][j], top);
+            corr[j] = mn == m[n][j] ? 1.f : fast_exp2(m[n][j] - mn);
+            l[n][j] *= corr[j];
+            corr[j] *= shrink;
+            m[n][j] = mn;
+          }
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+            o[n][i][0] *= corr[0], o[n][i][1] *= corr[1], o[n][i][2] *= corr[0], o[n][i][3] *= corr[1];
         }
       }
       const float up = __uint_as_float((uint32_t)f << 23);
-      const float vs0 = sc[0].y * up, vs1 = sc[1].y * up;
-      uint32_t P[PARTS][NT][2];
+      uint32_t P[TK][PARTS][NT][2];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float w[4];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float p0 = fast_exp2(s[n][j] - m[n][j]), p1 = fast_exp2(s[n][2 + j] - m[n][j]);
-          l[n][j] += p0 + p1;
-          w[j] = p0 * vs0, w[2 + j] = p1 * vs1;
-        }
-        P[0][n][0] = transposed(pack_half(w[0], w[1]));
-        P[0][n][1] = transposed(pack_half(w[2], w[3]));
-        if constexpr (PARTS == 2) {
-          P[1][n][0] = transposed(pack_half(half_rest(w[0]), half_rest(w[1])));
-          P[1][n][1] = transposed(pack_half(half_rest(w[2]), half_rest(w[3])));
-        }
-      }
-      const auto add = [&](int i, const uint32_t (&A)[4]) {
+      for (int q = 0; q < TK; ++q) {
+        const float vs0 = sc[2 * q].y * up, vs1 = sc[2 * q + 1].y * up;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          if constexpr (PARTS == 2) {
-            float d[4] = {0.f, 0.f, 0.f, 0.f};
-            mma_f16(d, A, P[1][n][0], P[1][n][1]);
-            mma_f16(d, A, P[0][n][0], P[0][n][1]);
+          float w[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[n][i][e] += d[e];
-          } else {
-            mma_f16(o[n][i], A, P[0][n][0], P[0][n][1]);
+          for (int j = 0; j < 2; ++j) {
+            const float p0 = fast_exp2(s[q][n][j] - m[n][j]), p1 = fast_exp2(s[q][n][2 + j] - m[n][j]);
+            l[n][j] += p0 + p1;
+            w[j] = p0 * vs0, w[2 + j] = p1 * vs1;
+          }
+          P[q][0][n][0] = transposed(pack_half(w[0], w[1]));
+          P[q][0][n][1] = transposed(pack_half(w[2], w[3]));
+          if constexpr (PARTS == 2) {
+            P[q][PARTS - 1][n][0] = transposed(pack_half(half_rest(w[0]), half_rest(w[1])));
+            P[q][PARTS - 1][n][1] = transposed(pack_half(half_rest(w[2]), half_rest(w[3])));
           }
         }
-      };
+      }
 #pragma unroll
       for (int j = 0; j < HD / (8 * VW); ++j) {
-        constexpr int WORDS = VW >= 4 ? VW / 4 : 1;
-        uint32_t v[4][WORDS];          // keys 2t, 2t + 1, 2t + 8, 2t + 9
+        constexpr int WORDS = VW >= 4 ? VW / 4 : 1, PER = VW >= 4 ? 2 : 1;
+        float d[WORDS * PER][NT][4];       // 32-bit results: a tile's products are added up outside the tensor cores
+        if constexpr (PARTS == 2)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          read_bytes<VW>(stage + (TILE + 2 * t + (i & 1) + 8 * (i >> 1)) * ROW + (j * 8 + g) * VW, v[i]);
-          if constexpr (!FP8) {
+          for (int i = 0; i < WORDS * PER; ++i)
 #pragma unroll
-            for (int w = 0; w < WORDS; ++w) v[i][w] ^= 0x80808080u;
+            for (int n = 0; n < NT; ++n) d[i][n][0] = d[i][n][1] = d[i][n][2] = d[i][n][3] = 0.f;
+#pragma unroll
+        for (int q = 0; q < TK; ++q) {
+          uint32_t v[4][WORDS];            // keys 2t, 2t + 1, 2t + 8, 2t + 9 of the 16
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            read_bytes<VW>(stage + (TILE + 16 * q + 2 * t + (i & 1) + 8 * (i >> 1)) * ROW + (j * 8 + g) * VW, v[i]);
+            if constexpr (!FP8) {
+#pragma unroll
+              for (int w = 0; w < WORDS; ++w) v[i][w] ^= 0x80808080u;
+            }
           }
-        }
 #pragma unroll
-        for (int w = 0; w < WORDS; ++w) {
-          const uint32_t u0 = __byte_perm(v[0][w], v[1][w], 0x5140), u1 = __byte_perm(v[2][w], v[3][w], 0x5140);
-          const uint32_t A[4] = {halves<FP8>(u0, 0), halves<FP8>(u0, 1), halves<FP8>(u1, 0), halves<FP8>(u1, 1)};
-          if constexpr (VW >= 4) {
-            add(2 * (j * WORDS + w), A);
-            const uint32_t y0 = __byte_perm(v[0][w], v[1][w], 0x7362), y1 = __byte_perm(v[2][w], v[3][w], 0x7362);
-            const uint32_t C[4] = {halves<FP8>(y0, 0), halves<FP8>(y0, 1), halves<FP8>(y1, 0), halves<FP8>(y1, 1)};
-            add(2 * (j * WORDS + w) + 1, C);
-          } else {
-            add(j, A);
-          }
+          for (int w = 0; w < WORDS; ++w)
+#pragma unroll
+            for (int y = 0; y < PER; ++y) {
+              const uint32_t u0 = __byte_perm(v[0][w], v[1][w], y ? 0x7362 : 0x5140);
+              const uint32_t u1 = __byte_perm(v[2][w], v[3][w], y ? 0x7362 : 0x5140);
+              const uint32_t A[4] = {halves<FP8>(u0, 0), halves<FP8>(u0, 1), halves<FP8>(u1, 0), halves<FP8>(u1, 1)};
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                if constexpr (PARTS == 2) {
+                  mma_f16(d[w * PER + y][n], A, P[q][1][n][0], P[q][1][n][1]);
+                  mma_f16(d[w * PER + y][n], A, P[q][0][n][0], P[q][0][n][1]);
+                } else {
+                  mma_f16(o[n][(j * WORDS + w) * PER + y], A, P[q][0][n][0], P[q][0][n][1]);
+                }
+              }
+            }
         }
+        if constexpr (PARTS == 2)
+#pragma unroll
+          for (int i = 0; i < WORDS * PER; ++i)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[n][j * WORDS * PER + i][e] += d[i][n][e];
       }
     }
   }
@@ -791,7 +838,7 @@ quant_decode_kernel(const DecodeArgs a) {
 // A block an item and `gridDim.y`-th of its heads: the pieces' results, weighted by their shares of the sum.
 // A team of HD / 4 threads takes a head where there are few pieces, else every TEAMS-th piece of every head:
 // its loads are then under way together, and the teams' sums are added in order.
-constexpr int JOIN_THREADS = 256, TEAM = HD / 4, TEAMS = JOIN_THREADS / TEAM, JOIN_AT_ONCE = 8, FEW_PIECES = 8;
+constexpr int JOIN_THREADS = 512, TEAM = HD / 4, TEAMS = JOIN_THREADS / TEAM, JOIN_AT_ONCE = 8, FEW_PIECES = 8;
 struct Joined {
   float4 o;
   float m, l;
@@ -899,7 +946,7 @@ int launch_decode(DecodeArgs a, int sms, void* scratch, size_t scratch_bytes, cu
   const int heads = a.nkv * a.chunks;
   const long long items = (long long)a.B * heads;
   const long long keys = a.span ? std::min(std::abs((long long)a.span), (long long)a.limit) : a.limit;
-  a.stream = keys > kShortKeys;
+  a.stream = keys > kMiddleKeys || (keys > kShortKeys && items < sms);
   const long long blocks = a.stream ? (long long)sms * std::min(std::max(1, blocks_a_sm[dev]), kMostBlocks) : items;
   if (items > 0x7fffffffLL || blocks > 0x7fffffffLL) return -5;
   if (a.stream) {
@@ -923,47 +970,65 @@ using namespace gf;
 
 GF_DEFINE_PDL_SWITCH
 
-// Scratch that any call with these sizes is content with.
-GF_EXPORT long long gf_quant_decode_scratch(int B, int nh, int nkv, int sms) {
-  const int G = nh / nkv, chunks = (G + 15) / 16, rows = (G + chunks - 1) / chunks;
-  return (long long)sms * kMostBlocks * 2 * rows * (HD + 2) * 4 + 8LL * B * nkv * chunks + 16;
-}
+// A call: q [B, nh HD], or with `step` q | k | v [B, (nh + 2 nkv) HD] and the table of angles as gf_quant_write takes
+// it.  Scratch: room for two parts of an item a block, of at most kMostBlocks blocks an SM, and 8 bytes an item;
+// none is needed where no request sees more than kShortKeys keys.
+struct DecodeCall {
+  const void* q;
+  long long q_stride, f32;
+  void* codes;
+  long long fp8;
+  float* scales;
+  const int* block_table;
+  long long table_stride, table_width;
+  const int* lengths;
+  long long pages;
+  void* out;
+  long long B, nh, nkv, page, span, step;
+  const float* table;
+  long long table_rows, rot, neighbours, sms;
+  void* scratch;
+  long long scratch_bytes;
+  cudaStream_t stream;
+  double scale;
+};
+static_assert(sizeof(DecodeCall) == 27 * 8, "the caller packs it");
 
-// q [B, nh HD], or with `step` q | k | v [B, (nh + 2 nkv) HD] and the table of angles as gf_quant_write takes it.
-GF_EXPORT int gf_quant_decode(const void* q, int q_stride, int f32, void* codes, int fp8, float* scales,
-                              const int* block_table, int table_stride, int table_width, const int* lengths, int pages,
-                              void* out, int B, int nh, int nkv, int page, int span, float scale,
-                              int step, const float* table, int table_rows, int rot, int neighbours, int sms,
-                              void* scratch, long long scratch_bytes, void* stream) {
-  if (B <= 0) return B < 0 ? -3 : 0;
-  if (nkv < 1 || nh < nkv || nh % nkv || page < 1 || pages < 1 || table_width < 0 || B > 65535 || sms < 1)
+GF_EXPORT int gf_quant_decode(const DecodeCall* call) {
+  const DecodeCall& c = *call;
+  if (c.B <= 0) return c.B < 0 ? -3 : 0;
+  if (c.nkv < 1 || c.nh < c.nkv || c.nh % c.nkv || c.nh > 1 << 20 || c.page < 1 || c.pages < 1 || c.table_width < 0 ||
+      c.B > 1 << 24 || c.sms < 1 || c.span > 0x7fffffff || c.span < -0x7fffffff)
     return -3;
-  if ((size_t)codes % 16 || (size_t)scales % 8) return -3;
-  if (step && (rot < 0 || rot % 2 || rot > HD || (rot && (!table || table_rows < 1)))) return -3;
+  if (c.step && (c.rot < 0 || c.rot % 2 || c.rot > HD || (c.rot && (!c.table || c.table_rows < 1)))) return -3;
+  if ((size_t)c.codes % 16 || (size_t)c.scales % 8) return -3;
+  if (c.q_stride > 0x7fffffff || c.q_stride < 0 || c.table_stride > 0x7fffffff) return -3;
   DecodeArgs a = {};
-  a.q = q, a.q_stride = q_stride;
-  a.codes = (uint8_t*)codes, a.scales = scales;
-  a.block_table = block_table, a.table_stride = table_stride;
-  a.limit = (int)min((long long)table_width * page, 0x7fffffe0LL);
-  a.pages = pages, a.lengths = lengths, a.out = out, a.out_f32 = f32;
-  a.B = B, a.nh = nh, a.nkv = nkv, a.page = page, a.span = span, a.scale = scale;
-  a.page_shift = (page & (page - 1)) == 0 ? __builtin_ctz(page) : -1;
-  a.table = table, a.table_rows = table_rows > 0 ? table_rows : 1, a.rot = rot, a.neighbours = neighbours;
-  const int G = nh / nkv;
+  a.q = c.q, a.q_stride = (int)c.q_stride;
+  a.codes = (uint8_t*)c.codes, a.scales = c.scales;
+  a.block_table = c.block_table, a.table_stride = (int)c.table_stride;
+  a.limit = (int)std::min(c.table_width * c.page, 0x7fffffe0LL - 64);
+  a.pages = (int)c.pages, a.lengths = c.lengths, a.out = c.out, a.out_f32 = c.f32 != 0;
+  a.B = (int)c.B, a.nh = (int)c.nh, a.nkv = (int)c.nkv, a.page = (int)c.page, a.span = (int)c.span;
+  a.scale = (float)c.scale;
+  a.page_shift = (a.page & (a.page - 1)) == 0 ? __builtin_ctz(a.page) : -1;
+  a.table = c.table, a.table_rows = c.table_rows > 0 ? (int)c.table_rows : 1, a.rot = (int)c.rot;
+  a.neighbours = c.neighbours != 0;
+  const int G = a.nh / a.nkv;
   a.chunks = (G + 15) / 16, a.rows = (G + a.chunks - 1) / a.chunks;
   const auto go = [&](auto nt, auto kind, auto type, auto whole, auto fused) {
     return launch_decode<decltype(nt)::value, decltype(kind)::value, decltype(type), decltype(whole)::value,
-                         decltype(fused)::value>(a, sms, scratch, (size_t)scratch_bytes, (cudaStream_t)stream);
+                         decltype(fused)::value>(a, (int)c.sms, c.scratch, (size_t)c.scratch_bytes, c.stream);
   };
   const auto pick_bool = [](bool x, auto next) {
     return x ? next(std::true_type()) : next(std::false_type());
   };
-  return pick_bool(fp8 != 0, [&](auto kind) {
-    return pick_bool(page % TILE == 0 && (size_t)scales % 16 == 0, [&](auto whole) {
-      return pick_bool(step != 0, [&](auto fused) {
+  return pick_bool(c.fp8 != 0, [&](auto kind) {
+    return pick_bool(a.page % 16 == 0 && (size_t)c.scales % 16 == 0, [&](auto whole) {
+      return pick_bool(c.step != 0, [&](auto fused) {
         using One = std::integral_constant<int, 1>;
         using Two = std::integral_constant<int, 2>;
-        if (f32) return a.rows > 8 ? go(Two(), kind, float(), whole, fused) : go(One(), kind, float(), whole, fused);
+        if (c.f32) return a.rows > 8 ? go(Two(), kind, float(), whole, fused) : go(One(), kind, float(), whole, fused);
         return a.rows > 8 ? go(Two(), kind, bf16(), whole, fused) : go(One(), kind, bf16(), whole, fused);
       });
     });

@@ -239,46 +239,77 @@ using namespace gf;
 GF_DEFINE_PDL_SWITCH
 
 // qkv [T, >= (nh + 2 nkv) hd] with `row_stride`; table [table_rows, rot] fp32 (cosines, sines) or null with
-// rot 0; q_out [T, nh hd].  A slot outside [0, num_slots) is not written, a position outside the table takes
-// its nearest row.
-GF_EXPORT int gf_quant_write(const void* qkv, int row_stride, int dtype, int tokens, int nh, int nkv, int hd,
-                             const float* table, int table_rows, int rot, int neighbours, const int* positions,
-                             const int* slots, void* q_out, void* codes, int fp8, float* scales, int page,
-                             int num_slots, void* stream) {
-  if (tokens <= 0) return tokens < 0 ? -3 : 0;
-  if (hd % 16 || hd < 16 || hd > 256 || nh < 1 || nkv < 1 || page < 1 || rot < 0 || rot % 2 || rot > hd ||
-      (rot && (!table || table_rows < 1)))
+// rot 0; q_out [T, nh hd].  A slot outside the cache is not written, a position outside the table takes its
+// nearest row.
+struct WriteCall {
+  const void* qkv;
+  long long row_stride, dtype, tokens, nh, nkv, hd;
+  const float* table;
+  long long table_rows, rot, neighbours;
+  const int *positions, *slots;
+  void *q_out, *codes;
+  long long fp8;
+  float* scales;
+  long long page, pages;
+  cudaStream_t stream;
+};
+static_assert(sizeof(WriteCall) == 20 * 8, "the caller packs it");
+
+GF_EXPORT int gf_quant_write(const WriteCall* call) {
+  const WriteCall& c = *call;
+  if (c.tokens <= 0) return c.tokens < 0 ? -3 : 0;
+  if (c.hd % 16 || c.hd < 16 || c.hd > 256 || c.nh < 1 || c.nkv < 1 || c.nh > 1 << 20 || c.nkv > 1 << 20 || c.page < 1 ||
+      c.pages < 0 || c.page * c.pages > 0x7fffffffLL || c.rot < 0 || c.rot % 2 || c.rot > c.hd ||
+      (c.rot && (!c.table || c.table_rows < 1)) || c.tokens > 0x7fffffff || c.row_stride > 0x7fffffff || c.row_stride < 0)
     return -3;
-  const size_t es = dtype == GF_F32 ? 4 : 2;
-  if ((size_t)codes % 16 || (size_t)scales % 8) return -3;
+  const size_t es = c.dtype == GF_F32 ? 4 : 2;
+  if ((size_t)c.codes % 16 || (size_t)c.scales % 8) return -3;
   // whether rows (1) and the table (2) can be read 16 bytes at a time
-  const int vec = ((size_t)qkv % 16 == 0 && (size_t)row_stride * es % 16 == 0 ? 1 : 0) | ((size_t)table % 16 == 0 ? 2 : 0);
+  const int vec = ((size_t)c.qkv % 16 == 0 && (size_t)c.row_stride * es % 16 == 0 ? 1 : 0) |
+                  ((size_t)c.table % 16 == 0 ? 2 : 0);
   const auto go = [&](auto tag) {
     using T = decltype(tag);
     const auto run = [&](auto launch) {
-      return launch(qkv, row_stride, tokens, nh, nkv, hd, table, table_rows, rot, neighbours, positions, slots,
-                    q_out, (uint8_t*)codes, fp8, scales, page, num_slots, vec, (cudaStream_t)stream);
+      return launch(c.qkv, (int)c.row_stride, (int)c.tokens, (int)c.nh, (int)c.nkv, (int)c.hd, c.table, (int)c.table_rows,
+                    (int)c.rot, c.neighbours != 0, c.positions, c.slots, c.q_out, (uint8_t*)c.codes, (int)c.fp8, c.scales,
+                    (int)c.page, (int)(c.page * c.pages), vec, c.stream);
     };
-    if (hd <= 64) return run(launch_write<T, 4>);
-    if (hd <= 128) return run(launch_write<T, 8>);
+    if (c.hd <= 64) return run(launch_write<T, 4>);
+    if (c.hd <= 128) return run(launch_write<T, 8>);
     return run(launch_write<T, 16>);
   };
-  return dtype == GF_F32 ? go(float()) : go(bf16());
+  return c.dtype == GF_F32 ? go(float()) : go(bf16());
 }
 
 // block_table, lengths (and first, may be null) of B requests, out [2, B, S, nkv, hd]; or slots [S] with B = 1.
-GF_EXPORT int gf_quant_read(const void* codes, int fp8, const float* scales, const int* block_table,
-                            int table_stride, const int* lengths, const int* first, const int* slots,
-                            int num_slots, int B, int S, int nkv, int hd, int page, void* out, int dtype,
-                            void* stream) {
-  if (B <= 0 || S <= 0) return B < 0 || S < 0 ? -3 : 0;
-  if (hd % 16 || hd < 16 || hd > 256 || nkv < 1 || page < 1 || B > 65535 || (size_t)codes % 16) return -3;
-  const dim3 grid((unsigned)(((long long)S + READ_SPAN - 1) / READ_SPAN), (unsigned)B);
+struct ReadCall {
+  const void* codes;
+  long long fp8;
+  const float* scales;
+  const int* block_table;
+  long long table_stride;
+  const int *lengths, *first, *slots;
+  long long pages, B, S, nkv, hd, page;
+  void* out;
+  long long dtype;
+  cudaStream_t stream;
+};
+static_assert(sizeof(ReadCall) == 17 * 8, "the caller packs it");
+
+GF_EXPORT int gf_quant_read(const ReadCall* call) {
+  const ReadCall& c = *call;
+  if (c.B <= 0 || c.S <= 0) return c.B < 0 || c.S < 0 ? -3 : 0;
+  if (c.hd % 16 || c.hd < 16 || c.hd > 256 || c.nkv < 1 || c.nkv > 1 << 20 || c.page < 1 || c.pages < 0 ||
+      c.page * c.pages > 0x7fffffffLL || c.B > 65535 || c.S > 0x7fffffff - READ_SPAN || c.table_stride > 0x7fffffff ||
+      (size_t)c.codes % 16)
+    return -3;
+  const dim3 grid((unsigned)((c.S + READ_SPAN - 1) / READ_SPAN), (unsigned)c.B);
   const auto go = [&](auto tag) {
     using T = decltype(tag);
-    return launch_kernel(quant_read_kernel<T>, grid, dim3(READ_THREADS), 0, (cudaStream_t)stream, (const uint8_t*)codes,
-                         fp8, scales, block_table, table_stride, lengths, first, slots, num_slots, S, nkv, hd,
-                         page, (T*)out);
+    return launch_kernel(quant_read_kernel<T>, grid, dim3(READ_THREADS), 0, c.stream,
+                         (const uint8_t*)c.codes, (int)c.fp8, c.scales, c.block_table, (int)c.table_stride, c.lengths,
+                         c.first, c.slots, (int)(c.page * c.pages), (int)c.S, (int)c.nkv, (int)c.hd, (int)c.page,
+                         (T*)c.out);
   };
-  return dtype == GF_F32 ? go(float()) : go(bf16());
+  return c.dtype == GF_F32 ? go(float()) : go(bf16());
 }

@@ -63,14 +63,14 @@ class _Counter:
 _fns: dict = {}
 
 
-def _fn(lib_name: str, fn_name: str, argtypes, defines=(), kernels: int = 1, restype=c_int):
+def _fn(lib_name: str, fn_name: str, argtypes, defines=(), kernels: int = 1):
     key = (lib_name, tuple(defines), fn_name)
     g = _fns.get(key)
     if g is None:
         lib = load_library(lib_name, tuple(defines))
         f = getattr(lib, fn_name)
         f.argtypes = argtypes
-        f.restype = restype
+        f.restype = c_int
 
         def g(*args, _f=f, _k=kernels):
             _Counter.launches += _k

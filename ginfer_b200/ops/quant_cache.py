@@ -11,20 +11,29 @@ with ``Q`` 127 or 448; a row with an infinity or a NaN reads back as NaN.  A tok
 * page + place in the page``; ``block_table [B, W]`` int32 names a request's pages in order (entries behind
 its length are not read), ``lengths [B]`` int32 its tokens, the new one among them.
 
-All work goes to the current stream; nothing is kept between calls.
+All work goes to the current stream; nothing but scratch memory (one buffer a stream) is kept between calls.
+
+A call's integers and addresses reach the library as one block of 64-bit words: a decode step makes a call a
+layer, and converting two dozen arguments one by one costs more than the small kernels run.
 """
 from __future__ import annotations
 
-from ctypes import c_float, c_int, c_longlong, c_void_p
+import struct
+from ctypes import c_char_p, c_int
 
 import torch
 
-from . import _code, _fn, _ok, _p, _stream
+from . import _Counter, _ok
+from .build import load_library
 from .gemm_bf16 import num_sms
 
 KINDS = {"int8": torch.int8, "fp8": torch.float8_e4m3fn}
-_FP8 = {torch.int8: 0, torch.float8_e4m3fn: 1}
 MAX_HEAD_DIM = 256
+_FP8 = {torch.int8: 0, torch.float8_e4m3fn: 1}
+_CODE = {torch.float32: 0, torch.bfloat16: 1}
+_WRITE, _READ, _DECODE = struct.Struct("=20q"), struct.Struct("=17q"), struct.Struct("=26qd")
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+_int32, _float32 = torch.int32, torch.float32
 
 
 def supports(head_dim: int, heads: int, kv_heads: int) -> bool:
@@ -40,18 +49,31 @@ def make_cache(kind: str, pages: int, kv_heads: int, page: int, head_dim: int, d
             torch.zeros(pages, kv_heads, page, 2, dtype=torch.float32, device=device))
 
 
+# ----------------------------------------------------------------------------- arguments
+_functions: dict = {}
+
+
+def _function(lib: str, name: str, defines=()):
+    f = _functions.get((name, defines))
+    if f is None:
+        f = getattr(load_library(lib, defines), name)
+        f.argtypes, f.restype = [c_char_p], c_int
+        _functions[name, defines] = f
+    return f
+
+
 def _cache(cache):
     """The checked facts of a cache: codes, scales, kind, pages, kv heads, page, head size."""
     codes, scales = cache
     fp8 = _FP8.get(codes.dtype)
     if fp8 is None:
         raise TypeError(f"codes are int8 or float8_e4m3fn, not {codes.dtype}")
-    if codes.dim() != 5 or codes.shape[2] != 2 or not codes.is_contiguous():
-        raise ValueError("codes are [pages, kv heads, 2, page, head size], contiguous; got "
-                         f"{tuple(codes.shape)}")
-    pages, nkv, _, page, hd = codes.shape
-    if scales.dtype != torch.float32 or scales.shape != (pages, nkv, page, 2) or not scales.is_contiguous():
-        raise ValueError(f"the scales of codes {tuple(codes.shape)} are fp32 {(pages, nkv, page, 2)}, "
+    shape = codes.shape
+    if len(shape) != 5 or shape[2] != 2 or not codes.is_contiguous():
+        raise ValueError(f"codes are [pages, kv heads, 2, page, head size], contiguous; got {tuple(shape)}")
+    pages, nkv, _, page, hd = shape
+    if scales.dtype is not _float32 or scales.shape != (pages, nkv, page, 2) or not scales.is_contiguous():
+        raise ValueError(f"the scales of codes {tuple(shape)} are fp32 {(pages, nkv, page, 2)}, "
                          f"contiguous; got {scales.dtype} {tuple(scales.shape)}")
     if hd % 16 or not 16 <= hd <= MAX_HEAD_DIM:
         raise ValueError(f"a cache of 8 bits takes head sizes that are a multiple of 16, at most "
@@ -61,29 +83,57 @@ def _cache(cache):
     return codes, scales, fp8, pages, nkv, page, hd
 
 
-def _ints(t, shape, what):
-    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
+def _elsewhere(t):
+    raise RuntimeError("ginfer_b200 kernels run on a CUDA device only, the current one, where all of a call's tensors "
+                       f"are; got a tensor on {t.device}")
+
+
+def _device(codes) -> int:
+    """The number of the device that a call runs on."""
+    device = codes.get_device()
+    if device < 0 or device != _current_device():
+        _elsewhere(codes)
+    return device
+
+
+def _at(t, device: int):
+    """The address of a tensor on the call's device."""
+    if t.get_device() != device:
+        _elsewhere(t)
+    return t.data_ptr()
+
+
+def _ints(t, shape, what, device):
+    if t.dtype is not _int32 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{what} is int32 {tuple(shape)}, contiguous; got {t.dtype} {tuple(t.shape)}")
-    return _p(t)
+    return _at(t, device)
 
 
-def _rows(x, columns, what):
+def _code(dtype):
+    code = _CODE.get(dtype)
+    if code is None:
+        raise TypeError(f"kernels take float32 or bfloat16 activations, not {dtype}")
+    return code
+
+
+def _rows(x, columns, what, device):
+    """(address, stride, type) of rows."""
     if x.dim() != 2 or x.shape[1] < columns or x.stride(1) != 1:
         raise ValueError(f"{what} has rows of at least {columns} channels without gaps; got "
                          f"{tuple(x.shape)}, strides {tuple(x.stride())}")
-    return _p(x), x.stride(0), _code(x.dtype)
+    return _at(x, device), x.stride(0), _code(x.dtype)
 
 
-def _angles(table, hd):
+def _angles(table, hd, device):
     """(address, rows, rotated channels) of a table of cosines and sines."""
     if table is None:
-        return None, 0, 0
+        return 0, 0, 0
     rot = table.shape[-1]
-    if (table.dtype != torch.float32 or table.dim() != 2 or not table.is_contiguous() or rot % 2 or rot > hd
+    if (table.dtype is not _float32 or table.dim() != 2 or not table.is_contiguous() or rot % 2 or rot > hd
             or table.shape[0] < 1):
         raise ValueError(f"the table of angles is fp32 [positions, an even number up to {hd}], contiguous; "
                          f"got {table.dtype} {tuple(table.shape)}")
-    return _p(table), table.shape[0], rot
+    return _at(table, device), table.shape[0], rot
 
 
 def _heads(nh, nkv):
@@ -91,6 +141,7 @@ def _heads(nh, nkv):
         raise ValueError(f"{nh} query heads are not a multiple of {nkv} kv heads")
 
 
+# ----------------------------------------------------------------------------- the operators
 def write(qkv: torch.Tensor, nh: int, table, positions: torch.Tensor, slots: torch.Tensor, cache, *,
           neighbours: bool = False) -> torch.Tensor:
     """Rows ``qkv [T, (nh + 2 kv heads) * head size]`` (bf16 or fp32) of a step: q and k are rotated by
@@ -100,82 +151,115 @@ def write(qkv: torch.Tensor, nh: int, table, positions: torch.Tensor, slots: tor
     ``table [positions, rot]`` fp32: cosines, then sines, of the angles of ``rot / 2`` pairs; the first
     ``rot`` channels of a head turn in pairs ``(j, j + rot/2)``, or ``(2j, 2j + 1)`` with ``neighbours``.
     ``None``: nothing turns.  ``positions``, ``slots`` int32 ``[T]``: a token whose slot is negative (or
-    beyond the cache) is not written; two tokens of one call have different slots."""
+    beyond the cache) is not written; two tokens of one call have different slots.  A position beyond the
+    table takes its last row."""
     codes, scales, fp8, pages, nkv, page, hd = _cache(cache)
     _heads(nh, nkv)
-    x, stride, code = _rows(qkv, (nh + 2 * nkv) * hd, "qkv")
+    dev = _device(codes)
+    x, stride, code = _rows(qkv, (nh + 2 * nkv) * hd, "qkv", dev)
     T = qkv.shape[0]
-    at, rows, rot = _angles(table, hd)
+    at, rows, rot = _angles(table, hd, dev)
     q = torch.empty((T, nh * hd), dtype=qkv.dtype, device=qkv.device)
-    f = _fn("quant_cache", "gf_quant_write",
-            [c_void_p] + [c_int] * 6 + [c_void_p] + [c_int] * 3 + [c_void_p] * 4
-            + [c_int, c_void_p, c_int, c_int, c_void_p])
-    _ok(f(x, stride, code, T, nh, nkv, hd, at, rows, rot, int(neighbours), _ints(positions, (T,), "positions"),
-          _ints(slots, (T,), "slots"), _p(q), _p(codes), fp8, _p(scales), page, pages * page, _stream()),
-        "quant_cache.write")
+    f = _function("quant_cache", "gf_quant_write")
+    rc = f(_WRITE.pack(x, stride, code, T, nh, nkv, hd, at, rows, rot, neighbours,
+                       _ints(positions, (T,), "positions", dev), _ints(slots, (T,), "slots", dev), q.data_ptr(),
+                       codes.data_ptr(), fp8, _at(scales, dev), page, pages, _raw_stream(dev)))
+    _Counter.launches += 1
+    if rc:
+        _ok(rc, "quant_cache.write")
     return q
 
 
-_READ_ARGS = [c_void_p, c_int, c_void_p, c_void_p, c_int] + [c_void_p] * 3 + [c_int] * 6 + [c_void_p, c_int, c_void_p]
+def _read(facts, block_table, W, lengths, first, slots, B, S, dtype, dev):
+    codes, scales, fp8, pages, nkv, page, hd = facts
+    out = torch.empty((2, B, S, nkv, hd) if slots == 0 else (2, S, nkv, hd), dtype=dtype, device=codes.device)
+    rc = _function("quant_cache", "gf_quant_read")(
+        _READ.pack(codes.data_ptr(), fp8, _at(scales, dev), block_table, W, lengths, first, slots, pages, B, S,
+                   nkv, hd, page, out.data_ptr(), _code(dtype), _raw_stream(dev)))
+    _Counter.launches += 1
+    if rc:
+        _ok(rc, "quant_cache.read")
+    return out
 
 
 def read(cache, block_table: torch.Tensor, lengths: torch.Tensor, dtype: torch.dtype, first=None
          ) -> torch.Tensor:
     """``[2, B, W * page, kv heads, head size]`` in ``dtype`` (bf16 or fp32): the keys and values of the
     tokens ``first[b] <= c < lengths[b]`` (``first`` ``None``: from the first one), zeros elsewhere."""
-    codes, scales, fp8, pages, nkv, page, hd = _cache(cache)
+    facts = _cache(cache)
+    _code(dtype)
+    dev = _device(facts[0])
     B, W = block_table.shape
-    out = torch.empty((2, B, W * page, nkv, hd), dtype=dtype, device=codes.device)
-    f = _fn("quant_cache", "gf_quant_read", _READ_ARGS)
-    _ok(f(_p(codes), fp8, _p(scales), _ints(block_table, (B, W), "block_table"), W,
-          _ints(lengths, (B,), "lengths"), None if first is None else _ints(first, (B,), "first"), None,
-          pages * page, B, W * page, nkv, hd, page, _p(out), _code(dtype), _stream()), "quant_cache.read")
-    return out
+    return _read(facts, _ints(block_table, (B, W), "block_table", dev), W, _ints(lengths, (B,), "lengths", dev),
+                 0 if first is None else _ints(first, (B,), "first", dev), 0, B, W * facts[5], dtype, dev)
 
 
 def read_slots(cache, slots: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     """``[2, N, kv heads, head size]``: the keys and values in ``slots [N]``, zeros for a negative one."""
-    codes, scales, fp8, pages, nkv, page, hd = _cache(cache)
+    facts = _cache(cache)
+    _code(dtype)
+    dev = _device(facts[0])
     N = slots.shape[0]
-    out = torch.empty((2, N, nkv, hd), dtype=dtype, device=codes.device)
-    f = _fn("quant_cache", "gf_quant_read", _READ_ARGS)
-    _ok(f(_p(codes), fp8, _p(scales), None, 0, None, None, _ints(slots, (N,), "slots"), pages * page, 1, N,
-          nkv, hd, page, _p(out), _code(dtype), _stream()), "quant_cache.read_slots")
-    return out
+    if N == 0:
+        return torch.empty((2, 0, facts[4], facts[6]), dtype=dtype, device=slots.device)
+    return _read(facts, 0, 0, 0, 0, _ints(slots, (N,), "slots", dev), 1, N, dtype, dev)
 
 
-_DECODE_ARGS = ([c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p]
-                + [c_int] * 5 + [c_float, c_int, c_void_p] + [c_int] * 4 + [c_void_p, c_longlong, c_void_p])
-_F32 = {torch.float32: 1, torch.bfloat16: 0}
 # Requests of at most this many visible tokens are one block's work a kv head and need no scratch (the kernel has the
 # same line: kShortKeys).
-_SHORT = 1024
+_SHORT = 256
+_scratch: dict = {}
+_sms: dict = {}
+
+
+def _scratch_for(words: int, device: int, stream: int) -> torch.Tensor:
+    """A buffer that only this stream's calls use; a graph that is being captured keeps one of its own."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(words, dtype=torch.float32, device=device)
+    buf = _scratch.get((device, stream))
+    if buf is None or buf.numel() < words:
+        buf = _scratch[device, stream] = torch.empty(max(words, 1 << 18), dtype=torch.float32, device=device)
+    return buf
 
 
 def _decode(q, nh, facts, block_table, lengths, scale, span, fused=None):
-    """``fused``: ``(address, rows, rotated channels)`` of the table of angles and ``neighbours``."""
+    """``fused``: ``(table of angles, neighbours)``."""
     codes, scales, fp8, pages, nkv, page, hd = facts
     _heads(nh, nkv)
-    x, stride, code = _rows(q, (nh if fused is None else nh + 2 * nkv) * hd, "q" if fused is None else "qkv")
+    dev = _device(codes)
+    x, stride, code = _rows(q, nh * hd, "q", dev) if fused is None else _rows(q, (nh + 2 * nkv) * hd, "qkv", dev)
     B, W = block_table.shape
     if q.shape[0] != B:
         raise ValueError(f"{q.shape[0]} queries for {B} requests")
+    table, rows, rot = (0, 0, 0) if fused is None else _angles(fused[0], hd, dev)
     out = torch.empty((B, nh * hd), dtype=q.dtype, device=q.device)
-    defines = (f"GF_HEAD_DIM={hd}",)
-    sms = num_sms(q.device)
+    sms = _sms.get(dev)
+    if sms is None:
+        sms = _sms[dev] = num_sms(dev)
+    stream = _raw_stream(dev)
     scratch, words = None, 0
     if W * page > _SHORT:
-        size = _fn("quant_attention", "gf_quant_decode_scratch", [c_int] * 4, defines, kernels=0, restype=c_longlong)
-        words = size(B, nh, nkv, sms) // 4
-        scratch = torch.empty(words, dtype=torch.float32, device=q.device)
-    f = _fn("quant_attention", "gf_quant_decode", _DECODE_ARGS, defines)
-    table, rows, rot, neighbours = (None, 0, 0, 0) if fused is None else fused
-    f32 = _F32[q.dtype]
-    _ok(f(x, stride, f32, _p(codes), fp8, _p(scales), _ints(block_table, (B, W), "block_table"), W, W,
-          _ints(lengths, (B,), "lengths"), pages, _p(out), B, nh, nkv, page, int(span), float(scale),
-          int(fused is not None), table, rows, rot, int(neighbours), sms, _p(scratch), 4 * words, _stream()),
-        "quant_cache.decode")
+        words = scratch_words(B, nh, nkv, hd, sms)
+        scratch = _scratch_for(words, dev, stream)
+    rc = _function("quant_attention", "gf_quant_decode", (f"GF_HEAD_DIM={hd}",))(
+        _DECODE.pack(x, stride, code == 0, codes.data_ptr(), fp8, _at(scales, dev),
+                     _ints(block_table, (B, W), "block_table", dev), W, W, _ints(lengths, (B,), "lengths", dev), pages,
+                     out.data_ptr(), B, nh, nkv, page, span, fused is not None, table, rows, rot,
+                     fused is not None and fused[1], sms, 0 if scratch is None else scratch.data_ptr(), 4 * words,
+                     stream, scale))
+    _Counter.launches += 1 if scratch is None else 2
+    if rc:
+        _ok(rc, "quant_cache.decode" if fused is None else "quant_cache.step")
     return out
+
+
+def scratch_words(B: int, nh: int, nkv: int, hd: int, sms: int) -> int:
+    """32-bit words that the attention kernels are content with: two parts of an item a block (at most 8 blocks an
+    SM), a head's result with its maximum and sum, and two words an item (see ``csrc/quant_attention.cu``)."""
+    G = nh // nkv
+    chunks = (G + 15) // 16
+    rows = -(-G // chunks)
+    return sms * 8 * 2 * rows * (hd + 2) + 2 * B * nkv * chunks + 4
 
 
 def decode(q: torch.Tensor, nh: int, cache, block_table: torch.Tensor, lengths: torch.Tensor, scale: float,
@@ -189,8 +273,7 @@ def decode(q: torch.Tensor, nh: int, cache, block_table: torch.Tensor, lengths: 
 
 def step(qkv: torch.Tensor, nh: int, table, cache, block_table: torch.Tensor, lengths: torch.Tensor,
          scale: float, window: int = 0, *, neighbours: bool = False) -> torch.Tensor:
-    """What a decode step does to a layer's cache: row ``b`` of ``qkv [B, (nh + 2 kv heads) * head size]`` is
-    the last of request ``b``'s ``lengths[b]`` tokens; q and k are rotated, k and v written (as
+    """What a decode step does to a layer's cache, in one launch: row ``b`` of ``qkv [B, (nh + 2 kv heads) *
+    head size]`` is the last of request ``b``'s ``lengths[b]`` tokens; q and k are rotated, k and v written (as
     :func:`write` does), and the token attends over the cache, itself among the keys (as :func:`decode`)."""
-    facts = _cache(cache)
-    return _decode(qkv, nh, facts, block_table, lengths, scale, window, (*_angles(table, facts[6]), neighbours))
+    return _decode(qkv, nh, _cache(cache), block_table, lengths, scale, window, (table, neighbours))

@@ -67,7 +67,7 @@ constexpr int STAGES = GF_STAGES;
 constexpr int kLeastTiles = 4 * WARPS / TK;
 // Requests that see at most kShortKeys keys are one block's work a kv head; up to kMiddleKeys they are where that
 // gives the SMs enough blocks: the joining kernel costs 4 us, as much as 500 keys.
-constexpr int kShortKeys = 256, kMiddleKeys = 1024;
+constexpr int kShortKeys = 512, kMiddleKeys = 1024;
 constexpr int kMostBlocks = 8;          // of the blocks that fit an SM, so many are counted on
 
 struct DecodeArgs {
@@ -838,7 +838,7 @@ quant_decode_kernel(const DecodeArgs a) {
 // A block an item and `gridDim.y`-th of its heads: the pieces' results, weighted by their shares of the sum.
 // A team of HD / 4 threads takes a head where there are few pieces, else every TEAMS-th piece of every head:
 // its loads are then under way together, and the teams' sums are added in order.
-constexpr int JOIN_THREADS = 512, TEAM = HD / 4, TEAMS = JOIN_THREADS / TEAM, JOIN_AT_ONCE = 8, FEW_PIECES = 8;
+constexpr int TEAM = HD / 4, JOIN_AT_ONCE = 8, FEW_PIECES = 8;
 struct Joined {
   float4 o;
   float m, l;
@@ -851,8 +851,10 @@ struct Joined {
     l = mine * l + w, m = top;
   }
 };
+template <int JOIN_THREADS>
 __global__ void __launch_bounds__(JOIN_THREADS)
 quant_join_kernel(const DecodeArgs a) {
+  constexpr int TEAMS = JOIN_THREADS / TEAM;
   __shared__ float4 part[TEAMS][TEAM];
   __shared__ float2 part_ml[TEAMS];
   pdl_trigger();
@@ -958,9 +960,10 @@ int launch_decode(DecodeArgs a, int sms, void* scratch, size_t scratch_bytes, cu
   }
   const int e = launch_kernel(kernel, dim3((unsigned)blocks), dim3(THREADS), smem, stream, a);
   if (e || !a.stream) return e;
-  // few items: a block a head
-  const int split = items * a.rows <= 8LL * sms ? a.rows : 1;
-  return launch_kernel(quant_join_kernel, dim3((unsigned)items, split), dim3(JOIN_THREADS), 0, stream, a);
+  // few items (which have many parts): a block a head, with more teams
+  if (items * a.rows <= 8LL * sms)
+    return launch_kernel(quant_join_kernel<512>, dim3((unsigned)items, a.rows), dim3(512), 0, stream, a);
+  return launch_kernel(quant_join_kernel<256>, dim3((unsigned)items), dim3(256), 0, stream, a);
 }
 
 }  // namespace

@@ -207,7 +207,7 @@ def read_slots(cache, slots: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
 
 # Requests of at most this many visible tokens are one block's work a kv head and need no scratch (the kernel has the
 # same line: kShortKeys).
-_SHORT = 256
+_SHORT = 512
 _scratch: dict = {}
 _sms: dict = {}
 

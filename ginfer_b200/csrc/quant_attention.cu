@@ -225,6 +225,11 @@ template <bool WHOLE> struct Tiles {
     const int c0 = tile * TILE;
     const size_t values = (size_t)a.page * HD;
     const uint8_t* half[TK];
+    Place own = {nullptr, nullptr};               // of the lane's row (a row that is masked: one that is there)
+    if constexpr (!WHOLE) {
+      const int c = max(row_key(tile, lane & (TILE - 1)), 0);
+      own = place_of(a, kvh, page_number, c - logical_page(a, c) * a.page);
+    }
     if constexpr (WHOLE) {
 #pragma unroll
       for (int h = 0; h < TK; ++h) {
@@ -238,17 +243,12 @@ template <bool WHOLE> struct Tiles {
       const int idx = lane + 32 * i, row = idx / CH, ch = idx - row * CH;
       const bool used = TILE * CH % 32 == 0 || idx < TILE * CH;
       const bool there = c0 + row >= lo && c0 + row < end;
-      const uint8_t* src = a.codes;
-      if constexpr (WHOLE) {
-        src = (TK == 1 || row < 16 ? half[0] : half[TK - 1] - 16 * HD) + idx * 16;
-      } else {
-        const int pg = __shfl_sync(0xffffffffu, page_number, row & (TILE - 1));
-        const int c = row_key(tile, row);
-        if (there) src = place_of(a, kvh, pg, c - logical_page(a, c) * a.page).codes + ch * 16;
-      }
+      const uint8_t* src = nullptr;
+      if constexpr (WHOLE) src = (TK == 1 || row < 16 ? half[0] : half[TK - 1] - 16 * HD) + idx * 16;
+      else src = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, (unsigned long long)own.codes, row & (TILE - 1))) + ch * 16;
       if (used) {
         copy16(stage + row * ROW + ch * 16, src, there);
-        copy16(stage + (TILE + row) * ROW + ch * 16, there ? src + values : src, there);
+        copy16(stage + (TILE + row) * ROW + ch * 16, src + values, there);
       }
     }
     // the scales: pairs of keys; where a key's neighbour lies elsewhere, the 16 bytes that its own are in
@@ -259,9 +259,8 @@ template <bool WHOLE> struct Tiles {
         copy16(stage + SCALES_AT + lane * 16,
                place_of(a, kvh, pg, c - logical_page(a, c) * a.page).scales + 2 * (lane & 7), true);
     } else if (lane < TILE) {
-      const int c = row_key(tile, lane);
       const bool there = c0 + lane >= lo && c0 + lane < end;
-      const size_t at = there ? (size_t)place_of(a, kvh, page_number, c - logical_page(a, c) * a.page).scales : (size_t)a.codes;
+      const size_t at = (size_t)own.scales;
       const uint32_t odd = (uint32_t)at & 8u;
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(smem_u32(stage + SCALES_AT + lane * 16)),
                    "l"(at - odd), "r"(there ? (odd ? 16 : 8) : 0) : "memory");
@@ -346,6 +345,17 @@ struct Angles {
     }
   }
 };
+// Where they turn in halves of a whole head or with neighbours, a channel's partner is in the warp's registers.
+__device__ __forceinline__ bool partners_here(const DecodeArgs& a) {
+  return a.rot == 0 || (HD % 64 == 0 && a.rot == HD && !a.neighbours) || a.neighbours;
+}
+__device__ __forceinline__ void take_partners(const DecodeArgs& a, const float (&x)[N], float (&y)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float n = __shfl_xor_sync(0xffffffffu, x[i], 1);
+    y[i] = a.neighbours ? n : x[N % 2 ? i : i < N / 2 ? i + N / 2 : i - N / 2];
+  }
+}
 template <typename T>
 __device__ __forceinline__ void load_partners(const DecodeArgs& a, size_t at, bool there, int lane, float (&y)[N]) {
 #pragma unroll
@@ -420,7 +430,8 @@ quant_decode_kernel(const DecodeArgs a) {
   const auto head_of = [&](int hc) { return (hc / a.chunks) * G + (hc % a.chunks) * a.rows; };
   const auto rows_of = [&](int hc) { return min(a.rows, G - (hc % a.chunks) * a.rows); };
   // The block's next item that has tokens; the others get their zeros.
-  int ahead_len = 0;                       // the length of the request behind the cursor's, on its way
+  // lengths on their way: of the request that the cursor will be on after this item, and of the one behind that
+  int soon_b = -1, soon_len = 0, later_b = -1, later_len = 0;
   const auto next_item = [&](Item& it) {
     while (cur.todo > 0) {
       const int len = cur.len, t0 = first_tile(a, len), n = request_tiles(a, len);
@@ -455,6 +466,7 @@ quant_decode_kernel(const DecodeArgs a) {
   Item it, done;
   bool have = next_item(it), had = false;
   if (have) ask_pages(it);
+  if (cur.todo > 0) soon_b = cur.b, soon_len = request_length(a, cur.b);
   while (true) {
     // ---- an item's start: all that it waits for is asked for before anything is used
     const int kvh = it.hc / a.chunks, h0 = head_of(it.hc), nrows = rows_of(it.hc), p = it.len - 1;
@@ -471,15 +483,17 @@ quant_decode_kernel(const DecodeArgs a) {
         load_row<T>(a, row + (size_t)(h0 + warp + i * WARPS) * HD, warp + i * WARPS < nrows, lane, x[i]);
       if constexpr (STEP) {
         an.load(a, p, lane);
-#pragma unroll
-        for (int i = 0; i < RW; ++i)
-          load_partners<T>(a, row + (size_t)(h0 + warp + i * WARPS) * HD, warp + i * WARPS < nrows, lane, y[i]);
         const size_t new_at = row + (size_t)(a.nh + (keys ? 0 : a.nkv) + kvh) * HD;
-        load_row<T>(a, new_at, news, lane, nx);
-        load_partners<T>(a, new_at, news && keys, lane, ny);
+        if (news) load_row<T>(a, new_at, true, lane, nx);
+        if (!partners_here(a)) {
+#pragma unroll
+          for (int i = 0; i < RW; ++i)
+            load_partners<T>(a, row + (size_t)(h0 + warp + i * WARPS) * HD, warp + i * WARPS < nrows, lane, y[i]);
+          if (news && keys) load_partners<T>(a, new_at, true, lane, ny);
+        }
         if (news) new_page = page_in(a, fresh_index(tiles.tbl + logical_page(a, p)));
       }
-      if (cur.todo > 0) ahead_len = request_length(a, cur.b);
+      if (cur.todo > 0) later_b = cur.b + 1 == a.B ? 0 : cur.b + 1, later_len = request_length(a, later_b);
       // (of the new token nothing is read)
       int stage = at_stage;
 #pragma unroll
@@ -557,7 +571,10 @@ quant_decode_kernel(const DecodeArgs a) {
       // The block that has the item's last tile writes the new token (every chunk of heads the same bytes) and
       // keeps it for its own tile.
       if (news) {
-        if (keys) turn_row(a, an, lane, nx, ny);
+        if (keys) {
+          if (partners_here(a)) take_partners(a, nx, ny);
+          turn_row(a, an, lane, nx, ny);
+        }
         const RowScale rs = row_scale(row_top(nx), FP8);
         const Place pl = place_of(a, kvh, new_page, p - logical_page(a, p) * a.page);
         const int which = keys ? 0 : 1;
@@ -570,7 +587,10 @@ quant_decode_kernel(const DecodeArgs a) {
           reinterpret_cast<float*>(const_cast<float2*>(pl.scales))[which] = fresh_scale[which] = rs.scale;
       }
 #pragma unroll
-      for (int i = 0; i < RW; ++i) turn_row(a, an, lane, x[i], y[i]);
+      for (int i = 0; i < RW; ++i) {
+        if (partners_here(a)) take_partners(a, x[i], y[i]);
+        turn_row(a, an, lane, x[i], y[i]);
+      }
     }
     // q in halves, a row's largest element in [2^14, 2^15)
 #pragma unroll
@@ -627,8 +647,9 @@ quant_decode_kernel(const DecodeArgs a) {
     // ---- where the block goes next (its pages are there when this item's tiles are done)
     done = it, had = true;
     const int lo = it.lo, len = it.len, last = it.last, first = it.first;
-    cur.len = ahead_len;
+    if (cur.todo > 0) cur.len = soon_b == cur.b ? soon_len : request_length(a, cur.b);
     have = next_item(it);
+    soon_b = later_b, soon_len = later_len;
     if (have) ask_pages(it);
 
     // ---- the tiles

@@ -4,7 +4,8 @@ The reference allocates one tensor ``[2, L, num_blocks, block, nkv, hd]`` sized 
 (``ginfer/engine/model_runner.cc:52-87``).  Here caches with the same needs (what a token keeps,
 window) form a group with one tensor ``[caches, 2, num_pages, page, nkv, hd]``; a cache's K and V
 pages are ``tensor[i, 0]`` and ``tensor[i, 1]``.  A group whose spec names its own planes has one
-tensor ``[caches, num_pages, page, heads, width]`` per plane instead.  Mixers with state of fixed
+tensor ``[caches, num_pages, page, heads, width]`` per plane instead; a group kept in 8 bits has codes
+``[caches, num_pages, heads, 2, page, width]`` and scales ``[caches, num_pages, heads, page, 2]``.  Mixers with state of fixed
 size get a tensor ``[num_slots + 1, *shape]`` each: the last slot belongs to no request (the rows
 that pad a step up to a CUDA graph's batch size read and write there, as they do on the page
 that no request owns).
@@ -17,6 +18,8 @@ import torch
 
 from ..parts.base import PagedKVSpec, StateSpec
 
+EIGHT_BITS = {"int8": torch.int8, "fp8": torch.float8_e4m3fn}
+
 
 @dataclass(frozen=True)
 class GroupLayout:
@@ -25,8 +28,11 @@ class GroupLayout:
     window: int
     cache_ids: tuple[int, ...]
     chunk: int = 0                            # chunked mask: pages stay until the request ends
+    kept: str = ""                            # "int8", "fp8": codes and a 32-bit scale a (token, head) row
 
     def bytes_per_page(self, page_size: int, itemsize: int) -> int:
+        if self.kept:
+            return len(self.cache_ids) * page_size * sum(h * (w + 4) for h, w in self.planes)
         per_token = sum(h * w for h, w in self.planes)
         return len(self.cache_ids) * page_size * per_token * itemsize
 
@@ -48,8 +54,8 @@ def plan_groups(cache_specs: dict[int, object]) -> tuple[list[GroupLayout], dict
     for cid in sorted(cache_specs):
         s = cache_specs[cid]
         if isinstance(s, PagedKVSpec):
-            by_key.setdefault((s.layout(), s.planes is None, s.window, s.chunk), []).append(cid)
-    groups = [GroupLayout(k[0], k[1], k[2], tuple(v), k[3]) for k, v in by_key.items()]
+            by_key.setdefault((s.layout(), s.planes is None, s.window, s.chunk, s.kept), []).append(cid)
+    groups = [GroupLayout(k[0], k[1], k[2], tuple(v), k[3], k[4]) for k, v in by_key.items()]
     where = {cid: g for g, gl in enumerate(groups) for cid in gl.cache_ids}
     return groups, where
 
@@ -65,7 +71,14 @@ class CacheStorage:
         # rows that pad a step up to a CUDA graph's batch size write and read there
         self.kv = []
         for g, n in zip(groups, num_pages):
-            if g.stacked:
+            if g.kept:
+                heads, width = g.planes[0]
+                caches = len(g.cache_ids)
+                self.kv.append((torch.zeros((caches, n + 1, heads, 2, page_size, width), device=device,
+                                            dtype=EIGHT_BITS[g.kept]),
+                                torch.zeros((caches, n + 1, heads, page_size, 2), dtype=torch.float32,
+                                            device=device)))
+            elif g.stacked:
                 heads, width = g.planes[0]
                 self.kv.append(torch.zeros((len(g.cache_ids), 2, n + 1, page_size, heads, width),
                                            dtype=dtype, device=device))
@@ -90,7 +103,7 @@ class CacheStorage:
 
     def pages_of(self, cache_id: int):
         gi, i = self._where[cache_id]
-        if self.groups[gi].stacked:
+        if self.groups[gi].stacked and not self.groups[gi].kept:
             return self.kv[gi][i]
         return tuple(t[i] for t in self.kv[gi])
 

@@ -2,7 +2,8 @@
 (``ginfer/engine/config.h:8-21``): ``model_path``, ``max_num_batched_tokens``, ``max_num_seqs``,
 ``max_seq_len``, ``gpu_memory_utilization``, ``kvcache_block_size``.  Added here: the compute
 ``dtype``, an explicit page count (``num_kvcache_blocks``; tests use very few so that pages are
-used again) and ``enforce_eager`` (no CUDA-graph replay of decode steps).
+used again), ``enforce_eager`` (no CUDA-graph replay of decode steps) and ``kv_cache_dtype`` (keys
+and values in 8 bits, half or a quarter of the bytes: for models whose attention reads such a cache).
 """
 from __future__ import annotations
 
@@ -21,10 +22,13 @@ class EngineConfig:
     num_kvcache_blocks: int | None = None  # pages per layer group; None: from free memory
     enforce_eager: bool = False
     device: str = "cuda:0"
+    kv_cache_dtype: str = "auto"          # "auto" (that of the activations) | "int8" | "fp8" (e4m3)
 
     def validate(self) -> None:
         if self.dtype not in ("bfloat16", "float32"):
             raise ValueError(f"dtype must be 'bfloat16' or 'float32', got {self.dtype!r}")
+        if self.kv_cache_dtype not in ("auto", "int8", "fp8"):
+            raise ValueError(f"kv_cache_dtype must be 'auto', 'int8' or 'fp8', got {self.kv_cache_dtype!r}")
         for k in ("max_num_batched_tokens", "max_num_seqs", "max_seq_len", "kvcache_block_size"):
             if getattr(self, k) <= 0:
                 raise ValueError(f"{k} must be positive")

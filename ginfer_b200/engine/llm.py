@@ -61,15 +61,18 @@ class Engine:
                  max_seq_len: int = 4096, gpu_memory_utilization: float = 0.8,
                  kvcache_block_size: int = 16, num_kvcache_blocks: int | None = None,
                  enforce_eager: bool = False, device: str = "cuda:0", seed: int = 0,
-                 pipeline: bool = True, warmup: bool = True, capture_graphs: bool = False):
+                 pipeline: bool = True, warmup: bool = True, capture_graphs: bool = False,
+                 kv_cache_dtype: str = "auto"):
         """``model_path``: a folder with ``config.json`` and ``model.safetensors``; or give
         ``config`` (a ``config.json`` as a dict) and ``weights_seed`` for random weights.
         ``pipeline``: prepare each step on the host while the device runs the one before.
         ``warmup``: run one token through the model before the first request;
-        ``capture_graphs``: also capture the decode steps' CUDA graphs then, not on first use."""
+        ``capture_graphs``: also capture the decode steps' CUDA graphs then, not on first use.
+        ``kv_cache_dtype``: ``"int8"`` or ``"fp8"`` keep keys and values in 8 bits."""
         self.cfg = EngineConfig(model_path or "<random>", dtype, max_num_batched_tokens,
                                 max_num_seqs, max_seq_len, gpu_memory_utilization,
-                                kvcache_block_size, num_kvcache_blocks, enforce_eager, device)
+                                kvcache_block_size, num_kvcache_blocks, enforce_eager, device,
+                                kv_cache_dtype)
         self.cfg.validate()
         self._weights_from = (model_path, int(weights_seed))
         if model_path is not None:
@@ -82,7 +85,8 @@ class Engine:
             self.model, page_size=kvcache_block_size, max_num_seqs=max_num_seqs,
             max_seq_len=max_seq_len, num_pages=num_kvcache_blocks,
             gpu_memory_utilization=gpu_memory_utilization,
-            max_num_batched_tokens=max_num_batched_tokens, enforce_eager=enforce_eager)
+            max_num_batched_tokens=max_num_batched_tokens, enforce_eager=enforce_eager,
+            kv_cache_dtype=kv_cache_dtype)
         if warmup:
             self.runner.warmup(capture_graphs=capture_graphs)
         self.scheduler = Scheduler(self.runner.cache, max_num_seqs, max_num_batched_tokens,

@@ -62,7 +62,9 @@ class ModelRunner:
     def __init__(self, model: DecoderModel, *, page_size: int, max_num_seqs: int,
                  max_seq_len: int, num_pages: int | None = None,
                  gpu_memory_utilization: float = 0.8, max_num_batched_tokens: int = 8192,
-                 enforce_eager: bool = True):
+                 enforce_eager: bool = True, kv_cache_dtype: str = "auto"):
+        if kv_cache_dtype not in ("auto", "int8", "fp8"):
+            raise ValueError(f"kv_cache_dtype must be 'auto', 'int8' or 'fp8', got {kv_cache_dtype!r}")
         if model.device is None or model.device.type != "cuda":
             raise RuntimeError("the model must be loaded on a CUDA device before a runner is made")
         self.model = model
@@ -73,7 +75,8 @@ class ModelRunner:
         self.max_num_seqs = int(max_num_seqs)
         self.max_num_batched_tokens = int(max_num_batched_tokens)
         self.enforce_eager = bool(enforce_eager)
-        specs = model.cache_specs()
+        specs = model.cache_specs() if kv_cache_dtype == "auto" \
+            else model.cache_specs_in_8_bits(kv_cache_dtype)
         self.groups, self._group_of_cache = plan_groups(specs)
         itemsize = torch.empty((), dtype=self.dtype).element_size()
         counts = self._page_counts(num_pages, gpu_memory_utilization, itemsize)
@@ -287,7 +290,7 @@ class ModelRunner:
                 g = self.storage.group_of(cid)
                 return PagedKVBinding(self.storage.pages_of(cid), dev[f"block_table{g}"],
                                       dev[f"slot_mapping{g}"], self.page_size,
-                                      self.groups[g].window, write, self.groups[g].chunk)
+                                      self.groups[g].window, write, self.groups[g].chunk, self.groups[g].kept)
             if cid in self.storage.state:
                 return StateBinding(self.storage.state[cid], write)
             return None

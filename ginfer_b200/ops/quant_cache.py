@@ -277,3 +277,75 @@ def step(qkv: torch.Tensor, nh: int, table, cache, block_table: torch.Tensor, le
     head size]`` is the last of request ``b``'s ``lengths[b]`` tokens; q and k are rotated, k and v written (as
     :func:`write` does), and the token attends over the cache, itself among the keys (as :func:`decode`)."""
     return _decode(qkv, nh, _cache(cache), block_table, lengths, scale, window, (table, neighbours))
+
+
+# ----------------------------------------------------------------------------- a layer's attention
+# Tokens that a step's portions read back at a time: their requests are taken together while the longest of them times
+# their number stays below this (a dense copy of 32,768 tokens of 4 heads of 128 takes 67 MB).
+READ_AT_ONCE = 32768
+
+
+def portion_groups(pages_of: list[int], page: int) -> list[tuple[int, int]]:
+    """Runs ``[i, j)`` of neighbouring requests whose dense copies (``pages_of`` pages each) fit READ_AT_ONCE together;
+    a longer request is alone."""
+    groups, i = [], 0
+    while i < len(pages_of):
+        j, widest = i + 1, pages_of[i]
+        while j < len(pages_of) and (j + 1 - i) * max(widest, pages_of[j]) * page <= READ_AT_ONCE:
+            widest = max(widest, pages_of[j])
+            j += 1
+        groups.append((i, j))
+        i = j
+    return groups
+
+
+def attention(qkv: torch.Tensor, nh: int, table, cache, block_table: torch.Tensor, ctx, scale: float, span: int,
+              slots) -> torch.Tensor:
+    """A step's attention over a layer's cache: ``qkv [T, (nh + 2 kv heads) * head size]`` unrotated, ``slots [T]``
+    where the new keys and values go (``None``: they are not written, the cache is another layer's).  Single tokens
+    attend over the codes; prompt portions read what they see back (in the activations' type) and take the kernels of
+    an unquantised cache, so a portion sees the same keys and values as the tokens after it.  Returns ``[T, nh * head
+    size]``."""
+    from . import attention_bf16, paged_attention_simt
+    codes, page, hd = cache[0], cache[0].shape[3], cache[0].shape[4]
+    nkv = codes.shape[1]
+    if ctx.decode_only and slots is not None:
+        return step(qkv, nh, table, cache, block_table, ctx.kv_lens, scale, span)
+    q = write(qkv, nh, table, ctx.positions, torch.full_like(ctx.positions, -1) if slots is None else slots, cache)
+    if ctx.decode_only:
+        return decode(q, nh, cache, block_table, ctx.kv_lens, scale, span)
+    # single tokens first (as the scheduler orders them), the portions behind them
+    B, q_lens, nd = ctx.num_seqs, ctx.q_lens_host, 0
+    while nd < B and q_lens[nd] == 1:
+        nd += 1
+    out = torch.empty_like(q)
+    if nd:
+        out[:nd] = decode(q[:nd], nh, cache, block_table[:nd], ctx.kv_lens[:nd], scale, span)
+    cu, W = ctx.cu_seqlens_q, block_table.shape[1]
+    first = None
+    if span:
+        # the first key that each portion's first token sees
+        p = ctx.positions[cu[nd:B].long()]
+        first = (p - (span - 1)).clamp(min=0) if span > 0 else p // -span * -span
+    # (a captured step is replayed with other lengths: there every request may fill its table)
+    pages_of = [W if ctx.capturing else -(-(s + n) // page) for s, n in
+                zip(ctx.q_starts_host[nd:], q_lens[nd:])]
+    row = nd
+    for i, j in portion_groups(pages_of, page):
+        wide, n = max(pages_of[i:j]), j - i
+        b0, b1 = nd + i, nd + j
+        rows = sum(q_lens[b0:b1])
+        dense = read(cache, block_table[b0:b1, :wide].contiguous(), ctx.kv_lens[b0:b1], qkv.dtype,
+                     None if first is None else first[i:j])
+        pages = dense.view(2, n * wide, page, nkv, hd)
+        own = torch.arange(n * wide, dtype=_int32, device=q.device).view(n, wide)
+        if qkv.dtype is _float32:
+            out[row:row + rows] = paged_attention_simt(q[row:row + rows], pages, own, ctx.seq_of_token[row:row + rows] - b0,
+                                                       ctx.positions[row:row + rows], nh, nkv, hd, scale, span, page)
+        else:
+            args = (q, pages, own, cu[b0:b1 + 1], ctx.kv_lens[b0:b1], n, max(q_lens[b0:b1]), nh, nkv, hd, scale, span, page)
+            long = max(q_lens[b0:b1]) >= attention_bf16.TC_MIN_QUERY_ROWS
+            if not long or attention_bf16.prefill_tc(*args, out=out) is None:
+                attention_bf16.prefill(*args, out=out)
+        row += rows
+    return out

@@ -10,7 +10,8 @@ projection.  Scores: key ``c`` is visible to the query at position ``p`` iff ``c
 ``p - c < window``.
 
 Here q, k and v come from one product over joined weights; one kernel rotates q in place,
-rotates k into its page and copies v into its page; softmax statistics stay in fp32.
+rotates k into its page and copies v into its page; softmax statistics stay in fp32.  A cache kept
+in 8 bits takes the same q, k and v (``ops/quant_cache.py``).
 """
 from __future__ import annotations
 
@@ -26,6 +27,7 @@ from .plan import PartSpec
 class Attention(Mixer):
     takes_lazy_norm = True        # the joined q/k/v product normalises its own operand
     adds_residual = True          # the output product adds the residual and leaves statistics
+    reads_8_bits = True
 
     def __init__(self, hidden_size: int, num_heads: int, num_kv_heads: int, head_dim: int,
                  position: PartSpec, window: int = 0, qkv_bias: bool = True,
@@ -83,7 +85,7 @@ class Attention(Mixer):
     def forward(self, x, ctx, cache, residual=None, then=None):
         nh, nkv, hd = self.num_heads, self.num_kv_heads, self.head_dim
         fused = self.position.rotary_table()
-        if fused is not None and cache.write and not hasattr(x, "materialize"):
+        if not cache.kept and fused is not None and cache.write and not hasattr(x, "materialize"):
             # many tokens: one kernel multiplies, adds the bias, rotates q and k and writes the cache
             qkv = ops.qkv_rope_write(x, self.qkv, fused[0], fused[1], ctx.positions,
                                      cache.slot_mapping, cache.pages, nh, nkv, hd)
@@ -99,6 +101,10 @@ class Attention(Mixer):
             table, rot = None, 0
         else:
             table, rot = fused
+        if cache.kept:
+            o = ops.quant_cache.attention(qkv, nh, table, cache.pages, cache.block_table, ctx, self.scale,
+                                          cache.window, cache.slot_mapping if cache.write else None)
+            return self._project(o, residual, then)
         if fused is not None and ops.attention_fuses_rope(qkv, ctx, nh, nkv, hd):
             # decode steps: the attention kernel rotates q and k and writes the cache itself
             o = ops.paged_attention(qkv, cache.pages, cache.block_table, ctx, nh, nkv, hd,

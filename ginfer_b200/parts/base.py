@@ -57,6 +57,9 @@ class PagedKVSpec:
     window: int = 0
     planes: tuple[tuple[int, int], ...] | None = None
     chunk: int = 0        # > 0: a query sees only the keys of its own chunk of this many positions
+    # "int8" or "fp8": keys and values as 8-bit codes with a scale a row (``ops.quant_cache``); set by the runner for
+    # mixers that say ``reads_8_bits``
+    kept: str = ""
 
     def layout(self) -> tuple[tuple[int, int], ...]:
         return self.planes or ((self.num_kv_heads, self.head_dim),) * 2
@@ -72,7 +75,8 @@ class StateSpec:
 @dataclass
 class PagedKVBinding:
     # [2, num_pages, page_size, num_kv_heads, head_dim] (0 = K, 1 = V); for a spec with ``planes``
-    # a tuple of tensors [num_pages, page_size, heads, width], one per plane
+    # a tuple of tensors [num_pages, page_size, heads, width], one per plane; for one with ``kept`` the pair
+    # (codes, scales) of ``ops.quant_cache``
     pages: torch.Tensor | tuple
     block_table: torch.Tensor    # [B, W] int32, logical page -> physical page, -1 where none
     slot_mapping: torch.Tensor   # [T] int32, physical token slot (page * page_size + offset)
@@ -80,6 +84,7 @@ class PagedKVBinding:
     window: int
     write: bool
     chunk: int = 0
+    kept: str = ""
 
 
 @dataclass
@@ -268,6 +273,8 @@ class Mixer(Part):
     # instead of its output, with ``scaled`` made for the norm ``then`` (the one that follows).
     takes_lazy_norm = False
     adds_residual = False
+    # A mixer that sets this works on a cache whose binding says ``kept`` (8-bit codes and scales).
+    reads_8_bits = False
 
     def cache_spec(self) -> PagedKVSpec | StateSpec | tuple | None:
         """What the mixer keeps; a tuple for a mixer made of several, which then gets a tuple of

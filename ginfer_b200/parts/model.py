@@ -7,9 +7,11 @@ is computed only at the rows whose logits are wanted.
 """
 from __future__ import annotations
 
+from dataclasses import replace
+
 import torch
 
-from .base import MixedInput, StepContext, Summed, TensorSpec, make_part
+from .base import MixedInput, PagedKVSpec, StepContext, Summed, TensorSpec, make_part
 from .plan import ModelPlan
 
 
@@ -106,6 +108,25 @@ class DecoderModel:
                         raise ValueError(f"layer {e.layer} cannot read cache {c}: it holds "
                                          f"{out[c]} but the layer expects {mine}")
         return out
+
+    def cache_specs_in_8_bits(self, kind: str) -> dict[int, object]:
+        """:meth:`cache_specs` with keys and values kept as 8-bit codes (``kind`` ``"int8"`` or ``"fp8"``); a model
+        one of whose mixers keeps pages that it cannot read that way is refused."""
+        from ..ops import quant_cache
+        specs = self.cache_specs()
+        for e in self.plan.run:
+            mixer = self.blocks[e.layer].mixer
+            for c in e.caches():
+                spec = specs.get(c)
+                if not isinstance(spec, PagedKVSpec):
+                    continue
+                if not mixer.reads_8_bits or spec.planes is not None:
+                    raise ValueError(f"layer {e.layer} ({type(mixer).__name__}) does not read a cache of 8 bits")
+                if not quant_cache.supports(spec.head_dim, spec.num_kv_heads, spec.num_kv_heads):
+                    raise ValueError(f"a cache of 8 bits takes head sizes that are a multiple of 16, at most "
+                                     f"{quant_cache.MAX_HEAD_DIM}; layer {e.layer} has {spec.head_dim}")
+                specs[c] = replace(spec, kept=kind)
+        return specs
 
     def _next_input(self, blk, entry, own_state):
         """What ``blk`` may prepare for ``entry``'s run behind it: nothing where that run's block needs

@@ -26,7 +26,7 @@ namespace gf {
 // one by one.
 constexpr int WRITE_THREADS = 128;
 template <typename T, int LANES, int HU>
-__global__ void __launch_bounds__(WRITE_THREADS)
+__global__ void __launch_bounds__(WRITE_THREADS, 8)
 quant_write_kernel(const T* __restrict__ qkv, int row_stride, int tokens, int nh, int nkv, int hd,
                    const float* __restrict__ table, int table_rows, int rot, int neighbours,
                    const int* __restrict__ positions, const int* __restrict__ slots, T* __restrict__ q_out,
@@ -140,7 +140,7 @@ int launch_write(const void* qkv, int row_stride, int tokens, int nh, int nkv, i
                  cudaStream_t stream) {
   const int heads = nh + 2 * nkv;
   const bool one = (long long)tokens * heads * LANES <= 148 * 1024;
-  const int hu = one ? 1 : 4, sets = (heads + hu - 1) / hu, each = WRITE_THREADS / LANES;
+  const int hu = one ? 1 : 2, sets = (heads + hu - 1) / hu, each = WRITE_THREADS / LANES;
   if (sets > 65535) return -5;
   const dim3 grid((unsigned)((tokens + each - 1) / each), (unsigned)sets);
   const auto run = [&](auto kernel) {
@@ -148,7 +148,7 @@ int launch_write(const void* qkv, int row_stride, int tokens, int nh, int nkv, i
                          tokens, nh, nkv, hd, table, table_rows, rot, neighbours, positions, slots, (T*)q_out,
                          codes, fp8, scales, page, num_slots, vec);
   };
-  return one ? run(quant_write_kernel<T, LANES, 1>) : run(quant_write_kernel<T, LANES, 4>);
+  return one ? run(quant_write_kernel<T, LANES, 1>) : run(quant_write_kernel<T, LANES, 2>);
 }
 
 // -------------------------------------------------------------------------------------- read

@@ -33,6 +33,7 @@ _FP8 = {torch.int8: 0, torch.float8_e4m3fn: 1}
 _CODE = {torch.float32: 0, torch.bfloat16: 1}
 _WRITE, _READ, _DECODE = struct.Struct("=20q"), struct.Struct("=17q"), struct.Struct("=26qd")
 _current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+_capturing = torch.cuda.is_current_stream_capturing
 _int32, _float32 = torch.int32, torch.float32
 
 
@@ -159,7 +160,7 @@ def write(qkv: torch.Tensor, nh: int, table, positions: torch.Tensor, slots: tor
     x, stride, code = _rows(qkv, (nh + 2 * nkv) * hd, "qkv", dev)
     T = qkv.shape[0]
     at, rows, rot = _angles(table, hd, dev)
-    q = torch.empty((T, nh * hd), dtype=qkv.dtype, device=qkv.device)
+    q = qkv.new_empty(T, nh * hd)
     f = _function("quant_cache", "gf_quant_write")
     rc = f(_WRITE.pack(x, stride, code, T, nh, nkv, hd, at, rows, rot, neighbours,
                        _ints(positions, (T,), "positions", dev), _ints(slots, (T,), "slots", dev), q.data_ptr(),
@@ -172,7 +173,8 @@ def write(qkv: torch.Tensor, nh: int, table, positions: torch.Tensor, slots: tor
 
 def _read(facts, block_table, W, lengths, first, slots, B, S, dtype, dev):
     codes, scales, fp8, pages, nkv, page, hd = facts
-    out = torch.empty((2, B, S, nkv, hd) if slots == 0 else (2, S, nkv, hd), dtype=dtype, device=codes.device)
+    shape = (2, B, S, nkv, hd) if slots == 0 else (2, S, nkv, hd)
+    out = scales.new_empty(*shape) if dtype is _float32 else scales.new_empty(shape, dtype=dtype)
     rc = _function("quant_cache", "gf_quant_read")(
         _READ.pack(codes.data_ptr(), fp8, _at(scales, dev), block_table, W, lengths, first, slots, pages, B, S,
                    nkv, hd, page, out.data_ptr(), _code(dtype), _raw_stream(dev)))
@@ -214,7 +216,7 @@ _sms: dict = {}
 
 def _scratch_for(words: int, device: int, stream: int) -> torch.Tensor:
     """A buffer that only this stream's calls use; a graph that is being captured keeps one of its own."""
-    if torch.cuda.is_current_stream_capturing():
+    if _capturing():
         return torch.empty(words, dtype=torch.float32, device=device)
     buf = _scratch.get((device, stream))
     if buf is None or buf.numel() < words:
@@ -232,7 +234,7 @@ def _decode(q, nh, facts, block_table, lengths, scale, span, fused=None):
     if q.shape[0] != B:
         raise ValueError(f"{q.shape[0]} queries for {B} requests")
     table, rows, rot = (0, 0, 0) if fused is None else _angles(fused[0], hd, dev)
-    out = torch.empty((B, nh * hd), dtype=q.dtype, device=q.device)
+    out = q.new_empty(B, nh * hd)
     sms = _sms.get(dev)
     if sms is None:
         sms = _sms[dev] = num_sms(dev)

@@ -22,16 +22,17 @@ namespace gf {
 // A head's row is held by hd / 16 lanes of two times eight channels each, such that a lane's channels turn with
 // each other: 8 l .. and half + 8 l .. where halves turn (what does not turn follows in runs of 16), 16 l .. where
 // neighbours do.  A group of lanes takes HU heads of one token: their loads are under way together, and the angles
-// of the token's position are read once for them.  Halves that are no multiple of eight take the angles and partners
-// one by one.
+// of the token's position are read once for them.
 constexpr int WRITE_THREADS = 128;
-template <typename T, int LANES, int HU>
-__global__ void __launch_bounds__(WRITE_THREADS, 8)
+// REGULAR: neighbours, or halves that are a multiple of eight.
+template <typename T, int LANES, int HU, bool REGULAR>
+__global__ void __launch_bounds__(WRITE_THREADS, REGULAR ? 8 : 6)
 quant_write_kernel(const T* __restrict__ qkv, int row_stride, int tokens, int nh, int nkv, int hd,
                    const float* __restrict__ table, int table_rows, int rot, int neighbours,
                    const int* __restrict__ positions, const int* __restrict__ slots, T* __restrict__ q_out,
                    uint8_t* __restrict__ codes, int fp8, float* __restrict__ scales, int page, int num_slots,
                    int vec) {
+  __shared__ float staged[REGULAR ? 1 : WRITE_THREADS * 17];
   pdl_trigger();
   pdl_wait();
   const int heads = nh + 2 * nkv;
@@ -40,7 +41,7 @@ quant_write_kernel(const T* __restrict__ qkv, int row_stride, int tokens, int nh
   const int t = blockIdx.x * (WRITE_THREADS / LANES) + threadIdx.x / LANES, h0 = blockIdx.y * HU;
   const bool here = t < tokens && lane * 16 < hd;
   const int half = rot >> 1;
-  const bool plain = !neighbours && (half & 7) == 0;
+  const bool plain = REGULAR && !neighbours;
   const bool turns = lane * 16 < rot;              // (all of a lane's channels, or with neighbours some)
   const int ca = plain && turns ? lane * 8 : lane * 16, cb = plain && turns ? half + lane * 8 : lane * 16 + 8;
   const T* row = qkv + (size_t)(here ? t : 0) * row_stride;
@@ -59,10 +60,9 @@ quant_write_kernel(const T* __restrict__ qkv, int row_stride, int tokens, int nh
   const float* cs = table;
   float c[8], s[8];
   const int j0 = lane * 8;                         // the first of the lane's eight pairs
-  const bool regular = neighbours || plain;
   if (here && rot > 0 && h0 < nh + nkv) {
     cs += (size_t)min(max(fresh_index(positions + t), 0), table_rows - 1) * rot;
-    if (turns && (half & 7) == 0 && (vec & 2)) {
+    if (REGULAR && turns && (half & 7) == 0 && (vec & 2)) {
 #pragma unroll
       for (int e = 0; e < 8; e += 4) {             // (a row of the table is a multiple of 64 bytes)
         const float4 cv = __ldg(reinterpret_cast<const float4*>(cs + j0 + e));
@@ -70,7 +70,7 @@ quant_write_kernel(const T* __restrict__ qkv, int row_stride, int tokens, int nh
         c[e] = cv.x, c[e + 1] = cv.y, c[e + 2] = cv.z, c[e + 3] = cv.w;
         s[e] = sv.x, s[e + 1] = sv.y, s[e + 2] = sv.z, s[e + 3] = sv.w;
       }
-    } else if (turns && regular) {
+    } else if (REGULAR && turns) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int j = min(j0 + e, half - 1);
@@ -86,11 +86,11 @@ quant_write_kernel(const T* __restrict__ qkv, int row_stride, int tokens, int nh
 #pragma unroll
     for (int e = 0; e < 8; ++e) lo[e] = hi[e] = 0.f;
     if (here) ra[i].get(lo), rb[i].get(hi);
-    if (here && turns && h < nh + nkv) {
+    if (REGULAR && here && turns && h < nh + nkv) {
       if (plain) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) turn_pair(lo[e], hi[e], c[e], s[e]);
-      } else if (neighbours) {
+      } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           if (j0 + e < half) turn_pair(lo[2 * e], lo[2 * e + 1], c[e], s[e]);
@@ -98,17 +98,25 @@ quant_write_kernel(const T* __restrict__ qkv, int row_stride, int tokens, int nh
         }
       }
     }
-    if (here && !regular && h < nh + nkv && lane * 16 < rot) {
+    if (!REGULAR && h < nh + nkv) {                // (halves that are no multiple of eight: partners through shared memory)
+      float* mine = staged + threadIdx.x * 17;
+      const float* first = staged + (threadIdx.x - lane) * 17;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int ch = lane * 16 + e;
-        float& own = e < 8 ? lo[e & 7] : hi[e & 7];
-        if (ch >= rot) continue;
-        const int j = ch < half ? ch : ch - half;
-        const float o = fresh(row + (size_t)h * hd + (ch < half ? ch + half : j));
-        own = ch < half ? turned_first(own, o, __ldg(cs + j), __ldg(cs + half + j))
-                        : turned_second(o, own, __ldg(cs + j), __ldg(cs + half + j));
+      for (int e = 0; e < 8; ++e) mine[e] = lo[e], mine[8 + e] = hi[e];
+      __syncwarp(mask);
+      if (here) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int ch = lane * 16 + e;
+          float& own = e < 8 ? lo[e & 7] : hi[e & 7];
+          if (ch >= rot) continue;
+          const int j = ch < half ? ch : ch - half, other = ch < half ? ch + half : j;
+          const float o = first[(other >> 4) * 17 + (other & 15)];
+          own = ch < half ? turned_first(own, o, __ldg(cs + j), __ldg(cs + half + j))
+                          : turned_second(o, own, __ldg(cs + j), __ldg(cs + half + j));
+        }
       }
+      __syncwarp(mask);
     }
     if (h < nh) {
       if (here) {
@@ -148,7 +156,9 @@ int launch_write(const void* qkv, int row_stride, int tokens, int nh, int nkv, i
                          tokens, nh, nkv, hd, table, table_rows, rot, neighbours, positions, slots, (T*)q_out,
                          codes, fp8, scales, page, num_slots, vec);
   };
-  return one ? run(quant_write_kernel<T, LANES, 1>) : run(quant_write_kernel<T, LANES, 2>);
+  if (neighbours || rot % 16 == 0)
+    return one ? run(quant_write_kernel<T, LANES, 1, true>) : run(quant_write_kernel<T, LANES, 2, true>);
+  return one ? run(quant_write_kernel<T, LANES, 1, false>) : run(quant_write_kernel<T, LANES, 2, false>);
 }
 
 // -------------------------------------------------------------------------------------- read

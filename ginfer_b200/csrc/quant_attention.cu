@@ -32,6 +32,7 @@
 #include <type_traits>
 
 #include "quant.cuh"
+#include "tc_common.cuh"
 
 #ifndef GF_HEAD_DIM
 #define GF_HEAD_DIM 128
@@ -52,17 +53,32 @@ constexpr int VW = HD % 128 == 0 ? 16 : HD % 64 == 0 ? 8 : HD % 32 == 0 ? 4 : 2;
 constexpr int KWORDS = HD / 16;                                  // words of a key a thread holds
 constexpr int MT = HD / 16;                                      // row tiles of O^T
 constexpr int CH = HD / 16;                                      // 16-byte chunks of a row
-// Rows in shared memory are 16 bytes apart in banks: a quarter warp's reads of keys (two rows, four
-// places of 16 bytes) and of values (four rows, two places) then hit every bank once.
-constexpr int ROW = HD + 16;
-constexpr int SCALES_AT = 2 * TILE * ROW, STAGE = SCALES_AT + TILE * 16 + TILE;
-#ifndef GF_STAGES
-#define GF_STAGES 3
-#endif
-#ifndef GF_OCC
-#define GF_OCC 3
-#endif
-constexpr int STAGES = GF_STAGES;
+// A tile in shared memory.  Head sizes that are a multiple of 64 lie as TMA's swizzle leaves them: rows of SW bytes
+// (a wider head is several such tiles), the 16-byte chunks of eight neighbouring rows in turn, so that a quarter
+// warp's reads of keys (two rows, four chunks) and of values (four rows, two chunks) hit every bank once (half the
+// values of a head of 64: twice).  Others lie in rows 16 bytes apart in banks.
+constexpr bool SWIZZLED = HD % 64 == 0;
+constexpr int SW = HD % 128 == 0 ? 128 : 64, SUBS = SWIZZLED ? HD / SW : 1, ROW = HD + 16;
+constexpr int STAGE = SWIZZLED ? 2 * TILE * HD : 2 * TILE * ROW;
+constexpr int SCALES = TILE * 16 + TILE;                         // bytes of a stage's scales
+// Keys of a unit (8 or 16 neighbours in a page) are followed by their values: what one TMA copy brings.
+struct Layout {
+  int eight, values;          // from a row to the one eight behind, from a key to its value
+  __device__ __forceinline__ int at(int which, int r, int chunk) const {
+    if constexpr (SWIZZLED) {
+      const int sub = chunk / (SW / 16), c = chunk % (SW / 16), turn = SW == 128 ? r & 7 : (r >> 1) & 3;
+      return sub * (2 * TILE * SW) + (r >> 4) * (32 * SW) + ((r >> 3) & 1) * eight + which * values + (r & 7) * SW +
+             ((c ^ turn) << 4);
+    } else {
+      return (which * TILE + r) * ROW + chunk * 16;
+    }
+  }
+};
+constexpr int STAGES = 2;
+// Blocks an SM: as many as their registers allow without spilling to memory in a tile's work.
+constexpr int blocks_an_sm(int nt, int type_bytes) {
+  return nt == 1 ? (HD <= 128 && type_bytes == 2 ? 4 : 3) : (HD <= 128 ? 3 : 2);
+}
 // the fewest tiles of a block's run
 constexpr int kLeastTiles = 4 * WARPS / TK;
 // Requests that see at most kShortKeys keys are one block's work a kv head; up to kMiddleKeys they are where that
@@ -82,6 +98,8 @@ struct DecodeArgs {
   void* out;
   int out_f32, B, nh, nkv, page, page_shift, span;
   float scale;
+  int unit;                   // keys of a TMA copy
+  int* err;
   int chunks, rows;           // a kv head's query heads in `chunks` blocks of up to `rows`
   int stream;                 // blocks share the tiles evenly (see Cursor), else a block an item
   int2* info;                 // [heads * B], stream: the block an item starts in, how many it is spread over
@@ -209,71 +227,101 @@ __device__ __forceinline__ int page_in(const DecodeArgs& a, int number) {
 __device__ __forceinline__ int logical_page(const DecodeArgs& a, int c) {
   return a.page_shift >= 0 ? c >> a.page_shift : c / a.page;
 }
-// A warp's view of an item's tiles.  A lane knows the page of a tile's row `lane`: where pages are a multiple of 16
-// (WHOLE) lanes 0 .. 15 know the first 16 rows', the others the next 16 rows'.  Rows outside [lo, end) are zeros
-// and nothing of them is read.
-template <bool WHOLE> struct Tiles {
+// A warp's view of an item's tiles.
+// TMA: pages are a multiple of 8 (unit 8) or 16 (unit 16); a unit comes by one copy of keys and values (for each SW
+// bytes of a head) and one of scales, and counts on the stage's barrier.  Lane u knows unit u's page.  Rows that are
+// masked come too, and are cleared where they matter (clear_masked).
+// Else: lane r knows row r's page, cp.async brings 16 bytes a lane, rows outside [lo, end) are zeros and nothing of
+// them is read.
+template <bool TMA> struct Tiles {
   const DecodeArgs& a;
   const int* tbl;
   int kvh, lo, end, last, lane;
+  Layout lay;
   __device__ __forceinline__ int row_key(int tile, int r) const { return min(max(tile * TILE + r, lo), end - 1); }
   __device__ __forceinline__ int page_of(int tile) const {
     if (tile >= last || lo >= end) return 0;
-    return page_in(a, fresh_index(tbl + logical_page(a, row_key(tile, WHOLE ? lane & (TILE - 16) : lane & (TILE - 1)))));
+    return page_in(a, fresh_index(tbl + logical_page(a, row_key(tile, TMA ? (lane * a.unit) & (TILE - 1) : lane & (TILE - 1)))));
   }
-  __device__ __forceinline__ void copy(uint8_t* stage, int tile, int page_number) const {
+  __device__ __forceinline__ void copy(const CUtensorMap* map, uint64_t* bar, uint8_t* stage, uint8_t* scales, int tile,
+                                       int page_number) const {
     const int c0 = tile * TILE;
-    const size_t values = (size_t)a.page * HD;
-    const uint8_t* half[TK];
-    Place own = {nullptr, nullptr};               // of the lane's row (a row that is masked: one that is there)
-    if constexpr (!WHOLE) {
-      const int c = max(row_key(tile, lane & (TILE - 1)), 0);
-      own = place_of(a, kvh, page_number, c - logical_page(a, c) * a.page);
-    }
-    if constexpr (WHOLE) {
+    if constexpr (TMA) {
+      const int c = c0 + lane * a.unit;
+      const bool mine = lane * a.unit < TILE && c < end && c + a.unit > lo;
+      const int units = __popc(__ballot_sync(0xffffffffu, mine));
+      if (lane == 0) mbar_expect_tx(bar, units * a.unit * (2 * HD + 8));
+      __syncwarp();
+      if (mine) {
+        const int off = c - logical_page(a, c) * a.page;
 #pragma unroll
-      for (int h = 0; h < TK; ++h) {
-        const int c = c0 + 16 * h;
-        half[h] = place_of(a, kvh, TK == 1 ? page_number : __shfl_sync(0xffffffffu, page_number, 16 * h),
-                           c - logical_page(a, c) * a.page).codes;
+        for (int sub = 0; sub < SUBS; ++sub)
+          asm volatile(
+              "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+              "[%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(stage + sub * (2 * TILE * SW) + lane * a.unit * 2 * SW)),
+              "l"(map), "r"(smem_u32(bar)), "r"(sub * SW), "r"(off), "r"(2 * kvh), "r"(page_number)
+              : "memory");
+        const float2* from = place_of(a, kvh, page_number, off).scales;
+        asm volatile(
+            "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                smem_u32(scales + lane * a.unit * 8)),
+            "l"(from), "r"(a.unit * 8), "r"(smem_u32(bar))
+            : "memory");
       }
-    }
+    } else {
+      const size_t values = (size_t)a.page * HD;
+      const int c = max(row_key(tile, lane & (TILE - 1)), 0);      // (a row that is masked: one that is there)
+      const Place own = place_of(a, kvh, page_number, c - logical_page(a, c) * a.page);
 #pragma unroll
-    for (int i = 0; i < (TILE * CH + 31) / 32; ++i) {
-      const int idx = lane + 32 * i, row = idx / CH, ch = idx - row * CH;
-      const bool used = TILE * CH % 32 == 0 || idx < TILE * CH;
-      const bool there = c0 + row >= lo && c0 + row < end;
-      const uint8_t* src = nullptr;
-      if constexpr (WHOLE) src = (TK == 1 || row < 16 ? half[0] : half[TK - 1] - 16 * HD) + idx * 16;
-      else src = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, (unsigned long long)own.codes, row & (TILE - 1))) + ch * 16;
-      if (used) {
-        copy16(stage + row * ROW + ch * 16, src, there);
-        copy16(stage + (TILE + row) * ROW + ch * 16, src + values, there);
+      for (int i = 0; i < (TILE * CH + 31) / 32; ++i) {
+        const int idx = lane + 32 * i, row = idx / CH, ch = idx - row * CH;
+        const bool there = c0 + row >= lo && c0 + row < end;
+        const uint8_t* src =
+            reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, (unsigned long long)own.codes, row & (TILE - 1))) + ch * 16;
+        if (TILE * CH % 32 == 0 || idx < TILE * CH) {
+          copy16(stage + lay.at(0, row, ch), src, there);
+          copy16(stage + lay.at(1, row, ch), src + values, there);
+        }
       }
-    }
-    // the scales: pairs of keys; where a key's neighbour lies elsewhere, the 16 bytes that its own are in
-    if constexpr (WHOLE) {
-      const int h = lane / 8, c = c0 + 16 * h;
-      const int pg = TK == 1 ? page_number : __shfl_sync(0xffffffffu, page_number, (16 * h) & 31);
-      if (lane < TILE / 2)
-        copy16(stage + SCALES_AT + lane * 16,
-               place_of(a, kvh, pg, c - logical_page(a, c) * a.page).scales + 2 * (lane & 7), true);
-    } else if (lane < TILE) {
-      const bool there = c0 + lane >= lo && c0 + lane < end;
-      const size_t at = (size_t)own.scales;
-      const uint32_t odd = (uint32_t)at & 8u;
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(smem_u32(stage + SCALES_AT + lane * 16)),
-                   "l"(at - odd), "r"(there ? (odd ? 16 : 8) : 0) : "memory");
-      stage[SCALES_AT + TILE * 16 + lane] = (uint8_t)odd;
+      // the scales: the 16 bytes that a key's own are in
+      if (lane < TILE) {
+        const bool there = c0 + lane >= lo && c0 + lane < end;
+        const size_t at = (size_t)own.scales;
+        const uint32_t odd = (uint32_t)at & 8u;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(smem_u32(scales + lane * 16)),
+                     "l"(at - odd), "r"(there ? (odd ? 16 : 8) : 0) : "memory");
+        scales[TILE * 16 + lane] = (uint8_t)odd;
+      }
     }
   }
   // The (key, value) scales of key r of a tile.
-  __device__ __forceinline__ float2 scales(const uint8_t* stage, int r) const {
-    const uint8_t* at = stage + SCALES_AT;
-    return *reinterpret_cast<const float2*>(WHOLE ? at + r * 8 : at + r * 16 + at[TILE * 16 + r]);
+  __device__ __forceinline__ float2 scales(const uint8_t* at, int r) const {
+    return *reinterpret_cast<const float2*>(TMA ? at + r * 8 : at + r * 16 + at[TILE * 16 + r]);
+  }
+  // Masked values count as nothing, whatever lies there (their weight is zero, but zero times no number is none).
+  __device__ __forceinline__ void clear_masked(uint8_t* stage, int tile, int len) const {
+    if constexpr (TMA) {
+      for (int i = lane; i < TILE * CH; i += 32) {
+        const int row = i / CH, c = tile * TILE + row;
+        if (c < lo || c >= len) *reinterpret_cast<uint4*>(stage + lay.at(1, row, i - row * CH)) = make_uint4(0u, 0u, 0u, 0u);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // (the stage's next copy comes behind this)
+      __syncwarp();
+    }
   }
 };
 
+// The channel that a key's word w of the thread's places t stands for: a quarter of every SW bytes, four a word.
+__device__ __forceinline__ constexpr int key_channel(int t, int w) {
+  constexpr int SPAN = SWIZZLED ? SW : HD, WORDS = SPAN / 16;
+  return w / WORDS * SPAN + t * (SPAN / 4) + w % WORDS * 4;
+}
+// Where channel c of head r stands in a block's q (see quant_decode_kernel).
+__device__ __forceinline__ int q_place(int r, int c) {
+  constexpr int SPAN = SWIZZLED ? SW : HD, WORDS = SPAN / 16;
+  const int in = c % SPAN, t = in / (SPAN / 4), w = c / SPAN * WORDS + in % (SPAN / 4) / 4;
+  return (((r >> 3) * KWORDS + w) * 32 + (r & 7) * 4 + t) * 4 + (c & 3);
+}
 // Two codes plus 128 (the bytes 2i, 2i + 1 of a word) as the halves 2^-24 (code + 128), below the smallest normal one:
 // a byte permutation, no arithmetic.
 __device__ __forceinline__ uint32_t raised_halves(uint32_t w, int i) {
@@ -383,29 +431,49 @@ __device__ __forceinline__ uint32_t row_top(const float (&x)[N]) {
 }
 
 // ------------------------------------------------------------------------------------- a block's run
+// Floats from a head's result to the next one's in shared memory: two rows in other banks, where a warp's results then
+// still fit a stage or the head is short enough for room of their own.
+__host__ __device__ constexpr int result_row(int nt) { return HD > 128 && 8 * nt * HD * 4 <= STAGE ? HD : HD + 2; }
 struct Item {
   int b, hc, len, lo, first, last;         // its tiles here
   bool starts, ends;                       // whether they are its first, its last
 };
+// What a block goes on with behind an item's tiles.
+struct Kept {
+  Item next, done;
+  Cursor cur;
+  int soon_b, soon_len;
+};
 // NT: tiles of 8 query heads.  T: the type of q and the result (32-bit ones take two halves each).  STEP: q | k | v
 // rows, unrotated.
-template <int NT, bool FP8, typename T, bool WHOLE, bool STEP>
-__global__ void __launch_bounds__(THREADS, (NT == 1 && HD <= 128 && sizeof(T) == 2) ? GF_OCC : 2)
-quant_decode_kernel(const DecodeArgs a) {
+template <int NT, bool FP8, typename T, bool TMA, bool STEP>
+__global__ void __launch_bounds__(THREADS, blocks_an_sm(NT, sizeof(T)))
+quant_decode_kernel(const DecodeArgs a, const __grid_constant__ CUtensorMap map) {
   constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;
   constexpr int R = 8 * NT, RW = R / WARPS;                      // rows of q in all, and a warp
   constexpr bool RAISED = !FP8 && PARTS == 1;                    // K's codes as halves of code + 128
-  constexpr int OROW = HD + 2;                                   // (floats: two rows apart, other banks)
-  // [WARPS][STAGES][keys | values][TILE][ROW]; a warp's results at an item's end go into its stage that is not under
+  constexpr int OROW = result_row(NT);
+  // [WARPS][STAGES][STAGE], [WARPS][STAGES][SCALES]; a warp's results at an item's end go into its stage that is not under
   // way, or where that is too small behind the ring
-  extern __shared__ __align__(16) uint8_t ring[];
+  extern __shared__ uint8_t raw[];
+  uint8_t* ring = raw + ((0u - smem_u32(raw)) & 1023u);          // (a swizzle counts from 1 KB)
   constexpr bool IN_STAGE = R * OROW * 4 <= STAGE;
-  __shared__ __align__(16) __half qh[PARTS][R][HD];
+  // q as the products want it: [half][tile of heads][word of a key][lane][four channels]; read again for every tile,
+  // so that four blocks' registers fit an SM
+  __shared__ __align__(16) __half qh[PARTS][NT][KWORDS][32][4];
   __shared__ float qs[R], q_sum[R], sm[WARPS][R], sl[WARPS][R], back[WARPS];
   __shared__ int so_at[WARPS];
   __shared__ __align__(16) uint8_t fresh_row[2][HD];             // STEP: the new token's codes and scales
   __shared__ float fresh_scale[2];
-  pdl_trigger();
+  __shared__ uint64_t bars[WARPS][STAGES];
+  __shared__ Kept kept[WARPS];
+  if (TMA && (threadIdx.x & 31) == 0) {
+#pragma unroll
+    for (int i = 0; i < STAGES; ++i) mbar_init(&bars[threadIdx.x >> 5][i], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  __syncwarp();
   if (a.stream) {
     // what an item's start waits for comes from far off (the cache has swept it out of L2): asked for early
     const auto ask = [](const void* at) { asm volatile("prefetch.global.L2 [%0];" ::"l"(at)); };
@@ -420,9 +488,17 @@ quant_decode_kernel(const DecodeArgs a) {
   const int heads = a.nkv * a.chunks, G = a.nh / a.nkv;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   uint8_t* mine = ring + warp * STAGES * STAGE;
+  uint8_t* my_scales = ring + WARPS * STAGES * STAGE + warp * STAGES * SCALES;
+  const Layout lay = {TMA && a.unit == 8 ? 16 * SW : 8 * SW, TMA && a.unit == 8 ? 8 * SW : 16 * SW};
+  uint32_t phases = 0;                     // of the stages' barriers, a bit each
+  bool lost = false;                       // a copy has not come within the limit: nothing more is waited for
   Cursor cur;
+  // The joining kernel is let in early only where this one leaves SMs idle: else its waiting blocks take the places of
+  // the next call's, which then start late (12 us of 76 with 592 blocks).
+  if (!a.stream) pdl_trigger();
   if (a.stream) {
     cur = find_run(a, blockIdx.x, gridDim.x, heads);
+    if (cur.todo == 0 || cur.run == kLeastTiles) pdl_trigger();
   } else {
     cur.b = blockIdx.x / heads, cur.hc = blockIdx.x - cur.b * heads, cur.len = request_length(a, cur.b);
     cur.off = 0, cur.todo = cur.run = request_tiles(a, cur.len);
@@ -452,8 +528,8 @@ quant_decode_kernel(const DecodeArgs a) {
 
   int pages[STAGES];
   const auto tiles_of = [&](const Item& it) {
-    return Tiles<WHOLE>{a, a.block_table + (size_t)it.b * a.table_stride, it.hc / a.chunks, it.lo,
-                        STEP ? it.len - 1 : it.len, it.last, lane};
+    return Tiles<TMA>{a, a.block_table + (size_t)it.b * a.table_stride, it.hc / a.chunks, it.lo,
+                      STEP && !TMA ? it.len - 1 : it.len, it.last, lane, lay};
   };
   const auto ask_pages = [&](const Item& it) {
 #pragma unroll
@@ -471,7 +547,7 @@ quant_decode_kernel(const DecodeArgs a) {
     // ---- an item's start: all that it waits for is asked for before anything is used
     const int kvh = it.hc / a.chunks, h0 = head_of(it.hc), nrows = rows_of(it.hc), p = it.len - 1;
     const size_t row = (size_t)it.b * a.q_stride;
-    const Tiles<WHOLE> tiles = tiles_of(it);
+    const Tiles<TMA> tiles = tiles_of(it);
     float x[RW][N], y[RW][N], nx[N], ny[N];
     Angles an;
     // the new token's row of keys (the last warp's, whose rows of q may not exist) and of values (the one before)
@@ -499,13 +575,14 @@ quant_decode_kernel(const DecodeArgs a) {
 #pragma unroll
       for (int i = 0; i < STAGES - 1; ++i) {
         const int tile = it.first + warp + i * WARPS;
-        if (tile < it.last) tiles.copy(mine + stage * STAGE, tile, pages[i]);
-        asm volatile("cp.async.commit_group;\n");
+        if (tile < it.last && !lost) tiles.copy(&map, &bars[warp][stage], mine + stage * STAGE, my_scales + stage * SCALES, tile, pages[i]);
+        if constexpr (!TMA) asm volatile("cp.async.commit_group;\n");
         stage = stage + 1 == STAGES ? 0 : stage + 1;
       }
       page_number = pages[STAGES - 1];
     }
 
+    if (!have) pdl_trigger();
     // ---- the end of the item before: the four warps' results
     if (had) {
 #pragma unroll
@@ -517,7 +594,7 @@ quant_decode_kernel(const DecodeArgs a) {
           l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 16);
           if (g == 0) sm[warp][n * 8 + 2 * t + j] = m[n][j], sl[warp][n * 8 + 2 * t + j] = l[n][j];
         }
-      const int place = IN_STAGE ? (warp * STAGES + to_stage) * STAGE : WARPS * STAGES * STAGE + warp * R * OROW * 4;
+      const int place = IN_STAGE ? (warp * STAGES + to_stage) * STAGE : WARPS * STAGES * (STAGE + SCALES) + warp * R * OROW * 4;
       if (lane == 0) back[warp] = power_back(f), so_at[warp] = place;
       __syncwarp();                        // (the stage's tile has been read)
       float* so = reinterpret_cast<float*>(ring + place);
@@ -533,6 +610,7 @@ quant_decode_kernel(const DecodeArgs a) {
           *reinterpret_cast<float2*>(at + OROW) = make_float2(o[n][i][1], o[n][i][3]);
         }
       }
+      if constexpr (TMA && IN_STAGE) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncthreads();
       const bool whole = done.starts && done.ends;
       const size_t part = ((size_t)blockIdx.x * 2 + (done.starts ? 1 : 0)) * a.rows;
@@ -605,9 +683,10 @@ quant_decode_kernel(const DecodeArgs a) {
       for (int i = 0; i < N; ++i) {
         const int c = i * 32 + lane;
         if (c < HD) {
-          qh[0][r][c] = __float2half_rn(x[j][i] * scale_up);
+          const int at = q_place(r, c);
+          (&qh[0][0][0][0][0])[at] = __float2half_rn(x[j][i] * scale_up);
           if constexpr (RAISED) sum += __half2float(__float2half_rn(x[j][i] * scale_up));
-          if constexpr (PARTS == 2) qh[1][r][c] = __float2half_rn(half_rest(x[j][i] * scale_up));
+          if constexpr (PARTS == 2) (&qh[PARTS - 1][0][0][0][0])[at] = __float2half_rn(half_rest(x[j][i] * scale_up));
         }
       }
       if constexpr (RAISED) sum = warp_sum(sum);
@@ -617,17 +696,6 @@ quant_decode_kernel(const DecodeArgs a) {
       }
     }
     __syncthreads();
-    uint32_t qf[PARTS][NT][KWORDS][2];
-#pragma unroll
-    for (int w = 0; w < KWORDS; ++w)
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < PARTS; ++i) {
-          // (a thread's channels: a quarter of the head, four a word)
-          const uint2 two = *reinterpret_cast<const uint2*>(&qh[i][n * 8 + g][t * (HD / 4) + 4 * w]);
-          qf[i][n][w][0] = two.x, qf[i][n][w][1] = two.y;
-        }
     // a score is (product * qscale + qshift) * the key's scale
     float qscale[NT][2], qshift[NT][2];
 #pragma unroll
@@ -650,35 +718,48 @@ quant_decode_kernel(const DecodeArgs a) {
     if (cur.todo > 0) cur.len = soon_b == cur.b ? soon_len : request_length(a, cur.b);
     have = next_item(it);
     soon_b = later_b, soon_len = later_len;
+    if (lane == 0) kept[warp] = {it, done, cur, soon_b, soon_len};       // (no use of registers for it meanwhile)
+    __syncwarp();
     if (have) ask_pages(it);
 
     // ---- the tiles
 #pragma unroll 1
-    for (int tile = first + warp; tile < last; tile += WARPS) {
-      wait_copies<STAGES - 2>();
+    for (int tile = first + warp; tile < last && !lost; tile += WARPS) {
+      if constexpr (TMA) {
+        lost = !mbar_wait(&bars[warp][at_stage], phases >> at_stage & 1u, a.err, 1);
+        lost = __any_sync(0xffffffffu, lost);
+        phases ^= 1u << at_stage;
+      } else {
+        wait_copies<STAGES - 2>();
+      }
       __syncwarp();            // every lane's copies have landed, and the stage before has been read
       uint8_t* stage = mine + at_stage * STAGE;
+      const uint8_t* stage_scales = my_scales + at_stage * SCALES;
       const int c0 = tile * TILE;
       {
         const int far = tile + (STAGES - 1) * WARPS;
         const int next_page = tiles.page_of(far + WARPS);
-        if (far < last) tiles.copy(mine + to_stage * STAGE, far, page_number);
-        asm volatile("cp.async.commit_group;\n");
+        if (far < last)
+          tiles.copy(&map, &bars[warp][to_stage], mine + to_stage * STAGE, my_scales + to_stage * SCALES, far, page_number);
+        if constexpr (!TMA) asm volatile("cp.async.commit_group;\n");
         page_number = next_page;
       }
       at_stage = at_stage + 1 == STAGES ? 0 : at_stage + 1;
       to_stage = to_stage + 1 == STAGES ? 0 : to_stage + 1;
       float2 sc[2 * TK];           // of keys g, g + 8, ...
 #pragma unroll
-      for (int i = 0; i < 2 * TK; ++i) sc[i] = tiles.scales(stage, g + 8 * i);
+      for (int i = 0; i < 2 * TK; ++i) sc[i] = tiles.scales(stage_scales, g + 8 * i);
+      const bool edge = c0 < lo || c0 + TILE > len;
+      if (edge) tiles.clear_masked(stage, tile, len);
       if constexpr (STEP) {
         if (c0 + TILE >= len) {     // the tile of the new token
           const int r = len - 1 - c0;
           for (int i = lane; i < 2 * CH; i += 32) {
             const int which = i / CH, ch = i - which * CH;
-            *reinterpret_cast<uint4*>(stage + (which * TILE + r) * ROW + ch * 16) =
+            *reinterpret_cast<uint4*>(stage + lay.at(which, r, ch)) =
                 *reinterpret_cast<const uint4*>(&fresh_row[which][ch * 16]);
           }
+          if constexpr (TMA) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           const float2 mine_sc = make_float2(fresh_scale[0], fresh_scale[1]);
 #pragma unroll
@@ -701,7 +782,8 @@ quant_decode_kernel(const DecodeArgs a) {
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int j = 0; j < KWORDS / (KW / 4); ++j)
-            read_bytes<KW>(stage + (16 * q + g + 8 * i) * ROW + t * (HD / 4) + j * KW, &k[i][j * (KW / 4)]);
+            read_bytes<KW>(stage + lay.at(0, 16 * q + 8 * i + g, key_channel(t, j * (KW / 4)) / 16) +
+                               key_channel(t, j * (KW / 4)) % 16, &k[i][j * (KW / 4)]);
 #pragma unroll
         for (int w = 0; w < KWORDS; ++w) {
           const uint32_t k0 = FP8 ? k[0][w] : k[0][w] ^ 0x80808080u, k1 = FP8 ? k[1][w] : k[1][w] ^ 0x80808080u;
@@ -714,7 +796,10 @@ quant_decode_kernel(const DecodeArgs a) {
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int i = PARTS - 1; i >= 0; --i) mma_f16(s2[w % CHAINS][n], A, qf[i][n][w][0], qf[i][n][w][1]);
+            for (int i = PARTS - 1; i >= 0; --i) {
+              const uint2 two = *reinterpret_cast<const uint2*>(&qh[i][n][w][lane][0]);
+              mma_f16(s2[w % CHAINS][n], A, two.x, two.y);
+            }
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -724,7 +809,7 @@ quant_decode_kernel(const DecodeArgs a) {
       bool seen[2 * TK];
 #pragma unroll
       for (int i = 0; i < 2 * TK; ++i) seen[i] = true;
-      if (c0 < lo || c0 + TILE > len) {
+      if (edge) {
         // masked keys: whatever lies there counts as nothing (their codes are zeros already)
 #pragma unroll
         for (int i = 0; i < 2 * TK; ++i) {
@@ -820,7 +905,8 @@ quant_decode_kernel(const DecodeArgs a) {
           uint32_t v[4][WORDS];            // keys 2t, 2t + 1, 2t + 8, 2t + 9 of the 16
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            read_bytes<VW>(stage + (TILE + 16 * q + 2 * t + (i & 1) + 8 * (i >> 1)) * ROW + (j * 8 + g) * VW, v[i]);
+            read_bytes<VW>(stage + lay.at(1, 16 * q + 8 * (i >> 1) + 2 * t + (i & 1), (j * 8 + g) * VW / 16) +
+                               (j * 8 + g) * VW % 16, v[i]);
             if constexpr (!FP8) {
 #pragma unroll
               for (int w = 0; w < WORDS; ++w) v[i][w] ^= 0x80808080u;
@@ -853,6 +939,9 @@ quant_decode_kernel(const DecodeArgs a) {
               for (int e = 0; e < 4; ++e) o[n][j * WORDS * PER + i][e] += d[i][n][e];
       }
     }
+    it = kept[warp].next, done = kept[warp].done, cur = kept[warp].cur;
+    soon_b = kept[warp].soon_b, soon_len = kept[warp].soon_len;
+    __syncwarp();
   }
 }
 
@@ -863,13 +952,15 @@ constexpr int TEAM = HD / 4, JOIN_AT_ONCE = 8, FEW_PIECES = 8;
 struct Joined {
   float4 o;
   float m, l;
-  __device__ __forceinline__ void add(float4 v, float vm, float vl) {
-    const float top = fmaxf(m, vm);
+  // (a part whose scores are no numbers has a maximum of -inf and passes its sum on)
+  __device__ __forceinline__ void raise(float top) {
     const float mine = m == -INFINITY ? 0.f : fast_exp2(m - top);
-    const float w = (vm == -INFINITY ? 0.f : fast_exp2(vm - top)) * vl;
-    o.x = fmaf(w, v.x, mine * o.x), o.y = fmaf(w, v.y, mine * o.y);
-    o.z = fmaf(w, v.z, mine * o.z), o.w = fmaf(w, v.w, mine * o.w);
-    l = mine * l + w, m = top;
+    o.x *= mine, o.y *= mine, o.z *= mine, o.w *= mine, l *= mine, m = top;
+  }
+  __device__ __forceinline__ void add(float4 v, float vm, float vl) {      // of a part not above m
+    const float w = (vm == -INFINITY ? 0.f : fast_exp2(vm - m)) * vl;
+    o.x = fmaf(w, v.x, o.x), o.y = fmaf(w, v.y, o.y), o.z = fmaf(w, v.z, o.z), o.w = fmaf(w, v.w, o.w);
+    l += w;
   }
 };
 template <int JOIN_THREADS>
@@ -920,6 +1011,10 @@ quant_join_kernel(const DecodeArgs a) {
             v[k] = __ldcg(reinterpret_cast<const float4*>(po + part * HD));
           }
         }
+        float top = sum.m;
+#pragma unroll
+        for (int k = 0; k < JOIN_AT_ONCE; ++k) top = fmaxf(top, x[k].x);
+        sum.raise(top);
 #pragma unroll
         for (int k = 0; k < JOIN_AT_ONCE; ++k) sum.add(v[k], x[k].x, x[k].y);
       }
@@ -933,28 +1028,29 @@ quant_join_kernel(const DecodeArgs a) {
     if (team < TEAMS && c == 0) part_ml[team] = make_float2(sum.m, sum.l);
     __syncthreads();
     if (team == 0) {
-      // a team's o is not divided by its sum
+      float top = part_ml[0].x;
 #pragma unroll
-      for (int i = 1; i < TEAMS; ++i) {
+      for (int i = 1; i < TEAMS; ++i) top = fmaxf(top, part_ml[i].x);
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      float l = 0.f;
+#pragma unroll
+      for (int i = 0; i < TEAMS; ++i) {                   // (a team's o is not divided by its sum)
         const float4 v = part[i][c];
         const float2 x = part_ml[i];
-        const float top = fmaxf(sum.m, x.x);
-        const float mine = sum.m == -INFINITY ? 0.f : fast_exp2(sum.m - top);
         const float w = x.x == -INFINITY ? 0.f : fast_exp2(x.x - top);
-        sum.o.x = fmaf(w, v.x, mine * sum.o.x), sum.o.y = fmaf(w, v.y, mine * sum.o.y);
-        sum.o.z = fmaf(w, v.z, mine * sum.o.z), sum.o.w = fmaf(w, v.w, mine * sum.o.w);
-        sum.l = mine * sum.l + w * x.y, sum.m = top;
+        o.x = fmaf(w, v.x, o.x), o.y = fmaf(w, v.y, o.y), o.z = fmaf(w, v.z, o.z), o.w = fmaf(w, v.w, o.w);
+        l = fmaf(w, x.y, l);
       }
-      store(r, sum.o, 1.f / sum.l);
+      store(r, o, 1.f / l);
     }
   }
 }
 
-template <int NT, bool FP8, typename T, bool WHOLE, bool STEP>
+template <int NT, bool FP8, typename T, bool TMA, bool STEP>
 int launch_decode(DecodeArgs a, int sms, void* scratch, size_t scratch_bytes, cudaStream_t stream) {
-  constexpr auto kernel = quant_decode_kernel<NT, FP8, T, WHOLE, STEP>;
-  constexpr int results = 8 * NT * (HD + 2) * 4;
-  constexpr int smem = WARPS * (STAGES * STAGE + (results <= STAGE ? 0 : results));
+  constexpr auto kernel = quant_decode_kernel<NT, FP8, T, TMA, STEP>;
+  constexpr int results = 8 * NT * result_row(NT) * 4;
+  constexpr int smem = 1024 + WARPS * (STAGES * (STAGE + SCALES) + (results <= STAGE ? 0 : results));
   static OncePerDevice once;
   static int blocks_a_sm[OncePerDevice::kMaxDevices];
   int dev = 0;
@@ -979,7 +1075,20 @@ int launch_decode(DecodeArgs a, int sms, void* scratch, size_t scratch_bytes, cu
     a.po = (float*)((char*)scratch + head);
     a.pml = (float2*)(a.po + rows * HD);
   }
-  const int e = launch_kernel(kernel, dim3((unsigned)blocks), dim3(THREADS), smem, stream, a);
+  CUtensorMap map = {};
+  if constexpr (TMA) {
+    // a head's channels, the places of a page, a page's rows of heads (keys, then values), pages
+    const EncodeTiledFn encode = encode_fn();
+    const cuuint64_t dims[4] = {HD, (cuuint64_t)a.page, 2 * (cuuint64_t)a.nkv, (cuuint64_t)a.pages};
+    const cuuint64_t strides[3] = {HD, (cuuint64_t)a.page * HD, 2 * (cuuint64_t)a.nkv * a.page * HD};
+    const cuuint32_t box[4] = {SW, (cuuint32_t)a.unit, 2, 1}, steps[4] = {1, 1, 1, 1};
+    if (!encode || encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, a.codes, dims, strides, box, steps,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          SW == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return -8;
+  }
+  const int e = launch_kernel(kernel, dim3((unsigned)blocks), dim3(THREADS), smem, stream, a, map);
   if (e || !a.stream) return e;
   // few items (which have many parts): a block a head, with more teams
   if (items * a.rows <= 8LL * sms)
@@ -1014,9 +1123,10 @@ struct DecodeCall {
   void* scratch;
   long long scratch_bytes;
   cudaStream_t stream;
+  int* err;                   // set where a copy does not come within the limit of a wait
   double scale;
 };
-static_assert(sizeof(DecodeCall) == 27 * 8, "the caller packs it");
+static_assert(sizeof(DecodeCall) == 28 * 8, "the caller packs it");
 
 GF_EXPORT int gf_quant_decode(const DecodeCall* call) {
   const DecodeCall& c = *call;
@@ -1038,6 +1148,7 @@ GF_EXPORT int gf_quant_decode(const DecodeCall* call) {
   a.page_shift = (a.page & (a.page - 1)) == 0 ? __builtin_ctz(a.page) : -1;
   a.table = c.table, a.table_rows = c.table_rows > 0 ? (int)c.table_rows : 1, a.rot = (int)c.rot;
   a.neighbours = c.neighbours != 0;
+  a.unit = a.page % 16 ? 8 : 16, a.err = c.err;
   const int G = a.nh / a.nkv;
   a.chunks = (G + 15) / 16, a.rows = (G + a.chunks - 1) / a.chunks;
   const auto go = [&](auto nt, auto kind, auto type, auto whole, auto fused) {
@@ -1048,7 +1159,12 @@ GF_EXPORT int gf_quant_decode(const DecodeCall* call) {
     return x ? next(std::true_type()) : next(std::false_type());
   };
   return pick_bool(c.fp8 != 0, [&](auto kind) {
-    return pick_bool(a.page % 16 == 0 && (size_t)c.scales % 16 == 0, [&](auto whole) {
+    // (whole copies: keys of a unit lie in one page)
+    const auto pick_tma = [&](auto next) {
+      if constexpr (SWIZZLED) return pick_bool(a.page % 8 == 0 && (size_t)c.scales % 16 == 0, next);
+      else return next(std::false_type());
+    };
+    return pick_tma([&](auto whole) {
       return pick_bool(c.step != 0, [&](auto fused) {
         using One = std::integral_constant<int, 1>;
         using Two = std::integral_constant<int, 2>;

@@ -25,13 +25,13 @@ import torch
 
 from . import _Counter, _ok
 from .build import load_library
-from .gemm_bf16 import num_sms
+from .gemm_bf16 import error_word, num_sms
 
 KINDS = {"int8": torch.int8, "fp8": torch.float8_e4m3fn}
 MAX_HEAD_DIM = 256
 _FP8 = {torch.int8: 0, torch.float8_e4m3fn: 1}
 _CODE = {torch.float32: 0, torch.bfloat16: 1}
-_WRITE, _READ, _DECODE = struct.Struct("=20q"), struct.Struct("=17q"), struct.Struct("=26qd")
+_WRITE, _READ, _DECODE = struct.Struct("=20q"), struct.Struct("=17q"), struct.Struct("=27qd")
 _current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 _capturing = torch.cuda.is_current_stream_capturing
 _int32, _float32 = torch.int32, torch.float32
@@ -211,7 +211,7 @@ def read_slots(cache, slots: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
 # same line: kShortKeys).
 _SHORT = 512
 _scratch: dict = {}
-_sms: dict = {}
+_devices: dict = {}       # SMs, and the address of the word that kernels set when a bounded wait runs out
 
 
 def _scratch_for(words: int, device: int, stream: int) -> torch.Tensor:
@@ -235,9 +235,10 @@ def _decode(q, nh, facts, block_table, lengths, scale, span, fused=None):
         raise ValueError(f"{q.shape[0]} queries for {B} requests")
     table, rows, rot = (0, 0, 0) if fused is None else _angles(fused[0], hd, dev)
     out = q.new_empty(B, nh * hd)
-    sms = _sms.get(dev)
-    if sms is None:
-        sms = _sms[dev] = num_sms(dev)
+    facts_of_device = _devices.get(dev)
+    if facts_of_device is None:
+        facts_of_device = _devices[dev] = num_sms(dev), error_word(dev).data_ptr()
+    sms, err = facts_of_device
     stream = _raw_stream(dev)
     scratch, words = None, 0
     if W * page > _SHORT:
@@ -248,7 +249,7 @@ def _decode(q, nh, facts, block_table, lengths, scale, span, fused=None):
                      _ints(block_table, (B, W), "block_table", dev), W, W, _ints(lengths, (B,), "lengths", dev), pages,
                      out.data_ptr(), B, nh, nkv, page, span, fused is not None, table, rows, rot,
                      fused is not None and fused[1], sms, 0 if scratch is None else scratch.data_ptr(), 4 * words,
-                     stream, scale))
+                     stream, err, scale))
     _Counter.launches += 1 if scratch is None else 2
     if rc:
         _ok(rc, "quant_cache.decode" if fused is None else "quant_cache.step")

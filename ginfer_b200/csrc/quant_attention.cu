@@ -80,7 +80,7 @@ constexpr int blocks_an_sm(int nt, int type_bytes) {
   return nt == 1 ? (HD <= 128 && type_bytes == 2 ? 4 : 3) : (HD <= 128 ? 3 : 2);
 }
 // the fewest tiles of a block's run
-constexpr int kLeastTiles = 4 * WARPS / TK;
+constexpr int kLeastTiles = 2 * WARPS / TK;
 // Requests that see at most kShortKeys keys are one block's work a kv head; up to kMiddleKeys they are where that
 // gives the SMs enough blocks: the joining kernel costs 4 us, as much as 500 keys.
 constexpr int kShortKeys = 512, kMiddleKeys = 1024;
@@ -167,7 +167,8 @@ __device__ __forceinline__ Cursor find_run(const DecodeArgs& a, int k, int block
   const unsigned long long all = (unsigned long long)total * heads;
   const bool narrow = all < 0xffff0000ull;         // (64-bit divisions cost more than the rest of this)
   const unsigned long long share = narrow ? ((unsigned)all + blocks - 1) / (unsigned)blocks : (all + blocks - 1) / blocks;
-  const unsigned long long run = max(share, (unsigned long long)kLeastTiles), at = run * k;
+  // (a multiple of the warps, which end together)
+  const unsigned long long run = max((share + WARPS - 1) / WARPS * WARPS, (unsigned long long)kLeastTiles), at = run * k;
   if (at < all) {
     const unsigned hc = narrow ? (unsigned)at / total : (unsigned)(at / total);
     const unsigned rest = (unsigned)(at - (unsigned long long)hc * total);
@@ -467,6 +468,7 @@ quant_decode_kernel(const DecodeArgs a, const __grid_constant__ CUtensorMap map)
   __shared__ float fresh_scale[2];
   __shared__ uint64_t bars[WARPS][STAGES];
   __shared__ Kept kept[WARPS];
+  if (TMA && threadIdx.x == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(&map) : "memory");
   if (TMA && (threadIdx.x & 31) == 0) {
 #pragma unroll
     for (int i = 0; i < STAGES; ++i) mbar_init(&bars[threadIdx.x >> 5][i], 1);
@@ -728,6 +730,14 @@ quant_decode_kernel(const DecodeArgs a, const __grid_constant__ CUtensorMap map)
       if constexpr (TMA) {
         lost = !mbar_wait(&bars[warp][at_stage], phases >> at_stage & 1u, a.err, 1);
         lost = __any_sync(0xffffffffu, lost);
+        if (lost) {            // (what is under way must not find another block's shared memory)
+#pragma unroll 1
+          for (int i = 0; i < STAGES - 1; ++i) {
+            const int st = (at_stage + i) % STAGES;
+            if (tile + i * WARPS < last) mbar_wait(&bars[warp][st], phases >> st & 1u, nullptr, 0);
+          }
+          break;
+        }
         phases ^= 1u << at_stage;
       } else {
         wait_copies<STAGES - 2>();

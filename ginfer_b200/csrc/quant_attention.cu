@@ -45,8 +45,9 @@ namespace {
 constexpr int HD = GF_HEAD_DIM;
 static_assert(HD % 16 == 0 && HD >= 16 && HD <= 256, "head size must be a multiple of 16, <= 256");
 constexpr float kLog2E = 1.4426950408889634f;
-// Keys of a tile: 32 where a head is short, so that a tile is as many bytes and its steps overlap.
-constexpr int TK = HD <= 64 ? 2 : 1, TILE = 16 * TK, TILE_SHIFT = TK == 2 ? 5 : 4;
+// Keys of a tile: 32 while their products fit the registers.  What a tile costs beside its bytes (waiting, copies,
+// maxima, q from shared memory) is half, and two chains of steps overlap: 304 MB of heads of 128 59 us after 63.
+constexpr int TK = HD <= 128 ? 2 : 1, TILE = 16 * TK, TILE_SHIFT = TK == 2 ? 5 : 4;
 constexpr int WARPS = 4, THREADS = WARPS * 32;
 constexpr int KW = HD % 64 == 0 ? 16 : HD % 32 == 0 ? 8 : 4;     // bytes of a key a thread reads at once
 constexpr int VW = HD % 128 == 0 ? 16 : HD % 64 == 0 ? 8 : HD % 32 == 0 ? 4 : 2;
@@ -77,7 +78,7 @@ struct Layout {
 constexpr int STAGES = 2;
 // Blocks an SM: as many as their registers allow without spilling to memory in a tile's work.
 constexpr int blocks_an_sm(int nt, int type_bytes) {
-  return nt == 1 ? (HD <= 128 && type_bytes == 2 ? 4 : 3) : (HD <= 128 ? 3 : 2);
+  return nt == 1 ? (HD <= 64 && type_bytes == 2 ? 4 : 3) : (HD <= 128 ? 3 : 2);
 }
 // the fewest tiles of a block's run
 constexpr int kLeastTiles = 2 * WARPS / TK;
@@ -432,9 +433,11 @@ __device__ __forceinline__ uint32_t row_top(const float (&x)[N]) {
 }
 
 // ------------------------------------------------------------------------------------- a block's run
-// Floats from a head's result to the next one's in shared memory: two rows in other banks, where a warp's results then
-// still fit a stage or the head is short enough for room of their own.
-__host__ __device__ constexpr int result_row(int nt) { return HD > 128 && 8 * nt * HD * 4 <= STAGE ? HD : HD + 2; }
+// Floats from a head's result to the next one's in shared memory: two rows in other banks, unless a warp's results then no
+// longer fit a stage.
+__host__ __device__ constexpr int result_row(int nt) {
+  return 8 * nt * (HD + 2) * 4 > STAGE && 8 * nt * HD * 4 <= STAGE ? HD : HD + 2;
+}
 struct Item {
   int b, hc, len, lo, first, last;         // its tiles here
   bool starts, ends;                       // whether they are its first, its last

@@ -5,18 +5,22 @@
 // first_visible_key(p, span) .. p.  out = sum_c softmax_c(scale <q, K_c>) V_c; a request without a
 // token gives zeros.
 //
-// What bounds it is reading the cache: 2 HD + 8 bytes a key and kv head, used once.  So a code goes from
-// memory to the registers of the one thread that multiplies it, without shared memory between:
+// What bounds it is reading the cache: 2 HD + 8 bytes a key and kv head, used once.  For q, K_c and V_c of one kv head
+// that is 2 multiply-adds a byte and query head, far too many for the plain cores and a tenth of what the tensor cores
+// do: so both products run there, and a tile of codes becomes operands with as few instructions as possible.
 //
 //  * S^T = K q^T on mma.sync.m16n8k16 (half precision in, 32-bit sums): 16 keys are the rows, up to 8 query
 //    heads of a kv head the columns.  The order of a product's reduction is free as long as both operands
 //    share it, so the channels are dealt to the instruction's places such that a thread's places are
-//    neighbours in memory: it loads up to 16 bytes of its two keys at a time.
+//    neighbours in memory: it reads up to 16 bytes of its two keys at a time.
 //  * O^T = V^T P^T: the rows are channels, the reduction runs over the 16 keys.  A thread's rows are again
 //    chosen to be neighbours in memory; two keys' codes of a channel are put side by side by a byte
 //    permutation.  P^T comes from S^T by movmatrix.
 //  * Codes become halves exactly: e4m3 by one conversion of two, int8 as 1024 + 128 + code, whose bits are
-//    0x64 above the code's, minus 1152.
+//    0x64 above the code's, minus 1152; or, for keys, as 2^-24 (code + 128) without any arithmetic, the 128 sum(q)
+//    taken off the score.
+//  (With 8 query heads a kv head the operands of tcgen05 would be 128 rows of keys that have to be unpacked into
+//  shared memory as halves first, four times the bytes that this reads there.)
 //
 // Half precision holds q and the weights in 11 bits (a row of q is scaled by a power of two so that its
 // largest element is in [2^14, 2^15); a weight, p times its value row's scale, so that the largest value
@@ -24,9 +28,17 @@
 // are the sum of two halves (22 bits), and tiles' products are added up outside the tensor cores.  Scores,
 // maxima, sums and O are 32-bit.
 //
-// A block is four warps, which take the tiles of its share of the work in turn (how it is shared out: see
-// Cursor), each through a ring of stages of its own that cp.async fills: nothing but an item's start and end
-// synchronises the block.
+// A block is four warps, which take the tiles of its share of the work in turn (how it is shared out: see Cursor),
+// each through a ring of two stages of its own: nothing but an item's start and end synchronises the block, and an
+// item's first tiles are on their way while the one before is being joined.  Head sizes that are a multiple of 64
+// come by TMA, 8 or 16 keys with their values a copy, swizzled so that no read meets another's bank; others, pages
+// that are no multiple of 8 and scales that are not aligned come by cp.async.
+//
+// Measured (bfloat16 q, 4 kv heads of 128 with 7 query heads each, pages of 16, the cache not in L2): 64 requests of
+// 4,500 keys on average, 304 MB: 59.5 us, 5.1 TB/s (e4m3; integers 61.6); one request of 131,071 keys, 138 MB: 32.9 us,
+// 4.2 TB/s, of which the first tile's chain length -> page -> codes takes 4, blocks that end apart 5, and the join with
+// its launch 5.  A ring that only copies reads 6.6 TB/s here, one of cp.async 5.4; tiles straight to registers came to
+// 4.0 with the rest of this kernel.
 #include <algorithm>
 #include <cstdlib>
 #include <type_traits>
@@ -76,9 +88,10 @@ struct Layout {
   }
 };
 constexpr int STAGES = 2;
-// Blocks an SM: as many as their registers allow without spilling to memory in a tile's work.
+// Blocks an SM: as many as their registers allow without spilling in a tile's work.  (Two tiles of heads: 50 us with
+// two of them, 53 with three, at 16 query heads of 128 a kv head; one of heads with 32-bit q: 71 with three, 78 with two.)
 constexpr int blocks_an_sm(int nt, int type_bytes) {
-  return nt == 1 ? (HD <= 64 && type_bytes == 2 ? 4 : 3) : (HD <= 128 ? 3 : 2);
+  return nt == 1 ? (HD <= 64 && type_bytes == 2 ? 4 : 3) : (HD <= 96 ? 3 : 2);
 }
 // the fewest tiles of a block's run
 constexpr int kLeastTiles = 2 * WARPS / TK;
@@ -119,7 +132,7 @@ __device__ __forceinline__ float fast_exp2(float x) {
 
 // ------------------------------------------------------------------------------------- division of the work
 // An item is a (chunk of query heads that share a kv head, request), request by request within a chunk, and its
-// tiles are the positions first_visible .. len - 1 cut at multiples of 16; a request without a token counts as one.
+// tiles are the positions first_visible .. len - 1 cut at multiples of TILE; a request without a token counts as one.
 // Where requests are short (DecodeArgs.stream 0) a block takes an item.  Else the items' tiles are one long
 // sequence, and every block takes an equal run of it: they all end at the same time, whatever the lengths.  A run
 // begins and ends inside items; such parts are joined by a second kernel.

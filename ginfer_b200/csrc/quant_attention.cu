@@ -95,9 +95,12 @@ constexpr int blocks_an_sm(int nt, int type_bytes) {
 }
 // the fewest tiles of a block's run
 constexpr int kLeastTiles = 2 * WARPS / TK;
-// Requests that see at most kShortKeys keys are one block's work a kv head; up to kMiddleKeys they are where that
-// gives the SMs enough blocks: the joining kernel costs 4 us, as much as 500 keys.
-constexpr int kShortKeys = 512, kMiddleKeys = 1024;
+// How the work is shared out (launch_decode).  A cluster of up to kMostOfCluster blocks takes an item where the blocks that
+// fit the GPU allow two or more and a request that fills its table keeps them at most as much longer than equal runs would
+// as the joining kernel costs, kUnevenKeys keys a block: 8 requests of 576 keys, tables of 4,096, 12 query heads on 2 kv
+// heads of 128: 10.9 us after 16.7 with equal runs; one of 8,000 keys, where the rule says equal runs: 16.3 after 19.0.
+// kShortKeys keys are one block's work.  Where there are as many items as SMs, up to kMiddleKeys are, too.
+constexpr int kShortKeys = 128, kMiddleKeys = 1024, kMostOfCluster = 8, kUnevenKeys = 700;
 constexpr int kMostBlocks = 8;          // of the blocks that fit an SM, so many are counted on
 
 struct DecodeArgs {
@@ -115,7 +118,8 @@ struct DecodeArgs {
   int unit;                   // keys of a TMA copy
   int* err;
   int chunks, rows;           // a kv head's query heads in `chunks` blocks of up to `rows`
-  int stream;                 // blocks share the tiles evenly (see Cursor), else a block an item
+  int stream;                 // blocks share the tiles evenly (see Cursor), else `cluster` blocks an item
+  int cluster;
   int2* info;                 // [heads * B], stream: the block an item starts in, how many it is spread over
   float* po;                  // [blocks][2][rows][HD]: the parts of the item a block ends in the middle of or starts
   float2* pml;                // [blocks][2][rows]      in the middle of (0: it has begun before this block)
@@ -133,8 +137,8 @@ __device__ __forceinline__ float fast_exp2(float x) {
 // ------------------------------------------------------------------------------------- division of the work
 // An item is a (chunk of query heads that share a kv head, request), request by request within a chunk, and its
 // tiles are the positions first_visible .. len - 1 cut at multiples of TILE; a request without a token counts as one.
-// Where requests are short (DecodeArgs.stream 0) a block takes an item.  Else the items' tiles are one long
-// sequence, and every block takes an equal run of it: they all end at the same time, whatever the lengths.  A run
+// Where requests are short (DecodeArgs.stream 0) a block takes an item, or a cluster of blocks, which joins its own
+// results.  Else the items' tiles are one long sequence, and every block takes an equal run of it: they all end at the same time, whatever the lengths.  A run
 // begins and ends inside items; such parts are joined by a second kernel.
 __device__ __forceinline__ int request_length(const DecodeArgs& a, int b) {
   return max(min(fresh_index(a.lengths + b), a.limit), 0);
@@ -396,7 +400,7 @@ __device__ __forceinline__ int partner(const DecodeArgs& a, int c, bool& second)
   return a.neighbours ? c ^ 1 : second ? c - half : c + half;
 }
 struct Angles {
-  float c[N], s[N];
+  float c[N], s[N];                        // a first of a pair takes off what a second adds: -s
   __device__ __forceinline__ void load(const DecodeArgs& a, int p, int lane) {
     const float* cs = a.table + (size_t)min(p, a.table_rows - 1) * a.rot;
 #pragma unroll
@@ -404,7 +408,8 @@ struct Angles {
       const int ch = i * 32 + lane, half = a.rot >> 1;
       const int j = a.neighbours ? ch >> 1 : ch >= half ? ch - half : ch;
       c[i] = ch < a.rot ? __ldg(cs + j) : 1.f;
-      s[i] = ch < a.rot ? __ldg(cs + half + j) : 0.f;
+      const float sine = ch < a.rot ? __ldg(cs + half + j) : 0.f;
+      s[i] = (a.neighbours ? ch & 1 : ch >= half) ? sine : -sine;
     }
   }
 };
@@ -430,13 +435,8 @@ __device__ __forceinline__ void load_partners(const DecodeArgs& a, size_t at, bo
 }
 __device__ __forceinline__ void turn_row(const DecodeArgs& a, const Angles& an, int lane, float (&x)[N], const float (&y)[N]) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    bool second;
-    const int c = i * 32 + lane;
-    partner(a, c, second);
-    if (c < a.rot)
-      x[i] = second ? turned_second(y[i], x[i], an.c[i], an.s[i]) : turned_first(x[i], y[i], an.c[i], an.s[i]);
-  }
+  for (int i = 0; i < N; ++i)
+    if (i * 32 + lane < a.rot) x[i] = __fadd_rn(__fmul_rn(x[i], an.c[i]), __fmul_rn(y[i], an.s[i]));
 }
 __device__ __forceinline__ uint32_t row_top(const float (&x)[N]) {
   uint32_t top = 0;
@@ -484,6 +484,7 @@ quant_decode_kernel(const DecodeArgs a, const __grid_constant__ CUtensorMap map)
   __shared__ float fresh_scale[2];
   __shared__ uint64_t bars[WARPS][STAGES];
   __shared__ Kept kept[WARPS];
+  __shared__ int parts_of_item;                                  // a cluster's
   if (TMA && threadIdx.x == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(&map) : "memory");
   if (TMA && (threadIdx.x & 31) == 0) {
 #pragma unroll
@@ -518,8 +519,12 @@ quant_decode_kernel(const DecodeArgs a, const __grid_constant__ CUtensorMap map)
     cur = find_run(a, blockIdx.x, gridDim.x, heads);
     if (cur.todo == 0 || cur.run == kLeastTiles) pdl_trigger();
   } else {
-    cur.b = blockIdx.x / heads, cur.hc = blockIdx.x - cur.b * heads, cur.len = request_length(a, cur.b);
-    cur.off = 0, cur.todo = cur.run = request_tiles(a, cur.len);
+    const int item = blockIdx.x / a.cluster, rank = blockIdx.x - item * a.cluster;
+    cur.b = item / heads, cur.hc = item - cur.b * heads, cur.len = request_length(a, cur.b);
+    const int n = request_tiles(a, cur.len);
+    cur.run = ((n + a.cluster - 1) / a.cluster + WARPS - 1) / WARPS * WARPS;
+    cur.off = rank * cur.run, cur.todo = max(min(n - cur.off, cur.run), 0);
+    if (threadIdx.x == 0) parts_of_item = (n + cur.run - 1) / cur.run;
   }
   const auto head_of = [&](int hc) { return (hc / a.chunks) * G + (hc % a.chunks) * a.rows; };
   const auto rows_of = [&](int hc) { return min(a.rows, G - (hc % a.chunks) * a.rows); };
@@ -739,6 +744,10 @@ quant_decode_kernel(const DecodeArgs a, const __grid_constant__ CUtensorMap map)
     if (lane == 0) kept[warp] = {it, done, cur, soon_b, soon_len};       // (no use of registers for it meanwhile)
     __syncwarp();
     if (have) ask_pages(it);
+    if constexpr (STEP) {      // (the angles of that item's position)
+      const float* cs = a.table + (size_t)min(max(it.len - 1, 0), a.table_rows - 1) * a.rot;
+      if (have && threadIdx.x * 32 < a.rot) asm volatile("prefetch.global.L2 [%0];" ::"l"(cs + threadIdx.x * 32));
+    }
 
     // ---- the tiles
 #pragma unroll 1
@@ -969,6 +978,42 @@ quant_decode_kernel(const DecodeArgs a, const __grid_constant__ CUtensorMap map)
     soon_b = kept[warp].soon_b, soon_len = kept[warp].soon_len;
     __syncwarp();
   }
+  // ---- a cluster's parts, every block a share of the channels
+  if (!a.stream && a.cluster > 1) {
+    __syncwarp();
+    cluster_sync();
+    const int parts = parts_of_item, item = blockIdx.x / a.cluster, rank = blockIdx.x - item * a.cluster;
+    if (parts == 1) return;
+    const int b = item / heads, hc = item - b * heads, n_out = rows_of(hc) * (HD / 2);
+    const size_t out_at = ((size_t)b * a.nh + head_of(hc)) * HD, part0 = (size_t)item * a.cluster * 2;
+    for (int i = rank * THREADS + threadIdx.x; i < n_out; i += a.cluster * THREADS) {
+      const int r = i / (HD / 2), c = 2 * (i - r * (HD / 2));
+      float2 ml[kMostOfCluster], v[kMostOfCluster];
+#pragma unroll
+      for (int k = 0; k < kMostOfCluster; ++k) {
+        ml[k] = make_float2(-INFINITY, 0.f), v[k] = make_float2(0.f, 0.f);
+        if (k < parts) {
+          const size_t part = (part0 + (k ? 2 * k : 1)) * a.rows + r;
+          ml[k] = __ldcg(a.pml + part), v[k] = __ldcg(reinterpret_cast<const float2*>(a.po + part * HD + c));
+        }
+      }
+      float top = ml[0].x, sum = 0.f, v0 = 0.f, v1 = 0.f;
+#pragma unroll
+      for (int k = 1; k < kMostOfCluster; ++k) top = fmaxf(top, ml[k].x);
+#pragma unroll
+      for (int k = 0; k < kMostOfCluster; ++k) {
+        // (a part whose scores are no numbers has a maximum of -inf and passes its sum on)
+        const float w = (ml[k].x == -INFINITY ? 0.f : fast_exp2(ml[k].x - top)) * ml[k].y;
+        sum += w, v0 = fmaf(w, v[k].x, v0), v1 = fmaf(w, v[k].y, v1);
+      }
+      const float inv = 1.f / sum;
+      if constexpr (sizeof(T) == 4)
+        *reinterpret_cast<float2*>(reinterpret_cast<float*>(a.out) + out_at + 2 * i) = make_float2(v0 * inv, v1 * inv);
+      else
+        *reinterpret_cast<__nv_bfloat162*>(reinterpret_cast<bf16*>(a.out) + out_at + 2 * i) =
+            __floats2bfloat162_rn(v0 * inv, v1 * inv);
+    }
+  }
 }
 
 // A block an item and `gridDim.y`-th of its heads: the pieces' results, weighted by their shares of the sum.
@@ -1072,6 +1117,7 @@ quant_join_kernel(const DecodeArgs a) {
   }
 }
 
+constexpr int kTwoLaunches = -100;        // not an error: the joining kernel was launched too
 template <int NT, bool FP8, typename T, bool TMA, bool STEP>
 int launch_decode(DecodeArgs a, int sms, void* scratch, size_t scratch_bytes, cudaStream_t stream) {
   constexpr auto kernel = quant_decode_kernel<NT, FP8, T, TMA, STEP>;
@@ -1091,10 +1137,15 @@ int launch_decode(DecodeArgs a, int sms, void* scratch, size_t scratch_bytes, cu
   const int heads = a.nkv * a.chunks;
   const long long items = (long long)a.B * heads;
   const long long keys = a.span ? std::min(std::abs((long long)a.span), (long long)a.limit) : a.limit;
-  a.stream = keys > kMiddleKeys || (keys > kShortKeys && items < sms);
-  const long long blocks = a.stream ? (long long)sms * std::min(std::max(1, blocks_a_sm[dev]), kMostBlocks) : items;
+  const long long places = (long long)sms * std::min(std::max(1, blocks_a_sm[dev]), kMostBlocks);
+  a.cluster = 1;
+  if (keys > kShortKeys)
+    while (a.cluster < kMostOfCluster && items * a.cluster * 2 <= places && a.cluster * kLeastTiles * TILE < keys) a.cluster *= 2;
+  if (a.cluster > 1 && keys * (places - items * a.cluster) > kUnevenKeys * places * a.cluster) a.cluster = 1;
+  a.stream = a.cluster == 1 && (keys > kMiddleKeys || (keys > kShortKeys && items < sms));
+  const long long blocks = a.stream ? places : items * a.cluster;
   if (items > 0x7fffffffLL || blocks > 0x7fffffffLL) return -5;
-  if (a.stream) {
+  if (a.stream || a.cluster > 1) {
     const size_t rows = (size_t)blocks * 2 * a.rows, head = ((size_t)items * 8 + 15) / 16 * 16;
     if (scratch_bytes < head + rows * (HD + 2) * 4) return -7;
     a.info = (int2*)scratch;
@@ -1114,12 +1165,13 @@ int launch_decode(DecodeArgs a, int sms, void* scratch, size_t scratch_bytes, cu
                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
       return -8;
   }
-  const int e = launch_kernel(kernel, dim3((unsigned)blocks), dim3(THREADS), smem, stream, a, map);
+  const int e = launch_kernel_cluster_dims(kernel, dim3((unsigned)blocks), dim3(THREADS), smem, stream, a.cluster, true, a, map);
   if (e || !a.stream) return e;
   // few items (which have many parts): a block a head, with more teams
-  if (items * a.rows <= 8LL * sms)
-    return launch_kernel(quant_join_kernel<512>, dim3((unsigned)items, a.rows), dim3(512), 0, stream, a);
-  return launch_kernel(quant_join_kernel<256>, dim3((unsigned)items), dim3(256), 0, stream, a);
+  const int j = items * a.rows <= 8LL * sms
+                    ? launch_kernel(quant_join_kernel<512>, dim3((unsigned)items, a.rows), dim3(512), 0, stream, a)
+                    : launch_kernel(quant_join_kernel<256>, dim3((unsigned)items), dim3(256), 0, stream, a);
+  return j ? j : kTwoLaunches;
 }
 
 }  // namespace
@@ -1131,7 +1183,7 @@ GF_DEFINE_PDL_SWITCH
 
 // A call: q [B, nh HD], or with `step` q | k | v [B, (nh + 2 nkv) HD] and the table of angles as gf_quant_write takes
 // it.  Scratch: room for two parts of an item a block, of at most kMostBlocks blocks an SM, and 8 bytes an item;
-// none is needed where no request sees more than kShortKeys keys.
+// none is needed where tables hold no more than kShortKeys keys.
 struct DecodeCall {
   const void* q;
   long long q_stride, f32;
@@ -1154,6 +1206,7 @@ struct DecodeCall {
 };
 static_assert(sizeof(DecodeCall) == 28 * 8, "the caller packs it");
 
+// Returns 0, or kTwoLaunches, or an error.
 GF_EXPORT int gf_quant_decode(const DecodeCall* call) {
   const DecodeCall& c = *call;
   if (c.B <= 0) return c.B < 0 ? -3 : 0;

@@ -207,9 +207,9 @@ def read_slots(cache, slots: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     return _read(facts, 0, 0, 0, 0, _ints(slots, (N,), "slots", dev), 1, N, dtype, dev)
 
 
-# Requests of at most this many visible tokens are one block's work a kv head and need no scratch (the kernel has the
-# same line: kShortKeys).
-_SHORT = 512
+# Where tables hold at most this many tokens the kernel needs no scratch (it has the same line: kShortKeys).
+_SHORT = 128
+_TWO_LAUNCHES = -100      # what the attention's entry point returns when the joining kernel went out too
 _scratch: dict = {}
 _devices: dict = {}       # SMs, and the address of the word that kernels set when a bounded wait runs out
 
@@ -250,8 +250,8 @@ def _decode(q, nh, facts, block_table, lengths, scale, span, fused=None):
                      out.data_ptr(), B, nh, nkv, page, span, fused is not None, table, rows, rot,
                      fused is not None and fused[1], sms, 0 if scratch is None else scratch.data_ptr(), 4 * words,
                      stream, err, scale))
-    _Counter.launches += 1 if scratch is None else 2
-    if rc:
+    _Counter.launches += 2 if rc == _TWO_LAUNCHES else 1
+    if rc and rc != _TWO_LAUNCHES:
         _ok(rc, "quant_cache.decode" if fused is None else "quant_cache.step")
     return out
 

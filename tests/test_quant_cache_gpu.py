@@ -392,6 +392,33 @@ def test_step(dtype, kind, rot, neighbours, span, nh, nkv, hd, page, lens):
     check_attention(got, want, top, dtype)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+@pytest.mark.parametrize("nh,nkv,hd,page,lens", [
+    (14, 2, 64, 16, (300, 0, 1, 2000)), (28, 4, 128, 16, (1000, 33, 0, 64)), (8, 8, 64, 24, (129, 5)),
+    (9, 1, 80, 24, (77, 500)), (4, 2, 256, 64, (700, 64, 65)), (12, 2, 128, 16, tuple(range(0, 280, 7))),
+    (40, 1, 128, 8, (99, 3000))])
+def test_step_in_wide_tables(dtype, kind, nh, nkv, hd, page, lens):
+    """Tables that are far wider than the lengths (the work is then shared out in equal runs)."""
+    g = torch.Generator(device=DEV).manual_seed(hd)
+    t, pages, _ = tables(lens, page, g)
+    wide = torch.full((len(lens), 40000 // page), -1, dtype=torch.int32, device=DEV)
+    wide[:, :t.shape[1]] = t
+    cache = random_cache(kind, pages, nkv, page, hd, g)
+    table = angles(hd, max(lens) + 1)
+    x = (1.5 * torch.randn(len(lens), (nh + 2 * nkv) * hd, generator=g, device=DEV)).to(dtype)
+    last = (torch.tensor(lens, device=DEV) - 1).clamp(min=0)
+    for span in (0, 100):
+        got = qc().step(x, nh, table, cache, wide, i32(lens), hd ** -0.5, span)
+        q = rotated(x.double().view(len(lens), -1, hd)[:, :nh], table, last, False).flatten(1)
+        check_attention(got, *attend(cache, t, lens, q, nh, hd ** -0.5, span), dtype)
+        assert torch.equal(got, qc().step(x, nh, table, cache, wide, i32(lens), hd ** -0.5, span))
+    # a value that is no number, in the last request's first page: its first head's queries, and no others
+    cache[1][t[-1, 0].long(), 0, 0, 1] = math.nan
+    got = qc().step(x, nh, table, cache, wide, i32(lens), hd ** -0.5).view(len(lens), nkv, -1)
+    assert got[-1, 0].isnan().all() and torch.isfinite(got[:-1]).all() and torch.isfinite(got[-1, 1:]).all()
+
+
 # ------------------------------------------------------------------------------------------- use
 def test_streams_and_graphs():
     """On a side stream, and replayed from a graph after the lengths, the queries and the cache have changed."""

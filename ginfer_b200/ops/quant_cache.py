@@ -224,8 +224,8 @@ def _scratch_for(words: int, device: int, stream: int) -> torch.Tensor:
     return buf
 
 
-def _decode(q, nh, facts, block_table, lengths, scale, span, fused=None):
-    """``fused``: ``(table of angles, neighbours)``."""
+def _decode(q, nh, facts, block_table, lengths, scale, span, fused=None, out=None):
+    """``fused``: ``(table of angles, neighbours)``.  ``out``: where the result goes, if not into a tensor of its own."""
     codes, scales, fp8, pages, nkv, page, hd = facts
     _heads(nh, nkv)
     dev = _device(codes)
@@ -234,7 +234,8 @@ def _decode(q, nh, facts, block_table, lengths, scale, span, fused=None):
     if q.shape[0] != B:
         raise ValueError(f"{q.shape[0]} queries for {B} requests")
     table, rows, rot = (0, 0, 0) if fused is None else _angles(fused[0], hd, dev)
-    out = q.new_empty(B, nh * hd)
+    if out is None:
+        out = q.new_empty(B, nh * hd)
     facts_of_device = _devices.get(dev)
     if facts_of_device is None:
         facts_of_device = _devices[dev] = num_sms(dev), error_word(dev).data_ptr()
@@ -323,32 +324,38 @@ def attention(qkv: torch.Tensor, nh: int, table, cache, block_table: torch.Tenso
         nd += 1
     out = torch.empty_like(q)
     if nd:
-        out[:nd] = decode(q[:nd], nh, cache, block_table[:nd], ctx.kv_lens[:nd], scale, span)
+        _decode(q[:nd], nh, _cache(cache), block_table[:nd], ctx.kv_lens[:nd], scale, span, out=out[:nd])
     cu, W = ctx.cu_seqlens_q, block_table.shape[1]
-    first = None
-    if span:
-        # the first key that each portion's first token sees
-        p = ctx.positions[cu[nd:B].long()]
-        first = (p - (span - 1)).clamp(min=0) if span > 0 else p // -span * -span
     # (a captured step is replayed with other lengths: there every request may fill its table)
     pages_of = [W if ctx.capturing else -(-(s + n) // page) for s, n in
                 zip(ctx.q_starts_host[nd:], q_lens[nd:])]
-    row = nd
-    for i, j in portion_groups(pages_of, page):
-        wide, n = max(pages_of[i:j]), j - i
-        b0, b1 = nd + i, nd + j
-        rows = sum(q_lens[b0:b1])
-        dense = read(cache, block_table[b0:b1, :wide].contiguous(), ctx.kv_lens[b0:b1], qkv.dtype,
-                     None if first is None else first[i:j])
+    # what the groups' calls take besides the cache is the same for all of the step's layers with this mask (a graph
+    # works it out itself)
+    same = ("read back", page, span, W, _capturing())
+    groups = ctx.extras.get(same)
+    if groups is None:
+        groups = ctx.extras[same] = []
+        first, row = None, nd
+        if span:
+            # the first key that each portion's first token sees
+            p = ctx.positions[cu[nd:B].long()]
+            first = (p - (span - 1)).clamp(min=0) if span > 0 else p // -span * -span
+        for i, j in portion_groups(pages_of, page):
+            wide, n, b0, b1 = max(pages_of[i:j]), j - i, nd + i, nd + j
+            rows = sum(q_lens[b0:b1])
+            groups.append((b0, b1, row, rows, wide, ctx.kv_lens[b0:b1], None if first is None else first[i:j],
+                           torch.arange(n * wide, dtype=_int32, device=q.device).view(n, wide), cu[b0:b1 + 1],
+                           ctx.seq_of_token[row:row + rows] - b0 if qkv.dtype is _float32 else None, max(q_lens[b0:b1])))
+            row += rows
+    for b0, b1, row, rows, wide, lens, low, own, cu_own, seq, most in groups:
+        n = b1 - b0
+        dense = read(cache, block_table[b0:b1, :wide].contiguous(), lens, qkv.dtype, low)
         pages = dense.view(2, n * wide, page, nkv, hd)
-        own = torch.arange(n * wide, dtype=_int32, device=q.device).view(n, wide)
         if qkv.dtype is _float32:
-            out[row:row + rows] = paged_attention_simt(q[row:row + rows], pages, own, ctx.seq_of_token[row:row + rows] - b0,
-                                                       ctx.positions[row:row + rows], nh, nkv, hd, scale, span, page)
+            out[row:row + rows] = paged_attention_simt(q[row:row + rows], pages, own, seq, ctx.positions[row:row + rows],
+                                                       nh, nkv, hd, scale, span, page)
         else:
-            args = (q, pages, own, cu[b0:b1 + 1], ctx.kv_lens[b0:b1], n, max(q_lens[b0:b1]), nh, nkv, hd, scale, span, page)
-            long = max(q_lens[b0:b1]) >= attention_bf16.TC_MIN_QUERY_ROWS
-            if not long or attention_bf16.prefill_tc(*args, out=out) is None:
+            args = (q, pages, own, cu_own, lens, n, most, nh, nkv, hd, scale, span, page)
+            if most < attention_bf16.TC_MIN_QUERY_ROWS or attention_bf16.prefill_tc(*args, out=out) is None:
                 attention_bf16.prefill(*args, out=out)
-        row += rows
     return out

@@ -18,6 +18,7 @@ layer, and converting two dozen arguments one by one costs more than the small k
 """
 from __future__ import annotations
 
+import functools
 import struct
 from ctypes import c_char_p, c_int
 
@@ -257,6 +258,7 @@ def _decode(q, nh, facts, block_table, lengths, scale, span, fused=None, out=Non
     return out
 
 
+@functools.lru_cache(maxsize=1024)
 def scratch_words(B: int, nh: int, nkv: int, hd: int, sms: int) -> int:
     """32-bit words that the attention kernels are content with: two parts of an item a block (at most 8 blocks an
     SM), a head's result with its maximum and sum, and two words an item (see ``csrc/quant_attention.cu``)."""

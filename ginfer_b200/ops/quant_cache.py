@@ -11,7 +11,8 @@ with ``Q`` 127 or 448; a row with an infinity or a NaN reads back as NaN.  A tok
 * page + place in the page``; ``block_table [B, W]`` int32 names a request's pages in order (entries behind
 its length are not read), ``lengths [B]`` int32 its tokens, the new one among them.
 
-All work goes to the current stream; nothing but scratch memory (one buffer a stream) is kept between calls.
+All work goes to the current stream; nothing but scratch memory (one buffer a stream) is kept between calls.  Threads
+may share a stream: a call's kernels go out together (see ``_launching``).
 
 A call's integers and addresses reach the library as one block of 64-bit words: a decode step makes a call a
 layer, and converting two dozen arguments one by one costs more than the small kernels run.
@@ -20,6 +21,7 @@ from __future__ import annotations
 
 import functools
 import struct
+import threading
 from ctypes import c_char_p, c_int
 
 import torch
@@ -212,6 +214,10 @@ def read_slots(cache, slots: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
 _SHORT = 128
 _TWO_LAUNCHES = -100      # what the attention's entry point returns when the joining kernel went out too
 _scratch: dict = {}
+# Held from the choice of the scratch until the kernels that use it are in their stream: the foreign call lets other
+# threads run, and between the attention kernel and the joining one another call on the stream would overwrite the parts
+# (or put a larger buffer in this one's place).
+_launching = threading.Lock()
 _devices: dict = {}       # SMs, and the address of the word that kernels set when a bounded wait runs out
 
 
@@ -242,16 +248,15 @@ def _decode(q, nh, facts, block_table, lengths, scale, span, fused=None, out=Non
         facts_of_device = _devices[dev] = num_sms(dev), error_word(dev).data_ptr()
     sms, err = facts_of_device
     stream = _raw_stream(dev)
-    scratch, words = None, 0
-    if W * page > _SHORT:
-        words = scratch_words(B, nh, nkv, hd, sms)
-        scratch = _scratch_for(words, dev, stream)
-    rc = _function("quant_attention", "gf_quant_decode", (f"GF_HEAD_DIM={hd}",))(
-        _DECODE.pack(x, stride, code == 0, codes.data_ptr(), fp8, _at(scales, dev),
-                     _ints(block_table, (B, W), "block_table", dev), W, W, _ints(lengths, (B,), "lengths", dev), pages,
-                     out.data_ptr(), B, nh, nkv, page, span, fused is not None, table, rows, rot,
-                     fused is not None and fused[1], sms, 0 if scratch is None else scratch.data_ptr(), 4 * words,
-                     stream, err, scale))
+    words = scratch_words(B, nh, nkv, hd, sms) if W * page > _SHORT else 0
+    f = _function("quant_attention", "gf_quant_decode", (f"GF_HEAD_DIM={hd}",))
+    with _launching:
+        scratch = _scratch_for(words, dev, stream) if words else None
+        rc = f(_DECODE.pack(x, stride, code == 0, codes.data_ptr(), fp8, _at(scales, dev),
+                            _ints(block_table, (B, W), "block_table", dev), W, W, _ints(lengths, (B,), "lengths", dev),
+                            pages, out.data_ptr(), B, nh, nkv, page, span, fused is not None, table, rows, rot,
+                            fused is not None and fused[1], sms, 0 if scratch is None else scratch.data_ptr(), 4 * words,
+                            stream, err, scale))
     _Counter.launches += 2 if rc == _TWO_LAUNCHES else 1
     if rc and rc != _TWO_LAUNCHES:
         _ok(rc, "quant_cache.decode" if fused is None else "quant_cache.step")

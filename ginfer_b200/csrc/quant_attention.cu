@@ -307,8 +307,11 @@ template <bool TMA> struct Tiles {
         const bool there = c0 + lane >= lo && c0 + lane < end;
         const size_t at = (size_t)own.scales;
         const uint32_t odd = (uint32_t)at & 8u;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(smem_u32(scales + lane * 16)),
-                     "l"(at - odd), "r"(there ? (odd ? 16 : 8) : 0) : "memory");
+        if (there && at - odd < (size_t)a.scales)          // (the cache's first ones, where those bytes start before it)
+          *reinterpret_cast<float2*>(scales + lane * 16 + 8) = __ldcg(own.scales);
+        else
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(smem_u32(scales + lane * 16)),
+                       "l"(at - odd), "r"(there ? (odd ? 16 : 8) : 0) : "memory");
         scales[TILE * 16 + lane] = (uint8_t)odd;
       }
     }

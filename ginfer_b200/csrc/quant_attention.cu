@@ -578,7 +578,7 @@ quant_decode_kernel(const DecodeArgs a, const __grid_constant__ CUtensorMap map)
     Angles an;
     // the new token's row of keys (the last warp's, whose rows of q may not exist) and of values (the one before)
     const bool news = STEP && it.ends && warp >= WARPS - 2, keys = warp == WARPS - 1;
-    int new_page = 0, page_number = 0;
+    int new_page = 0, new_len = 0, page_number = 0;
     if (have) {
 #pragma unroll
       for (int i = 0; i < RW; ++i)
@@ -593,7 +593,7 @@ quant_decode_kernel(const DecodeArgs a, const __grid_constant__ CUtensorMap map)
             load_partners<T>(a, row + (size_t)(h0 + warp + i * WARPS) * HD, warp + i * WARPS < nrows, lane, y[i]);
           if (news && keys) load_partners<T>(a, new_at, true, lane, ny);
         }
-        if (news) new_page = page_in(a, fresh_index(tiles.tbl + logical_page(a, p)));
+        if (news) new_page = fresh_index(tiles.tbl + logical_page(a, p)), new_len = fresh_index(a.lengths + it.b);
       }
       if (cur.todo > 0) later_b = cur.b + 1 == a.B ? 0 : cur.b + 1, later_len = request_length(a, later_b);
       // (of the new token nothing is read)
@@ -680,15 +680,22 @@ quant_decode_kernel(const DecodeArgs a, const __grid_constant__ CUtensorMap map)
           turn_row(a, an, lane, nx, ny);
         }
         const RowScale rs = row_scale(row_top(nx), FP8);
-        const Place pl = place_of(a, kvh, new_page, p - logical_page(a, p) * a.page);
+        // (an entry that is no page, or a token behind the table's end: nowhere to write it to)
+        const bool stays = (unsigned)new_page < (unsigned)a.pages && new_len <= a.limit;
+        const Place pl = place_of(a, kvh, stays ? new_page : 0, p - logical_page(a, p) * a.page);
         const int which = keys ? 0 : 1;
         uint8_t* dst = const_cast<uint8_t*>(pl.codes) + (size_t)which * a.page * HD;
 #pragma unroll
         for (int i = 0; i < N; ++i)
-          if (i * 32 + lane < HD)
-            dst[i * 32 + lane] = fresh_row[which][i * 32 + lane] = (uint8_t)code_of(nx[i], rs, FP8);
-        if (lane == 0)
-          reinterpret_cast<float*>(const_cast<float2*>(pl.scales))[which] = fresh_scale[which] = rs.scale;
+          if (i * 32 + lane < HD) {
+            const uint8_t code = (uint8_t)code_of(nx[i], rs, FP8);
+            fresh_row[which][i * 32 + lane] = code;
+            if (stays) dst[i * 32 + lane] = code;
+          }
+        if (lane == 0) {
+          fresh_scale[which] = rs.scale;
+          if (stays) reinterpret_cast<float*>(const_cast<float2*>(pl.scales))[which] = rs.scale;
+        }
       }
 #pragma unroll
       for (int i = 0; i < RW; ++i) {

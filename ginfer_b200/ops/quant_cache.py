@@ -286,7 +286,8 @@ def step(qkv: torch.Tensor, nh: int, table, cache, block_table: torch.Tensor, le
          scale: float, window: int = 0, *, neighbours: bool = False) -> torch.Tensor:
     """What a decode step does to a layer's cache, in one launch: row ``b`` of ``qkv [B, (nh + 2 kv heads) *
     head size]`` is the last of request ``b``'s ``lengths[b]`` tokens; q and k are rotated, k and v written (as
-    :func:`write` does), and the token attends over the cache, itself among the keys (as :func:`decode`)."""
+    :func:`write` does: not where the table has no page of the cache for it, an entry outside the cache or a length beyond
+    ``W * page``), and the token attends over the cache, itself among the keys (as :func:`decode`)."""
     return _decode(qkv, nh, _cache(cache), block_table, lengths, scale, window, (table, neighbours))
 
 

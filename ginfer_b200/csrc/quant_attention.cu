@@ -22,11 +22,14 @@
 //  (With 8 query heads a kv head the operands of tcgen05 would be 128 rows of keys that have to be unpacked into
 //  shared memory as halves first, four times the bytes that this reads there.)
 //
-// Half precision holds q and the weights in 11 bits (a row of q is scaled by a power of two so that its
-// largest element is in [2^14, 2^15); a weight, p times its value row's scale, so that the largest value
-// scale seen so far gives [2^14, 2^15)): more than the 8 bits of a bfloat16 q and result.  For 32-bit q both
-// are the sum of two halves (22 bits), and tiles' products are added up outside the tensor cores.  Scores,
-// maxima, sums and O are 32-bit.
+// Half precision holds q and the weights in 11 bits, more than the 8 of a bfloat16 q and result.  A row of q is scaled
+// by a power of two so that its largest element is in [2^14, 2^15).  A weight is p times its value row's scale, and these
+// are scaled by powers of two, one for all heads that follows the largest value scale and one a head that follows its
+// largest weight, such that a head's largest weight so far is above 1 (2^7 as a rule) and all are below 2^15: one that
+// is small beside it is off by at most 2^-25 of it.  So neither a large value scale without weight nor a weight without
+// value takes bits from the others.  For 32-bit q both are the sum of two halves (22 bits, weights down to 2^-3 after
+// scaling; off by 2^-25 below), and tiles' products are added up outside the tensor cores.  Scores, maxima, sums and O
+// are 32-bit.
 //
 // A block is four warps, which take the tiles of its share of the work in turn (how it is shared out: see Cursor),
 // each through a ring of two stages of its own: nothing but an item's start and end synchronises the block, and an
@@ -131,6 +134,11 @@ struct DecodeArgs {
 __device__ __forceinline__ float fast_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float fast_log2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -376,14 +384,18 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
 }
 // what a float loses when it is rounded to a half
 __device__ __forceinline__ float half_rest(float x) { return x - __half2float(__float2half_rn(x)); }
-// Weights are p times a value's scale times 2^(f - 127).  p is at most 2^kSlack; with a scale's exponent (biased) e,
-// f <= kTop - e keeps the weight below 2^15.
+// p is 2^(score - m).  m + h, h of a head as a rule 0, is the whole number kSlack above the largest score that there was when
+// it was raised last.  Weights are p times a value's scale times 2^(f - 127), where f = kSafe - e with the largest
+// (biased) exponent e of the scales: below 2^15 for every p up to 1, and the largest at 2^7 or 2^6 when m is raised, if its
+// scale is the largest too.  Where the largest weight of a head would be below 1, its h takes it to [1, 2).
 constexpr float kSlack = 7.f;
-constexpr int kTop = 127 + 127 + 14 - 7;
+constexpr int kSafe = 127 + 127 + 14, kMostExtra = 100;
 // 2^(127 - f) for 7 <= f <= 254
 __device__ __forceinline__ float power_back(int f) {
   return __uint_as_float(f == 254 ? 0x00400000u : (uint32_t)(254 - f) << 23);
 }
+// The bits of the first power of two that is too large a scale for a weight of p = 1 and f (with its head's h).
+__device__ __forceinline__ uint32_t scale_limit(int f) { return (uint32_t)min(kSafe + 1 - f, 255) << 23; }
 
 // ------------------------------------------------------------------------------------- q, and the new token
 // A lane's channels of head rows: lane, lane + 32, ...  Everything is asked for before anything is used.
@@ -564,6 +576,7 @@ quant_decode_kernel(const DecodeArgs a, const __grid_constant__ CUtensorMap map)
 
   float o[NT][MT][4], m[NT][2], l[NT][2];
   int f = 254;                             // weights are multiplied by 2^(f - 127)
+  uint32_t extra = 0, too_large = 0;       // the heads' h, 8 bits each; scale_limit of f and the largest of them
   int at_stage = 0, to_stage = STAGES - 1;
   Item it, done;
   bool have = next_item(it), had = false;
@@ -652,9 +665,9 @@ quant_decode_kernel(const DecodeArgs a, const __grid_constant__ CUtensorMap map)
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
           // (a warp without tiles has sums of zero; one whose scores are no numbers passes that on)
-          const float e = sm[w][r] == -INFINITY ? 0.f : fast_exp2(sm[w][r] - top), eb = e * back[w];
+          const float e = sm[w][r] == -INFINITY ? 0.f : fast_exp2(sm[w][r] - top), b = back[w];
           const float2 v = *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(ring + so_at[w]) + r * OROW + c);
-          sum += e * sl[w][r], v0 += eb * v.x, v1 += eb * v.y;
+          sum += e * sl[w][r], v0 += e * v.x * b, v1 += e * v.y * b;
         }
         const float inv = __fdividef(1.f, sum);
         v0 *= inv, v1 *= inv;
@@ -743,7 +756,7 @@ quant_decode_kernel(const DecodeArgs a, const __grid_constant__ CUtensorMap map)
 #pragma unroll
       for (int i = 0; i < MT; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
     }
-    f = 254;
+    f = 254, extra = 0, too_large = scale_limit(254);
 
     // ---- where the block goes next (its pages are there when this item's tiles are done)
     done = it, had = true;
@@ -863,8 +876,8 @@ quant_decode_kernel(const DecodeArgs a, const __grid_constant__ CUtensorMap map)
           if (!seen[i]) sc[i] = make_float2(0.f, 0.f);
         }
       }
-      // Scores in units of log2.  m and f are raised only when a score is 2^7 times what m stands for, or a value's
-      // scale above what f stands for: a weight is below 2^15 until then.
+      // Scores in units of log2.  m, f and h are looked at again only when a score is above m, or a value's scale too
+      // large for a p of 1.
       bool above = false;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -878,41 +891,56 @@ quant_decode_kernel(const DecodeArgs a, const __grid_constant__ CUtensorMap map)
             r = seen[i] ? r * sc[i].x : -INFINITY;
             top = fmaxf(top, r);
           }
-          above |= top > m[n][j] + kSlack;
+          above |= top > m[n][j];
         }
-      // (a scale's bits against those of the first power of two that is too large for f)
       uint32_t vtop = 0;
 #pragma unroll
       for (int i = 0; i < 2 * TK; ++i) {
         const uint32_t bits = __float_as_uint(sc[i].y);
         vtop = max(vtop, bits < 0x7f800000u ? bits : 0u);
       }
-      above |= vtop >= (uint32_t)(kTop - f + 1) << 23;
+      above |= vtop >= too_large;
       if (__any_sync(0xffffffffu, above)) {
-        const int fn = min(f, kTop - (int)(__reduce_max_sync(0xffffffffu, vtop) >> 23));
-        const float shrink = fn == f ? 1.f : f - fn > 126 ? 0.f : __uint_as_float((uint32_t)(127 + fn - f) << 23);
-        f = fn;
+        const int f_new = min(f, kSafe - (int)(__reduce_max_sync(0xffffffffu, vtop) >> 23));
+        float size[2 * TK];
+#pragma unroll
+        for (int i = 0; i < 2 * TK; ++i) size[i] = fast_log2(sc[i].y);
+        uint32_t h_new = 0, h_most = 0;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           float corr[2];
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            float top = -INFINITY;
+            float top = -INFINITY, weight = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 2 * TK; ++i) top = fmaxf(top, s[i >> 1][n][2 * (i & 1) + j]);
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-            const float mn = fmaxf(m[n][j], top);
-            corr[j] = mn == m[n][j] ? 1.f : fast_exp2(m[n][j] - mn);
-            l[n][j] *= corr[j];
-            corr[j] *= shrink;
-            m[n][j] = mn;
+            for (int i = 0; i < 2 * TK; ++i) {
+              const float r = s[i >> 1][n][2 * (i & 1) + j];
+              top = fmaxf(top, r), weight = fmaxf(weight, r + size[i]);
+            }
+#pragma unroll
+            for (int lanes = 4; lanes <= 16; lanes *= 2) {
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, lanes));
+              weight = fmaxf(weight, __shfl_xor_sync(0xffffffffu, weight, lanes));
+            }
+            const int h = extra >> (8 * (2 * n + j)) & 255u;
+            const float highest = m[n][j] + (float)h, mn = top > highest ? ceilf(top + kSlack) : highest;
+            const float rise = mn == highest ? 0.f : mn - highest;
+            // what the weights so far lose, in whole powers of two, h may give them; need is what takes this tile's
+            // largest to [1, 2)
+            const int need = 127 - (int)floorf(fminf(fmaxf(weight - mn, -127.f), 120.f));
+            const int both = min((int)fminf((float)(f + h) + rise, (float)(f_new + kMostExtra)), max(f_new, need));
+            const uint32_t now = (uint32_t)(both - f_new);
+            const float to = mn - (float)now, less = to == m[n][j] ? 0.f : m[n][j] - to;
+            l[n][j] *= fast_exp2(less);
+            corr[j] = fast_exp2(less + (float)(f_new - f));
+            m[n][j] = to;
+            h_new |= now << (8 * (2 * n + j)), h_most = max(h_most, now);
           }
 #pragma unroll
           for (int i = 0; i < MT; ++i)
             o[n][i][0] *= corr[0], o[n][i][1] *= corr[1], o[n][i][2] *= corr[0], o[n][i][3] *= corr[1];
         }
+        f = f_new, extra = h_new, too_large = scale_limit(f + (int)h_most);
       }
       const float up = __uint_as_float((uint32_t)f << 23);
       uint32_t P[TK][PARTS][NT][2];

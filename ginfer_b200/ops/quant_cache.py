@@ -297,6 +297,15 @@ def step(qkv: torch.Tensor, nh: int, table, cache, block_table: torch.Tensor, le
 READ_AT_ONCE = 32768
 
 
+def portion_pages(starts, counts, page: int, span: int, W: int, capturing: bool = False) -> list[int]:
+    """Pages that the portions' tokens see, from the first one's first key (without a window: from the request's) to the
+    last one: portion ``i`` is the tokens ``starts[i] .. starts[i] + counts[i] - 1``.  ``capturing``: the most that there are
+    wherever the portions start, in tables of ``W`` pages."""
+    if capturing:
+        return [W if span <= 0 else min(W, (span + n - 3) // page + 2) for n in counts]
+    return [-(-(s + n) // page) - (max(0, s - span + 1) // page if span > 0 else 0) for s, n in zip(starts, counts)]
+
+
 def portion_groups(pages_of: list[int], page: int) -> list[tuple[int, int]]:
     """Runs ``[i, j)`` of neighbouring requests whose dense copies (``pages_of`` pages each) fit READ_AT_ONCE together;
     a longer request is alone."""
@@ -327,41 +336,52 @@ def attention(qkv: torch.Tensor, nh: int, table, cache, block_table: torch.Tenso
     if ctx.decode_only:
         return decode(q, nh, cache, block_table, ctx.kv_lens, scale, span)
     # single tokens first (as the scheduler orders them), the portions behind them
-    B, q_lens, nd = ctx.num_seqs, ctx.q_lens_host, 0
+    B, q_lens, q_starts, nd = ctx.num_seqs, ctx.q_lens_host, ctx.q_starts_host, 0
     while nd < B and q_lens[nd] == 1:
         nd += 1
     out = torch.empty_like(q)
     if nd:
         _decode(q[:nd], nh, _cache(cache), block_table[:nd], ctx.kv_lens[:nd], scale, span, out=out[:nd])
     cu, W = ctx.cu_seqlens_q, block_table.shape[1]
-    # (a captured step is replayed with other lengths: there every request may fill its table)
-    pages_of = [W if ctx.capturing else -(-(s + n) // page) for s, n in
-                zip(ctx.q_starts_host[nd:], q_lens[nd:])]
+    # (a captured step is replayed with other starts)
+    pages_of = portion_pages(q_starts[nd:], q_lens[nd:], page, span, W, ctx.capturing)
     # what the groups' calls take besides the cache is the same for all of the step's layers with this mask (a graph
     # works it out itself)
     same = ("read back", page, span, W, _capturing())
     groups = ctx.extras.get(same)
     if groups is None:
         groups = ctx.extras[same] = []
-        first, row = None, nd
+        first = below = None
+        row = nd
         if span:
             # the first key that each portion's first token sees
             p = ctx.positions[cu[nd:B].long()]
             first = (p - (span - 1)).clamp(min=0) if span > 0 else p // -span * -span
+        if span > 0:
+            below = first // page            # pages that it does not see any more: nothing of them is read back
         for i, j in portion_groups(pages_of, page):
             wide, n, b0, b1 = max(pages_of[i:j]), j - i, nd + i, nd + j
             rows = sum(q_lens[b0:b1])
-            groups.append((b0, b1, row, rows, wide, ctx.kv_lens[b0:b1], None if first is None else first[i:j],
-                           torch.arange(n * wide, dtype=_int32, device=q.device).view(n, wide), cu[b0:b1 + 1],
-                           ctx.seq_of_token[row:row + rows] - b0 if qkv.dtype is _float32 else None, max(q_lens[b0:b1])))
+            at = torch.arange(wide, dtype=_int32, device=q.device)
+            lens, low, columns, pos = ctx.kv_lens[b0:b1], None if first is None else first[i:j], None, None
+            seq = ctx.seq_of_token[row:row + rows] - b0 if qkv.dtype is _float32 else None
+            if seq is not None:
+                pos = ctx.positions[row:row + rows]
+            if below is not None:            # (positions are counted from the first page that is read back)
+                gone = below[i:j] * page
+                lens, low, columns = lens - gone, low - gone, (below[i:j, None] + at).clamp_(max=W - 1).long()
+                pos = None if seq is None else pos - gone[seq.long()]
+            own = torch.arange(n * wide, dtype=_int32, device=q.device).view(n, wide)
+            groups.append((b0, b1, row, rows, wide, columns, lens, low, own, cu[b0:b1 + 1], seq, pos, max(q_lens[b0:b1])))
             row += rows
-    for b0, b1, row, rows, wide, lens, low, own, cu_own, seq, most in groups:
+    for b0, b1, row, rows, wide, columns, lens, low, own, cu_own, seq, pos, most in groups:
         n = b1 - b0
-        dense = read(cache, block_table[b0:b1, :wide].contiguous(), lens, qkv.dtype, low)
+        seen = block_table[b0:b1, :wide].contiguous() if columns is None else block_table[b0:b1].gather(1, columns)
+        dense = read(cache, seen, lens, qkv.dtype, low)
         pages = dense.view(2, n * wide, page, nkv, hd)
         if qkv.dtype is _float32:
-            out[row:row + rows] = paged_attention_simt(q[row:row + rows], pages, own, seq, ctx.positions[row:row + rows],
-                                                       nh, nkv, hd, scale, span, page)
+            out[row:row + rows] = paged_attention_simt(q[row:row + rows], pages, own, seq, pos, nh, nkv, hd, scale, span,
+                                                       page)
         else:
             args = (q, pages, own, cu_own, lens, n, most, nh, nkv, hd, scale, span, page)
             if most < attention_bf16.TC_MIN_QUERY_ROWS or attention_bf16.prefill_tc(*args, out=out) is None:

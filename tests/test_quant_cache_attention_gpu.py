@@ -98,3 +98,27 @@ def test_attention(dtype, writes, capturing, span, step):
     check_attention(got[:front], want[:front], top[:front], dtype)
     lim = 2.0 ** -8 * (read.abs() + read_top) if dtype == BF16 else 2e-5 * read_top + 0 * read
     assert torch.isfinite(got).all() and ((got.double() - read).abs() <= lim)[front:].all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("capturing", [False, True])
+def test_memory_of_a_window(dtype, capturing):
+    """A portion far into a long prompt takes memory for what its window sees, not for the prompt."""
+    nh, nkv, hd, page, start, n, span = 28, 4, 128, 16, 20000, 200, 1024
+    g = torch.Generator(device=DEV).manual_seed(1)
+    t, pages, _ = tables((start + n,), page, g)
+    t[0, :(start - span + 1) // page] = -1
+    cache = random_cache("int8", pages, nkv, page, hd, g)
+    x = torch.randn(n, (nh + 2 * nkv) * hd, generator=g, device=DEV).to(dtype)
+    ctx = context((start,), (n,), dtype, capturing)
+    slots = (t[0, ctx.positions.long() // page].long() * page + ctx.positions % page).int()
+    qc().attention(x, nh, None, cache, t, ctx, hd ** -0.5, span, slots)
+    torch.cuda.synchronize()
+    ctx.extras.clear()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    qc().attention(x, nh, None, cache, t, ctx, hd ** -0.5, span, slots)
+    took = torch.cuda.max_memory_allocated() - before
+    dense = 2 * (span + n + 2 * page) * nkv * hd * x.element_size()
+    rows = 2 * n * nh * hd * x.element_size()                      # q, and the result
+    assert took <= 2 * rows + dense + (1 << 20), (took, dense, rows)

@@ -101,8 +101,9 @@ class ModelRunner:
         """Pages for every cache group.  A group never gets more than it can hold at once
         (:meth:`GroupLayout.pages_for`: a windowed group needs few).  ``num_pages``: a count for
         every group, or one per group, or ``None``: the share ``utilization`` of the free device
-        memory is divided so that the groups can hold the same number of tokens, what the
-        windowed groups do not need going to the others."""
+        memory (less what prompt portions read back of a cache of 8 bits) is divided so that the
+        groups can hold the same number of tokens, what the windowed groups do not need going to
+        the others."""
         caps = [g.pages_for(self.max_num_seqs, self.max_seq_len, self.max_num_batched_tokens,
                             self.page_size) for g in self.groups]
         if num_pages is not None:
@@ -112,7 +113,7 @@ class ModelRunner:
                 raise ValueError(f"{len(asked)} page counts for {len(self.groups)} cache groups")
             return [max(1, min(int(n), cap)) for n, cap in zip(asked, caps)]
         free, _total = torch.cuda.mem_get_info(self.device)
-        budget = int(free * utilization)
+        budget = int(max(0, free - self._read_back_bytes(itemsize)) * utilization)
         per_page = [g.bytes_per_page(self.page_size, itemsize) for g in self.groups]
         counts = [0] * len(self.groups)
         open_groups = list(range(len(self.groups)))
@@ -128,6 +129,15 @@ class ModelRunner:
                 budget -= caps[g] * per_page[g]
                 open_groups.remove(g)
         return counts
+
+    def _read_back_bytes(self, itemsize: int) -> int:
+        """Memory for the dense keys and values of a step's portions, a layer at a time; steps that are
+        replayed from graphs have theirs in the graphs' pool, beside the eager ones'."""
+        from ..ops import quant_cache
+        most = max((quant_cache.read_back_bytes(*g.planes[0], itemsize, self.page_size, self.max_seq_len,
+                                                min(self.max_num_batched_tokens, self.max_seq_len), g.window)
+                    for g in self.groups if g.kept), default=0)
+        return most if self.enforce_eager else 2 * most
 
     # ------------------------------------------------------------------ requests
     def end(self, request_id) -> None:

@@ -306,6 +306,16 @@ def portion_pages(starts, counts, page: int, span: int, W: int, capturing: bool 
     return [-(-(s + n) // page) - (max(0, s - span + 1) // page if span > 0 else 0) for s, n in zip(starts, counts)]
 
 
+def read_back_bytes(kv_heads: int, head_dim: int, itemsize: int, page: int, longest: int, portion: int, window: int = 0
+                    ) -> int:
+    """The most memory that a layer's portions take for keys and values read back (the next layer's take the same):
+    requests of up to ``longest`` tokens, portions of up to ``portion``."""
+    tokens = -(-longest // page) * page
+    if window:
+        tokens = min(tokens, portion_pages([0], [portion], page, window, tokens // page, capturing=True)[0] * page)
+    return 2 * max(READ_AT_ONCE, tokens) * kv_heads * head_dim * itemsize
+
+
 def portion_groups(pages_of: list[int], page: int) -> list[tuple[int, int]]:
     """Runs ``[i, j)`` of neighbouring requests whose dense copies (``pages_of`` pages each) fit READ_AT_ONCE together;
     a longer request is alone."""

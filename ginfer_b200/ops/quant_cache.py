@@ -387,8 +387,7 @@ def attention(qkv: torch.Tensor, nh: int, table, cache, block_table: torch.Tenso
     for b0, b1, row, rows, wide, columns, lens, low, own, cu_own, seq, pos, most in groups:
         n = b1 - b0
         seen = block_table[b0:b1, :wide].contiguous() if columns is None else block_table[b0:b1].gather(1, columns)
-        dense = read(cache, seen, lens, qkv.dtype, low)
-        pages = dense.view(2, n * wide, page, nkv, hd)
+        pages = read(cache, seen, lens, qkv.dtype, low).view(2, n * wide, page, nkv, hd)
         if qkv.dtype is _float32:
             out[row:row + rows] = paged_attention_simt(q[row:row + rows], pages, own, seq, pos, nh, nkv, hd, scale, span,
                                                        page)
@@ -396,4 +395,6 @@ def attention(qkv: torch.Tensor, nh: int, table, cache, block_table: torch.Tenso
             args = (q, pages, own, cu_own, lens, n, most, nh, nkv, hd, scale, span, page)
             if most < attention_bf16.TC_MIN_QUERY_ROWS or attention_bf16.prefill_tc(*args, out=out) is None:
                 attention_bf16.prefill(*args, out=out)
+            del args
+        del pages                            # (the next group's take their place)
     return out

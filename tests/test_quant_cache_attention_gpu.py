@@ -122,3 +122,26 @@ def test_memory_of_a_window(dtype, capturing):
     dense = 2 * (span + n + 2 * page) * nkv * hd * x.element_size()
     rows = 2 * n * nh * hd * x.element_size()                      # q, and the result
     assert took <= 2 * rows + dense + (1 << 20), (took, dense, rows)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_memory_of_several_groups(dtype):
+    """Requests that are read back one by one take the memory of one."""
+    nh, nkv, hd, page, starts, counts = 14, 2, 64, 16, (20000, 17000, 19000), (70, 70, 70)
+    g = torch.Generator(device=DEV).manual_seed(2)
+    lens = [s + n for s, n in zip(starts, counts)]
+    t, pages, _ = tables(lens, page, g)
+    cache = random_cache("fp8", pages, nkv, page, hd, g)
+    x = torch.randn(sum(counts), (nh + 2 * nkv) * hd, generator=g, device=DEV).to(dtype)
+    ctx = context(starts, counts, dtype)
+    slots = (t[ctx.seq_of_token.long(), ctx.positions.long() // page].long() * page + ctx.positions % page).int()
+    qc().attention(x, nh, None, cache, t, ctx, hd ** -0.5, 0, slots)
+    torch.cuda.synchronize()
+    ctx.extras.clear()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    qc().attention(x, nh, None, cache, t, ctx, hd ** -0.5, 0, slots)
+    took = torch.cuda.max_memory_allocated() - before
+    most = qc().read_back_bytes(nkv, hd, x.element_size(), page, max(lens), max(counts))
+    rows = 2 * len(x) * nh * hd * x.element_size()                 # q, and the result
+    assert took <= 2 * rows + most + (1 << 20), (took, most, rows)

@@ -135,11 +135,5 @@ __device__ __forceinline__ void values4(uint32_t w, int fp8, float* v) {
     for (int e = 0; e < 4; ++e) v[e] = (float)(int8_t)(w >> (8 * e));
   }
 }
-__device__ __forceinline__ void values16(const uint4& raw, int fp8, float (&v)[16]) {
-  values4(raw.x, fp8, v);
-  values4(raw.y, fp8, v + 4);
-  values4(raw.z, fp8, v + 8);
-  values4(raw.w, fp8, v + 12);
-}
 
 }  // namespace gf

@@ -147,10 +147,15 @@ quant_write_kernel(const T* __restrict__ qkv, int row_stride, int tokens, int nh
 template <typename T, int LANES>
 int launch_write(const void* qkv, int row_stride, int tokens, int nh, int nkv, int hd, const float* table,
                  int table_rows, int rot, int neighbours, const int* positions, const int* slots, void* q_out,
-                 uint8_t* codes, int fp8, float* scales, int page, int num_slots, int vec,
+                 uint8_t* codes, int fp8, float* scales, int page, int num_slots, int vec, int sms,
                  cudaStream_t stream) {
   const int heads = nh + 2 * nkv;
-  const bool one = (long long)tokens * heads * LANES <= 148 * 1024;
+  // One head a group while that is at most two rounds of 1,024 threads an SM: more groups, so that loads are under way
+  // everywhere; beyond it, two heads read a position's angles once.  One / two, us: 28 + 2 x 4 heads of 128 in bfloat16 at a
+  // quarter round 2.9 / 3.4, one round (526 tokens) 3.8 / 4.6, two 5.6 / 5.6, three 7.5 / 7.4, eight 18.7 / 16.3; 14 + 2 x 2 of 64
+  // 4.0 / 4.9 at one, 5.9 / 6.0 at two, 8.1 / 8.2 at three, 20.6 / 17.8 at eight; 12 + 2 x 2 of 128 in 32 bits 8.2 / 8.5 at two,
+  // 12.0 / 13.0 at three, 28.0 / 27.9 at eight.
+  const bool one = (long long)tokens * heads * LANES <= 2048LL * sms;
   const int hu = one ? 1 : 2, sets = (heads + hu - 1) / hu, each = WRITE_THREADS / LANES;
   if (sets > 65535) return -5;
   const dim3 grid((unsigned)((tokens + each - 1) / each), (unsigned)sets);
@@ -271,15 +276,16 @@ struct WriteCall {
   float* scales;
   long long page, pages;
   cudaStream_t stream;
+  long long sms;
 };
-static_assert(sizeof(WriteCall) == 20 * 8, "the caller packs it");
+static_assert(sizeof(WriteCall) == 21 * 8, "the caller packs it");
 
 GF_EXPORT int gf_quant_write(const WriteCall* call) {
   const WriteCall& c = *call;
   if (c.tokens <= 0) return c.tokens < 0 ? -3 : 0;
   if (c.hd % 16 || c.hd < 16 || c.hd > 256 || c.nh < 1 || c.nkv < 1 || c.nh > 1 << 20 || c.nkv > 1 << 20 || c.page < 1 ||
       c.pages < 0 || c.page * c.pages > 0x7fffffffLL || c.rot < 0 || c.rot % 2 || c.rot > c.hd ||
-      (c.rot && (!c.table || c.table_rows < 1)) || c.tokens > 0x7fffffff || c.row_stride > 0x7fffffff || c.row_stride < 0)
+      (c.rot && (!c.table || c.table_rows < 1)) || c.tokens > 0x7fffffff || c.row_stride > 0x7fffffff || c.row_stride < 0 || c.sms < 1 || c.sms > 1 << 20)
     return -3;
   const size_t es = c.dtype == GF_F32 ? 4 : 2;
   if ((size_t)c.codes % 16 || (size_t)c.scales % 8) return -3;
@@ -291,7 +297,7 @@ GF_EXPORT int gf_quant_write(const WriteCall* call) {
     const auto run = [&](auto launch) {
       return launch(c.qkv, (int)c.row_stride, (int)c.tokens, (int)c.nh, (int)c.nkv, (int)c.hd, c.table, (int)c.table_rows,
                     (int)c.rot, c.neighbours != 0, c.positions, c.slots, c.q_out, (uint8_t*)c.codes, (int)c.fp8, c.scales,
-                    (int)c.page, (int)(c.page * c.pages), vec, c.stream);
+                    (int)c.page, (int)(c.page * c.pages), vec, (int)c.sms, c.stream);
     };
     if (c.hd <= 64) return run(launch_write<T, 4>);
     if (c.hd <= 128) return run(launch_write<T, 8>);

@@ -34,7 +34,7 @@ KINDS = {"int8": torch.int8, "fp8": torch.float8_e4m3fn}
 MAX_HEAD_DIM = 256
 _FP8 = {torch.int8: 0, torch.float8_e4m3fn: 1}
 _CODE = {torch.float32: 0, torch.bfloat16: 1}
-_WRITE, _READ, _DECODE = struct.Struct("=20q"), struct.Struct("=17q"), struct.Struct("=27qd")
+_WRITE, _READ, _DECODE = struct.Struct("=21q"), struct.Struct("=17q"), struct.Struct("=27qd")
 _current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 _capturing = torch.cuda.is_current_stream_capturing
 _int32, _float32 = torch.int32, torch.float32
@@ -98,6 +98,17 @@ def _device(codes) -> int:
     if device < 0 or device != _current_device():
         _elsewhere(codes)
     return device
+
+
+_devices: dict = {}
+
+
+def _of_device(device: int):
+    """(SMs, the address of the word that kernels set when a bounded wait runs out)."""
+    facts = _devices.get(device)
+    if facts is None:
+        facts = _devices[device] = num_sms(device), error_word(device).data_ptr()
+    return facts
 
 
 def _at(t, device: int):
@@ -167,7 +178,7 @@ def write(qkv: torch.Tensor, nh: int, table, positions: torch.Tensor, slots: tor
     f = _function("quant_cache", "gf_quant_write")
     rc = f(_WRITE.pack(x, stride, code, T, nh, nkv, hd, at, rows, rot, neighbours,
                        _ints(positions, (T,), "positions", dev), _ints(slots, (T,), "slots", dev), q.data_ptr(),
-                       codes.data_ptr(), fp8, _at(scales, dev), page, pages, _raw_stream(dev)))
+                       codes.data_ptr(), fp8, _at(scales, dev), page, pages, _raw_stream(dev), _of_device(dev)[0]))
     _Counter.launches += 1
     if rc:
         _ok(rc, "quant_cache.write")
@@ -218,7 +229,6 @@ _scratch: dict = {}
 # threads run, and between the attention kernel and the joining one another call on the stream would overwrite the parts
 # (or put a larger buffer in this one's place).
 _launching = threading.Lock()
-_devices: dict = {}       # SMs, and the address of the word that kernels set when a bounded wait runs out
 
 
 def _scratch_for(words: int, device: int, stream: int) -> torch.Tensor:
@@ -243,10 +253,7 @@ def _decode(q, nh, facts, block_table, lengths, scale, span, fused=None, out=Non
     table, rows, rot = (0, 0, 0) if fused is None else _angles(fused[0], hd, dev)
     if out is None:
         out = q.new_empty(B, nh * hd)
-    facts_of_device = _devices.get(dev)
-    if facts_of_device is None:
-        facts_of_device = _devices[dev] = num_sms(dev), error_word(dev).data_ptr()
-    sms, err = facts_of_device
+    sms, err = _of_device(dev)
     stream = _raw_stream(dev)
     words = scratch_words(B, nh, nkv, hd, sms) if W * page > _SHORT else 0
     f = _function("quant_attention", "gf_quant_decode", (f"GF_HEAD_DIM={hd}",))

@@ -102,8 +102,14 @@ constexpr int kLeastTiles = 2 * WARPS / TK;
 // fit the GPU allow two or more and a request that fills its table keeps them at most as much longer than equal runs would
 // as the joining kernel costs, kUnevenKeys keys a block: 8 requests of 576 keys, tables of 4,096, 12 query heads on 2 kv
 // heads of 128: 10.9 us after 16.7 with equal runs; one of 8,000 keys, where the rule says equal runs: 16.3 after 19.0.
-// kShortKeys keys are one block's work.  Where there are as many items as SMs, up to kMiddleKeys are, too.
-constexpr int kShortKeys = 128, kMiddleKeys = 1024, kMostOfCluster = 8, kUnevenKeys = 700;
+// kShortKeys keys are one block's work: parts that meet cost more than their keys.  One block / as the rule goes on above it, us,
+// full tables of 256 keys: 28 heads on 4 kv heads of 128, one request 7.2 / 8.2, eight 7.4 / 8.3; 14 on 2 of 64, one 6.4 / 6.7,
+// 64 6.8 / 8.3; 32 on 2 of 128, eight 9.3 / 10.5; 32-bit q, 28 on 4 of 128, 32 requests 8.2 / 10.8; 8 on 2 of 256, eight
+// 10.4 / 9.8; of 384 keys 8.3 / 7.7, 8.6 / 8.2, 7.5 / 6.6, 8.1 / 10.0 (the first four).
+// Where there are as many items as SMs, up to kMiddleKeys are one block's, too.  One block / equal runs, us, 28 heads on 4 of 128,
+// 128 requests of 102 to 1,024 keys, tables of 1,024 28.0 / 33.1, all full 35.5 / 34.1; to 1,536 36.0 / 38.4, 47.7 / 43.0; to 2,048
+// 44.2 / 44.4, 59.3 / 55.1; 14 on 2 of 64, 256 requests, tables of 1,024 19.4 / 25.4, 37.5 / 47.1; 2,048 32.1 / 32.9, 69.5 / 83.7.
+constexpr int kShortKeys = 256, kMiddleKeys = 1024, kMostOfCluster = 8, kUnevenKeys = 700;
 constexpr int kMostBlocks = 8;          // of the blocks that fit an SM, so many are counted on
 
 struct DecodeArgs {

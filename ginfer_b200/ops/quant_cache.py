@@ -222,7 +222,7 @@ def read_slots(cache, slots: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
 
 
 # Where tables hold at most this many tokens the kernel needs no scratch (it has the same line: kShortKeys).
-_SHORT = 128
+_SHORT = 256
 _TWO_LAUNCHES = -100      # what the attention's entry point returns when the joining kernel went out too
 _scratch: dict = {}
 # Held from the choice of the scratch until the kernels that use it are in their stream: the foreign call lets other

@@ -33,3 +33,12 @@ def test_rules_follow_the_device(monkeypatch, sms):
     qc.decode(torch.zeros(1, 256), 4, cache, i32(1, 20), i32(1), 1.0)
     assert qc._WRITE.unpack(calls["gf_quant_write"])[-2:] == (5, sms)
     assert qc._DECODE.unpack(calls["gf_quant_decode"])[22] == sms
+
+
+def test_the_line_of_short_tables():
+    """Both sides of the call know from which width on the kernel needs scratch memory."""
+    import os
+    import re
+    from ginfer_b200.ops.build import CSRC_DIR
+    with open(os.path.join(CSRC_DIR, "quant_attention.cu")) as f:
+        assert int(re.search(r"\bkShortKeys = (\d+)", f.read())[1]) == qc._SHORT

@@ -51,7 +51,7 @@ def test_place_of_the_scratch(library):
     buf = qc._scratch["cpu", 0]
     assert library.calls == [(buf.data_ptr(), 4 * qc.scratch_words(1, 4, 2, 64, 148))]
     assert struct.calcsize("=%dq" % SCRATCH) == 8 * SCRATCH
-    # tables of at most 128 tokens take none
+    # the shortest tables take none
     qc.decode(torch.zeros(1, 256), 4, cache, torch.zeros(1, 8, dtype=torch.int32), torch.zeros(1, dtype=torch.int32), 1.0)
     assert library.calls[1] == (0, 0)
 

@@ -142,7 +142,9 @@ def weight_bytes(c, layers: int, itemsize: int = 2) -> int:
     return (layers * per_layer + h + head) * itemsize
 
 
-def kv_bytes_per_token(c, layers: int, itemsize: int = 2) -> int:
+def kv_bytes_per_token(c, layers: int, itemsize: int = 2, kept: str = "auto") -> int:
+    if kept != "auto":                     # 8-bit codes and a 32-bit scale a row
+        return layers * 2 * c["num_key_value_heads"] * (c["head_dim"] + 4)
     return layers * 2 * c["num_key_value_heads"] * c["head_dim"] * itemsize
 
 
@@ -676,7 +678,7 @@ REF256_PUBLISHED = {"hardware": "A40", "prefill_tok_s": 31590.0, "decode_tok_s":
 
 
 def run_long_context(shape: str, layers: int | None, context: int = 32768,
-                     portion: int | None = None) -> int:
+                     portion: int | None = None, kept: str = "auto") -> int:
     """One prompt of ``context`` tokens fed in portions of 2,048 (``--portion``: another size; each portion timed on the device
     with CUDA events; the whole prompt three times, the last pass reported: the first two let the
     portions' CUDA graphs be captured), then single tokens decoded
@@ -696,7 +698,7 @@ def run_long_context(shape: str, layers: int | None, context: int = 32768,
     V, portion, B = cfg["vocab_size"], int(portion or PREFILL_TOKENS), 8
     eng = Engine(config=cfg, dtype="bfloat16", max_num_seqs=B, max_seq_len=context + 128,
                  max_num_batched_tokens=portion, kvcache_block_size=PAGE,
-                 num_kvcache_blocks=B * ((context + 128) // PAGE + 2))
+                 num_kvcache_blocks=B * ((context + 128) // PAGE + 2), kv_cache_dtype=kept)
     runner = eng.runner
     peaks, peaks_from = load_peaks()
     g = torch.Generator().manual_seed(1)
@@ -750,11 +752,12 @@ def run_long_context(shape: str, layers: int | None, context: int = 32768,
         stop.record()
         torch.cuda.synchronize()
         ms = start.elapsed_time(stop) / 32
-        nbytes = weight_bytes(cfg, L) + batch * (context + 24) * kv_bytes_per_token(cfg, L)
+        nbytes = weight_bytes(cfg, L) + batch * (context + 24) * kv_bytes_per_token(cfg, L, kept=kept)
         decode[f"b{batch}"] = {"tok_s": round(batch / (ms * 1e-3), 1), "ms": round(ms, 4),
                                "frac": round(nbytes / (ms * 1e-3) / 1e9 / peaks["hbm_gbs"], 4)}
     print(json.dumps({"scenario": "longctx", "model": SHAPE_NAMES[shape], "layers_run": L,
                       "layers_config": full_layers, "context": context, "kv_block": PAGE,
+                      "kv_cache_dtype": kept, "memory_gb": round(torch.cuda.max_memory_allocated() / 1e9, 2),
                       "prefill": prefill, "decode": decode, "peaks": peaks_from}))
     return 0
 
@@ -796,7 +799,7 @@ def scenario_plan(name: str, shape: str, layers: int | None):
     return cfg, full_layers, prompts, params, kwargs
 
 
-def run_scenario(name: str, shape: str, layers: int | None) -> int:
+def run_scenario(name: str, shape: str, layers: int | None, kept: str = "auto") -> int:
     """The serving workloads the baseline names beside the headline, through the Python entry
     point (scheduler, chunked prompts, decode graphs), wall clock, third pass reported (the first
     two capture graphs: of decode steps at first sight, of steps with portions at second).  ``serve64``: continuous batching of 64 requests, prompts of 128..2048
@@ -813,7 +816,7 @@ def run_scenario(name: str, shape: str, layers: int | None) -> int:
 
     from ginfer_b200.engine.llm import Engine
     cfg, full_layers, prompts, params, kwargs = scenario_plan(name, shape, layers)
-    eng = Engine(config=cfg, dtype="bfloat16", kvcache_block_size=PAGE, **kwargs)
+    eng = Engine(config=cfg, dtype="bfloat16", kvcache_block_size=PAGE, kv_cache_dtype=kept, **kwargs)
     result = None
     for _ in range(3):
         torch.cuda.synchronize()
@@ -824,7 +827,7 @@ def run_scenario(name: str, shape: str, layers: int | None) -> int:
         dt, steps = time.perf_counter() - t0, eng.runner.steps_run - s0
         tin, tout = sum(map(len, prompts)), sum(map(len, outs))
         result = {"scenario": name, "model": SHAPE_NAMES[shape], "layers_run": cfg["num_hidden_layers"],
-                  "layers_config": full_layers, "requests": len(prompts), "prompt_tokens": tin,
+                  "layers_config": full_layers, "kv_cache_dtype": kept, "requests": len(prompts), "prompt_tokens": tin,
                   "generated_tokens": tout, "seconds": round(dt, 4), "steps": steps,
                   "ms_per_step": round(1e3 * dt / steps, 3),
                   "total_tok_s": round((tin + tout) / dt, 1),
@@ -880,6 +883,8 @@ def main() -> int:
     ap.add_argument("--design", choices=["vilepel", "zolapel", "pimidra", "bapivik", "lasizen", "daburax"],
                     default=None,
                     help="measure another design beside Qwen2 at equal size instead of the benchmark")
+    ap.add_argument("--kv-cache-dtype", choices=["auto", "int8", "fp8"], default="auto",
+                    help="keys and values in 8 bits (with the benchmark or --scenario)")
     ap.add_argument("--size", default=None, help="with --design: sizes to run, e.g. s,m")
     args = ap.parse_args()
     if args.micro:
@@ -891,8 +896,8 @@ def main() -> int:
             print(json.dumps({"error": "this engine runs on one GPU", "n_gpus": args.gpus}))
             return 2
         if args.scenario == "longctx":
-            return run_long_context(args.shape, args.layers, portion=args.portion)
-        return run_scenario(args.scenario, args.shape, args.layers)
+            return run_long_context(args.shape, args.layers, portion=args.portion, kept=args.kv_cache_dtype)
+        return run_scenario(args.scenario, args.shape, args.layers, args.kv_cache_dtype)
 
     if args.impl == "reference":
         print(json.dumps({"impl": "reference", "unavailable":
@@ -918,7 +923,7 @@ def main() -> int:
     eng = Engine(config=cfg, weights_seed=0, dtype="bfloat16", max_num_batched_tokens=8192,
                  max_num_seqs=64, max_seq_len=CONTEXT, kvcache_block_size=PAGE,
                  num_kvcache_blocks=64 * (PROMPT + 256) // PAGE + PREFILL_TOKENS // PAGE + 64,
-                 enforce_eager=args.enforce_eager)
+                 enforce_eager=args.enforce_eager, kv_cache_dtype=args.kv_cache_dtype)
     B = args.batch
 
     clocks = ClockSampler()
@@ -933,7 +938,7 @@ def main() -> int:
         """(GB/s, fraction of the copy bandwidth) of a decode step: every weight once and the
         cache of the live requests at their mean length over the timed steps."""
         mean_ctx = PROMPT + args.warmup + steps / 2
-        nbytes = weight_bytes(cfg, layers) + batch * mean_ctx * kv_bytes_per_token(cfg, layers)
+        nbytes = weight_bytes(cfg, layers) + batch * mean_ctx * kv_bytes_per_token(cfg, layers, kept=args.kv_cache_dtype)
         gbs = nbytes / (step_ms * 1e-3) / 1e9
         return gbs, gbs / peaks["hbm_gbs"]
 
@@ -980,6 +985,8 @@ def main() -> int:
         "ms_per_step_all": [round(t, 4) for t in all_ms],
         "clocks": clock_info,
     }
+    if args.kv_cache_dtype != "auto":
+        line["config"]["kv_cache_dtype"] = args.kv_cache_dtype
     print(json.dumps(line))
     return 0
 

@@ -42,3 +42,13 @@ def test_the_line_of_short_tables():
     from ginfer_b200.ops.build import CSRC_DIR
     with open(os.path.join(CSRC_DIR, "quant_attention.cu")) as f:
         assert int(re.search(r"\bkShortKeys = (\d+)", f.read())[1]) == qc._SHORT
+
+
+def test_bytes_that_the_benchmark_counts():
+    import bench
+    from ginfer_b200.cache.storage import GroupLayout
+    cfg = bench.SHAPES["1.5b"]
+    heads, width = cfg["num_key_value_heads"], cfg["head_dim"]
+    for kept in ("auto", "int8", "fp8"):
+        page = GroupLayout(((heads, width),) * 2, True, 0, (0,), 0, "" if kept == "auto" else kept).bytes_per_page(16, 2)
+        assert bench.kv_bytes_per_token(cfg, 3, kept=kept) * 16 == 3 * page

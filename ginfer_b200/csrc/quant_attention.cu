@@ -499,7 +499,9 @@ quant_decode_kernel(const DecodeArgs a, const __grid_constant__ CUtensorMap map)
   // q as the products want it: [half][tile of heads][word of a key][lane][four channels]; read again for every tile,
   // so that four blocks' registers fit an SM
   __shared__ __align__(16) __half qh[PARTS][NT][KWORDS][32][4];
-  __shared__ float qs[R], q_sum[R], sm[WARPS][R], sl[WARPS][R], back[WARPS];
+  // a score is (product * x + y) * the key's scale
+  __shared__ __align__(16) float2 q_back[R];
+  __shared__ float sm[WARPS][R], sl[WARPS][R], back[WARPS];
   __shared__ int so_at[WARPS];
   __shared__ __align__(16) uint8_t fresh_row[2][HD];             // STEP: the new token's codes and scales
   __shared__ float fresh_scale[2];
@@ -584,7 +586,7 @@ quant_decode_kernel(const DecodeArgs a, const __grid_constant__ CUtensorMap map)
   int f = 254;                             // weights are multiplied by 2^(f - 127)
   uint32_t extra = 0, too_large = 0;       // the heads' h, 8 bits each; scale_limit of f and the largest of them
   int at_stage = 0, to_stage = STAGES - 1;
-  Item it, done;
+  Item it;
   bool have = next_item(it), had = false;
   if (have) ask_pages(it);
   if (cur.todo > 0) soon_b = cur.b, soon_len = request_length(a, cur.b);
@@ -597,7 +599,7 @@ quant_decode_kernel(const DecodeArgs a, const __grid_constant__ CUtensorMap map)
     Angles an;
     // the new token's row of keys (the last warp's, whose rows of q may not exist) and of values (the one before)
     const bool news = STEP && it.ends && warp >= WARPS - 2, keys = warp == WARPS - 1;
-    int new_page = 0, new_len = 0, page_number = 0;
+    int new_page = 0, page_number = 0;
     if (have) {
 #pragma unroll
       for (int i = 0; i < RW; ++i)
@@ -612,7 +614,9 @@ quant_decode_kernel(const DecodeArgs a, const __grid_constant__ CUtensorMap map)
             load_partners<T>(a, row + (size_t)(h0 + warp + i * WARPS) * HD, warp + i * WARPS < nrows, lane, y[i]);
           if (news && keys) load_partners<T>(a, new_at, true, lane, ny);
         }
-        if (news) new_page = fresh_index(tiles.tbl + logical_page(a, p)), new_len = fresh_index(a.lengths + it.b);
+        // (an entry that is no page, or a token behind the table's end: nowhere to write it to)
+        if (news) new_page = fresh_index(tiles.tbl + logical_page(a, p));
+        if (news && it.len == a.limit && fresh_index(a.lengths + it.b) > a.limit) new_page = -1;
       }
       if (cur.todo > 0) later_b = cur.b + 1 == a.B ? 0 : cur.b + 1, later_len = request_length(a, later_b);
       // (of the new token nothing is read)
@@ -630,6 +634,7 @@ quant_decode_kernel(const DecodeArgs a, const __grid_constant__ CUtensorMap map)
     if (!have) pdl_trigger();
     // ---- the end of the item before: the four warps' results
     if (had) {
+      const Item done = kept[warp].done;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -699,21 +704,18 @@ quant_decode_kernel(const DecodeArgs a, const __grid_constant__ CUtensorMap map)
           turn_row(a, an, lane, nx, ny);
         }
         const RowScale rs = row_scale(row_top(nx), FP8);
-        // (an entry that is no page, or a token behind the table's end: nowhere to write it to)
-        const bool stays = (unsigned)new_page < (unsigned)a.pages && new_len <= a.limit;
-        const Place pl = place_of(a, kvh, stays ? new_page : 0, p - logical_page(a, p) * a.page);
+        const Place pl = place_of(a, kvh, page_in(a, new_page), p - logical_page(a, p) * a.page);
         const int which = keys ? 0 : 1;
         uint8_t* dst = const_cast<uint8_t*>(pl.codes) + (size_t)which * a.page * HD;
 #pragma unroll
         for (int i = 0; i < N; ++i)
-          if (i * 32 + lane < HD) {
-            const uint8_t code = (uint8_t)code_of(nx[i], rs, FP8);
-            fresh_row[which][i * 32 + lane] = code;
-            if (stays) dst[i * 32 + lane] = code;
-          }
-        if (lane == 0) {
-          fresh_scale[which] = rs.scale;
-          if (stays) reinterpret_cast<float*>(const_cast<float2*>(pl.scales))[which] = rs.scale;
+          if (i * 32 + lane < HD) fresh_row[which][i * 32 + lane] = (uint8_t)code_of(nx[i], rs, FP8);
+        if (lane == 0) fresh_scale[which] = rs.scale;
+        if (new_page == page_in(a, new_page)) {
+#pragma unroll
+          for (int i = 0; i < N; ++i)
+            if (i * 32 + lane < HD) dst[i * 32 + lane] = fresh_row[which][i * 32 + lane];
+          if (lane == 0) reinterpret_cast<float*>(const_cast<float2*>(pl.scales))[which] = rs.scale;
         }
       }
 #pragma unroll
@@ -743,20 +745,15 @@ quant_decode_kernel(const DecodeArgs a, const __grid_constant__ CUtensorMap map)
       }
       if constexpr (RAISED) sum = warp_sum(sum);
       if (lane == 0) {
-        qs[r] = a.scale * kLog2E * __uint_as_float((uint32_t)(127 - up) << 23);
-        q_sum[r] = sum;
+        const float qs = a.scale * kLog2E * __uint_as_float((uint32_t)(127 - up) << 23);
+        q_back[r] = make_float2(RAISED ? qs * 16777216.f : qs, -128.f * sum * qs);
       }
     }
     __syncthreads();
-    // a score is (product * qscale + qshift) * the key's scale
-    float qscale[NT][2], qshift[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        qscale[n][j] = qs[n * 8 + 2 * t + j];
-        qshift[n][j] = -128.f * q_sum[n * 8 + 2 * t + j] * qscale[n][j];
-        if constexpr (RAISED) qscale[n][j] *= 16777216.f;
         m[n][j] = -INFINITY, l[n][j] = 0.f;
       }
 #pragma unroll
@@ -765,7 +762,8 @@ quant_decode_kernel(const DecodeArgs a, const __grid_constant__ CUtensorMap map)
     f = 254, extra = 0, too_large = scale_limit(254);
 
     // ---- where the block goes next (its pages are there when this item's tiles are done)
-    done = it, had = true;
+    const Item done = it;
+    had = true;
     const int lo = it.lo, len = it.len, last = it.last, first = it.first;
     if (cur.todo > 0) cur.len = soon_b == cur.b ? soon_len : request_length(a, cur.b);
     have = next_item(it);
@@ -886,19 +884,21 @@ quant_decode_kernel(const DecodeArgs a, const __grid_constant__ CUtensorMap map)
       // large for a p of 1.
       bool above = false;
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n) {
+        const float4 qb = *reinterpret_cast<const float4*>(&q_back[n * 8 + 2 * t]);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           float top = -INFINITY;
 #pragma unroll
           for (int i = 0; i < 2 * TK; ++i) {
             float& r = s[i >> 1][n][2 * (i & 1) + j];
-            r = RAISED ? fmaf(r, qscale[n][j], qshift[n][j]) : r * qscale[n][j];
+            r = RAISED ? fmaf(r, j ? qb.z : qb.x, j ? qb.w : qb.y) : r * (j ? qb.z : qb.x);
             r = seen[i] ? r * sc[i].x : -INFINITY;
             top = fmaxf(top, r);
           }
           above |= top > m[n][j];
         }
+      }
       uint32_t vtop = 0;
 #pragma unroll
       for (int i = 0; i < 2 * TK; ++i) {
@@ -1018,7 +1018,7 @@ quant_decode_kernel(const DecodeArgs a, const __grid_constant__ CUtensorMap map)
               for (int e = 0; e < 4; ++e) o[n][j * WORDS * PER + i][e] += d[i][n][e];
       }
     }
-    it = kept[warp].next, done = kept[warp].done, cur = kept[warp].cur;
+    it = kept[warp].next, cur = kept[warp].cur;
     soon_b = kept[warp].soon_b, soon_len = kept[warp].soon_len;
     __syncwarp();
   }

@@ -45,7 +45,8 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--kvcache-block-size", type=int, default=16)
     ap.add_argument("--num-kvcache-blocks", type=int, default=None)
     ap.add_argument("--kv-cache-dtype", default="auto", choices=["auto", "int8", "fp8"],
-                    help="keys and values in 8 bits (default: in the compute dtype)")
+                    help="keys and values in 8 bits, for models of plain grouped-query attention (Qwen2); "
+                         "default: in the compute dtype")
     ap.add_argument("--enforce-eager", action="store_true")
     ap.add_argument("--capture-graphs", action="store_true",
                     help="capture the decode steps' CUDA graphs at start-up, not on first use")

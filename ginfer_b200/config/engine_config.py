@@ -3,7 +3,8 @@
 ``max_seq_len``, ``gpu_memory_utilization``, ``kvcache_block_size``.  Added here: the compute
 ``dtype``, an explicit page count (``num_kvcache_blocks``; tests use very few so that pages are
 used again), ``enforce_eager`` (no CUDA-graph replay of decode steps) and ``kv_cache_dtype`` (keys
-and values in 8 bits, half or a quarter of the bytes: for models whose attention reads such a cache).
+and values in 8 bits, half or a quarter of the bytes: for models whose attention reads such a cache;
+with ``dtype="float32"`` single tokens' attention then multiplies in 22 bits, not in 32).
 """
 from __future__ import annotations
 

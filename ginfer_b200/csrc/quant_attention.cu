@@ -38,10 +38,10 @@
 // that are no multiple of 8 and scales that are not aligned come by cp.async.
 //
 // Measured (bfloat16 q, 4 kv heads of 128 with 7 query heads each, pages of 16, the cache not in L2): 64 requests of
-// 4,500 keys on average, 304 MB: 59.5 us, 5.1 TB/s (e4m3; integers 61.6); one request of 131,071 keys, 138 MB: 32.9 us,
-// 4.2 TB/s, of which the first tile's chain length -> page -> codes takes 4, blocks that end apart 5, and the join with
-// its launch 5.  A ring that only copies reads 6.6 TB/s here, one of cp.async 5.4; tiles straight to registers came to
-// 4.0 with the rest of this kernel.
+// 4,500 keys on average, 304 MB: 60.1 us, 5.1 TB/s (e4m3; integers 62.4); one request of 131,071 keys, 138 MB: 33.6 us,
+// 4.1 TB/s: an SM has blocks for 78 % of the kernel's time (the first tile's chain length -> page -> codes is 4 us, and
+// blocks end apart), and the join's launch adds to it.  A ring that only copies reads 6.6 TB/s here, one of cp.async 5.4;
+// tiles straight to registers came to 4.0 with the rest of this kernel.
 #include <algorithm>
 #include <cstdlib>
 #include <type_traits>
@@ -61,7 +61,7 @@ constexpr int HD = GF_HEAD_DIM;
 static_assert(HD % 16 == 0 && HD >= 16 && HD <= 256, "head size must be a multiple of 16, <= 256");
 constexpr float kLog2E = 1.4426950408889634f;
 // Keys of a tile: 32 while their products fit the registers.  What a tile costs beside its bytes (waiting, copies,
-// maxima, q from shared memory) is half, and two chains of steps overlap: 304 MB of heads of 128 59 us after 63.
+// maxima, q from shared memory) is half, and two chains of steps overlap: 304 MB of heads of 128 60 us after 70.
 constexpr int TK = HD <= 128 ? 2 : 1, TILE = 16 * TK, TILE_SHIFT = TK == 2 ? 5 : 4;
 constexpr int WARPS = 4, THREADS = WARPS * 32;
 constexpr int KW = HD % 64 == 0 ? 16 : HD % 32 == 0 ? 8 : 4;     // bytes of a key a thread reads at once
@@ -91,8 +91,9 @@ struct Layout {
   }
 };
 constexpr int STAGES = 2;
-// Blocks an SM: as many as their registers allow without spilling in a tile's work.  (Two tiles of heads: 50 us with
-// two of them, 53 with three, at 16 query heads of 128 a kv head; one of heads with 32-bit q: 71 with three, 78 with two.)
+// Blocks an SM: as many as their registers allow without spilling in a tile's work.  (Two tiles of heads: 52 us with
+// two of them, 53 with three, at 16 query heads of 128 a kv head in equal runs; one of heads with 32-bit q: 73 with three,
+// 81 with two.)
 constexpr int blocks_an_sm(int nt, int type_bytes) {
   return nt == 1 ? (HD <= 64 && type_bytes == 2 ? 4 : 3) : (HD <= 96 ? 3 : 2);
 }
@@ -101,7 +102,7 @@ constexpr int kLeastTiles = 2 * WARPS / TK;
 // How the work is shared out (launch_decode).  A cluster of up to kMostOfCluster blocks takes an item where the blocks that
 // fit the GPU allow two or more and a request that fills its table keeps them at most as much longer than equal runs would
 // as the joining kernel costs, kUnevenKeys keys a block: 8 requests of 576 keys, tables of 4,096, 12 query heads on 2 kv
-// heads of 128: 10.9 us after 16.7 with equal runs; one of 8,000 keys, where the rule says equal runs: 16.3 after 19.0.
+// heads of 128: 11.1 us after 16.6 with equal runs; one of 8,000 keys, where the rule says equal runs: 16.1 after 19.4.
 // kShortKeys keys are one block's work: parts that meet cost more than their keys.  One block / as the rule goes on above it, us,
 // full tables of 256 keys: 28 heads on 4 kv heads of 128, one request 7.2 / 8.2, eight 7.4 / 8.3; 14 on 2 of 64, one 6.4 / 6.7,
 // 64 6.8 / 8.3; 32 on 2 of 128, eight 9.3 / 10.5; 32-bit q, 28 on 4 of 128, 32 requests 8.2 / 10.8; 8 on 2 of 256, eight

@@ -285,13 +285,17 @@ def decode(q: torch.Tensor, nh: int, cache, block_table: torch.Tensor, lengths: 
     """Attention of one new token a request, the last of its ``lengths[b]`` tokens, over its cache:
     ``[B, nh * head size]`` in ``q``'s type (bf16 or fp32).  ``q [B, >= nh * head size]`` is rotated and the
     new token's keys and values are in the cache already.  ``window``: the mask as ``ops.mask_span`` gives
-    it.  A request without a token gets zeros."""
+    it.  A request without a token gets zeros.
+
+    The products on the tensor cores take q and a key's weight (its ``p`` times its values' scale) in 11 bits, with an
+    fp32 q in 22; a weight that is small beside the heaviest is off by at most 2^-25 of it, whatever the scales.  Scores,
+    maxima and sums are 32-bit; a key whose ``p`` is below 2^-119 counts as nothing."""
     return _decode(q, nh, _cache(cache), block_table, lengths, scale, window)
 
 
 def step(qkv: torch.Tensor, nh: int, table, cache, block_table: torch.Tensor, lengths: torch.Tensor,
          scale: float, window: int = 0, *, neighbours: bool = False) -> torch.Tensor:
-    """What a decode step does to a layer's cache, in one launch: row ``b`` of ``qkv [B, (nh + 2 kv heads) *
+    """What a decode step does to a layer's cache, in one call: row ``b`` of ``qkv [B, (nh + 2 kv heads) *
     head size]`` is the last of request ``b``'s ``lengths[b]`` tokens; q and k are rotated, k and v written (as
     :func:`write` does: not where the table has no page of the cache for it, an entry outside the cache or a length beyond
     ``W * page``), and the token attends over the cache, itself among the keys (as :func:`decode`)."""
@@ -341,9 +345,9 @@ def attention(qkv: torch.Tensor, nh: int, table, cache, block_table: torch.Tenso
               slots) -> torch.Tensor:
     """A step's attention over a layer's cache: ``qkv [T, (nh + 2 kv heads) * head size]`` unrotated, ``slots [T]``
     where the new keys and values go (``None``: they are not written, the cache is another layer's).  Single tokens
-    attend over the codes; prompt portions read what they see back (in the activations' type) and take the kernels of
-    an unquantised cache, so a portion sees the same keys and values as the tokens after it.  Returns ``[T, nh * head
-    size]``."""
+    attend over the codes; prompt portions read what they see back and take the kernels of an unquantised cache, so a
+    portion sees the keys and values that the tokens after it see: in fp32 the same numbers, in bf16 rounded to the 8 bits
+    of that type, which the codes' values are not when single tokens read them.  Returns ``[T, nh * head size]``."""
     from . import attention_bf16, paged_attention_simt
     codes, page, hd = cache[0], cache[0].shape[3], cache[0].shape[4]
     nkv = codes.shape[1]

@@ -37,7 +37,7 @@ def _attend(dtype, heads, kv_heads, dim, page, batch, prefix, longest, queries=1
 
 
 def _verify(dtype, batch, drafts, vocab, drafter, greedy=False, gap=0):
-    """``drafter``: whether a model drafted (its logits are there) or a look-up; ``greedy``: every third request has
+    """``drafter``: whether a model drafted (its logits stand beside the target's) or a look-up; ``greedy``: every third request has
     temperature zero; ``gap``: channels between one row of logits and the next."""
     return dict(op="verify", dtype=dtype, batch=batch, drafts=drafts, vocab=vocab, drafter=drafter, greedy=greedy,
                 gap=gap)
@@ -214,10 +214,9 @@ def _prepare_verify(case, g):
     said = target[~last]                                              # the rows that drafts are held against
     draft = None
     if case["drafter"]:
-        draft = said.clone()
-        draft.scatter_add_(1, likely[~last], 0.8 * torch.randn(D, 24, generator=g, device=DEV))
-        draft += 0.1 * torch.randn(D, V, generator=g, device=DEV)
-        said = draft
+        draft = target + 0.1 * torch.randn(R, V, generator=g, device=DEV)
+        draft.scatter_add_(1, likely, 0.8 * torch.randn(R, 24, generator=g, device=DEV))
+        said = draft[~last]
     if case["greedy"]:
         temperature[::3] = 0.0
     # drafts as the drafter draws them; a look-up finds a wrong one now and then
@@ -305,15 +304,11 @@ def _plain_verify(s):
     best = s["logits"].argmax(1)
     # the drafts: the i-th is the (i + 1)-th row's token, held against the i-th row
     guess, row = tokens[rows[:, 1:]], rows[:, :-1]
-    p = _softmax(s["logits"], t[of_row])
-    if s["draft"] is not None and s["draft"].shape[0]:
-        at = (rows[:, :-1] - every[:, None]).clamp(max=s["draft"].shape[0] - 1)
-        owner = torch.zeros(s["draft"].shape[0], dtype=torch.int64, device=DEV)
-        owner[at[there[:, 1:]]] = every[:, None].expand(-1, wide - 1)[there[:, 1:]]
-        q = _softmax(s["draft"], t[owner])
-        share = q[at, guess]
-    else:
-        q, share = None, torch.ones(guess.shape, dtype=torch.float64, device=DEV)
+    p, q = _softmax(s["logits"], t[of_row]), None
+    share = torch.ones(guess.shape, dtype=torch.float64, device=DEV)
+    if s["draft"] is not None:
+        q = _softmax(s["draft"], t[of_row])
+        share = q[row, guess]
     stays = torch.where(greedy[:, None], best[row] == guess, s["u"][row].double() * share < p[row, guess])
     accepted = (stays & there[:, 1:]).long().cumprod(1).sum(1) if wide > 1 else torch.zeros_like(count)
     # the token behind them
@@ -321,11 +316,10 @@ def _plain_verify(s):
     w = p[stop]
     if wide > 1:
         refused = (accepted < count)[:, None]
-        i = accepted.clamp(max=wide - 2)[:, None]
         if q is not None:
-            w = torch.where(refused, (w - q[at.gather(1, i)[:, 0]]).clamp(min=0.0), w)
+            w = torch.where(refused, (w - q[stop]).clamp(min=0.0), w)
         else:
-            w = torch.where(refused, w.scatter(1, guess.gather(1, i), 0.0), w)
+            w = torch.where(refused, w.scatter(1, guess.gather(1, accepted.clamp(max=wide - 2)[:, None]), 0.0), w)
     run_up = w.cumsum(1)
     u = s["u"][s["cu"][1:].long() - 1].double()
     hit = (run_up >= u[:, None] * run_up[:, -1:]) & (w > 0)
@@ -392,7 +386,7 @@ def _exact_verify(case, s):
                 if s["draft"] is None:
                     other = torch.nn.functional.one_hot(torch.tensor(d, device=DEV), x.numel()).double()
                 else:
-                    other = torch.softmax(s["draft"][row - b].double() / t, 0)
+                    other = torch.softmax(s["draft"][row].double() / t, 0)
                 stays = u[row] * float(other[d]) < float(rest[d])
                 if not stays:
                     rest = torch.relu(rest - other)

@@ -454,4 +454,4 @@ def bmm_f32_out(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
 from . import attention_bf16, gemm_bf16, gemm_prefill  # noqa: E402,F401
 from .linear import GatedLinear, Linear, add_to  # noqa: E402,F401
 from . import prenorm  # noqa: E402,F401
-from . import depth, hyper, quant_cache, rotary, shift  # noqa: E402,F401
+from . import depth, drafts, hyper, quant_cache, rotary, shared_prefix, shift  # noqa: E402,F401

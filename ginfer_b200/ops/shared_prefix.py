@@ -1,0 +1,105 @@
+"""Attention for a batch whose requests share a long prefix, computed once for all (``csrc/shared_prefix.cu``).
+
+Requests come in groups; the requests of a group share a prefix (a system prompt, a document) whose keys and values are in
+the cache once.  Every request brings its newest tokens, one or several (a last token and drafted ones), and each of
+them attends over its group's prefix and over the request's own tokens up to itself.
+
+All work goes to the current stream; nothing but scratch memory is kept between calls.
+"""
+from __future__ import annotations
+
+import struct
+
+import torch
+
+from . import _Counter, _ok
+from .quant_cache import _at, _code, _device, _function, _raw_stream
+
+MAX_HEAD_DIM = 256
+_ATTEND = struct.Struct("=25qd")
+_int32 = torch.int32
+
+
+def supports(head_dim: int, heads: int, kv_heads: int) -> bool:
+    """Whether the kernels take these heads."""
+    return head_dim % 16 == 0 and 16 <= head_dim <= MAX_HEAD_DIM and kv_heads > 0 and heads > 0 and heads % kv_heads == 0
+
+
+def _table(t, count, what, device):
+    """(address, row stride, columns) of a table of pages."""
+    if t.dtype is not _int32 or t.dim() != 2 or t.shape[0] != count or (t.stride(1) != 1 and t.shape[1] > 1):
+        raise ValueError(f"{what} is int32 [{count}, pages], its columns side by side; got {t.dtype} {tuple(t.shape)}, strides "
+                         f"{tuple(t.stride())}")
+    return _at(t, device), t.stride(0), t.shape[1]
+
+
+def _vector(t, count, what, device):
+    if t.dtype is not _int32 or t.dim() != 1 or t.shape[0] != count or not t.is_contiguous():
+        raise ValueError(f"{what} is int32 [{count}], contiguous; got {t.dtype} {tuple(t.shape)}")
+    return _at(t, device)
+
+
+def attend(q: torch.Tensor, nh: int, pages, prefix_table: torch.Tensor, prefix_lens: torch.Tensor,
+           block_table: torch.Tensor, lengths: torch.Tensor, scale: float, *, cu_groups=None, cu_seqlens_q=None,
+           max_q_len: int | None = None, out=None) -> torch.Tensor:
+    """Attention of the rows ``q [T, >= nh * head size]`` (bf16 or fp32, rotated) over shared prefixes and over each
+    request's own tokens: ``[T, nh * head size]`` in ``q``'s type.
+
+    ``pages``: the cache, ``[2, pages, page, kv heads, head size]`` or its two planes, keys and values rotated and written.
+    ``prefix_table [G, P]``, ``prefix_lens [G]`` int32: the pages of every group's prefix in order and how many tokens it
+    has (it may end inside a page).  ``block_table [B, W]``, ``lengths [B]`` int32: likewise of every request's own
+    tokens, the new ones among them, counted from behind the prefix.  (Of tables that name all of a request's pages, with
+    whole pages shared, these are ``table[first requests, :P]`` and ``table[:, P:]``; rows may have any stride.)
+    ``cu_groups [G + 1]`` int32: group ``g`` is the requests ``cu_groups[g] .. cu_groups[g + 1] - 1``, and a request of no
+    group has no prefix; ``None``: one group of all requests.  ``cu_seqlens_q [B + 1]`` int32: request ``b`` has the rows
+    ``cu_seqlens_q[b] .. cu_seqlens_q[b + 1] - 1``; ``None``: row ``b`` alone.  ``max_q_len``: about how many rows a request
+    has at most (a hint: the kernels' tiles go by it; ``None``: ``T / B``).
+
+    The ``i``-th of a request's ``n`` rows sees the whole prefix and the own tokens ``0 .. length - n + i``; a row that
+    sees nothing gives zeros.  Rows that belong to no request are not written: with ``out`` (``[T, nh * head size]``,
+    contiguous, ``q``'s type) they stay as they were.  Entries of the tables behind a sequence's length are not read."""
+    k, v = pages[0], pages[1]
+    if k.dim() != 4 or k.shape != v.shape or not k.is_contiguous() or not v.is_contiguous() or v.dtype != k.dtype:
+        raise ValueError(f"the cache's planes are [pages, page, kv heads, head size], contiguous, of one shape and type; got "
+                         f"{tuple(k.shape)}, {tuple(v.shape)}")
+    count, page, nkv, hd = k.shape
+    if not supports(hd, nh, nkv):
+        raise ValueError(f"attention over shared prefixes takes head sizes that are a multiple of 16, at most "
+                         f"{MAX_HEAD_DIM}, and a multiple of the kv heads; got head_dim={hd}, heads={nh}, kv_heads={nkv}")
+    if count < 1 or page < 1 or count * page >= 1 << 31:
+        raise ValueError(f"{count} pages of {page} tokens: a cache has at least one, and slots are 32-bit integers")
+    dev = _device(k)
+    if q.dim() != 2 or q.shape[1] < nh * hd or (q.stride(1) != 1 and q.shape[1] > 1) or q.dtype != k.dtype:
+        raise ValueError(f"q has rows of at least {nh * hd} channels without gaps in the cache's type {k.dtype}; got "
+                         f"{q.dtype} {tuple(q.shape)}, strides {tuple(q.stride())}")
+    code, at = _code(q.dtype), _at(q, dev)
+    T, B, G = q.shape[0], lengths.shape[0], prefix_lens.shape[0]
+    prefix, prefix_stride, P = _table(prefix_table, G, "prefix_table", dev)
+    table, table_stride, W = _table(block_table, B, "block_table", dev)
+    groups = rows = 0
+    if cu_groups is not None:
+        groups = _vector(cu_groups, G + 1, "cu_groups", dev)
+    elif G > 1:
+        raise ValueError(f"{G} groups, and no cu_groups that says whose they are")
+    if cu_seqlens_q is not None:
+        rows = _vector(cu_seqlens_q, B + 1, "cu_seqlens_q", dev)
+    elif T < B:
+        raise ValueError(f"{T} rows for {B} requests of one row each")
+    if P * page >= 1 << 30 or W * page >= 1 << 30:
+        raise ValueError(f"tables of {P} and {W} pages of {page}: a sequence has fewer than 2^30 tokens")
+    if max_q_len is not None and max_q_len < 0:
+        raise ValueError(f"max_q_len is {max_q_len}")
+    if not scale > 0:
+        raise ValueError(f"the scale of the scores is positive, not {scale}")
+    if out is None:
+        out = q.new_empty(T, nh * hd)
+    elif out.dtype != q.dtype or out.shape != (T, nh * hd) or not out.is_contiguous():
+        raise ValueError(f"out is {q.dtype} {(T, nh * hd)}, contiguous; got {out.dtype} {tuple(out.shape)}")
+    rc = _function("shared_prefix", "gf_prefix_attend")(_ATTEND.pack(
+        at, q.stride(0), code, k.data_ptr(), _at(v, dev), count, page, prefix, prefix_stride,
+        _vector(prefix_lens, G, "prefix_lens", dev), G, P * page, table, table_stride, _vector(lengths, B, "lengths", dev),
+        B, W * page, groups, rows, _at(out, dev), T, nh, nkv, hd, _raw_stream(dev), scale))
+    _Counter.launches += 1
+    if rc:
+        _ok(rc, "shared_prefix.attend")
+    return out

@@ -1,9 +1,20 @@
-// What the kernels of attention over shared prefixes are told, and how they read it.
+// Attention over shared prefixes: what the kernels are told, and how the work is divided.
 //
 // Request b has the rows cu[b] .. cu[b + 1] - 1 of q (one row, its own number, without cu); the i-th of n sees the
 // prefix of the request's group and the request's own tokens 0 .. length - n + i.  Whatever the tables, lengths and
-// starts hold, nothing outside q, the cache and the result is touched: lengths are cut to their tables, rows to q, and
-// an entry that is no page of the cache is taken for the nearest.
+// starts hold, nothing outside q, the cache, the scratch and the result is touched: lengths are cut to their tables, rows to
+// q, and an entry that is no page of the cache is taken for the nearest.
+//
+// A kernel's row is a (token, query head) pair; the query heads of a kv head are in `chunks` chunks of up to `heads`, and a
+// tile of rows is `tokens` tokens of a chunk.  Keys come in tiles, too.  Two kinds of work leave pieces of results, each a
+// maximum (in log2 units), a sum and the weighted values of every row:
+//  * a group's prefix (PrefixItem): the group's rows in tiles, its keys in chunks of `chunk` tiles, the same for all groups;
+//    every item's piece has a place of its own.  Row tiles of one chunk of keys are neighbours, so that they read it at the
+//    same time.
+//  * a request's own tokens (Cursor): the tiles of all requests (and of their tiles of rows) are one long sequence, and
+//    every block takes an equal run of it, so that blocks end together whatever the lengths.  A run begins and ends inside
+//    requests; what is cut has the block's two places, the rest a row's own.
+// The joining kernel works the same arithmetic out again and adds a row's pieces up, in order: no atomics.
 #pragma once
 #include "common.cuh"
 
@@ -20,17 +31,20 @@ struct PrefixArgs {
   const int* cu_groups;        // [G + 1], or null: all requests are of group 0
   const int* cu;               // [B + 1], or null: a row a request
   void* out;                   // [T][nh][hd]
-  int q_stride, prefix_stride, table_stride, prefix_limit, limit, G, B, T, nh, nkv, hd, page, pages;
+  int q_stride, prefix_stride, table_stride, prefix_limit, limit, G, B, T, nh, nkv, hd, page, pages, page_shift;
   float scale;
 };
 
+// ------------------------------------------------------------------------------------- what a call says
 struct Rows {
   int first, count;
 };
+__device__ __forceinline__ int row_start(const PrefixArgs& a, int b) {
+  return a.cu ? min(max(fresh_index(a.cu + b), 0), a.T) : min(b, a.T);
+}
 __device__ __forceinline__ Rows rows_of(const PrefixArgs& a, int b) {
-  if (!a.cu) return {b, b < a.T ? 1 : 0};
-  const int first = min(max(fresh_index(a.cu + b), 0), a.T), end = min(fresh_index(a.cu + b + 1), a.T);
-  return {first, max(end - first, 0)};
+  const int first = row_start(a, b);
+  return {first, max((a.cu ? row_start(a, b + 1) : min(b + 1, a.T)) - first, 0)};
 }
 __device__ __forceinline__ int own_length(const PrefixArgs& a, int b) {
   return min(max(fresh_index(a.lengths + b), 0), a.limit);
@@ -49,8 +63,231 @@ __device__ __forceinline__ int group_of(const PrefixArgs& a, int b) {
   }
   return low < a.G && fresh_index(a.cu_groups + low) <= b ? low : -1;
 }
+// The rows of a group's requests.
+__device__ __forceinline__ Rows group_rows(const PrefixArgs& a, int g) {
+  const int b0 = a.cu_groups ? min(max(fresh_index(a.cu_groups + g), 0), a.B) : 0;
+  const int b1 = a.cu_groups ? min(max(fresh_index(a.cu_groups + g + 1), b0), a.B) : a.B;
+  const int first = row_start(a, b0);
+  return {first, max(row_start(a, b1) - first, 0)};
+}
 __device__ __forceinline__ int page_in(const PrefixArgs& a, int number) {
   return min(max(number, 0), a.pages - 1);
+}
+__device__ __forceinline__ int logical_page(const PrefixArgs& a, int c) {
+  return a.page_shift >= 0 ? c >> a.page_shift : c / a.page;
+}
+// The place of token c of the sequence that a row of a table names.
+__device__ __forceinline__ int slot_of(const PrefixArgs& a, const int* tbl, int c) {
+  const int lp = logical_page(a, c);
+  return page_in(a, fresh_index(tbl + lp)) * a.page + (c - lp * a.page);
+}
+
+// ------------------------------------------------------------------------------------- rows
+struct Shape {
+  int chunks, heads, tokens;    // chunks of a kv head's query heads, heads of a chunk at most, tokens of a row tile
+};
+__host__ __device__ __forceinline__ Shape row_shape_of(int nh, int nkv, int rows) {
+  const int each = nh / nkv, chunks = (each + rows - 1) / rows, heads = (each + chunks - 1) / chunks;
+  return {chunks, heads, rows / heads};
+}
+
+// ------------------------------------------------------------------------------------- prefixes
+struct PrefixItem {
+  int g, hc, split, m;          // hc: kv head * chunks + chunk; m: the tile of rows
+  int first, count;             // its tokens
+  int length, tiles;            // of the prefix
+};
+// Groups' numbers of row tiles and key tiles, a lane a group of 32.
+struct GroupTiles {
+  int mt, nt, first, count, length;
+  __device__ __forceinline__ void load(const PrefixArgs& a, int g, int tokens, int tile) {
+    mt = nt = first = count = length = 0;
+    if (g < a.G) {
+      const Rows r = group_rows(a, g);
+      first = r.first, count = r.count;
+      length = prefix_length(a, g);
+      mt = (count + tokens - 1) / tokens;
+      nt = (length + tile - 1) / tile;
+    }
+  }
+};
+// Tiles of a chunk of keys, by one warp.  With `workers` blocks the time is about (rounds of items) * (chunk + over),
+// over: what an item's start and end cost in tiles.  Looked at are the 32 lengths from one, a half and a third of an equal share
+// on; the longest prefix, which is always possible, is the last resort.
+__device__ __forceinline__ int plan_chunk(const PrefixArgs& a, int H, int tokens, int tile, int workers, int places, int over) {
+  const int lane = threadIdx.x & 31;
+  GroupTiles t;
+  t.load(a, lane, tokens, tile);
+  long long units = 0;
+  int most = 0;
+  for (int g0 = 0; g0 < a.G; g0 += 32) {
+    if (g0) t.load(a, g0 + lane, tokens, tile);
+    units += (long long)t.mt * H * t.nt;
+    most = max(most, t.mt ? t.nt : 0);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    units += __shfl_xor_sync(0xffffffffu, units, o);
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+  }
+  if (most == 0) return 1;
+  int len[3];
+  long long items[3] = {0, 0, 0};
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    const long long share = (units + (long long)workers * (k + 1) - 1) / ((long long)workers * (k + 1));
+    const int from = (int)(share < most ? share : most);
+    len[k] = min(most, max(1, from) + lane * max(1, from / 48));
+  }
+  if (lane == 31) len[0] = most;
+  for (int g0 = 0; g0 < a.G; g0 += 32) {
+    if (a.G > 32) t.load(a, g0 + lane, tokens, tile);
+    for (int i = 0; i < min(32, a.G - g0); ++i) {
+      const int mt = __shfl_sync(0xffffffffu, t.mt, i) * H, nt = __shfl_sync(0xffffffffu, t.nt, i);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) items[k] += (long long)mt * ((nt + len[k] - 1) / len[k]);
+    }
+  }
+  float best = INFINITY;
+  int chunk = most;
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    const float rounds = (float)((items[k] + workers - 1) / workers), cost = rounds * (len[k] + over);
+    if (items[k] <= places && (cost < best || (cost == best && len[k] > chunk))) best = cost, chunk = len[k];
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float other = __shfl_xor_sync(0xffffffffu, best, o);
+    const int c = __shfl_xor_sync(0xffffffffu, chunk, o);
+    if (other < best || (other == best && c > chunk)) best = other, chunk = c;
+  }
+  return chunk;
+}
+// Item `index` in the order groups, (kv head, chunk of heads), chunks of keys, tiles of rows; false behind the last.
+// By a whole warp; `t` keeps the first 32 groups' tiles.
+__device__ __forceinline__ bool find_item(const PrefixArgs& a, const GroupTiles& t, int H, int tokens, int tile, int chunk,
+                                          int index, PrefixItem& it) {
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  for (int g0 = 0; g0 < a.G; g0 += 32) {
+    GroupTiles mine = t;
+    if (g0) mine.load(a, g0 + lane, tokens, tile);
+    const int splits = (mine.nt + chunk - 1) / chunk, items = mine.mt * H * splits;
+    int sum = items;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += up;
+    }
+    const unsigned has = __ballot_sync(0xffffffffu, index < before + sum);
+    if (has) {
+      const int who = __ffs(has) - 1;
+      const int mt = __shfl_sync(0xffffffffu, mine.mt, who), s = __shfl_sync(0xffffffffu, splits, who);
+      const int rest = index - before - __shfl_sync(0xffffffffu, sum - items, who);
+      it.g = g0 + who;
+      it.m = rest % mt;
+      it.split = rest / mt % s;
+      it.hc = rest / mt / s;
+      const int all = __shfl_sync(0xffffffffu, mine.count, who);
+      it.first = __shfl_sync(0xffffffffu, mine.first, who) + it.m * tokens;
+      it.count = min(tokens, all - it.m * tokens);
+      it.length = __shfl_sync(0xffffffffu, mine.length, who);
+      it.tiles = __shfl_sync(0xffffffffu, mine.nt, who);
+      return true;
+    }
+    before += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return false;
+}
+
+// ------------------------------------------------------------------------------------- requests' own tokens
+struct Request {
+  int first, count, len, shared, g;     // its rows, its own tokens, tokens of the prefix (0 where that is another kernel's)
+  int far, near;                        // tiles of the prefix, of the own tokens
+  __device__ __forceinline__ int tiles() const { return max(1, far + near); }
+  __device__ __forceinline__ int row_tiles(int tokens) const { return (count + tokens - 1) / tokens; }
+};
+__device__ __forceinline__ Request request_of(const PrefixArgs& a, int b, bool both, int tile) {
+  Request r;
+  const Rows rows = rows_of(a, b);
+  r.first = rows.first, r.count = rows.count, r.len = own_length(a, b);
+  r.g = both ? group_of(a, b) : -1;
+  r.shared = prefix_length(a, r.g);
+  r.far = (r.shared + tile - 1) / tile, r.near = (r.len + tile - 1) / tile;
+  return r;
+}
+// Where a block's run is: tiles `off` on of the row tile `rt` of request b, for heads hc.
+struct Cursor {
+  int hc, b, rt, off;
+  long long todo;
+};
+// What the joining kernel needs of the division: a run's tiles, the tiles of one (kv head, chunk of heads), and the tiles
+// before every request's.
+struct OwnPlan {
+  long long run, each;
+  long long base[1];            // [B]
+};
+constexpr int kLeastRun = 4;    // the fewest tiles of a run
+
+// The run of block `k` of `blocks`, by the first `threads` threads of the block (a multiple of 32; all call); `plan`: where the
+// division is written down, by the block that is given it.
+template <int THREADS>
+__device__ __forceinline__ Cursor find_run(const PrefixArgs& a, int H, int tokens, int tile, bool both, int k, int blocks,
+                                           OwnPlan* plan) {
+  __shared__ long long counts[THREADS / 32];
+  __shared__ Cursor found;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int each = (a.B + THREADS - 1) / THREADS, b0 = min((int)threadIdx.x * each, a.B), b1 = min(b0 + each, a.B);
+  long long mine = 0, total = 0;
+  if (threadIdx.x < THREADS)
+    for (int b = b0; b < b1; ++b) {
+      const Request r = request_of(a, b, both, tile);
+      mine += (long long)r.row_tiles(tokens) * r.tiles();
+    }
+  long long sum = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long up = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += up;
+  }
+  if (lane == 31 && warp < THREADS / 32) counts[warp] = sum;
+  if (threadIdx.x == 0) found.todo = 0;
+  __syncthreads();
+  long long start = sum - mine;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < warp) start += counts[w];
+    total += counts[w];
+  }
+  const long long all = total * H, share = (all + blocks - 1) / blocks;
+  const long long run = share > kLeastRun ? share : kLeastRun, at = run * k;
+  if (plan && threadIdx.x < THREADS) {
+    if (threadIdx.x == 0) plan->run = run, plan->each = total;
+    long long base = start;
+    for (int b = b0; b < b1; ++b) {
+      const Request r = request_of(a, b, both, tile);
+      plan->base[b] = base;
+      base += (long long)r.row_tiles(tokens) * r.tiles();
+    }
+  }
+  if (at < all && threadIdx.x < THREADS) {
+    const int hc = (int)(at / total);
+    long long rest = at - hc * total;
+    if (rest >= start && rest < start + mine) {
+      rest -= start;
+      for (int b = b0; b < b1; ++b) {
+        const Request r = request_of(a, b, both, tile);
+        const long long tiles = r.tiles(), here = r.row_tiles(tokens) * tiles;
+        if (rest < here) {
+          found = {hc, b, (int)(rest / tiles), (int)(rest % tiles), min(run, all - at)};
+          break;
+        }
+        rest -= here;
+      }
+    }
+  }
+  __syncthreads();
+  return found;
 }
 
 }  // namespace gf

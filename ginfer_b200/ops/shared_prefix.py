@@ -8,15 +8,19 @@ All work goes to the current stream; nothing but scratch memory is kept between 
 """
 from __future__ import annotations
 
+import functools
 import struct
+import threading
+from ctypes import c_char_p, c_longlong
 
 import torch
 
 from . import _Counter, _ok
-from .quant_cache import _at, _code, _device, _function, _raw_stream
+from .build import load_library
+from .quant_cache import _at, _capturing, _code, _device, _function, _of_device, _raw_stream
 
 MAX_HEAD_DIM = 256
-_ATTEND = struct.Struct("=25qd")
+_ATTEND = struct.Struct("=29qd")
 _int32 = torch.int32
 
 
@@ -37,6 +41,31 @@ def _vector(t, count, what, device):
     if t.dtype is not _int32 or t.dim() != 1 or t.shape[0] != count or not t.is_contiguous():
         raise ValueError(f"{what} is int32 [{count}], contiguous; got {t.dtype} {tuple(t.shape)}")
     return _at(t, device)
+
+
+# What a call's scratch depends on, in the order of the words that the library takes.
+@functools.lru_cache(maxsize=1024)
+def _scratch_bytes(hd, code, G, prefix_limit, B, T, nh, nkv, sms) -> int:
+    f = load_library("shared_prefix", (f"GF_HEAD_DIM={hd}",)).gf_prefix_scratch
+    f.argtypes, f.restype = [c_char_p], c_longlong
+    return f(_ATTEND.pack(0, 0, code, 0, 0, 1, 1, 0, 0, 0, G, prefix_limit, 0, 0, 0, B, 0, 0, 0, 0, T, nh, nkv, sms, 0, 0, 0, 0, 0,
+                          1.0))
+
+
+_scratch: dict = {}
+# Held from the choice of the scratch until the kernels that use it are in their stream: the foreign call lets other
+# threads run, and another call on the stream between two of this one's kernels would overwrite its pieces.
+_launching = threading.Lock()
+
+
+def _scratch_for(size: int, device: int, stream: int) -> torch.Tensor:
+    """A buffer that only this stream's calls use; a graph that is being captured keeps one of its own."""
+    if _capturing():
+        return torch.empty(size, dtype=torch.uint8, device=device)
+    buf = _scratch.get((device, stream))
+    if buf is None or buf.numel() < size:
+        buf = _scratch[device, stream] = torch.empty(max(size, 1 << 20), dtype=torch.uint8, device=device)
+    return buf
 
 
 def attend(q: torch.Tensor, nh: int, pages, prefix_table: torch.Tensor, prefix_lens: torch.Tensor,
@@ -72,10 +101,14 @@ def attend(q: torch.Tensor, nh: int, pages, prefix_table: torch.Tensor, prefix_l
     if q.dim() != 2 or q.shape[1] < nh * hd or (q.stride(1) != 1 and q.shape[1] > 1) or q.dtype != k.dtype:
         raise ValueError(f"q has rows of at least {nh * hd} channels without gaps in the cache's type {k.dtype}; got "
                          f"{q.dtype} {tuple(q.shape)}, strides {tuple(q.stride())}")
-    code, at = _code(q.dtype), _at(q, dev)
+    code, at, stride = _code(q.dtype), _at(q, dev), q.stride(0)
+    if (at | stride * q.itemsize) & 15:            # (the kernels read 16 bytes at a time)
+        q = q[:, :nh * hd].contiguous()
+        at, stride = q.data_ptr(), nh * hd
     T, B, G = q.shape[0], lengths.shape[0], prefix_lens.shape[0]
     prefix, prefix_stride, P = _table(prefix_table, G, "prefix_table", dev)
     table, table_stride, W = _table(block_table, B, "block_table", dev)
+    prefix_tokens, own_tokens = _vector(prefix_lens, G, "prefix_lens", dev), _vector(lengths, B, "lengths", dev)
     groups = rows = 0
     if cu_groups is not None:
         groups = _vector(cu_groups, G + 1, "cu_groups", dev)
@@ -95,11 +128,21 @@ def attend(q: torch.Tensor, nh: int, pages, prefix_table: torch.Tensor, prefix_l
         out = q.new_empty(T, nh * hd)
     elif out.dtype != q.dtype or out.shape != (T, nh * hd) or not out.is_contiguous():
         raise ValueError(f"out is {q.dtype} {(T, nh * hd)}, contiguous; got {out.dtype} {tuple(out.shape)}")
-    rc = _function("shared_prefix", "gf_prefix_attend")(_ATTEND.pack(
-        at, q.stride(0), code, k.data_ptr(), _at(v, dev), count, page, prefix, prefix_stride,
-        _vector(prefix_lens, G, "prefix_lens", dev), G, P * page, table, table_stride, _vector(lengths, B, "lengths", dev),
-        B, W * page, groups, rows, _at(out, dev), T, nh, nkv, hd, _raw_stream(dev), scale))
-    _Counter.launches += 1
+    if (k.data_ptr() | v.data_ptr() | out.data_ptr()) & 15:
+        raise ValueError("the cache's planes and out start at multiples of 16 bytes")
+    if T == 0 or B == 0:
+        return out
+    sms, err = _of_device(dev)
+    stream = _raw_stream(dev)
+    size = _scratch_bytes(hd, code, G, P * page, B, T, nh, nkv, sms)
+    f = _function("shared_prefix", "gf_prefix_attend", (f"GF_HEAD_DIM={hd}",))
+    with _launching:
+        scratch = _scratch_for(size, dev, stream)
+        rc = f(_ATTEND.pack(at, stride, code, k.data_ptr(), _at(v, dev), count, page, prefix, prefix_stride,
+                            prefix_tokens, G, P * page, table, table_stride,
+                            own_tokens, B, W * page, groups, rows, _at(out, dev), T, nh, nkv, sms,
+                            max_q_len or -(-T // B), scratch.data_ptr(), size, err, stream, scale))
+    _Counter.launches += 3
     if rc:
         _ok(rc, "shared_prefix.attend")
     return out

@@ -15,6 +15,10 @@ def calls(monkeypatch):
     monkeypatch.setattr(shared_prefix, "_device", lambda t: "cpu")
     monkeypatch.setattr(shared_prefix, "_at", lambda t, device: t.data_ptr())
     monkeypatch.setattr(shared_prefix, "_raw_stream", lambda device: 5)
+    monkeypatch.setattr(shared_prefix, "_of_device", lambda device: (148, 0))
+    monkeypatch.setattr(shared_prefix, "_scratch_bytes", lambda *sizes: 64)
+    monkeypatch.setattr(shared_prefix, "_capturing", lambda: False)
+    monkeypatch.setattr(shared_prefix, "_scratch", {})
     return got
 
 
@@ -52,6 +56,7 @@ def test_what_is_served(calls):
     (dict(block_table=i32(4, 3).t()), ValueError), (dict(block_table=i32(2, 4)), ValueError), (dict(lengths=i32(4)), ValueError),
     (dict(lengths=i32(6)[::2]), ValueError), (dict(cu_groups=i32(3)), ValueError), (dict(cu_seqlens_q=i32(3)), ValueError),
     (dict(cu_seqlens_q=i32(4).long()), ValueError), (dict(max_q_len=-1), ValueError), (dict(scale=0.0), ValueError), (dict(scale=float("nan")), ValueError),
+    (dict(out=torch.zeros(769)[1:].view(3, 256)), ValueError), (dict(pages=torch.zeros(2 * 9 * 16 * 128 + 1)[1:].view(2, 9, 16, 2, 64)), ValueError),
     (dict(out=torch.zeros(3, 257)), ValueError), (dict(out=torch.zeros(3, 256).bfloat16()), ValueError), (dict(out=torch.zeros(256, 3).t()), ValueError)])
 def test_refusals(calls, changed, error):
     with pytest.raises(error):

@@ -1,12 +1,18 @@
 // Attention of a batch's newest tokens over a prefix that a group of requests shares and over their own tokens, compiled
 // for one head size (-DGF_HEAD_DIM=<multiple of 16, at most 256>):
 //   out[t, h] = sum_c softmax_c(scale <q[t, h], K_c>) V_c.
+#ifndef GF_HEAD_DIM
+#define GF_HEAD_DIM 128
+#endif
+
 #include "attention_tc.cuh"
 #include "mma_bits.cuh"
 #include "shared_prefix.cuh"
 
-#ifndef GF_HEAD_DIM
-#define GF_HEAD_DIM 128
+#if GF_HEAD_DIM == 64 || GF_HEAD_DIM == 128
+#define GF_PREFIX_TC 1
+#else
+#define GF_PREFIX_TC 0
 #endif
 
 // (Internal to this library: a static of a template would be shared with the libraries of other head sizes.)
@@ -15,6 +21,19 @@ namespace {
 
 constexpr int HD = GF_HEAD_DIM;
 static_assert(HD % 16 == 0 && HD >= 16 && HD <= 256, "head size must be a multiple of 16, <= 256");
+
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, int* err, int code) {
+  const uint32_t addr = smem_u32(bar);
+  for (uint32_t spin = 0; spin < kSpinLimit; ++spin) {
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done) : "r"(addr), "r"(parity) : "memory");
+    if (done) return true;
+    if (spin > 1024) __nanosleep(64);
+  }
+  if (err) atomicCAS(err, 0, code);
+  return false;
+}
 
 // ------------------------------------------------------------------------------------- pieces on mma.sync
 constexpr int TILE = 64;                         // keys of a tile
@@ -193,19 +212,6 @@ __device__ __forceinline__ void mma_step(const unsigned char* stage, int key, in
       mma16816(o[2 * n2 + 1], w, b[2], b[3]);
     }
   }
-}
-
-__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, int* err, int code) {
-  const uint32_t addr = smem_u32(bar);
-  for (uint32_t spin = 0; spin < kSpinLimit; ++spin) {
-    uint32_t done;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                 : "=r"(done) : "r"(addr), "r"(parity) : "memory");
-    if (done) return true;
-    if (spin > 1024) __nanosleep(64);
-  }
-  if (err) atomicCAS(err, 0, code);
-  return false;
 }
 
 __global__ void __launch_bounds__(THREADS, BLOCKS_AN_SM)
@@ -470,6 +476,16 @@ prefix_pieces_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
   }
 }
 
+}  // namespace
+}  // namespace gf
+
+#if GF_PREFIX_TC
+#include "shared_prefix_tc.cuh"
+#endif
+
+namespace gf {
+namespace {
+
 // ------------------------------------------------------------------------------------- joining
 // A row's pieces, a warp a row: those of its prefix, then those of its own tokens, in order.
 struct JoinArgs {
@@ -670,6 +686,20 @@ bool page_map(CUtensorMap* map, const void* plane, const PrefixArgs& a, int rows
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+#if GF_PREFIX_TC
+// 64 channels of the query heads of some rows
+bool query_map(CUtensorMap* map, const PrefixArgs& a, const Shape& shape) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[3] = {(cuuint64_t)HD, (cuuint64_t)a.nh, (cuuint64_t)a.T};
+  cuuint64_t strides[2] = {(cuuint64_t)HD * 2, (cuuint64_t)a.q_stride * 2};
+  cuuint32_t box[3] = {64u, (cuuint32_t)shape.heads, (cuuint32_t)shape.tokens}, steps[3] = {1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(a.q), dims, strides, box, steps,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+#endif
+
 }  // namespace
 }  // namespace gf
 
@@ -683,8 +713,8 @@ GF_DEFINE_PDL_SWITCH
 struct Call {
   PieceArgs p;
   JoinArgs j;
-  int type, blocks, longest;
-  bool shared;
+  int type, blocks, longest, sms;
+  bool shared, tensor;         // tensor: prefixes on the 5th-generation tensor cores
   char* scratch;
   long long room, need;
   cudaStream_t stream;
@@ -702,7 +732,7 @@ struct Call {
     a.table = (const int*)ptr(), a.table_stride = num(), a.lengths = (const int*)ptr(), a.B = num(), a.limit = num();
     a.cu_groups = (const int*)ptr(), a.cu = (const int*)ptr(), a.out = ptr();
     a.T = num(), a.nh = num(), a.nkv = num();
-    const int sms = num();
+    sms = num();
     longest = num();
     scratch = (char*)ptr(), room = w[i++];
     p.err = (int*)ptr(), stream = (cudaStream_t)ptr();
@@ -726,10 +756,14 @@ struct Call {
     p.cut_o = (float*)take(cut * HD * 4), p.cut_ml = (float2*)take(cut * 8);
     if (shared) {
       p.row_o = (float*)take(rows * HD * 4), p.row_ml = (float2*)take(rows * 8);
-      const long long tiles = (long long)p.H * ((a.T + p.shape.tokens - 1) / p.shape.tokens + a.G);
-      p.places = (int)(tiles > 2 * blocks ? tiles : 2 * blocks);
-      p.far_o = (float*)take((long long)p.places * MOST_ROWS * HD * 4);
-      p.far_ml = (float2*)take((long long)p.places * MOST_ROWS * 8);
+      tensor = GF_PREFIX_TC && type == GF_BF16 && a.page % 8 == 0 && 128 % a.page == 0;
+      j.far_tile = tensor ? 128 : TILE, j.far_rows = tensor ? 128 : MOST_ROWS;
+      j.far_shape = row_shape_of(a.nh, a.nkv, j.far_rows);
+      const long long tiles = (long long)a.nkv * j.far_shape.chunks * ((a.T + j.far_shape.tokens - 1) / j.far_shape.tokens + a.G);
+      const long long least = 2ll * (tensor ? sms : blocks);
+      p.places = (int)(tiles > least ? tiles : least);
+      p.far_o = (float*)take((long long)p.places * j.far_rows * HD * 4);
+      p.far_ml = (float2*)take((long long)p.places * j.far_rows * 8);
     }
   }
 };
@@ -759,10 +793,25 @@ GF_EXPORT int gf_prefix_attend(const char* words) {
   }
   JoinArgs& j = c.j;
   if (c.shared) {
-    p.mode = PREFIX;
-    const int rc = launch_kernel(prefix_pieces_kernel, dim3(c.blocks), dim3(THREADS), PIECES_SMEM, c.stream, mk, mv, p);
+    int rc;
+#if GF_PREFIX_TC
+    if (c.tensor) {
+      static OncePerDevice tc_attrs;
+      rc = tc_attrs.run([&] {
+        return cudaFuncSetAttribute(tc::prefix_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tc::SMEM);
+      });
+      if (rc) return rc;
+      const tc::Args t{a, j.far_shape, a.nkv * j.far_shape.chunks, p.places, a.pages * a.page, p.chunk, p.far_o, p.far_ml, p.err};
+      CUtensorMap tq, tk, tv;
+      if (!query_map(&tq, a, j.far_shape) || !page_map(&tk, a.k, a, a.page) || !page_map(&tv, a.v, a, a.page)) return -7;
+      rc = launch_kernel(tc::prefix_tc_kernel, dim3(c.sms), dim3(tc::NTHREADS_TC), tc::SMEM, c.stream, tq, tk, tv, t);
+    } else
+#endif
+    {
+      p.mode = PREFIX;
+      rc = launch_kernel(prefix_pieces_kernel, dim3(c.blocks), dim3(THREADS), PIECES_SMEM, c.stream, mk, mv, p);
+    }
     if (rc) return rc;
-    j.far_tile = TILE, j.far_rows = MOST_ROWS, j.far_shape = p.shape;
     p.after = 1;
   }
   p.mode = c.shared ? OWN : BOTH, p.joined = 1;

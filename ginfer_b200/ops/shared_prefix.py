@@ -102,7 +102,7 @@ def attend(q: torch.Tensor, nh: int, pages, prefix_table: torch.Tensor, prefix_l
         raise ValueError(f"q has rows of at least {nh * hd} channels without gaps in the cache's type {k.dtype}; got "
                          f"{q.dtype} {tuple(q.shape)}, strides {tuple(q.stride())}")
     code, at, stride = _code(q.dtype), _at(q, dev), q.stride(0)
-    if (at | stride * q.itemsize) & 15:            # (the kernels read 16 bytes at a time)
+    if (at | stride * q.itemsize) & 15 or stride < nh * hd:            # (the kernels read 16 bytes at a time)
         q = q[:, :nh * hd].contiguous()
         at, stride = q.data_ptr(), nh * hd
     T, B, G = q.shape[0], lengths.shape[0], prefix_lens.shape[0]

@@ -575,16 +575,27 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) prefix_join_kernel(const Join
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[c][e] *= keep;
       const int n = min(32, pieces - k);
-#pragma unroll 4
-      for (int q = 0; q < n; ++q) {
-        const float wq = __shfl_sync(0xffffffffu, w, q);
-        const float* from_o = (const float*)__shfl_sync(0xffffffffu, (unsigned long long)po, q);
+      // (eight pieces' values are on their way at once; what weighs nothing is not looked at)
+      for (int q0 = 0; q0 < n; q0 += 8) {
+        float4 y[8][JOIN_CH];
+        float wq[8];
 #pragma unroll
-        for (int c = 0; c < JOIN_CH; ++c)
-          if (128 * c + 4 * lane < HD && wq != 0.f) {
-            const float4 y = __ldcg(reinterpret_cast<const float4*>(from_o + 128 * c + 4 * lane));
-            acc[c][0] += wq * y.x, acc[c][1] += wq * y.y, acc[c][2] += wq * y.z, acc[c][3] += wq * y.w;
-          }
+        for (int q = 0; q < 8; ++q) {
+          wq[q] = __shfl_sync(0xffffffffu, w, (q0 + q) & 31);
+          const float* from_o = (const float*)__shfl_sync(0xffffffffu, (unsigned long long)po, min(q0 + q, n - 1));
+          if (q0 + q >= n) wq[q] = 0.f;
+#pragma unroll
+          for (int c = 0; c < JOIN_CH; ++c)
+            y[q][c] = 128 * c + 4 * lane < HD ? __ldcg(reinterpret_cast<const float4*>(from_o + 128 * c + 4 * lane))
+                                              : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+#pragma unroll
+          for (int c = 0; c < JOIN_CH; ++c)
+            if (wq[q] != 0.f)
+              acc[c][0] += wq[q] * y[q][c].x, acc[c][1] += wq[q] * y[q][c].y, acc[c][2] += wq[q] * y[q][c].z,
+                  acc[c][3] += wq[q] * y[q][c].w;
       }
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -818,5 +829,8 @@ GF_EXPORT int gf_prefix_attend(const char* words) {
   const int rc = launch_kernel(prefix_pieces_kernel, dim3(c.blocks), dim3(THREADS), PIECES_SMEM, c.stream, mk, mv, p);
   if (rc) return rc;
   j.p = p, j.own_blocks = c.blocks;
-  return launch_kernel(prefix_join_kernel<bf16>, dim3(a.B, a.nkv), dim3(32 * JOIN_WARPS), 0, c.stream, j);
+  // (a warp a row where the requests have as many as is said)
+  const long long per = (long long)(c.longest < 1 ? 1 : c.longest) * (a.nh / a.nkv);
+  const unsigned z = (unsigned)(per > 64 * JOIN_WARPS ? 64 : (per + JOIN_WARPS - 1) / JOIN_WARPS);
+  return launch_kernel(prefix_join_kernel<bf16>, dim3(a.B, a.nkv, z), dim3(32 * JOIN_WARPS), 0, c.stream, j);
 }

@@ -14,8 +14,10 @@ import torch
 
 from . import _Counter, _ok
 from .quant_cache import _at, _code, _device, _function, _raw_stream
+from .shared_prefix import _launching, _scratch_for
 
-_VERIFY = struct.Struct("=15q")
+PIECE = 4096                   # logits of a piece of a row (the library has the same number)
+_VERIFY = struct.Struct("=17q")
 
 
 def _rows(x, rows, columns, what, device):
@@ -64,15 +66,18 @@ def verify(logits: torch.Tensor, tokens: torch.Tensor, cu_rows: torch.Tensor, te
         if draft_logits.dtype != logits.dtype:
             raise TypeError(f"the drafter's logits have the target's type {logits.dtype}, not {draft_logits.dtype}")
         y, draft_stride = _rows(draft_logits, R, V, "draft_logits", dev)
-    if V >= 1 << 30 or R >= 1 << 30:
-        raise ValueError(f"{R} rows of {V} logits: both are below 2^30")
+    if V >= 1 << 28 or R >= 1 << 30 or B >= 1 << 28:
+        raise ValueError(f"{R} rows of {V} logits for {B} requests: fewer than 2^30 rows, 2^28 logits and requests")
+    facts = (x, stride, code, y, draft_stride, _vector(tokens, R, torch.int32, "tokens", dev),
+             _vector(cu_rows, B + 1, torch.int32, "cu_rows", dev),
+             _vector(temperature, B, torch.float32, "temperature", dev), _vector(u, R, torch.float32, "u", dev))
     accepted = tokens.new_empty(2, B)
-    rc = _function("drafts", "gf_verify")(_VERIFY.pack(
-        x, stride, code, y, draft_stride, _vector(tokens, R, torch.int32, "tokens", dev),
-        _vector(cu_rows, B + 1, torch.int32, "cu_rows", dev), _vector(temperature, B, torch.float32, "temperature", dev),
-        _vector(u, R, torch.float32, "u", dev), accepted.data_ptr(), accepted.data_ptr() + 4 * B, R, V, B,
-        _raw_stream(dev)))
-    _Counter.launches += 1
+    stream, size = _raw_stream(dev), 16 * R * (V // PIECE + 2)
+    with _launching:
+        scratch = _scratch_for(size, dev, stream)
+        rc = _function("drafts", "gf_verify")(_VERIFY.pack(*facts, accepted.data_ptr(), accepted.data_ptr() + 4 * B, R, V, B,
+                                                           scratch.data_ptr(), size, stream))
+    _Counter.launches += 2
     if rc:
         _ok(rc, "drafts.verify")
     return accepted[0], accepted[1]

@@ -12,6 +12,7 @@ def calls(monkeypatch):
     monkeypatch.setattr(drafts, "_device", lambda t: "cpu")
     monkeypatch.setattr(drafts, "_at", lambda t, device: t.data_ptr())
     monkeypatch.setattr(drafts, "_raw_stream", lambda device: 5)
+    monkeypatch.setattr(drafts, "_scratch_for", lambda size, device, stream: torch.empty(size, dtype=torch.uint8))
     return got
 
 
@@ -42,6 +43,16 @@ def test_refusals(calls, changed, error):
     with pytest.raises(error):
         drafts.verify(**good(**changed))
     assert not calls
+
+
+def test_the_pieces_of_a_row():
+    """Both sides of the call know how many there are."""
+    import os
+    import re
+    from ginfer_b200.ops.build import CSRC_DIR
+    with open(os.path.join(CSRC_DIR, "drafts.cu")) as f:
+        scan, each = re.search(r"kScan = (\d+), kEach = (\d+), kPiece = kScan \* kEach", f.read()).groups()
+    assert int(scan) * int(each) == drafts.PIECE
 
 
 def test_a_device_is_needed():

@@ -5,25 +5,30 @@
 // w = max(p - q, 0) (w = p behind the last draft) reaches u times the whole, among those with w > 0.
 //
 // What bounds it is reading the logits, once.  Two launches:
-//  * verify_scan_kernel: every row in pieces of kPiece logits, each leaves its maximum and, relative to that, the sum of its
-//    weights in 32 bits (requests of temperature zero: the maximum's first place).
+//  * verify_scan_kernel: every row in pieces, each leaves its maximum and, relative to that, the sum of its weights in 32 bits
+//    (requests of temperature zero: the maximum's first place).
 //  * verify_decide_kernel: a cluster of blocks a request adds the pieces up, goes through the drafts and draws the next token
 //    from the one row that it needs.
 // 32 bits are enough to decide on nearly every draft; where u q(d) and p(d) are within kMargin of one another, the two rows'
-// sums are taken again in 64 bits.  The drawn token is met by errors of the order of 2^-24 now and then (a border between two
-// tokens is as near as 1 / V), so that everything about it is in 64 bits: weights above e^-20 of the largest, and all sums;
-// a smaller weight's own error in 32 bits, 2^-22 of it, is below 2^-50 of the whole.
+// sums are taken again in 64 bits.  The drawn token is met by errors of the order of 2^-24 now and then (there are V borders
+// between tokens), so that its sums are in 64 bits, and so are the weights above e^-10 of the largest, of which there are
+// few in a row that a model is sure about.  A smaller weight's factors 2^(n/256) come from a table in 64 bits and what is left,
+// 1 + 1.4e-3 at most, from a short series in 32: off by 2e-10 of it, below 1e-14 of the largest.
+#include <cstdlib>
+
 #include "common.cuh"
 #include "tc_common.cuh"
 
 namespace gf {
 namespace {
 
-constexpr int kScan = 256, kEach = 16, kPiece = kScan * kEach;        // threads of a scanning block, logits of a thread
+constexpr int kPiece = 1024;                            // logits of a piece
+constexpr int kScan = 256, kScanBlocks = 2;             // threads of a scanning block, blocks an SM
+constexpr int kSearch = 1024;                           // requests whose first rows a scanning block keeps
 constexpr int kDecide = 512, kWarps = kDecide / 32, kBatch = 32;      // rows whose sums are at hand at a time
-constexpr int kMostCluster = 8;
+constexpr int kAhead = 4;                               // loads of a row that are under way
 // Relative error that the 32-bit sums may have: exponents are off by 2^-23 of up to 20 and the exponential by 2^-22, sums of
-// 16 and across threads by less: 4e-6 for p and for q; ten times that.
+// 64 and across lanes by less: 5e-6 for p and for q; eight times that for both.
 constexpr double kMargin = 8e-5;
 constexpr float kLog2E = 1.4426950408889634f;
 
@@ -42,6 +47,17 @@ struct VerifyArgs {
 };
 
 template <typename T> constexpr int kVec = 16 / (int)sizeof(T);
+template <typename T> constexpr int kLoads = kPiece / (32 * kVec<T>);              // a lane's of a piece
+template <typename T> __device__ __forceinline__ void unpack(const uint4& raw, float (&v)[kVec<T>]) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(w[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
 // A row in groups of 16 bytes that start at multiples of 16: group g has the logits g * kVec - mis on.
 template <typename T> struct Row {
   const T* x;
@@ -55,24 +71,20 @@ template <typename T> struct Row {
     const float y = j >= 0 && j < V ? fresh(x + j) : -INFINITY;
     return y == y ? y : -INFINITY;                    // (a NaN counts as nothing)
   }
-  // Group g's logits, -inf outside the row.
-  __device__ __forceinline__ void load(int g, float (&v)[kVec<T>]) const {
+  __device__ __forceinline__ bool whole(int g) const {
     const int j = g * kVec<T> - mis;
-    if (j >= 0 && j + kVec<T> <= V) {
-      const uint4 raw = __ldcg(reinterpret_cast<const uint4*>(x + j));
-      if constexpr (sizeof(T) == 4) {
-        v[0] = __uint_as_float(raw.x), v[1] = __uint_as_float(raw.y);
-        v[2] = __uint_as_float(raw.z), v[3] = __uint_as_float(raw.w);
-      } else {
-        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    return j >= 0 && j + kVec<T> <= V;
+  }
+  __device__ __forceinline__ uint4 raw(int g) const { return __ldcg(reinterpret_cast<const uint4*>(x + (g * kVec<T> - mis))); }
+  // Group g's logits, -inf outside the row and for a NaN.
+  __device__ __forceinline__ void load(int g, float (&v)[kVec<T>]) const {
+    if (whole(g)) {
+      unpack<T>(raw(g), v);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-      }
-#pragma unroll
-      for (int i = 0; i < kVec<T>; ++i) v[i] = v[i] == v[i] ? v[i] : -INFINITY;
+      for (int i = 0; i < kVec<T>; ++i) v[i] = fmaxf(v[i], -INFINITY);
     } else {
 #pragma unroll
-      for (int i = 0; i < kVec<T>; ++i) v[i] = at(j + i);
+      for (int i = 0; i < kVec<T>; ++i) v[i] = at(g * kVec<T> - mis + i);
     }
   }
 };
@@ -89,6 +101,25 @@ __device__ __forceinline__ float fast_exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Two fp32 operations in one instruction: the operands are pairs in 64-bit registers.
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 // log2(e) / T, finite: times a difference of zero it is zero
 __device__ __forceinline__ float inverse_heat(float heat) { return fminf(kLog2E / heat, 1e30f); }
 // A logit's weight beside the row's largest one, in 32 bits.
@@ -98,89 +129,194 @@ __device__ __forceinline__ float weight32(float x, float best, float c) {
 }
 
 // ------------------------------------------------------------------------------------- rows in pieces
+// A warp takes a piece after the other, the loads of the next one under way while it works on one.
 template <typename T>
-__global__ void __launch_bounds__(kScan) verify_scan_kernel(const VerifyArgs a) {
-  __shared__ float2 part[kScan / 32];
-  const int b = blockIdx.x, piece = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int G = kEach / kVec<T>;                  // groups of a thread
+__global__ void __launch_bounds__(kScan, kScanBlocks) verify_scan_kernel(const VerifyArgs a) {
+  __shared__ int starts[kSearch + 1];
+  constexpr int GROUPS = 32 * kLoads<T>;
+  const int lane = threadIdx.x & 31;
   pdl_trigger();
   pdl_wait();
-  const Span rows = rows_of(a, b);
-  const float heat = fresh(a.temperature + b);
-  const bool greedy = !(heat > 0.f);
-  const float c = inverse_heat(heat);
-  for (int row = rows.first + blockIdx.z; row < rows.end; row += gridDim.z) {
-    for (int which = 0; which < (a.draft && !greedy && row + 1 < rows.end ? 2 : 1); ++which) {
-      const Row<T> x(which ? a.draft : a.logits, which ? a.draft_stride : a.stride, row, a.V);
-      float v[G][kVec<T>], top = -INFINITY;
-      const int g0 = piece * (kPiece / kVec<T>) + threadIdx.x, end = x.groups();
+  const bool kept = a.B <= kSearch;
+  if (kept)
+    for (int i = threadIdx.x; i <= a.B; i += kScan) starts[i] = fresh_index(a.cu + i);
+  __syncthreads();
+  auto start_of = [&](int b) { return kept ? starts[b] : fresh_index(a.cu + b); };
+  // pieces of the target's rows, then of the drafter's; this warp's are `me`, `me` + `all`, ...
+  const long long half = (long long)a.R * a.pieces, units = a.draft ? 2 * half : half;
+  const long long me = (long long)blockIdx.x * (kScan / 32) + (threadIdx.x >> 5), all = (long long)gridDim.x * (kScan / 32);
+  for (long long u0 = me; u0 < units; u0 += 32 * all) {
+    // the next 32 of them, a lane each: row, piece and temperature, if somebody asks for it
+    const long long u = u0 + lane * all;
+    const int my_which = u >= half;
+    int my_row = 0, my_piece = 0;
+    float my_heat = 0.f;
+    bool there = u < units;
+    if (there) {
+      const long long at = my_which ? u - half : u;
+      my_row = at >> 32 ? (int)(at / a.pieces) : (int)((unsigned)at / (unsigned)a.pieces);
+      my_piece = (int)(at - (long long)my_row * a.pieces);
+      int low = 0, high = a.B;                          // the last request that does not start behind the row
+      while (high - low > 1) {
+        const int mid = (low + high) >> 1;
+        if (start_of(mid) <= my_row) low = mid;
+        else high = mid;
+      }
+      const int end = start_of(low + 1);
+      my_heat = fresh(a.temperature + low);
+      there = my_row >= start_of(low) && my_row < end && !(my_which && (!(my_heat > 0.f) || my_row + 1 >= min(end, a.R)));
+    }
+    unsigned left = __ballot_sync(0xffffffffu, there);
+    struct Unit {
+      int row, which, piece;
+      float heat;
+      bool whole;
+    };
+    auto fetch = [&](uint4 (&raw)[kLoads<T>]) {            // the next of the ballot's
+      const int who = __ffs(left) - 1;
+      left &= left - 1;
+      Unit x{__shfl_sync(0xffffffffu, my_row, who), __shfl_sync(0xffffffffu, my_which, who),
+             __shfl_sync(0xffffffffu, my_piece, who), __shfl_sync(0xffffffffu, my_heat, who), false};
+      const Row<T> r(x.which ? a.draft : a.logits, x.which ? a.draft_stride : a.stride, x.row, a.V);
+      x.whole = r.whole(x.piece * GROUPS) && r.whole(x.piece * GROUPS + GROUPS - 1);
+      if (x.whole) {
 #pragma unroll
-      for (int i = 0; i < G; ++i) {
-        if (g0 + i * kScan < end) {
-          x.load(g0 + i * kScan, v[i]);
+        for (int i = 0; i < kLoads<T>; ++i) raw[i] = r.raw(x.piece * GROUPS + i * 32 + lane);
+      }
+      return x;
+    };
+    auto work = [&](const Unit& x, const uint4 (&raw)[kLoads<T>]) {
+      const Row<T> r(x.which ? a.draft : a.logits, x.which ? a.draft_stride : a.stride, x.row, a.V);
+      const bool greedy = !(x.heat > 0.f);
+      const float c = inverse_heat(x.heat);
+      const int g0 = x.piece * GROUPS + lane;
+      float top = -INFINITY, second = 0.f;
+      if (x.whole) {
+        float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < kLoads<T>; ++i) {
+          float v[kVec<T>];
+          unpack<T>(raw[i], v);
+#pragma unroll
+          for (int k = 0; k < kVec<T>; ++k) t[k & 3] = fmaxf(t[k & 3], v[k]);       // (a NaN never is)
+        }
+        top = warp_max(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
+        if (greedy) {
+          int at = 0x7fffffff;
+#pragma unroll
+          for (int i = kLoads<T> - 1; i >= 0; --i) {
+            float v[kVec<T>];
+            unpack<T>(raw[i], v);
+#pragma unroll
+            for (int k = kVec<T> - 1; k >= 0; --k)
+              if (v[k] == top) at = (g0 + i * 32) * kVec<T> - r.mis + k;            // (the first of the lane's)
+          }
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) at = min(at, __shfl_xor_sync(0xffffffffu, at, o));
+          second = __int_as_float(at);
         } else {
+          // weights as they come; where one is no number (a NaN, infinities, a temperature of infinity) again with care
+          const uint64_t c2 = pack2(c, c), m2 = pack2(-top, -top);
+          uint64_t s2[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
 #pragma unroll
-          for (int k = 0; k < kVec<T>; ++k) v[i][k] = -INFINITY;
+          for (int i = 0; i < kLoads<T>; ++i) {
+            float v[kVec<T>];
+            unpack<T>(raw[i], v);
+#pragma unroll
+            for (int k = 0; k < kVec<T>; k += 2) {
+              float e0, e1;
+              unpack2(mul2(add2(pack2(v[k], v[k + 1]), m2), c2), e0, e1);
+              s2[(k >> 1) & 1] = add2(s2[(k >> 1) & 1], pack2(fast_exp2(e0), fast_exp2(e1)));
+            }
+          }
+          float s0, s1, s3, s4;
+          unpack2(s2[0], s0, s1);
+          unpack2(s2[1], s3, s4);
+          second = warp_sum((s0 + s1) + (s3 + s4));
         }
       }
+      if (!x.whole || (!greedy && !(second < INFINITY))) {
+        if (!x.whole) {
+#pragma unroll 1
+          for (int i = 0; i < kLoads<T>; ++i) {
+            float v[kVec<T>];
+            r.load(g0 + i * 32, v);
 #pragma unroll
-      for (int i = 0; i < G; ++i)
-#pragma unroll
-        for (int k = 0; k < kVec<T>; ++k) top = fmaxf(top, v[i][k]);
-      top = warp_max(top);
-      float second = 0.f;
-      if (greedy) {
+            for (int k = 0; k < kVec<T>; ++k) top = fmaxf(top, v[k]);
+          }
+          top = warp_max(top);
+        }
         int at = 0x7fffffff;
+        second = 0.f;
+#pragma unroll 1
+        for (int i = 0; i < kLoads<T> && top > -INFINITY; ++i) {
+          float v[kVec<T>];
+          r.load(g0 + i * 32, v);
 #pragma unroll
-        for (int i = 0; i < G; ++i)
-#pragma unroll
-          for (int k = 0; k < kVec<T>; ++k)
-            if (v[i][k] == top) at = min(at, (g0 + i * kScan) * kVec<T> - x.mis + k);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) at = min(at, __shfl_xor_sync(0xffffffffu, at, o));
-        second = __int_as_float(at);
-      } else if (top > -INFINITY) {
-        float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-        for (int i = 0; i < G; ++i)
-#pragma unroll
-          for (int k = 0; k < kVec<T>; k += 2) s0 += weight32(v[i][k], top, c), s1 += weight32(v[i][k + 1], top, c);
-        second = warp_sum(s0 + s1);
-      }
-      __syncthreads();
-      if (lane == 0) part[warp] = make_float2(top, second);
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        float2 y = part[0];
-        for (int w = 1; w < kScan / 32; ++w) {
-          const float2 z = part[w];
-          if (greedy) {
-            if (z.x > y.x || (z.x == y.x && __float_as_int(z.y) < __float_as_int(y.y))) y = z;
-          } else if (z.x > -INFINITY) {
-            const float best = fmaxf(y.x, z.x);
-            y.y = y.y * weight32(y.x, best, c) + z.y * weight32(z.x, best, c);
-            y.x = best;
+          for (int k = 0; k < kVec<T>; ++k) {
+            if (v[k] == top) at = min(at, (g0 + i * 32) * kVec<T> - r.mis + k);
+            second += weight32(v[k], top, c);
           }
         }
-        a.part[((size_t)row * 2 + which) * a.pieces + piece] = y;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) at = min(at, __shfl_xor_sync(0xffffffffu, at, o));
+        second = warp_sum(second);
+        if (greedy) second = __int_as_float(at);
       }
+      if (lane == 0) a.part[((size_t)x.row * 2 + x.which) * a.pieces + x.piece] = make_float2(top, second);
+    };
+    uint4 raw0[kLoads<T>], raw1[kLoads<T>];
+    Unit x0, x1;
+    if (left) x0 = fetch(raw0);
+    else continue;
+    while (true) {
+      const bool more = left != 0;
+      if (more) x1 = fetch(raw1);
+      work(x0, raw0);
+      if (!more) break;
+      const bool again = left != 0;
+      if (again) x0 = fetch(raw0);
+      work(x1, raw1);
+      if (!again) break;
     }
   }
 }
 
 // ------------------------------------------------------------------------------------- decisions
-// A logit's weight beside the row's largest one: in 64 bits where it counts (see above).
+constexpr int kTable = 256;
+// log2(e) / T in ways: for e^((x - best) / T) in 64 bits, times kTable as two floats, and as one.
 struct Heat {
   double inv;                  // 1 / T
-  float c;
+  float hi, lo, c;
+  const double* table;         // 2^(i / kTable)
+  __device__ __forceinline__ Heat(float heat, const double* table_) : inv(1. / (double)heat), table(table_) {
+    c = inverse_heat(heat);
+    const double whole = fmin(inv, 1e30) * (kTable * 1.4426950408889634);
+    hi = (float)whole, lo = (float)(whole - (double)hi);
+  }
 };
-__device__ __forceinline__ double weight64(float x, float best, const Heat& h) {
+__device__ __noinline__ double large_weight(float x, float best, double inv) {
   if (x == best) return x == -INFINITY ? 0. : 1.;
   if (x == -INFINITY || best == INFINITY) return 0.;
-  const float e = (x - best) * h.c;
-  if (e < -29.f) return (double)fast_exp2(e);         // (2^-29 is e^-20)
-  return exp(((double)x - (double)best) * h.inv);
+  return exp(((double)x - (double)best) * inv);
 }
+// A logit's weight beside the row's largest one, as exactly as it counts (see above).
+__device__ __forceinline__ double weight64(float x, float best, const Heat& h) {
+  const float d = x - best, e = d * h.c;
+  if (!(e < -14.4f) || best == INFINITY) return large_weight(x, best, h.inv);   // (2^-14.4 is e^-10; or e is no number)
+  if (e < -120.f) return 0.;                                       // (nothing beside the largest, 2^-100 of all V)
+  // d + rest is x - best, n whole and t what is left of (x - best) / T in units of ln 2 / kTable
+  const float back = d - x, rest = (x - (d - back)) + (-best - back);
+  const float shifted = fmaf(d, h.hi, 12582912.f), n = shifted - 12582912.f;
+  const float t = fmaf(rest, h.hi, fmaf(d, h.lo, fmaf(d, h.hi, -n)));
+  const float r = t * (0.6931471805599453f / kTable);
+  const float p = fmaf(r * r, fmaf(r, 1.f / 6.f, 0.5f), r);        // e^r - 1; r^4 / 24 is below 2e-13
+  const int whole = __float_as_int(shifted) - 0x4b400000;          // n
+  const double f = h.table[whole & (kTable - 1)];
+  const double w = fma(f, (double)p, f);
+  return __hiloint2double(__double2hiint(w) + ((whole >> 8) << 20), __double2loint(w));
+}
+static_assert(kTable == 256, "the shift above");
 __device__ __forceinline__ double shfl_xor(double v, int o) { return __shfl_xor_sync(0xffffffffu, v, o); }
 
 // What a row's weights are relative to, and their sum.
@@ -210,13 +346,45 @@ struct Cluster {
   }
 };
 
+// Loads of a row that are under way together: a lane's groups g, g + 32, ...
+template <typename T> struct Ahead {
+  uint4 raw[kAhead];
+  __device__ __forceinline__ void load(const Row<T>& x, int g, int end) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (g + 32 * i < end && x.whole(g + 32 * i)) raw[i] = x.raw(g + 32 * i);
+  }
+  __device__ __forceinline__ void get(const Row<T>& x, int i, int g, float (&v)[kVec<T>]) const {      // i: a constant
+    if (x.whole(g)) {
+      unpack<T>(raw[i], v);
+#pragma unroll
+      for (int k = 0; k < kVec<T>; ++k) v[k] = fmaxf(v[k], -INFINITY);
+    } else {
+      x.load(g, v);
+    }
+  }
+  __device__ __forceinline__ double sum(const Row<T>& x, int g, int end, float best, const Heat& h) const {
+    double s = 0.;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (g + 32 * i >= end) break;
+      float z[kVec<T>];
+      get(x, i, g + 32 * i, z);
+#pragma unroll
+      for (int k = 0; k < kVec<T>; ++k) s += weight64(z[k], best, h);
+    }
+    return s;
+  }
+};
+
 template <typename T>
-__global__ void __launch_bounds__(kDecide) verify_decide_kernel(const VerifyArgs a) {
+__global__ void __launch_bounds__(kDecide, 1) verify_decide_kernel(const VerifyArgs a) {
   __shared__ Total totals[kBatch][2];                 // of the batch's rows: the target's, the draft's
   __shared__ int places[kBatch];                      // greedy: the arg-max
   __shared__ double sums[kWarps][2];
   __shared__ __align__(16) double slots[2][2];
   __shared__ int verdict[2];
+  __shared__ double table[kTable];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   Cluster cl{cluster_rank(), 0, 0, slots};
   asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(cl.size));
@@ -231,27 +399,33 @@ __global__ void __launch_bounds__(kDecide) verify_decide_kernel(const VerifyArgs
   }
   const float heat = fresh(a.temperature + b);
   const bool greedy = !(heat > 0.f);
-  const Heat h{1. / (double)heat, inverse_heat(heat)};
+  if (threadIdx.x < kTable) table[threadIdx.x] = exp2((double)threadIdx.x / kTable);
+  const Heat h(heat, table);
   // this block's share of a row's groups of 16 bytes, and the warp's of that, in order
+  auto block_share = [&](int groups, int& g0, int& g1) {
+    const int each = (groups + (int)cl.size - 1) / (int)cl.size;
+    g0 = min(groups, (int)cl.rank * each), g1 = min(groups, g0 + each);
+  };
   auto share_of = [&](int groups, int& w0, int& w1) {
-    const int each = (groups + (int)cl.size - 1) / (int)cl.size, g0 = min(groups, (int)cl.rank * each), g1 = min(groups, g0 + each);
+    int g0, g1;
+    block_share(groups, g0, g1);
     const int per = (g1 - g0 + kWarps - 1) / kWarps;
     w0 = min(g1, g0 + warp * per), w1 = min(g1, w0 + per);
   };
   // both rows' sums of weights in 64 bits
   auto exact_totals = [&](int row, bool with_draft, float best, float draft_best, double& P, double& Q) {
     double s[2] = {0., 0.};
-    for (int which = 0; which < (with_draft ? 2 : 1); ++which) {
-      const Row<T> x(which ? a.draft : a.logits, which ? a.draft_stride : a.stride, row, a.V);
-      const float top = which ? draft_best : best;
-      int w0, w1;
-      share_of(x.groups(), w0, w1);
-      for (int g = w0 + lane; g < w1; g += 32) {
-        float v[kVec<T>];
-        x.load(g, v);
-#pragma unroll
-        for (int k = 0; k < kVec<T>; ++k) s[which] += weight64(v[k], top, h);
-      }
+    const Row<T> x(a.logits, a.stride, row, a.V), y(with_draft ? a.draft : a.logits, with_draft ? a.draft_stride : a.stride, row, a.V);
+    int x0, x1, y0, y1;
+    share_of(x.groups(), x0, x1);
+    share_of(y.groups(), y0, y1);
+    if (!with_draft) y1 = y0;
+    Ahead<T> vx, vy;
+    for (int gx = x0 + lane, gy = y0 + lane; gx < x1 || gy < y1; gx += 32 * kAhead, gy += 32 * kAhead) {
+      vx.load(x, gx, x1);
+      vy.load(y, gy, y1);
+      s[0] += vx.sum(x, gx, x1, best, h);
+      s[1] += vy.sum(y, gy, y1, draft_best, h);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s[0] += shfl_xor(s[0], o), s[1] += shfl_xor(s[1], o);
@@ -301,7 +475,7 @@ __global__ void __launch_bounds__(kDecide) verify_decide_kernel(const VerifyArgs
       }
       if (lane == 0) {
         totals[i][which] = {best, sum};
-        if (!which) places[i] = best == -INFINITY || at == 0x7fffffff ? 0 : at;
+        if (!which) places[i] = best == -INFINITY ? 0 : min(max(at, 0), a.V - 1);
       }
     }
     __syncthreads();
@@ -374,25 +548,17 @@ __global__ void __launch_bounds__(kDecide) verify_decide_kernel(const VerifyArgs
   // ---- the token behind the last draft that stays
   const bool with_draft = refused && a.draft;
   const float best = totals[in_batch][0].best, draft_best = with_draft ? totals[in_batch][1].best : 0.f;
-  if (!exact) exact_totals(row, with_draft, best, draft_best, P, Q);
+  if (with_draft && !exact) exact_totals(row, true, best, draft_best, P, Q);
   const Row<T> x(a.logits, a.stride, row, a.V), y(with_draft ? a.draft : a.logits, with_draft ? a.draft_stride : a.stride, row, a.V);
   const int d = refused ? fresh_index(a.tokens + row + 1) : -1;
-  const double inv_p = P > 0. ? 1. / P : 0., inv_q = with_draft && Q > 0. ? 1. / Q : 0.;
+  // (where nothing is taken off p its sum need not be known)
+  const double inv_p = !with_draft ? 1. : P > 0. ? 1. / P : 0., inv_q = Q > 0. ? 1. / Q : 0.;
   int w0, w1;
   share_of(x.groups(), w0, w1);
   // a group's weights: without `whole` what p has more than q
-  auto rest = [&](int g, bool whole, double (&w)[kVec<T>]) {
-    float v[kVec<T>], z[kVec<T>];
-    x.load(g, v);
+  const bool side_by_side = y.mis == x.mis;
+  auto rest = [&](int g, const float (&v)[kVec<T>], const float (&z)[kVec<T>], bool whole, double (&w)[kVec<T>]) {
     const int j = g * kVec<T> - x.mis;
-    if (with_draft && !whole) {
-      if (y.mis == x.mis) {
-        y.load(g, z);
-      } else {
-#pragma unroll
-        for (int k = 0; k < kVec<T>; ++k) z[k] = y.at(j + k);
-      }
-    }
 #pragma unroll
     for (int k = 0; k < kVec<T>; ++k) {
       w[k] = weight64(v[k], best, h) * inv_p;
@@ -400,14 +566,30 @@ __global__ void __launch_bounds__(kDecide) verify_decide_kernel(const VerifyArgs
       else if (refused && !whole && j + k == d) w[k] = 0.;
     }
   };
+  // what is taken off it: the draft's logits of the same tokens
+  auto beside = [&](int g, float (&z)[kVec<T>]) {
+#pragma unroll
+    for (int k = 0; k < kVec<T>; ++k) z[k] = y.at(g * kVec<T> - x.mis + k);
+  };
   const double u = fmin(fmax((double)fresh(a.u + rows.end - 1), 0.), 1. - 0x1p-24);     // (whatever is handed in)
   for (int whole = 0; whole < 2; ++whole) {           // (where nothing is left of p - q: p itself)
     double mine = 0.;
-    for (int g = w0 + lane; g < w1; g += 32) {
-      double w[kVec<T>];
-      rest(g, whole, w);
+    Ahead<T> vx, vy;
+    for (int g = w0 + lane; g < w1; g += 32 * kAhead) {
+      vx.load(x, g, w1);
+      if (with_draft && side_by_side) vy.load(y, g, w1);
 #pragma unroll
-      for (int k = 0; k < kVec<T>; ++k) mine += w[k];
+      for (int i = 0; i < kAhead; ++i) {
+        if (g + 32 * i >= w1) break;
+        float v[kVec<T>], z[kVec<T>] = {};
+        double w[kVec<T>];
+        vx.get(x, i, g + 32 * i, v);
+        if (with_draft && side_by_side) vy.get(y, i, g + 32 * i, z);
+        else if (with_draft) beside(g + 32 * i, z);
+        rest(g + 32 * i, v, z, whole, w);
+#pragma unroll
+        for (int k = 0; k < kVec<T>; ++k) mine += w[k];
+      }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mine += shfl_xor(mine, o);
@@ -431,25 +613,57 @@ __global__ void __launch_bounds__(kDecide) verify_decide_kernel(const VerifyArgs
         }
         ahead += sums[w][0];
       }
-      if (warp == owner) {
-        double run = owner_ahead;
+      // its share again, in smaller ones for all of the block's warps
+      int b0, b1;
+      block_share(x.groups(), b0, b1);
+      const int per = (b1 - b0 + kWarps - 1) / kWarps, seg0 = min(b1, b0 + owner * per), seg1 = min(b1, seg0 + per),
+                sub = (seg1 - seg0 + kWarps - 1) / kWarps;
+      const int s0 = min(seg1, seg0 + warp * sub), s1 = min(seg1, s0 + sub);
+      auto weights_at = [&](int g, double (&w)[kVec<T>]) {
+        if (g < s1) {
+          float v[kVec<T>], z[kVec<T>] = {};
+          x.load(g, v);
+          if (with_draft && side_by_side) y.load(g, z);
+          else if (with_draft) beside(g, z);
+          rest(g, v, z, whole, w);
+        } else {
+#pragma unroll
+          for (int k = 0; k < kVec<T>; ++k) w[k] = 0.;
+        }
+      };
+      double part = 0.;
+      for (int g = s0; g < s1; g += 32) {
+        double w[kVec<T>];
+        weights_at(g + lane, w);
+#pragma unroll
+        for (int k = 0; k < kVec<T>; ++k) part += w[k];
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) part += shfl_xor(part, o);
+      if (lane == 0) sums[warp][1] = part;
+      __syncthreads();
+      int finder = -1;
+      double run = 0.;
+      ahead = owner_ahead;
+      for (int w = 0; w < kWarps; ++w) {
+        if (sums[w][1] > 0. && (finder < 0 || ahead < target)) finder = w, run = ahead;
+        ahead += sums[w][1];
+      }
+      if (warp == finder) {
         int last = -1;
         bool found = false;
-        for (int g = w0; g < w1 && !found; g += 32) {
-          double w[kVec<T>], part = 0.;
-          if (g + lane < w1) rest(g + lane, whole, w);
-          else
+        for (int g = s0; g < s1 && !found; g += 32) {
+          double w[kVec<T>], mine_here = 0.;
+          weights_at(g + lane, w);
 #pragma unroll
-            for (int k = 0; k < kVec<T>; ++k) w[k] = 0.;
-#pragma unroll
-          for (int k = 0; k < kVec<T>; ++k) part += w[k];
-          double upto = part;
+          for (int k = 0; k < kVec<T>; ++k) mine_here += w[k];
+          double upto = mine_here;
 #pragma unroll
           for (int o = 1; o < 32; o <<= 1) {
             const double up = __shfl_up_sync(0xffffffffu, upto, o);
             if (lane >= o) upto += up;
           }
-          double at = run + (upto - part);
+          double at = run + (upto - mine_here);
           int pick = -1, latest = -1;
 #pragma unroll
           for (int k = 0; k < kVec<T>; ++k) {
@@ -482,7 +696,7 @@ using namespace gf;
 GF_DEFINE_PDL_SWITCH
 
 // `words`: logits, row stride, type, the drafter's logits, their row stride, tokens, cu, temperature, u, accepted, next, rows,
-// vocabulary, requests, scratch and its bytes, stream.
+// vocabulary, requests, scratch and its bytes, SMs, stream.
 GF_EXPORT int gf_verify(const char* words) {
   const long long* w = reinterpret_cast<const long long*>(words);
   VerifyArgs a;
@@ -496,18 +710,29 @@ GF_EXPORT int gf_verify(const char* words) {
   a.R = (int)w[i++], a.V = (int)w[i++], a.B = (int)w[i++];
   a.part = (float2*)ptr();
   const long long room = w[i++];
+  const int sms = (int)w[i++];
   cudaStream_t stream = (cudaStream_t)ptr();
   if (a.B <= 0) return 0;
   const bool half = type == GF_BF16;
   a.pieces = (a.V + (half ? kVec<bf16> : kVec<float>) - 1 + kPiece - 1) / kPiece;
   if ((long long)a.R * 2 * a.pieces * 8 > room) return -5;
-  if (a.pieces > 65535) return -6;
-  const int z = a.R > a.B ? (a.R + a.B - 1) / a.B : 1;
   int rc = 0;
-  if (a.R > 0)
-    rc = launch_kernel(half ? verify_scan_kernel<bf16> : verify_scan_kernel<float>, dim3(a.B, a.pieces, z < 64 ? z : 64),
+  if (a.R > 0) {
+    const long long units = (long long)a.R * a.pieces * (a.draft ? 2 : 1), most = (long long)sms * kScanBlocks;
+    const long long blocks = (units + kScan / 32 - 1) / (kScan / 32);
+    rc = launch_kernel(half ? verify_scan_kernel<bf16> : verify_scan_kernel<float>, dim3((unsigned)(blocks < most ? blocks : most)),
                        dim3(kScan), 0, stream, a);
+  }
   if (rc) return rc;
-  return launch_kernel_cluster_dims(half ? verify_decide_kernel<bf16> : verify_decide_kernel<float>, dim3(a.B * kMostCluster),
-                                    dim3(kDecide), 0, stream, kMostCluster, true, a);
+  static OncePerDevice attrs;
+  rc = attrs.run([&] {
+    const cudaError_t e = cudaFuncSetAttribute(verify_decide_kernel<bf16>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    return e != cudaSuccess ? e
+                            : cudaFuncSetAttribute(verify_decide_kernel<float>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  });
+  if (rc) return rc;
+  const char* env = getenv("GF_CLUSTER");
+  const int cluster = env ? atoi(env) : a.B <= 4 ? 16 : a.B <= 18 ? 8 : 4;
+  return launch_kernel_cluster_dims(half ? verify_decide_kernel<bf16> : verify_decide_kernel<float>, dim3(a.B * cluster),
+                                    dim3(kDecide), 0, stream, cluster, true, a);
 }

@@ -13,11 +13,11 @@ import struct
 import torch
 
 from . import _Counter, _ok
-from .quant_cache import _at, _code, _device, _function, _raw_stream
+from .quant_cache import _at, _code, _device, _function, _of_device, _raw_stream
 from .shared_prefix import _launching, _scratch_for
 
-PIECE = 4096                   # logits of a piece of a row (the library has the same number)
-_VERIFY = struct.Struct("=17q")
+PIECE = 1024                   # the least logits of a piece of a row (the library has the same number)
+_VERIFY = struct.Struct("=18q")
 
 
 def _rows(x, rows, columns, what, device):
@@ -72,11 +72,11 @@ def verify(logits: torch.Tensor, tokens: torch.Tensor, cu_rows: torch.Tensor, te
              _vector(cu_rows, B + 1, torch.int32, "cu_rows", dev),
              _vector(temperature, B, torch.float32, "temperature", dev), _vector(u, R, torch.float32, "u", dev))
     accepted = tokens.new_empty(2, B)
-    stream, size = _raw_stream(dev), 16 * R * (V // PIECE + 2)
+    stream, size, sms = _raw_stream(dev), 16 * R * (V // PIECE + 2), _of_device(dev)[0]
     with _launching:
         scratch = _scratch_for(size, dev, stream)
         rc = _function("drafts", "gf_verify")(_VERIFY.pack(*facts, accepted.data_ptr(), accepted.data_ptr() + 4 * B, R, V, B,
-                                                           scratch.data_ptr(), size, stream))
+                                                           scratch.data_ptr(), size, sms, stream))
     _Counter.launches += 2
     if rc:
         _ok(rc, "drafts.verify")

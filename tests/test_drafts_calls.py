@@ -12,6 +12,7 @@ def calls(monkeypatch):
     monkeypatch.setattr(drafts, "_device", lambda t: "cpu")
     monkeypatch.setattr(drafts, "_at", lambda t, device: t.data_ptr())
     monkeypatch.setattr(drafts, "_raw_stream", lambda device: 5)
+    monkeypatch.setattr(drafts, "_of_device", lambda device: (148, 0))
     monkeypatch.setattr(drafts, "_scratch_for", lambda size, device, stream: torch.empty(size, dtype=torch.uint8))
     return got
 
@@ -51,8 +52,7 @@ def test_the_pieces_of_a_row():
     import re
     from ginfer_b200.ops.build import CSRC_DIR
     with open(os.path.join(CSRC_DIR, "drafts.cu")) as f:
-        scan, each = re.search(r"kScan = (\d+), kEach = (\d+), kPiece = kScan \* kEach", f.read()).groups()
-    assert int(scan) * int(each) == drafts.PIECE
+        assert int(re.search(r"\bkPiece = (\d+)", f.read())[1]) == drafts.PIECE
 
 
 def test_a_device_is_needed():

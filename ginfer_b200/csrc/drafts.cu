@@ -8,12 +8,12 @@
 //  * verify_scan_kernel: every row in pieces, each leaves its maximum and, relative to that, the sum of its weights in 32 bits
 //    (requests of temperature zero: the maximum's first place).
 //  * verify_decide_kernel: a cluster of blocks a request adds the pieces up, goes through the drafts and draws the next token
-//    from the one row that it needs.
-// 32 bits are enough to decide on nearly every draft; where u q(d) and p(d) are within kMargin of one another, the two rows'
-// sums are taken again in 64 bits.  The drawn token is met by errors of the order of 2^-24 now and then (there are V borders
-// between tokens), so that its sums are in 64 bits, and so are the weights above e^-10 of the largest, of which there are
-// few in a row that a model is sure about.  A smaller weight's factors 2^(n/256) come from a table in 64 bits and what is left,
-// 1 + 1.4e-3 at most, from a short series in 32: off by 2e-10 of it, below 1e-14 of the largest.
+//    from the one row that it needs: from the pieces' sums and the piece that the token is in, or, where q is taken off p, from
+//    both rows, read again.
+// Sums and weights in 32 bits are enough nearly always: the numbers that are returned are whole, and a comparison says so itself when
+// its two sides are within what 32 bits may be off (kMargin, kDrawMargin).  Then, and then alone, the rows' sums are
+// taken again with weights in 64 bits: 2^(n / 65536) as a product of two from tables, and what is left, 1 + 5.3e-6 at most, from a
+// short series in 32 bits: off by 1e-12 of it.
 #include <cstdlib>
 
 #include "common.cuh"
@@ -27,9 +27,11 @@ constexpr int kScan = 256, kScanBlocks = 2;             // threads of a scanning
 constexpr int kSearch = 1024;                           // requests whose first rows a scanning block keeps
 constexpr int kDecide = 512, kWarps = kDecide / 32, kBatch = 32;      // rows whose sums are at hand at a time
 constexpr int kAhead = 4;                               // loads of a row that are under way
-// Relative error that the 32-bit sums may have: exponents are off by 2^-23 of up to 20 and the exponential by 2^-22, sums of
-// 64 and across lanes by less: 5e-6 for p and for q; eight times that for both.
+// Relative error that 32-bit sums may have: exponents are off by three roundings, 2^-24 each, of up to 20, and the exponential by
+// 2^-22, sums of a piece by 32 roundings at most: 5e-6 for p and for q; what is compared is both, with room.
 constexpr double kMargin = 8e-5;
+// The same of a running sum beside the whole, of p or of p and q: 1e-5 of 1 for each, with room.
+constexpr double kDrawMargin = 4e-5;
 constexpr float kLog2E = 1.4426950408889634f;
 
 struct VerifyArgs {
@@ -283,46 +285,44 @@ __global__ void __launch_bounds__(kScan, kScanBlocks) verify_scan_kernel(const V
 }
 
 // ------------------------------------------------------------------------------------- decisions
+__device__ __forceinline__ double shfl_xor(double v, int o) { return __shfl_xor_sync(0xffffffffu, v, o); }
+__device__ __forceinline__ double warp_total(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += shfl_xor(v, o);
+  return v;
+}
+
+// Weights in 64 bits: e^((x - best) / T) with log2(e) / T as two floats.
 constexpr int kTable = 256;
-// log2(e) / T in ways: for e^((x - best) / T) in 64 bits, times kTable as two floats, and as one.
-struct Heat {
-  double inv;                  // 1 / T
-  float hi, lo, c;
-  const double* table;         // 2^(i / kTable)
-  __device__ __forceinline__ Heat(float heat, const double* table_) : inv(1. / (double)heat), table(table_) {
-    c = inverse_heat(heat);
-    const double whole = fmin(inv, 1e30) * (kTable * 1.4426950408889634);
+struct Exact {
+  float hi, lo;
+  const double *coarse, *fine;                                       // 2^(i / 256), 2^(j / 65536)
+  __device__ __forceinline__ Exact(float heat, const double* tables) : coarse(tables), fine(tables + kTable) {
+    const double whole = fmin(1.4426950408889634 / (double)heat, 1e30);
     hi = (float)whole, lo = (float)(whole - (double)hi);
   }
+  // A logit's weight beside the row's largest one; below 2^-120 nothing.  (Without branches, so that several are under way.)
+  __device__ __forceinline__ double operator()(float x, float best) const {
+    const float d = x - best, e = d * hi;
+    // d + rest is x - best; k whole, i and j the next 16 bits, r what is left of it in natural units
+    const float back = d - x, rest = (x - (d - back)) + (-best - back);
+    const float off = fmaf(rest, hi, fmaf(d, lo, fmaf(d, hi, -e)));
+    const float k_at = e + 12582912.f, f = e - (k_at - 12582912.f);
+    const float n_at = fmaf(f, 65536.f, 12582912.f), left = fmaf(n_at - 12582912.f, -1.f / 65536.f, f);
+    const float r = (left + off) * 0.6931471805599453f, p = fmaf(0.5f * r, r, r);
+    const int n = ((__float_as_int(k_at) - 0x4b400000) << 16) + (__float_as_int(n_at) - 0x4b400000);
+    const double w = coarse[(n >> 8) & 255] * fine[n & 255];
+    const double y = fma(w, (double)p, w);
+    const double z = __hiloint2double(__double2hiint(y) + ((n >> 16) << 20), __double2loint(y));
+    // (e is no number beside an infinity or for -inf at a temperature of infinity)
+    return x == best ? (x > -INFINITY ? 1. : 0.) : e >= -120.f ? z : 0.;
+  }
 };
-__device__ __noinline__ double large_weight(float x, float best, double inv) {
-  if (x == best) return x == -INFINITY ? 0. : 1.;
-  if (x == -INFINITY || best == INFINITY) return 0.;
-  return exp(((double)x - (double)best) * inv);
-}
-// A logit's weight beside the row's largest one, as exactly as it counts (see above).
-__device__ __forceinline__ double weight64(float x, float best, const Heat& h) {
-  const float d = x - best, e = d * h.c;
-  if (!(e < -14.4f) || best == INFINITY) return large_weight(x, best, h.inv);   // (2^-14.4 is e^-10; or e is no number)
-  if (e < -120.f) return 0.;                                       // (nothing beside the largest, 2^-100 of all V)
-  // d + rest is x - best, n whole and t what is left of (x - best) / T in units of ln 2 / kTable
-  const float back = d - x, rest = (x - (d - back)) + (-best - back);
-  const float shifted = fmaf(d, h.hi, 12582912.f), n = shifted - 12582912.f;
-  const float t = fmaf(rest, h.hi, fmaf(d, h.lo, fmaf(d, h.hi, -n)));
-  const float r = t * (0.6931471805599453f / kTable);
-  const float p = fmaf(r * r, fmaf(r, 1.f / 6.f, 0.5f), r);        // e^r - 1; r^4 / 24 is below 2e-13
-  const int whole = __float_as_int(shifted) - 0x4b400000;          // n
-  const double f = h.table[whole & (kTable - 1)];
-  const double w = fma(f, (double)p, f);
-  return __hiloint2double(__double2hiint(w) + ((whole >> 8) << 20), __double2loint(w));
-}
-static_assert(kTable == 256, "the shift above");
-__device__ __forceinline__ double shfl_xor(double v, int o) { return __shfl_xor_sync(0xffffffffu, v, o); }
+static_assert(kTable == 256, "the shifts above");
 
 // What a row's weights are relative to, and their sum.
 struct Total {
-  float best;
-  double sum;
+  float best, sum;
 };
 struct Cluster {
   uint32_t rank, size;
@@ -334,13 +334,17 @@ struct Cluster {
     double* at = slots[round & 1];
     if (threadIdx.x == 0) at[0] = mine0, at[1] = mine1;
     cluster_sync();
+    // (a lane a block)
+    double x = 0., y = 0.;
+    const uint32_t lane = threadIdx.x & 31;
+    if (lane < size) {
+      const uint32_t from = dsmem_addr(smem_u32(at), lane);
+      asm volatile("ld.shared::cluster.v2.f64 {%0, %1}, [%2];" : "=d"(x), "=d"(y) : "r"(from) : "memory");
+    }
     all0 = all1 = before = 0.;
     for (uint32_t r = 0; r < size; ++r) {
-      const uint32_t from = dsmem_addr(smem_u32(at), r);
-      double x, y;
-      asm volatile("ld.shared::cluster.v2.f64 {%0, %1}, [%2];" : "=d"(x), "=d"(y) : "r"(from) : "memory");
       if (r == rank) before = all0;
-      all0 += x, all1 += y;
+      all0 += __shfl_sync(0xffffffffu, x, r), all1 += __shfl_sync(0xffffffffu, y, r);
     }
     ++round;                   // (two slots in turn: nobody writes one before all have read it)
   }
@@ -363,28 +367,236 @@ template <typename T> struct Ahead {
       x.load(g, v);
     }
   }
-  __device__ __forceinline__ double sum(const Row<T>& x, int g, int end, float best, const Heat& h) const {
-    double s = 0.;
+};
+
+// What a block needs for one request's row.
+template <typename T> struct Draw {
+  const VerifyArgs& a;
+  Cluster& cl;
+  double (*sums)[2];           // [kWarps][2]
+  Row<T> x, y;                 // the target's row and the draft's (the target's again where there is none)
+  bool with_draft, side_by_side;
+  float best, draft_best;
+  int d;                       // the token that is taken out; -1: none
+  int b0, b1, per, w0, w1;     // this block's groups, a warp's share of them, this warp's
+  __device__ __forceinline__ Draw(const VerifyArgs& a_, Cluster& cl_, double (*sums_)[2], int row, bool draft_, float best_,
+                                  float draft_best_, int d_)
+      : a(a_), cl(cl_), sums(sums_), x(a_.logits, a_.stride, row, a_.V),
+        y(draft_ ? a_.draft : a_.logits, draft_ ? a_.draft_stride : a_.stride, row, a_.V), with_draft(draft_),
+        best(best_), draft_best(draft_best_), d(d_) {
+    side_by_side = y.mis == x.mis;
+    const int groups = x.groups(), each = (groups + (int)cl.size - 1) / (int)cl.size, warp = threadIdx.x >> 5;
+    b0 = min(groups, (int)cl.rank * each), b1 = min(groups, b0 + each);
+    per = (b1 - b0 + kWarps - 1) / kWarps;
+    w0 = min(b1, b0 + warp * per), w1 = min(b1, w0 + per);
+  }
+  __device__ __forceinline__ void beside(int g, float (&z)[kVec<T>]) const {
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      if (g + 32 * i >= end) break;
-      float z[kVec<T>];
-      get(x, i, g + 32 * i, z);
+    for (int k = 0; k < kVec<T>; ++k) z[k] = y.at(g * kVec<T> - x.mis + k);
+  }
+  // Calls f(group, logits, the draft's logits) for the groups g, g + 32, ... up to `end`.  LONG: f is long (64 bits), so that its
+  // code stands here once, with the next group's loads under way; else kAhead groups' are.
+  template <bool LONG, typename F> __device__ __forceinline__ void each_group(int g, int end, F&& f) const {
+    if constexpr (LONG) {
+      uint4 rx{}, ry{};
+      const bool both = with_draft && side_by_side;
+      if (g < end && x.whole(g)) rx = x.raw(g);
+      if (both && g < end && y.whole(g)) ry = y.raw(g);
+#pragma unroll 1
+      for (; g < end; g += 32) {
+        float v[kVec<T>], z[kVec<T>] = {};
+        if (x.whole(g)) {
+          unpack<T>(rx, v);
+          if (both) unpack<T>(ry, z);
+        } else {
+          x.load(g, v);
+          if (both) y.load(g, z);
+        }
+        if (with_draft && !both) beside(g, z);
+        if (g + 32 < end && x.whole(g + 32)) {
+          rx = x.raw(g + 32);
+          if (both) ry = y.raw(g + 32);
+        }
 #pragma unroll
-      for (int k = 0; k < kVec<T>; ++k) s += weight64(z[k], best, h);
+        for (int k = 0; k < kVec<T>; ++k) v[k] = fmaxf(v[k], -INFINITY), z[k] = fmaxf(z[k], -INFINITY);
+        f(g, v, z);
+      }
+      return;
     }
-    return s;
+    Ahead<T> vx, vy;
+    for (; g < end; g += 32 * kAhead) {
+      vx.load(x, g, end);
+      if (with_draft && side_by_side) vy.load(y, g, end);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        if (g + 32 * i >= end) break;
+        float v[kVec<T>], z[kVec<T>] = {};
+        vx.get(x, i, g + 32 * i, v);
+        if (with_draft && side_by_side) vy.get(y, i, g + 32 * i, z);
+        else if (with_draft) beside(g + 32 * i, z);
+        f(g + 32 * i, v, z);
+      }
+    }
+  }
+  // The block's total of what the threads have, in the order of the warps; `sums` keeps theirs.
+  __device__ __forceinline__ double block_total(double mine, int which) const {
+    mine = warp_total(mine);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5][which] = mine;
+    __syncthreads();
+    double t = 0.;
+    for (int w = 0; w < kWarps; ++w) t += sums[w][which];
+    return t;
+  }
+  // Both rows' sums of weights in 64 bits.
+  __device__ __forceinline__ void totals(const Exact& e, double& P, double& Q) const {
+    double s0 = 0., s1 = 0., unused;
+    each_group<true>(w0 + (threadIdx.x & 31), w1, [&](int, const float (&v)[kVec<T>], const float (&z)[kVec<T>]) {
+#pragma unroll
+      for (int k = 0; k < kVec<T>; ++k) {
+        s0 += e(v[k], best);
+        if (with_draft) s1 += e(z[k], draft_best);
+      }
+    });
+    const double m0 = block_total(s0, 0), m1 = block_total(s1, 1);
+    cl.add(m0, m1, P, Q, unused);
+  }
+  // The first index at which the running sum of `weight(v, z, j)` reaches u times the whole, in the block that has it (-1 elsewhere, and
+  // everywhere where there is no weight); `low` and `high`: the sum in front of it and with it, as parts of the whole.  By the
+  // whole cluster.
+  template <bool LONG, typename W>
+  __device__ __forceinline__ int search(double u, const W& weight, double& total, double& target, double& low, double& high) const {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    double mine = 0., before, unused;
+    each_group<LONG>(w0 + lane, w1, [&](int g, const float (&v)[kVec<T>], const float (&z)[kVec<T>]) {
+      auto s = weight(v[0], z[0], g * kVec<T> - x.mis);
+#pragma unroll
+      for (int k = 1; k < kVec<T>; ++k) s += weight(v[k], z[k], g * kVec<T> - x.mis + k);
+      mine += (double)s;
+    });
+    const double block = block_total(mine, 0);
+    cl.add(block, 0., total, unused, before);
+    target = u * total;
+    // the block, in it the warp's share, and in that a smaller share, in which the sum is reached (the last one that weighs
+    // anything, should rounding leave it short)
+    if (!(total > 0.) || !(block > 0.) || !(before < target || before == 0.) || !(before + block >= target || before + block == total))
+      return -1;
+    auto pick = [&](int which, double& ahead) {
+      int owner = -1;
+      double at = ahead;
+      for (int w = 0; w < kWarps; ++w) {
+        const double s = sums[w][which];
+        if (s > 0. && (owner < 0 || at < target)) owner = w, ahead = at;
+        at += s;
+      }
+      return owner;
+    };
+    const int owner = pick(0, before);
+    const int seg0 = min(b1, b0 + owner * per), seg1 = min(b1, seg0 + per), sub = (seg1 - seg0 + kWarps - 1) / kWarps;
+    const int s0 = min(seg1, seg0 + warp * sub), s1 = min(seg1, s0 + sub);
+    double part = 0.;
+    each_group<true>(s0 + lane, s1, [&](int g, const float (&v)[kVec<T>], const float (&z)[kVec<T>]) {
+#pragma unroll
+      for (int k = 0; k < kVec<T>; ++k) part += (double)weight(v[k], z[k], g * kVec<T> - x.mis + k);
+    });
+    block_total(part, 1);
+    const int finder = pick(1, before);
+    if (warp != finder) return -1;
+    double run = before;
+    int last = -1;
+    for (int g = s0; g < s1; g += 32) {
+      float v[kVec<T>], z[kVec<T>] = {};
+      double w[kVec<T>], here = 0.;
+      if (g + lane < s1) {
+        x.load(g + lane, v);
+        if (with_draft && side_by_side) y.load(g + lane, z);
+        else if (with_draft) beside(g + lane, z);
+      }
+#pragma unroll
+      for (int k = 0; k < kVec<T>; ++k) {
+        w[k] = g + lane < s1 ? (double)weight(v[k], z[k], (g + lane) * kVec<T> - x.mis + k) : 0.;
+        here += w[k];
+      }
+      double upto = here;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double up = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += up;
+      }
+      double at = run + (upto - here), lo = 0., hi = 0.;
+      int hit = -1, latest = -1;
+      double latest_lo = 0., latest_hi = 0.;
+#pragma unroll
+      for (int k = 0; k < kVec<T>; ++k) {
+        const double from = at;
+        at += w[k];
+        if (w[k] > 0.) {
+          latest = (g + lane) * kVec<T> - x.mis + k, latest_lo = from, latest_hi = at;
+          if (hit < 0 && at >= target) hit = latest, lo = from, hi = at;
+        }
+      }
+      const unsigned hits = __ballot_sync(0xffffffffu, hit >= 0), some = __ballot_sync(0xffffffffu, latest >= 0);
+      if (hits) {
+        const int who = __ffs(hits) - 1;
+        low = __shfl_sync(0xffffffffu, lo, who), high = __shfl_sync(0xffffffffu, hi, who);
+        return __shfl_sync(0xffffffffu, hit, who);
+      }
+      if (some) {
+        const int who = 31 - __clz(some);
+        low = __shfl_sync(0xffffffffu, latest_lo, who), high = __shfl_sync(0xffffffffu, latest_hi, who);
+        last = __shfl_sync(0xffffffffu, latest, who);
+      }
+      run += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return last;
   }
 };
 
+// In 64 bits, by the whole cluster.  (Out of line: what nearly every request needs keeps its registers.)
+// Whether u q(d) < p(d).
 template <typename T>
-__global__ void __launch_bounds__(kDecide, 1) verify_decide_kernel(const VerifyArgs a) {
+__device__ __noinline__ bool exactly_stays(const VerifyArgs& a, Cluster& cl, double (*sums)[2], const double* tables, float heat,
+                                           int row, float best, float draft_best) {
+  const Draw<T> r(a, cl, sums, row, a.draft != nullptr, best, draft_best, -1);
+  const Exact e(heat, tables);
+  const int d = fresh_index(a.tokens + row + 1);
+  double P, Q;
+  r.totals(e, P, Q);
+  const double p = e(r.x.at(d), r.best) / P, q = a.draft ? (Q > 0. ? e(r.y.at(d), r.draft_best) / Q : 0.) : 1.;
+  return (double)fresh(a.u + row) * q < p;
+}
+// The token behind the drafts that stay, in the block that has it; -1 elsewhere.  `none`: the row has no weight at all.
+template <typename T>
+__device__ __noinline__ int exactly_drawn(const VerifyArgs& a, Cluster& cl, double (*sums)[2], const double* tables, float heat,
+                                          int row, bool with_draft, float best, float draft_best, int d, double u, bool& none) {
+  const Draw<T> r(a, cl, sums, row, with_draft, best, draft_best, d);
+  const Exact e(heat, tables);
+  double P = 1., Q = 1., total = 0., target, low, high;
+  if (with_draft) r.totals(e, P, Q);
+  const double inv_p = P > 0. ? 1. / P : 0., inv_q = Q > 0. ? 1. / Q : 0.;
+  none = false;
+  for (int whole = 0; whole < 2; ++whole) {           // (where nothing is left of p - q: p itself)
+    auto weight = [&](float v, float z, int j) {
+      double w = e(v, r.best) * inv_p;
+      if (with_draft && !whole) w = fmax(w - e(z, r.draft_best) * inv_q, 0.);
+      return j == r.d && !whole ? 0. : w;
+    };
+    const int token = r.template search<true>(u, weight, total, target, low, high);
+    if (total > 0.) return token;
+  }
+  none = true;
+  return -1;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kDecide, 2) verify_decide_kernel(const VerifyArgs a) {
   __shared__ Total totals[kBatch][2];                 // of the batch's rows: the target's, the draft's
+  __shared__ float drafted[kBatch][2];                // the logits that both give the draft
   __shared__ int places[kBatch];                      // greedy: the arg-max
   __shared__ double sums[kWarps][2];
   __shared__ __align__(16) double slots[2][2];
   __shared__ int verdict[2];
-  __shared__ double table[kTable];
+  __shared__ double tables[2 * kTable];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   Cluster cl{cluster_rank(), 0, 0, slots};
   asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(cl.size));
@@ -393,54 +605,24 @@ __global__ void __launch_bounds__(kDecide, 1) verify_decide_kernel(const VerifyA
   pdl_wait();
   const Span rows = rows_of(a, b);
   const int n = rows.end - rows.first;
+  const float heat = fresh(a.temperature + b);
   if (n == 0) {                                       // (the whole cluster)
     if (cl.rank == 0 && threadIdx.x == 0) a.accepted[b] = 0, a.next[b] = -1;
     return;
   }
-  const float heat = fresh(a.temperature + b);
   const bool greedy = !(heat > 0.f);
-  if (threadIdx.x < kTable) table[threadIdx.x] = exp2((double)threadIdx.x / kTable);
-  const Heat h(heat, table);
-  // this block's share of a row's groups of 16 bytes, and the warp's of that, in order
-  auto block_share = [&](int groups, int& g0, int& g1) {
-    const int each = (groups + (int)cl.size - 1) / (int)cl.size;
-    g0 = min(groups, (int)cl.rank * each), g1 = min(groups, g0 + each);
-  };
-  auto share_of = [&](int groups, int& w0, int& w1) {
-    int g0, g1;
-    block_share(groups, g0, g1);
-    const int per = (g1 - g0 + kWarps - 1) / kWarps;
-    w0 = min(g1, g0 + warp * per), w1 = min(g1, w0 + per);
-  };
-  // both rows' sums of weights in 64 bits
-  auto exact_totals = [&](int row, bool with_draft, float best, float draft_best, double& P, double& Q) {
-    double s[2] = {0., 0.};
-    const Row<T> x(a.logits, a.stride, row, a.V), y(with_draft ? a.draft : a.logits, with_draft ? a.draft_stride : a.stride, row, a.V);
-    int x0, x1, y0, y1;
-    share_of(x.groups(), x0, x1);
-    share_of(y.groups(), y0, y1);
-    if (!with_draft) y1 = y0;
-    Ahead<T> vx, vy;
-    for (int gx = x0 + lane, gy = y0 + lane; gx < x1 || gy < y1; gx += 32 * kAhead, gy += 32 * kAhead) {
-      vx.load(x, gx, x1);
-      vy.load(y, gy, y1);
-      s[0] += vx.sum(x, gx, x1, best, h);
-      s[1] += vy.sum(y, gy, y1, draft_best, h);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s[0] += shfl_xor(s[0], o), s[1] += shfl_xor(s[1], o);
+  const float c = inverse_heat(heat);
+  bool have_tables = false;
+  auto make_tables = [&] {
+    if (!have_tables)
+      for (int i = threadIdx.x; i < 2 * kTable; i += kDecide)
+        tables[i] = exp2(i < kTable ? (double)i / kTable : (double)(i - kTable) / (kTable * kTable));
     __syncthreads();
-    if (lane == 0) sums[warp][0] = s[0], sums[warp][1] = s[1];
-    __syncthreads();
-    double m0 = 0., m1 = 0., unused;
-    if (threadIdx.x == 0)
-      for (int w = 0; w < kWarps; ++w) m0 += sums[w][0], m1 += sums[w][1];
-    cl.add(m0, m1, P, Q, unused);
+    have_tables = true;
   };
 
   int stop = n - 1, in_batch = 0;
-  bool refused = false, exact = false;
-  double P = 0., Q = 0.;
+  bool refused = false;
   for (int i0 = 0; i0 < n; i0 += kBatch) {
     // the batch's totals, a warp a row
     const int here = min(kBatch, n - i0);
@@ -449,14 +631,31 @@ __global__ void __launch_bounds__(kDecide, 1) verify_decide_kernel(const VerifyA
       const int i = k >> 1, which = k & 1, row = rows.first + i0 + i;
       if (which && (!a.draft || greedy || i0 + i == n - 1)) continue;
       const float2* part = a.part + ((size_t)row * 2 + which) * a.pieces;
-      float best = -INFINITY;
+      // (-inf for a draft that is none)
+      float own = -INFINITY;
+      if (i0 + i < n - 1)
+        own = Row<T>(which ? a.draft : a.logits, which ? a.draft_stride : a.stride, row, a.V).at(fresh_index(a.tokens + row + 1));
+      float best = -INFINITY, sum = 0.f;
       int at = 0x7fffffff;
-      for (int q = lane; q < a.pieces; q += 32) {
-        const float2 y = __ldcg(part + q);
-        if (greedy && (y.x > best || (y.x == best && __float_as_int(y.y) < at))) at = __float_as_int(y.y);
-        best = fmaxf(best, y.x);
+      for (int q0 = lane; q0 < a.pieces; q0 += 32 * 8) {
+        float2 y[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) y[q] = q0 + 32 * q < a.pieces ? __ldcg(part + q0 + 32 * q) : make_float2(-INFINITY, 0.f);
+        float top = best;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          if (greedy && q0 + 32 * q < a.pieces && (y[q].x > top || (y[q].x == top && __float_as_int(y[q].y) < at)))
+            at = __float_as_int(y[q].y);
+          top = fmaxf(top, y[q].x);
+        }
+        if (!greedy && top > -INFINITY) {
+          sum = best > -INFINITY ? sum * weight32(best, top, c) : 0.f;
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            if (y[q].x > -INFINITY) sum += y[q].y * weight32(y[q].x, top, c);
+        }
+        best = top;
       }
-      double sum = 0.;
       if (greedy) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
@@ -465,21 +664,17 @@ __global__ void __launch_bounds__(kDecide, 1) verify_decide_kernel(const VerifyA
           if (ob > best || (ob == best && oa < at)) best = ob, at = oa;
         }
       } else {
-        best = warp_max(best);
-        for (int q = lane; q < a.pieces; q += 32) {
-          const float2 y = __ldcg(part + q);
-          sum += (double)y.y * weight64(y.x, best, h);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += shfl_xor(sum, o);
+        const float top = warp_max(best);
+        sum = warp_sum(best > -INFINITY ? sum * weight32(best, top, c) : 0.f);
+        best = top;
       }
       if (lane == 0) {
-        totals[i][which] = {best, sum};
+        totals[i][which] = {best, sum}, drafted[i][which] = own;
         if (!which) places[i] = best == -INFINITY ? 0 : min(max(at, 0), a.V - 1);
       }
     }
     __syncthreads();
-    // the first row of the batch at which it ends: 0 the draft stays, 1 it does not, 2 the sums have to be taken again, 3 the last row
+    // the first row of the batch at which it ends: 0 the draft stays, 1 it does not, 2 too near to say, 3 the last row
     int from = 0;
     bool done = false;
     while (true) {
@@ -490,22 +685,22 @@ __global__ void __launch_bounds__(kDecide, 1) verify_decide_kernel(const VerifyA
           if (i0 + i == n - 1) {
             what = 3;
           } else {
-            const int d = fresh_index(a.tokens + row + 1);
+            const float xd = drafted[i][0];
             if (greedy) {
-              what = d == places[i] ? 0 : 1;
-            } else if (d < 0 || d >= a.V || !(totals[i][0].sum > 0.)) {
+              what = fresh_index(a.tokens + row + 1) == places[i] ? 0 : 1;
+            } else if (!(xd > -INFINITY) || !(totals[i][0].sum > 0.f)) {
               what = 1;
             } else {
-              const float xd = Row<T>(a.logits, a.stride, row, a.V).at(d);
-              const double p = weight64(xd, totals[i][0].best, h) / totals[i][0].sum;
-              double q = 1.;
+              const float p = weight32(xd, totals[i][0].best, c) / totals[i][0].sum;
+              float q = 1.f;
               if (a.draft) {
-                const float yd = Row<T>(a.draft, a.draft_stride, row, a.V).at(d);
-                q = totals[i][1].sum > 0. ? weight64(yd, totals[i][1].best, h) / totals[i][1].sum : 0.;
+                const float yd = drafted[i][1];
+                q = totals[i][1].sum > 0.f && yd > -INFINITY ? weight32(yd, totals[i][1].best, c) / totals[i][1].sum : 0.f;
               }
-              const double left = (double)fresh(a.u + row) * q;
+              const float left = fresh(a.u + row) * q;
               what = left < p ? 0 : 1;
-              if (fabs(left - p) <= kMargin * fmax(left, p) && p > 0.) what = 2;
+              // (numbers that 32 bits do not hold well are not compared, either)
+              if (!(fabsf(left - p) > (float)kMargin * fmaxf(left, p) && fmaxf(left, p) > 1e-30f)) what = 2;
             }
           }
         }
@@ -519,17 +714,9 @@ __global__ void __launch_bounds__(kDecide, 1) verify_decide_kernel(const VerifyA
       __syncthreads();
       if (who < 0) break;                             // (all of the batch's drafts stay)
       in_batch = who, stop = i0 + who;
-      exact = false;
       if (what == 2) {
-        const int row = rows.first + stop;
-        exact_totals(row, a.draft != nullptr, totals[who][0].best, totals[who][1].best, P, Q);
-        exact = true;
-        const int d = fresh_index(a.tokens + row + 1);
-        const double p = weight64(Row<T>(a.logits, a.stride, row, a.V).at(d), totals[who][0].best, h) / P;
-        double q = 1.;
-        if (a.draft)
-          q = Q > 0. ? weight64(Row<T>(a.draft, a.draft_stride, row, a.V).at(d), totals[who][1].best, h) / Q : 0.;
-        if ((double)fresh(a.u + row) * q < p) {
+        make_tables();
+        if (exactly_stays<T>(a, cl, sums, tables, heat, rows.first + stop, totals[who][0].best, totals[who][1].best)) {
           from = who + 1;
           continue;
         }
@@ -547,145 +734,146 @@ __global__ void __launch_bounds__(kDecide, 1) verify_decide_kernel(const VerifyA
   }
   // ---- the token behind the last draft that stays
   const bool with_draft = refused && a.draft;
-  const float best = totals[in_batch][0].best, draft_best = with_draft ? totals[in_batch][1].best : 0.f;
-  if (with_draft && !exact) exact_totals(row, true, best, draft_best, P, Q);
-  const Row<T> x(a.logits, a.stride, row, a.V), y(with_draft ? a.draft : a.logits, with_draft ? a.draft_stride : a.stride, row, a.V);
-  const int d = refused ? fresh_index(a.tokens + row + 1) : -1;
-  // (where nothing is taken off p its sum need not be known)
-  const double inv_p = !with_draft ? 1. : P > 0. ? 1. / P : 0., inv_q = Q > 0. ? 1. / Q : 0.;
-  int w0, w1;
-  share_of(x.groups(), w0, w1);
-  // a group's weights: without `whole` what p has more than q
-  const bool side_by_side = y.mis == x.mis;
-  auto rest = [&](int g, const float (&v)[kVec<T>], const float (&z)[kVec<T>], bool whole, double (&w)[kVec<T>]) {
-    const int j = g * kVec<T> - x.mis;
-#pragma unroll
-    for (int k = 0; k < kVec<T>; ++k) {
-      w[k] = weight64(v[k], best, h) * inv_p;
-      if (with_draft && !whole) w[k] = fmax(w[k] - weight64(z[k], draft_best, h) * inv_q, 0.);
-      else if (refused && !whole && j + k == d) w[k] = 0.;
-    }
-  };
-  // what is taken off it: the draft's logits of the same tokens
-  auto beside = [&](int g, float (&z)[kVec<T>]) {
-#pragma unroll
-    for (int k = 0; k < kVec<T>; ++k) z[k] = y.at(g * kVec<T> - x.mis + k);
-  };
+  const Total tp = totals[in_batch][0], tq = with_draft ? totals[in_batch][1] : Total{0.f, 0.f};
+  const Draw<T> r(a, cl, sums, row, with_draft, tp.best, tq.best, refused && !with_draft ? fresh_index(a.tokens + row + 1) : -1);
   const double u = fmin(fmax((double)fresh(a.u + rows.end - 1), 0.), 1. - 0x1p-24);     // (whatever is handed in)
-  for (int whole = 0; whole < 2; ++whole) {           // (where nothing is left of p - q: p itself)
-    double mine = 0.;
-    Ahead<T> vx, vy;
-    for (int g = w0 + lane; g < w1; g += 32 * kAhead) {
-      vx.load(x, g, w1);
-      if (with_draft && side_by_side) vy.load(y, g, w1);
+  double total = 0., target, low = 0., high = 0.;
+  if (!with_draft) {
+    // from the pieces' sums, every block for itself (one warp): the piece in which the sum is reached, then the token in it
+    if (warp == 0) {
+      const float2* part = a.part + (size_t)row * 2 * a.pieces;
+      const float xd = r.d >= 0 ? drafted[in_batch][0] : -INFINITY;
+      const bool out = xd > -INFINITY;
+      const float wd = out ? weight32(xd, r.best, c) : 0.f;
+      const int d_piece = out ? (r.d + r.x.mis) / kPiece : -1;
+      total = (double)tp.sum - (double)wd;
+      target = u * total;
+      int piece = -1;
+      double ahead = 0.;
+      for (int q0 = 0; q0 < a.pieces && piece < 0; q0 += 32 * 8) {          // (eight neighbours a lane)
+        float2 y[8];
+        double s[8], mine = 0.;
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        if (g + 32 * i >= w1) break;
-        float v[kVec<T>], z[kVec<T>] = {};
-        double w[kVec<T>];
-        vx.get(x, i, g + 32 * i, v);
-        if (with_draft && side_by_side) vy.get(y, i, g + 32 * i, z);
-        else if (with_draft) beside(g + 32 * i, z);
-        rest(g + 32 * i, v, z, whole, w);
+        for (int q = 0; q < 8; ++q)
+          y[q] = q0 + 8 * lane + q < a.pieces ? __ldcg(part + q0 + 8 * lane + q) : make_float2(-INFINITY, 0.f);
 #pragma unroll
-        for (int k = 0; k < kVec<T>; ++k) mine += w[k];
-      }
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mine += shfl_xor(mine, o);
-    __syncthreads();
-    if (lane == 0) sums[warp][0] = mine;
-    __syncthreads();
-    double block = 0., total, unused, before;
-    for (int w = 0; w < kWarps; ++w) block += sums[w][0];
-    cl.add(block, 0., total, unused, before);
-    if (!(total > 0.)) continue;
-    const double target = u * total;
-    // the block, and in it the warp, in whose share the sum is reached (its last one, should rounding leave it short)
-    const bool own = block > 0. && (before < target || before == 0.) && (before + block >= target || before + block == total);
-    if (own) {
-      double ahead = before;
-      int owner = -1;
-      double owner_ahead = 0.;
-      for (int w = 0; w < kWarps; ++w) {
-        if (sums[w][0] > 0.) {
-          if (owner < 0 || ahead < target) owner = w, owner_ahead = ahead;
+        for (int q = 0; q < 8; ++q) {
+          s[q] = y[q].x > -INFINITY ? (double)y[q].y * (double)weight32(y[q].x, r.best, c) : 0.;
+          if (q0 + 8 * lane + q == d_piece) s[q] = fmax(s[q] - (double)wd, 0.);
+          mine += s[q];
         }
-        ahead += sums[w][0];
-      }
-      // its share again, in smaller ones for all of the block's warps
-      int b0, b1;
-      block_share(x.groups(), b0, b1);
-      const int per = (b1 - b0 + kWarps - 1) / kWarps, seg0 = min(b1, b0 + owner * per), seg1 = min(b1, seg0 + per),
-                sub = (seg1 - seg0 + kWarps - 1) / kWarps;
-      const int s0 = min(seg1, seg0 + warp * sub), s1 = min(seg1, s0 + sub);
-      auto weights_at = [&](int g, double (&w)[kVec<T>]) {
-        if (g < s1) {
-          float v[kVec<T>], z[kVec<T>] = {};
-          x.load(g, v);
-          if (with_draft && side_by_side) y.load(g, z);
-          else if (with_draft) beside(g, z);
-          rest(g, v, z, whole, w);
-        } else {
+        double upto = mine;
 #pragma unroll
-          for (int k = 0; k < kVec<T>; ++k) w[k] = 0.;
+        for (int o = 1; o < 32; o <<= 1) {
+          const double up = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += up;
         }
-      };
-      double part = 0.;
-      for (int g = s0; g < s1; g += 32) {
-        double w[kVec<T>];
-        weights_at(g + lane, w);
+        double at = ahead + (upto - mine), before = at;
+        int hit = -1;
 #pragma unroll
-        for (int k = 0; k < kVec<T>; ++k) part += w[k];
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) part += shfl_xor(part, o);
-      if (lane == 0) sums[warp][1] = part;
-      __syncthreads();
-      int finder = -1;
-      double run = 0.;
-      ahead = owner_ahead;
-      for (int w = 0; w < kWarps; ++w) {
-        if (sums[w][1] > 0. && (finder < 0 || ahead < target)) finder = w, run = ahead;
-        ahead += sums[w][1];
-      }
-      if (warp == finder) {
-        int last = -1;
-        bool found = false;
-        for (int g = s0; g < s1 && !found; g += 32) {
-          double w[kVec<T>], mine_here = 0.;
-          weights_at(g + lane, w);
-#pragma unroll
-          for (int k = 0; k < kVec<T>; ++k) mine_here += w[k];
-          double upto = mine_here;
-#pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const double up = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += up;
+        for (int q = 0; q < 8; ++q) {
+          if (hit < 0) {
+            if (s[q] > 0. && at + s[q] >= target) hit = q0 + 8 * lane + q, before = at;
+            at += s[q];
           }
-          double at = run + (upto - mine_here);
-          int pick = -1, latest = -1;
+        }
+        const unsigned hits = __ballot_sync(0xffffffffu, hit >= 0);
+        if (hits) {
+          piece = __shfl_sync(0xffffffffu, hit, __ffs(hits) - 1);
+          ahead = __shfl_sync(0xffffffffu, before, __ffs(hits) - 1);
+        } else {
+          ahead += __shfl_sync(0xffffffffu, upto, 31);
+        }
+      }
+      int token = -1;
+      if (piece >= 0) {
+        constexpr int G = kLoads<T>;
+        const int g0 = piece * (kPiece / kVec<T>) + lane * G;               // (neighbouring groups a lane: in order)
+        uint4 raw[G];
+#pragma unroll
+        for (int i = 0; i < G; ++i)
+          if (r.x.whole(g0 + i)) raw[i] = r.x.raw(g0 + i);
+        float w[G][kVec<T>];
+        double here = 0.;
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+          if (r.x.whole(g0 + i)) unpack<T>(raw[i], w[i]);
+          else r.x.load(g0 + i, w[i]);
 #pragma unroll
           for (int k = 0; k < kVec<T>; ++k) {
-            at += w[k];
-            if (w[k] > 0.) {
-              latest = (g + lane) * kVec<T> - x.mis + k;
-              if (pick < 0 && at >= target) pick = latest;
-            }
+            const int j = (g0 + i) * kVec<T> - r.x.mis + k;
+            const float v = fmaxf(w[i][k], -INFINITY);
+            w[i][k] = v > -INFINITY && j != r.d ? fast_exp2((v - r.best) * c) : 0.f;       // (c: see `sure`)
+            here += (double)w[i][k];
           }
-          const unsigned hits = __ballot_sync(0xffffffffu, pick >= 0), some = __ballot_sync(0xffffffffu, latest >= 0);
-          if (hits) last = __shfl_sync(0xffffffffu, pick, __ffs(hits) - 1), found = true;
-          else if (some) last = __shfl_sync(0xffffffffu, latest, 31 - __clz(some));
-          run += __shfl_sync(0xffffffffu, upto, 31);
         }
-        if (lane == 0) a.accepted[b] = stop, a.next[b] = last;
+        double upto = here;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double up = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += up;
+        }
+        double at = ahead + (upto - here), lo = 0., hi = 0.;
+        int hit = -1;
+#pragma unroll
+        for (int i = 0; i < G; ++i)
+#pragma unroll
+          for (int k = 0; k < kVec<T>; ++k) {
+            const double from = at;
+            at += (double)w[i][k];
+            if (hit < 0 && w[i][k] > 0.f && at >= target) hit = (g0 + i) * kVec<T> - r.x.mis + k, lo = from, hi = at;
+          }
+        const unsigned hits = __ballot_sync(0xffffffffu, hit >= 0);
+        if (hits) {
+          const int who = __ffs(hits) - 1;
+          token = __shfl_sync(0xffffffffu, hit, who);
+          low = __shfl_sync(0xffffffffu, lo, who), high = __shfl_sync(0xffffffffu, hi, who);
+        }
       }
+      // (off by a part of all of p, which `total` is where no draft is taken out)
+      const double room = kDrawMargin * (double)tp.sum;
+      const bool sure = token >= 0 && tp.best < INFINITY && c > 0.f && (target - low > room || (low == 0. && target > 0.)) && high - target > room;
+      if (lane == 0) verdict[0] = sure ? token : -1;
     }
-    cluster_sync();            // (nobody leaves while another reads its sums)
-    return;
+    __syncthreads();
+    if (verdict[0] >= 0) {
+      if (cl.rank == 0 && threadIdx.x == 0) a.accepted[b] = stop, a.next[b] = verdict[0];
+      if (cl.round) cluster_sync();
+      return;
+    }
+  } else {
+    // from both rows, in 32 bits
+    const float inv_p = tp.sum > 0.f ? 1.f / tp.sum : 0.f, inv_q = tq.sum > 0.f ? 1.f / tq.sum : 0.f;
+    auto weight = [&](float v, float z, int) {
+      const float p = fast_exp2((v - r.best) * c) * inv_p, q = fast_exp2((z - r.draft_best) * c) * inv_q;
+      return fmaxf(p - q, 0.f);
+    };
+    const bool plain = tp.sum > 0.f && tq.sum > 0.f && tp.best < INFINITY && tq.best < INFINITY && c > 0.f;
+    int token = -1;
+    if (plain) token = r.template search<false>(u, weight, total, target, low, high);
+    const bool sure = token >= 0 && target - low > kDrawMargin && high - target > kDrawMargin;
+    // whether some block is sure, known to all
+    if (threadIdx.x == 0) verdict[0] = 0;
+    __syncthreads();
+    if (sure && lane == 0) {
+      verdict[0] = 1;
+      a.accepted[b] = stop, a.next[b] = token;
+    }
+    __syncthreads();
+    double found, unused0, unused1;
+    cl.add((double)verdict[0], 0., found, unused0, unused1);
+    if (found > 0.) {
+      cluster_sync();          // (nobody leaves while another reads its sums)
+      return;
+    }
   }
-  if (cl.rank == 0 && threadIdx.x == 0) a.accepted[b] = stop, a.next[b] = 0;      // (a row without a number)
-  cluster_sync();
+  // ---- in 64 bits
+  make_tables();
+  bool none;
+  const int token = exactly_drawn<T>(a, cl, sums, tables, heat, row, with_draft, tp.best, tq.best, r.d, u, none);
+  if (token >= 0 && lane == 0) a.accepted[b] = stop, a.next[b] = token;
+  if (none && cl.rank == 0 && threadIdx.x == 0) a.accepted[b] = stop, a.next[b] = 0;      // (a row without a number)
+  cluster_sync();              // (nobody leaves while another reads its sums)
 }
 
 }  // namespace

@@ -22,10 +22,11 @@
 namespace gf {
 namespace {
 
-constexpr int kPiece = 1024;                            // logits of a piece
+constexpr int kLoads = 8;                               // 16-byte loads a lane of a piece
+constexpr int kPiece = 1024;                            // the least logits of a piece
 constexpr int kScan = 256, kScanBlocks = 2;             // threads of a scanning block, blocks an SM
 constexpr int kSearch = 1024;                           // requests whose first rows a scanning block keeps
-constexpr int kDecide = 512, kWarps = kDecide / 32, kBatch = 32;      // rows whose sums are at hand at a time
+constexpr int kDecide = 256, kWarps = kDecide / 32, kBatch = 32;      // rows whose sums are at hand at a time
 constexpr int kAhead = 4;                               // loads of a row that are under way
 // Relative error that 32-bit sums may have: exponents are off by three roundings, 2^-24 each, of up to 20, and the exponential by
 // 2^-22, sums of a piece by 32 roundings at most: 5e-6 for p and for q; what is compared is both, with room.
@@ -49,7 +50,8 @@ struct VerifyArgs {
 };
 
 template <typename T> constexpr int kVec = 16 / (int)sizeof(T);
-template <typename T> constexpr int kLoads = kPiece / (32 * kVec<T>);              // a lane's of a piece
+template <typename T> constexpr int kPieceOf = 32 * kLoads * kVec<T>;              // logits of a piece
+static_assert(kPieceOf<float> == kPiece, "the least");
 template <typename T> __device__ __forceinline__ void unpack(const uint4& raw, float (&v)[kVec<T>]) {
   const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
   if constexpr (sizeof(T) == 4) {
@@ -78,6 +80,20 @@ template <typename T> struct Row {
     return j >= 0 && j + kVec<T> <= V;
   }
   __device__ __forceinline__ uint4 raw(int g) const { return __ldcg(reinterpret_cast<const uint4*>(x + (g * kVec<T> - mis))); }
+  // A group that the row begins or ends in, or one outside it: -inf in places outside.
+  __device__ __forceinline__ uint4 pieced(int g) const {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        w[i] = __float_as_uint(at(g * kVec<T> - mis + i));
+      } else {
+        const int j = g * kVec<T> - mis + 2 * i;
+        w[i] = (__float_as_uint(at(j)) >> 16) | (__float_as_uint(at(j + 1)) & 0xffff0000u);
+      }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
   // Group g's logits, -inf outside the row and for a NaN.
   __device__ __forceinline__ void load(int g, float (&v)[kVec<T>]) const {
     if (whole(g)) {
@@ -131,11 +147,35 @@ __device__ __forceinline__ float weight32(float x, float best, float c) {
 }
 
 // ------------------------------------------------------------------------------------- rows in pieces
+// A piece with care, by a warp: one with a weight that is no number.  (Out of line: the others keep their registers.)
+template <typename T>
+__device__ __noinline__ float careful_sum(const Row<T>& r, int g0, float top, float c) {
+  float sum = 0.f;
+#pragma unroll 2
+  for (int i = 0; i < kLoads; ++i) {
+    float v[kVec<T>];
+    r.load(g0 + i * 32, v);
+#pragma unroll
+    for (int k = 0; k < kVec<T>; ++k) sum += weight32(v[k], top, c);
+  }
+  return warp_sum(sum);
+}
+// The largest of a group's logits (a NaN never is).
+template <typename T> __device__ __forceinline__ float group_max(const uint4& raw) {
+  if constexpr (sizeof(T) == 4) {
+    return fmaxf(fmaxf(__uint_as_float(raw.x), __uint_as_float(raw.y)), fmaxf(__uint_as_float(raw.z), __uint_as_float(raw.w)));
+  } else {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw);
+    const float2 m = __bfloat1622float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+    return fmaxf(m.x, m.y);
+  }
+}
+
 // A warp takes a piece after the other, the loads of the next one under way while it works on one.
 template <typename T>
 __global__ void __launch_bounds__(kScan, kScanBlocks) verify_scan_kernel(const VerifyArgs a) {
   __shared__ int starts[kSearch + 1];
-  constexpr int GROUPS = 32 * kLoads<T>;
+  constexpr int GROUPS = 32 * kLoads;
   const int lane = threadIdx.x & 31;
   pdl_trigger();
   pdl_wait();
@@ -157,7 +197,8 @@ __global__ void __launch_bounds__(kScan, kScanBlocks) verify_scan_kernel(const V
     if (there) {
       const long long at = my_which ? u - half : u;
       my_row = at >> 32 ? (int)(at / a.pieces) : (int)((unsigned)at / (unsigned)a.pieces);
-      my_piece = (int)(at - (long long)my_row * a.pieces);
+      // (turned by the row: a row's last piece, which costs more, is not always the same warps')
+      my_piece = (int)((at - (long long)my_row * a.pieces + my_row) % a.pieces);
       int low = 0, high = a.B;                          // the last request that does not start behind the row
       while (high - low > 1) {
         const int mid = (low + high) >> 1;
@@ -172,102 +213,75 @@ __global__ void __launch_bounds__(kScan, kScanBlocks) verify_scan_kernel(const V
     struct Unit {
       int row, which, piece;
       float heat;
-      bool whole;
     };
-    auto fetch = [&](uint4 (&raw)[kLoads<T>]) {            // the next of the ballot's
+    auto fetch = [&](uint4 (&raw)[kLoads]) {            // the next of the ballot's
       const int who = __ffs(left) - 1;
       left &= left - 1;
       Unit x{__shfl_sync(0xffffffffu, my_row, who), __shfl_sync(0xffffffffu, my_which, who),
-             __shfl_sync(0xffffffffu, my_piece, who), __shfl_sync(0xffffffffu, my_heat, who), false};
+             __shfl_sync(0xffffffffu, my_piece, who), __shfl_sync(0xffffffffu, my_heat, who)};
       const Row<T> r(x.which ? a.draft : a.logits, x.which ? a.draft_stride : a.stride, x.row, a.V);
-      x.whole = r.whole(x.piece * GROUPS) && r.whole(x.piece * GROUPS + GROUPS - 1);
-      if (x.whole) {
+      const int g0 = x.piece * GROUPS + lane;
+      if (r.whole(x.piece * GROUPS) && r.whole(x.piece * GROUPS + GROUPS - 1)) {
 #pragma unroll
-        for (int i = 0; i < kLoads<T>; ++i) raw[i] = r.raw(x.piece * GROUPS + i * 32 + lane);
+        for (int i = 0; i < kLoads; ++i) raw[i] = r.raw(g0 + i * 32);
+      } else {
+        const uint32_t none = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) raw[i] = r.whole(g0 + i * 32) ? r.raw(g0 + i * 32) : make_uint4(none, none, none, none);
+        // (the row's first and last group)
+        const int first = r.mis ? 0 : -1, last = (a.V + r.mis) % kVec<T> ? r.groups() - 1 : -1;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i)
+          if (g0 + i * 32 == first || g0 + i * 32 == last) raw[i] = r.pieced(g0 + i * 32);
       }
       return x;
     };
-    auto work = [&](const Unit& x, const uint4 (&raw)[kLoads<T>]) {
+    auto work = [&](const Unit& x, const uint4 (&raw)[kLoads]) {
       const Row<T> r(x.which ? a.draft : a.logits, x.which ? a.draft_stride : a.stride, x.row, a.V);
       const bool greedy = !(x.heat > 0.f);
       const float c = inverse_heat(x.heat);
       const int g0 = x.piece * GROUPS + lane;
       float top = -INFINITY, second = 0.f;
-      if (x.whole) {
-        float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < kLoads<T>; ++i) {
+      for (int i = 0; i < kLoads; ++i) top = fmaxf(top, group_max<T>(raw[i]));
+      top = warp_max(top);
+      if (greedy) {
+        int at = 0x7fffffff;
+#pragma unroll
+        for (int i = kLoads - 1; i >= 0; --i) {
           float v[kVec<T>];
           unpack<T>(raw[i], v);
 #pragma unroll
-          for (int k = 0; k < kVec<T>; ++k) t[k & 3] = fmaxf(t[k & 3], v[k]);       // (a NaN never is)
-        }
-        top = warp_max(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
-        if (greedy) {
-          int at = 0x7fffffff;
-#pragma unroll
-          for (int i = kLoads<T> - 1; i >= 0; --i) {
-            float v[kVec<T>];
-            unpack<T>(raw[i], v);
-#pragma unroll
-            for (int k = kVec<T> - 1; k >= 0; --k)
-              if (v[k] == top) at = (g0 + i * 32) * kVec<T> - r.mis + k;            // (the first of the lane's)
-          }
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) at = min(at, __shfl_xor_sync(0xffffffffu, at, o));
-          second = __int_as_float(at);
-        } else {
-          // weights as they come; where one is no number (a NaN, infinities, a temperature of infinity) again with care
-          const uint64_t c2 = pack2(c, c), m2 = pack2(-top, -top);
-          uint64_t s2[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
-#pragma unroll
-          for (int i = 0; i < kLoads<T>; ++i) {
-            float v[kVec<T>];
-            unpack<T>(raw[i], v);
-#pragma unroll
-            for (int k = 0; k < kVec<T>; k += 2) {
-              float e0, e1;
-              unpack2(mul2(add2(pack2(v[k], v[k + 1]), m2), c2), e0, e1);
-              s2[(k >> 1) & 1] = add2(s2[(k >> 1) & 1], pack2(fast_exp2(e0), fast_exp2(e1)));
-            }
-          }
-          float s0, s1, s3, s4;
-          unpack2(s2[0], s0, s1);
-          unpack2(s2[1], s3, s4);
-          second = warp_sum((s0 + s1) + (s3 + s4));
-        }
-      }
-      if (!x.whole || (!greedy && !(second < INFINITY))) {
-        if (!x.whole) {
-#pragma unroll 1
-          for (int i = 0; i < kLoads<T>; ++i) {
-            float v[kVec<T>];
-            r.load(g0 + i * 32, v);
-#pragma unroll
-            for (int k = 0; k < kVec<T>; ++k) top = fmaxf(top, v[k]);
-          }
-          top = warp_max(top);
-        }
-        int at = 0x7fffffff;
-        second = 0.f;
-#pragma unroll 1
-        for (int i = 0; i < kLoads<T> && top > -INFINITY; ++i) {
-          float v[kVec<T>];
-          r.load(g0 + i * 32, v);
-#pragma unroll
-          for (int k = 0; k < kVec<T>; ++k) {
-            if (v[k] == top) at = min(at, (g0 + i * 32) * kVec<T> - r.mis + k);
-            second += weight32(v[k], top, c);
-          }
+          for (int k = kVec<T> - 1; k >= 0; --k)
+            if (v[k] == top) at = (g0 + i * 32) * kVec<T> - r.mis + k;            // (the first of the lane's)
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) at = min(at, __shfl_xor_sync(0xffffffffu, at, o));
-        second = warp_sum(second);
-        if (greedy) second = __int_as_float(at);
+        second = __int_as_float(at);
+      } else {
+        // weights as they come; where one is no number (a NaN, infinities, a temperature of infinity) again with care
+        const uint64_t c2 = pack2(c, c), m2 = pack2(-top, -top);
+        uint64_t s2[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+          float v[kVec<T>];
+          unpack<T>(raw[i], v);
+#pragma unroll
+          for (int k = 0; k < kVec<T>; k += 2) {
+            float e0, e1;
+            unpack2(mul2(add2(pack2(v[k], v[k + 1]), m2), c2), e0, e1);
+            s2[(k >> 1) & 1] = add2(s2[(k >> 1) & 1], pack2(fast_exp2(e0), fast_exp2(e1)));
+          }
+        }
+        float s0, s1, s3, s4;
+        unpack2(s2[0], s0, s1);
+        unpack2(s2[1], s3, s4);
+        second = warp_sum((s0 + s1) + (s3 + s4));
       }
+      if (!greedy && !(second < INFINITY)) second = top > -INFINITY ? careful_sum<T>(r, g0, top, c) : 0.f;
       if (lane == 0) a.part[((size_t)x.row * 2 + x.which) * a.pieces + x.piece] = make_float2(top, second);
     };
-    uint4 raw0[kLoads<T>], raw1[kLoads<T>];
+    uint4 raw0[kLoads], raw1[kLoads];
     Unit x0, x1;
     if (left) x0 = fetch(raw0);
     else continue;
@@ -421,20 +435,20 @@ template <typename T> struct Draw {
         for (int k = 0; k < kVec<T>; ++k) v[k] = fmaxf(v[k], -INFINITY), z[k] = fmaxf(z[k], -INFINITY);
         f(g, v, z);
       }
-      return;
-    }
-    Ahead<T> vx, vy;
-    for (; g < end; g += 32 * kAhead) {
-      vx.load(x, g, end);
-      if (with_draft && side_by_side) vy.load(y, g, end);
+    } else {
+      Ahead<T> vx, vy;
+      for (; g < end; g += 32 * kAhead) {
+        vx.load(x, g, end);
+        if (with_draft && side_by_side) vy.load(y, g, end);
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        if (g + 32 * i >= end) break;
-        float v[kVec<T>], z[kVec<T>] = {};
-        vx.get(x, i, g + 32 * i, v);
-        if (with_draft && side_by_side) vy.get(y, i, g + 32 * i, z);
-        else if (with_draft) beside(g + 32 * i, z);
-        f(g + 32 * i, v, z);
+        for (int i = 0; i < kAhead; ++i) {
+          if (g + 32 * i >= end) break;
+          float v[kVec<T>], z[kVec<T>] = {};
+          vx.get(x, i, g + 32 * i, v);
+          if (with_draft && side_by_side) vy.get(y, i, g + 32 * i, z);
+          else if (with_draft) beside(g + 32 * i, z);
+          f(g + 32 * i, v, z);
+        }
       }
     }
   }
@@ -745,7 +759,7 @@ __global__ void __launch_bounds__(kDecide, 2) verify_decide_kernel(const VerifyA
       const float xd = r.d >= 0 ? drafted[in_batch][0] : -INFINITY;
       const bool out = xd > -INFINITY;
       const float wd = out ? weight32(xd, r.best, c) : 0.f;
-      const int d_piece = out ? (r.d + r.x.mis) / kPiece : -1;
+      const int d_piece = out ? (r.d + r.x.mis) / kPieceOf<T> : -1;
       total = (double)tp.sum - (double)wd;
       target = u * total;
       int piece = -1;
@@ -787,25 +801,30 @@ __global__ void __launch_bounds__(kDecide, 2) verify_decide_kernel(const VerifyA
       }
       int token = -1;
       if (piece >= 0) {
-        constexpr int G = kLoads<T>;
-        const int g0 = piece * (kPiece / kVec<T>) + lane * G;               // (neighbouring groups a lane: in order)
+        constexpr int G = kLoads;
+        const int g0 = piece * (kPieceOf<T> / kVec<T>) + lane * G;               // (neighbouring groups a lane: in order)
         uint4 raw[G];
 #pragma unroll
         for (int i = 0; i < G; ++i)
           if (r.x.whole(g0 + i)) raw[i] = r.x.raw(g0 + i);
-        float w[G][kVec<T>];
-        double here = 0.;
-#pragma unroll
-        for (int i = 0; i < G; ++i) {
-          if (r.x.whole(g0 + i)) unpack<T>(raw[i], w[i]);
-          else r.x.load(g0 + i, w[i]);
+        // (weights are computed twice rather than kept)
+        auto weights = [&](int i, float (&w)[kVec<T>]) {
+          if (r.x.whole(g0 + i)) unpack<T>(raw[i], w);
+          else r.x.load(g0 + i, w);
 #pragma unroll
           for (int k = 0; k < kVec<T>; ++k) {
-            const int j = (g0 + i) * kVec<T> - r.x.mis + k;
-            const float v = fmaxf(w[i][k], -INFINITY);
-            w[i][k] = v > -INFINITY && j != r.d ? fast_exp2((v - r.best) * c) : 0.f;       // (c: see `sure`)
-            here += (double)w[i][k];
+            const float v = fmaxf(w[k], -INFINITY);
+            w[k] = v > -INFINITY && (g0 + i) * kVec<T> - r.x.mis + k != r.d ? fast_exp2((v - r.best) * c) : 0.f;   // (c: see `sure`)
           }
+        };
+        double sums_of[G], here = 0.;
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+          float w[kVec<T>], s = 0.f;
+          weights(i, w);
+#pragma unroll
+          for (int k = 0; k < kVec<T>; ++k) s += w[k];
+          sums_of[i] = s, here += sums_of[i];
         }
         double upto = here;
 #pragma unroll
@@ -816,13 +835,22 @@ __global__ void __launch_bounds__(kDecide, 2) verify_decide_kernel(const VerifyA
         double at = ahead + (upto - here), lo = 0., hi = 0.;
         int hit = -1;
 #pragma unroll
-        for (int i = 0; i < G; ++i)
+        for (int i = 0; i < G; ++i) {
+          if (hit < 0 && sums_of[i] > 0. && at + sums_of[i] >= target) {
+            float w[kVec<T>];
+            weights(i, w);
+            double run = at;
 #pragma unroll
-          for (int k = 0; k < kVec<T>; ++k) {
-            const double from = at;
-            at += (double)w[i][k];
-            if (hit < 0 && w[i][k] > 0.f && at >= target) hit = (g0 + i) * kVec<T> - r.x.mis + k, lo = from, hi = at;
+            for (int k = 0; k < kVec<T>; ++k) {
+              if (w[k] > 0.f && hit < 0) {
+                lo = run, hi = run + (double)w[k];
+                if (hi >= target) hit = (g0 + i) * kVec<T> - r.x.mis + k;
+              }
+              run += (double)w[k];
+            }
           }
+          at += sums_of[i];
+        }
         const unsigned hits = __ballot_sync(0xffffffffu, hit >= 0);
         if (hits) {
           const int who = __ffs(hits) - 1;
@@ -902,7 +930,8 @@ GF_EXPORT int gf_verify(const char* words) {
   cudaStream_t stream = (cudaStream_t)ptr();
   if (a.B <= 0) return 0;
   const bool half = type == GF_BF16;
-  a.pieces = (a.V + (half ? kVec<bf16> : kVec<float>) - 1 + kPiece - 1) / kPiece;
+  const int piece = half ? kPieceOf<bf16> : kPieceOf<float>;
+  a.pieces = (a.V + (half ? kVec<bf16> : kVec<float>) - 1 + piece - 1) / piece;
   if ((long long)a.R * 2 * a.pieces * 8 > room) return -5;
   int rc = 0;
   if (a.R > 0) {
@@ -920,7 +949,7 @@ GF_EXPORT int gf_verify(const char* words) {
   });
   if (rc) return rc;
   const char* env = getenv("GF_CLUSTER");
-  const int cluster = env ? atoi(env) : a.B <= 4 ? 16 : a.B <= 18 ? 8 : 4;
+  const int cluster = env ? atoi(env) : 8;
   return launch_kernel_cluster_dims(half ? verify_decide_kernel<bf16> : verify_decide_kernel<float>, dim3(a.B * cluster),
                                     dim3(kDecide), 0, stream, cluster, true, a);
 }

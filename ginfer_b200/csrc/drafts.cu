@@ -12,10 +12,7 @@
 //    both rows, read again.
 // Sums and weights in 32 bits are enough nearly always: the numbers that are returned are whole, and a comparison says so itself when
 // its two sides are within what 32 bits may be off (kMargin, kDrawMargin).  Then, and then alone, the rows' sums are
-// taken again with weights in 64 bits: 2^(n / 65536) as a product of two from tables, and what is left, 1 + 5.3e-6 at most, from a
-// short series in 32 bits: off by 1e-12 of it.
-#include <cstdlib>
-
+// taken again with weights in 64 bits.
 #include "common.cuh"
 #include "tc_common.cuh"
 
@@ -27,6 +24,9 @@ constexpr int kPiece = 1024;                            // the least logits of a
 constexpr int kScan = 256, kScanBlocks = 2;             // threads of a scanning block, blocks an SM
 constexpr int kSearch = 1024;                           // requests whose first rows a scanning block keeps
 constexpr int kDecide = 256, kWarps = kDecide / 32, kBatch = 32;      // rows whose sums are at hand at a time
+// Blocks of a request: 8 up to this many requests, else 4.  8 / 4, us, 64 requests of 4 drafts and 152,064 logits with a draft
+// model 139.5 / 180.2, 256 of 7 in bfloat16 392.5 / 381.6, 33 of 6 and 32,003 logits 43.8 / 51.5 (2 and 16 are slower everywhere).
+constexpr int kManyRequests = 128;
 constexpr int kAhead = 4;                               // loads of a row that are under way
 // Relative error that 32-bit sums may have: exponents are off by three roundings, 2^-24 each, of up to 20, and the exponential by
 // 2^-22, sums of a piece by 32 roundings at most: 5e-6 for p and for q; what is compared is both, with room.
@@ -80,6 +80,8 @@ template <typename T> struct Row {
     return j >= 0 && j + kVec<T> <= V;
   }
   __device__ __forceinline__ uint4 raw(int g) const { return __ldcg(reinterpret_cast<const uint4*>(x + (g * kVec<T> - mis))); }
+  // The same for what is read in passing: it leaves L2 first.
+  __device__ __forceinline__ uint4 passing(int g) const { return __ldcs(reinterpret_cast<const uint4*>(x + (g * kVec<T> - mis))); }
   // A group that the row begins or ends in, or one outside it: -inf in places outside.
   __device__ __forceinline__ uint4 pieced(int g) const {
     uint32_t w[4];
@@ -223,11 +225,11 @@ __global__ void __launch_bounds__(kScan, kScanBlocks) verify_scan_kernel(const V
       const int g0 = x.piece * GROUPS + lane;
       if (r.whole(x.piece * GROUPS) && r.whole(x.piece * GROUPS + GROUPS - 1)) {
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) raw[i] = r.raw(g0 + i * 32);
+        for (int i = 0; i < kLoads; ++i) raw[i] = r.passing(g0 + i * 32);
       } else {
         const uint32_t none = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) raw[i] = r.whole(g0 + i * 32) ? r.raw(g0 + i * 32) : make_uint4(none, none, none, none);
+        for (int i = 0; i < kLoads; ++i) raw[i] = r.whole(g0 + i * 32) ? r.passing(g0 + i * 32) : make_uint4(none, none, none, none);
         // (the row's first and last group)
         const int first = r.mis ? 0 : -1, last = (a.V + r.mis) % kVec<T> ? r.groups() - 1 : -1;
 #pragma unroll
@@ -306,33 +308,32 @@ __device__ __forceinline__ double warp_total(double v) {
   return v;
 }
 
-// Weights in 64 bits: e^((x - best) / T) with log2(e) / T as two floats.
-constexpr int kTable = 256;
+// Weights in 64 bits: 2^y for y = (x - best) log2(e) / T as 2^(n / kTable), n the nearest whole number to kTable y, from a
+// table, times the power series of 2^f, |f| <= 1 / (2 kTable), to the fifth power (what is cut off is below 4e-17).
+constexpr int kTable = 64;
 struct Exact {
-  float hi, lo;
-  const double *coarse, *fine;                                       // 2^(i / 256), 2^(j / 65536)
-  __device__ __forceinline__ Exact(float heat, const double* tables) : coarse(tables), fine(tables + kTable) {
-    const double whole = fmin(1.4426950408889634 / (double)heat, 1e30);
-    hi = (float)whole, lo = (float)(whole - (double)hi);
-  }
+  double c;                    // log2(e) / T
+  float c32;
+  const double* table;         // 2^(i / kTable)
+  __device__ __forceinline__ Exact(float heat, const double* table_)
+      : c(fmin(1.4426950408889634 / (double)heat, 1e30)), c32((float)c), table(table_) {}
   // A logit's weight beside the row's largest one; below 2^-120 nothing.  (Without branches, so that several are under way.)
   __device__ __forceinline__ double operator()(float x, float best) const {
-    const float d = x - best, e = d * hi;
-    // d + rest is x - best; k whole, i and j the next 16 bits, r what is left of it in natural units
-    const float back = d - x, rest = (x - (d - back)) + (-best - back);
-    const float off = fmaf(rest, hi, fmaf(d, lo, fmaf(d, hi, -e)));
-    const float k_at = e + 12582912.f, f = e - (k_at - 12582912.f);
-    const float n_at = fmaf(f, 65536.f, 12582912.f), left = fmaf(n_at - 12582912.f, -1.f / 65536.f, f);
-    const float r = (left + off) * 0.6931471805599453f, p = fmaf(0.5f * r, r, r);
-    const int n = ((__float_as_int(k_at) - 0x4b400000) << 16) + (__float_as_int(n_at) - 0x4b400000);
-    const double w = coarse[(n >> 8) & 255] * fine[n & 255];
-    const double y = fma(w, (double)p, w);
-    const double z = __hiloint2double(__double2hiint(y) + ((n >> 16) << 20), __double2loint(y));
-    // (e is no number beside an infinity or for -inf at a temperature of infinity)
-    return x == best ? (x > -INFINITY ? 1. : 0.) : e >= -120.f ? z : 0.;
+    constexpr double kShift = 6755399441055744.0 / kTable;           // 1.5 * 2^52 / kTable: n in the last bits
+    const double d = (double)x - (double)best, at = fma(d, c, kShift), f = fma(d, c, -(at - kShift));
+    double p = fma(f, 0.0013333558146428443, 0.009618129107628477);  // ln(2)^k / k!
+    p = fma(p, f, 0.055504108664821576);
+    p = fma(p, f, 0.2402265069591007);
+    p = fma(p, f, 0.6931471805599453);
+    p = fma(p, f, 1.0);
+    const int n = __double2loint(at);
+    const double y = p * table[n & (kTable - 1)];
+    const double z = __hiloint2double(__double2hiint(y) + ((n >> 6) << 20), __double2loint(y));
+    // (a product that is no number: beside an infinity, or -inf at a temperature of infinity)
+    return x == best ? (x > -INFINITY ? 1. : 0.) : (x - best) * c32 >= -120.f ? z : 0.;
   }
 };
-static_assert(kTable == 256, "the shifts above");
+static_assert(kTable == 64, "the shift above");
 
 // What a row's weights are relative to, and their sum.
 struct Total {
@@ -603,14 +604,14 @@ __device__ __noinline__ int exactly_drawn(const VerifyArgs& a, Cluster& cl, doub
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kDecide, 2) verify_decide_kernel(const VerifyArgs a) {
+__global__ void __launch_bounds__(kDecide, 3) verify_decide_kernel(const VerifyArgs a) {
   __shared__ Total totals[kBatch][2];                 // of the batch's rows: the target's, the draft's
   __shared__ float drafted[kBatch][2];                // the logits that both give the draft
   __shared__ int places[kBatch];                      // greedy: the arg-max
   __shared__ double sums[kWarps][2];
   __shared__ __align__(16) double slots[2][2];
   __shared__ int verdict[2];
-  __shared__ double tables[2 * kTable];
+  __shared__ double tables[kTable];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   Cluster cl{cluster_rank(), 0, 0, slots};
   asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(cl.size));
@@ -629,8 +630,7 @@ __global__ void __launch_bounds__(kDecide, 2) verify_decide_kernel(const VerifyA
   bool have_tables = false;
   auto make_tables = [&] {
     if (!have_tables)
-      for (int i = threadIdx.x; i < 2 * kTable; i += kDecide)
-        tables[i] = exp2(i < kTable ? (double)i / kTable : (double)(i - kTable) / (kTable * kTable));
+      for (int i = threadIdx.x; i < kTable; i += kDecide) tables[i] = exp2((double)i / kTable);
     __syncthreads();
     have_tables = true;
   };
@@ -941,15 +941,7 @@ GF_EXPORT int gf_verify(const char* words) {
                        dim3(kScan), 0, stream, a);
   }
   if (rc) return rc;
-  static OncePerDevice attrs;
-  rc = attrs.run([&] {
-    const cudaError_t e = cudaFuncSetAttribute(verify_decide_kernel<bf16>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    return e != cudaSuccess ? e
-                            : cudaFuncSetAttribute(verify_decide_kernel<float>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  });
-  if (rc) return rc;
-  const char* env = getenv("GF_CLUSTER");
-  const int cluster = env ? atoi(env) : 8;
+  const int cluster = a.B > kManyRequests ? 4 : 8;
   return launch_kernel_cluster_dims(half ? verify_decide_kernel<bf16> : verify_decide_kernel<float>, dim3(a.B * cluster),
                                     dim3(kDecide), 0, stream, cluster, true, a);
 }

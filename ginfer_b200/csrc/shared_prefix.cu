@@ -5,6 +5,8 @@
 #define GF_HEAD_DIM 128
 #endif
 
+#include <cstdlib>
+
 #include "attention_tc.cuh"
 #include "mma_bits.cuh"
 #include "shared_prefix.cuh"
@@ -63,8 +65,12 @@ struct PieceArgs {
   PrefixArgs a;
   int mode, tma, joined;       // joined: another kernel adds a row's pieces up (else every item is whole)
   int after;                   // the launch runs beside the one before it, whose results the joining kernel reads, too
-  Shape shape;
-  int H;                       // kv heads * chunks
+  int sms;
+  Shape far_shape;             // of the prefixes' kernel, where there is one: its rows, tiles and cost of a tile
+  int far_tile, far_H;
+  float far_cost;
+  Shape shape, own_shape;      // own_shape: of own tokens
+  int H;                       // kv heads * chunks (of own tokens)
   int places;                  // for pieces of prefixes
   int* chunk;                  // PREFIX: where the length of a chunk is written down
   OwnPlan* plan;
@@ -90,12 +96,19 @@ struct Pieces {
   const PieceArgs& p;
   Cursor cur;
   Request req;
+  RawRequest ahead;            // the next request's numbers, on their way
   GroupTiles groups;
-  int chunk, index;
-  __device__ __forceinline__ void start(const Cursor& c, int chunk_) {
-    cur = c, chunk = chunk_, index = blockIdx.x;
-    if (p.mode == PREFIX) groups.load(p.a, threadIdx.x & 31, p.shape.tokens, TILE);
-    else if (cur.todo > 0) req = request_of(p.a, cur.b, p.mode == BOTH, TILE);
+  int chunk, index, stride;
+  __device__ __forceinline__ void start(const Cursor& c) {
+    cur = c;
+    if (cur.todo > 0) {
+      req = request_of(p.a, cur.b, p.mode == BOTH, TILE);
+      ahead.load(p.a, cur.b + 1 < p.a.B ? cur.b + 1 : 0, p.mode == BOTH);
+    }
+  }
+  __device__ __forceinline__ void start(const GroupTiles& g, int chunk_, int blocks) {
+    groups = g, chunk = chunk_, index = blockIdx.x, stride = blocks;
+    if (index >= blocks) index = p.places;
   }
   __device__ __forceinline__ bool next(Piece& x) {
     const PrefixArgs& a = p.a;
@@ -107,29 +120,48 @@ struct Pieces {
       x.far = it.tiles, x.far_len = it.length, x.near_len = 0, x.last = -1;
       x.far_table = a.prefix_table + (size_t)it.g * a.prefix_stride, x.near_table = nullptr;
       x.to = Piece::FAR, x.at = index;
-      index += gridDim.x;
+      index += stride;
       return true;
     }
-    if (cur.todo <= 0) return false;
-    const int tiles = req.tiles(), done = cur.rt * p.shape.tokens;
-    x.first = req.first + done, x.tokens = min(p.shape.tokens, req.count - done), x.hc = cur.hc;
-    x.from = cur.off, x.count = (int)min(cur.todo, (long long)(tiles - cur.off));
-    x.far = req.far, x.far_len = req.shared, x.near_len = req.len, x.last = req.len - req.count + done;
-    x.far_table = a.prefix_table + (size_t)max(req.g, 0) * a.prefix_stride;
-    x.near_table = a.table + (size_t)cur.b * a.table_stride;
-    const bool starts = cur.off == 0, ends = cur.off + x.count == tiles;
-    x.to = starts && ends ? (p.mode == BOTH ? Piece::FINAL : Piece::ROW) : Piece::CUT;
-    x.at = (size_t)blockIdx.x * 2 + (starts ? 1 : 0);
-    // on to the next
-    cur.todo -= x.count, cur.off = 0;
-    if (ends && cur.todo > 0 && ++cur.rt >= req.row_tiles(p.shape.tokens)) {
-      cur.rt = 0;
-      do {
-        if (++cur.b == a.B) cur.b = 0, ++cur.hc;
-        req = request_of(a, cur.b, p.mode == BOTH, TILE);
-      } while (req.count == 0);
+    if (!p.joined) {
+      const int done = cur.rt * p.shape.tokens;
+      if (done >= req.count) return false;
+      x.first = req.first + done, x.tokens = min(p.shape.tokens, req.count - done), x.hc = cur.hc;
+      x.from = 0, x.count = req.tiles();
+      x.far = req.far, x.far_len = req.shared, x.near_len = req.len, x.last = req.len - req.count + done;
+      x.far_table = a.prefix_table + (size_t)max(req.g, 0) * a.prefix_stride;
+      x.near_table = a.table + (size_t)cur.b * a.table_stride;
+      x.to = Piece::FINAL;
+      cur.rt += gridDim.x;
+      return true;
     }
-    return true;
+    while (cur.todo > 0) {
+      const int tiles = req.tiles(), units = req.units(), done = cur.rt * p.shape.tokens, from = cur.off;
+      const int count = (int)min(cur.todo, (long long)(units - from));
+      const bool some = from < tiles;              // (else only the item's end, which costs time and has no tiles)
+      if (some) {
+        x.first = req.first + done, x.tokens = min(p.shape.tokens, req.count - done), x.hc = cur.hc;
+        x.from = from, x.count = min(count, tiles - from);
+        x.far = req.far, x.far_len = req.shared, x.near_len = req.len, x.last = req.len - req.count + done;
+        x.far_table = a.prefix_table + (size_t)max(req.g, 0) * a.prefix_stride;
+        x.near_table = a.table + (size_t)cur.b * a.table_stride;
+        const bool starts = from == 0, ends = from + x.count == tiles;
+        x.to = starts && ends ? (p.mode == BOTH ? Piece::FINAL : Piece::ROW) : Piece::CUT;
+        x.at = (size_t)blockIdx.x * 2 + (starts ? 1 : 0);
+      }
+      // on to the next
+      cur.todo -= count, cur.off = 0;
+      if (cur.todo > 0 && ++cur.rt >= req.row_tiles(p.shape.tokens)) {
+        cur.rt = 0;
+        do {
+          if (++cur.b == a.B) cur.b = 0, ++cur.hc;
+          req = ahead.get(a, TILE);
+          ahead.load(a, cur.b + 1 < a.B ? cur.b + 1 : 0, p.mode == BOTH);
+        } while (req.count == 0);
+      }
+      if (some) return true;
+    }
+    return false;
   }
 };
 // Tile x of a piece's sequence: whose it is, its first key and the sequence's end.
@@ -221,7 +253,9 @@ prefix_pieces_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
   float* merge = reinterpret_cast<float*>(ring + STAGES * STAGE);
   uint64_t* full = reinterpret_cast<uint64_t*>(ring + STAGES * STAGE + MERGE);
   uint64_t* empty = full + STAGES;
-  __shared__ int chunk_s;
+  __shared__ int chunk_s, far_s;
+  __shared__ long long counts[CONSUMERS];
+  __shared__ Cursor found_s;
   const PrefixArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -233,28 +267,44 @@ prefix_pieces_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
   }
   if (!p.after) pdl_wait();
   if (p.mode == PREFIX) pdl_trigger();
-  Cursor c{};
-  if (p.mode == PREFIX) {
-    if (warp == 0) {
-      const int chunk = plan_chunk(a, p.H, p.shape.tokens, TILE, gridDim.x, p.places, 3);
-      if (lane == 0) {
-        chunk_s = chunk;
-        if (blockIdx.x == 0) *p.chunk = chunk;
+  Pieces pieces{p};
+  const bool both = p.mode == BOTH;
+  if (p.mode == PREFIX || p.after) {
+    // how the prefixes and the own tokens share the SMs, and the prefixes' chunks
+    GroupTiles t{};
+    FarWork f{};
+    if (warp == CONSUMERS) f = far_work(a, t, p.far_H, p.far_shape.tokens, p.far_tile);
+    const OwnWork w = own_work<32 * CONSUMERS>(a, p.own_shape.tokens, TILE, both, counts);
+    if (warp == CONSUMERS) {
+      const int share = far_share(p.sms, f.units, p.far_cost, w.total * p.H);
+      if (lane == 0) far_s = share;
+      if (p.mode == PREFIX) {
+        const int chunk = plan_chunk(a, t, f, p.far_H, p.far_shape.tokens, p.far_tile, max(1, share * BLOCKS_AN_SM), p.places, 3);
+        if (lane == 0) {
+          chunk_s = chunk;
+          if (blockIdx.x == 0) *p.chunk = chunk;
+        }
       }
     }
     __syncthreads();
+    const int far = far_s;
+    if (p.mode == PREFIX) {
+      if (warp != CONSUMERS) t.load(a, lane, p.shape.tokens, TILE);
+      pieces.start(t, chunk_s, far * BLOCKS_AN_SM);
+    } else {
+      pieces.start(find_run<32 * CONSUMERS>(a, w, p.H, p.shape.tokens, TILE, both, blockIdx.x, max(p.sms - far, 1) * BLOCKS_AN_SM,
+                                            blockIdx.x == 0 ? p.plan : nullptr, &found_s));
+    }
   } else if (p.joined) {
-    c = find_run<32 * CONSUMERS>(a, p.H, p.shape.tokens, TILE, p.mode == BOTH, blockIdx.x, gridDim.x,
-                                 blockIdx.x == 0 ? p.plan : nullptr);
+    const OwnWork w = own_work<32 * CONSUMERS>(a, p.shape.tokens, TILE, both, counts);
+    pieces.start(find_run<32 * CONSUMERS>(a, w, p.H, p.shape.tokens, TILE, both, blockIdx.x, gridDim.x,
+                                          blockIdx.x == 0 ? p.plan : nullptr, &found_s));
   } else {
-    // a block an item: (row tile, request, heads)
-    c.rt = blockIdx.x, c.b = blockIdx.y, c.hc = blockIdx.z;
-    const Request r = request_of(a, c.b, true, TILE);
-    c.todo = c.rt < r.row_tiles(p.shape.tokens) ? r.tiles() : 0;
+    // a block an item: (row tile, request, heads), and the row tiles behind it that the grid leaves out
+    pieces.cur = {(int)blockIdx.z, (int)blockIdx.y, (int)blockIdx.x, 0, 0};
+    pieces.req = request_of(a, blockIdx.y, true, TILE);
     __syncthreads();
   }
-  Pieces pieces{p};
-  pieces.start(c, chunk_s);
   Piece x;
   int st = 0;
   uint32_t ph = 0;
@@ -387,14 +437,10 @@ prefix_pieces_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
           if (sharing == 4) {
             if (k.key0 + share * 16 <= any_sees)
               mma_step<2>(stage, share * 16, k.key0, qf, o, m, l, seen, all_see, scale_log2, lane);
-          } else if (sharing == 2) {
-            if (k.key0 + share * 32 <= any_sees)
-              mma_step<4>(stage, share * 32, k.key0, qf, o, m, l, seen, all_see, scale_log2, lane);
           } else {
 #pragma unroll 1
-            for (int half = 0; half < 2; ++half)
-              if (k.key0 + half * 32 <= any_sees)
-                mma_step<4>(stage, half * 32, k.key0, qf, o, m, l, seen, all_see, scale_log2, lane);
+            for (int key = share * 32; key < TILE; key += 32 * sharing)
+              if (k.key0 + key <= any_sees) mma_step<4>(stage, key, k.key0, qf, o, m, l, seen, all_see, scale_log2, lane);
           }
         }
         __syncwarp();
@@ -527,15 +573,15 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) prefix_join_kernel(const Join
     }
   }
   const long long run = __ldcg(&p.plan->run), per = __ldcg(&p.plan->each), base = __ldcg(&p.plan->base[b]);
-  const int tiles = r.tiles();
+  const int tiles = r.tiles(), units = r.units();
   for (int i = blockIdx.z * JOIN_WARPS + warp; i < r.count * each; i += gridDim.z * JOIN_WARPS) {
     const int token = i / each, hh = i - token * each, t = r.first + token;
     const size_t row = (size_t)t * a.nh + kvh * each + hh;
     // its own tokens' pieces: the blocks whose runs have some of its tiles
     const int rt = token / p.shape.tokens, part = hh / p.shape.heads, heads = min(p.shape.heads, each - part * p.shape.heads);
     const int own_r = (token - rt * p.shape.tokens) * heads + hh - part * p.shape.heads;
-    const long long s0 = (kvh * p.shape.chunks + part) * per + base + (long long)rt * tiles;
-    const int k0 = (int)(s0 / run), k1 = (int)((s0 + tiles - 1) / run);
+    const long long s0 = (kvh * p.shape.chunks + part) * per + base + (long long)rt * units;
+    const int k0 = (int)quotient(s0, run), k1 = (int)quotient(s0 + tiles - 1, run);
     const bool cut = k1 > k0;
     if (!cut && both) continue;                          // (the row is written already)
     const int far_part = j.far_tile ? hh / j.far_shape.heads : 0;
@@ -718,6 +764,10 @@ using namespace gf;
 
 GF_DEFINE_PDL_SWITCH
 
+// What a tile of a prefix costs beside a tile of own tokens (64 keys that come from memory): 128 keys on the tensor cores with up to
+// 128 rows, 64 keys on mma.sync with up to 64 rows.
+constexpr float kTensorCost = 2.f, kPlainCost = 2.f;
+
 // `words`: q, its row stride and type, k, v, pages, page, prefix_table and its stride, prefix_lens, groups, prefix limit,
 // table and its stride, lengths, requests, limit, cu_groups, cu, out, rows, heads, kv heads, SMs, the rows that a request has
 // at most (a hint), scratch and its bytes, err, stream; then the scale as a double.
@@ -750,9 +800,11 @@ struct Call {
     a.scale = (float)*reinterpret_cast<const double*>(w + i);
     a.hd = HD;
     a.page_shift = (a.page & (a.page - 1)) == 0 ? 31 - __builtin_clz(a.page) : -1;
-    shared = a.G > 0 && a.prefix_limit > 0;
+    const char* env2 = getenv("GF_UNSHARED");
+    shared = a.G > 0 && a.prefix_limit > 0 && a.T > (env2 ? atoi(env2) : 2);
     p.shape = row_shape_of(a.nh, a.nkv, MOST_ROWS);
     p.H = a.nkv * p.shape.chunks;
+    p.own_shape = p.shape, p.sms = sms;
     blocks = sms * BLOCKS_AN_SM;
     // the scratch: the division, pieces of cut items, of rows, of prefixes
     need = 0;
@@ -770,6 +822,8 @@ struct Call {
       tensor = GF_PREFIX_TC && type == GF_BF16 && a.page % 8 == 0 && 128 % a.page == 0;
       j.far_tile = tensor ? 128 : TILE, j.far_rows = tensor ? 128 : MOST_ROWS;
       j.far_shape = row_shape_of(a.nh, a.nkv, j.far_rows);
+      p.far_shape = j.far_shape, p.far_tile = j.far_tile, p.far_H = a.nkv * j.far_shape.chunks;
+      p.far_cost = tensor ? kTensorCost : kPlainCost;
       const long long tiles = (long long)a.nkv * j.far_shape.chunks * ((a.T + j.far_shape.tokens - 1) / j.far_shape.tokens + a.G);
       const long long least = 2ll * (tensor ? sms : blocks);
       p.places = (int)(tiles > least ? tiles : least);
@@ -803,6 +857,13 @@ GF_EXPORT int gf_prefix_attend(const char* words) {
     if (!page_map(&mk, a.k, a, rows) || !page_map(&mv, a.v, a, rows)) return -7;
   }
   JoinArgs& j = c.j;
+  const char* env = getenv("GF_SHORT");
+  if (a.prefix_limit + a.limit <= (env ? atoi(env) : 512) && a.B <= 65535 && p.H <= 65535) {
+    p.mode = BOTH, p.joined = 0;
+    const int row_tiles = (c.longest + p.shape.tokens - 1) / p.shape.tokens;
+    return launch_kernel(prefix_pieces_kernel, dim3(row_tiles > 1 ? row_tiles : 1, a.B, p.H), dim3(THREADS), PIECES_SMEM, c.stream,
+                         mk, mv, p);
+  }
   if (c.shared) {
     int rc;
 #if GF_PREFIX_TC
@@ -812,7 +873,7 @@ GF_EXPORT int gf_prefix_attend(const char* words) {
         return cudaFuncSetAttribute(tc::prefix_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tc::SMEM);
       });
       if (rc) return rc;
-      const tc::Args t{a, j.far_shape, a.nkv * j.far_shape.chunks, p.places, a.pages * a.page, p.chunk, p.far_o, p.far_ml, p.err};
+      const tc::Args t{a, j.far_shape, p.shape, p.far_H, p.H, p.places, a.pages * a.page, c.sms, TILE, p.far_cost, p.chunk, p.far_o, p.far_ml, p.err};
       CUtensorMap tq, tk, tv;
       if (!query_map(&tq, a, j.far_shape) || !page_map(&tk, a.k, a, a.page) || !page_map(&tv, a.v, a, a.page)) return -7;
       rc = launch_kernel(tc::prefix_tc_kernel, dim3(c.sms), dim3(tc::NTHREADS_TC), tc::SMEM, c.stream, tq, tk, tv, t);

@@ -82,6 +82,11 @@ __device__ __forceinline__ int slot_of(const PrefixArgs& a, const int* tbl, int 
   return page_in(a, fresh_index(tbl + lp)) * a.page + (c - lp * a.page);
 }
 
+// a / b for numbers that are small as a rule (a 64-bit division takes longer than the rest of the division of the work).
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  return (a | b) >> 32 ? a / b : (long long)((unsigned)a / (unsigned)b);
+}
+
 // ------------------------------------------------------------------------------------- rows
 struct Shape {
   int chunks, heads, tokens;    // chunks of a kv head's query heads, heads of a chunk at most, tokens of a row tile
@@ -111,45 +116,55 @@ struct GroupTiles {
     }
   }
 };
-// Tiles of a chunk of keys, by one warp.  With `workers` blocks the time is about (rounds of items) * (chunk + over),
-// over: what an item's start and end cost in tiles.  Looked at are the 32 lengths from one, a half and a third of an equal share
-// on; the longest prefix, which is always possible, is the last resort.
-__device__ __forceinline__ int plan_chunk(const PrefixArgs& a, int H, int tokens, int tile, int workers, int places, int over) {
+// The prefixes' work, by one warp: row tiles times key tiles of all heads, and the longest prefix.  `t` keeps the first 32 groups.
+struct FarWork {
+  long long units;
+  int most;
+};
+__device__ __forceinline__ FarWork far_work(const PrefixArgs& a, GroupTiles& t, int H, int tokens, int tile) {
   const int lane = threadIdx.x & 31;
-  GroupTiles t;
   t.load(a, lane, tokens, tile);
-  long long units = 0;
-  int most = 0;
-  for (int g0 = 0; g0 < a.G; g0 += 32) {
-    if (g0) t.load(a, g0 + lane, tokens, tile);
-    units += (long long)t.mt * H * t.nt;
-    most = max(most, t.mt ? t.nt : 0);
+  FarWork w{(long long)t.mt * H * t.nt, t.mt ? t.nt : 0};
+  for (int g0 = 32; g0 < a.G; g0 += 32) {
+    GroupTiles u;
+    u.load(a, g0 + lane, tokens, tile);
+    w.units += (long long)u.mt * H * u.nt;
+    w.most = max(w.most, u.mt ? u.nt : 0);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    units += __shfl_xor_sync(0xffffffffu, units, o);
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    w.units += __shfl_xor_sync(0xffffffffu, w.units, o);
+    w.most = max(w.most, __shfl_xor_sync(0xffffffffu, w.most, o));
   }
-  if (most == 0) return 1;
+  return w;
+}
+// Tiles of a chunk of keys, by one warp.  With `workers` blocks the time is about (rounds of items) * (chunk + over),
+// over: what an item's start and end cost in tiles.  Looked at are the 32 lengths from one, a half and a third of an equal share
+// on; the longest prefix, which is always possible, is the last resort.
+__device__ __forceinline__ int plan_chunk(const PrefixArgs& a, const GroupTiles& first, const FarWork& all, int H, int tokens, int tile,
+                                          int workers, int places, int over) {
+  const int lane = threadIdx.x & 31;
+  if (all.most == 0) return 1;
+  GroupTiles t = first;
   int len[3];
-  long long items[3] = {0, 0, 0};
+  int items[3] = {0, 0, 0};
 #pragma unroll
   for (int k = 0; k < 3; ++k) {
-    const long long share = (units + (long long)workers * (k + 1) - 1) / ((long long)workers * (k + 1));
-    const int from = (int)(share < most ? share : most);
-    len[k] = min(most, max(1, from) + lane * max(1, from / 48));
+    const long long share = quotient(all.units + (long long)workers * (k + 1) - 1, (long long)workers * (k + 1));
+    const int from = (int)(share < all.most ? share : all.most);
+    len[k] = min(all.most, max(1, from) + lane * max(1, from / 48));
   }
-  if (lane == 31) len[0] = most;
+  if (lane == 31) len[0] = all.most;
   for (int g0 = 0; g0 < a.G; g0 += 32) {
-    if (a.G > 32) t.load(a, g0 + lane, tokens, tile);
+    if (g0) t.load(a, g0 + lane, tokens, tile);
     for (int i = 0; i < min(32, a.G - g0); ++i) {
       const int mt = __shfl_sync(0xffffffffu, t.mt, i) * H, nt = __shfl_sync(0xffffffffu, t.nt, i);
 #pragma unroll
-      for (int k = 0; k < 3; ++k) items[k] += (long long)mt * ((nt + len[k] - 1) / len[k]);
+      for (int k = 0; k < 3; ++k) items[k] += mt * ((nt + len[k] - 1) / len[k]);
     }
   }
   float best = INFINITY;
-  int chunk = most;
+  int chunk = all.most;
 #pragma unroll
   for (int k = 0; k < 3; ++k) {
     const float rounds = (float)((items[k] + workers - 1) / workers), cost = rounds * (len[k] + over);
@@ -201,85 +216,110 @@ __device__ __forceinline__ bool find_item(const PrefixArgs& a, const GroupTiles&
 }
 
 // ------------------------------------------------------------------------------------- requests' own tokens
+// What a request's start and end cost beside its tiles, in tiles: waiting for its numbers, its rows of q, joining the warps.
+constexpr int kItemTiles = 2;
 struct Request {
   int first, count, len, shared, g;     // its rows, its own tokens, tokens of the prefix (0 where that is another kernel's)
   int far, near;                        // tiles of the prefix, of the own tokens
   __device__ __forceinline__ int tiles() const { return max(1, far + near); }
+  __device__ __forceinline__ int units() const { return tiles() + kItemTiles; }
   __device__ __forceinline__ int row_tiles(int tokens) const { return (count + tokens - 1) / tokens; }
 };
+// A request's numbers as they are loaded, for when they are wanted.
+struct RawRequest {
+  int cu0, cu1, len, g;
+  __device__ __forceinline__ void load(const PrefixArgs& a, int b, bool both) {
+    cu0 = a.cu ? fresh_index(a.cu + b) : b, cu1 = a.cu ? fresh_index(a.cu + b + 1) : b + 1;
+    len = fresh_index(a.lengths + b);
+    g = both ? group_of(a, b) : -1;
+  }
+  __device__ __forceinline__ Request get(const PrefixArgs& a, int tile) const {
+    Request r;
+    r.first = min(max(cu0, 0), a.T), r.count = max(min(max(cu1, 0), a.T) - r.first, 0);
+    r.len = min(max(len, 0), a.limit);
+    r.g = g, r.shared = prefix_length(a, g);
+    r.far = (r.shared + tile - 1) / tile, r.near = (r.len + tile - 1) / tile;
+    return r;
+  }
+};
 __device__ __forceinline__ Request request_of(const PrefixArgs& a, int b, bool both, int tile) {
-  Request r;
-  const Rows rows = rows_of(a, b);
-  r.first = rows.first, r.count = rows.count, r.len = own_length(a, b);
-  r.g = both ? group_of(a, b) : -1;
-  r.shared = prefix_length(a, r.g);
-  r.far = (r.shared + tile - 1) / tile, r.near = (r.len + tile - 1) / tile;
-  return r;
+  RawRequest raw;
+  raw.load(a, b, both);
+  return raw.get(a, tile);
 }
-// Where a block's run is: tiles `off` on of the row tile `rt` of request b, for heads hc.
+// Where a block's run is: units `off` on of the row tile `rt` of request b, for heads hc.
 struct Cursor {
   int hc, b, rt, off;
   long long todo;
 };
-// What the joining kernel needs of the division: a run's tiles, the tiles of one (kv head, chunk of heads), and the tiles
+// What the joining kernel needs of the division: a run's units, the units of one (kv head, chunk of heads), and the units
 // before every request's.
 struct OwnPlan {
   long long run, each;
   long long base[1];            // [B]
 };
-constexpr int kLeastRun = 4;    // the fewest tiles of a run
+constexpr int kLeastRun = 4;    // the fewest units of a run
 
-// The run of block `k` of `blocks`, by the first `threads` threads of the block (a multiple of 32; all call); `plan`: where the
-// division is written down, by the block that is given it.
+// The units of the requests of a block's first THREADS threads, a neighbouring share of all requests each, and of all before and
+// in all.
+struct OwnWork {
+  int b0, b1;
+  long long mine, start, total;
+};
 template <int THREADS>
-__device__ __forceinline__ Cursor find_run(const PrefixArgs& a, int H, int tokens, int tile, bool both, int k, int blocks,
-                                           OwnPlan* plan) {
-  __shared__ long long counts[THREADS / 32];
-  __shared__ Cursor found;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int each = (a.B + THREADS - 1) / THREADS, b0 = min((int)threadIdx.x * each, a.B), b1 = min(b0 + each, a.B);
-  long long mine = 0, total = 0;
+__device__ __forceinline__ OwnWork own_work(const PrefixArgs& a, int tokens, int tile, bool both, long long* counts) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, each = (a.B + THREADS - 1) / THREADS;
+  OwnWork w{min((int)threadIdx.x * each, a.B), 0, 0, 0, 0};
+  w.b1 = min(w.b0 + each, a.B);
   if (threadIdx.x < THREADS)
-    for (int b = b0; b < b1; ++b) {
+    for (int b = w.b0; b < w.b1; ++b) {
       const Request r = request_of(a, b, both, tile);
-      mine += (long long)r.row_tiles(tokens) * r.tiles();
+      w.mine += (long long)r.row_tiles(tokens) * r.units();
     }
-  long long sum = mine;
+  long long sum = w.mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const long long up = __shfl_up_sync(0xffffffffu, sum, o);
     if (lane >= o) sum += up;
   }
   if (lane == 31 && warp < THREADS / 32) counts[warp] = sum;
-  if (threadIdx.x == 0) found.todo = 0;
   __syncthreads();
-  long long start = sum - mine;
+  w.start = sum - w.mine;
 #pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) {
-    if (w < warp) start += counts[w];
-    total += counts[w];
+  for (int i = 0; i < THREADS / 32; ++i) {
+    if (i < warp) w.start += counts[i];
+    w.total += counts[i];
   }
-  const long long all = total * H, share = (all + blocks - 1) / blocks;
+  return w;
+}
+// The run of block `k` of `blocks`; all call.  `plan`: where the division is written down, by the block that is given it.
+template <int THREADS>
+__device__ __forceinline__ Cursor find_run(const PrefixArgs& a, const OwnWork& w, int H, int tokens, int tile, bool both, int k,
+                                           int blocks, OwnPlan* plan, Cursor* found) {
+  if (threadIdx.x == 0) found->todo = 0;
+  __syncthreads();
+  const long long all = w.total * H, share = quotient(all + blocks - 1, blocks);
   const long long run = share > kLeastRun ? share : kLeastRun, at = run * k;
   if (plan && threadIdx.x < THREADS) {
-    if (threadIdx.x == 0) plan->run = run, plan->each = total;
-    long long base = start;
-    for (int b = b0; b < b1; ++b) {
+    if (threadIdx.x == 0) plan->run = run, plan->each = w.total;
+    long long base = w.start;
+    for (int b = w.b0; b < w.b1; ++b) {
       const Request r = request_of(a, b, both, tile);
       plan->base[b] = base;
-      base += (long long)r.row_tiles(tokens) * r.tiles();
+      base += (long long)r.row_tiles(tokens) * r.units();
     }
   }
-  if (at < all && threadIdx.x < THREADS) {
-    const int hc = (int)(at / total);
-    long long rest = at - hc * total;
-    if (rest >= start && rest < start + mine) {
-      rest -= start;
-      for (int b = b0; b < b1; ++b) {
+  if (at < all && k < blocks && threadIdx.x < THREADS) {
+    const int hc = (int)quotient(at, w.total);
+    long long rest = at - hc * w.total;
+    if (rest >= w.start && rest < w.start + w.mine) {
+      rest -= w.start;
+      for (int b = w.b0; b < w.b1; ++b) {
         const Request r = request_of(a, b, both, tile);
-        const long long tiles = r.tiles(), here = r.row_tiles(tokens) * tiles;
+        const long long units = r.units(), here = r.row_tiles(tokens) * units;
         if (rest < here) {
-          found = {hc, b, (int)(rest / tiles), (int)(rest % tiles), min(run, all - at)};
+          const int rt = (int)quotient(rest, units);
+          *found = {hc, b, rt, (int)(rest - rt * units), min(run, all - at)};
           break;
         }
         rest -= here;
@@ -287,7 +327,16 @@ __device__ __forceinline__ Cursor find_run(const PrefixArgs& a, int H, int token
     }
   }
   __syncthreads();
-  return found;
+  return *found;
+}
+
+// Prefixes and own tokens are worked on side by side, by two launches: of `sms` SMs this many have the prefixes.  A tile of a
+// prefix costs kFarCost of what a tile of own tokens does.
+__device__ __forceinline__ int far_share(int sms, long long far_units, float far_cost, long long own_units) {
+  if (far_units == 0) return 0;
+  const float far = (float)far_units * far_cost, own = (float)own_units;
+  const int share = (int)(sms * far / (far + own) + 0.5f);
+  return min(max(share, 1), own_units > 0 ? sms - 1 : sms);
 }
 
 }  // namespace gf

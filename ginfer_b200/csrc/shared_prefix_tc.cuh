@@ -27,22 +27,25 @@ static_assert(256 * REGS_SMALL + 256 * REGS_SOFTMAX <= 65536, "the register file
 constexpr uint32_t OPERAND = HALVES * ATOM_BYTES;   // [128 rows][HD]
 constexpr uint32_t TMEM_COLS = 512;                 // S_0 / P_0: 0..127, S_1 / P_1: 128..255, O_0, O_1: 256..
 constexpr float kRescaleStep = 8.f;                 // log2 units a maximum may grow before O is rescaled
-constexpr int kItemTiles = 2;                       // what an item costs beside its tiles
+constexpr int kOver = 2;                            // what an item costs beside its tiles
 
 struct Barriers {
   uint64_t q_full, q_empty;
   uint64_t k_full[NS * KS], k_empty[NS * KS], v_full[NS * VS], v_empty[NS * VS];
   uint64_t s_full[NS], p_ready[NS], pv_done[NS], stat_ready, o_free, drained;
   uint32_t tmem_base;
-  int abort_flag, chunk;
+  int abort_flag, chunk, workers;
+  GroupTiles groups[32];       // the first 32 groups'
+  long long own[4];
   float stat_m[NS][QT], stat_l[NS][QT];
 };
 constexpr uint32_t SMEM = OPERAND * (1 + NS * KS + NS * VS) + sizeof(Barriers);
 
 struct Args {
   PrefixArgs a;
-  Shape shape;
-  int H, places, oob_row;
+  Shape shape, own_shape;      // rows of this kernel's tiles, of the one's that works on own tokens beside it
+  int H, own_H, places, oob_row, sms, own_tile;
+  float cost;                  // of a tile beside one of own tokens
   int* chunk;
   float* far_o;                // [places][QT][HD]
   float2* far_ml;
@@ -103,10 +106,17 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  // how the prefixes and the own tokens share the SMs: own tokens counted by the first four warps
+  GroupTiles t{};
+  FarWork f{};
+  if (warp == 5) f = far_work(a, t, g.H, g.shape.tokens, KT);
+  const OwnWork own = own_work<128>(a, g.own_shape.tokens, g.own_tile, false, bars->own);
   if (warp == 5) {
-    const int chunk = plan_chunk(a, g.H, g.shape.tokens, KT, gridDim.x, g.places, kItemTiles);
+    const int workers = min((int)gridDim.x, far_share(g.sms, f.units, g.cost, own.total * g.own_H));
+    const int chunk = plan_chunk(a, t, f, g.H, g.shape.tokens, KT, max(workers, 1), g.places, kOver);
+    bars->groups[lane] = t;
     if (lane == 0) {
-      bars->chunk = chunk;
+      bars->chunk = chunk, bars->workers = workers;
       if (blockIdx.x == 0) *g.chunk = chunk;
     }
   }
@@ -118,14 +128,13 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = bars->tmem_base, tmem_s = tmem, tmem_o = tmem + NS * KT;
-  const int chunk = bars->chunk;
-  GroupTiles groups;
-  groups.load(a, lane, g.shape.tokens, KT);
+  const int chunk = bars->chunk, workers = bars->workers;
+  const GroupTiles groups = bars->groups[lane];
   PrefixItem it;
   // the block's n-th item; by whole warps
   auto item_of = [&](int n) {
-    const int index = n * (int)gridDim.x + (int)blockIdx.x;
-    return index < g.places && find_item(a, groups, g.H, g.shape.tokens, KT, chunk, index, it);
+    const int index = n * workers + (int)blockIdx.x;
+    return (int)blockIdx.x < workers && index < g.places && find_item(a, groups, g.H, g.shape.tokens, KT, chunk, index, it);
   };
   auto tiles_of = [](int ntiles, int s) { return (ntiles - s + 1) >> 1; };     // of stream s
 
@@ -402,7 +411,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
       const float f0 = s == 0 ? f_me : f_o, f1 = s == 0 ? f_o : f_me;
       const bool two = ntiles > 1;
       const uint32_t o0 = tmem_o + lane_addr + s * (HD / 2), o1 = o0 + HD;
-      const size_t at = (size_t)(n * (int)gridDim.x + (int)blockIdx.x) * QT + r;
+      const size_t at = (size_t)(n * workers + (int)blockIdx.x) * QT + r;
       float* to = g.far_o + at * HD + s * (HD / 2);
       if (live && s == 0) g.far_ml[at] = make_float2(m_all, l * f_me + l_o * f_o);
 #pragma unroll 1

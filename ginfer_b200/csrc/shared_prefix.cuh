@@ -12,8 +12,8 @@
 //    every item's piece has a place of its own.  Row tiles of one chunk of keys are neighbours, so that they read it at the
 //    same time.
 //  * a request's own tokens (Cursor): the tiles of all requests (and of their tiles of rows) are one long sequence, and
-//    every block takes an equal run of it, so that blocks end together whatever the lengths.  A run begins and ends inside
-//    requests; what is cut has the block's two places, the rest a row's own.
+//    every warp takes an equal run of it, so that warps end together whatever the lengths.  A run begins and ends inside
+//    requests; what is cut has the warp's two places, the rest a row's own.
 // The joining kernel works the same arithmetic out again and adds a row's pieces up, in order: no atomics.
 #pragma once
 #include "common.cuh"
@@ -217,7 +217,7 @@ __device__ __forceinline__ bool find_item(const PrefixArgs& a, const GroupTiles&
 
 // ------------------------------------------------------------------------------------- requests' own tokens
 // What a request's start and end cost beside its tiles, in tiles: waiting for its numbers, its rows of q, joining the warps.
-constexpr int kItemTiles = 2;
+constexpr int kItemTiles = 4;
 struct Request {
   int first, count, len, shared, g;     // its rows, its own tokens, tokens of the prefix (0 where that is another kernel's)
   int far, near;                        // tiles of the prefix, of the own tokens
@@ -225,29 +225,16 @@ struct Request {
   __device__ __forceinline__ int units() const { return tiles() + kItemTiles; }
   __device__ __forceinline__ int row_tiles(int tokens) const { return (count + tokens - 1) / tokens; }
 };
-// A request's numbers as they are loaded, for when they are wanted.
-struct RawRequest {
-  int cu0, cu1, len, g;
-  __device__ __forceinline__ void load(const PrefixArgs& a, int b, bool both) {
-    cu0 = a.cu ? fresh_index(a.cu + b) : b, cu1 = a.cu ? fresh_index(a.cu + b + 1) : b + 1;
-    len = fresh_index(a.lengths + b);
-    g = both ? group_of(a, b) : -1;
-  }
-  __device__ __forceinline__ Request get(const PrefixArgs& a, int tile) const {
-    Request r;
-    r.first = min(max(cu0, 0), a.T), r.count = max(min(max(cu1, 0), a.T) - r.first, 0);
-    r.len = min(max(len, 0), a.limit);
-    r.g = g, r.shared = prefix_length(a, g);
-    r.far = (r.shared + tile - 1) / tile, r.near = (r.len + tile - 1) / tile;
-    return r;
-  }
-};
 __device__ __forceinline__ Request request_of(const PrefixArgs& a, int b, bool both, int tile) {
-  RawRequest raw;
-  raw.load(a, b, both);
-  return raw.get(a, tile);
+  Request r;
+  const Rows rows = rows_of(a, b);
+  r.first = rows.first, r.count = rows.count, r.len = own_length(a, b);
+  r.g = both ? group_of(a, b) : -1;
+  r.shared = prefix_length(a, r.g);
+  r.far = (r.shared + tile - 1) / tile, r.near = (r.len + tile - 1) / tile;
+  return r;
 }
-// Where a block's run is: units `off` on of the row tile `rt` of request b, for heads hc.
+// Where a warp's run is: units `off` on of the row tile `rt` of request b, for heads hc.
 struct Cursor {
   int hc, b, rt, off;
   long long todo;
@@ -258,7 +245,7 @@ struct OwnPlan {
   long long run, each;
   long long base[1];            // [B]
 };
-constexpr int kLeastRun = 4;    // the fewest units of a run
+constexpr int kLeastRun = 8;    // the fewest units of a run
 
 // The units of the requests of a block's first THREADS threads, a neighbouring share of all requests each, and of all before and
 // in all.
@@ -292,14 +279,15 @@ __device__ __forceinline__ OwnWork own_work(const PrefixArgs& a, int tokens, int
   }
   return w;
 }
-// The run of block `k` of `blocks`; all call.  `plan`: where the division is written down, by the block that is given it.
-template <int THREADS>
-__device__ __forceinline__ Cursor find_run(const PrefixArgs& a, const OwnWork& w, int H, int tokens, int tile, bool both, int k,
-                                           int blocks, OwnPlan* plan, Cursor* found) {
-  if (threadIdx.x == 0) found->todo = 0;
+// The runs of the WARPS warps of block `k` of `blocks`; all threads call.  `plan`: where the division is written down, by the block
+// that is given it.
+template <int THREADS, int WARPS>
+__device__ __forceinline__ void find_runs(const PrefixArgs& a, const OwnWork& w, int H, int tokens, int tile, bool both, int k,
+                                          int blocks, OwnPlan* plan, Cursor* found) {
+  if (threadIdx.x < WARPS) found[threadIdx.x].todo = 0;
   __syncthreads();
-  const long long all = w.total * H, share = quotient(all + blocks - 1, blocks);
-  const long long run = share > kLeastRun ? share : kLeastRun, at = run * k;
+  const long long all = w.total * H, runs = (long long)blocks * WARPS, share = quotient(all + runs - 1, runs);
+  const long long run = share > kLeastRun ? share : kLeastRun;
   if (plan && threadIdx.x < THREADS) {
     if (threadIdx.x == 0) plan->run = run, plan->each = w.total;
     long long base = w.start;
@@ -309,17 +297,20 @@ __device__ __forceinline__ Cursor find_run(const PrefixArgs& a, const OwnWork& w
       base += (long long)r.row_tiles(tokens) * r.units();
     }
   }
-  if (at < all && k < blocks && threadIdx.x < THREADS) {
-    const int hc = (int)quotient(at, w.total);
-    long long rest = at - hc * w.total;
-    if (rest >= w.start && rest < w.start + w.mine) {
-      rest -= w.start;
+  if (k < blocks && threadIdx.x < THREADS && w.mine > 0) {
+    long long hc_units = -1, hc = 0;
+    for (int i = 0; i < WARPS; ++i) {
+      const long long at = run * ((long long)k * WARPS + i);
+      if (at >= all) break;
+      if (hc_units < 0 || at >= hc_units + w.total) hc = quotient(at, w.total), hc_units = hc * w.total;
+      long long rest = at - hc_units - w.start;
+      if (rest < 0 || rest >= w.mine) continue;
       for (int b = w.b0; b < w.b1; ++b) {
         const Request r = request_of(a, b, both, tile);
         const long long units = r.units(), here = r.row_tiles(tokens) * units;
         if (rest < here) {
           const int rt = (int)quotient(rest, units);
-          *found = {hc, b, rt, (int)(rest - rt * units), min(run, all - at)};
+          found[i] = {(int)hc, b, rt, (int)(rest - rt * units), min(run, all - at)};
           break;
         }
         rest -= here;
@@ -327,7 +318,6 @@ __device__ __forceinline__ Cursor find_run(const PrefixArgs& a, const OwnWork& w
     }
   }
   __syncthreads();
-  return *found;
 }
 
 // Prefixes and own tokens are worked on side by side, by two launches: of `sms` SMs this many have the prefixes.  A tile of a

@@ -1,0 +1,397 @@
+// Requests' own tokens (with their prefixes where nobody else reads those) on mma.sync, a warp by itself: few rows, many keys
+// that are read once (see shared_prefix.cuh for how the work is divided).
+//
+// S^T = K q^T and O^T = V^T P^T: keys, then channels, are the instruction's 16 rows and up to 8 rows of q its columns, NG times.
+// A warp has a ring of its own, fills it itself and waits for nobody, so that whatever one of them waits for (a request's
+// numbers, its pages, its rows of q) the others' copies are under way.  A tile within its sequence comes by TMA where that
+// serves the pages, a box of a page and 64 channels; the last of a sequence comes by cp.async, which leaves zeros behind its
+// end: what lies there may be anything.
+#pragma once
+#include "shared_prefix.cuh"
+
+namespace gf {
+namespace {
+namespace own {
+
+constexpr int KEYS = HD <= 64 ? 32 : 16;         // of a tile
+constexpr int WARPS = HD <= 128 ? 8 : 4, STAGES = 3;
+constexpr int THREADS = 32 * WARPS;
+constexpr int KCH = HD / 16;
+// A plane of a tile: head sizes that are a multiple of 64 as TMA's 128-byte swizzle leaves them (64 channels of the keys, then the
+// next 64), others in rows of an odd number of 16-byte chunks.
+constexpr bool SWIZZLED = HD % 64 == 0;
+constexpr int HALVES = SWIZZLED ? HD / 64 : 1, PADDED = HD + 8;
+constexpr uint32_t PLANE = SWIZZLED ? KEYS * HD * 2 : (KEYS * PADDED * 2 + 127) / 128 * 128, STAGE = 2 * PLANE;
+constexpr uint32_t RING = WARPS * STAGES * STAGE;
+__device__ __forceinline__ uint32_t place(int key, int ch) {       // byte offset of 8 channels of a key
+  if constexpr (SWIZZLED)
+    return (uint32_t)(ch >> 6) * (KEYS * 128) + (uint32_t)key * 128u + (uint32_t)((((ch >> 3) & 7) ^ (key & 7)) << 4);
+  else
+    return (uint32_t)key * (PADDED * 2) + (uint32_t)ch * 2u;
+}
+// (joining warps inside a block takes the ring's memory, and what it has not)
+__host__ __device__ constexpr uint32_t smem_bytes(int ng) {
+  const uint32_t exchange = WARPS * 8 * ng * (HD + 2) * 4;
+  return (RING > exchange ? RING : exchange) + WARPS * STAGES * 8 + 1024;
+}
+// Groups of 8 rows at most: their results and their q have to fit the registers.
+constexpr int MOST_GROUPS = HD <= 128 ? 4 : 2;
+
+struct Args {
+  PrefixArgs a;
+  int both, tma;               // both: prefixes, too
+  int joined;                  // another kernel adds a row's pieces up; else a block's warps have an item, and it is written here
+  int after;                   // the launch runs beside the one before it, whose results the joining kernel reads, too
+  Shape shape;
+  int H, rows;                 // kv heads * chunks; rows of a tile
+  int sms;
+  Shape far_shape;             // of the prefixes' kernel beside this one
+  int far_tile, far_H;
+  float far_cost;              // what a tile of a prefix costs, in tiles of this kernel
+  OwnPlan* plan;
+  float* cut_o;                // [warps][2][rows][HD]: pieces of cut items
+  float2* cut_ml;
+  float* row_o;                // [T][nh][HD]: of whole items, where a prefix is to be joined
+  float2* row_ml;
+  int* err;
+};
+
+// A part of an item: tiles [from, from + count) of its prefix's tiles, then its own tokens'.
+struct Piece {
+  int first, tokens, hc, from, count, far, far_len, near_len;
+  int last;                    // the last own token that the first token sees; the next one sees one more
+  const int *far_table, *near_table;
+  int to;
+  size_t at;                   // CUT: the place
+};
+enum { FINAL, ROW, CUT };
+struct Keys {
+  const int* table;
+  int key0, end;
+};
+__device__ __forceinline__ Keys keys_of(const Piece& x, int tile) {
+  if (tile < x.far) return {x.far_table, tile * KEYS, x.far_len};
+  return {x.near_table, (tile - x.far) * KEYS, x.near_len};
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+  return d;
+}
+
+template <int NG>
+__global__ void __launch_bounds__(THREADS, 1)
+prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const Args p) {
+  extern __shared__ __align__(1024) unsigned char raw[];
+  unsigned char* base = raw + ((0u - smem_u32(raw)) & 1023u);               // (a swizzle counts from 1 KB)
+  __shared__ long long counts[4];
+  __shared__ Cursor found[WARPS];
+  __shared__ int far_s;
+  const PrefixArgs& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  unsigned char* ring = base + warp * (STAGES * STAGE);
+  uint64_t* full = reinterpret_cast<uint64_t*>(base + smem_bytes(NG) - 1024 - WARPS * STAGES * 8) + warp * STAGES;
+  if (lane == 0) {
+    for (int i = 0; i < STAGES; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&full[i])), "r"(32));
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (!p.after) pdl_wait();
+  Cursor cur{};
+  Request req{};
+  if (p.joined) {
+    // this block's warps' runs
+    GroupTiles gt{};
+    FarWork f{};
+    if (p.after && warp == WARPS - 1) f = far_work(a, gt, p.far_H, p.far_shape.tokens, p.far_tile);
+    const OwnWork w = own_work<128>(a, p.shape.tokens, KEYS, p.both, counts);
+    if (threadIdx.x == THREADS - 1) far_s = p.after ? far_share(p.sms, f.units, p.far_cost, w.total * p.H) : 0;
+    __syncthreads();
+    const int blocks = p.after ? max(p.sms - far_s, 1) : (int)gridDim.x;
+    find_runs<128, WARPS>(a, w, p.H, p.shape.tokens, KEYS, p.both, blockIdx.x, blocks, blockIdx.x == 0 ? p.plan : nullptr, found);
+    cur = found[warp];
+    if (cur.todo > 0) req = request_of(a, cur.b, p.both, KEYS);
+  } else {
+    cur = {(int)blockIdx.z, (int)blockIdx.y, (int)blockIdx.x, 0, 0};
+    req = request_of(a, cur.b, p.both, KEYS);
+    __syncthreads();
+  }
+  const int each = a.nh / a.nkv;
+  const float scale_log2 = a.scale * LOG2E;
+  const int box = min(a.page, KEYS), boxes = KEYS / box;
+  const bool tma = SWIZZLED && p.tma;
+  uint32_t phases = 0;         // a bit a stage
+  int st = 0;
+  bool ok = true;
+  // the next piece of this warp's run (or its share of the block's item)
+  auto next = [&](Piece& x) {
+    auto set = [&](int from, int count) {
+      const int done = cur.rt * p.shape.tokens;
+      x.first = req.first + done, x.tokens = min(p.shape.tokens, req.count - done), x.hc = cur.hc;
+      x.from = from, x.count = count;
+      x.far = req.far, x.far_len = req.shared, x.near_len = req.len, x.last = req.len - req.count + done;
+      x.far_table = a.prefix_table + (size_t)max(req.g, 0) * a.prefix_stride;
+      x.near_table = a.table + (size_t)cur.b * a.table_stride;
+    };
+    if (!p.joined) {
+      if (cur.rt * p.shape.tokens >= req.count) return false;
+      const int tiles = req.far + req.near, w0 = tiles * warp / WARPS, w1 = tiles * (warp + 1) / WARPS;
+      set(w0, w1 - w0);
+      x.to = FINAL;
+      cur.rt += gridDim.x;
+      return true;
+    }
+    while (cur.todo > 0) {
+      const int tiles = req.tiles(), units = req.units(), from = cur.off;
+      const int count = (int)min(cur.todo, (long long)(units - from));
+      const bool some = from < tiles;              // (else only the item's end, which costs time and has no tiles)
+      if (some) {
+        set(from, min(count, tiles - from));
+        const bool starts = from == 0, ends = from + x.count == tiles;
+        x.to = starts && ends ? (p.both ? FINAL : ROW) : CUT;
+        x.at = ((size_t)blockIdx.x * WARPS + warp) * 2 + (starts ? 1 : 0);
+        if (req.far + req.near == 0) x.count = 0;  // (an item without a key)
+      }
+      cur.todo -= count, cur.off = 0;
+      if (cur.todo > 0 && ++cur.rt >= req.row_tiles(p.shape.tokens)) {
+        cur.rt = 0;
+        do {
+          if (++cur.b == a.B) cur.b = 0, ++cur.hc;
+          req = request_of(a, cur.b, p.both, KEYS);
+        } while (req.count == 0);
+      }
+      if (some) return true;
+    }
+    return false;
+  };
+  Piece x;
+  while (next(x)) {
+    const int kvh = x.hc / p.shape.chunks, part = x.hc - kvh * p.shape.chunks;
+    const int h0 = kvh * each + part * p.shape.heads, heads = min(p.shape.heads, each - part * p.shape.heads);
+    const int rows = x.tokens * heads;
+    // ---- copies: a tile's places are looked up one tile ahead
+    auto look = [&](int i) {
+      const Keys k = keys_of(x, x.from + i);
+      return slot_of(a, k.table, min(k.key0 + (lane & (KEYS - 1)), k.end - 1));
+    };
+    auto issue = [&](int i, int slot, int stage_i) {
+      const Keys k = keys_of(x, x.from + i);
+      unsigned char* stage = ring + stage_i * STAGE;
+      uint64_t* bar = &full[stage_i];
+      if (tma && k.key0 + KEYS <= k.end) {
+        // (what this warp's cp.async wrote there is out of the way of the copies)
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        if (lane == 0)
+          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(STAGE) : "memory");
+        else
+          asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+        __syncwarp();
+        const int bx = lane % boxes, half = lane / boxes % HALVES, plane = lane / (boxes * HALVES);
+        const int row = __shfl_sync(0xffffffffu, slot, bx * box);
+        if (plane < 2)
+          tma_load_2d(stage + plane * PLANE + half * (KEYS * 128) + bx * box * 128, plane ? &vmap : &kmap, bar, kvh * HD + half * 64, row);
+      } else {
+        constexpr int CH = HD / 8;
+        const bf16* kp = static_cast<const bf16*>(a.k) + (size_t)kvh * HD;
+        const bf16* vp = static_cast<const bf16*>(a.v) + (size_t)kvh * HD;
+#pragma unroll 2
+        for (int j = 0; j < KEYS * CH / 32; ++j) {
+          const int idx = j * 32 + lane, row = idx / CH, ch = (idx - row * CH) * 8;
+          const size_t off = (size_t)__shfl_sync(0xffffffffu, slot, row) * (a.nkv * HD) + ch;
+          const bool there = k.key0 + row < k.end;
+          cp_async16(stage + place(row, ch), kp + off, there);
+          cp_async16(stage + PLANE + place(row, ch), vp + off, there);
+        }
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+      }
+    };
+    int slot = 0;
+    if (!ok) x.count = 0;      // (behind a wait that ran out: the warps still meet where they join)
+    for (int i = 0; i < min(STAGES, x.count); ++i) issue(i, look(i), (st + i) % STAGES);
+    if (STAGES < x.count) slot = look(STAGES);
+    // ---- q as the 8-column operand: thread (g, t) has channels 16 kc + 2t, + 1 and + 8, + 9 of row 8 ng + g
+    uint32_t qf[NG][KCH][2];
+    int see[NG][2];            // the last own token that rows 2t and 2t + 1 see (rows that are none see all, and nobody sees them)
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+      const int r = 8 * n + g, token = r < rows ? r / heads : 0, head = r < rows ? r - token * heads : 0;
+      const bf16* q = static_cast<const bf16*>(a.q) + (size_t)(x.first + token) * a.q_stride + (size_t)(h0 + head) * HD + 2 * t;
+#pragma unroll
+      for (int kc = 0; kc < KCH; ++kc) {
+        qf[n][kc][0] = r < rows ? __ldcg(reinterpret_cast<const unsigned*>(q + kc * 16)) : 0u;
+        qf[n][kc][1] = r < rows ? __ldcg(reinterpret_cast<const unsigned*>(q + kc * 16 + 8)) : 0u;
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) see[n][e] = 8 * n + 2 * t + e < rows ? x.last + (8 * n + 2 * t + e) / heads : 0x7fffffff;
+    }
+    float o[NG][HD / 16][4], m[NG][2], l[NG][2];
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+      m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < HD / 16; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+    }
+    // ---- tiles
+    for (int i = 0; i < x.count && ok; ++i) {
+      const Keys k = keys_of(x, x.from + i);
+      const bool far = x.from + i < x.far;
+      ok = wait_bar(&full[st], (phases >> st) & 1u, p.err, 22);
+      if (!ok) break;
+      phases ^= 1u << st;
+      const unsigned char* stage = ring + st * STAGE;
+      // what all rows see needs no comparison: the first token's sight, the sequence's end
+      const bool masked = k.key0 + KEYS > k.end || (!far && k.key0 + KEYS - 1 > x.last);
+#pragma unroll
+      for (int sub = 0; sub < KEYS / 16; ++sub) {
+        float s[NG][4];
+#pragma unroll
+        for (int n = 0; n < NG; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+        for (int kc = 0; kc < KCH; ++kc) {
+          uint32_t af[4];
+          ldsm_x4(af, stage + place(sub * 16 + (lane & 15), kc * 16 + (lane >> 4) * 8));
+#pragma unroll
+          for (int n = 0; n < NG; ++n) mma16816(s[n], af, qf[n][kc][0], qf[n][kc][1]);
+        }
+        uint32_t b0[NG], b1[NG];
+        bool grew = false;
+        float corr[NG][2];
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+          const int ka = k.key0 + sub * 16 + g, kb = ka + 8;
+          float mx[2], base_m[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            s[n][e] *= scale_log2, s[n][2 + e] *= scale_log2;
+            if (masked) {
+              const int end = far ? k.end - 1 : min(see[n][e], k.end - 1);
+              if (ka > end) s[n][e] = -INFINITY;
+              if (kb > end) s[n][2 + e] = -INFINITY;
+            }
+            mx[e] = fmaxf(s[n][e], s[n][2 + e]);
+          }
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], d));
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float top = fmaxf(m[n][e], mx[e]);
+            base_m[e] = top == -INFINITY ? 0.f : top;      // (keeps -inf - -inf out of the exponent)
+            corr[n][e] = fast_exp2(m[n][e] - base_m[e]);
+            grew |= corr[n][e] != 1.f;
+            m[n][e] = top;
+          }
+          const float p0 = fast_exp2(s[n][0] - base_m[0]), p1 = fast_exp2(s[n][1] - base_m[1]);
+          const float p2 = fast_exp2(s[n][2] - base_m[0]), p3 = fast_exp2(s[n][3] - base_m[1]);
+          l[n][0] = l[n][0] * corr[n][0] + (p0 + p2);
+          l[n][1] = l[n][1] * corr[n][1] + (p1 + p3);
+          // (weights are rounded to bfloat16 for the product, as everywhere in this package; their sum is not)
+          b0[n] = transposed(pack_bf16(p0, p1));
+          b1[n] = transposed(pack_bf16(p2, p3));
+        }
+        if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+          for (int n = 0; n < NG; ++n)
+#pragma unroll
+            for (int c = 0; c < HD / 16; ++c)
+              o[n][c][0] *= corr[n][0], o[n][c][1] *= corr[n][1], o[n][c][2] *= corr[n][0], o[n][c][3] *= corr[n][1];
+        }
+#pragma unroll
+        for (int c = 0; c < HD / 16; ++c) {
+          uint32_t af[4];
+          ldsm_x4_t(af, stage + PLANE + place(sub * 16 + (lane >> 4) * 8 + (lane & 7), c * 16 + ((lane >> 3) & 1) * 8));
+#pragma unroll
+          for (int n = 0; n < NG; ++n) mma16816(o[n][c], af, b0[n], b1[n]);
+        }
+      }
+      __syncwarp();
+      if (i + STAGES < x.count) {
+        issue(i + STAGES, slot, st);
+        if (i + STAGES + 1 < x.count) slot = look(i + STAGES + 1);
+      }
+      st = st + 1 == STAGES ? 0 : st + 1;
+    }
+    // ---- the rows' results
+#pragma unroll
+    for (int n = 0; n < NG; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], d);
+    if (!p.joined) {
+      // the block's warps have parts of the same item
+      __syncthreads();
+      float* so = reinterpret_cast<float*>(base);                            // [WARPS][rows][HD], then (maximum, sum)
+      float2* sml = reinterpret_cast<float2*>(so + WARPS * rows * HD);
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = 8 * n + 2 * t + e;
+          if (r >= rows) continue;
+          float* to = so + (warp * rows + r) * HD + g;
+#pragma unroll
+          for (int c = 0; c < HD / 16; ++c) to[c * 16] = o[n][c][e], to[c * 16 + 8] = o[n][c][2 + e];
+          if (g == 0) sml[warp * rows + r] = make_float2(m[n][e], l[n][e]);
+        }
+      __syncthreads();
+      for (int i = threadIdx.x; i < rows * (HD / 4); i += THREADS) {
+        const int r = i / (HD / 4), ch = (i - r * (HD / 4)) * 4, token = r / heads, head = r - token * heads;
+        float top = -INFINITY, sum = 0.f, y[4] = {};
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) top = fmaxf(top, sml[w * rows + r].x);
+        const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+          const float2 ml = sml[w * rows + r];
+          const float f = fast_exp2(ml.x - ref);
+          const float4 v = *reinterpret_cast<const float4*>(so + (w * rows + r) * HD + ch);
+          sum += ml.y * f;
+          y[0] += v.x * f, y[1] += v.y * f, y[2] += v.z * f, y[3] += v.w * f;
+        }
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;                      // (no key: zeros)
+        const float z[4] = {y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv};
+        if (ok) Quad<bf16>::store(static_cast<bf16*>(a.out) + ((size_t)(x.first + token) * a.nh + h0 + head) * HD + ch, z);
+      }
+      __syncthreads();           // (the ring lies there again)
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      continue;
+    }
+    if (!ok) continue;
+#pragma unroll
+    for (int n = 0; n < NG; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = 8 * n + 2 * t + e;
+        if (r >= rows) continue;
+        const int token = r / heads;
+        const size_t row = (size_t)(x.first + token) * a.nh + h0 + r - token * heads;
+        if (x.to == FINAL) {
+          const float inv = l[n][e] == 0.f ? 0.f : 1.f / l[n][e];
+          bf16* to = static_cast<bf16*>(a.out) + row * HD + g;
+#pragma unroll
+          for (int c = 0; c < HD / 16; ++c)
+            to[c * 16] = __float2bfloat16_rn(o[n][c][e] * inv), to[c * 16 + 8] = __float2bfloat16_rn(o[n][c][2 + e] * inv);
+        } else {
+          const size_t at = x.to == ROW ? row : x.at * p.rows + r;
+          float* to = (x.to == ROW ? p.row_o : p.cut_o) + at * HD + g;
+#pragma unroll
+          for (int c = 0; c < HD / 16; ++c) to[c * 16] = o[n][c][e], to[c * 16 + 8] = o[n][c][2 + e];
+          if (g == 0) (x.to == ROW ? p.row_ml : p.cut_ml)[at] = make_float2(m[n][e], l[n][e]);
+        }
+      }
+  }
+  // (a wait that ran out: nothing may still be on its way into this warp's memory when the block ends)
+  if (!ok)
+    for (int i = 0; i < STAGES; ++i) wait_bar(&full[i], (phases >> i) & 1u, p.err, 23);
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  if (p.joined) {
+    pdl_trigger();
+    // the joining kernel waits for this launch alone: its last block ends behind the one that ran beside it
+    if (p.after && blockIdx.x == gridDim.x - 1) pdl_wait();
+  }
+}
+
+}  // namespace own
+}  // namespace
+}  // namespace gf

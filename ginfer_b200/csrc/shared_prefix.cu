@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) prefix_join_kernel(const Join
   pdl_trigger();
   pdl_wait();
   const bool both = p.both;
-  const Request r = request_of(a, b, both, own::KEYS);
+  const Request r = request_of(a, b, both, own::Tile<T>::KEYS);
   if (r.count == 0) return;
   // where its prefix's pieces are
   int splits = 0, far_mt = 0, far_first = 0;
@@ -500,67 +500,6 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) prefix_join_kernel(const Join
   }
 }
 
-// ------------------------------------------------------------------------------------- 32 bits
-constexpr int kWarps = 4, kMostChannels = 256 / 32;
-
-template <typename T>
-__global__ void __launch_bounds__(32 * kWarps) prefix_simple_kernel(const PrefixArgs a) {
-  __shared__ float part[kWarps][256], part_m[kWarps], part_l[kWarps];
-  const int b = blockIdx.x, h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int kvh = h / (a.nh / a.nkv);
-  pdl_trigger();
-  pdl_wait();
-  const Rows rows = rows_of(a, b);
-  const int g = group_of(a, b), shared = prefix_length(a, g), len = own_length(a, b);
-  const T* k = static_cast<const T*>(a.k);
-  const T* v = static_cast<const T*>(a.v);
-  for (int i = 0; i < rows.count; ++i) {
-    const size_t row = rows.first + i;
-    const T* q = static_cast<const T*>(a.q) + row * a.q_stride + (size_t)h * a.hd;
-    float x[kMostChannels], o[kMostChannels], m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int j = 0; j < kMostChannels; ++j) {
-      x[j] = 32 * j + lane < a.hd ? to_f32(q[32 * j + lane]) * a.scale : 0.f;
-      o[j] = 0.f;
-    }
-    const int keys = shared + max(len - rows.count + i + 1, 0);
-    for (int c = warp; c < keys; c += kWarps) {
-      const int* tbl = c < shared ? a.prefix_table + (size_t)g * a.prefix_stride : a.table + (size_t)b * a.table_stride;
-      const int at = c < shared ? c : c - shared;
-      const size_t slot = (size_t)page_in(a, fresh_index(tbl + at / a.page)) * a.page + at % a.page;
-      const size_t off = (slot * a.nkv + kvh) * a.hd;
-      float s = 0.f;
-#pragma unroll
-      for (int j = 0; j < kMostChannels; ++j)
-        if (32 * j + lane < a.hd) s = fmaf(x[j], to_f32(k[off + 32 * j + lane]), s);
-      s = warp_sum(s);
-      const float top = fmaxf(m, s), base = top == -INFINITY ? 0.f : top;
-      const float w = expf(s - base), keep = expf(m - base);
-      m = top;
-      l = l * keep + w;
-#pragma unroll
-      for (int j = 0; j < kMostChannels; ++j)
-        if (32 * j + lane < a.hd) o[j] = o[j] * keep + w * to_f32(v[off + 32 * j + lane]);
-    }
-    __syncthreads();
-    if (lane == 0) part_m[warp] = m, part_l[warp] = l;
-#pragma unroll
-    for (int j = 0; j < kMostChannels; ++j)
-      if (32 * j + lane < a.hd) part[warp][32 * j + lane] = o[j];
-    __syncthreads();
-    float top = -INFINITY, sum = 0.f;
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, part_m[w]);
-    const float base = top == -INFINITY ? 0.f : top;
-    for (int w = 0; w < kWarps; ++w) sum += part_l[w] * expf(part_m[w] - base);
-    T* out = static_cast<T*>(a.out) + (row * a.nh + h) * a.hd;
-    for (int d = threadIdx.x; d < a.hd; d += 32 * kWarps) {
-      float y = 0.f;
-      for (int w = 0; w < kWarps; ++w) y += part[w][d] * expf(part_m[w] - base);
-      out[d] = from_f32<T>(keys > 0 ? y / sum : 0.f);
-    }
-  }
-}
-
 // ------------------------------------------------------------------------------------- host side
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                   const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -650,8 +589,11 @@ struct Call {
     a.page_shift = (a.page & (a.page - 1)) == 0 ? 31 - __builtin_clz(a.page) : -1;
     if (longest < 1) longest = 1;
     // groups of 8 rows: as many as a request has, or the registers hold
+    const bool half = type == GF_BF16;
+    const int most = half ? own::kMostGroups<bf16> : own::kMostGroups<float>;
     const long long wanted = (long long)longest * (a.nh / a.nkv);
-    groups = wanted <= 8 ? 1 : wanted <= 16 || own::MOST_GROUPS == 2 ? 2 : 4;
+    groups = wanted <= 8 || most == 1 ? 1 : wanted <= 16 || most == 2 ? 2 : 4;
+    const int keys = half ? own::Tile<bf16>::KEYS : own::Tile<float>::KEYS, warps = half ? own::Tile<bf16>::WARPS : own::Tile<float>::WARPS;
     p.rows = 8 * groups;
     p.shape = row_shape_of(a.nh, a.nkv, p.rows);
     p.H = a.nkv * p.shape.chunks;
@@ -668,23 +610,23 @@ struct Call {
       return here;
     };
     if (direct) return;
-    const long long rows = (long long)a.T * a.nh, cut = (long long)p.sms * own::WARPS * 2 * p.rows;
+    const long long rows = (long long)a.T * a.nh, cut = (long long)p.sms * warps * 2 * p.rows;
     p.plan = (OwnPlan*)take(16 + 8ll * a.B);
     p.cut_o = (float*)take(cut * HD * 4), p.cut_ml = (float2*)take(cut * 8);
     if (!shared) return;
-    tensor = GF_PREFIX_TC && a.page % 8 == 0 && 128 % a.page == 0;
+    tensor = GF_PREFIX_TC && half && a.page % 8 == 0 && 128 % a.page == 0;
     p.row_o = (float*)take(rows * HD * 4), p.row_ml = (float2*)take(rows * 8);
-    j.far_rows = tensor ? 128 : MOST_ROWS;
-    p.far_shape = row_shape_of(a.nh, a.nkv, j.far_rows), p.far_tile = tensor ? 128 : TILE, p.far_H = a.nkv * p.far_shape.chunks;
-    p.far_cost = getenv("GF_COST") ? (float)atof(getenv("GF_COST")) : tensor ? kTensorCost : kPlainCost;
+    j.far_rows = tensor ? 128 : half ? MOST_ROWS : 8 * most;
+    p.far_shape = row_shape_of(a.nh, a.nkv, j.far_rows), p.far_tile = tensor ? 128 : half ? TILE : keys, p.far_H = a.nkv * p.far_shape.chunks;
+    p.far_cost = getenv("GF_COST") ? (float)atof(getenv("GF_COST")) : tensor ? kTensorCost : half ? kPlainCost : 1.f;
     const long long tiles = (long long)p.far_H * ((a.T + p.far_shape.tokens - 1) / p.far_shape.tokens + a.G);
-    const long long least = 2ll * p.sms * (tensor ? 1 : BLOCKS_AN_SM);
+    const long long least = 2ll * p.sms * (tensor ? 1 : half ? BLOCKS_AN_SM : warps);
     j.places = (int)(tiles > least ? tiles : least);
     int* chunk = (int*)take(4);
     float* far_o = (float*)take((long long)j.places * j.far_rows * HD * 4);
     float2* far_ml = (float2*)take((long long)j.places * j.far_rows * 8);
     j.chunk = chunk, j.far_o = far_o, j.far_ml = far_ml;
-    f = FarArgs{a, 0, p.far_shape, p.shape, p.far_H, p.H, j.places, p.sms, own::KEYS, p.far_cost, chunk, far_o, far_ml, p.err};
+    f = FarArgs{a, 0, p.far_shape, p.shape, p.far_H, p.H, j.places, p.sms, keys, p.far_cost, chunk, far_o, far_ml, p.err};
   }
 };
 
@@ -694,14 +636,22 @@ GF_EXPORT long long gf_prefix_scratch(const char* words) { return Call(words).ne
 // What gf_prefix_attend returns when it launched one kernel or two; 0: three.
 constexpr int kOneLaunch = -101, kTwoLaunches = -102;
 
-template <int NG>
-static int launch_own(const Call& c, const CUtensorMap& mk, const CUtensorMap& mv, dim3 grid) {
+template <typename T, int NG, bool FAR>
+static int launch_own(const own::Args& p, const CUtensorMap& mk, const CUtensorMap& mv, dim3 grid, cudaStream_t stream) {
   static OncePerDevice attrs;
   if (int rc = attrs.run([&] {
-        return cudaFuncSetAttribute(own::prefix_own_kernel<NG>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)own::smem_bytes(NG));
+        return cudaFuncSetAttribute(own::prefix_own_kernel<T, NG, FAR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    (int)own::smem_bytes<T>(NG));
       }))
     return rc;
-  return launch_kernel(own::prefix_own_kernel<NG>, grid, dim3(own::THREADS), own::smem_bytes(NG), c.stream, mk, mv, c.p);
+  return launch_kernel(own::prefix_own_kernel<T, NG, FAR>, grid, dim3(32 * own::Tile<T>::WARPS), own::smem_bytes<T>(NG), stream, mk, mv, p);
+}
+template <typename T>
+static int launch_near(const Call& c, const CUtensorMap& mk, const CUtensorMap& mv, dim3 grid) {
+  constexpr int most = own::kMostGroups<T>;
+  if (c.groups == 1) return launch_own<T, 1, false>(c.p, mk, mv, grid, c.stream);
+  if (c.groups == 2) return launch_own<T, most < 2 ? most : 2, false>(c.p, mk, mv, grid, c.stream);
+  return launch_own<T, most, false>(c.p, mk, mv, grid, c.stream);
 }
 
 GF_EXPORT int gf_prefix_attend(const char* words) {
@@ -709,10 +659,7 @@ GF_EXPORT int gf_prefix_attend(const char* words) {
   own::Args& p = c.p;
   PrefixArgs& a = p.a;
   if (a.B <= 0 || a.T <= 0) return 0;
-  if (c.type != GF_BF16) {
-    const int rc = launch_kernel(prefix_simple_kernel<float>, dim3(a.B, a.nh), dim3(32 * kWarps), 0, c.stream, a);
-    return rc ? rc : kOneLaunch;
-  }
+  const bool half = c.type == GF_BF16;
   if (c.need > c.room) return -5;
   // tensor maps: a box is a page's rows of a tile
   auto maps = [&](CUtensorMap& k, CUtensorMap& v, int tile) {
@@ -721,8 +668,8 @@ GF_EXPORT int gf_prefix_attend(const char* words) {
   };
   auto serves = [&](int tile) { return a.page % 8 == 0 && (tile % a.page == 0 || a.page % tile == 0); };
   CUtensorMap ok{}, ov{};
-  p.tma = own::SWIZZLED && serves(own::KEYS);
-  if (p.tma && !maps(ok, ov, own::KEYS)) return -7;
+  p.tma = half && own::Tile<bf16>::SWIZZLED && serves(own::Tile<bf16>::KEYS);
+  if (p.tma && !maps(ok, ov, own::Tile<bf16>::KEYS)) return -7;
   if (c.shared) {
     int rc;
 #if GF_PREFIX_TC
@@ -740,7 +687,12 @@ GF_EXPORT int gf_prefix_attend(const char* words) {
       rc = launch_kernel(tc::prefix_tc_kernel, dim3(p.sms), dim3(tc::NTHREADS_TC), tc::SMEM, c.stream, tq, tk, tv, t);
     } else
 #endif
-    {
+    if (!half) {
+      own::Args f = p;
+      f.shape = p.far_shape, f.H = p.far_H, f.rows = c.j.far_rows, f.own_shape = p.shape, f.own_H = p.H;
+      f.places = c.j.places, f.chunk = c.f.chunk, f.far_o = c.f.far_o, f.far_ml = c.f.far_ml, f.after = 0;
+      rc = launch_own<float, own::kMostGroups<float>, true>(f, ok, ov, dim3(p.sms), c.stream);
+    } else {
       static OncePerDevice attrs;
       rc = attrs.run([&] {
         return cudaFuncSetAttribute(prefix_pieces_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PIECES_SMEM);
@@ -755,13 +707,13 @@ GF_EXPORT int gf_prefix_attend(const char* words) {
   }
   const int row_tiles = (c.longest + p.shape.tokens - 1) / p.shape.tokens;
   const dim3 grid = c.direct ? dim3(row_tiles, a.B, p.H) : dim3(p.sms);
-  int rc = c.groups == 1 ? launch_own<1>(c, ok, ov, grid) : c.groups == 2 ? launch_own<2>(c, ok, ov, grid)
-                                                          : launch_own<own::MOST_GROUPS>(c, ok, ov, grid);
+  int rc = half ? launch_near<bf16>(c, ok, ov, grid) : launch_near<float>(c, ok, ov, grid);
   if (rc || c.direct) return rc ? rc : kOneLaunch;
   c.j.p = p;
   // (a warp a row where the requests have as many as is said)
   const long long per = (long long)c.longest * (a.nh / a.nkv);
   const unsigned z = (unsigned)(per > 64 * JOIN_WARPS ? 64 : (per + JOIN_WARPS - 1) / JOIN_WARPS);
-  rc = launch_kernel(prefix_join_kernel<bf16>, dim3(a.B, a.nkv, z), dim3(32 * JOIN_WARPS), 0, c.stream, c.j);
+  rc = launch_kernel(half ? prefix_join_kernel<bf16> : prefix_join_kernel<float>, dim3(a.B, a.nkv, z), dim3(32 * JOIN_WARPS), 0, c.stream,
+                     c.j);
   return rc ? rc : c.shared ? 0 : kTwoLaunches;
 }

@@ -1,11 +1,14 @@
-// Requests' own tokens (with their prefixes where nobody else reads those) on mma.sync, a warp by itself: few rows, many keys
-// that are read once (see shared_prefix.cuh for how the work is divided).
+// Requests' own tokens (with their prefixes where nobody else reads those), and in 32 bits the groups' prefixes, too, on mma.sync, a
+// warp by itself: few rows, many keys that are read once (see shared_prefix.cuh for how the work is divided).
 //
 // S^T = K q^T and O^T = V^T P^T: keys, then channels, are the instruction's 16 rows and up to 8 rows of q its columns, NG times.
 // A warp has a ring of its own, fills it itself and waits for nobody, so that whatever one of them waits for (a request's
 // numbers, its pages, its rows of q) the others' copies are under way.  A tile within its sequence comes by TMA where that
 // serves the pages, a box of a page and 64 channels; the last of a sequence comes by cp.async, which leaves zeros behind its
 // end: what lies there may be anything.
+//
+// In 32 bits both factors of a product are the sum of two tf32 numbers, 22 bits, and a product three of theirs (what is left out
+// is 2^-22 of it); sums are 32-bit.
 #pragma once
 #include "shared_prefix.cuh"
 
@@ -13,29 +16,40 @@ namespace gf {
 namespace {
 namespace own {
 
-constexpr int KEYS = HD <= 64 ? 32 : 16;         // of a tile
-constexpr int WARPS = HD <= 128 ? 8 : 4, STAGES = 3;
-constexpr int THREADS = 32 * WARPS;
+// A tile of KEYS keys in shared memory, keys, then values.  bfloat16: head sizes that are a multiple of 64 as TMA's 128-byte swizzle
+// leaves them (64 channels of the keys, then the next 64), others in rows of an odd number of 16-byte chunks.  32 bits: rows 4
+// (keys) and 8 (values) banks apart, so that a warp's reads of 8 keys and 4 channels, or of 4 keys and 8 channels, meet every bank once.
+template <typename T> struct Tile;
+template <> struct Tile<bf16> {
+  static constexpr int KEYS = HD <= 64 ? 32 : 16, WARPS = HD <= 128 ? 8 : 4, STAGES = 3;
+  static constexpr bool SWIZZLED = HD % 64 == 0;
+  static constexpr int HALVES = SWIZZLED ? HD / 64 : 1, PADDED = HD + 8, CHUNK = 8;
+  static constexpr uint32_t PLANE = SWIZZLED ? KEYS * HD * 2 : (KEYS * PADDED * 2 + 127) / 128 * 128, STAGE = 2 * PLANE;
+  static __device__ __forceinline__ uint32_t place(int plane, int key, int ch) {       // byte offset of CHUNK channels of a key
+    if constexpr (SWIZZLED)
+      return plane * PLANE + (uint32_t)(ch >> 6) * (KEYS * 128) + (uint32_t)key * 128u + (uint32_t)((((ch >> 3) & 7) ^ (key & 7)) << 4);
+    else
+      return plane * PLANE + (uint32_t)key * (PADDED * 2) + (uint32_t)ch * 2u;
+  }
+};
+template <> struct Tile<float> {
+  static constexpr int KEYS = 16, WARPS = HD <= 64 ? 8 : HD <= 128 ? 4 : 2, STAGES = 3;
+  static constexpr bool SWIZZLED = false;
+  static constexpr int HALVES = 1, CHUNK = 4;
+  static constexpr uint32_t PLANE = KEYS * (HD + 4) * 4, STAGE = PLANE + KEYS * (HD + 8) * 4;
+  static __device__ __forceinline__ uint32_t place(int plane, int key, int ch) {
+    return plane * PLANE + (uint32_t)(key * (HD + 4 + 4 * plane) + ch) * 4u;
+  }
+};
 constexpr int KCH = HD / 16;
-// A plane of a tile: head sizes that are a multiple of 64 as TMA's 128-byte swizzle leaves them (64 channels of the keys, then the
-// next 64), others in rows of an odd number of 16-byte chunks.
-constexpr bool SWIZZLED = HD % 64 == 0;
-constexpr int HALVES = SWIZZLED ? HD / 64 : 1, PADDED = HD + 8;
-constexpr uint32_t PLANE = SWIZZLED ? KEYS * HD * 2 : (KEYS * PADDED * 2 + 127) / 128 * 128, STAGE = 2 * PLANE;
-constexpr uint32_t RING = WARPS * STAGES * STAGE;
-__device__ __forceinline__ uint32_t place(int key, int ch) {       // byte offset of 8 channels of a key
-  if constexpr (SWIZZLED)
-    return (uint32_t)(ch >> 6) * (KEYS * 128) + (uint32_t)key * 128u + (uint32_t)((((ch >> 3) & 7) ^ (key & 7)) << 4);
-  else
-    return (uint32_t)key * (PADDED * 2) + (uint32_t)ch * 2u;
-}
 // (joining warps inside a block takes the ring's memory, and what it has not)
-__host__ __device__ constexpr uint32_t smem_bytes(int ng) {
-  const uint32_t exchange = WARPS * 8 * ng * (HD + 2) * 4;
-  return (RING > exchange ? RING : exchange) + WARPS * STAGES * 8 + 1024;
+template <typename T> __host__ __device__ constexpr uint32_t smem_bytes(int ng) {
+  using G = Tile<T>;
+  const uint32_t ring = G::WARPS * G::STAGES * G::STAGE, exchange = G::WARPS * 8 * ng * (HD + 2) * 4;
+  return (ring > exchange ? ring : exchange) + G::WARPS * G::STAGES * 8 + 1024;
 }
 // Groups of 8 rows at most: their results and their q have to fit the registers.
-constexpr int MOST_GROUPS = HD <= 128 ? 4 : 2;
+template <typename T> constexpr int kMostGroups = HD <= 128 ? (sizeof(T) == 2 ? 4 : 2) : (sizeof(T) == 2 ? 2 : 1);
 
 struct Args {
   PrefixArgs a;
@@ -54,6 +68,12 @@ struct Args {
   float* row_o;                // [T][nh][HD]: of whole items, where a prefix is to be joined
   float2* row_ml;
   int* err;
+  // prefixes in 32 bits: rows of this kernel's tiles are far_shape's, and own tokens' are
+  Shape own_shape;
+  int own_H, places;
+  int* chunk;                  // where the length of a chunk is written down
+  float* far_o;                // [places][rows][HD]
+  float2* far_ml;
 };
 
 // A part of an item: tiles [from, from + count) of its prefix's tiles, then its own tokens'.
@@ -62,16 +82,16 @@ struct Piece {
   int last;                    // the last own token that the first token sees; the next one sees one more
   const int *far_table, *near_table;
   int to;
-  size_t at;                   // CUT: the place
+  size_t at;                   // CUT, FAR: the place
 };
-enum { FINAL, ROW, CUT };
+enum { FINAL, ROW, CUT, FAR_PIECE };
 struct Keys {
   const int* table;
   int key0, end;
 };
-__device__ __forceinline__ Keys keys_of(const Piece& x, int tile) {
-  if (tile < x.far) return {x.far_table, tile * KEYS, x.far_len};
-  return {x.near_table, (tile - x.far) * KEYS, x.near_len};
+__device__ __forceinline__ Keys keys_of(const Piece& x, int tile, int keys) {
+  if (tile < x.far) return {x.far_table, tile * keys, x.far_len};
+  return {x.near_table, (tile - x.far) * keys, x.near_len};
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {
   uint32_t d;
@@ -79,35 +99,78 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {
   return d;
 }
 
-template <int NG>
-__global__ void __launch_bounds__(THREADS, 1)
+// 32 bits as two tf32 numbers.
+struct Split {
+  uint32_t hi, lo;
+};
+__device__ __forceinline__ Split split(float x) {
+  Split s;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(s.hi) : "f"(x));
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(s.lo) : "f"(x - __uint_as_float(s.hi)));
+  return s;
+}
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <typename T, int NG, bool FAR>
+__global__ void __launch_bounds__(32 * Tile<T>::WARPS, 1)
 prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const Args p) {
+  using G = Tile<T>;
+  constexpr int KEYS = G::KEYS, WARPS = G::WARPS, STAGES = G::STAGES, THREADS = 32 * WARPS;
+  constexpr int COUNTING = THREADS < 128 ? THREADS : 128;
+  constexpr uint32_t STAGE = G::STAGE;
   extern __shared__ __align__(1024) unsigned char raw[];
   unsigned char* base = raw + ((0u - smem_u32(raw)) & 1023u);               // (a swizzle counts from 1 KB)
   __shared__ long long counts[4];
   __shared__ Cursor found[WARPS];
-  __shared__ int far_s;
+  __shared__ int far_s, chunk_s;
+  __shared__ GroupTiles groups_s[FAR ? 32 : 1];
   const PrefixArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   unsigned char* ring = base + warp * (STAGES * STAGE);
-  uint64_t* full = reinterpret_cast<uint64_t*>(base + smem_bytes(NG) - 1024 - WARPS * STAGES * 8) + warp * STAGES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(base + smem_bytes<T>(NG) - 1024 - WARPS * STAGES * 8) + warp * STAGES;
   if (lane == 0) {
     for (int i = 0; i < STAGES; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&full[i])), "r"(32));
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (!p.after) pdl_wait();
+  if (FAR) pdl_trigger();      // (behind the wait: the kernel beside this one reads what was waited for)
   Cursor cur{};
   Request req{};
-  if (p.joined) {
+  GroupTiles groups{};
+  int chunk = 1, index = 0, stride = 0;
+  if constexpr (FAR) {
+    // how the prefixes and the own tokens share the SMs, and the prefixes' chunks
+    FarWork f{};
+    if (warp == WARPS - 1) f = far_work(a, groups, p.H, p.shape.tokens, KEYS);
+    const OwnWork w = own_work<COUNTING>(a, p.own_shape.tokens, KEYS, false, counts);
+    if (warp == WARPS - 1) {
+      const int workers = far_share(p.sms, f.units, p.far_cost, w.total * p.own_H) * WARPS;
+      const int c = plan_chunk(a, groups, f, p.H, p.shape.tokens, KEYS, max(workers, 1), p.places, kItemTiles);
+      groups_s[lane] = groups;
+      if (lane == 0) {
+        chunk_s = c, far_s = workers;
+        if (blockIdx.x == 0) *p.chunk = c;
+      }
+    }
+    __syncthreads();
+    groups = groups_s[lane], chunk = chunk_s, stride = far_s;
+    index = blockIdx.x * WARPS + warp;
+    if (index >= stride) index = p.places;
+  } else if (p.joined) {
     // this block's warps' runs
     GroupTiles gt{};
     FarWork f{};
     if (p.after && warp == WARPS - 1) f = far_work(a, gt, p.far_H, p.far_shape.tokens, p.far_tile);
-    const OwnWork w = own_work<128>(a, p.shape.tokens, KEYS, p.both, counts);
+    const OwnWork w = own_work<COUNTING>(a, p.shape.tokens, KEYS, p.both, counts);
     if (threadIdx.x == THREADS - 1) far_s = p.after ? far_share(p.sms, f.units, p.far_cost, w.total * p.H) : 0;
     __syncthreads();
     const int blocks = p.after ? max(p.sms - far_s, 1) : (int)gridDim.x;
-    find_runs<128, WARPS>(a, w, p.H, p.shape.tokens, KEYS, p.both, blockIdx.x, blocks, blockIdx.x == 0 ? p.plan : nullptr, found);
+    find_runs<COUNTING, WARPS>(a, w, p.H, p.shape.tokens, KEYS, p.both, blockIdx.x, blocks, blockIdx.x == 0 ? p.plan : nullptr, found);
     cur = found[warp];
     if (cur.todo > 0) req = request_of(a, cur.b, p.both, KEYS);
   } else {
@@ -118,7 +181,7 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
   const int each = a.nh / a.nkv;
   const float scale_log2 = a.scale * LOG2E;
   const int box = min(a.page, KEYS), boxes = KEYS / box;
-  const bool tma = SWIZZLED && p.tma;
+  const bool tma = G::SWIZZLED && p.tma;
   uint32_t phases = 0;         // a bit a stage
   int st = 0;
   bool ok = true;
@@ -132,6 +195,17 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
       x.far_table = a.prefix_table + (size_t)max(req.g, 0) * a.prefix_stride;
       x.near_table = a.table + (size_t)cur.b * a.table_stride;
     };
+    if constexpr (FAR) {
+      PrefixItem it;
+      if (index >= p.places || !find_item(a, groups, p.H, p.shape.tokens, KEYS, chunk, index, it)) return false;
+      x.first = it.first, x.tokens = it.count, x.hc = it.hc;
+      x.from = it.split * chunk, x.count = min(chunk, it.tiles - x.from);
+      x.far = it.tiles, x.far_len = it.length, x.near_len = 0, x.last = -1;
+      x.far_table = a.prefix_table + (size_t)it.g * a.prefix_stride, x.near_table = nullptr;
+      x.to = FAR_PIECE, x.at = index;
+      index += stride;
+      return true;
+    }
     if (!p.joined) {
       if (cur.rt * p.shape.tokens >= req.count) return false;
       const int tiles = req.far + req.near, w0 = tiles * warp / WARPS, w1 = tiles * (warp + 1) / WARPS;
@@ -170,11 +244,11 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
     const int rows = x.tokens * heads;
     // ---- copies: a tile's places are looked up one tile ahead
     auto look = [&](int i) {
-      const Keys k = keys_of(x, x.from + i);
+      const Keys k = keys_of(x, x.from + i, KEYS);
       return slot_of(a, k.table, min(k.key0 + (lane & (KEYS - 1)), k.end - 1));
     };
     auto issue = [&](int i, int slot, int stage_i) {
-      const Keys k = keys_of(x, x.from + i);
+      const Keys k = keys_of(x, x.from + i, KEYS);
       unsigned char* stage = ring + stage_i * STAGE;
       uint64_t* bar = &full[stage_i];
       if (tma && k.key0 + KEYS <= k.end) {
@@ -185,21 +259,21 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
         else
           asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
         __syncwarp();
-        const int bx = lane % boxes, half = lane / boxes % HALVES, plane = lane / (boxes * HALVES);
+        const int bx = lane % boxes, half = lane / boxes % G::HALVES, plane = lane / (boxes * G::HALVES);
         const int row = __shfl_sync(0xffffffffu, slot, bx * box);
         if (plane < 2)
-          tma_load_2d(stage + plane * PLANE + half * (KEYS * 128) + bx * box * 128, plane ? &vmap : &kmap, bar, kvh * HD + half * 64, row);
+          tma_load_2d(stage + plane * G::PLANE + half * (KEYS * 128) + bx * box * 128, plane ? &vmap : &kmap, bar, kvh * HD + half * 64, row);
       } else {
-        constexpr int CH = HD / 8;
-        const bf16* kp = static_cast<const bf16*>(a.k) + (size_t)kvh * HD;
-        const bf16* vp = static_cast<const bf16*>(a.v) + (size_t)kvh * HD;
+        constexpr int CH = HD / G::CHUNK;
+        const T* kp = static_cast<const T*>(a.k) + (size_t)kvh * HD;
+        const T* vp = static_cast<const T*>(a.v) + (size_t)kvh * HD;
 #pragma unroll 2
         for (int j = 0; j < KEYS * CH / 32; ++j) {
-          const int idx = j * 32 + lane, row = idx / CH, ch = (idx - row * CH) * 8;
+          const int idx = j * 32 + lane, row = idx / CH, ch = (idx - row * CH) * G::CHUNK;
           const size_t off = (size_t)__shfl_sync(0xffffffffu, slot, row) * (a.nkv * HD) + ch;
           const bool there = k.key0 + row < k.end;
-          cp_async16(stage + place(row, ch), kp + off, there);
-          cp_async16(stage + PLANE + place(row, ch), vp + off, there);
+          cp_async16(stage + G::place(0, row, ch), kp + off, there);
+          cp_async16(stage + G::place(1, row, ch), vp + off, there);
         }
         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
       }
@@ -208,17 +282,26 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
     if (!ok) x.count = 0;      // (behind a wait that ran out: the warps still meet where they join)
     for (int i = 0; i < min(STAGES, x.count); ++i) issue(i, look(i), (st + i) % STAGES);
     if (STAGES < x.count) slot = look(STAGES);
-    // ---- q as the 8-column operand: thread (g, t) has channels 16 kc + 2t, + 1 and + 8, + 9 of row 8 ng + g
-    uint32_t qf[NG][KCH][2];
+    // ---- q as the 8-column operand: thread (g, t) has of row 8 ng + g the channels 16 kc + 2t, + 1 and + 8, + 9 (bfloat16), or
+    // 8 kc + t and + 4 (32 bits)
+    uint32_t qf[NG][sizeof(T) == 2 ? KCH : 2 * KCH][2];
     int see[NG][2];            // the last own token that rows 2t and 2t + 1 see (rows that are none see all, and nobody sees them)
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
       const int r = 8 * n + g, token = r < rows ? r / heads : 0, head = r < rows ? r - token * heads : 0;
-      const bf16* q = static_cast<const bf16*>(a.q) + (size_t)(x.first + token) * a.q_stride + (size_t)(h0 + head) * HD + 2 * t;
+      const T* q = static_cast<const T*>(a.q) + (size_t)(x.first + token) * a.q_stride + (size_t)(h0 + head) * HD;
+      if constexpr (sizeof(T) == 2) {
 #pragma unroll
-      for (int kc = 0; kc < KCH; ++kc) {
-        qf[n][kc][0] = r < rows ? __ldcg(reinterpret_cast<const unsigned*>(q + kc * 16)) : 0u;
-        qf[n][kc][1] = r < rows ? __ldcg(reinterpret_cast<const unsigned*>(q + kc * 16 + 8)) : 0u;
+        for (int kc = 0; kc < KCH; ++kc) {
+          qf[n][kc][0] = r < rows ? __ldcg(reinterpret_cast<const unsigned*>(q + 2 * t + kc * 16)) : 0u;
+          qf[n][kc][1] = r < rows ? __ldcg(reinterpret_cast<const unsigned*>(q + 2 * t + kc * 16 + 8)) : 0u;
+        }
+      } else {
+#pragma unroll
+        for (int kc = 0; kc < 2 * KCH; ++kc) {
+          qf[n][kc][0] = r < rows ? __ldcg(reinterpret_cast<const unsigned*>(q + t + kc * 8)) : 0u;
+          qf[n][kc][1] = r < rows ? __ldcg(reinterpret_cast<const unsigned*>(q + t + kc * 8 + 4)) : 0u;
+        }
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) see[n][e] = 8 * n + 2 * t + e < rows ? x.last + (8 * n + 2 * t + e) / heads : 0x7fffffff;
@@ -232,7 +315,7 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
     }
     // ---- tiles
     for (int i = 0; i < x.count && ok; ++i) {
-      const Keys k = keys_of(x, x.from + i);
+      const Keys k = keys_of(x, x.from + i, KEYS);
       const bool far = x.from + i < x.far;
       ok = wait_bar(&full[st], (phases >> st) & 1u, p.err, 22);
       if (!ok) break;
@@ -245,14 +328,34 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
         float s[NG][4];
 #pragma unroll
         for (int n = 0; n < NG; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+        if constexpr (sizeof(T) == 2) {
 #pragma unroll
-        for (int kc = 0; kc < KCH; ++kc) {
-          uint32_t af[4];
-          ldsm_x4(af, stage + place(sub * 16 + (lane & 15), kc * 16 + (lane >> 4) * 8));
+          for (int kc = 0; kc < KCH; ++kc) {
+            uint32_t af[4];
+            ldsm_x4(af, stage + G::place(0, sub * 16 + (lane & 15), kc * 16 + (lane >> 4) * 8));
 #pragma unroll
-          for (int n = 0; n < NG; ++n) mma16816(s[n], af, qf[n][kc][0], qf[n][kc][1]);
+            for (int n = 0; n < NG; ++n) mma16816(s[n], af, qf[n][kc][0], qf[n][kc][1]);
+          }
+        } else {
+#pragma unroll
+          for (int kc = 0; kc < 2 * KCH; ++kc) {
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const Split y = split(*reinterpret_cast<const float*>(stage + G::place(0, g + 8 * (i & 1), kc * 8 + t + 4 * (i >> 1))));
+              hi[i] = y.hi, lo[i] = y.lo;
+            }
+#pragma unroll
+            for (int n = 0; n < NG; ++n) {
+              const Split q0 = split(__uint_as_float(qf[n][kc][0])), q1 = split(__uint_as_float(qf[n][kc][1]));
+              mma_tf32(s[n], lo, q0.hi, q1.hi);
+              mma_tf32(s[n], hi, q0.lo, q1.lo);
+              mma_tf32(s[n], hi, q0.hi, q1.hi);
+            }
+          }
         }
-        uint32_t b0[NG], b1[NG];
+        uint32_t b0[NG], b1[NG];           // bfloat16: weights as the 8-column operand
+        float w[NG][4];                    // 32 bits: weights as they are
         bool grew = false;
         float corr[NG][2];
 #pragma unroll
@@ -286,8 +389,12 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
           l[n][0] = l[n][0] * corr[n][0] + (p0 + p2);
           l[n][1] = l[n][1] * corr[n][1] + (p1 + p3);
           // (weights are rounded to bfloat16 for the product, as everywhere in this package; their sum is not)
-          b0[n] = transposed(pack_bf16(p0, p1));
-          b1[n] = transposed(pack_bf16(p2, p3));
+          if constexpr (sizeof(T) == 2) {
+            b0[n] = transposed(pack_bf16(p0, p1));
+            b1[n] = transposed(pack_bf16(p2, p3));
+          } else {
+            w[n][0] = p0, w[n][1] = p1, w[n][2] = p2, w[n][3] = p3;
+          }
         }
         if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
@@ -296,12 +403,42 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
             for (int c = 0; c < HD / 16; ++c)
               o[n][c][0] *= corr[n][0], o[n][c][1] *= corr[n][1], o[n][c][2] *= corr[n][0], o[n][c][3] *= corr[n][1];
         }
+        if constexpr (sizeof(T) == 2) {
 #pragma unroll
-        for (int c = 0; c < HD / 16; ++c) {
-          uint32_t af[4];
-          ldsm_x4_t(af, stage + PLANE + place(sub * 16 + (lane >> 4) * 8 + (lane & 7), c * 16 + ((lane >> 3) & 1) * 8));
+          for (int c = 0; c < HD / 16; ++c) {
+            uint32_t af[4];
+            ldsm_x4_t(af, stage + G::place(1, sub * 16 + (lane >> 4) * 8 + (lane & 7), c * 16 + ((lane >> 3) & 1) * 8));
 #pragma unroll
-          for (int n = 0; n < NG; ++n) mma16816(o[n][c], af, b0[n], b1[n]);
+            for (int n = 0; n < NG; ++n) mma16816(o[n][c], af, b0[n], b1[n]);
+          }
+        } else {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {     // eight keys each
+            // the weight of key t (and t + 4) for row g: thread (key, row / 2) has it
+            Split p0[NG], p1[NG];
+#pragma unroll
+            for (int n = 0; n < NG; ++n) {
+              const float e0 = __shfl_sync(0xffffffffu, w[n][2 * half], t * 4 + (g >> 1)), e1 = __shfl_sync(0xffffffffu, w[n][2 * half + 1], t * 4 + (g >> 1));
+              const float f0 = __shfl_sync(0xffffffffu, w[n][2 * half], (t + 4) * 4 + (g >> 1));
+              const float f1 = __shfl_sync(0xffffffffu, w[n][2 * half + 1], (t + 4) * 4 + (g >> 1));
+              p0[n] = split(g & 1 ? e1 : e0), p1[n] = split(g & 1 ? f1 : f0);
+            }
+#pragma unroll
+            for (int c = 0; c < HD / 16; ++c) {
+              uint32_t hi[4], lo[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const Split y = split(*reinterpret_cast<const float*>(stage + G::place(1, half * 8 + t + 4 * (i >> 1), c * 16 + g + 8 * (i & 1))));
+                hi[i] = y.hi, lo[i] = y.lo;
+              }
+#pragma unroll
+              for (int n = 0; n < NG; ++n) {
+                mma_tf32(o[n][c], lo, p0[n].hi, p1[n].hi);
+                mma_tf32(o[n][c], hi, p0[n].lo, p1[n].lo);
+                mma_tf32(o[n][c], hi, p0[n].hi, p1[n].hi);
+              }
+            }
+          }
         }
       }
       __syncwarp();
@@ -351,7 +488,7 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
         }
         const float inv = sum == 0.f ? 0.f : 1.f / sum;                      // (no key: zeros)
         const float z[4] = {y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv};
-        if (ok) Quad<bf16>::store(static_cast<bf16*>(a.out) + ((size_t)(x.first + token) * a.nh + h0 + head) * HD + ch, z);
+        if (ok) Quad<T>::store(static_cast<T*>(a.out) + ((size_t)(x.first + token) * a.nh + h0 + head) * HD + ch, z);
       }
       __syncthreads();           // (the ring lies there again)
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -368,16 +505,16 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
         const size_t row = (size_t)(x.first + token) * a.nh + h0 + r - token * heads;
         if (x.to == FINAL) {
           const float inv = l[n][e] == 0.f ? 0.f : 1.f / l[n][e];
-          bf16* to = static_cast<bf16*>(a.out) + row * HD + g;
+          T* to = static_cast<T*>(a.out) + row * HD + g;
 #pragma unroll
           for (int c = 0; c < HD / 16; ++c)
-            to[c * 16] = __float2bfloat16_rn(o[n][c][e] * inv), to[c * 16 + 8] = __float2bfloat16_rn(o[n][c][2 + e] * inv);
+            to[c * 16] = from_f32<T>(o[n][c][e] * inv), to[c * 16 + 8] = from_f32<T>(o[n][c][2 + e] * inv);
         } else {
           const size_t at = x.to == ROW ? row : x.at * p.rows + r;
-          float* to = (x.to == ROW ? p.row_o : p.cut_o) + at * HD + g;
+          float* to = (x.to == ROW ? p.row_o : x.to == CUT ? p.cut_o : p.far_o) + at * HD + g;
 #pragma unroll
           for (int c = 0; c < HD / 16; ++c) to[c * 16] = o[n][c][e], to[c * 16 + 8] = o[n][c][2 + e];
-          if (g == 0) (x.to == ROW ? p.row_ml : p.cut_ml)[at] = make_float2(m[n][e], l[n][e]);
+          if (g == 0) (x.to == ROW ? p.row_ml : x.to == CUT ? p.cut_ml : p.far_ml)[at] = make_float2(m[n][e], l[n][e]);
         }
       }
   }
@@ -385,7 +522,7 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
   if (!ok)
     for (int i = 0; i < STAGES; ++i) wait_bar(&full[i], (phases >> i) & 1u, p.err, 23);
   asm volatile("cp.async.wait_all;" ::: "memory");
-  if (p.joined) {
+  if (!FAR && p.joined) {
     pdl_trigger();
     // the joining kernel waits for this launch alone: its last block ends behind the one that ran beside it
     if (p.after && blockIdx.x == gridDim.x - 1) pdl_wait();

@@ -22,13 +22,13 @@ _VERIFY = struct.Struct("=18q")
 
 def _rows(x, rows, columns, what, device):
     """(address, row stride) of rows of logits."""
-    if x.dim() != 2 or x.shape != (rows, columns) or (x.stride(1) != 1 and columns > 1):
+    if x.shape != (rows, columns) or (x.stride(1) != 1 and columns > 1):
         raise ValueError(f"{what} is [{rows}, {columns}], a row without gaps; got {tuple(x.shape)}, strides {tuple(x.stride())}")
     return _at(x, device), x.stride(0)
 
 
 def _vector(t, count, dtype, what, device):
-    if t.dtype is not dtype or t.dim() != 1 or t.shape[0] != count or not t.is_contiguous():
+    if t.dtype is not dtype or t.shape != (count,) or not t.is_contiguous():
         raise ValueError(f"{what} is {dtype} [{count}], contiguous; got {t.dtype} {tuple(t.shape)}")
     return _at(t, device)
 

@@ -17,12 +17,13 @@ import torch
 
 from . import _Counter, _ok
 from .build import load_library
-from .quant_cache import _at, _capturing, _code, _device, _function, _of_device, _raw_stream
+from .quant_cache import _CODE, _at, _capturing, _device, _function, _of_device, _raw_stream
 
 MAX_HEAD_DIM = 256
 _ATTEND = struct.Struct("=29qd")
 _LAUNCHES = {-101: 1, -102: 2}          # what the entry point returns when it launched fewer than three kernels
-_int32 = torch.int32
+_int32, _INF = torch.int32, float("inf")
+_attend_functions: dict = {}
 
 
 def supports(head_dim: int, heads: int, kv_heads: int) -> bool:
@@ -39,7 +40,7 @@ def _table(t, count, what, device):
 
 
 def _vector(t, count, what, device):
-    if t.dtype is not _int32 or t.dim() != 1 or t.shape[0] != count or not t.is_contiguous():
+    if t.dtype is not _int32 or t.shape != (count,) or not t.is_contiguous():
         raise ValueError(f"{what} is int32 [{count}], contiguous; got {t.dtype} {tuple(t.shape)}")
     return _at(t, device)
 
@@ -88,24 +89,40 @@ def attend(q: torch.Tensor, nh: int, pages, prefix_table: torch.Tensor, prefix_l
     The ``i``-th of a request's ``n`` rows sees the whole prefix and the own tokens ``0 .. length - n + i``; a row that
     sees nothing gives zeros.  Rows that belong to no request are not written: with ``out`` (``[T, nh * head size]``,
     contiguous, ``q``'s type) they stay as they were.  Entries of the tables behind a sequence's length are not read."""
-    k, v = pages[0], pages[1]
-    if k.dim() != 4 or k.shape != v.shape or not k.is_contiguous() or not v.is_contiguous() or v.dtype != k.dtype:
-        raise ValueError(f"the cache's planes are [pages, page, kv heads, head size], contiguous, of one shape and type; got "
-                         f"{tuple(k.shape)}, {tuple(v.shape)}")
-    count, page, nkv, hd = k.shape
+    # (what follows is the host's time of a call: a plane of its own would be two tensors made, a helper a call)
+    if torch.is_tensor(pages):
+        shape, dtype = pages.shape, pages.dtype
+        if len(shape) != 5 or shape[0] != 2 or not pages.is_contiguous():
+            raise ValueError(f"the cache is [2, pages, page, kv heads, head size], contiguous; got {tuple(shape)}")
+        _, count, page, nkv, hd = shape
+        dev = _device(pages)
+        k_at = pages.data_ptr()
+        v_at = k_at + count * page * nkv * hd * pages.itemsize
+    else:
+        k, v = pages
+        shape, dtype = k.shape, k.dtype
+        if len(shape) != 4 or v.shape != shape or not k.is_contiguous() or not v.is_contiguous() or v.dtype != dtype:
+            raise ValueError(f"the cache's planes are [pages, page, kv heads, head size], contiguous, of one shape and type; got "
+                             f"{tuple(shape)}, {tuple(v.shape)}")
+        count, page, nkv, hd = shape
+        dev = _device(k)
+        k_at, v_at = k.data_ptr(), _at(v, dev)
+    code = _CODE.get(dtype)
+    if code is None:
+        raise TypeError(f"kernels take float32 or bfloat16 activations, not {dtype}")
     if not supports(hd, nh, nkv):
         raise ValueError(f"attention over shared prefixes takes head sizes that are a multiple of 16, at most "
                          f"{MAX_HEAD_DIM}, and a multiple of the kv heads; got head_dim={hd}, heads={nh}, kv_heads={nkv}")
     if count < 1 or page < 1 or count * page >= 1 << 31:
         raise ValueError(f"{count} pages of {page} tokens: a cache has at least one, and slots are 32-bit integers")
-    dev = _device(k)
-    if q.dim() != 2 or q.shape[1] < nh * hd or (q.stride(1) != 1 and q.shape[1] > 1) or q.dtype != k.dtype:
-        raise ValueError(f"q has rows of at least {nh * hd} channels without gaps in the cache's type {k.dtype}; got "
+    width = nh * hd
+    if q.dim() != 2 or q.dtype is not dtype or q.shape[1] < width or (q.stride(1) != 1 and q.shape[1] > 1):
+        raise ValueError(f"q has rows of at least {width} channels without gaps in the cache's type {dtype}; got "
                          f"{q.dtype} {tuple(q.shape)}, strides {tuple(q.stride())}")
-    code, at, stride = _code(q.dtype), _at(q, dev), q.stride(0)
-    if (at | stride * q.itemsize) & 15 or stride < nh * hd:            # (the kernels read 16 bytes at a time)
-        q = q[:, :nh * hd].contiguous()
-        at, stride = q.data_ptr(), nh * hd
+    at, stride = _at(q, dev), q.stride(0)
+    if (at | stride * q.itemsize) & 15 or stride < width:            # (the kernels read 16 bytes at a time)
+        q = q[:, :width].contiguous()
+        at, stride = q.data_ptr(), width
     T, B, G = q.shape[0], lengths.shape[0], prefix_lens.shape[0]
     prefix, prefix_stride, P = _table(prefix_table, G, "prefix_table", dev)
     table, table_stride, W = _table(block_table, B, "block_table", dev)
@@ -119,31 +136,36 @@ def attend(q: torch.Tensor, nh: int, pages, prefix_table: torch.Tensor, prefix_l
         rows = _vector(cu_seqlens_q, B + 1, "cu_seqlens_q", dev)
     elif T < B:
         raise ValueError(f"{T} rows for {B} requests of one row each")
-    if P * page >= 1 << 30 or W * page >= 1 << 30:
-        raise ValueError(f"tables of {P} and {W} pages of {page}: a sequence has fewer than 2^30 tokens")
+    P, W = P * page, W * page
+    if P >= 1 << 30 or W >= 1 << 30:
+        raise ValueError(f"tables of {P} and {W} tokens: a sequence has fewer than 2^30")
     if max_q_len is not None and max_q_len < 0:
         raise ValueError(f"max_q_len is {max_q_len}")
-    if not scale > 0:
-        raise ValueError(f"the scale of the scores is positive, not {scale}")
+    if not 0 < scale < _INF:
+        raise ValueError(f"the scale of the scores is a positive number, not {scale}")
     if out is None:
-        out = q.new_empty(T, nh * hd)
-    elif out.dtype != q.dtype or out.shape != (T, nh * hd) or not out.is_contiguous():
-        raise ValueError(f"out is {q.dtype} {(T, nh * hd)}, contiguous; got {out.dtype} {tuple(out.shape)}")
-    if (k.data_ptr() | v.data_ptr() | out.data_ptr()) & 15:
+        out = q.new_empty(T, width)
+        out_at = out.data_ptr()
+    else:
+        if out.dtype is not dtype or out.shape != (T, width) or not out.is_contiguous():
+            raise ValueError(f"out is {dtype} {(T, width)}, contiguous; got {out.dtype} {tuple(out.shape)}")
+        out_at = _at(out, dev)
+    if (k_at | v_at | out_at) & 15:
         raise ValueError("the cache's planes and out start at multiples of 16 bytes")
     if T == 0 or B == 0:
         return out
     sms, err = _of_device(dev)
     stream = _raw_stream(dev)
     longest = min(max_q_len or -(-T // B), T)
-    size = _scratch_bytes(hd, code, G, P * page, B, W * page, T, nh, nkv, sms, longest, page)
-    f = _function("shared_prefix", "gf_prefix_attend", (f"GF_HEAD_DIM={hd}",))
+    size = _scratch_bytes(hd, code, G, P, B, W, T, nh, nkv, sms, longest, page)
+    f = _attend_functions.get(hd)
+    if f is None:
+        f = _attend_functions[hd] = _function("shared_prefix", "gf_prefix_attend", (f"GF_HEAD_DIM={hd}",))
     with _launching:
-        scratch = _scratch_for(size, dev, stream)
-        rc = f(_ATTEND.pack(at, stride, code, k.data_ptr(), _at(v, dev), count, page, prefix, prefix_stride,
-                            prefix_tokens, G, P * page, table, table_stride,
-                            own_tokens, B, W * page, groups, rows, _at(out, dev), T, nh, nkv, sms,
-                            longest, scratch.data_ptr(), size, err, stream, scale))
+        scratch = _scratch_for(size, dev, stream).data_ptr() if size else 0
+        rc = f(_ATTEND.pack(at, stride, code, k_at, v_at, count, page, prefix, prefix_stride, prefix_tokens, G, P, table,
+                            table_stride, own_tokens, B, W, groups, rows, out_at, T, nh, nkv, sms, longest, scratch, size, err,
+                            stream, scale))
     _Counter.launches += _LAUNCHES.get(rc, 3)
     if rc and rc not in _LAUNCHES:
         _ok(rc, "shared_prefix.attend")

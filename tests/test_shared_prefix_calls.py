@@ -19,6 +19,7 @@ def calls(monkeypatch):
     monkeypatch.setattr(shared_prefix, "_scratch_bytes", lambda *sizes: 64)
     monkeypatch.setattr(shared_prefix, "_capturing", lambda: False)
     monkeypatch.setattr(shared_prefix, "_scratch", {})
+    monkeypatch.setattr(shared_prefix, "_attend_functions", {})
     return got
 
 

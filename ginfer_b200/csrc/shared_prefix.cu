@@ -65,7 +65,7 @@ struct FarArgs {
   Shape shape, own_shape;      // rows of this kernel's tiles, of the one's that works on own tokens beside it
   int H, own_H, places, sms, own_tile;
   float cost;                  // of a tile beside one of own tokens
-  int* chunk;                  // where the length of a chunk is written down
+  FarPlan* far_plan;           // [G]
   float* far_o;                // [places][MOST_ROWS][HD]
   float2* far_ml;
   int* err;
@@ -173,10 +173,8 @@ prefix_pieces_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
       const int workers = far_share(p.sms, f.units, p.cost, w.total * p.own_H) * BLOCKS_AN_SM;
       const int chunk = plan_chunk(a, t, f, p.H, p.shape.tokens, TILE, max(workers, 1), p.places, 3);
       groups_s[lane] = t;
-      if (lane == 0) {
-        chunk_s = chunk, workers_s = workers;
-        if (blockIdx.x == 0) *p.chunk = chunk;
-      }
+      if (lane == 0) chunk_s = chunk, workers_s = workers;
+      if (blockIdx.x == 0) write_far_plan(a, t, p.H, p.shape.tokens, TILE, chunk, p.far_plan);
     }
     __syncthreads();
   }
@@ -380,14 +378,14 @@ namespace {
 struct JoinArgs {
   own::Args p;
   int far_rows, places;        // rows of a place of the prefixes' pieces (0: there are none), places
-  const int* chunk;
+  const FarPlan* far_plan;
   const float* far_o;
   const float2* far_ml;
 };
 constexpr int JOIN_WARPS = 8, JOIN_CH = (HD / 4 + 31) / 32;      // a lane has channels 4 lane, 128 + 4 lane
 
 template <typename T>
-__global__ void __launch_bounds__(32 * JOIN_WARPS) prefix_join_kernel(const JoinArgs j) {
+__global__ void __launch_bounds__(32 * JOIN_WARPS, HD <= 128 ? 4 : 3) prefix_join_kernel(const JoinArgs j) {
   const own::Args& p = j.p;
   const PrefixArgs& a = p.a;
   const Shape& far_shape = p.far_shape;
@@ -395,32 +393,17 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) prefix_join_kernel(const Join
   pdl_trigger();
   pdl_wait();
   const bool both = p.both;
-  const Request r = request_of(a, b, both, own::Tile<T>::KEYS);
-  if (r.count == 0) return;
+  const OwnPlan::Entry& e = p.plan->of[b];
+  const int2 rows = __ldcg(reinterpret_cast<const int2*>(&e.first)), more = __ldcg(reinterpret_cast<const int2*>(&e.tiles));
+  const long long run = __ldcg(&p.plan->run), per = __ldcg(&p.plan->each), base = __ldcg(&e.base);
+  const int first = rows.x, count = rows.y, tiles = more.x, units = tiles + kItemTiles;
+  if (count == 0) return;
   // where its prefix's pieces are
-  int splits = 0, far_mt = 0, far_first = 0;
-  long long far_base = 0;
-  if (j.far_rows) {
-    const int g = group_of(a, b), H = a.nkv * far_shape.chunks, chunk = max(fresh_index(j.chunk), 1);
-    for (int g0 = 0; g0 < a.G && g0 <= g; g0 += 32) {
-      GroupTiles t;
-      t.load(a, g0 + lane, far_shape.tokens, p.far_tile);
-      const int s = (t.nt + chunk - 1) / chunk;
-      long long items = g0 + lane < g ? (long long)t.mt * H * s : 0;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) items += __shfl_xor_sync(0xffffffffu, items, o);
-      far_base += items;
-      if (g - g0 < 32) {
-        splits = __shfl_sync(0xffffffffu, s, g - g0);
-        far_mt = __shfl_sync(0xffffffffu, t.mt, g - g0);
-        far_first = __shfl_sync(0xffffffffu, t.first, g - g0);
-      }
-    }
-  }
-  const long long run = __ldcg(&p.plan->run), per = __ldcg(&p.plan->each), base = __ldcg(&p.plan->base[b]);
-  const int tiles = r.tiles(), units = r.units();
-  for (int i = blockIdx.z * JOIN_WARPS + warp; i < r.count * each; i += gridDim.z * JOIN_WARPS) {
-    const int token = i / each, hh = i - token * each, t = r.first + token;
+  int4 far{};
+  if (j.far_rows && more.y >= 0) far = __ldcg(reinterpret_cast<const int4*>(j.far_plan + more.y));
+  const int far_base = far.x, splits = far.y, far_mt = far.z, far_first = far.w;
+  for (int i = blockIdx.z * JOIN_WARPS + warp; i < count * each; i += gridDim.z * JOIN_WARPS) {
+    const int token = i / each, hh = i - token * each, t = first + token;
     const size_t row = (size_t)t * a.nh + kvh * each + hh;
     // its own tokens' pieces: the blocks whose runs have some of its tiles
     const int rt = token / p.shape.tokens, part = hh / p.shape.heads, heads = min(p.shape.heads, each - part * p.shape.heads);
@@ -435,7 +418,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) prefix_join_kernel(const Join
     // (the tensor cores' tiles leave room for the heads that a chunk may have, the others for those that it has)
     const int far_r = j.far_rows ? (from - m * far_shape.tokens) * (j.far_rows == 128 ? far_shape.heads : far_heads) + hh -
                                        far_part * far_shape.heads : 0;
-    const long long far_at = far_base + (long long)(kvh * far_shape.chunks + far_part) * splits * far_mt + m;
+    const long long far_at = (long long)far_base + (long long)(kvh * far_shape.chunks + far_part) * splits * far_mt + m;
     const int own = cut ? k1 - k0 + 1 : 1, pieces = splits + own;
     auto find = [&](int k, const float*& o, const float2*& ml) {
       if (k < splits) {
@@ -611,7 +594,7 @@ struct Call {
     };
     if (direct) return;
     const long long rows = (long long)a.T * a.nh, cut = (long long)p.sms * warps * 2 * p.rows;
-    p.plan = (OwnPlan*)take(16 + 8ll * a.B);
+    p.plan = (OwnPlan*)take(16 + (long long)sizeof(OwnPlan::Entry) * a.B);
     p.cut_o = (float*)take(cut * HD * 4), p.cut_ml = (float2*)take(cut * 8);
     if (!shared) return;
     tensor = GF_PREFIX_TC && half && a.page % 8 == 0 && 128 % a.page == 0;
@@ -620,13 +603,13 @@ struct Call {
     p.far_shape = row_shape_of(a.nh, a.nkv, j.far_rows), p.far_tile = tensor ? 128 : half ? TILE : keys, p.far_H = a.nkv * p.far_shape.chunks;
     p.far_cost = getenv("GF_COST") ? (float)atof(getenv("GF_COST")) : tensor ? kTensorCost : half ? kPlainCost : 1.f;
     const long long tiles = (long long)p.far_H * ((a.T + p.far_shape.tokens - 1) / p.far_shape.tokens + a.G);
-    const long long least = 2ll * p.sms * (tensor ? 1 : half ? BLOCKS_AN_SM : warps);
+    const long long least = 4ll * p.sms * (tensor ? 1 : half ? BLOCKS_AN_SM : warps);
     j.places = (int)(tiles > least ? tiles : least);
-    int* chunk = (int*)take(4);
+    FarPlan* far_plan = (FarPlan*)take((long long)sizeof(FarPlan) * a.G);
     float* far_o = (float*)take((long long)j.places * j.far_rows * HD * 4);
     float2* far_ml = (float2*)take((long long)j.places * j.far_rows * 8);
-    j.chunk = chunk, j.far_o = far_o, j.far_ml = far_ml;
-    f = FarArgs{a, 0, p.far_shape, p.shape, p.far_H, p.H, j.places, p.sms, keys, p.far_cost, chunk, far_o, far_ml, p.err};
+    j.far_plan = far_plan, j.far_o = far_o, j.far_ml = far_ml;
+    f = FarArgs{a, 0, p.far_shape, p.shape, p.far_H, p.H, j.places, p.sms, keys, p.far_cost, far_plan, far_o, far_ml, p.err};
   }
 };
 
@@ -680,7 +663,7 @@ GF_EXPORT int gf_prefix_attend(const char* words) {
       });
       if (rc) return rc;
       const FarArgs& f = c.f;
-      const tc::Args t{a, f.shape, f.own_shape, f.H, f.own_H, f.places, a.pages * a.page, f.sms, f.own_tile, f.cost, f.chunk, f.far_o,
+      const tc::Args t{a, f.shape, f.own_shape, f.H, f.own_H, f.places, a.pages * a.page, f.sms, f.own_tile, f.cost, f.far_plan, f.far_o,
                        f.far_ml, f.err};
       CUtensorMap tq, tk, tv;
       if (!query_map(&tq, a, f.shape) || !maps(tk, tv, 128)) return -7;
@@ -690,7 +673,7 @@ GF_EXPORT int gf_prefix_attend(const char* words) {
     if (!half) {
       own::Args f = p;
       f.shape = p.far_shape, f.H = p.far_H, f.rows = c.j.far_rows, f.own_shape = p.shape, f.own_H = p.H;
-      f.places = c.j.places, f.chunk = c.f.chunk, f.far_o = c.f.far_o, f.far_ml = c.f.far_ml, f.after = 0;
+      f.places = c.j.places, f.far_plan = c.f.far_plan, f.far_o = c.f.far_o, f.far_ml = c.f.far_ml, f.after = 0;
       rc = launch_own<float, own::kMostGroups<float>, true>(f, ok, ov, dim3(p.sms), c.stream);
     } else {
       static OncePerDevice attrs;

@@ -178,6 +178,29 @@ __device__ __forceinline__ int plan_chunk(const PrefixArgs& a, const GroupTiles&
   }
   return chunk;
 }
+// What the joining kernel needs of a group: its first item, its prefix's chunks, its tiles of rows and its first row.
+struct FarPlan {
+  int base, splits, mt, first;
+};
+// By one warp; `t` has the first 32 groups.
+__device__ __forceinline__ void write_far_plan(const PrefixArgs& a, const GroupTiles& first, int H, int tokens, int tile, int chunk,
+                                               FarPlan* plan) {
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  GroupTiles t = first;
+  for (int g0 = 0; g0 < a.G; g0 += 32) {
+    if (g0) t.load(a, g0 + lane, tokens, tile);
+    const int splits = (t.nt + chunk - 1) / chunk, items = t.mt * H * splits;
+    int sum = items;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += up;
+    }
+    if (g0 + lane < a.G) plan[g0 + lane] = {before + sum - items, splits, t.mt, t.first};
+    before += __shfl_sync(0xffffffffu, sum, 31);
+  }
+}
 // Item `index` in the order groups, (kv head, chunk of heads), chunks of keys, tiles of rows; false behind the last.
 // By a whole warp; `t` keeps the first 32 groups' tiles.
 __device__ __forceinline__ bool find_item(const PrefixArgs& a, const GroupTiles& t, int H, int tokens, int tile, int chunk,
@@ -239,11 +262,14 @@ struct Cursor {
   int hc, b, rt, off;
   long long todo;
 };
-// What the joining kernel needs of the division: a run's units, the units of one (kv head, chunk of heads), and the units
-// before every request's.
+// What the joining kernel needs of the division: a run's units, the units of one (kv head, chunk of heads), and of every request
+// the units before it, its rows, its tiles and its group.
 struct OwnPlan {
   long long run, each;
-  long long base[1];            // [B]
+  struct Entry {
+    long long base;
+    int first, count, tiles, g;
+  } of[1];                      // [B]
 };
 constexpr int kLeastRun = 8;    // the fewest units of a run
 
@@ -252,15 +278,20 @@ constexpr int kLeastRun = 8;    // the fewest units of a run
 struct OwnWork {
   int b0, b1;
   long long mine, start, total;
+  Request first;                // b0's
+  __device__ __forceinline__ Request request(const PrefixArgs& a, int b, bool both, int tile) const {
+    return b == b0 ? first : request_of(a, b, both, tile);
+  }
 };
 template <int THREADS>
 __device__ __forceinline__ OwnWork own_work(const PrefixArgs& a, int tokens, int tile, bool both, long long* counts) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, each = (a.B + THREADS - 1) / THREADS;
-  OwnWork w{min((int)threadIdx.x * each, a.B), 0, 0, 0, 0};
+  OwnWork w{min((int)threadIdx.x * each, a.B), 0, 0, 0, 0, {}};
   w.b1 = min(w.b0 + each, a.B);
   if (threadIdx.x < THREADS)
     for (int b = w.b0; b < w.b1; ++b) {
       const Request r = request_of(a, b, both, tile);
+      if (b == w.b0) w.first = r;
       w.mine += (long long)r.row_tiles(tokens) * r.units();
     }
   long long sum = w.mine;
@@ -292,8 +323,8 @@ __device__ __forceinline__ void find_runs(const PrefixArgs& a, const OwnWork& w,
     if (threadIdx.x == 0) plan->run = run, plan->each = w.total;
     long long base = w.start;
     for (int b = w.b0; b < w.b1; ++b) {
-      const Request r = request_of(a, b, both, tile);
-      plan->base[b] = base;
+      const Request r = w.request(a, b, both, tile);
+      plan->of[b] = {base, r.first, r.count, r.tiles(), both ? r.g : group_of(a, b)};
       base += (long long)r.row_tiles(tokens) * r.units();
     }
   }
@@ -306,7 +337,7 @@ __device__ __forceinline__ void find_runs(const PrefixArgs& a, const OwnWork& w,
       long long rest = at - hc_units - w.start;
       if (rest < 0 || rest >= w.mine) continue;
       for (int b = w.b0; b < w.b1; ++b) {
-        const Request r = request_of(a, b, both, tile);
+        const Request r = w.request(a, b, both, tile);
         const long long units = r.units(), here = r.row_tiles(tokens) * units;
         if (rest < here) {
           const int rt = (int)quotient(rest, units);

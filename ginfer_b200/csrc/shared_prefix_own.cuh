@@ -49,6 +49,7 @@ template <typename T> __host__ __device__ constexpr uint32_t smem_bytes(int ng) 
   return (ring > exchange ? ring : exchange) + G::WARPS * G::STAGES * 8 + 1024;
 }
 // Groups of 8 rows at most: their results and their q have to fit the registers.
+constexpr float kGrowth = 8.f;   // log2 units: weights stay below 2^8
 template <typename T> constexpr int kMostGroups = HD <= 128 ? (sizeof(T) == 2 ? 4 : 2) : (sizeof(T) == 2 ? 2 : 1);
 
 struct Args {
@@ -71,7 +72,7 @@ struct Args {
   // prefixes in 32 bits: rows of this kernel's tiles are far_shape's, and own tokens' are
   Shape own_shape;
   int own_H, places;
-  int* chunk;                  // where the length of a chunk is written down
+  FarPlan* far_plan;           // [G]
   float* far_o;                // [places][rows][HD]
   float2* far_ml;
 };
@@ -116,6 +117,14 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// A TMA copy of what is read once: it leaves L2 first.
+__device__ __forceinline__ void copy_once(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4}], [%2], %5;"
+      ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "l"(policy)
+      : "memory");
+}
+
 template <typename T, int NG, bool FAR>
 __global__ void __launch_bounds__(32 * Tile<T>::WARPS, 1)
 prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const Args p) {
@@ -154,8 +163,8 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
       groups_s[lane] = groups;
       if (lane == 0) {
         chunk_s = c, far_s = workers;
-        if (blockIdx.x == 0) *p.chunk = c;
       }
+      if (blockIdx.x == 0) write_far_plan(a, groups, p.H, p.shape.tokens, KEYS, c, p.far_plan);
     }
     __syncthreads();
     groups = groups_s[lane], chunk = chunk_s, stride = far_s;
@@ -182,6 +191,8 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
   const float scale_log2 = a.scale * LOG2E;
   const int box = min(a.page, KEYS), boxes = KEYS / box;
   const bool tma = G::SWIZZLED && p.tma;
+  uint64_t once;
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(once));
   uint32_t phases = 0;         // a bit a stage
   int st = 0;
   bool ok = true;
@@ -262,7 +273,8 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
         const int bx = lane % boxes, half = lane / boxes % G::HALVES, plane = lane / (boxes * G::HALVES);
         const int row = __shfl_sync(0xffffffffu, slot, bx * box);
         if (plane < 2)
-          tma_load_2d(stage + plane * G::PLANE + half * (KEYS * 128) + bx * box * 128, plane ? &vmap : &kmap, bar, kvh * HD + half * 64, row);
+          copy_once(stage + plane * G::PLANE + half * (KEYS * 128) + bx * box * 128, plane ? &vmap : &kmap, bar, kvh * HD + half * 64, row,
+                    once);
       } else {
         constexpr int CH = HD / G::CHUNK;
         const T* kp = static_cast<const T*>(a.k) + (size_t)kvh * HD;
@@ -280,8 +292,15 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
     };
     int slot = 0;
     if (!ok) x.count = 0;      // (behind a wait that ran out: the warps still meet where they join)
-    for (int i = 0; i < min(STAGES, x.count); ++i) issue(i, look(i), (st + i) % STAGES);
-    if (STAGES < x.count) slot = look(STAGES);
+    {
+      int first[STAGES];
+#pragma unroll
+      for (int i = 0; i < STAGES; ++i) first[i] = i < x.count ? look(i) : 0;
+      if (STAGES < x.count) slot = look(STAGES);
+#pragma unroll
+      for (int i = 0; i < STAGES; ++i)
+        if (i < x.count) issue(i, first[i], (st + i) % STAGES);
+    }
     // ---- q as the 8-column operand: thread (g, t) has of row 8 ng + g the channels 16 kc + 2t, + 1 and + 8, + 9 (bfloat16), or
     // 8 kc + t and + 4 (32 bits)
     uint32_t qf[NG][sizeof(T) == 2 ? KCH : 2 * KCH][2];
@@ -356,12 +375,12 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
         }
         uint32_t b0[NG], b1[NG];           // bfloat16: weights as the 8-column operand
         float w[NG][4];                    // 32 bits: weights as they are
+        // what weights are relative to follows a row's largest score only when that has outgrown it by 2^kGrowth: as a rule a
+        // tile needs no exchange between lanes
         bool grew = false;
-        float corr[NG][2];
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
           const int ka = k.key0 + sub * 16 + g, kb = ka + 8;
-          float mx[2], base_m[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             s[n][e] *= scale_log2, s[n][2 + e] *= scale_log2;
@@ -370,24 +389,32 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
               if (ka > end) s[n][e] = -INFINITY;
               if (kb > end) s[n][2 + e] = -INFINITY;
             }
-            mx[e] = fmaxf(s[n][e], s[n][2 + e]);
+            grew |= fmaxf(s[n][e], s[n][2 + e]) > m[n][e] + kGrowth;
           }
+        }
+        if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
-          for (int d = 4; d < 32; d <<= 1)
+          for (int n = 0; n < NG; ++n)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], d));
+            for (int e = 0; e < 2; ++e) {
+              float top = fmaxf(s[n][e], s[n][2 + e]);
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float top = fmaxf(m[n][e], mx[e]);
-            base_m[e] = top == -INFINITY ? 0.f : top;      // (keeps -inf - -inf out of the exponent)
-            corr[n][e] = fast_exp2(m[n][e] - base_m[e]);
-            grew |= corr[n][e] != 1.f;
-            m[n][e] = top;
-          }
-          const float p0 = fast_exp2(s[n][0] - base_m[0]), p1 = fast_exp2(s[n][1] - base_m[1]);
-          const float p2 = fast_exp2(s[n][2] - base_m[0]), p3 = fast_exp2(s[n][3] - base_m[1]);
-          l[n][0] = l[n][0] * corr[n][0] + (p0 + p2);
-          l[n][1] = l[n][1] * corr[n][1] + (p1 + p3);
+              for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+              if (!(top > m[n][e] + kGrowth)) continue;
+              const float corr = fast_exp2(m[n][e] - top);                       // (0 for the first)
+              m[n][e] = top, l[n][e] *= corr;
+#pragma unroll
+              for (int c = 0; c < HD / 16; ++c) o[n][c][e] *= corr, o[n][c][2 + e] *= corr;
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+          // (-inf - -inf is no number)
+          const float base0 = m[n][0] == -INFINITY ? 0.f : m[n][0], base1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
+          const float p0 = fast_exp2(s[n][0] - base0), p1 = fast_exp2(s[n][1] - base1);
+          const float p2 = fast_exp2(s[n][2] - base0), p3 = fast_exp2(s[n][3] - base1);
+          l[n][0] += p0 + p2;
+          l[n][1] += p1 + p3;
           // (weights are rounded to bfloat16 for the product, as everywhere in this package; their sum is not)
           if constexpr (sizeof(T) == 2) {
             b0[n] = transposed(pack_bf16(p0, p1));
@@ -395,13 +422,6 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
           } else {
             w[n][0] = p0, w[n][1] = p1, w[n][2] = p2, w[n][3] = p3;
           }
-        }
-        if (__any_sync(0xffffffffu, grew)) {
-#pragma unroll
-          for (int n = 0; n < NG; ++n)
-#pragma unroll
-            for (int c = 0; c < HD / 16; ++c)
-              o[n][c][0] *= corr[n][0], o[n][c][1] *= corr[n][1], o[n][c][2] *= corr[n][0], o[n][c][3] *= corr[n][1];
         }
         if constexpr (sizeof(T) == 2) {
 #pragma unroll
@@ -524,8 +544,8 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
   asm volatile("cp.async.wait_all;" ::: "memory");
   if (!FAR && p.joined) {
     pdl_trigger();
-    // the joining kernel waits for this launch alone: its last block ends behind the one that ran beside it
-    if (p.after && blockIdx.x == gridDim.x - 1) pdl_wait();
+    // the joining kernel waits for this launch alone: its first block ends behind the one that ran beside it
+    if (p.after && blockIdx.x == 0) pdl_wait();
   }
 }
 

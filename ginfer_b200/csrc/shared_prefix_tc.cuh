@@ -46,7 +46,7 @@ struct Args {
   Shape shape, own_shape;      // rows of this kernel's tiles, of the one's that works on own tokens beside it
   int H, own_H, places, oob_row, sms, own_tile;
   float cost;                  // of a tile beside one of own tokens
-  int* chunk;
+  FarPlan* far_plan;           // [G]
   float* far_o;                // [places][QT][HD]
   float2* far_ml;
   int* err;
@@ -117,8 +117,8 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
     bars->groups[lane] = t;
     if (lane == 0) {
       bars->chunk = chunk, bars->workers = workers;
-      if (blockIdx.x == 0) *g.chunk = chunk;
     }
+    if (blockIdx.x == 0) write_far_plan(a, t, g.H, g.shape.tokens, KT, chunk, g.far_plan);
   }
   // rows that no token fills are zeros, so that their scores are numbers
   for (int i = box_rows * 8 + threadIdx.x; i < QT * 8; i += NTHREADS_TC)
@@ -429,7 +429,10 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
 #pragma unroll
           for (int k = 0; k < 16; ++k) x[k] = two ? fmaf(y[k], f1, x[k] * f0) : x[k] * f0;
 #pragma unroll
-          for (int k = 0; k < 16; k += 4) *reinterpret_cast<float4*>(to + cc + k) = make_float4(x[k], x[k + 1], x[k + 2], x[k + 3]);
+          for (int k = 0; k < 16; k += 8)            // (a whole sector a thread)
+            asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to + cc + k), "f"(x[k]), "f"(x[k + 1]),
+                         "f"(x[k + 2]), "f"(x[k + 3]), "f"(x[k + 4]), "f"(x[k + 5]), "f"(x[k + 6]), "f"(x[k + 7])
+                         : "memory");
         }
       }
       ++seq;

@@ -533,7 +533,7 @@ GF_DEFINE_PDL_SWITCH
 
 // What a tile of a prefix costs beside a tile of own tokens (which come from memory): 128 keys on the tensor cores with up to 128
 // rows, 64 keys on mma.sync with up to 64 rows.
-constexpr float kTensorCost = 6.f, kPlainCost = 6.f;
+constexpr float kTensorCost = 8.f, kPlainCost = 4.f;
 // Tables of up to this many tokens in all are a block's work an item.
 constexpr int kShortKeys = 512;
 
@@ -601,7 +601,7 @@ struct Call {
     p.row_o = (float*)take(rows * HD * 4), p.row_ml = (float2*)take(rows * 8);
     j.far_rows = tensor ? 128 : half ? MOST_ROWS : 8 * most;
     p.far_shape = row_shape_of(a.nh, a.nkv, j.far_rows), p.far_tile = tensor ? 128 : half ? TILE : keys, p.far_H = a.nkv * p.far_shape.chunks;
-    p.far_cost = getenv("GF_COST") ? (float)atof(getenv("GF_COST")) : tensor ? kTensorCost : half ? kPlainCost : 1.f;
+    p.far_cost = tensor ? (getenv("GF_COST") ? (float)atof(getenv("GF_COST")) : kTensorCost) : half ? (getenv("GF_COST2") ? (float)atof(getenv("GF_COST2")) : kPlainCost) : (getenv("GF_COST3") ? (float)atof(getenv("GF_COST3")) : 1.f);
     const long long tiles = (long long)p.far_H * ((a.T + p.far_shape.tokens - 1) / p.far_shape.tokens + a.G);
     const long long least = 4ll * p.sms * (tensor ? 1 : half ? BLOCKS_AN_SM : warps);
     j.places = (int)(tiles > least ? tiles : least);

@@ -138,11 +138,13 @@ __device__ __forceinline__ FarWork far_work(const PrefixArgs& a, GroupTiles& t, 
   }
   return w;
 }
+// A row's pieces are read one after the other when they are joined: no prefix is cut into more chunks than this.
+constexpr int kMostSplits = 24, kMostSplitsOfWarps = 64;      // (by blocks, by single warps)
 // Tiles of a chunk of keys, by one warp.  With `workers` blocks the time is about (rounds of items) * (chunk + over),
 // over: what an item's start and end cost in tiles.  Looked at are the 32 lengths from one, a half and a third of an equal share
 // on; the longest prefix, which is always possible, is the last resort.
 __device__ __forceinline__ int plan_chunk(const PrefixArgs& a, const GroupTiles& first, const FarWork& all, int H, int tokens, int tile,
-                                          int workers, int places, int over) {
+                                          int workers, int places, int over, int most_splits = kMostSplits) {
   const int lane = threadIdx.x & 31;
   if (all.most == 0) return 1;
   GroupTiles t = first;
@@ -151,7 +153,7 @@ __device__ __forceinline__ int plan_chunk(const PrefixArgs& a, const GroupTiles&
 #pragma unroll
   for (int k = 0; k < 3; ++k) {
     const long long share = quotient(all.units + (long long)workers * (k + 1) - 1, (long long)workers * (k + 1));
-    const int from = (int)(share < all.most ? share : all.most);
+    const int from = max((int)(share < all.most ? share : all.most), (all.most + most_splits - 1) / most_splits);
     len[k] = min(all.most, max(1, from) + lane * max(1, from / 48));
   }
   if (lane == 31) len[0] = all.most;
@@ -250,10 +252,16 @@ struct Request {
 };
 __device__ __forceinline__ Request request_of(const PrefixArgs& a, int b, bool both, int tile) {
   Request r;
+  r.g = -1, r.shared = 0;
+  if (both && a.G == 1) {
+    // (one group: nothing waits for anything)
+    const int length = prefix_length(a, 0);
+    const bool in = !a.cu_groups || (fresh_index(a.cu_groups) <= b && b < fresh_index(a.cu_groups + 1));
+    r.g = in ? 0 : -1, r.shared = in ? length : 0;
+  }
   const Rows rows = rows_of(a, b);
   r.first = rows.first, r.count = rows.count, r.len = own_length(a, b);
-  r.g = both ? group_of(a, b) : -1;
-  r.shared = prefix_length(a, r.g);
+  if (both && a.G > 1) r.g = group_of(a, b), r.shared = prefix_length(a, r.g);
   r.far = (r.shared + tile - 1) / tile, r.near = (r.len + tile - 1) / tile;
   return r;
 }
@@ -261,6 +269,7 @@ __device__ __forceinline__ Request request_of(const PrefixArgs& a, int b, bool b
 struct Cursor {
   int hc, b, rt, off;
   long long todo;
+  Request req;
 };
 // What the joining kernel needs of the division: a run's units, the units of one (kv head, chunk of heads), and of every request
 // the units before it, its rows, its tiles and its group.
@@ -310,15 +319,24 @@ __device__ __forceinline__ OwnWork own_work(const PrefixArgs& a, int tokens, int
   }
   return w;
 }
-// The runs of the WARPS warps of block `k` of `blocks`; all threads call.  `plan`: where the division is written down, by the block
-// that is given it.
-template <int THREADS, int WARPS>
-__device__ __forceinline__ void find_runs(const PrefixArgs& a, const OwnWork& w, int H, int tokens, int tile, bool both, int k,
-                                          int blocks, OwnPlan* plan, Cursor* found) {
-  if (threadIdx.x < WARPS) found[threadIdx.x].todo = 0;
+// What the threads that counted leave for the warps' searches.
+template <int THREADS> struct OwnShares {
+  long long start[THREADS + 1];
+  Request first[THREADS];
+};
+// The run of warp `me` of `runs` of them, by that warp; all threads of the block call.  `plan`: where the division is written down, by
+// the block that is given it.
+template <int THREADS>
+__device__ __forceinline__ Cursor find_run(const PrefixArgs& a, const OwnWork& w, OwnShares<THREADS>& shares, int H, int tokens,
+                                           int tile, bool both, long long me, long long runs, OwnPlan* plan) {
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x < THREADS) {
+    shares.start[threadIdx.x] = w.start, shares.first[threadIdx.x] = w.first;
+    if (threadIdx.x == 0) shares.start[THREADS] = w.total;
+  }
   __syncthreads();
-  const long long all = w.total * H, runs = (long long)blocks * WARPS, share = quotient(all + runs - 1, runs);
-  const long long run = share > kLeastRun ? share : kLeastRun;
+  const long long all = w.total * H, share = quotient(all + runs - 1, runs);
+  const long long run = share > kLeastRun ? share : kLeastRun, at = run * me;
   if (plan && threadIdx.x < THREADS) {
     if (threadIdx.x == 0) plan->run = run, plan->each = w.total;
     long long base = w.start;
@@ -328,27 +346,31 @@ __device__ __forceinline__ void find_runs(const PrefixArgs& a, const OwnWork& w,
       base += (long long)r.row_tiles(tokens) * r.units();
     }
   }
-  if (k < blocks && threadIdx.x < THREADS && w.mine > 0) {
-    long long hc_units = -1, hc = 0;
-    for (int i = 0; i < WARPS; ++i) {
-      const long long at = run * ((long long)k * WARPS + i);
-      if (at >= all) break;
-      if (hc_units < 0 || at >= hc_units + w.total) hc = quotient(at, w.total), hc_units = hc * w.total;
-      long long rest = at - hc_units - w.start;
-      if (rest < 0 || rest >= w.mine) continue;
-      for (int b = w.b0; b < w.b1; ++b) {
-        const Request r = w.request(a, b, both, tile);
-        const long long units = r.units(), here = r.row_tiles(tokens) * units;
-        if (rest < here) {
-          const int rt = (int)quotient(rest, units);
-          found[i] = {(int)hc, b, rt, (int)(rest - rt * units), min(run, all - at)};
-          break;
-        }
-        rest -= here;
-      }
-    }
+  Cursor c{};
+  if (me >= runs || at >= all) return c;
+  c.hc = (int)quotient(at, w.total);
+  long long rest = at - c.hc * w.total;
+  // the thread that counted the request
+  int who = 0;
+#pragma unroll
+  for (int j = 0; j < THREADS / 32; ++j) {
+    const unsigned hit = __ballot_sync(0xffffffffu, shares.start[32 * j + lane] <= rest && rest < shares.start[32 * j + lane + 1]);
+    if (hit) who = 32 * j + __ffs(hit) - 1;
   }
-  __syncthreads();
+  rest -= shares.start[who];
+  const int each = (a.B + THREADS - 1) / THREADS;
+  c.b = who * each, c.req = shares.first[who];
+  for (;;) {
+    const long long units = c.req.units(), here = c.req.row_tiles(tokens) * units;
+    if (rest < here || c.b + 1 >= a.B) {
+      c.rt = (int)quotient(rest, units), c.off = (int)(rest - c.rt * units);
+      break;
+    }
+    rest -= here;
+    c.req = request_of(a, ++c.b, both, tile);
+  }
+  c.todo = min(run, all - at);
+  return c;
 }
 
 // Prefixes and own tokens are worked on side by side, by two launches: of `sms` SMs this many have the prefixes.  A tile of a

@@ -135,7 +135,7 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
   extern __shared__ __align__(1024) unsigned char raw[];
   unsigned char* base = raw + ((0u - smem_u32(raw)) & 1023u);               // (a swizzle counts from 1 KB)
   __shared__ long long counts[4];
-  __shared__ Cursor found[WARPS];
+  __shared__ OwnShares<COUNTING> shares;
   __shared__ int far_s, chunk_s;
   __shared__ GroupTiles groups_s[FAR ? 32 : 1];
   const PrefixArgs& a = p.a;
@@ -147,7 +147,9 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (!p.after) pdl_wait();
-  if (FAR) pdl_trigger();      // (behind the wait: the kernel beside this one reads what was waited for)
+  // FAR: behind the wait, since the kernel beside this one reads what was waited for.  Else the joining kernel's blocks may stand
+  // by: every block of this one is running by then.
+  if (FAR || p.joined) pdl_trigger();
   Cursor cur{};
   Request req{};
   GroupTiles groups{};
@@ -159,7 +161,7 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
     const OwnWork w = own_work<COUNTING>(a, p.own_shape.tokens, KEYS, false, counts);
     if (warp == WARPS - 1) {
       const int workers = far_share(p.sms, f.units, p.far_cost, w.total * p.own_H) * WARPS;
-      const int c = plan_chunk(a, groups, f, p.H, p.shape.tokens, KEYS, max(workers, 1), p.places, kItemTiles);
+      const int c = plan_chunk(a, groups, f, p.H, p.shape.tokens, KEYS, max(workers, 1), p.places, kItemTiles, kMostSplitsOfWarps);
       groups_s[lane] = groups;
       if (lane == 0) {
         chunk_s = c, far_s = workers;
@@ -179,11 +181,11 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
     if (threadIdx.x == THREADS - 1) far_s = p.after ? far_share(p.sms, f.units, p.far_cost, w.total * p.H) : 0;
     __syncthreads();
     const int blocks = p.after ? max(p.sms - far_s, 1) : (int)gridDim.x;
-    find_runs<COUNTING, WARPS>(a, w, p.H, p.shape.tokens, KEYS, p.both, blockIdx.x, blocks, blockIdx.x == 0 ? p.plan : nullptr, found);
-    cur = found[warp];
-    if (cur.todo > 0) req = request_of(a, cur.b, p.both, KEYS);
+    cur = find_run<COUNTING>(a, w, shares, p.H, p.shape.tokens, KEYS, p.both, (long long)blockIdx.x * WARPS + warp,
+                             (long long)blocks * WARPS, blockIdx.x == 0 ? p.plan : nullptr);
+    req = cur.req;
   } else {
-    cur = {(int)blockIdx.z, (int)blockIdx.y, (int)blockIdx.x, 0, 0};
+    cur = {(int)blockIdx.z, (int)blockIdx.y, (int)blockIdx.x, 0, 0, {}};
     req = request_of(a, cur.b, p.both, KEYS);
     __syncthreads();
   }
@@ -193,7 +195,7 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
   const bool tma = G::SWIZZLED && p.tma;
   uint64_t once;
   asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(once));
-  uint32_t phases = 0;         // a bit a stage
+  uint32_t phases = 0, written = 0;      // a bit a stage; written: by cp.async
   int st = 0;
   bool ok = true;
   // the next piece of this warp's run (or its share of the block's item)
@@ -264,7 +266,10 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
       uint64_t* bar = &full[stage_i];
       if (tma && k.key0 + KEYS <= k.end) {
         // (what this warp's cp.async wrote there is out of the way of the copies)
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        if (written >> stage_i & 1) {
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          written &= ~(1u << stage_i);
+        }
         if (lane == 0)
           asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(STAGE) : "memory");
         else
@@ -288,19 +293,15 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
           cp_async16(stage + G::place(1, row, ch), vp + off, there);
         }
         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+        written |= 1u << stage_i;
       }
     };
     int slot = 0;
     if (!ok) x.count = 0;      // (behind a wait that ran out: the warps still meet where they join)
-    {
-      int first[STAGES];
+    int first[STAGES];
 #pragma unroll
-      for (int i = 0; i < STAGES; ++i) first[i] = i < x.count ? look(i) : 0;
-      if (STAGES < x.count) slot = look(STAGES);
-#pragma unroll
-      for (int i = 0; i < STAGES; ++i)
-        if (i < x.count) issue(i, first[i], (st + i) % STAGES);
-    }
+    for (int i = 0; i < STAGES; ++i) first[i] = i < x.count ? look(i) : 0;
+    if (STAGES < x.count) slot = look(STAGES);
     // ---- q as the 8-column operand: thread (g, t) has of row 8 ng + g the channels 16 kc + 2t, + 1 and + 8, + 9 (bfloat16), or
     // 8 kc + t and + 4 (32 bits)
     uint32_t qf[NG][sizeof(T) == 2 ? KCH : 2 * KCH][2];
@@ -325,6 +326,9 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
 #pragma unroll
       for (int e = 0; e < 2; ++e) see[n][e] = 8 * n + 2 * t + e < rows ? x.last + (8 * n + 2 * t + e) / heads : 0x7fffffff;
     }
+#pragma unroll
+    for (int i = 0; i < STAGES; ++i)
+      if (i < x.count) issue(i, first[i], (st + i) % STAGES);
     float o[NG][HD / 16][4], m[NG][2], l[NG][2];
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
@@ -348,12 +352,21 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
 #pragma unroll
         for (int n = 0; n < NG; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
         if constexpr (sizeof(T) == 2) {
+          // (few groups: two sums of every other 16 channels, half as long a chain of products)
+          constexpr int SUMS = NG <= 2 && KCH > 1 ? 2 : 1;
+          float part[NG][4] = {};
 #pragma unroll
           for (int kc = 0; kc < KCH; ++kc) {
             uint32_t af[4];
             ldsm_x4(af, stage + G::place(0, sub * 16 + (lane & 15), kc * 16 + (lane >> 4) * 8));
 #pragma unroll
-            for (int n = 0; n < NG; ++n) mma16816(s[n], af, qf[n][kc][0], qf[n][kc][1]);
+            for (int n = 0; n < NG; ++n) mma16816(kc % SUMS ? part[n] : s[n], af, qf[n][kc][0], qf[n][kc][1]);
+          }
+          if constexpr (SUMS == 2) {
+#pragma unroll
+            for (int n = 0; n < NG; ++n)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) s[n][i] += part[n][i];
           }
         } else {
 #pragma unroll
@@ -543,7 +556,6 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
     for (int i = 0; i < STAGES; ++i) wait_bar(&full[i], (phases >> i) & 1u, p.err, 23);
   asm volatile("cp.async.wait_all;" ::: "memory");
   if (!FAR && p.joined) {
-    pdl_trigger();
     // the joining kernel waits for this launch alone: its first block ends behind the one that ran beside it
     if (p.after && blockIdx.x == 0) pdl_wait();
   }

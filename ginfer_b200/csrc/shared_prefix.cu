@@ -5,8 +5,6 @@
 #define GF_HEAD_DIM 128
 #endif
 
-#include <cstdlib>
-
 #include "attention_tc.cuh"
 #include "mma_bits.cuh"
 #include "shared_prefix.cuh"
@@ -531,11 +529,25 @@ using namespace gf;
 
 GF_DEFINE_PDL_SWITCH
 
-// What a tile of a prefix costs beside a tile of own tokens (which come from memory): 128 keys on the tensor cores with up to 128
-// rows, 64 keys on mma.sync with up to 64 rows.
-constexpr float kTensorCost = 8.f, kPlainCost = 4.f;
-// Tables of up to this many tokens in all are a block's work an item.
-constexpr int kShortKeys = 512;
+// Which way a call goes, by its sizes alone (the tables' widths, not the lengths in them).
+//
+// Direct: a block an item (request, kv head), whose warps share the keys of prefix and own tokens; one launch.  Where a
+// request's tables hold at most kDirectKeys bytes of keys of a kv head, and requests read at most kDirectBytes of prefixes.
+// Direct / equal runs and their join, us: 28 heads on 4 of 128, one request of 500 tokens 8.7 / 17.1, of 1,000 13.1 / 17.2; 64 of
+// 1,000 26.5 / 27.3, of 2,000 42.0 / 41.3; 14 on 2 of 64, 64 of 1,000 9.6 / 19.1, of 2,000 13.3 / 20.1; those in fp32 22.0 / 28.8, 38.3 / 41.2.
+constexpr long long kDirectKeys = 256 << 10, kDirectBytes = 128 << 20;
+// Unshared: every request reads its prefix itself (from L2 but for the first), in equal runs.  Where that is at most so many
+// bytes; 2 launches instead of 3.  Unshared / shared, us: 28 on 4 of 128, 8 requests behind 1,000 tokens (16 MB) 19.0 / 21.8, 16 of
+// 1,000 (33 MB) 19.5 / 22.5, 8 of 4,000 (66 MB) 22.7 / 25.4, 64 of 1,000 (131 MB) 30.4 / 27.9, 8 of 16,000 (262 MB) 45 / 28; 14 on 2 of
+// 64, 8 of 4,000 (16 MB) 20.2 / 23.6, 8 of 16,000 (66 MB) 28.3 / 24.4; 16 on 4 of 96, 8 of 1,000 (12 MB) 19.0 / 21.2, 4 of 8,000 (49 MB) 27.0 / 23.8.
+// fp32, 14 on 2 of 64: 16 of 1,000 (16 MB) 27.6 / 29.4, 64 of 2,000 (131 MB) 43.4 / 40.4, 128 of 4,000 (524 MB) 127 / 100.  In 32 bits with heads
+// above 64 registers leave 8 rows a tile, with or without groups: 28 on 4 of 128, 128 of 4,000, 543 unshared, 785 shared; so not at all there.
+constexpr long long kUnsharedBytes = 48 << 20, kUnsharedBytes32 = 128 << 20;
+// What a tile of a prefix costs beside a tile of own tokens (which come from memory), for the SMs' shares: 128 keys on the
+// tensor cores with up to 128 rows, 64 keys on mma.sync with up to 64 rows, 16 keys in 32 bits.  By the first, us: 256 requests behind
+// 32,768 tokens 322 at 6, 287 at 8, 291 at 10, 381 at 15; 64 behind 8,192 46, 38, 41, 45.  By the second, 24 requests behind two
+// prompts of 96-wide heads: 30.0 at 2, 29.5 at 4, 30.8 at 6.  By the third, 39.3 at 0.5 and at 1, 39.7 at 2.5.
+constexpr float kTensorCost = 8.f, kPlainCost = 4.f, kCost32 = 1.f;
 
 // `words`: q, its row stride and type, k, v, pages, page, prefix_table and its stride, prefix_lens, groups, prefix limit,
 // table and its stride, lengths, requests, limit, cu_groups, cu, out, rows, heads, kv heads, SMs, the rows that a request has
@@ -545,7 +557,7 @@ struct Call {
   JoinArgs j;
   FarArgs f;
   int type, longest, groups;
-  bool shared, tensor, direct; // tensor: prefixes on the 5th-generation tensor cores; direct: one launch, nothing to join
+  bool shared, tensor, direct; // tensor: prefixes on the 5th-generation tensor cores
   char* scratch;
   long long room, need;
   cudaStream_t stream;
@@ -571,19 +583,17 @@ struct Call {
     a.hd = HD;
     a.page_shift = (a.page & (a.page - 1)) == 0 ? 31 - __builtin_clz(a.page) : -1;
     if (longest < 1) longest = 1;
-    // groups of 8 rows: as many as a request has, or the registers hold
     const bool half = type == GF_BF16;
-    const int most = half ? own::kMostGroups<bf16> : own::kMostGroups<float>;
-    const long long wanted = (long long)longest * (a.nh / a.nkv);
-    groups = wanted <= 8 || most == 1 ? 1 : wanted <= 16 || most == 2 ? 2 : 4;
+    groups = half && (long long)longest * (a.nh / a.nkv) > own::kOneGroup ? own::kNearGroups<bf16> : 1;
     const int keys = half ? own::Tile<bf16>::KEYS : own::Tile<float>::KEYS, warps = half ? own::Tile<bf16>::WARPS : own::Tile<float>::WARPS;
     p.rows = 8 * groups;
     p.shape = row_shape_of(a.nh, a.nkv, p.rows);
     p.H = a.nkv * p.shape.chunks;
-    const char* env = getenv("GF_SHORT");
-    const char* env2 = getenv("GF_UNSHARED");
-    direct = a.prefix_limit + a.limit <= (env ? atoi(env) : kShortKeys) && a.B <= 65535 && p.H <= 65535;
-    shared = !direct && a.G > 0 && a.prefix_limit > 0 && a.T > (env2 ? atoi(env2) : 2);
+    const long long item = half ? 2 : 4, prefixes = (long long)a.B * a.prefix_limit * a.nkv * HD * 2 * item;
+    const bool any = a.G > 0 && a.prefix_limit > 0;
+    direct = ((any ? a.prefix_limit : 0ll) + a.limit) * HD * item <= kDirectKeys && (!any || prefixes <= kDirectBytes) &&
+             a.B <= 65535 && p.H <= 65535;
+    shared = !direct && any && (half ? prefixes > kUnsharedBytes : own::kFarGroups > 0 && prefixes > kUnsharedBytes32);
     p.both = !shared, p.joined = !direct, p.after = shared;
     // the scratch: the division, pieces of cut items, of rows, of prefixes
     need = 0;
@@ -599,9 +609,9 @@ struct Call {
     if (!shared) return;
     tensor = GF_PREFIX_TC && half && a.page % 8 == 0 && 128 % a.page == 0;
     p.row_o = (float*)take(rows * HD * 4), p.row_ml = (float2*)take(rows * 8);
-    j.far_rows = tensor ? 128 : half ? MOST_ROWS : 8 * most;
+    j.far_rows = tensor ? 128 : half ? MOST_ROWS : 8 * own::kFarGroups;
     p.far_shape = row_shape_of(a.nh, a.nkv, j.far_rows), p.far_tile = tensor ? 128 : half ? TILE : keys, p.far_H = a.nkv * p.far_shape.chunks;
-    p.far_cost = tensor ? (getenv("GF_COST") ? (float)atof(getenv("GF_COST")) : kTensorCost) : half ? (getenv("GF_COST2") ? (float)atof(getenv("GF_COST2")) : kPlainCost) : (getenv("GF_COST3") ? (float)atof(getenv("GF_COST3")) : 1.f);
+    p.far_cost = tensor ? kTensorCost : half ? kPlainCost : kCost32;
     const long long tiles = (long long)p.far_H * ((a.T + p.far_shape.tokens - 1) / p.far_shape.tokens + a.G);
     const long long least = 4ll * p.sms * (tensor ? 1 : half ? BLOCKS_AN_SM : warps);
     j.places = (int)(tiles > least ? tiles : least);
@@ -631,10 +641,8 @@ static int launch_own(const own::Args& p, const CUtensorMap& mk, const CUtensorM
 }
 template <typename T>
 static int launch_near(const Call& c, const CUtensorMap& mk, const CUtensorMap& mv, dim3 grid) {
-  constexpr int most = own::kMostGroups<T>;
-  if (c.groups == 1) return launch_own<T, 1, false>(c.p, mk, mv, grid, c.stream);
-  if (c.groups == 2) return launch_own<T, most < 2 ? most : 2, false>(c.p, mk, mv, grid, c.stream);
-  return launch_own<T, most, false>(c.p, mk, mv, grid, c.stream);
+  return c.groups == 1 ? launch_own<T, 1, false>(c.p, mk, mv, grid, c.stream)
+                       : launch_own<T, own::kNearGroups<T>, false>(c.p, mk, mv, grid, c.stream);
 }
 
 GF_EXPORT int gf_prefix_attend(const char* words) {
@@ -671,10 +679,13 @@ GF_EXPORT int gf_prefix_attend(const char* words) {
     } else
 #endif
     if (!half) {
-      own::Args f = p;
-      f.shape = p.far_shape, f.H = p.far_H, f.rows = c.j.far_rows, f.own_shape = p.shape, f.own_H = p.H;
-      f.places = c.j.places, f.far_plan = c.f.far_plan, f.far_o = c.f.far_o, f.far_ml = c.f.far_ml, f.after = 0;
-      rc = launch_own<float, own::kMostGroups<float>, true>(f, ok, ov, dim3(p.sms), c.stream);
+      rc = -6;                   // (no call comes here without kFarGroups: see `shared`)
+      if constexpr (own::kFarGroups > 0) {
+        own::Args f = p;
+        f.shape = p.far_shape, f.H = p.far_H, f.rows = c.j.far_rows, f.own_shape = p.shape, f.own_H = p.H;
+        f.places = c.j.places, f.far_plan = c.f.far_plan, f.far_o = c.f.far_o, f.far_ml = c.f.far_ml, f.after = 0;
+        rc = launch_own<float, own::kFarGroups, true>(f, ok, ov, dim3(p.sms), c.stream);
+      }
     } else {
       static OncePerDevice attrs;
       rc = attrs.run([&] {

@@ -48,9 +48,14 @@ template <typename T> __host__ __device__ constexpr uint32_t smem_bytes(int ng) 
   const uint32_t ring = G::WARPS * G::STAGES * G::STAGE, exchange = G::WARPS * 8 * ng * (HD + 2) * 4;
   return (ring > exchange ? ring : exchange) + G::WARPS * G::STAGES * 8 + 1024;
 }
-// Groups of 8 rows at most: their results and their q have to fit the registers.
 constexpr float kGrowth = 8.f;   // log2 units: weights stay below 2^8
-template <typename T> constexpr int kMostGroups = HD <= 128 ? (sizeof(T) == 2 ? 4 : 2) : (sizeof(T) == 2 ? 2 : 1);
+// Groups of 8 rows at most, of own tokens and of prefixes (in 32 bits): their results and their q have to fit the registers, and
+// a tile's steps follow one another: 16 rows of q share what a warp reads, more rows are other warps' work, which reads it
+// again from L2.  32 requests of up to 5 rows, 12 heads on 2 kv heads of 128, us: 8 rows 41, 16 38, 32 50; 24 of up to 3, 16 on 4
+// of 96 (12 rows): 8 rows 31, 16 35; 32-bit, 12 of up to 2, 14 on 2 of 64 (14 rows): 8 rows 41, 16 48.
+template <typename T> constexpr int kNearGroups = sizeof(T) == 2 ? 2 : 1;
+constexpr int kOneGroup = 16;    // rows of a request up to which 8 are a tile
+constexpr int kFarGroups = HD <= 64 ? 2 : 0;
 
 struct Args {
   PrefixArgs a;
@@ -130,11 +135,11 @@ __global__ void __launch_bounds__(32 * Tile<T>::WARPS, 1)
 prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const Args p) {
   using G = Tile<T>;
   constexpr int KEYS = G::KEYS, WARPS = G::WARPS, STAGES = G::STAGES, THREADS = 32 * WARPS;
-  constexpr int COUNTING = THREADS < 128 ? THREADS : 128;
+  constexpr int COUNTING = THREADS;
   constexpr uint32_t STAGE = G::STAGE;
   extern __shared__ __align__(1024) unsigned char raw[];
   unsigned char* base = raw + ((0u - smem_u32(raw)) & 1023u);               // (a swizzle counts from 1 KB)
-  __shared__ long long counts[4];
+  __shared__ long long counts[WARPS];
   __shared__ OwnShares<COUNTING> shares;
   __shared__ int far_s, chunk_s;
   __shared__ GroupTiles groups_s[FAR ? 32 : 1];

@@ -36,7 +36,7 @@ struct Barriers {
   uint32_t tmem_base;
   int abort_flag, chunk, workers;
   GroupTiles groups[32];       // the first 32 groups'
-  long long own[4];
+  long long own[8];
   float stat_m[NS][QT], stat_l[NS][QT];
 };
 constexpr uint32_t SMEM = OPERAND * (1 + NS * KS + NS * VS) + sizeof(Barriers);
@@ -110,7 +110,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
   GroupTiles t{};
   FarWork f{};
   if (warp == 5) f = far_work(a, t, g.H, g.shape.tokens, KT);
-  const OwnWork own = own_work<128>(a, g.own_shape.tokens, g.own_tile, false, bars->own);
+  const OwnWork own = own_work<256>(a, g.own_shape.tokens, g.own_tile, false, bars->own);
   if (warp == 5) {
     const int workers = min((int)gridDim.x, far_share(g.sms, f.units, g.cost, own.total * g.own_H));
     const int chunk = plan_chunk(a, t, f, g.H, g.shape.tokens, KT, max(workers, 1), g.places, kOver);

@@ -3,11 +3,13 @@
 Tolerances.  bfloat16: a weight is rounded to 8 bits for the product with the values (off by 2^-8 of itself at most, so the result by 2^-8 of the largest value
 seen) and the result is rounded once (2^-8 of itself); scores and sums in 32 bits add 2e-5 of the largest value: scores of up to 32 are
 off by a few 2^-24 of that.  32 bits: those 2e-5 alone."""
+import threading
+
 import pytest
 import torch
 
 import plain_shared_prefix as plain
-from ginfer_b200.ops import shared_prefix
+from ginfer_b200.ops import _Counter, shared_prefix
 
 pytestmark = pytest.mark.gpu
 DEV, BF16, F32 = "cuda", torch.bfloat16, torch.float32
@@ -15,6 +17,31 @@ DEV, BF16, F32 = "cuda", torch.bfloat16, torch.float32
 
 def i32(x):
     return torch.as_tensor(x, dtype=torch.int32, device=DEV)
+
+
+WIDER = {"narrow": lambda c: (0, 0), "own": lambda c: (0, 4096), "prefix": lambda c: (_columns(c), 0)}
+
+
+def _columns(c):
+    """So many columns more that reading prefixes for each request looks expensive: 128 MB of them and a bit."""
+    _, _, page, nkv, hd = c["pages"].shape
+    return (130 << 20) // (max(1, len(c["lengths"])) * nkv * hd * 2 * c["pages"].itemsize * page) + 1
+
+
+@pytest.fixture(params=WIDER, autouse=True)
+def way(request, monkeypatch):
+    """How a call goes depends on its sizes, the tables' widths among them: every test with tables as wide as they need to be,
+    with wide ones of own tokens (runs over warps, joined) and with wide ones of prefixes (read once for a group)."""
+    monkeypatch.setitem(globals(), "wider_by", WIDER[request.param])
+    return request.param
+
+
+def wider_by(c):
+    return 0, 0
+
+
+def widen(table, by):
+    return torch.cat([table, table.new_full((table.shape[0], by), -1)], 1) if by else table
 
 
 def make_tables(counts, page, free, wider=0):
@@ -39,8 +66,11 @@ def make(dtype, nh, nkv, hd, page, prefix, own, new=None, groups=None, seed=0, w
     cu = None
     if new is not None:
         cu = i32([sum(new[:b]) for b in range(len(new) + 1)])
-    return dict(q=q, nh=nh, pages=pages, prefix_table=prefix_table, prefix_lens=i32(prefix), block_table=table,
-                lengths=i32(own), scale=hd ** -0.5, cu_groups=None if groups is None else i32(groups), cu=cu)
+    c = dict(q=q, nh=nh, pages=pages, prefix_table=prefix_table, prefix_lens=i32(prefix), block_table=table,
+             lengths=i32(own), scale=hd ** -0.5, cu_groups=None if groups is None else i32(groups), cu=cu)
+    for name, by in zip(("prefix_table", "block_table"), wider_by(c)):
+        c[name] = widen(c[name], by)
+    return c
 
 
 def call(c, **more):
@@ -183,9 +213,10 @@ def test_strides(dtype):
         q[:, :6 * 64] = c["q"][:, :6 * 64]
         check(call(dict(c, q=q)), dict(c, q=q))
         assert torch.equal(call(dict(c, q=q)), want)
+    P = c["prefix_table"].shape[1]
     table = torch.cat([c["prefix_table"].expand(3, -1), c["block_table"]], 1)
     pages = (c["pages"][0].clone(), c["pages"][1].clone())
-    got = call(dict(c, pages=pages, prefix_table=table[:1, :4], block_table=table[:, 4:]))
+    got = call(dict(c, pages=pages, prefix_table=table[:1, :P], block_table=table[:, P:]))
     assert torch.equal(got, want)
 
 
@@ -194,7 +225,7 @@ def test_entries_that_are_no_page(dtype):
     """Behind the lengths they are not read; within them the call stays inside the cache and the other requests' results stay."""
     c = make(dtype, 6, 2, 64, 16, [64], [40, 17, 33])
     want = call(c)
-    c["block_table"][1] = torch.tensor([1 << 30, -(1 << 30), 77], device=DEV, dtype=torch.int32)[:c["block_table"].shape[1]]
+    c["block_table"][1, :3] = i32([1 << 30, -(1 << 30), 77])
     got = call(c)
     assert torch.equal(got[0], want[0]) and torch.equal(got[2], want[2]) and torch.isfinite(got).all()
 
@@ -274,3 +305,56 @@ def test_far_into_a_large_cache():
     small = call(dict(c, prefix_table=c["prefix_table"] - (count - n), block_table=c["block_table"] - (count - n)))
     c["pages"] = pages
     assert torch.equal(call(c), small)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_ways(dtype, hd, way):
+    """One launch for short tables, two where every request reads its own prefix, three where groups read them together (in
+    32 bits only for heads of at most 64)."""
+    c = make(dtype, 8, 2, hd, 16, [77], [1, 30, 9], [1, 2, 1])
+    call(c)
+    before = _Counter.launches
+    check(call(c), c)
+    shared = 3 if dtype is BF16 or hd <= 64 else 2
+    assert _Counter.launches - before == {"narrow": 1, "own": 2, "prefix": shared}[way]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("hd", [64, 80])
+def test_many_groups(dtype, hd):
+    """More groups than a warp has lanes, more requests than a block has threads; groups of none, of one, of many."""
+    sizes = [(g * 5) % 13 for g in range(70)]
+    first = [2 + sum(sizes[:g]) for g in range(71)]
+    batch = first[-1] + 3
+    counts = [(b * 3) % 4 for b in range(batch)]
+    c = make(dtype, 6, 2, hd, 16, [(g * 37) % 300 for g in range(70)], [(b * 11) % 90 for b in range(batch)], counts, groups=first)
+    check(call(c), c)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("heads", [(14, 2, 64), (28, 4, 128)])
+def test_hints_that_are_wrong(dtype, heads):
+    c = make(dtype, *heads, 16, [290], [40, 9, 100, 64], [1, 9, 30, 2])
+    for hint in (0, 1, 2, 7, 100, 1 << 20):
+        check(call(c, max_q_len=hint), c)
+
+
+def test_threads_on_one_stream(way):
+    """Scratch memory is a stream's: calls of several threads on it follow one another whole."""
+    cs = [make(BF16, 28, 4, 128, 16, [1200 + 100 * i], [200 + i, 5] * 20, seed=i) for i in range(4)]
+    want = [call(c) for c in cs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        for _ in range(50):
+            if not torch.equal(call(cs[i]), want[i]):
+                wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong

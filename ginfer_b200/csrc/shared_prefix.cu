@@ -107,14 +107,16 @@ __device__ __forceinline__ void mma_step(const unsigned char* stage, int key, in
     corr[i] = fast_exp2(m[i] - base[i]);
     m[i] = top;
   }
+  // (weights are rounded to bfloat16 for the product, as everywhere in this package; what is summed are the rounded ones: a row
+  // that one key takes nearly all of gets its value as it is)
   float sum[2] = {0.f, 0.f};
+  uint32_t w[NT][2];
 #pragma unroll
   for (int j = 0; j < NT; ++j)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float w = fast_exp2(s[j][e] - base[e >> 1]);
-      s[j][e] = w;
-      sum[e >> 1] += w;
+    for (int i = 0; i < 2; ++i) {
+      w[j][i] = pack_bf16(fast_exp2(s[j][2 * i] - base[i]), fast_exp2(s[j][2 * i + 1] - base[i]));
+      sum[i] += __uint_as_float(w[j][i] << 16) + __uint_as_float(w[j][i] & 0xffff0000u);
     }
 #pragma unroll
   for (int i = 0; i < 2; ++i) l[i] = l[i] * corr[i] + sum[i];
@@ -124,18 +126,13 @@ __device__ __forceinline__ void mma_step(const unsigned char* stage, int key, in
   }
 #pragma unroll
   for (int kc = 0; kc < NT / 2; ++kc) {
-    // (weights are rounded to bfloat16 for the product, as everywhere in this package; their sum is not)
-    uint32_t w[4];
-    w[0] = pack_bf16(s[2 * kc][0], s[2 * kc][1]);
-    w[1] = pack_bf16(s[2 * kc][2], s[2 * kc][3]);
-    w[2] = pack_bf16(s[2 * kc + 1][0], s[2 * kc + 1][1]);
-    w[3] = pack_bf16(s[2 * kc + 1][2], s[2 * kc + 1][3]);
+    const uint32_t x[4] = {w[2 * kc][0], w[2 * kc][1], w[2 * kc + 1][0], w[2 * kc + 1][1]};
 #pragma unroll
     for (int n2 = 0; n2 < HD / 16; ++n2) {
       uint32_t b[4];
       ldsm_x4_t(b, stage + PLANE + place(key + kc * 16 + (mi & 1) * 8 + r, n2 * 16 + (mi >> 1) * 8));
-      mma16816(o[2 * n2], w, b[0], b[1]);
-      mma16816(o[2 * n2 + 1], w, b[2], b[3]);
+      mma16816(o[2 * n2], x, b[0], b[1]);
+      mma16816(o[2 * n2 + 1], x, b[2], b[3]);
     }
   }
 }

@@ -8,7 +8,8 @@
 // end: what lies there may be anything.
 //
 // In 32 bits both factors of a product are the sum of two tf32 numbers, 22 bits, and a product three of theirs (what is left out
-// is 2^-22 of it); sums are 32-bit.
+// is 2^-22 of it).  The instruction cuts its sums off instead of rounding them: it adds eight products up from zero, the long
+// sums are additions of their own.  (Left to the instruction, results were off by three times as much, heads of 256 by eight times.)
 #pragma once
 #include "shared_prefix.cuh"
 
@@ -334,10 +335,10 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
 #pragma unroll
     for (int i = 0; i < STAGES; ++i)
       if (i < x.count) issue(i, first[i], (st + i) % STAGES);
-    float o[NG][HD / 16][4], m[NG][2], l[NG][2];
+    float o[NG][HD / 16][4], m[NG][2], l[NG][4];
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
-      m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.f;
+      m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = l[n][2] = l[n][3] = 0.f;
 #pragma unroll
       for (int i = 0; i < HD / 16; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
     }
@@ -385,9 +386,12 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
 #pragma unroll
             for (int n = 0; n < NG; ++n) {
               const Split q0 = split(__uint_as_float(qf[n][kc][0])), q1 = split(__uint_as_float(qf[n][kc][1]));
-              mma_tf32(s[n], lo, q0.hi, q1.hi);
-              mma_tf32(s[n], hi, q0.lo, q1.lo);
-              mma_tf32(s[n], hi, q0.hi, q1.hi);
+              float y[4] = {};
+              mma_tf32(y, lo, q0.hi, q1.hi);
+              mma_tf32(y, hi, q0.lo, q1.lo);
+              mma_tf32(y, hi, q0.hi, q1.hi);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) s[n][i] += y[i];
             }
           }
         }
@@ -431,13 +435,16 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
           const float base0 = m[n][0] == -INFINITY ? 0.f : m[n][0], base1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
           const float p0 = fast_exp2(s[n][0] - base0), p1 = fast_exp2(s[n][1] - base1);
           const float p2 = fast_exp2(s[n][2] - base0), p3 = fast_exp2(s[n][3] - base1);
-          l[n][0] += p0 + p2;
-          l[n][1] += p1 + p3;
-          // (weights are rounded to bfloat16 for the product, as everywhere in this package; their sum is not)
+          // (weights are rounded to bfloat16 for the product, as everywhere in this package; what is summed are the rounded ones,
+          // by a product with ones: a row that one key takes nearly all of gets its value as it is)
           if constexpr (sizeof(T) == 2) {
+            const uint32_t ones[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
             b0[n] = transposed(pack_bf16(p0, p1));
             b1[n] = transposed(pack_bf16(p2, p3));
+            mma16816(l[n], ones, b0[n], b1[n]);
           } else {
+            l[n][0] += p0 + p2;
+            l[n][1] += p1 + p3;
             w[n][0] = p0, w[n][1] = p1, w[n][2] = p2, w[n][3] = p3;
           }
         }
@@ -471,9 +478,12 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
               }
 #pragma unroll
               for (int n = 0; n < NG; ++n) {
-                mma_tf32(o[n][c], lo, p0[n].hi, p1[n].hi);
-                mma_tf32(o[n][c], hi, p0[n].lo, p1[n].lo);
-                mma_tf32(o[n][c], hi, p0[n].hi, p1[n].hi);
+                float y[4] = {};
+                mma_tf32(y, lo, p0[n].hi, p1[n].hi);
+                mma_tf32(y, hi, p0[n].lo, p1[n].lo);
+                mma_tf32(y, hi, p0[n].hi, p1[n].hi);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[n][c][i] += y[i];
               }
             }
           }
@@ -487,12 +497,14 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
       st = st + 1 == STAGES ? 0 : st + 1;
     }
     // ---- the rows' results
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int n = 0; n < NG; ++n)
+      for (int n = 0; n < NG; ++n)
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
+        for (int e = 0; e < 2; ++e)
 #pragma unroll
-        for (int d = 4; d < 32; d <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], d);
+          for (int d = 4; d < 32; d <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], d);
+    }
     if (!p.joined) {
       // the block's warps have parts of the same item
       __syncthreads();

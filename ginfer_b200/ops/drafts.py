@@ -18,13 +18,15 @@ from .shared_prefix import _launching, _scratch_for
 
 PIECE = 1024                   # the least logits of a piece of a row (the library has the same number)
 _VERIFY = struct.Struct("=18q")
+_entry = None                  # the library's function, once it is loaded
 
 
 def _rows(x, rows, columns, what, device):
     """(address, row stride) of rows of logits."""
-    if x.shape != (rows, columns) or (x.stride(1) != 1 and columns > 1):
-        raise ValueError(f"{what} is [{rows}, {columns}], a row without gaps; got {tuple(x.shape)}, strides {tuple(x.stride())}")
-    return _at(x, device), x.stride(0)
+    strides = x.stride()
+    if x.shape != (rows, columns) or (strides[1] != 1 and columns > 1):
+        raise ValueError(f"{what} is [{rows}, {columns}], a row without gaps; got {tuple(x.shape)}, strides {strides}")
+    return _at(x, device), strides[0]
 
 
 def _vector(t, count, dtype, what, device):
@@ -52,9 +54,12 @@ def verify(logits: torch.Tensor, tokens: torch.Tensor, cu_rows: torch.Tensor, te
     running sum reaches ``u`` times the whole.  A temperature of zero or below: a draft stays if it is the arg-max
     (the lowest index among equals), and the next token is the arg-max.
 
-    A NaN counts as ``-inf``, logits of ``+inf`` share all of a row's weight.  Where nothing is left of ``p - q`` the next token is
-    drawn from ``p``, where nothing is left of that either it is the arg-max (0 in a row without a number).  A draft that is no
-    index of the vocabulary does not stay.  A request without rows has ``(0, -1)``."""
+    A weight below ``2^-120`` of its row's largest counts as none, a ``u`` outside of ``[0, 1)`` as the nearest number in it
+    (for the draw; a draft is compared with ``u`` as it is).  A NaN counts as ``-inf``, logits of ``+inf`` share all of a
+    row's weight.  Where nothing is left of ``p - q`` the next token is drawn from ``p``, where nothing is left of that either it is
+    the arg-max (0 in a row without a number).  A draft that is no index of the vocabulary does not stay.  A request without
+    rows has ``(0, -1)``."""
+    global _entry
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError(f"logits are [rows, vocabulary]; got {tuple(logits.shape)}")
     (R, V), code = logits.shape, _code(logits.dtype)
@@ -73,11 +78,13 @@ def verify(logits: torch.Tensor, tokens: torch.Tensor, cu_rows: torch.Tensor, te
              _vector(temperature, B, torch.float32, "temperature", dev), _vector(u, R, torch.float32, "u", dev))
     accepted = tokens.new_empty(2, B)
     stream, size, sms = _raw_stream(dev), 16 * R * (V // PIECE + 2), _of_device(dev)[0]
+    if _entry is None:
+        _entry = _function("drafts", "gf_verify")
     with _launching:
         scratch = _scratch_for(size, dev, stream)
-        rc = _function("drafts", "gf_verify")(_VERIFY.pack(*facts, accepted.data_ptr(), accepted.data_ptr() + 4 * B, R, V, B,
-                                                           scratch.data_ptr(), size, sms, stream))
+        rc = _entry(_VERIFY.pack(*facts, accepted.data_ptr(), accepted.data_ptr() + 4 * B, R, V, B, scratch.data_ptr(), size, sms,
+                                 stream))
     _Counter.launches += 2
     if rc:
         _ok(rc, "drafts.verify")
-    return accepted[0], accepted[1]
+    return accepted.unbind()

@@ -33,10 +33,13 @@ def supports(head_dim: int, heads: int, kv_heads: int) -> bool:
 
 def _table(t, count, what, device):
     """(address, row stride, columns) of a table of pages."""
-    if t.dtype is not _int32 or t.dim() != 2 or t.shape[0] != count or (t.stride(1) != 1 and t.shape[1] > 1):
-        raise ValueError(f"{what} is int32 [{count}, pages], its columns side by side; got {t.dtype} {tuple(t.shape)}, strides "
-                         f"{tuple(t.stride())}")
-    return _at(t, device), t.stride(0), t.shape[1]
+    shape, strides = t.shape, t.stride()
+    if t.dtype is not _int32 or len(shape) != 2 or shape[0] != count or (strides[1] != 1 and shape[1] > 1):
+        raise ValueError(f"{what} is int32 [{count}, pages], its columns side by side; got {t.dtype} {tuple(shape)}, strides "
+                         f"{strides}")
+    if count > 1 and strides[0] >= 1 << 31:
+        raise ValueError(f"{what}'s rows are {strides[0]} entries apart: fewer than 2^31")
+    return _at(t, device), strides[0] if count > 1 else 0, shape[1]
 
 
 def _vector(t, count, what, device):
@@ -87,8 +90,9 @@ def attend(q: torch.Tensor, nh: int, pages, prefix_table: torch.Tensor, prefix_l
     has at most (a hint: the kernels' tiles go by it; ``None``: ``T / B``).
 
     The ``i``-th of a request's ``n`` rows sees the whole prefix and the own tokens ``0 .. length - n + i``; a row that
-    sees nothing gives zeros.  Rows that belong to no request are not written: with ``out`` (``[T, nh * head size]``,
-    contiguous, ``q``'s type) they stay as they were.  Entries of the tables behind a sequence's length are not read."""
+    sees nothing gives zeros.  What a row sees is finite (an infinity there leaves no number); what none sees may be
+    anything.  Rows that belong to no request are not written: with ``out`` (``[T, nh * head size]``, contiguous, ``q``'s
+    type) they stay as they were.  Entries of the tables behind a sequence's length are not read."""
     # (what follows is the host's time of a call: a plane of its own would be two tensors made, a helper a call)
     if torch.is_tensor(pages):
         shape, dtype = pages.shape, pages.dtype
@@ -116,14 +120,15 @@ def attend(q: torch.Tensor, nh: int, pages, prefix_table: torch.Tensor, prefix_l
     if count < 1 or page < 1 or count * page >= 1 << 31:
         raise ValueError(f"{count} pages of {page} tokens: a cache has at least one, and slots are 32-bit integers")
     width = nh * hd
-    if q.dim() != 2 or q.dtype is not dtype or q.shape[1] < width or (q.stride(1) != 1 and q.shape[1] > 1):
+    shape, strides = q.shape, q.stride()
+    if len(shape) != 2 or q.dtype is not dtype or shape[1] < width or (strides[1] != 1 and shape[1] > 1):
         raise ValueError(f"q has rows of at least {width} channels without gaps in the cache's type {dtype}; got "
-                         f"{q.dtype} {tuple(q.shape)}, strides {tuple(q.stride())}")
-    at, stride = _at(q, dev), q.stride(0)
-    if (at | stride * q.itemsize) & 15 or stride < width:            # (the kernels read 16 bytes at a time)
+                         f"{q.dtype} {tuple(shape)}, strides {strides}")
+    at, stride = _at(q, dev), strides[0]
+    if (at | stride * q.itemsize) & 15 or not width <= stride < 1 << 31:            # (the kernels read 16 bytes at a time)
         q = q[:, :width].contiguous()
         at, stride = q.data_ptr(), width
-    T, B, G = q.shape[0], lengths.shape[0], prefix_lens.shape[0]
+    T, B, G = shape[0], lengths.shape[0], prefix_lens.shape[0]
     prefix, prefix_stride, P = _table(prefix_table, G, "prefix_table", dev)
     table, table_stride, W = _table(block_table, B, "block_table", dev)
     prefix_tokens, own_tokens = _vector(prefix_lens, G, "prefix_lens", dev), _vector(lengths, B, "lengths", dev)

@@ -65,6 +65,21 @@ def test_refusals(calls, changed, error):
     assert not calls
 
 
+def test_strides_beyond_32_bits(calls):
+    """Tables' rows that far apart are refused, q's made dense; of a single row the stride says nothing."""
+    far = torch.empty((1 << 32) + 512, device="meta")
+    table = torch.empty((1 << 32) + 5, dtype=torch.int32, device="meta")
+    with pytest.raises(ValueError, match="2\\^31"):
+        shared_prefix.attend(**good(block_table=table.as_strided((3, 4), (1 << 31, 1))))
+    with pytest.raises(ValueError, match="2\\^31"):
+        shared_prefix.attend(**good(prefix_table=table.as_strided((2, 5), (1 << 31, 1)), prefix_lens=i32(2), cu_groups=i32(3)))
+    assert not calls
+    shared_prefix.attend(**good(prefix_table=table.as_strided((1, 5), (1 << 32, 1))))
+    assert shared_prefix._ATTEND.unpack(calls[-1][2])[8] == 0
+    shared_prefix.attend(**good(q=far.as_strided((3, 256), (1 << 31, 1)), out=torch.zeros(3, 256)))
+    assert shared_prefix._ATTEND.unpack(calls[-1][2])[1] == 256
+
+
 def test_a_device_is_needed():
     with pytest.raises(RuntimeError, match="CUDA device"):
         shared_prefix.attend(**good())

@@ -173,7 +173,8 @@ template <typename T> __device__ __forceinline__ float group_max(const uint4& ra
   }
 }
 
-// A warp takes a piece after the other, the loads of the next one under way while it works on one.
+// A warp takes a piece after the other, the loads of the next one under way while it works on one.  Memory bounds it: 512 rows of
+// 152,064 logits in 32 bits, 311 MB, 55 us, 5.65 TB/s; 1,011 MB in bfloat16 191 us, 5.3 TB/s (twice the exponentials a byte).
 template <typename T>
 __global__ void __launch_bounds__(kScan, kScanBlocks) verify_scan_kernel(const VerifyArgs a) {
   __shared__ int starts[kSearch + 1];
@@ -603,6 +604,9 @@ __device__ __noinline__ int exactly_drawn(const VerifyArgs& a, Cluster& cl, doub
   return -1;
 }
 
+// Latency bounds it: a request's rows, its pieces' totals and its verdict take 4.6 us, a draw in 32 bits 8 more, one in 64 bits 30 to
+// 50 (64 requests of 152,064 logits: 85 us with 15 of them in 64 bits, 30 with none).  In 64 bits a row of two takes 38,000
+// weights of 40 instructions a block.
 template <typename T>
 __global__ void __launch_bounds__(kDecide, 3) verify_decide_kernel(const VerifyArgs a) {
   __shared__ Total totals[kBatch][2];                 // of the batch's rows: the target's, the draft's

@@ -25,7 +25,7 @@ constexpr int kScan = 256, kScanBlocks = 2;             // threads of a scanning
 constexpr int kSearch = 1024;                           // requests whose first rows a scanning block keeps
 constexpr int kDecide = 256, kWarps = kDecide / 32, kBatch = 32;      // rows whose sums are at hand at a time
 // Blocks of a request: 8 up to this many requests, else 4.  8 / 4, us, 64 requests of 4 drafts and 152,064 logits with a draft
-// model 139.5 / 180.2, 256 of 7 in bfloat16 392.5 / 381.6, 33 of 6 and 32,003 logits 43.8 / 51.5 (2 and 16 are slower everywhere).
+// model 139.5 / 180.2, 256 of 7 in bfloat16 392.5 / 381.6, 33 of 6 and 32,003 logits 43.8 / 51.5 (2, 5, 6 and 16 are slower).
 constexpr int kManyRequests = 128;
 constexpr int kAhead = 4;                               // loads of a row that are under way
 // Relative error that 32-bit sums may have: exponents are off by three roundings, 2^-24 each, of up to 20, and the exponential by
@@ -310,31 +310,38 @@ __device__ __forceinline__ double warp_total(double v) {
 }
 
 // Weights in 64 bits: 2^y for y = (x - best) log2(e) / T as 2^(n / kTable), n the nearest whole number to kTable y, from a
-// table, times the power series of 2^f, |f| <= 1 / (2 kTable), to the fifth power (what is cut off is below 4e-17).
-constexpr int kTable = 64;
-struct Exact {
+// table, times the power series of 2^f, |f| <= 1 / (2 kTable), to the sixth power (what is cut off is at most 4.4e-16 of it).
+// The table has as many entries as there are pairs of banks: a warp's look-ups never wait for one another.  INFINITE: for rows
+// whose largest logit is infinite; the others do without its comparisons.  (64 entries, the fifth power and the comparisons
+// everywhere: 139 us for 64 requests of 152,064 logits, 132 like this.)
+constexpr int kTable = 16;
+template <bool INFINITE> struct Exact {
   double c;                    // log2(e) / T
   float c32;
   const double* table;         // 2^(i / kTable)
   __device__ __forceinline__ Exact(float heat, const double* table_)
       : c(fmin(1.4426950408889634 / (double)heat, 1e30)), c32((float)c), table(table_) {}
-  // A logit's weight beside the row's largest one; below 2^-120 nothing.  (Without branches, so that several are under way.)
+  // A logit's weight beside the row's largest one; below 2^-120, and for a NaN, nothing.  (Without branches, so that several
+  // are under way.)
   __device__ __forceinline__ double operator()(float x, float best) const {
     constexpr double kShift = 6755399441055744.0 / kTable;           // 1.5 * 2^52 / kTable: n in the last bits
     const double d = (double)x - (double)best, at = fma(d, c, kShift), f = fma(d, c, -(at - kShift));
-    double p = fma(f, 0.0013333558146428443, 0.009618129107628477);  // ln(2)^k / k!
+    double p = fma(f, 0.00015403530393381608, 0.0013333558146428443);                  // ln(2)^k / k!
+    p = fma(p, f, 0.009618129107628477);
     p = fma(p, f, 0.055504108664821576);
     p = fma(p, f, 0.2402265069591007);
     p = fma(p, f, 0.6931471805599453);
     p = fma(p, f, 1.0);
     const int n = __double2loint(at);
     const double y = p * table[n & (kTable - 1)];
-    const double z = __hiloint2double(__double2hiint(y) + ((n >> 6) << 20), __double2loint(y));
-    // (a product that is no number: beside an infinity, or -inf at a temperature of infinity)
-    return x == best ? (x > -INFINITY ? 1. : 0.) : (x - best) * c32 >= -120.f ? z : 0.;
+    const double z = __hiloint2double(__double2hiint(y) + ((n >> 4) << 20), __double2loint(y));
+    // (the product is no number for a NaN and for -inf at a temperature of infinity)
+    const double w = (x - best) * c32 >= -120.f ? z : 0.;
+    if constexpr (INFINITE) return x == best ? (x > -INFINITY ? 1. : 0.) : w;
+    return w;
   }
 };
-static_assert(kTable == 64, "the shift above");
+static_assert(kTable == 16, "the shift above");
 
 // What a row's weights are relative to, and their sum.
 struct Total {
@@ -406,36 +413,53 @@ template <typename T> struct Draw {
     per = (b1 - b0 + kWarps - 1) / kWarps;
     w0 = min(b1, b0 + warp * per), w1 = min(b1, w0 + per);
   }
+  // Four of a group's logits: in 32 bits all of them.
+  static __device__ __forceinline__ void quarter(const uint4& raw, int h, float (&v)[4]) {
+    if constexpr (sizeof(T) == 4) {
+      unpack<T>(raw, v);
+    } else {
+      const uint32_t w0 = h ? raw.z : raw.x, w1 = h ? raw.w : raw.y;
+      v[0] = __uint_as_float(w0 << 16), v[1] = __uint_as_float(w0 & 0xffff0000u);
+      v[2] = __uint_as_float(w1 << 16), v[3] = __uint_as_float(w1 & 0xffff0000u);
+    }
+  }
   __device__ __forceinline__ void beside(int g, float (&z)[kVec<T>]) const {
 #pragma unroll
     for (int k = 0; k < kVec<T>; ++k) z[k] = y.at(g * kVec<T> - x.mis + k);
   }
-  // Calls f(group, logits, the draft's logits) for the groups g, g + 32, ... up to `end`.  LONG: f is long (64 bits), so that its
-  // code stands here once, with the next group's loads under way; else kAhead groups' are.
+  // Calls f(a logit's number, logits from there, the draft's logits) for the groups g, g + 32, ... up to `end`.  LONG: f is long (64
+  // bits) and knows what a NaN is: its code stands here once, for four logits at a time, with the next group's loads under way;
+  // else kAhead groups' are.
   template <bool LONG, typename F> __device__ __forceinline__ void each_group(int g, int end, F&& f) const {
     if constexpr (LONG) {
       uint4 rx{}, ry{};
       const bool both = with_draft && side_by_side;
-      if (g < end && x.whole(g)) rx = x.raw(g);
-      if (both && g < end && y.whole(g)) ry = y.raw(g);
+      auto fetch = [&](int h) {
+        if (h < end && x.whole(h)) {
+          rx = x.raw(h);
+          if (both) ry = y.raw(h);
+        }
+      };
+      fetch(g);
 #pragma unroll 1
       for (; g < end; g += 32) {
-        float v[kVec<T>], z[kVec<T>] = {};
-        if (x.whole(g)) {
-          unpack<T>(rx, v);
-          if (both) unpack<T>(ry, z);
-        } else {
-          x.load(g, v);
-          if (both) y.load(g, z);
+        if (!x.whole(g)) {
+          rx = x.pieced(g);
+          if (both) ry = y.pieced(g);
         }
-        if (with_draft && !both) beside(g, z);
-        if (g + 32 < end && x.whole(g + 32)) {
-          rx = x.raw(g + 32);
-          if (both) ry = y.raw(g + 32);
-        }
+        const uint4 vx = rx, vy = ry;
+        fetch(g + 32);
+#pragma unroll 1
+        for (int h = 0; h < kVec<T> / 4; ++h) {
+          const int j = g * kVec<T> - x.mis + 4 * h;
+          float v[4], z[4] = {};
+          quarter(vx, h, v);
+          if (both) quarter(vy, h, z);
+          else if (with_draft)
 #pragma unroll
-        for (int k = 0; k < kVec<T>; ++k) v[k] = fmaxf(v[k], -INFINITY), z[k] = fmaxf(z[k], -INFINITY);
-        f(g, v, z);
+            for (int k = 0; k < 4; ++k) z[k] = y.at(j + k);
+          f(j, v, z);
+        }
       }
     } else {
       Ahead<T> vx, vy;
@@ -449,7 +473,7 @@ template <typename T> struct Draw {
           vx.get(x, i, g + 32 * i, v);
           if (with_draft && side_by_side) vy.get(y, i, g + 32 * i, z);
           else if (with_draft) beside(g + 32 * i, z);
-          f(g + 32 * i, v, z);
+          f((g + 32 * i) * kVec<T> - x.mis, v, z);
         }
       }
     }
@@ -465,11 +489,11 @@ template <typename T> struct Draw {
     return t;
   }
   // Both rows' sums of weights in 64 bits.
-  __device__ __forceinline__ void totals(const Exact& e, double& P, double& Q) const {
+  template <bool INFINITE> __device__ __forceinline__ void totals(const Exact<INFINITE>& e, double& P, double& Q) const {
     double s0 = 0., s1 = 0., unused;
-    each_group<true>(w0 + (threadIdx.x & 31), w1, [&](int, const float (&v)[kVec<T>], const float (&z)[kVec<T>]) {
+    each_group<true>(w0 + (threadIdx.x & 31), w1, [&](int, const float (&v)[4], const float (&z)[4]) {
 #pragma unroll
-      for (int k = 0; k < kVec<T>; ++k) {
+      for (int k = 0; k < 4; ++k) {
         s0 += e(v[k], best);
         if (with_draft) s1 += e(z[k], draft_best);
       }
@@ -484,10 +508,10 @@ template <typename T> struct Draw {
   __device__ __forceinline__ int search(double u, const W& weight, double& total, double& target, double& low, double& high) const {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     double mine = 0., before, unused;
-    each_group<LONG>(w0 + lane, w1, [&](int g, const float (&v)[kVec<T>], const float (&z)[kVec<T>]) {
-      auto s = weight(v[0], z[0], g * kVec<T> - x.mis);
+    each_group<LONG>(w0 + lane, w1, [&](int j, const auto& v, const auto& z) {
+      auto s = weight(v[0], z[0], j);
 #pragma unroll
-      for (int k = 1; k < kVec<T>; ++k) s += weight(v[k], z[k], g * kVec<T> - x.mis + k);
+      for (int k = 1; k < (int)(sizeof(v) / sizeof(float)); ++k) s += weight(v[k], z[k], j + k);
       mine += (double)s;
     });
     const double block = block_total(mine, 0);
@@ -511,9 +535,10 @@ template <typename T> struct Draw {
     const int seg0 = min(b1, b0 + owner * per), seg1 = min(b1, seg0 + per), sub = (seg1 - seg0 + kWarps - 1) / kWarps;
     const int s0 = min(seg1, seg0 + warp * sub), s1 = min(seg1, s0 + sub);
     double part = 0.;
-    each_group<true>(s0 + lane, s1, [&](int g, const float (&v)[kVec<T>], const float (&z)[kVec<T>]) {
+    each_group<true>(s0 + lane, s1, [&](int j, const float (&v)[4], const float (&z)[4]) {
 #pragma unroll
-      for (int k = 0; k < kVec<T>; ++k) part += (double)weight(v[k], z[k], g * kVec<T> - x.mis + k);
+      for (int k = 0; k < 4; ++k)
+        part += (double)(LONG ? weight(v[k], z[k], j + k) : weight(fmaxf(v[k], -INFINITY), fmaxf(z[k], -INFINITY), j + k));
     });
     block_total(part, 1);
     const int finder = pick(1, before);
@@ -570,11 +595,11 @@ template <typename T> struct Draw {
 
 // In 64 bits, by the whole cluster.  (Out of line: what nearly every request needs keeps its registers.)
 // Whether u q(d) < p(d).
-template <typename T>
+template <typename T, bool INFINITE>
 __device__ __noinline__ bool exactly_stays(const VerifyArgs& a, Cluster& cl, double (*sums)[2], const double* tables, float heat,
                                            int row, float best, float draft_best) {
   const Draw<T> r(a, cl, sums, row, a.draft != nullptr, best, draft_best, -1);
-  const Exact e(heat, tables);
+  const Exact<INFINITE> e(heat, tables);
   const int d = fresh_index(a.tokens + row + 1);
   double P, Q;
   r.totals(e, P, Q);
@@ -582,11 +607,11 @@ __device__ __noinline__ bool exactly_stays(const VerifyArgs& a, Cluster& cl, dou
   return (double)fresh(a.u + row) * q < p;
 }
 // The token behind the drafts that stay, in the block that has it; -1 elsewhere.  `none`: the row has no weight at all.
-template <typename T>
+template <typename T, bool INFINITE>
 __device__ __noinline__ int exactly_drawn(const VerifyArgs& a, Cluster& cl, double (*sums)[2], const double* tables, float heat,
                                           int row, bool with_draft, float best, float draft_best, int d, double u, bool& none) {
   const Draw<T> r(a, cl, sums, row, with_draft, best, draft_best, d);
-  const Exact e(heat, tables);
+  const Exact<INFINITE> e(heat, tables);
   double P = 1., Q = 1., total = 0., target, low, high;
   if (with_draft) r.totals(e, P, Q);
   const double inv_p = P > 0. ? 1. / P : 0., inv_q = Q > 0. ? 1. / Q : 0.;
@@ -605,10 +630,11 @@ __device__ __noinline__ int exactly_drawn(const VerifyArgs& a, Cluster& cl, doub
 }
 
 // Latency bounds it: a request's rows, its pieces' totals and its verdict take 4.6 us, a draw in 32 bits 8 more, one in 64 bits 30 to
-// 50 (64 requests of 152,064 logits: 85 us with 15 of them in 64 bits, 30 with none).  In 64 bits a row of two takes 38,000
-// weights of 40 instructions a block.
+// 45 (64 requests of 152,064 logits: 78 us with 15 of them in 64 bits, 30 with none).  In 64 bits a request with a draft model takes
+// 38,000 weights a block and pass, which two warps a scheduler work on: instructions that are not there yet and waits for results
+// keep them at a third of its rate.  Blocks of 512 threads 149 us for the call, of 256 132; four a SM 139 (registers), two or three 132.
 template <typename T>
-__global__ void __launch_bounds__(kDecide, 3) verify_decide_kernel(const VerifyArgs a) {
+__global__ void __launch_bounds__(kDecide, 2) verify_decide_kernel(const VerifyArgs a) {
   __shared__ Total totals[kBatch][2];                 // of the batch's rows: the target's, the draft's
   __shared__ float drafted[kBatch][2];                // the logits that both give the draft
   __shared__ int places[kBatch];                      // greedy: the arg-max
@@ -734,7 +760,10 @@ __global__ void __launch_bounds__(kDecide, 3) verify_decide_kernel(const VerifyA
       in_batch = who, stop = i0 + who;
       if (what == 2) {
         make_tables();
-        if (exactly_stays<T>(a, cl, sums, tables, heat, rows.first + stop, totals[who][0].best, totals[who][1].best)) {
+        const Total* t = totals[who];
+        const bool infinite = t[0].best == INFINITY || (a.draft && t[1].best == INFINITY);
+        if (infinite ? exactly_stays<T, true>(a, cl, sums, tables, heat, rows.first + stop, t[0].best, t[1].best)
+                     : exactly_stays<T, false>(a, cl, sums, tables, heat, rows.first + stop, t[0].best, t[1].best)) {
           from = who + 1;
           continue;
         }
@@ -902,7 +931,9 @@ __global__ void __launch_bounds__(kDecide, 3) verify_decide_kernel(const VerifyA
   // ---- in 64 bits
   make_tables();
   bool none;
-  const int token = exactly_drawn<T>(a, cl, sums, tables, heat, row, with_draft, tp.best, tq.best, r.d, u, none);
+  const bool infinite = tp.best == INFINITY || tq.best == INFINITY;
+  const int token = infinite ? exactly_drawn<T, true>(a, cl, sums, tables, heat, row, with_draft, tp.best, tq.best, r.d, u, none)
+                             : exactly_drawn<T, false>(a, cl, sums, tables, heat, row, with_draft, tp.best, tq.best, r.d, u, none);
   if (token >= 0 && lane == 0) a.accepted[b] = stop, a.next[b] = token;
   if (none && cl.rank == 0 && threadIdx.x == 0) a.accepted[b] = stop, a.next[b] = 0;      // (a row without a number)
   cluster_sync();              // (nobody leaves while another reads its sums)

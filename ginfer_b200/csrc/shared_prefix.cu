@@ -5,6 +5,8 @@
 #define GF_HEAD_DIM 128
 #endif
 
+#include <climits>
+
 #include "attention_tc.cuh"
 #include "mma_bits.cuh"
 #include "shared_prefix.cuh"
@@ -413,7 +415,8 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS, HD <= 128 ? 4 : 3) prefix_joi
     if (!cut && both) continue;                          // (the row is written already)
     const int far_part = j.far_rows ? hh / far_shape.heads : 0;
     const int far_heads = j.far_rows ? min(far_shape.heads, each - far_part * far_shape.heads) : 1;
-    const int from = t - far_first, m = j.far_rows ? from / far_shape.tokens : 0;
+    // (starts that do not rise may put a row in front of its group's first: it has no piece there)
+    const int from = t - far_first, m = !j.far_rows ? 0 : from < 0 ? -1 : from / far_shape.tokens;
     // (the tensor cores' tiles leave room for the heads that a chunk may have, the others for those that it has)
     const int far_r = j.far_rows ? (from - m * far_shape.tokens) * (j.far_rows == 128 ? far_shape.heads : far_heads) + hh -
                                        far_part * far_shape.heads : 0;
@@ -615,10 +618,11 @@ struct Call {
     p.far_cost = tensor ? kTensorCost : half ? kPlainCost : kCost32;
     const long long tiles = (long long)p.far_H * ((a.T + p.far_shape.tokens - 1) / p.far_shape.tokens + a.G);
     const long long least = 4ll * p.sms * (tensor ? 1 : half ? BLOCKS_AN_SM : warps);
-    j.places = (int)(tiles > least ? tiles : least);
+    const long long places = tiles > least ? tiles : least;          // (beyond 2^31 there is no memory for them)
+    j.places = (int)(places < INT_MAX ? places : INT_MAX);
     FarPlan* far_plan = (FarPlan*)take((long long)sizeof(FarPlan) * a.G);
-    float* far_o = (float*)take((long long)j.places * j.far_rows * HD * 4);
-    float2* far_ml = (float2*)take((long long)j.places * j.far_rows * 8);
+    float* far_o = (float*)take(places * j.far_rows * HD * 4);
+    float2* far_ml = (float2*)take(places * j.far_rows * 8);
     j.far_plan = far_plan, j.far_o = far_o, j.far_ml = far_ml;
     f = FarArgs{a, 0, p.far_shape, p.shape, p.far_H, p.H, j.places, p.sms, keys, p.far_cost, far_plan, far_o, far_ml, p.err};
   }

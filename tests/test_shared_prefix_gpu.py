@@ -245,6 +245,29 @@ def test_numbers_that_are_none(dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_starts_that_do_not_rise(dtype, hd):
+    """A group's later requests may have rows in front of its first one's: they are no piece's.  The request behind is served."""
+    c = make(dtype, 6, 2, hd, 16, [64], [40, 17, 33], [5, 1, 2])
+    for cu in ([3, 1, 8, 8], [6, 0, 7, 8], [7, 2, 0, 8]):
+        out = torch.zeros(8, 6 * hd, dtype=dtype, device=DEV)
+        call(dict(c, cu=i32(cu)), out=out)
+    torch.cuda.synchronize()
+    check(call(c), c)
+
+
+def test_more_requests_than_a_grid_has_rows():
+    """70,000 requests are one call; halves of them, another way each, say the same."""
+    batch = 70000
+    c = make(F32, 4, 2, 16, 4, [9], [1 + b % 7 for b in range(batch)])
+    got = call(c)
+    half = batch // 2
+    for b in (0, half):
+        part = dict(c, q=c["q"][b:b + half], block_table=c["block_table"][b:b + half], lengths=c["lengths"][b:b + half])
+        assert (got[b:b + half] - call(part)).abs().max() <= 4e-5 * c["pages"].abs().max()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 def test_streams_and_graphs(dtype):
     """Another stream than the tensors' own; a captured call replayed with other lengths; two graphs and a call between."""
     c = make(dtype, 28, 4, 128, 16, [700], [60, 300, 9, 128] * 4, [1, 3, 1, 2] * 4)

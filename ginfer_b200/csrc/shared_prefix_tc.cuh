@@ -9,8 +9,8 @@
 // zero, and the values are made zero too, since zero times no number is none.
 // An item's result is the unnormalised sum of both streams with its maximum and sum, in 32 bits.
 //
-// What bounds it is the softmax between the products: a tile of 128 by 128 takes 1.1 us a stream pair, 0.55 of that its
-// 16,384 exponentials at 16 a clock.  On all SMs, without own tokens beside it: 256 requests behind 32,768 tokens, 40 heads on 8 of
+// What bounds it is a stream's chain of product, softmax and product: with two streams a tile of 128 by 128 takes 1.1 to 1.3 us,
+// 0.55 of that its 16,384 exponentials at 16 a clock.  On all SMs, without own tokens beside it: 256 requests behind 32,768 tokens, 40 heads on 8 of
 // 128, 233 us, 737 TFLOP/s; 64 behind 8,192, 28 on 4 of 128, 27.5 us, 273 TFLOP/s (10 us of that are starts, division and results).
 // Summing the weights as they are rounded for the product, as the other kernels do, costs 3 % here and changes nothing that
 // can be measured (error against 64 bits beside plain torch's 1.14 with and without), so they are summed as they come.

@@ -83,7 +83,8 @@ def attend(q: torch.Tensor, nh: int, pages, prefix_table: torch.Tensor, prefix_l
     ``prefix_table [G, P]``, ``prefix_lens [G]`` int32: the pages of every group's prefix in order and how many tokens it
     has (it may end inside a page).  ``block_table [B, W]``, ``lengths [B]`` int32: likewise of every request's own
     tokens, the new ones among them, counted from behind the prefix.  (Of tables that name all of a request's pages, with
-    whole pages shared, these are ``table[first requests, :P]`` and ``table[:, P:]``; rows may have any stride.)
+    whole pages shared, these are ``table[first requests, :P]`` and ``table[:, P:]``; rows may have any stride.  How a call
+    is carried out goes by the tables' widths: short sequences are fastest in narrow ones.)
     ``cu_groups [G + 1]`` int32: group ``g`` is the requests ``cu_groups[g] .. cu_groups[g + 1] - 1``, and a request of no
     group has no prefix; ``None``: one group of all requests.  ``cu_seqlens_q [B + 1]`` int32: request ``b`` has the rows
     ``cu_seqlens_q[b] .. cu_seqlens_q[b + 1] - 1``; ``None``: row ``b`` alone.  ``max_q_len``: about how many rows a request

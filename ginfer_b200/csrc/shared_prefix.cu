@@ -535,11 +535,16 @@ GF_DEFINE_PDL_SWITCH
 
 // Which way a call goes, by its sizes alone (the tables' widths, not the lengths in them).
 //
-// Direct: a block an item (request, kv head), whose warps share the keys of prefix and own tokens; one launch.  Where a
-// request's tables hold at most kDirectKeys bytes of keys of a kv head, and requests read at most kDirectBytes of prefixes.
-// Direct / equal runs and their join, us: 28 heads on 4 of 128, one request of 500 tokens 8.7 / 17.1, of 1,000 13.1 / 17.2; 64 of
-// 1,000 26.5 / 27.3, of 2,000 42.0 / 41.3; 14 on 2 of 64, 64 of 1,000 9.6 / 19.1, of 2,000 13.3 / 20.1; those in fp32 22.0 / 28.8, 38.3 / 41.2.
-constexpr long long kDirectKeys = 256 << 10, kDirectBytes = 128 << 20;
+// Direct: an item (request, kv head) is a block's, or a cluster's of 2, 4 or 8 blocks while there are SMs for twice as many and a
+// block has more than kBlockKeys bytes of the item's keys, a single one twice that (clusters of 8 find places for three quarters of the SMs: one more had
+// to wait for another's end); its warps share the keys of prefix and own tokens; one launch.  Where a block has at most
+// kDirectKeys, in a cluster (but for 32-bit heads above 64) twice as many, and requests read at most kDirectBytes of prefixes.
+// Direct / equal runs and their join, us: 28 heads on 4 of 128, 64 requests of 1,000 tokens (a block) 26.5 / 27.3, of 2,000 42.0 /
+// 41.3; 16 of 2,500 (2 blocks) 17.2 / 23.6; 8 of 4,100 (4) 16 / 25; one of 4,000 (8) 11.0 / 20.2, of 16,000 23.7 / 31.1; 14 on 2 of
+// 64, 32 of 5,000 (2) 16.9 / 24.9, one of 4,000 (8) 8.1 / 19.9; that in fp32 14.9 / 30.1, 12 of up to 2,600 (2) 27.0 / 30.9; fp32, 28 on
+// 4 of 128, one of 4,000 (256 KB a block) 29.7 / 35.2, of 16,000 110 / 52.  Blocks of 128 KB, 64 KB, 32 KB: 28 on 4 of 128, one of 1,000 10.6,
+// 8.8, 8.1, one of 500 9.1, 8.5, 7.7; 14 on 2 of 64, 2 of 340 one block 6.2, two 6.7; in fp32, one of 1,000 14.4, 10.6, 8.7.
+constexpr long long kDirectKeys = 256 << 10, kDirectBytes = 128 << 20, kBlockKeys = 32 << 10;
 // Unshared: every request reads its prefix itself (from L2 but for the first), in equal runs.  Where that is at most so many
 // bytes; 2 launches instead of 3.  Unshared / shared, us: 28 on 4 of 128, 8 requests behind 1,000 tokens (16 MB) 19.0 / 21.8, 16 of
 // 1,000 (33 MB) 19.5 / 22.5, 8 of 4,000 (66 MB) 22.7 / 25.4, 64 of 1,000 (131 MB) 30.4 / 27.9, 8 of 16,000 (262 MB) 45 / 28; 14 on 2 of
@@ -595,8 +600,13 @@ struct Call {
     p.H = a.nkv * p.shape.chunks;
     const long long item = half ? 2 : 4, prefixes = (long long)a.B * a.prefix_limit * a.nkv * HD * 2 * item;
     const bool any = a.G > 0 && a.prefix_limit > 0;
-    direct = ((any ? a.prefix_limit : 0ll) + a.limit) * HD * item <= kDirectKeys && (!any || prefixes <= kDirectBytes) &&
-             a.B <= 65535 && p.H <= 65535;
+    const long long held = ((any ? a.prefix_limit : 0ll) + a.limit) * HD * item;
+    const long long items = (long long)((longest + p.shape.tokens - 1) / p.shape.tokens) * a.B * p.H;
+    p.cluster = 1;
+    while (p.cluster < 8 && held > kBlockKeys * (p.cluster > 1 ? p.cluster : 2) && items * p.cluster * 2 <= (p.cluster == 4 ? p.sms * 3 / 4 : p.sms))
+      p.cluster *= 2;
+    const long long most = p.cluster > 1 && (half || HD <= 64) ? 2 * kDirectKeys : kDirectKeys;
+    direct = held <= most * p.cluster && (!any || prefixes <= kDirectBytes) && a.B <= 65535 && p.H <= 65535;
     shared = !direct && any && (half ? prefixes > kUnsharedBytes : own::kFarGroups > 0 && prefixes > kUnsharedBytes32);
     p.both = !shared, p.joined = !direct, p.after = shared;
     // the scratch: the division, pieces of cut items, of rows, of prefixes
@@ -636,13 +646,17 @@ constexpr int kOneLaunch = -101, kTwoLaunches = -102;
 
 template <typename T, int NG, bool FAR>
 static int launch_own(const own::Args& p, const CUtensorMap& mk, const CUtensorMap& mv, dim3 grid, cudaStream_t stream) {
+  constexpr int threads = 32 * own::Tile<T>::WARPS;
   static OncePerDevice attrs;
   if (int rc = attrs.run([&] {
         return cudaFuncSetAttribute(own::prefix_own_kernel<T, NG, FAR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     (int)own::smem_bytes<T>(NG));
       }))
     return rc;
-  return launch_kernel(own::prefix_own_kernel<T, NG, FAR>, grid, dim3(32 * own::Tile<T>::WARPS), own::smem_bytes<T>(NG), stream, mk, mv, p);
+  if (!p.joined && p.cluster > 1)
+    return launch_kernel_cluster_dims(own::prefix_own_kernel<T, NG, FAR>, grid, dim3(threads), own::smem_bytes<T>(NG), stream, p.cluster,
+                                      true, mk, mv, p);
+  return launch_kernel(own::prefix_own_kernel<T, NG, FAR>, grid, dim3(threads), own::smem_bytes<T>(NG), stream, mk, mv, p);
 }
 template <typename T>
 static int launch_near(const Call& c, const CUtensorMap& mk, const CUtensorMap& mv, dim3 grid) {
@@ -705,7 +719,7 @@ GF_EXPORT int gf_prefix_attend(const char* words) {
     if (rc) return rc;
   }
   const int row_tiles = (c.longest + p.shape.tokens - 1) / p.shape.tokens;
-  const dim3 grid = c.direct ? dim3(row_tiles, a.B, p.H) : dim3(p.sms);
+  const dim3 grid = c.direct ? dim3(row_tiles * p.cluster, a.B, p.H) : dim3(p.sms);
   int rc = half ? launch_near<bf16>(c, ok, ov, grid) : launch_near<float>(c, ok, ov, grid);
   if (rc || c.direct) return rc ? rc : kOneLaunch;
   c.j.p = p;

@@ -51,7 +51,7 @@ constexpr int KCH = HD / 16;
 // (joining warps inside a block takes the ring's memory, and what it has not)
 template <typename T> __host__ __device__ constexpr uint32_t smem_bytes(int ng) {
   using G = Tile<T>;
-  const uint32_t ring = G::WARPS * G::STAGES * G::STAGE, exchange = G::WARPS * 8 * ng * (HD + 2) * 4;
+  const uint32_t ring = G::WARPS * G::STAGES * G::STAGE, exchange = (G::WARPS + 1) * 8 * ng * (HD + 2) * 4;
   return (ring > exchange ? ring : exchange) + G::WARPS * G::STAGES * 8 + 1024;
 }
 constexpr float kGrowth = 8.f;   // log2 units: weights stay below 2^8
@@ -66,7 +66,8 @@ constexpr int kFarGroups = HD <= 64 ? 2 : 0;
 struct Args {
   PrefixArgs a;
   int both, tma;               // both: prefixes, too
-  int joined;                  // another kernel adds a row's pieces up; else a block's warps have an item, and it is written here
+  int joined;                  // another kernel adds a row's pieces up; else a cluster's warps have an item, and it is written here
+  int cluster;                 // blocks of a cluster then (neighbours along x)
   int after;                   // the launch runs beside the one before it, whose results the joining kernel reads, too
   Shape shape;
   int H, rows;                 // kv heads * chunks; rows of a tile
@@ -126,6 +127,19 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], 
       "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// All threads of a cluster's blocks.
+__device__ __forceinline__ void cluster_meet() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// What `addr` of this block is in another one of the cluster.
+__device__ __forceinline__ uint32_t in_block(uint32_t addr, int rank) {
+  uint32_t there;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
+  return there;
 }
 
 // A TMA copy of what is read once: it leaves L2 first.
@@ -196,7 +210,7 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
                              (long long)blocks * WARPS, blockIdx.x == 0 ? p.plan : nullptr);
     req = cur.req;
   } else {
-    cur = {(int)blockIdx.z, (int)blockIdx.y, (int)blockIdx.x, 0, 0, {}};
+    cur = {(int)blockIdx.z, (int)blockIdx.y, (int)blockIdx.x / p.cluster, 0, 0, {}};
     req = request_of(a, cur.b, p.both, KEYS);
     __syncthreads();
   }
@@ -232,10 +246,11 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
     }
     if (!p.joined) {
       if (cur.rt * p.shape.tokens >= req.count) return false;
-      const int tiles = req.far + req.near, w0 = tiles * warp / WARPS, w1 = tiles * (warp + 1) / WARPS;
+      const int tiles = req.far + req.near, all = WARPS * p.cluster, me = (int)blockIdx.x % p.cluster * WARPS + warp;
+      const int w0 = tiles * me / all, w1 = tiles * (me + 1) / all;
       set(w0, w1 - w0);
       x.to = FINAL;
-      cur.rt += gridDim.x;
+      cur.rt += gridDim.x / p.cluster;
       return true;
     }
     while (cur.todo > 0) {
@@ -515,6 +530,14 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
       __syncthreads();
       float* so = reinterpret_cast<float*>(base);                            // [WARPS][rows][HD], then (maximum, sum)
       float2* sml = reinterpret_cast<float2*>(so + WARPS * rows * HD);
+      float* bo = so + WARPS * 8 * NG * (HD + 2);                            // the block's: [rows][HD], then (maximum, sum)
+      float2* bml = reinterpret_cast<float2*>(bo + 8 * NG * HD);
+      auto write = [&](int r, int ch, float sum, const float (&y)[4]) {
+        const int token = r / heads, head = r - token * heads;
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;                      // (no key: zeros)
+        const float z[4] = {y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv};
+        if (ok) Quad<T>::store(static_cast<T*>(a.out) + ((size_t)(x.first + token) * a.nh + h0 + head) * HD + ch, z);
+      };
 #pragma unroll
       for (int n = 0; n < NG; ++n)
 #pragma unroll
@@ -528,7 +551,7 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
         }
       __syncthreads();
       for (int i = threadIdx.x; i < rows * (HD / 4); i += THREADS) {
-        const int r = i / (HD / 4), ch = (i - r * (HD / 4)) * 4, token = r / heads, head = r - token * heads;
+        const int r = i / (HD / 4), ch = (i - r * (HD / 4)) * 4;
         float top = -INFINITY, sum = 0.f, y[4] = {};
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) top = fmaxf(top, sml[w * rows + r].x);
@@ -541,9 +564,42 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
           sum += ml.y * f;
           y[0] += v.x * f, y[1] += v.y * f, y[2] += v.z * f, y[3] += v.w * f;
         }
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;                      // (no key: zeros)
-        const float z[4] = {y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv};
-        if (ok) Quad<T>::store(static_cast<T*>(a.out) + ((size_t)(x.first + token) * a.nh + h0 + head) * HD + ch, z);
+        if (p.cluster > 1) {
+          *reinterpret_cast<float4*>(bo + r * HD + ch) = make_float4(y[0], y[1], y[2], y[3]);
+          if (ch == 0) bml[r] = make_float2(top, sum);
+        } else {
+          write(r, ch, sum, y);
+        }
+      }
+      if (p.cluster > 1) {
+        // the same over the cluster's blocks, a share of the channels each
+        cluster_meet();
+        for (int i = (int)blockIdx.x % p.cluster * THREADS + threadIdx.x; i < rows * (HD / 4); i += p.cluster * THREADS) {
+          const int r = i / (HD / 4), ch = (i - r * (HD / 4)) * 4;
+          const uint32_t at_ml = smem_u32(bml + r), at_o = smem_u32(bo + r * HD + ch);
+          float top = -INFINITY, sum = 0.f, y[4] = {};
+          float2 ml[8];
+          float4 v[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            ml[k] = make_float2(-INFINITY, 0.f), v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (k >= p.cluster) continue;
+            asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(ml[k].x), "=f"(ml[k].y) : "r"(in_block(at_ml, k)) : "memory");
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(v[k].x), "=f"(v[k].y), "=f"(v[k].z), "=f"(v[k].w) : "r"(in_block(at_o, k)) : "memory");
+          }
+#pragma unroll
+          for (int k = 0; k < 8; ++k) top = fmaxf(top, ml[k].x);
+          const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float f = fast_exp2(ml[k].x - ref);
+            sum += ml[k].y * f;
+            y[0] += v[k].x * f, y[1] += v[k].y * f, y[2] += v[k].z * f, y[3] += v[k].w * f;
+          }
+          write(r, ch, sum, y);
+        }
+        cluster_meet();          // (nobody leaves, or fills its ring again, while another reads it)
       }
       __syncthreads();           // (the ring lies there again)
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");

@@ -19,7 +19,13 @@ def i32(x):
     return torch.as_tensor(x, dtype=torch.int32, device=DEV)
 
 
-WIDER = {"narrow": lambda c: (0, 0), "own": lambda c: (0, 4096), "prefix": lambda c: (_columns(c), 0)}
+WIDER = {"narrow": lambda c: (0, 0), "cluster": lambda c: (0, _some(c)), "own": lambda c: (0, 4096),
+         "prefix": lambda c: (_columns(c), 0)}
+
+
+def _some(c):
+    """So many columns more that a head's keys, a quarter of a megabyte, look like some blocks' work."""
+    return (250 << 10) // (c["pages"].shape[4] * c["pages"].itemsize * c["pages"].shape[2])
 
 
 def _columns(c):
@@ -31,7 +37,8 @@ def _columns(c):
 @pytest.fixture(params=WIDER, autouse=True)
 def way(request, monkeypatch):
     """How a call goes depends on its sizes, the tables' widths among them: every test with tables as wide as they need to be,
-    with wide ones of own tokens (runs over warps, joined) and with wide ones of prefixes (read once for a group)."""
+    with somewhat wider ones of own tokens (clusters of blocks), with wide ones of them (runs over warps, joined) and with
+    wide ones of prefixes (read once for a group)."""
     monkeypatch.setitem(globals(), "wider_by", WIDER[request.param])
     return request.param
 
@@ -340,7 +347,7 @@ def test_ways(dtype, hd, way):
     before = _Counter.launches
     check(call(c), c)
     shared = 3 if dtype is BF16 or hd <= 64 else 2
-    assert _Counter.launches - before == {"narrow": 1, "own": 2, "prefix": shared}[way]
+    assert _Counter.launches - before == {"narrow": 1, "cluster": 1, "own": 2, "prefix": shared}[way]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])

@@ -76,15 +76,15 @@ def verify(logits: torch.Tensor, tokens: torch.Tensor, cu_rows: torch.Tensor, te
     facts = (x, stride, code, y, draft_stride, _vector(tokens, R, torch.int32, "tokens", dev),
              _vector(cu_rows, B + 1, torch.int32, "cu_rows", dev),
              _vector(temperature, B, torch.float32, "temperature", dev), _vector(u, R, torch.float32, "u", dev))
-    accepted = tokens.new_empty(2, B)
+    accepted, following = tokens.new_empty(B), tokens.new_empty(B)
     stream, size, sms = _raw_stream(dev), 16 * R * (V // PIECE + 2), _of_device(dev)[0]
     if _entry is None:
         _entry = _function("drafts", "gf_verify")
     with _launching:
         scratch = _scratch_for(size, dev, stream)
-        rc = _entry(_VERIFY.pack(*facts, accepted.data_ptr(), accepted.data_ptr() + 4 * B, R, V, B, scratch.data_ptr(), size, sms,
+        rc = _entry(_VERIFY.pack(*facts, accepted.data_ptr(), following.data_ptr(), R, V, B, scratch.data_ptr(), size, sms,
                                  stream))
     _Counter.launches += 2
     if rc:
         _ok(rc, "drafts.verify")
-    return accepted.unbind()
+    return accepted, following

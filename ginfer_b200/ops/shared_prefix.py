@@ -126,8 +126,9 @@ def attend(q: torch.Tensor, nh: int, pages, prefix_table: torch.Tensor, prefix_l
         raise ValueError(f"q has rows of at least {width} channels without gaps in the cache's type {dtype}; got "
                          f"{q.dtype} {tuple(shape)}, strides {strides}")
     at, stride = _at(q, dev), strides[0]
-    if (at | stride * q.itemsize) & 15 or not width <= stride < 1 << 31:            # (the kernels read 16 bytes at a time)
-        q = q[:, :width].contiguous()
+    # (The kernels read 16 bytes at a time.  A clone: `contiguous` gives dense rows back as they are, wherever they start.)
+    if (at | stride * q.itemsize) & 15 or not width <= stride < 1 << 31:
+        q = q[:, :width].clone(memory_format=torch.contiguous_format)
         at, stride = q.data_ptr(), width
     T, B, G = shape[0], lengths.shape[0], prefix_lens.shape[0]
     prefix, prefix_stride, P = _table(prefix_table, G, "prefix_table", dev)

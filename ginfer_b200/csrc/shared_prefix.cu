@@ -207,7 +207,8 @@ prefix_pieces_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
       for (int i = 0; i < count; ++i) {
         const int key0 = (from + i) * TILE;
         if (i + 1 < count) look(from + i + 1, ahead);
-        if (!wait_bar(&empty[st], ph ^ 1u, p.err, 21)) {
+        // (the warp's verdict: a lane that left by itself would leave the others at the exchanges that follow)
+        if (!__all_sync(0xffffffffu, wait_bar(&empty[st], ph ^ 1u, p.err, 21))) {
           ok = false;
           break;
         }
@@ -288,7 +289,7 @@ prefix_pieces_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
       for (int c = 0; c < HD / 8; ++c) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
       for (int i = 0; i < count && ok; ++i) {
         const int key0 = (from + i) * TILE, end = it.length - 1;
-        ok = wait_bar(&full[st], ph, p.err, 22);
+        ok = __all_sync(0xffffffffu, wait_bar(&full[st], ph, p.err, 22));
         if (!ok) break;
         const unsigned char* stage = ring + st * STAGE;
         if (active) {

@@ -366,7 +366,8 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
     for (int i = 0; i < x.count && ok; ++i) {
       const Keys k = keys_of(x, x.from + i, KEYS);
       const bool far = x.from + i < x.far;
-      ok = wait_bar(&full[st], (phases >> st) & 1u, p.err, 22);
+      // (the warp's verdict: a lane that left by itself would leave the others at the exchanges that follow)
+      ok = __all_sync(0xffffffffu, wait_bar(&full[st], (phases >> st) & 1u, p.err, 22));
       if (!ok) break;
       phases ^= 1u << st;
       const unsigned char* stage = ring + st * STAGE;

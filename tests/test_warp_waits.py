@@ -1,0 +1,21 @@
+"""Waits of the kernels of shared prefixes and drafts whose end a whole warp goes by: a wait that runs out in some lanes only cannot be
+made to show, so the sources are read."""
+import re
+
+import pytest
+
+from test_early_reads import code_of
+
+
+@pytest.mark.parametrize("name", ["shared_prefix.cu", "shared_prefix_own.cuh", "shared_prefix_tc.cuh"])
+def test_a_wait_ends_for_all_lanes(name):
+    """Its verdict is voted on, or one lane's that the others are told; what is only waited for has no verdict."""
+    code = re.sub(r"bool wait_bar\(", "", code_of(name))
+    waits = list(re.finditer(r"\b(?:wait_bar|mbar_wait(?:<true>)?)\(", code))
+    assert waits
+    for w in waits:
+        line = code[code.rfind("\n", 0, w.start()) + 1:code.find("\n", w.end())]
+        voted = "__all_sync(0xffffffffu, " + w[0] in line
+        unused = re.search(r"(?:^\s*|\) )" + re.escape(w[0]), line) and line.rstrip().endswith(");")
+        told = re.match(r"\s*ok = mbar_wait\(", line) and "__shfl_sync(0xffffffffu, ok, 0)" in code[w.end():w.end() + 900]
+        assert voted or unused or told, line

@@ -347,6 +347,12 @@ static_assert(kTable == 16, "the shift above");
 struct Total {
   float best, sum;
 };
+// All threads of a cluster's blocks.  (The barrier's instructions want a warp as one; what stands in front of them are stores of
+// single lanes.)
+__device__ __forceinline__ void cluster_meet() {
+  __syncwarp();
+  cluster_sync();
+}
 struct Cluster {
   uint32_t rank, size;
   int round;
@@ -356,7 +362,7 @@ struct Cluster {
   __device__ __forceinline__ void add(double mine0, double mine1, double& all0, double& all1, double& before) {
     double* at = slots[round & 1];
     if (threadIdx.x == 0) at[0] = mine0, at[1] = mine1;
-    cluster_sync();
+    cluster_meet();
     // (a lane a block)
     double x = 0., y = 0.;
     const uint32_t lane = threadIdx.x & 31;
@@ -899,7 +905,7 @@ __global__ void __launch_bounds__(kDecide, 2) verify_decide_kernel(const VerifyA
     __syncthreads();
     if (verdict[0] >= 0) {
       if (cl.rank == 0 && threadIdx.x == 0) a.accepted[b] = stop, a.next[b] = verdict[0];
-      if (cl.round) cluster_sync();
+      if (cl.round) cluster_meet();
       return;
     }
   } else {
@@ -924,7 +930,7 @@ __global__ void __launch_bounds__(kDecide, 2) verify_decide_kernel(const VerifyA
     double found, unused0, unused1;
     cl.add((double)verdict[0], 0., found, unused0, unused1);
     if (found > 0.) {
-      cluster_sync();          // (nobody leaves while another reads its sums)
+      cluster_meet();          // (nobody leaves while another reads its sums)
       return;
     }
   }
@@ -936,7 +942,7 @@ __global__ void __launch_bounds__(kDecide, 2) verify_decide_kernel(const VerifyA
                              : exactly_drawn<T, false>(a, cl, sums, tables, heat, row, with_draft, tp.best, tq.best, r.d, u, none);
   if (token >= 0 && lane == 0) a.accepted[b] = stop, a.next[b] = token;
   if (none && cl.rank == 0 && threadIdx.x == 0) a.accepted[b] = stop, a.next[b] = 0;      // (a row without a number)
-  cluster_sync();              // (nobody leaves while another reads its sums)
+  cluster_meet();              // (nobody leaves while another reads its sums)
 }
 
 }  // namespace

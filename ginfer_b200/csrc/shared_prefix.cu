@@ -312,6 +312,7 @@ prefix_pieces_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
       }
       if (sharing > 1) {
         // the others' results into the first one's registers
+        __syncwarp();            // (the barrier wants a warp as one)
         asm volatile("bar.sync 1, 128;" ::: "memory");
         if (share > 0) {
           float* to = merge + (groups16 == 1 ? share - 1 : mine) * 16 * (MERGE_ROW + 2);
@@ -325,6 +326,7 @@ prefix_pieces_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             ml[g] = make_float2(m[0], l[0]), ml[g + 8] = make_float2(m[1], l[1]);
           }
         }
+        __syncwarp();
         asm volatile("bar.sync 1, 128;" ::: "memory");
         if (share == 0) {
           for (int w = 0; w < sharing - 1; ++w) {

@@ -449,6 +449,7 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
 #pragma unroll
               for (int c = 0; c < HD / 16; ++c) o[n][c][e] *= corr, o[n][c][2 + e] *= corr;
             }
+          __syncwarp();              // (the matrix instructions want the warp as one)
         }
 #pragma unroll
         for (int n = 0; n < NG; ++n) {

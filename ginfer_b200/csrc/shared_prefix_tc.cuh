@@ -325,6 +325,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (r == 0) mbar_arrive(&bars->k_empty[s * KS + cnt % KS]);   // S is computed: its K tile is free
+        __syncwarp();                  // (tensor memory's instructions want the warp as one)
         const int left = end - (j0 + 2 * t + s) * KT;                 // keys of the tile that are the prefix's
         float v[KT];
 #pragma unroll
@@ -343,6 +344,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
               for (int c = 0; c < 8; ++c)
                 reinterpret_cast<uint4*>(v_s + (size_t)st * OPERAND + h * ATOM_BYTES + r * 128)[c] = make_uint4(0u, 0u, 0u, 0u);
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
         }
         float mx8[8];
 #pragma unroll
@@ -423,6 +425,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
 #pragma unroll 1
       for (int cc = 0; cc < HD / 2; cc += 16) {
         float x[16], y[16];
+        __syncwarp();
         tmem_ld16(o0 + cc, x);
         if (two) tmem_ld16(o1 + cc, y);
         tmem_ld_wait();

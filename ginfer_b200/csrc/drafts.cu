@@ -80,8 +80,14 @@ template <typename T> struct Row {
     return j >= 0 && j + kVec<T> <= V;
   }
   __device__ __forceinline__ uint4 raw(int g) const { return __ldcg(reinterpret_cast<const uint4*>(x + (g * kVec<T> - mis))); }
-  // The same for what is read in passing: it leaves L2 first.
-  __device__ __forceinline__ uint4 passing(int g) const { return __ldcs(reinterpret_cast<const uint4*>(x + (g * kVec<T> - mis))); }
+  // The same for what is read in passing, past L1, too: it leaves L2 first.  (`once`: a policy that says so.)
+  __device__ __forceinline__ uint4 passing(int g, uint64_t once) const {
+    uint4 v;
+    asm volatile("ld.global.cg.L2::cache_hint.v4.u32 {%0, %1, %2, %3}, [%4], %5;"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(x + (g * kVec<T> - mis)), "l"(once));
+    return v;
+  }
   // A group that the row begins or ends in, or one outside it: -inf in places outside.
   __device__ __forceinline__ uint4 pieced(int g) const {
     uint32_t w[4];
@@ -180,6 +186,8 @@ __global__ void __launch_bounds__(kScan, kScanBlocks) verify_scan_kernel(const V
   __shared__ int starts[kSearch + 1];
   constexpr int GROUPS = 32 * kLoads;
   const int lane = threadIdx.x & 31;
+  uint64_t once;
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(once));
   pdl_trigger();
   pdl_wait();
   const bool kept = a.B <= kSearch;
@@ -226,11 +234,11 @@ __global__ void __launch_bounds__(kScan, kScanBlocks) verify_scan_kernel(const V
       const int g0 = x.piece * GROUPS + lane;
       if (r.whole(x.piece * GROUPS) && r.whole(x.piece * GROUPS + GROUPS - 1)) {
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) raw[i] = r.passing(g0 + i * 32);
+        for (int i = 0; i < kLoads; ++i) raw[i] = r.passing(g0 + i * 32, once);
       } else {
         const uint32_t none = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) raw[i] = r.whole(g0 + i * 32) ? r.passing(g0 + i * 32) : make_uint4(none, none, none, none);
+        for (int i = 0; i < kLoads; ++i) raw[i] = r.whole(g0 + i * 32) ? r.passing(g0 + i * 32, once) : make_uint4(none, none, none, none);
         // (the row's first and last group)
         const int first = r.mis ? 0 : -1, last = (a.V + r.mis) % kVec<T> ? r.groups() - 1 : -1;
 #pragma unroll

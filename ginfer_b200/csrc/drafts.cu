@@ -907,7 +907,10 @@ __global__ void __launch_bounds__(kDecide, 2) verify_decide_kernel(const VerifyA
       }
       // (off by a part of all of p, which `total` is where no draft is taken out)
       const double room = kDrawMargin * (double)tp.sum;
-      const bool sure = token >= 0 && tp.best < INFINITY && c > 0.f && (target - low > room || (low == 0. && target > 0.)) && high - target > room;
+      // (Nothing in front of the token: whatever the target is, it is reached there.  Behind the piece that the draft is taken out of
+      // that cannot be said: what is beside the draft there may be lost in its sum.)
+      const bool first = low == 0. && target > 0. && (d_piece < 0 || piece <= d_piece);
+      const bool sure = token >= 0 && tp.best < INFINITY && c > 0.f && (target - low > room || first) && high - target > room;
       if (lane == 0) verdict[0] = sure ? token : -1;
     }
     __syncthreads();

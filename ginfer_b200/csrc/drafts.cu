@@ -28,10 +28,12 @@ constexpr int kDecide = 256, kWarps = kDecide / 32, kBatch = 32;      // rows wh
 // model 139.5 / 180.2, 256 of 7 in bfloat16 392.5 / 381.6, 33 of 6 and 32,003 logits 43.8 / 51.5 (2, 5, 6 and 16 are slower).
 constexpr int kManyRequests = 128;
 constexpr int kAhead = 4;                               // loads of a row that are under way
-// Relative error that 32-bit sums may have: exponents are off by three roundings, 2^-24 each, of up to 20, and the exponential by
-// 2^-22, sums of a piece by 32 roundings at most: 5e-6 for p and for q; what is compared is both, with room.
+// Relative error that numbers in 32 bits may have.  A weight's: 3.5 roundings of its exponent (difference, 1 / T, product), 1.45e-7
+// of it in the weight, and 2^-22 of each exponential; what is summed weighs its own exponents, log2 V = 28 at most in the mean,
+// 4e-6.  A piece's sum: 64 roundings at most, 3.8e-6; pieces are added up in 64 bits.  So a row's sum is off by 9e-6, a draft's
+// weight, compared down to 1e-30, an exponent of 100, by 1.5e-5, and u q(d) beside p(d) by 5e-5.
 constexpr double kMargin = 8e-5;
-// The same of a running sum beside the whole, of p or of p and q: 1e-5 of 1 for each, with room.
+// The same of a running sum beside u times the whole, in parts of 1: 5e-6 for its weights and 9e-6 for the row's sum, of p and of q: 2.8e-5.
 constexpr double kDrawMargin = 4e-5;
 constexpr float kLog2E = 1.4426950408889634f;
 
@@ -693,7 +695,8 @@ __global__ void __launch_bounds__(kDecide, 2) verify_decide_kernel(const VerifyA
       float own = -INFINITY;
       if (i0 + i < n - 1)
         own = Row<T>(which ? a.draft : a.logits, which ? a.draft_stride : a.stride, row, a.V).at(fresh_index(a.tokens + row + 1));
-      float best = -INFINITY, sum = 0.f;
+      float best = -INFINITY;
+      double sum = 0.;                                // (there may be 2^18 pieces)
       int at = 0x7fffffff;
       for (int q0 = lane; q0 < a.pieces; q0 += 32 * 8) {
         float2 y[8];
@@ -707,10 +710,10 @@ __global__ void __launch_bounds__(kDecide, 2) verify_decide_kernel(const VerifyA
           top = fmaxf(top, y[q].x);
         }
         if (!greedy && top > -INFINITY) {
-          sum = best > -INFINITY ? sum * weight32(best, top, c) : 0.f;
+          sum = best > -INFINITY ? sum * (double)weight32(best, top, c) : 0.;
 #pragma unroll
           for (int q = 0; q < 8; ++q)
-            if (y[q].x > -INFINITY) sum += y[q].y * weight32(y[q].x, top, c);
+            if (y[q].x > -INFINITY) sum += (double)(y[q].y * weight32(y[q].x, top, c));
         }
         best = top;
       }
@@ -723,11 +726,11 @@ __global__ void __launch_bounds__(kDecide, 2) verify_decide_kernel(const VerifyA
         }
       } else {
         const float top = warp_max(best);
-        sum = warp_sum(best > -INFINITY ? sum * weight32(best, top, c) : 0.f);
+        sum = warp_total(best > -INFINITY ? sum * (double)weight32(best, top, c) : 0.);
         best = top;
       }
       if (lane == 0) {
-        totals[i][which] = {best, sum}, drafted[i][which] = own;
+        totals[i][which] = {best, (float)sum}, drafted[i][which] = own;
         if (!which) places[i] = best == -INFINITY ? 0 : min(max(at, 0), a.V - 1);
       }
     }

@@ -12,8 +12,6 @@
 // What bounds it is a stream's chain of product, softmax and product: with two streams a tile of 128 by 128 takes 1.1 to 1.3 us,
 // 0.55 of that its 16,384 exponentials at 16 a clock.  On all SMs, without own tokens beside it: 256 requests behind 32,768 tokens, 40 heads on 8 of
 // 128, 233 us, 737 TFLOP/s; 64 behind 8,192, 28 on 4 of 128, 27.5 us, 273 TFLOP/s (10 us of that are starts, division and results).
-// Summing the weights as they are rounded for the product, as the other kernels do, costs 3 % here and changes nothing that
-// can be measured (error against 64 bits beside plain torch's 1.14 with and without), so they are summed as they come.
 //
 // Warps: 0, 1 load K (and Q), 2, 3 load V, 4 issues products, 8 .. 11 and 12 .. 15 are the streams' softmax, a thread a row.
 // Every wait on an mbarrier is bounded; when one runs out, an abort flag tells the other roles, all meet at the final barrier
@@ -63,6 +61,15 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, u
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
       ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
       : "memory");
+}
+// Weights are summed as they are rounded for the product, as in the other kernels: a row that one key takes nearly all of gets
+// its value as it is.  (Summed as they come, in packed additions, the kernel is 2 to 5 % faster and such rows are off by a step of
+// bfloat16; unpacked by integer instructions first, 3 to 8 % slower than that.)
+__device__ __forceinline__ void add_rounded(float& a, float& b, uint32_t pair) {
+  uint16_t lo, hi;
+  asm("mov.b32 {%0, %1}, %2;" : "=h"(lo), "=h"(hi) : "r"(pair));
+  asm("add.rn.f32.bf16 %0, %1, %0;" : "+f"(a) : "h"(lo));
+  asm("add.rn.f32.bf16 %0, %1, %0;" : "+f"(b) : "h"(hi));
 }
 
 __global__ void __launch_bounds__(NTHREADS_TC, 1)
@@ -370,7 +377,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
             tmem_st16(my_o + cc, ob);
           }
         }
-        uint64_t sum2[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
+        float sum[4] = {};
         const uint64_t scale2 = pack2(scale_log2, scale_log2), msub2 = pack2(-msub, -msub);
 #pragma unroll
         for (int cc = 0; cc < KT / 32; ++cc) {
@@ -379,18 +386,12 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
           for (int k = 0; k < 32; k += 2) {
             float a0, a1;
             unpack2(fma2(pack2(v[32 * cc + k], v[32 * cc + k + 1]), scale2, msub2), a0, a1);
-            const float e0 = fast_exp2(a0), e1 = fast_exp2(a1);
-            sum2[(k >> 1) & 1] = add2(sum2[(k >> 1) & 1], pack2(e0, e1));
-            w[k / 2] = pack_bf16(e0, e1);
+            w[k / 2] = pack_bf16(fast_exp2(a0), fast_exp2(a1));
+            add_rounded(sum[k & 2], sum[(k & 2) + 1], w[k / 2]);
           }
           tmem_st16(my_s + 16 * cc, w);
         }
-        {
-          float s0, s1, s2, s3;
-          unpack2(sum2[0], s0, s1);
-          unpack2(sum2[1], s2, s3);
-          l = l * corr + ((s0 + s1) + (s2 + s3));
-        }
+        l = l * corr + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
         m_used = m_new;
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");

@@ -93,7 +93,10 @@ def attend(q: torch.Tensor, nh: int, pages, prefix_table: torch.Tensor, prefix_l
     The ``i``-th of a request's ``n`` rows sees the whole prefix and the own tokens ``0 .. length - n + i``; a row that
     sees nothing gives zeros.  What a row sees is finite (an infinity there leaves no number); what none sees may be
     anything.  Rows that belong to no request are not written: with ``out`` (``[T, nh * head size]``, contiguous, ``q``'s
-    type) they stay as they were.  Entries of the tables behind a sequence's length are not read."""
+    type) they stay as they were.  Entries of the tables behind a sequence's length are not read.  Starts rise or stay; of those
+    that fall nothing but named rows is written, and a request whose rows lie in front of its group's first start does
+    without the prefix there.  A wait inside that runs out leaves rows unwritten and is reported by
+    ``gemm_bf16.check_errors``."""
     # (what follows is the host's time of a call: a plane of its own would be two tensors made, a helper a call)
     if torch.is_tensor(pages):
         shape, dtype = pages.shape, pages.dtype

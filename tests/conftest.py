@@ -25,3 +25,12 @@ def pytest_collection_modifyitems(config, items):
     for item in items:
         if "gpu" in item.keywords:
             item.add_marker(skip)
+
+
+@pytest.fixture(autouse=True)
+def waits_of_shared_prefixes(request):
+    """Kernels whose bounded waits ran out leave rows unwritten and say so in a word on the device: no test passes by them."""
+    yield
+    if request.node.path.name.startswith("test_shared_prefix") and "gpu" in request.keywords:
+        from ginfer_b200.ops import gemm_bf16
+        gemm_bf16.check_errors()

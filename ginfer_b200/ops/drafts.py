@@ -18,7 +18,6 @@ from .shared_prefix import _launching, _scratch_for
 
 PIECE = 1024                   # the least logits of a piece of a row (the library has the same number)
 _VERIFY = struct.Struct("=18q")
-_entry = None                  # the library's function, once it is loaded
 
 
 def _rows(x, rows, columns, what, device):
@@ -59,7 +58,6 @@ def verify(logits: torch.Tensor, tokens: torch.Tensor, cu_rows: torch.Tensor, te
     row's weight.  Where nothing is left of ``p - q`` the next token is drawn from ``p``, where nothing is left of that either it is
     the arg-max (0 in a row without a number).  A draft that is no index of the vocabulary does not stay.  A request without
     rows has ``(0, -1)``."""
-    global _entry
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError(f"logits are [rows, vocabulary]; got {tuple(logits.shape)}")
     (R, V), code = logits.shape, _code(logits.dtype)
@@ -78,12 +76,10 @@ def verify(logits: torch.Tensor, tokens: torch.Tensor, cu_rows: torch.Tensor, te
              _vector(temperature, B, torch.float32, "temperature", dev), _vector(u, R, torch.float32, "u", dev))
     accepted, following = tokens.new_empty(B), tokens.new_empty(B)
     stream, size, sms = _raw_stream(dev), 16 * R * (V // PIECE + 2), _of_device(dev)[0]
-    if _entry is None:
-        _entry = _function("drafts", "gf_verify")
+    f = _function("drafts", "gf_verify")
     with _launching:
         scratch = _scratch_for(size, dev, stream)
-        rc = _entry(_VERIFY.pack(*facts, accepted.data_ptr(), following.data_ptr(), R, V, B, scratch.data_ptr(), size, sms,
-                                 stream))
+        rc = f(_VERIFY.pack(*facts, accepted.data_ptr(), following.data_ptr(), R, V, B, scratch.data_ptr(), size, sms, stream))
     _Counter.launches += 2
     if rc:
         _ok(rc, "drafts.verify")

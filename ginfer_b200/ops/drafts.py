@@ -80,7 +80,7 @@ def verify(logits: torch.Tensor, tokens: torch.Tensor, cu_rows: torch.Tensor, te
     with _launching:
         scratch = _scratch_for(size, dev, stream)
         rc = f(_VERIFY.pack(*facts, accepted.data_ptr(), following.data_ptr(), R, V, B, scratch.data_ptr(), size, sms, stream))
-    _Counter.launches += 2
     if rc:
         _ok(rc, "drafts.verify")
+    _Counter.launches += (2 if R else 1) if B else 0
     return accepted, following

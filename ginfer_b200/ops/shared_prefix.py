@@ -21,7 +21,7 @@ from .quant_cache import _CODE, _at, _capturing, _device, _function, _of_device,
 
 MAX_HEAD_DIM = 256
 _ATTEND = struct.Struct("=29qd")
-_LAUNCHES = {-101: 1, -102: 2}          # what the entry point returns when it launched fewer than three kernels
+_LAUNCHES = {0: 3, -101: 1, -102: 2}    # what the entry point returns: how many kernels it launched
 _int32, _INF = torch.int32, float("inf")
 _attend_functions: dict = {}
 
@@ -176,7 +176,7 @@ def attend(q: torch.Tensor, nh: int, pages, prefix_table: torch.Tensor, prefix_l
         rc = f(_ATTEND.pack(at, stride, code, k_at, v_at, count, page, prefix, prefix_stride, prefix_tokens, G, P, table,
                             table_stride, own_tokens, B, W, groups, rows, out_at, T, nh, nkv, sms, longest, scratch, size, err,
                             stream, scale))
-    _Counter.launches += _LAUNCHES.get(rc, 3)
-    if rc and rc not in _LAUNCHES:
+    if rc not in _LAUNCHES:
         _ok(rc, "shared_prefix.attend")
+    _Counter.launches += _LAUNCHES[rc]
     return out

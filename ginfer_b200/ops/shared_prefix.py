@@ -22,7 +22,7 @@ from .quant_cache import _CODE, _at, _capturing, _device, _function, _of_device,
 MAX_HEAD_DIM = 256
 _ATTEND = struct.Struct("=29qd")
 _LAUNCHES = {0: 3, -101: 1, -102: 2}    # what the entry point returns: how many kernels it launched
-_int32, _INF = torch.int32, float("inf")
+_int32 = torch.int32
 _attend_functions: dict = {}
 
 
@@ -151,8 +151,8 @@ def attend(q: torch.Tensor, nh: int, pages, prefix_table: torch.Tensor, prefix_l
         raise ValueError(f"tables of {P} and {W} tokens: a sequence has fewer than 2^30")
     if max_q_len is not None and max_q_len < 0:
         raise ValueError(f"max_q_len is {max_q_len}")
-    if not 0 < scale < _INF:
-        raise ValueError(f"the scale of the scores is a positive number, not {scale}")
+    if not 0 < scale <= 1e38:                               # (in 32 bits, and times log2(e))
+        raise ValueError(f"the scale of the scores is a positive number up to 1e38, not {scale}")
     if out is None:
         out = q.new_empty(T, width)
         out_at = out.data_ptr()

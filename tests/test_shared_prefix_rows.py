@@ -1,4 +1,5 @@
-"""The rows of q that ``ops.shared_prefix.attend`` hands to the library start at multiples of 16 bytes, without a GPU."""
+"""What ``ops.shared_prefix.attend`` hands to the library, without a GPU: rows of q start at multiples of 16 bytes, and the scale is a
+number in 32 bits."""
 import pytest
 import torch
 
@@ -26,3 +27,14 @@ def test_rows_of_q_are_aligned(calls, dtype, rows, gap, offset):  # noqa: F811
     assert at % 16 == 0 and (rows == 1 or stride * q.itemsize % 16 == 0)
     if q.data_ptr() % 16 == 0 and q.stride(0) * q.itemsize % 16 == 0:
         assert (at, stride) == (q.data_ptr(), 256 + gap)                # (nothing is copied without need)
+
+
+@pytest.mark.parametrize("scale", [1e39, 3e38, 1e300, float("inf"), -1.0])
+def test_scales_that_32_bits_do_not_hold(calls, scale):  # noqa: F811
+    """(Zero and NaN: with the other refusals.)"""
+    with pytest.raises(ValueError, match="scale"):
+        shared_prefix.attend(**good(scale=scale))
+    assert not calls
+    for fine in (1e38, 1e-30, 1):
+        shared_prefix.attend(**good(scale=fine))
+    assert len(calls) == 3

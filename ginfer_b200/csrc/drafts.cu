@@ -24,9 +24,15 @@ constexpr int kPiece = 1024;                            // the least logits of a
 constexpr int kScan = 256, kScanBlocks = 2;             // threads of a scanning block, blocks an SM
 constexpr int kSearch = 1024;                           // requests whose first rows a scanning block keeps
 constexpr int kDecide = 256, kWarps = kDecide / 32, kBatch = 32;      // rows whose sums are at hand at a time
-// Blocks of a request: 8 up to this many requests, else 4.  8 / 4, us, 64 requests of 4 drafts and 152,064 logits with a draft
-// model 139.5 / 180.2, 256 of 7 in bfloat16 392.5 / 381.6, 33 of 6 and 32,003 logits 43.8 / 51.5 (2, 5, 6 and 16 are slower).
-constexpr int kManyRequests = 128;
+// Blocks of a request: 8 up to a number of requests, else 4 (2, 5, 6 and 16 are slower): the more logits a draw goes through, a
+// row of the target and one of the drafter, the longer twice the blocks are worth their starts and barriers.  8 / 4, us, requests of
+// 4 drafts: 152,064 logits and a drafter, 64 requests 134 / 155, 128 220 / 230, 160 257 / 257, 256 399 / 378, the same in bfloat16
+// 124 / 135, 195 / 193 (128), 353 / 311 (256); of 1 draft 77 / 115, 115 / 134, 220 / 213, of 8 185 / 210, 320 / 324, 599 / 558; 100,000 logits, 64
+// 102 / 108, 128 166 / 162; 64,000, 64 68 / 75, 96 92 / 92, 128 122 / 112; 32,003, 32 36 / 42, 64 48 / 45, 128 80 / 68; 8,000, 32 22 / 21, 64
+// 31 / 24; look-ups, 152,064, 32 50 / 63, 64 80 / 79, 128 136 / 118; 32,003, 32 26 / 27, 64 40 / 33.
+__host__ inline int blocks_of_request(int requests, int vocabulary, bool drafter) {
+  return requests > 28 + vocabulary / (drafter ? 1500 : 3000) ? 4 : 8;
+}
 constexpr int kAhead = 4;                               // loads of a row that are under way
 // Relative error that numbers in 32 bits may have.  A weight's: 3.5 roundings of its exponent (difference, 1 / T, product), 1.45e-7
 // of it in the weight, and 2^-22 of each exponential; what is summed weighs its own exponents, log2 V = 28 at most in the mean,
@@ -996,7 +1002,7 @@ GF_EXPORT int gf_verify(const char* words) {
                        dim3(kScan), 0, stream, a);
   }
   if (rc) return rc;
-  const int cluster = a.B > kManyRequests ? 4 : 8;
+  const int cluster = blocks_of_request(a.B, a.V, a.draft != nullptr);
   return launch_kernel_cluster_dims(half ? verify_decide_kernel<bf16> : verify_decide_kernel<float>, dim3(a.B * cluster),
                                     dim3(kDecide), 0, stream, cluster, true, a);
 }

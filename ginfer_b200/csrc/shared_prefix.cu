@@ -555,11 +555,20 @@ constexpr long long kDirectKeys = 256 << 10, kDirectBytes = 128 << 20, kBlockKey
 // fp32, 14 on 2 of 64: 16 of 1,000 (16 MB) 27.6 / 29.4, 64 of 2,000 (131 MB) 43.4 / 40.4, 128 of 4,000 (524 MB) 127 / 100.  In 32 bits with heads
 // above 64 registers leave 8 rows a tile, with or without groups: 28 on 4 of 128, 128 of 4,000, 543 unshared, 785 shared; so not at all there.
 constexpr long long kUnsharedBytes = 48 << 20, kUnsharedBytes32 = 128 << 20;
-// What a tile of a prefix costs beside a tile of own tokens (which come from memory), for the SMs' shares: 128 keys on the
-// tensor cores with up to 128 rows, 64 keys on mma.sync with up to 64 rows, 16 keys in 32 bits.  By the first, us: 256 requests behind
-// 32,768 tokens 322 at 6, 287 at 8, 291 at 10, 381 at 15; 64 behind 8,192 46, 38, 41, 45.  By the second, 24 requests behind two
-// prompts of 96-wide heads: 30.0 at 2, 29.5 at 4, 30.8 at 6.  By the third, 39.3 at 0.5 and at 1, 39.7 at 2.5.
-constexpr float kTensorCost = 8.f, kPlainCost = 4.f, kCost32 = 1.f;
+// What a tile of a prefix costs beside a tile of own tokens (which come from memory), for the SMs' shares: 128 keys on the tensor
+// cores with up to 128 rows, 64 keys on mma.sync with up to 64 rows, 16 keys in 32 bits.  Own tokens' tiles are 16 keys, 32 for heads
+// of up to 64.  us at (costs):
+//  * tensor cores, 128 (6, 8, 10, 12): 28 heads on 4, 64 requests behind 8,192 tokens with up to 1,024 of their own 48.8 / 41.4 / 40.9 / 45.7,
+//    128 behind 4,096, 4,096 165 / 160 / 126 / 126, 256 behind 32,768, 512 242 / 194 / 193 / 215; 40 on 8, the same 84 / 64 / 67 / 65,
+//    317 / 281 / 241 / 233, 334 / 298 / 293 / 320.  64 (6, 8, 10), 14 on 2: 28.8 / 28.8 / 29.0, 54.8 / 48.2 / 53.7, 94.8 / 93.7 / 103.7.
+//  * mma.sync, up to 128 (3, 4, 5, 6): 16 on 4 of 96, 128 behind 4,096, 2,048 159 / 126 / 135 / 121, 24 of up to 3 rows behind two prompts of 3,001
+//    30.2 / 30.7 / 31.9 / 31.5, 64 of up to 3 behind 4,000, 600 64.9 / 59.9 / 57.1 / 66.8, 128 behind 16,000, 200 114 / 118 / 122 / 129.  192 and
+//    256, whose blocks have an SM to themselves (4, 6, 8, 10, 12): 10 on 2 of 192, 64 behind 8,192, 1,024 57.0 / 46.3 / 47.9 / 54.9 / 60.4,
+//    32 of up to 4 behind 16,000 71 / 67 / 83 / 97 / 115; 8 on 4 of 256, the first 104 / 81 / 72 / 69 / 64, 128 behind 4,096, 2,048 336 / 225 / 169 / 158 / 126,
+//    16 on 2 of 256, 32 of up to 4 behind 16,000 153 / 137 / 180 / 179 / 224.
+//  * 32 bits, 64 (1, 1.25, 1.5, 1.75, 2): 14 on 2, 128 behind 4,000, 600 128 / 118 / 120 / 129 / 145; 8 on 8, the same 142 / 130 / 119 / 120 / 124;
+//    20 on 1, 256 behind 2,000, 300 244 / 207 / 208 / 209 / 217.
+constexpr float kTensorCost = HD <= 64 ? 8.f : 10.f, kPlainCost = HD <= 128 ? 4.f : HD <= 192 ? 7.f : 9.f, kCost32 = 1.5f;
 
 // `words`: q, its row stride and type, k, v, pages, page, prefix_table and its stride, prefix_lens, groups, prefix limit,
 // table and its stride, lengths, requests, limit, cu_groups, cu, out, rows, heads, kv heads, SMs, the rows that a request has

@@ -39,8 +39,8 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, int* er
 
 // ------------------------------------------------------------------------------------- pieces on mma.sync
 // Prefixes where the tensor cores' own kernel does not serve (heads other than 64 and 128, pages that are not multiples of 8 up
-// to 128): a loading warp and four that share a tile's keys, 16 rows of q a product, up to 64 a block.  By itself 13 us for 24
-// requests behind prompts of 3,001 and 1,331 tokens, 16 heads on 4 of 96, most of it starts (0.4 GFLOP).
+// to 128): a loading warp and four that share a tile's keys, 16 rows of q a product, up to 64 a block.  18 us for 24
+// requests behind prompts of 3,001 and 1,331 tokens, 16 heads on 4 of 96, beside their own tokens, most of it starts (0.4 GFLOP).
 constexpr int TILE = 64;                         // keys of a tile
 constexpr int MOST_ROWS = 64;                    // rows of a tile of them
 constexpr int CONSUMERS = 4, THREADS = 32 * (CONSUMERS + 1);
@@ -601,7 +601,6 @@ struct Call {
     scratch = (char*)ptr(), room = w[i++];
     p.err = (int*)ptr(), stream = (cudaStream_t)ptr();
     a.scale = (float)*reinterpret_cast<const double*>(w + i);
-    a.hd = HD;
     a.page_shift = (a.page & (a.page - 1)) == 0 ? 31 - __builtin_clz(a.page) : -1;
     if (longest < 1) longest = 1;
     const bool half = type == GF_BF16;

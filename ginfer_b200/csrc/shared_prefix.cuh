@@ -31,7 +31,7 @@ struct PrefixArgs {
   const int* cu_groups;        // [G + 1], or null: all requests are of group 0
   const int* cu;               // [B + 1], or null: a row a request
   void* out;                   // [T][nh][hd]
-  int q_stride, prefix_stride, table_stride, prefix_limit, limit, G, B, T, nh, nkv, hd, page, pages, page_shift;
+  int q_stride, prefix_stride, table_stride, prefix_limit, limit, G, B, T, nh, nkv, page, pages, page_shift;
   float scale;
 };
 
@@ -374,7 +374,7 @@ __device__ __forceinline__ Cursor find_run(const PrefixArgs& a, const OwnWork& w
 }
 
 // Prefixes and own tokens are worked on side by side, by two launches: of `sms` SMs this many have the prefixes.  A tile of a
-// prefix costs kFarCost of what a tile of own tokens does.
+// prefix costs `far_cost` of what a tile of own tokens does.
 __device__ __forceinline__ int far_share(int sms, long long far_units, float far_cost, long long own_units) {
   if (far_units == 0) return 0;
   const float far = (float)far_units * far_cost, own = (float)own_units;

@@ -9,8 +9,8 @@
 //
 // What bounds it is latency: a request's numbers, its run, its pages and its q come one after the other (about 10 us from the start to
 // the first product), then a tile costs a warp 0.8 us.  Own tokens of 64 requests of up to 1,024, 28 heads on 4 of 128, 72 MB, on
-// all SMs 27.6 us, 2.7 TB/s; 12 of up to 600 behind up to 2,000 in 32 bits, 14 on 2 of 64, 27.5 us.  Rings a warp of its own and equal runs
-// replaced blocks that share a tile (the call 52 -> 41 us).
+// all SMs 28 us, 2.6 TB/s; in 32 bits 12 requests of up to 600 behind up to 2,000, 14 on 2 of 64, as clusters of two blocks 27 us, prefixes among
+// them.  Rings a warp of its own and equal runs replaced blocks that share a tile (the call 52 -> 41 us).
 //
 // In 32 bits both factors of a product are the sum of two tf32 numbers, 22 bits, and a product three of theirs (what is left out
 // is 2^-22 of it).  The instruction cuts its sums off instead of rounding them: it adds eight products up from zero, the long
@@ -57,8 +57,9 @@ template <typename T> __host__ __device__ constexpr uint32_t smem_bytes(int ng) 
 constexpr float kGrowth = 8.f;   // log2 units: weights stay below 2^8
 // Groups of 8 rows at most, of own tokens and of prefixes (in 32 bits): their results and their q have to fit the registers, and
 // a tile's steps follow one another: 16 rows of q share what a warp reads, more rows are other warps' work, which reads it
-// again from L2.  32 requests of up to 5 rows, 12 heads on 2 kv heads of 128, us: 8 rows 41, 16 38, 32 50; 24 of up to 3, 16 on 4
-// of 96 (12 rows): 8 rows 31, 16 35; 32-bit, 12 of up to 2, 14 on 2 of 64 (14 rows): 8 rows 41, 16 48.
+// again from L2.  us, 8 rows / 16 rows: 32 requests of up to 5 rows, 12 heads on 2 kv heads of 128 (30 rows) 43.1 / 38.5 (32 rows 50);
+// 64 of up to 3, 28 on 4 of 128 (21 rows, which 16 hold no better than 8 do) 67.1 / 74.9; 24 of up to 3, 16 on 4 of 96 (12 rows) 31 / 35.
+// 32-bit, 14 on 2 of 64, requests of up to 2 (14 rows): 64 behind 8,000 145 / 176; 12 behind 2,000, a cluster an item, 27.3 / 23.5.
 template <typename T> constexpr int kNearGroups = sizeof(T) == 2 ? 2 : 1;
 constexpr int kOneGroup = 16;    // rows of a request up to which 8 are a tile
 constexpr int kFarGroups = HD <= 64 ? 2 : 0;

@@ -9,9 +9,10 @@
 // zero, and the values are made zero too, since zero times no number is none.
 // An item's result is the unnormalised sum of both streams with its maximum and sum, in 32 bits.
 //
-// What bounds it is a stream's chain of product, softmax and product: with two streams a tile of 128 by 128 takes 1.1 to 1.3 us,
-// 0.55 of that its 16,384 exponentials at 16 a clock.  On all SMs, without own tokens beside it: 256 requests behind 32,768 tokens, 40 heads on 8 of
-// 128, 233 us, 737 TFLOP/s; 64 behind 8,192, 28 on 4 of 128, 27.5 us, 273 TFLOP/s (10 us of that are starts, division and results).
+// What bounds it is a stream's chain of product, softmax and product: with two streams a tile of 128 by 128 takes 1.5 us, 0.55 of
+// that its 16,384 exponentials at 16 a clock; the tensor pipe is at work for 44 % of the time, the special-function unit for 46 %.
+// Beside own tokens, which have the other SMs: 256 requests behind 32,768 tokens, 40 heads on 8 of 128, 276 us on 123 SMs, 183 tiles each;
+// 64 behind 8,192, 28 on 4 of 128, 28 us, 10 of them starts, division and results.
 //
 // Warps: 0, 1 load K (and Q), 2, 3 load V, 4 issues products, 8 .. 11 and 12 .. 15 are the streams' softmax, a thread a row.
 // Every wait on an mbarrier is bounded; when one runs out, an abort flag tells the other roles, all meet at the final barrier
@@ -119,7 +120,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  // how the prefixes and the own tokens share the SMs: own tokens counted by the first four warps
+  // how the prefixes and the own tokens share the SMs: own tokens counted by the first eight warps
   GroupTiles t{};
   FarWork f{};
   if (warp == 5) f = far_work(a, t, g.H, g.shape.tokens, KT);

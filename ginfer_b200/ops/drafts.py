@@ -57,7 +57,8 @@ def verify(logits: torch.Tensor, tokens: torch.Tensor, cu_rows: torch.Tensor, te
     (for the draw; a draft is compared with ``u`` as it is).  A NaN counts as ``-inf``, logits of ``+inf`` share all of a
     row's weight.  Where nothing is left of ``p - q`` the next token is drawn from ``p``, where nothing is left of that either it is
     the arg-max (0 in a row without a number).  A draft that is no index of the vocabulary does not stay.  A request without
-    rows has ``(0, -1)``."""
+    rows has ``(0, -1)``.  Starts rise or stay; where they do not, nothing but the results is written, and what these are is
+    not said."""
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError(f"logits are [rows, vocabulary]; got {tuple(logits.shape)}")
     (R, V), code = logits.shape, _code(logits.dtype)

@@ -170,7 +170,7 @@ prefix_pieces_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     if (warp == CONSUMERS) f = far_work(a, t, p.H, p.shape.tokens, TILE);
     const OwnWork w = own_work<32 * CONSUMERS>(a, p.own_shape.tokens, p.own_tile, false, counts);
     if (warp == CONSUMERS) {
-      const int workers = far_share(p.sms, f.units, p.cost, w.total * p.own_H) * BLOCKS_AN_SM;
+      const int workers = far_share(p.sms, f.priced, p.cost, w.total * p.own_H) * BLOCKS_AN_SM;
       const int chunk = plan_chunk(a, t, f, p.H, p.shape.tokens, TILE, max(workers, 1), p.places, 3);
       groups_s[lane] = t;
       if (lane == 0) chunk_s = chunk, workers_s = workers;
@@ -557,18 +557,18 @@ constexpr long long kDirectKeys = 256 << 10, kDirectBytes = 128 << 20, kBlockKey
 constexpr long long kUnsharedBytes = 48 << 20, kUnsharedBytes32 = 128 << 20;
 // What a tile of a prefix costs beside a tile of own tokens (which come from memory), for the SMs' shares: 128 keys on the tensor
 // cores with up to 128 rows, 64 keys on mma.sync with up to 64 rows, 16 keys in 32 bits.  Own tokens' tiles are 16 keys, 32 for heads
-// of up to 64.  us at (costs):
-//  * tensor cores, 128 (6, 8, 10, 12): 28 heads on 4, 64 requests behind 8,192 tokens with up to 1,024 of their own 48.8 / 41.4 / 40.9 / 45.7,
-//    128 behind 4,096, 4,096 165 / 160 / 126 / 126, 256 behind 32,768, 512 242 / 194 / 193 / 215; 40 on 8, the same 84 / 64 / 67 / 65,
-//    317 / 281 / 241 / 233, 334 / 298 / 293 / 320.  64 (6, 8, 10), 14 on 2: 28.8 / 28.8 / 29.0, 54.8 / 48.2 / 53.7, 94.8 / 93.7 / 103.7.
-//  * mma.sync, up to 128 (3, 4, 5, 6): 16 on 4 of 96, 128 behind 4,096, 2,048 159 / 126 / 135 / 121, 24 of up to 3 rows behind two prompts of 3,001
-//    30.2 / 30.7 / 31.9 / 31.5, 64 of up to 3 behind 4,000, 600 64.9 / 59.9 / 57.1 / 66.8, 128 behind 16,000, 200 114 / 118 / 122 / 129.  192 and
-//    256, whose blocks have an SM to themselves (4, 6, 8, 10, 12): 10 on 2 of 192, 64 behind 8,192, 1,024 57.0 / 46.3 / 47.9 / 54.9 / 60.4,
-//    32 of up to 4 behind 16,000 71 / 67 / 83 / 97 / 115; 8 on 4 of 256, the first 104 / 81 / 72 / 69 / 64, 128 behind 4,096, 2,048 336 / 225 / 169 / 158 / 126,
-//    16 on 2 of 256, 32 of up to 4 behind 16,000 153 / 137 / 180 / 179 / 224.
-//  * 32 bits, 64 (1, 1.25, 1.5, 1.75, 2): 14 on 2, 128 behind 4,000, 600 128 / 118 / 120 / 129 / 145; 8 on 8, the same 142 / 130 / 119 / 120 / 124;
-//    20 on 1, 256 behind 2,000, 300 244 / 207 / 208 / 209 / 217.
-constexpr float kTensorCost = HD <= 64 ? 8.f : 10.f, kPlainCost = HD <= 128 ? 4.f : HD <= 192 ? 7.f : 9.f, kCost32 = 1.5f;
+// of up to 64.  (kFarOver is what an item costs beside its tiles.)  us at (costs):
+//  * tensor cores, 128 (7, 8, 9, 10): 28 heads on 4, 64 requests behind 8,192 tokens with up to 1,024 of their own 41.5 / 40.9 / 41.0 / 41.4,
+//    128 behind 4,096, 4,096 160 / 125 / 125 / 126, 256 behind 2,048, 300 70 / 55 / 55 / 56; 40 on 8, 256 behind 32,768, 512 334 / 304 / 300 / 308,
+//    128 behind 4,096, 4,096 247 / 244 / 238 / 233; 12 on 2, 32 of up to 5 rows behind 4,099, 2,048 38.7 / 38.8 / 37.6 / 39.0.  64 (5, 6, 7, 8), 14 on 2: the
+//    first 28.9 / 29.8 / 29.8 / 29.4, the second 53.8 / 47.8 / 48.5 / 53.7, the third 40.0 / 32.7 / 31.5 / 31.7, 256 behind 32,768, 512 108 / 99 / 98 / 95.
+//  * mma.sync, up to 128 (2.5, 3, 3.5, 4): 16 on 4 of 96, 24 of up to 3 rows behind two prompts of up to 3,001, 700 30.0 / 30.2 / 30.1 / 31.2, 128 behind
+//    4,096, 2,048 162 / 133 / 127 / 133, 64 behind 8,192, 1,024 63.4 / 62.1 / 66.6 / 65.0; 28 on 4 of 128 in pages of 24, the second 201 / 201 / 167 / 160.  192
+//    and 256, whose blocks have an SM to themselves: 8 on 4 of 256 (6, 7, 8, 9, 10), 64 behind 8,192, 1,024 81 / 72 / 71 / 69 / 68, 128 behind 4,096, 2,048
+//    188 / 169 / 158 / 158 / 127, 16 on 2, 32 of up to 4 behind 16,000, 300 137 / 149 / 179 / 179 / 179; 10 on 2 of 192 (4, 6, 8, 10), the first 57 / 46 / 48 / 55.
+//  * 32 bits, 64 (1, 1.2, 1.5): 14 on 2, 128 behind 4,000, 600 128 / 129 / 120; 8 on 8, the same 143 / 131 / 119; 20 on 1, 256 behind 2,000, 300
+//    245 / 208 / 210.
+constexpr float kTensorCost = HD <= 64 ? 7.f : 9.f, kPlainCost = HD <= 128 ? 3.5f : HD <= 192 ? 7.f : 9.f, kCost32 = 1.5f;
 
 // `words`: q, its row stride and type, k, v, pages, page, prefix_table and its stride, prefix_lens, groups, prefix limit,
 // table and its stride, lengths, requests, limit, cu_groups, cu, out, rows, heads, kv heads, SMs, the rows that a request has

@@ -116,24 +116,30 @@ struct GroupTiles {
     }
   }
 };
-// The prefixes' work, by one warp: row tiles times key tiles of all heads, and the longest prefix.  `t` keeps the first 32 groups.
+// The prefixes' work, by one warp: row tiles times key tiles of all heads, the same with what starts and ends cost, and the longest
+// prefix.  `t` keeps the first 32 groups.
+// Tiles that an item costs beside its own.  (Without it few key tiles of many rows had too few SMs: 252 requests of up to 5 rows behind
+// 74 tokens, 40 heads on 8 of 128, 496 us, 199 at 3, 196 at 6; 64 of one row behind 400, 28 on 4, 42.6, 40.9, 31.8.)
+constexpr int kFarOver = 6;
 struct FarWork {
-  long long units;
+  long long units, priced;
   int most;
 };
 __device__ __forceinline__ FarWork far_work(const PrefixArgs& a, GroupTiles& t, int H, int tokens, int tile) {
   const int lane = threadIdx.x & 31;
   t.load(a, lane, tokens, tile);
-  FarWork w{(long long)t.mt * H * t.nt, t.mt ? t.nt : 0};
+  FarWork w{(long long)t.mt * H * t.nt, t.nt ? (long long)t.mt * H * (t.nt + kFarOver) : 0, t.mt ? t.nt : 0};
   for (int g0 = 32; g0 < a.G; g0 += 32) {
     GroupTiles u;
     u.load(a, g0 + lane, tokens, tile);
     w.units += (long long)u.mt * H * u.nt;
+    w.priced += u.nt ? (long long)u.mt * H * (u.nt + kFarOver) : 0;
     w.most = max(w.most, u.mt ? u.nt : 0);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     w.units += __shfl_xor_sync(0xffffffffu, w.units, o);
+    w.priced += __shfl_xor_sync(0xffffffffu, w.priced, o);
     w.most = max(w.most, __shfl_xor_sync(0xffffffffu, w.most, o));
   }
   return w;

@@ -186,7 +186,7 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
     if (warp == WARPS - 1) f = far_work(a, groups, p.H, p.shape.tokens, KEYS);
     const OwnWork w = own_work<COUNTING>(a, p.own_shape.tokens, KEYS, false, counts);
     if (warp == WARPS - 1) {
-      const int workers = far_share(p.sms, f.units, p.far_cost, w.total * p.own_H) * WARPS;
+      const int workers = far_share(p.sms, f.priced, p.far_cost, w.total * p.own_H) * WARPS;
       const int c = plan_chunk(a, groups, f, p.H, p.shape.tokens, KEYS, max(workers, 1), p.places, kItemTiles, kMostSplitsOfWarps);
       groups_s[lane] = groups;
       if (lane == 0) {
@@ -204,7 +204,7 @@ prefix_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
     FarWork f{};
     if (p.after && warp == WARPS - 1) f = far_work(a, gt, p.far_H, p.far_shape.tokens, p.far_tile);
     const OwnWork w = own_work<COUNTING>(a, p.shape.tokens, KEYS, p.both, counts);
-    if (threadIdx.x == THREADS - 1) far_s = p.after ? far_share(p.sms, f.units, p.far_cost, w.total * p.H) : 0;
+    if (threadIdx.x == THREADS - 1) far_s = p.after ? far_share(p.sms, f.priced, p.far_cost, w.total * p.H) : 0;
     __syncthreads();
     const int blocks = p.after ? max(p.sms - far_s, 1) : (int)gridDim.x;
     cur = find_run<COUNTING>(a, w, shares, p.H, p.shape.tokens, KEYS, p.both, (long long)blockIdx.x * WARPS + warp,

@@ -126,7 +126,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_consta
   if (warp == 5) f = far_work(a, t, g.H, g.shape.tokens, KT);
   const OwnWork own = own_work<256>(a, g.own_shape.tokens, g.own_tile, false, bars->own);
   if (warp == 5) {
-    const int workers = min((int)gridDim.x, far_share(g.sms, f.units, g.cost, own.total * g.own_H));
+    const int workers = min((int)gridDim.x, far_share(g.sms, f.priced, g.cost, own.total * g.own_H));
     const int chunk = plan_chunk(a, t, f, g.H, g.shape.tokens, KT, max(workers, 1), g.places, kOver);
     bars->groups[lane] = t;
     if (lane == 0) {

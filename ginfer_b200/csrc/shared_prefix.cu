@@ -541,20 +541,28 @@ GF_DEFINE_PDL_SWITCH
 // Direct: an item (request, kv head) is a block's, or a cluster's of 2, 4 or 8 blocks while there are SMs for twice as many and a
 // block has more than kBlockKeys bytes of the item's keys, a single one twice that (clusters of 8 find places for three quarters of the SMs: one more had
 // to wait for another's end); its warps share the keys of prefix and own tokens; one launch.  Where a block has at most
-// kDirectKeys, in a cluster (but for 32-bit heads above 64) twice as many, and requests read at most kDirectBytes of prefixes.
+// kDirectKeys, in a cluster (but for 32-bit heads above 64) twice as many, requests read at most kDirectBytes of prefixes, and the items
+// are at most kDirectWaves blocks an SM: behind one another, they pay their starts.
 // Direct / equal runs and their join, us: 28 heads on 4 of 128, 64 requests of 1,000 tokens (a block) 26.5 / 27.3, of 2,000 42.0 /
 // 41.3; 16 of 2,500 (2 blocks) 17.2 / 23.6; 8 of 4,100 (4) 16 / 25; one of 4,000 (8) 11.0 / 20.2, of 16,000 23.7 / 31.1; 14 on 2 of
 // 64, 32 of 5,000 (2) 16.9 / 24.9, one of 4,000 (8) 8.1 / 19.9; that in fp32 14.9 / 30.1, 12 of up to 2,600 (2) 27.0 / 30.9; fp32, 28 on
 // 4 of 128, one of 4,000 (256 KB a block) 29.7 / 35.2, of 16,000 110 / 52.  Blocks of 128 KB, 64 KB, 32 KB: 28 on 4 of 128, one of 1,000 10.6,
 // 8.8, 8.1, one of 500 9.1, 8.5, 7.7; 14 on 2 of 64, 2 of 340 one block 6.2, two 6.7; in fp32, one of 1,000 14.4, 10.6, 8.7.
-constexpr long long kDirectKeys = 256 << 10, kDirectBytes = 128 << 20, kBlockKeys = 32 << 10;
-// Unshared: every request reads its prefix itself (from L2 but for the first), in equal runs.  Where that is at most so many
-// bytes; 2 launches instead of 3.  Unshared / shared, us: 28 on 4 of 128, 8 requests behind 1,000 tokens (16 MB) 19.0 / 21.8, 16 of
-// 1,000 (33 MB) 19.5 / 22.5, 8 of 4,000 (66 MB) 22.7 / 25.4, 64 of 1,000 (131 MB) 30.4 / 27.9, 8 of 16,000 (262 MB) 45 / 28; 14 on 2 of
-// 64, 8 of 4,000 (16 MB) 20.2 / 23.6, 8 of 16,000 (66 MB) 28.3 / 24.4; 16 on 4 of 96, 8 of 1,000 (12 MB) 19.0 / 21.2, 4 of 8,000 (49 MB) 27.0 / 23.8.
-// fp32, 14 on 2 of 64: 16 of 1,000 (16 MB) 27.6 / 29.4, 64 of 2,000 (131 MB) 43.4 / 40.4, 128 of 4,000 (524 MB) 127 / 100.  In 32 bits with heads
-// above 64 registers leave 8 rows a tile, with or without groups: 28 on 4 of 128, 128 of 4,000, 543 unshared, 785 shared; so not at all there.
-constexpr long long kUnsharedBytes = 48 << 20, kUnsharedBytes32 = 128 << 20;
+// Waves: 28 on 4 of 128, 64 requests of up to 400 (1.7) 16.5 / 20.8, 96 (2.6) 23.1 / 21.1, 128 of 110 (3.5) 22.2 / 20.8, 256 of 300 (6.9) 48.8 / 33.4; 40 on
+// 8, 32 of 400 (1.7) 15.8 / 20.4, 64 (3.5) 28.5 / 22.6, 512 of 150 (28) 160 / 64; 14 on 2 of 64, 128 of 600 (1.7) 14.0 / 20.5, 256 of 110 (3.5) 19.7 / 19.5, 512
+// of 150 (6.9) 34.9 / 24.1; that in fp32, 128 of 400 22.9 / 29.7, 256 of 110 25.4 / 28.1, of 400 42.3 / 36.6.
+constexpr long long kDirectKeys = 256 << 10, kDirectBytes = 128 << 20, kBlockKeys = 32 << 10, kDirectWaves = 2;
+// Unshared: every request reads its prefix itself (from L2 but for the first), in equal runs; 2 launches instead of 3.  Where
+// that is at most so many bytes, the fewer the longer a prefix is: a long one keeps warps busy that have one request's chain of
+// keys to go through.  Unshared / shared, us: 28 on 4 of 128, 64 requests behind 400 tokens (52 MB) 27.5 / 31.6, 700 (92 MB) 31.5 / 32.5,
+// 1,000 (131 MB) 35.6 / 33.6, 2,000 (262 MB) 51.1 / 37.0; 128 behind 400 (105 MB) 36.0 / 41.9, 700 (184 MB) 44.2 / 38.6; 16 behind 4,000 (131 MB)
+// 33.5 / 30.9; 4 behind 8,000 (66 MB) 28.8 / 30.5, 6 (98 MB) 30.8 / 29.4; 2 behind 16,000 (66 MB) 35.1 / 29.4; 14 on 2 of 64, 64 behind 2,000 (66 MB)
+// 22.5 / 26.9, 128 (131 MB) 34.0 / 32.1; 16 on 4 of 96, 64 behind 400 (39 MB) 30.2 / 44.6, 1,000 (98 MB) 40.3 / 44.9, 2,000 (197 MB) 59.7 / 53.1, 6 behind
+// 16,000 (147 MB) 47.0 / 42.5; 8 on 4 of 256, 64 behind 400 (105 MB) 43.8 / 42.8, 700 (184 MB) 53.1 / 40.5.  fp32, 14 on 2 of 64: 64 behind 1,000 (66 MB)
+// 34.3 / 37.6, 2,000 (131 MB) 48.4 / 48.6; 128 behind 1,000 (131 MB) 50.6 / 54.1, 2,000 (262 MB) 76.4 / 75.2, 4,000 (524 MB) 130 / 117.  Of 601 drawn calls
+// the way that this takes is 1.4 % slower than the better one in the mean.  In 32 bits with heads above 64 registers leave 8 rows a tile, with or
+// without groups: 28 on 4 of 128, 128 of 4,000, 543 unshared, 785 shared; so not at all there.
+constexpr long long kUnsharedBytes = 144 << 20, kUnsharedToken = 8 << 10, kUnsharedLeast = 16 << 20;
 // What a tile of a prefix costs beside a tile of own tokens (which come from memory), for the SMs' shares: 128 keys on the tensor
 // cores with up to 128 rows, 64 keys on mma.sync with up to 64 rows, 16 keys in 32 bits.  Own tokens' tiles are 16 keys, 32 for heads
 // of up to 64.  (kFarOver is what an item costs beside its tiles.)  us at (costs):
@@ -609,16 +617,21 @@ struct Call {
     p.rows = 8 * groups;
     p.shape = row_shape_of(a.nh, a.nkv, p.rows);
     p.H = a.nkv * p.shape.chunks;
-    const long long item = half ? 2 : 4, prefixes = (long long)a.B * a.prefix_limit * a.nkv * HD * 2 * item;
+    const long long item = half ? 2 : 4;
     const bool any = a.G > 0 && a.prefix_limit > 0;
     const long long held = ((any ? a.prefix_limit : 0ll) + a.limit) * HD * item;
     const long long items = (long long)((longest + p.shape.tokens - 1) / p.shape.tokens) * a.B * p.H;
+    // (as many of them as there can be: the hint is the longest request's)
+    const long long some = ((long long)a.T + (long long)a.B * (p.shape.tokens - 1)) / p.shape.tokens * p.H, reading = items < some ? items : some;
+    const long long prefixes = reading * a.prefix_limit * HD * 2 * item;
     p.cluster = 1;
     while (p.cluster < 8 && held > kBlockKeys * (p.cluster > 1 ? p.cluster : 2) && items * p.cluster * 2 <= (p.cluster == 4 ? p.sms * 3 / 4 : p.sms))
       p.cluster *= 2;
     const long long most = p.cluster > 1 && (half || HD <= 64) ? 2 * kDirectKeys : kDirectKeys;
-    direct = held <= most * p.cluster && (!any || prefixes <= kDirectBytes) && a.B <= 65535 && p.H <= 65535;
-    shared = !direct && any && (half ? prefixes > kUnsharedBytes : own::kFarGroups > 0 && prefixes > kUnsharedBytes32);
+    direct = held <= most * p.cluster && (!any || prefixes <= kDirectBytes) && a.B <= 65535 && p.H <= 65535 &&
+             reading <= kDirectWaves * p.sms;
+    const long long line = kUnsharedBytes - kUnsharedToken * a.prefix_limit;
+    shared = !direct && any && (half || own::kFarGroups > 0) && prefixes > (line > kUnsharedLeast ? line : kUnsharedLeast);
     p.both = !shared, p.joined = !direct, p.after = shared;
     // the scratch: the division, pieces of cut items, of rows, of prefixes
     need = 0;
